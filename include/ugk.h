@@ -321,6 +321,117 @@ int ugk_bbb_step_fused(float *mu, float *rho, float *m_mu, float *v_mu,
                        float klw, float bc1, float bc2, float lr, float beta1,
                        float beta2, float aeps, float wd);
 
+/* ---- dropout ------------------------------------------------------------
+ * No counterpart in the reference, whose network has none. Element i of n is
+ * kept where word i % 4 of Philox4x32-10 with counter {i / 4 low, i / 4 high,
+ * step, 1 + site} and key {seed low, seed high} is at least p * 2^32 (rounded to
+ * an integer); dropout(x)_i is then x_i * s with s = 1 / (1 - p) rounded once,
+ * else +0, whatever x_i is. The mask is drawn again by each call that names the
+ * same (seed, step, site) and never stored: a backward takes its forward's. The
+ * fourth counter word is 0 for the eps draws above, so one seed serves both.
+ * 0 <= p < 1, site >= 0 (one number per place of the network: sites differ, and
+ * two calls of one site see the same mask). Results are bit-identical to
+ * these formulas in IEEE single precision. */
+
+/* out = dropout(inp); out may be inp. */
+int ugk_dropout_forward(float *out, const float *inp, size_t n, float p,
+                        unsigned long long seed, int step, int site);
+/* dinp += dropout(dout). */
+int ugk_dropout_backward(float *dinp, const float *dout, size_t n, float p,
+                         unsigned long long seed, int step, int site);
+/* out = x + dropout(y): a block's residual add. out may be x or y. */
+int ugk_dropout_residual_forward(float *out, const float *x, const float *y,
+                                 size_t n, float p, unsigned long long seed,
+                                 int step, int site);
+/* dx += dout; dy += dropout(dout). dx == dy adds both, in that order. */
+int ugk_dropout_residual_backward(float *dx, float *dy, const float *dout,
+                                  size_t n, float p, unsigned long long seed,
+                                  int step, int site);
+/* ugk_dropout_residual_forward (element i of the B*T*C) then
+ * ugk_layernorm_forward of its output in one pass, with the results of the two,
+ * as ugk_residual_layernorm_forward for the pair without dropout. */
+int ugk_dropout_residual_layernorm_forward(float *res, float *out, float *mean,
+                                           float *rstd, const float *x,
+                                           const float *y, const float *weight,
+                                           const float *bias, int B, int T, int C,
+                                           float p, unsigned long long seed,
+                                           int step, int site);
+/* ugk_layernorm_backward then ugk_dropout_residual_backward(dx, dy, dinp), with
+ * the results of the two. dinp must differ from dx and dy. */
+int ugk_layernorm_dropout_residual_backward(float *dinp, float *dweight,
+                                            float *dbias, float *dx, float *dy,
+                                            const float *dout, const float *inp,
+                                            const float *weight, const float *mean,
+                                            const float *rstd, int B, int T, int C,
+                                            float p, unsigned long long seed,
+                                            int step, int site);
+
+/* ---- attention between the dense ops --------------------------------------
+ * gpt2_kernels.cuh:416-498 (k_attention_forward) and :500-619
+ * (k_attention_backward) compute causal attention of B sequences of equal length
+ * from rows that hold q, k and v side by side, one key/value head per query
+ * head, head size 64. These entry points take that layout and, beyond it, grouped
+ * heads, sequences of different lengths packed one behind the other, and few
+ * query rows against the keys and values of a cache. For query row i of a
+ * sequence with Lq query and Lk key rows, head h and its key/value head:
+ *     s_j = scale * q_i . k_j     over the allowed keys j < Lk, with causal
+ *                                 also j <= i + Lk - Lq (the last query row
+ *                                 sees every key)
+ *     out_i = sum_j softmax(s)_j v_j,   lse_i = log sum_j exp(s_j)
+ * A row without an allowed key has out 0, lse -infinity and gradients 0.
+ * What a row must not see does not reach it, infinities and NaN included.
+ * Rows of the buffers outside every sequence are neither read nor written. */
+typedef struct {
+  int nseq;           /* sequences */
+  int NH, NKV, HS;    /* query heads, key/value heads (NKV divides NH; query
+                         head h reads key/value head h / (NH / NKV)), floats
+                         per head (1 to 128) */
+  int rows_q, rows_k; /* rows of q, dq, out, dout, lse and of k, v, dk, dv */
+  int max_q, max_k;   /* the most query rows and keys of a sequence */
+  int causal;         /* nonzero: the causal limit above */
+  float scale;        /* of the scores; 1/sqrt(HS) in the reference */
+  /* DEVICE arrays of nseq ints each: sequence b is the rows [q_start[b],
+   * q_end[b]) and [k_start[b], k_end[b]). For packed sequences with nseq + 1
+   * ascending offsets cu: start = cu, end = cu + 1. For a cache: end = start +
+   * the filled length. Both of a pair NULL: sequence b is the rows [b max, (b +
+   * 1) max), and rows must be nseq * max. The kernels clamp what they read to
+   * the buffers; offsets outside them, an end before its start or a sequence
+   * longer than max is reported by the next ugk_synchronize. */
+  const int *q_start, *q_end, *k_start, *k_end;
+  /* floats from a row to the next (head h starts HS * h into it): of q and dq,
+   * of k and dk, of v and dv, of out and dout. 0: rows without gaps. */
+  long long ldq, ldk, ldv, ldo;
+} ugk_attention;
+
+/* lse (rows_q, NH) may be NULL. out must not overlap q, k or v. Sequences may
+ * share key rows, not query rows. */
+int ugk_attention_forward(float *out, float *lse, const float *q, const float *k,
+                          const float *v, ugk_attention a);
+
+/* dq += ..., dk += ..., dv += ... of the forward that gave out and lse. The
+ * gradients must not overlap each other's elements (they may lie side by side
+ * in one buffer, as q, k and v do) or the inputs, and the sequences must not
+ * share rows. Deterministic. Waits for nothing and allocates on first use like
+ * the other entry points (rows_q * NH floats of workspace). */
+int ugk_attention_backward(float *dq, float *dk, float *dv, const float *dout,
+                           const float *q, const float *k, const float *v,
+                           const float *out, const float *lse, ugk_attention a);
+
+/* ugk_attention_backward for callers whose dq, dk and dv are zero before the
+ * call: the rows of the sequences are written without being read. */
+int ugk_attention_backward_zeroed(float *dq, float *dk, float *dv, const float *dout,
+                                  const float *q, const float *k, const float *v,
+                                  const float *out, const float *lse, ugk_attention a);
+
+/* The two as callbacks of ugk_dense_ops (ctx is not used): scale 1/sqrt(C/NH),
+ * q, k and v in rows of 3C, C a multiple of NH. The backward does not
+ * get the forward's out and lse, and computes them again, into the workspace.
+ * It adds into dqkv, as the dense callbacks do. */
+int ugk_dense_attention_forward(void *ctx, float *out, const float *qkv, int B,
+                                int T, int C, int NH);
+int ugk_dense_attention_backward(void *ctx, float *dqkv, const float *dout,
+                                 const float *qkv, int B, int T, int C, int NH);
+
 /* ---- library control (no counterpart in the reference: its kernels run on
  * the CUDA legacy default stream and abort on error, gpt2_kernels.cuh:88-101) */
 
@@ -353,6 +464,8 @@ int ugk_synchronize(void);
 #define UGK_IDS_ENCODER_LAYERNORM_FORWARD 3
 #define UGK_IDS_SOFTMAX_CROSSENTROPY 4
 #define UGK_IDS_CROSSENTROPY_BACKWARD 5
+#define UGK_IDS_ATTENTION_FORWARD 6 /* the offsets of the sequences */
+#define UGK_IDS_ATTENTION_BACKWARD 7
 int ugk_ids_guard(int *ids, int n, int bound, int fill, int code);
 /* The ops that index a table by ids with that check inside their own kernels:
  * ugk_ids_guard over the B*T ids (bound V, the fill and code of the op; fill -1

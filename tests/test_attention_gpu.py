@@ -1,0 +1,411 @@
+"""GPU: attention forward and backward against 64 bits at the lengths, heads, strides and masks where it can go
+wrong, its refusals of bad offsets, graphs, streams, and a run of it inside the step driver."""
+import math
+
+import pytest
+import torch
+
+import att_ref
+from att_ref import Seqs
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def rand(g, *shape, scale=1.0):
+    return torch.randn(*shape, generator=g, device=DEV) * scale
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+class Call:
+    """Inputs of one call: q, k, v as views (rows, heads, HS) into buffers with `pad` floats between rows, the first
+    element `off` floats into its buffer."""
+
+    def __init__(self, gpu, s, NH, NKV, HS, causal=True, scale=None, pad=0, off=0, seed=1, sizes=(1.0, 1.0, 1.0), packed=False):
+        g = torch.Generator(device=DEV)
+        g.manual_seed(seed)
+        self.gpu, self.s, self.causal = gpu, s, causal
+        self.scale = HS ** -0.5 if scale is None else scale
+        self.NH, self.NKV, self.HS = NH, NKV, HS
+        if packed:  # q, k and v side by side, as the step driver's buffers hold them
+            self.ldq = self.ldk = self.ldv = (NH + 2 * NKV) * HS + pad
+            buf = rand(g, off + s.rows_q * self.ldq)
+            self.q = self.view(buf[off:], s.rows_q, NH, self.ldq)
+            self.k = self.view(buf[off + NH * HS:], s.rows_k, NKV, self.ldk)
+            self.v = self.view(buf[off + (NH + NKV) * HS:], s.rows_k, NKV, self.ldv)
+        else:
+            self.ldq, self.ldk, self.ldv = NH * HS + pad, NKV * HS + pad, NKV * HS + 2 * pad
+            mk = lambda rows, n, ld, z: self.view(rand(g, off + rows * ld + pad, scale=z)[off:], rows, n, ld)  # noqa: E731
+            self.q = mk(s.rows_q, NH, self.ldq, sizes[0])
+            self.k = mk(s.rows_k, NKV, self.ldk, sizes[1])
+            self.v = mk(s.rows_k, NKV, self.ldv, sizes[2])
+        self.ldo = NH * HS + pad
+        self.dout = self.view(rand(g, off + s.rows_q * self.ldo)[off:], s.rows_q, NH, self.ldo)
+        self.off = off
+
+    def view(self, buf, rows, heads, ld):
+        return buf.as_strided((rows, heads, self.HS), (ld, self.HS, 1), buf.storage_offset())
+
+    def att(self, offsets=True):
+        s = self.s
+        o = {}
+        if offsets:
+            o = {"q_start": ints(s.q), "q_end": ints([a + n for a, n in zip(s.q, s.lq)]), "k_start": ints(s.k),
+                 "k_end": ints([a + n for a, n in zip(s.k, s.lk)])}
+        return self.gpu.Attention(nseq=len(s.lq), NH=self.NH, NKV=self.NKV, HS=self.HS, rows_q=s.rows_q, rows_k=s.rows_k,
+                                  max_q=max(s.lq, default=0), max_k=max(s.lk, default=0), causal=self.causal, scale=self.scale,
+                                  ldq=self.ldq, ldk=self.ldk, ldv=self.ldv, ldo=self.ldo, **o)
+
+    def forward(self, offsets=True, lse=True):
+        out = self.view(torch.full((self.off + self.s.rows_q * self.ldo,), 7.0, device=DEV)[self.off:], self.s.rows_q, self.NH, self.ldo)
+        L = torch.full((self.s.rows_q, self.NH), 7.0, device=DEV)
+        self.gpu.attention_forward(out, L if lse else None, self.q, self.k, self.v, self.att(offsets))
+        return out, L
+
+    def grads(self, value=0.0):
+        mk = lambda rows, n, ld: self.view(torch.full((self.off + rows * ld,), value, device=DEV)[self.off:], rows, n, ld)  # noqa: E731
+        return [mk(self.s.rows_q, self.NH, self.ldq), mk(self.s.rows_k, self.NKV, self.ldk), mk(self.s.rows_k, self.NKV, self.ldv)]
+
+    def backward(self, out, lse, grads, zeroed=False):
+        fn = self.gpu.attention_backward_zeroed if zeroed else self.gpu.attention_backward
+        fn(*grads, self.dout, self.q, self.k, self.v, out, lse, self.att())
+
+
+def inside(got, want, tol, what):
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol) & ~(got.double() == want)  # infinities equal
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst {float((err / tol.clamp(min=1e-300))[bad].nan_to_num(1e9).max()):.3g} of the bound"
+
+
+def rows_of(starts, lens, n):
+    m = torch.zeros(n, dtype=torch.bool, device=DEV)
+    for a, b in zip(starts, lens):
+        m[a:a + b] = True
+    return m
+
+
+def check_forward(c, out, lse):
+    w, wl, tol, tol_l = att_ref.forward(c.s, c.q, c.k, c.v, c.scale, c.causal)
+    m = rows_of(c.s.q, c.s.lq, c.s.rows_q)
+    inside(out[m], w[m], tol[m], "out")
+    inside(lse[m], wl[m], tol_l[m], "lse")
+    assert (out[~m] == 7.0).all() and (lse[~m] == 7.0).all(), "rows outside the sequences were written"
+
+
+def check_backward(c, out, lse):
+    """Both forms: added onto what the gradients hold, and written over it."""
+    want, tol = att_ref.backward(c.s, c.q, c.k, c.v, out, lse, c.dout, c.scale, c.causal)
+    mq, mk = rows_of(c.s.q, c.s.lq, c.s.rows_q), rows_of(c.s.k, c.s.lk, c.s.rows_k)
+    for zeroed, start in ((False, 0.5), (True, 9.0)):
+        g = c.grads(start)
+        c.backward(out, lse, g, zeroed)
+        for name, x, w, t, m in zip(("dq", "dk", "dv"), g, want, tol, (mq, mk, mk)):
+            base = 0.0 if zeroed else start
+            inside(x[m], w[m] + base, t[m] + 2.0 ** -24 * (w[m].abs() + t[m] + base), f"{name} zeroed={zeroed}")
+            assert (x[~m] == start).all(), f"{name}: rows outside the sequences were written"
+
+
+LENGTHS = {
+    "one": ([1], None), "two": ([2, 1], None), "short": ([5, 0, 17, 1, 31, 32, 33], None),
+    "tile": ([63, 64, 65], None), "edge": ([127, 128, 129], None), "long": ([300, 257, 1], None),
+    "chunk": ([3, 16, 40], [50, 16, 333]), "token": ([1, 1, 1, 1], [1, 700, 64, 129]), "few": ([2, 4, 3], [300, 5, 1030]),
+    "later": ([20, 70, 5], [7, 64, 0]),  # more query rows than keys: the first rows see nothing
+    "nokeys": ([3, 1], [0, 0]), "noqueries": ([0, 0], [5, 40]),
+}
+
+
+@pytest.mark.parametrize("NH,NKV,HS", [(1, 1, 64), (6, 2, 64), (3, 3, 128), (8, 1, 16), (4, 4, 50), (5, 1, 33), (2, 2, 1), (2, 1, 80)])
+@pytest.mark.parametrize("lens", LENGTHS)
+def test_forward_and_backward(gpu, lens, NH, NKV, HS):
+    s = Seqs(*LENGTHS[lens], gap=1, tail=3)
+    c = Call(gpu, s, NH, NKV, HS)
+    out, lse = c.forward()
+    check_forward(c, out, lse)
+    check_backward(c, out, lse)
+
+
+@pytest.mark.parametrize("NH,NKV,HS,pad,off", [(2, 2, 64, 0, 1), (4, 2, 64, 3, 2), (3, 1, 96, 5, 3), (2, 2, 128, 4, 4), (2, 2, 7, 1, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_strides_alignment_and_no_causal_limit(gpu, causal, NH, NKV, HS, pad, off):
+    for lens, lk in (([70, 130], None), ([9, 33], [100, 20]), ([1, 2], [90, 300])):
+        c = Call(gpu, Seqs(lens, lk, gap=2, tail=1), NH, NKV, HS, causal, pad=pad, off=off, packed=lk is None)
+        out, lse = c.forward()
+        check_forward(c, out, lse)
+        check_backward(c, out, lse)
+
+
+@pytest.mark.parametrize("B,T,NH", [(4, 64, 6), (2, 100, 3), (3, 1, 2)])
+def test_equal_lengths_without_offsets(gpu, B, T, NH):
+    c = Call(gpu, Seqs([T] * B), NH, NH, 64, packed=True)
+    out, lse = c.forward(offsets=False)
+    again, _ = c.forward(offsets=True, lse=False)
+    assert torch.equal(out, again)
+    check_forward(c, out, lse)
+
+
+@pytest.mark.parametrize("sizes,scale", [((30.0, 30.0, 1.0), None), ((1e-6, 1e-4, 1e-3), None), ((1e-6, 1e6, 1e6), None),
+                                         ((1e10, 1e-10, 1e20), None), ((1e-15, 1e15, 1e-25), None), ((1.0, 1.0, 1.0), 0.0),
+                                         ((1.0, 1.0, 1.0), -3.0)])
+def test_sizes_of_values(gpu, sizes, scale):
+    """Values far from 1, scores up to thousands (one key takes all), equal scores, a negative scale."""
+    for lens, lk in (([130, 65], None), ([1], [200])):
+        c = Call(gpu, Seqs(lens, lk), 2, 1, 64, scale=scale, sizes=sizes)
+        out, lse = c.forward()
+        check_forward(c, out, lse)
+        if max(sizes) <= 1e6 and min(sizes) >= 1e-6:
+            check_backward(c, out, lse)
+
+
+def test_one_row_of_outliers(gpu):
+    """One key and one value a million times the others': what lies below them keeps its digits."""
+    c = Call(gpu, Seqs([150]), 2, 2, 64)
+    c.k[70] *= 1e4
+    c.v[90] *= 1e6
+    out, lse = c.forward()
+    check_forward(c, out, lse)
+    check_backward(c, out, lse)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, -3.4028234663852886e38])
+def test_what_a_row_must_not_see_does_not_reach_it(gpu, value):
+    """Unusable values behind the sequences, between them, and in the rows that come later than a row."""
+    for lens, lk, NH, NKV, HS in (([100, 37], None, 2, 1, 64), ([9, 1], [70, 90], 2, 2, 64), ([64, 64], None, 1, 1, 128), ([40], None, 2, 2, 50)):
+        s = Seqs(lens, lk, gap=2, tail=5)
+        c = Call(gpu, s, NH, NKV, HS)
+        out0, lse0 = c.forward()
+        g0 = c.grads()
+        c.backward(out0, lse0, g0)
+        mq, mk = rows_of(s.q, s.lq, s.rows_q), rows_of(s.k, s.lk, s.rows_k)
+        for t, m in ((c.q, mq), (c.k, mk), (c.v, mk), (c.dout, mq)):
+            t[~m] = value
+        out, lse = c.forward()
+        assert torch.equal(out, out0) and torch.equal(lse, lse0)
+        g = c.grads()
+        c.backward(out, lse, g)
+        for x, y in zip(g, g0):
+            assert torch.equal(x, y)
+        # the last key of each sequence: only the last query row sees it (bounds of 64 bits without it)
+        last_k = [a + n - 1 for a, n in zip(s.k, s.lk) if n]
+        last_q = [a + n - 1 for a, n in zip(s.q, s.lq) if n]
+        w, wl, tol, tol_l = att_ref.forward(s, c.q, c.k, c.v, c.scale, True)
+        c.k[last_k] = value
+        c.v[last_k] = value
+        out, lse = c.forward()
+        m = mq.clone()
+        m[last_q] = False
+        inside(out[m], w[m], tol[m], "out of the rows before the last")
+        inside(lse[m], wl[m], tol_l[m], "lse of the rows before the last")
+
+
+def test_values_that_cannot_be_used_in_the_backward(gpu):
+    """NaN in the last query row's q and dout and in the last key: gradients of what does not meet them are finite and
+    equal to 64 bits."""
+    s = Seqs([100])
+    c = Call(gpu, s, 1, 1, 64)
+    out, lse = c.forward()
+    c.k[99], c.v[99] = math.nan, math.nan
+    c2 = Call(gpu, Seqs([99], tail=1), 1, 1, 64)  # the same inputs without the last row
+    assert torch.equal(c.q, c2.q)
+    g = c.grads()
+    c.backward(out, lse, g)
+    want, tol = att_ref.backward(c2.s, c2.q, c2.k, c2.v, out, lse, c2.dout, c.scale, True)
+    inside(g[0][:99], want[0][:99], tol[0][:99], "dq")
+
+
+def test_infinite_values_that_a_row_sees(gpu):
+    """An infinite value with weight: the output of the rows that see it is that infinity, as in any arithmetic."""
+    c = Call(gpu, Seqs([80]), 1, 1, 64)
+    c.v[20, 0, 3] = math.inf
+    c.v[20, 0, 4] = -math.inf
+    out, lse = c.forward()
+    assert (out[20:, 0, 3] == math.inf).all() and (out[20:, 0, 4] == -math.inf).all()
+    assert out[:20].isfinite().all() and out[:, 0, 5:].isfinite().all() and lse.isfinite().all()
+    c.k[30, 0, 0] = math.nan
+    out, lse = c.forward()
+    assert out[30:].isnan().all() and lse[30:].isnan().all() and lse[:30].isfinite().all()
+
+
+@pytest.mark.parametrize("lens,lk,NH,NKV,HS", [([700, 900], None, 12, 12, 64), ([1025, 3, 500], None, 8, 2, 128),
+                                               ([1] * 6, [4000, 1, 513, 2222, 63, 64], 8, 2, 64), ([64], [3001], 4, 4, 64)])
+def test_larger(gpu, lens, lk, NH, NKV, HS):
+    c = Call(gpu, Seqs(lens, lk), NH, NKV, HS, packed=lk is None)
+    out, lse = c.forward()
+    check_forward(c, out, lse)
+    check_backward(c, out, lse)
+    again, lse2 = c.forward()
+    assert torch.equal(out, again) and torch.equal(lse, lse2), "two calls differ"
+    g1, g2 = c.grads(), c.grads()
+    c.backward(out, lse, g1)
+    c.backward(out, lse, g2)
+    assert all(torch.equal(a, b) for a, b in zip(g1, g2)), "two backward calls differ"
+
+
+def test_shared_prefix_rows_in_the_forward(gpu):
+    """Sequences may share key rows."""
+    c = Call(gpu, Seqs([1, 1, 2], [80, 80, 80]), 4, 2, 64)
+    s = c.s
+    s.k = [0, 0, 10]
+    out, lse = c.forward()
+    check_forward(c, out, lse)
+
+
+def test_gradient_against_differences(gpu):
+    """The directional derivative of sum(out * dout), by central differences in 64 bits: off by h^2 / 6 of its third
+    derivative (for h = 1e-4 and values of order 1 below 1e-6 of the sum of the terms' sizes) and by the gradient's bound."""
+    c = Call(gpu, Seqs([40, 9], [40, 30]), 4, 2, 64)
+    out, lse = c.forward()
+    g = c.grads()
+    c.backward(out, lse, g)
+    _, tol = att_ref.backward(c.s, c.q, c.k, c.v, out, lse, c.dout, c.scale, True)
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(9)
+    for which in range(3):
+        d = torch.randn(g[which].shape, generator=gen, device=DEV, dtype=torch.float64)
+        h, f = 1e-4, []
+        for sign in (1, -1):
+            t = [x.double() for x in (c.q, c.k, c.v)]
+            t[which] = t[which] + sign * h * d
+            f.append(float((att_ref.forward(c.s, *t, c.scale, True)[0] * c.dout.double()).sum()))
+        got = float((g[which].double() * d).sum())
+        bound = float((tol[which] * d.abs()).sum()) + 1e-6 * float((g[which].double().abs() * d.abs()).sum())
+        assert abs(got - (f[0] - f[1]) / (2 * h)) <= bound
+
+
+@pytest.mark.parametrize("bad", ["start", "end", "order", "long"])
+def test_bad_offsets_are_clamped_and_reported(gpu, bad):
+    c = Call(gpu, Seqs([20, 30], tail=2), 2, 2, 64)
+    a = c.att()
+    t = {"start": a._tensors[0], "end": a._tensors[3], "order": a._tensors[1], "long": a._tensors[1]}[bad]
+    t[0] = {"start": -5, "end": 1000, "order": -7, "long": 45}[bad]
+    out, lse = torch.zeros(52, 2, 64, device=DEV), torch.zeros(52, 2, device=DEV)
+    gpu.attention_forward(out, lse, c.q, c.k, c.v, a)
+    with pytest.raises(gpu.UgkError, match="attention_forward"):
+        gpu.synchronize()
+    g = c.grads()
+    gpu.attention_backward(*g, c.dout, c.q, c.k, c.v, out, lse, a)
+    with pytest.raises(gpu.UgkError, match="attention_backward"):
+        gpu.synchronize()
+    gpu.synchronize()  # the report is cleared
+    assert out[50:].eq(0).all()
+
+
+@pytest.mark.parametrize("lens,lk", [([100, 60], None), ([1, 1], [700, 90])])
+def test_captured_and_replayed(gpu, lens, lk):
+    """A captured forward and backward replayed with eager calls of another shape between, each replay checked."""
+    c, other = Call(gpu, Seqs(lens, lk), 4, 2, 64), Call(gpu, Seqs([33, 80]), 2, 2, 64, seed=5)
+    a, oa = c.att(), other.att()
+    out, lse = c.forward()
+    g = c.grads()
+    c.backward(out, lse, g)
+    want = [t.clone() for t in (out, lse, *g)]
+    o_out, o_lse = other.forward()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gpu.set_stream(stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for t in g:
+                t.zero_()
+            gpu.attention_forward(out, lse, c.q, c.k, c.v, a)
+            gpu.attention_backward(*g, c.dout, c.q, c.k, c.v, out, lse, a)
+        for _ in range(3):
+            for t in (out, lse, *g):
+                t.fill_(3.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, w in zip((out, lse, *g), want):
+                assert torch.equal(x, w)
+            x, y = torch.empty_like(o_out), torch.empty_like(o_lse)
+            with torch.cuda.stream(stream):
+                gpu.attention_forward(x, y, other.q, other.k, other.v, oa)
+                gpu.attention_backward(*other.grads(), other.dout, other.q, other.k, other.v, x, y, oa)
+            stream.synchronize()
+            assert torch.equal(x, o_out) and torch.equal(y, o_lse)
+    finally:
+        gpu.set_stream(None)
+
+
+def test_dense_callbacks_in_the_step_driver(gpu):
+    """The step driver with the library's attention and torch's products: the attention buffers of every block hold
+    what 64 bits give for the block's qkv, and the gradients accumulate onto the callback's dqkv."""
+    cfg = gpu.Config(B=3, T=40, C=128, V=50, NH=2, maxT=64, L=2)
+    B, T, C, NH = cfg.B, cfg.T, cfg.C, cfg.NH
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    qkv = rand(g, B * T, 3 * C)
+    dout, base = rand(g, B * T, C), rand(g, B * T, 3 * C)
+    s = Seqs([T] * B)
+    q, k, v = (qkv[:, i * C:(i + 1) * C].unflatten(1, (NH, C // NH)) for i in range(3))
+    w, wl, tol, _ = att_ref.forward(s, q, k, v, (C // NH) ** -0.5, True)
+    out = torch.empty(B * T, C, device=DEV)
+    gpu.dense_attention_forward(out, qkv, B, T, C, NH)
+    inside(out.view(B * T, NH, -1), w, tol, "dense forward")
+    dqkv = base.clone()
+    gpu.dense_attention_backward(dqkv, dout, qkv, B, T, C, NH)
+    # the callback's own out and lse are within tol of these, which moves D by at most sum |dout| tol
+    grads, gt = att_ref.backward(s, q, k, v, w.float(), wl.float(), dout.unflatten(1, (NH, C // NH)), (C // NH) ** -0.5, True)
+    for i, (x, t) in enumerate(zip(grads, gt)):
+        got = (dqkv - base)[:, i * C:(i + 1) * C].unflatten(1, (NH, C // NH))
+        inside(got, x, 4 * t + 2.0 ** -23 * base[:, i * C:(i + 1) * C].unflatten(1, (NH, C // NH)).abs() + 2.0 ** -23, f"dense gradient {i}")
+    # inside the driver: the qkv buffers as they are (no products), attention by the library
+    params = rand(g, gpu.param_count(cfg), scale=0.02)
+    acts = rand(g, gpu.act_count(cfg))
+    inp = torch.randint(0, cfg.V, (B * T,), generator=g, device=DEV, dtype=torch.int32)
+    ops = gpu.DenseOps(**gpu.dense_attention_callbacks())
+    n = B * T * C
+    block = 18 * n + 4 * B * T
+    gpu.gpt2_layers_forward(acts, params, inp, cfg, ops)
+    for l in range(cfg.L):
+        at = n + l * block + n + 2 * B * T
+        blk_qkv, atty = acts[at:at + 3 * n].view(B * T, 3 * C), acts[at + 3 * n:at + 4 * n]
+        gpu.dense_attention_forward(out, blk_qkv.contiguous(), B, T, C, NH)
+        assert torch.equal(atty, out.view(-1)), f"block {l}"
+    grads, ga = torch.zeros(gpu.param_count(cfg), device=DEV), torch.zeros(gpu.act_count(cfg), device=DEV)
+    ga[n + cfg.L * block:n + cfg.L * block + n] = rand(g, n)
+    for l in range(cfg.L):
+        at = n + l * block + n + 2 * B * T
+        ga[at + 3 * n:at + 4 * n] = rand(g, n)
+    gpu.gpt2_layers_backward(grads, ga, acts, params, inp, cfg, ops)
+    for l in range(cfg.L):
+        at = n + l * block + n + 2 * B * T
+        want = torch.zeros(3 * n, device=DEV)
+        gpu.dense_attention_backward(want, ga[at + 3 * n:at + 4 * n].clone(), acts[at:at + 3 * n].clone(), B, T, C, NH)
+        assert torch.equal(ga[at:at + 3 * n], want), f"gradient of block {l}"
+    gpu.synchronize()
+
+
+def test_caller_owned_workspace(gpu):
+    """Inside a workspace sized for the config, and refused by one too small."""
+    cfg = gpu.Config(B=2, T=64, C=128, V=50, NH=2, maxT=64, L=1)
+    c, big = Call(gpu, Seqs([64, 64]), 2, 2, 64, packed=True), Call(gpu, Seqs([1] * 4000), 64, 64, 4)
+    out, lse = c.forward()
+    g = c.grads()
+    c.backward(out, lse, g)
+    b_out, b_lse = big.forward()
+    n = gpu.workspace_bytes(cfg)
+    ws = torch.empty(n + 256, dtype=torch.uint8, device=DEV)
+    at = (-ws.data_ptr()) % 256
+    try:
+        gpu.set_workspace(ws[at:at + n], cfg)
+        out2, lse2 = c.forward()
+        g2 = c.grads()
+        c.backward(out2, lse2, g2)
+        assert torch.equal(out, out2) and all(torch.equal(x, y) for x, y in zip(g, g2))
+        rows = attention_rows_beyond(gpu, cfg, n)
+        huge = Call(gpu, Seqs([1] * rows), 64, 64, 1)
+        h_out, h_lse = torch.zeros(rows, 64, device=DEV), torch.zeros(rows, 64, device=DEV)
+        with pytest.raises(gpu.UgkError) as err:
+            huge.backward(h_out, h_lse, huge.grads())
+        assert err.value.status == 3 and "attention" in str(err.value)
+    finally:
+        gpu.set_workspace(None, cfg)
+
+
+def attention_rows_beyond(gpu, cfg, n):
+    """Rows whose 64 row sums each exceed any region of a workspace of n bytes."""
+    return n // 256 + 1

@@ -16,6 +16,7 @@
 
 #include "../../include/ugk.h"
 #include "ugk_internal.h"
+#include "ugk_philox.h"
 
 namespace ugk {
 
@@ -27,7 +28,7 @@ constexpr int kMaxDevices = 64;
 constexpr size_t kAlign = 256;
 size_t align_up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 const char *const kRegionName[kNumRegions] = {"LayerNorm partial rows", "encoder bucket state", "KL partial sums",
-                                              "softmax row statistics"};
+                                              "softmax row statistics", "attention row sums and parts"};
 
 // Per device: the library's own region allocations, or the caller's workspace
 // and the offset and capacity of each region in it.
@@ -37,7 +38,7 @@ struct DevWorkspace {
   char *user = nullptr;
   size_t user_bytes = 0;
   size_t off[kNumRegions] = {}, cap[kNumRegions] = {};
-  bool fresh[kNumRegions] = {true, true, true, true};
+  bool fresh[kNumRegions] = {true, true, true, true, true};
 };
 DevWorkspace g_ws[kMaxDevices];
 
@@ -51,9 +52,16 @@ int current_device(const char *what) {
   return dev;
 }
 
+// Attention's region: parts of a split key axis, two floats per row and head
+// (row sums, lse), and out.
+size_t attention_scratch(size_t rows, size_t C, size_t NH, size_t parts) {
+  return align_up(parts) + 2 * align_up(rows * NH * sizeof(float)) + align_up(rows * C * sizeof(float));
+}
+
 // Region sizes for every entry point at shapes up to cfg: the step driver's
 // 2L+1 LayerNorm slots (at least the one slot of a per-op call), the encoder
-// state, the KL partial sums and the softmax statistics of B*T rows.
+// state, the KL partial sums, the softmax statistics of B*T rows, and attention
+// over B*T rows of C channels in NH heads (the dense callback's backward).
 void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
   const int rows = cfg.B * cfg.T;
   const size_t slot = align_up(layernorm_backward_scratch(rows, cfg.C));
@@ -61,6 +69,7 @@ void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
   out[kRegEncoder] = encoder_backward_scratch();
   out[kRegKl] = kl_forward_scratch();
   out[kRegSoftmax] = softmax_scratch(rows, cfg.V);
+  out[kRegAttention] = attention_scratch(rows, cfg.C, cfg.NH > 0 ? cfg.NH : 0, attention_parts_bound());
 }
 
 // Grow the library-owned region r of device dev to `bytes` (lock held).
@@ -301,6 +310,107 @@ int xent_backward(const char *fn, bool zeroed, float *dlogits, const float *prob
   const float dloss = 1.0f / (B * T);  // train_bnn.c:360
   if (int e = launch_crossentropy_softmax_backward(dlogits, probs, targets, B * T, V, dloss, zeroed, ids)) return e;
   return ok();
+}
+
+// *d for dropout with probability p.
+int drop_params(const char *fn, float p, unsigned long long seed, int step, int site, UgkDrop *d) {
+  if (!(p >= 0.0f && p < 1.0f)) return bad(fn, "p must be in [0, 1)");
+  if (site < 0) return bad(fn, "site must be >= 0");
+  d->seed = seed;
+  d->step = step;
+  d->stream = (uint32_t)site + 1u;
+  d->below = (uint32_t)llrint((double)p * 4294967296.0);  // p <= 1 - 2^-24: below 2^32
+  d->scale = (float)(1.0 / (1.0 - (double)p));
+  return UGK_OK;
+}
+
+// *a with its strides filled in; *none: there is nothing to compute.
+int check_attention(const char *fn, ugk_attention *a, bool *none) {
+  *none = false;
+  if (a->nseq < 0 || a->rows_q < 0 || a->rows_k < 0 || a->max_q < 0 || a->max_k < 0)
+    return bad(fn, "nseq, rows and max must be >= 0");
+  if (a->NH < 1 || a->NKV < 1 || a->NH % a->NKV) return bad(fn, "NKV must be >= 1 and divide NH");
+  if (a->HS < 1 || a->HS > kMaxHead) return set_error(UGK_EINVAL, "%s: HS must be 1 to %d, got %d", fn, kMaxHead, a->HS);
+  if ((long long)a->NH * a->HS > INT_MAX) return bad(fn, "NH*HS exceeds INT_MAX");
+  if (isnan(a->scale) || isinf(a->scale)) return bad(fn, "scale must be finite");
+  if (!a->q_start != !a->q_end || !a->k_start != !a->k_end) return bad(fn, "start and end come together");
+  if (!a->q_start && (long long)a->nseq * a->max_q != a->rows_q) return bad(fn, "rows_q must be nseq * max_q without offsets");
+  if (!a->k_start && (long long)a->nseq * a->max_k != a->rows_k) return bad(fn, "rows_k must be nseq * max_k without offsets");
+  const long long wq = (long long)a->NH * a->HS, wk = (long long)a->NKV * a->HS;
+  if (!a->ldq) a->ldq = wq;
+  if (!a->ldo) a->ldo = wq;
+  if (!a->ldk) a->ldk = wk;
+  if (!a->ldv) a->ldv = wk;
+  if (a->ldq < wq || a->ldo < wq || a->ldk < wk || a->ldv < wk)
+    return bad(fn, "a row stride is less than its row (NH*HS, or NKV*HS for k and v)");
+  // the addresses of the last rows, in bytes
+  const long long most = (long long)1 << 60;
+  const long long rows = (a->rows_q > a->rows_k ? a->rows_q : a->rows_k) + 1LL;
+  if (a->ldq > most / rows || a->ldo > most / rows || a->ldk > most / rows || a->ldv > most / rows)
+    return bad(fn, "rows * stride exceeds the address space");
+  if ((long long)a->max_q * (a->NH / a->NKV) > INT_MAX / 2 || a->max_k > INT_MAX / 2)
+    return bad(fn, "max_q * NH / NKV or max_k exceeds 2^30");
+  // a workgroup takes a few rows of q, or of k, at a time, for each sequence and key/value head
+  const long long blocks = ((long long)a->max_q * (a->NH / a->NKV) + a->max_k) / 4 + 1;
+  if ((long long)a->nseq * a->NKV > INT_MAX / 4 / blocks) return bad(fn, "nseq * heads * rows exceeds the grid");
+  *none = a->nseq == 0 || a->max_q == 0 || a->rows_q == 0;
+  return UGK_OK;
+}
+
+int attention_forward(const char *fn, float *out, float *lse, const float *q, const float *k, const float *v,
+                      ugk_attention a) {
+  bool none;
+  if (int e = check_attention(fn, &a, &none)) return e;
+  if (none) return ok();
+  if (any_null({out, q})) return bad(fn, "NULL pointer");
+  if (a.rows_k > 0 && any_null({k, v})) return bad(fn, "NULL pointer");
+  if (out == q || out == k || out == v) return bad(fn, "out must be distinct from q, k and v");
+  float *parts = nullptr;
+  if (const size_t bytes = attention_parts_bytes(a)) {
+    parts = static_cast<float *>(workspace(kRegAttention, bytes));
+    if (!parts) return UGK_ENOMEM;
+  }
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  if (int e = launch_attention_forward(out, lse, q, k, v, parts, a, word)) return e;
+  return ok();
+}
+
+int attention_backward(const char *fn, float *dq, float *dk, float *dv, const float *dout, const float *q, const float *k,
+                       const float *v, const float *out, const float *lse, ugk_attention a, bool assign) {
+  bool none;
+  if (int e = check_attention(fn, &a, &none)) return e;
+  if (none && (a.nseq == 0 || a.rows_k == 0 || a.max_k == 0)) return ok();
+  if (a.rows_q > 0 && any_null({dq, dout, q, out, lse})) return bad(fn, "NULL pointer");
+  if (a.rows_k > 0 && any_null({dk, dv, k, v})) return bad(fn, "NULL pointer");
+  if (a.rows_q > 0 && a.rows_k > 0 && any_same({dq, dk, dv})) return bad(fn, "dq, dk and dv must be distinct buffers");
+  for (const float *g : {dq, dk, dv})
+    for (const float *x : {dout, q, k, v, out, lse})
+      if (g && g == x) return bad(fn, "the gradients must be distinct from the inputs");
+  float *dsum = static_cast<float *>(workspace(kRegAttention, (size_t)a.rows_q * a.NH * sizeof(float) + kAlign));
+  if (!dsum) return UGK_ENOMEM;
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  if (int e = launch_attention_backward(dq, dk, dv, dout, q, k, v, out, lse, dsum, a, assign, word)) return e;
+  return ok();
+}
+
+// The dense callbacks' shape: q, k and v side by side in rows of 3C.
+int dense_attention(const char *fn, int B, int T, int C, int NH, ugk_attention *a) {
+  if (int e = check_btc(fn, B, T, C)) return e;
+  if (C < 1 || NH < 1 || C % NH) return bad(fn, "C must be a multiple of NH, both >= 1");
+  if (C > INT_MAX / 3) return bad(fn, "3C exceeds INT_MAX");
+  *a = ugk_attention{};
+  a->nseq = B;
+  a->NH = a->NKV = NH;
+  a->HS = C / NH;
+  a->rows_q = a->rows_k = B * T;
+  a->max_q = a->max_k = T;
+  a->causal = 1;
+  a->scale = 1.0f / sqrtf((float)a->HS);
+  a->ldq = a->ldk = a->ldv = 3LL * C;
+  bool none;
+  return check_attention(fn, a, &none);
 }
 }  // namespace
 
@@ -577,6 +687,126 @@ int ugk_bbb_step_fused(float *mu, float *rho, float *m_mu, float *v_mu, float *m
   return ok();
 }
 
+int ugk_dropout_forward(float *out, const float *inp, size_t n, float p, unsigned long long seed, int step, int site) {
+  const char *fn = "ugk_dropout_forward";
+  UgkDrop d;
+  if (int e = drop_params(fn, p, seed, step, site, &d)) return e;
+  if (n == 0) return ok();
+  if (any_null({out, inp})) return bad(fn, "NULL pointer");
+  if (int e = launch_dropout(kDrop, out, nullptr, inp, nullptr, n, d)) return e;
+  return ok();
+}
+
+int ugk_dropout_backward(float *dinp, const float *dout, size_t n, float p, unsigned long long seed, int step,
+                         int site) {
+  const char *fn = "ugk_dropout_backward";
+  UgkDrop d;
+  if (int e = drop_params(fn, p, seed, step, site, &d)) return e;
+  if (n == 0) return ok();
+  if (any_null({dinp, dout})) return bad(fn, "NULL pointer");
+  if (int e = launch_dropout(kDropAcc, dinp, nullptr, dout, nullptr, n, d)) return e;
+  return ok();
+}
+
+int ugk_dropout_residual_forward(float *out, const float *x, const float *y, size_t n, float p, unsigned long long seed,
+                                 int step, int site) {
+  const char *fn = "ugk_dropout_residual_forward";
+  UgkDrop d;
+  if (int e = drop_params(fn, p, seed, step, site, &d)) return e;
+  if (n == 0) return ok();
+  if (any_null({out, x, y})) return bad(fn, "NULL pointer");
+  if (int e = launch_dropout(kDropAddTo, out, nullptr, x, y, n, d)) return e;
+  return ok();
+}
+
+int ugk_dropout_residual_backward(float *dx, float *dy, const float *dout, size_t n, float p, unsigned long long seed,
+                                  int step, int site) {
+  const char *fn = "ugk_dropout_residual_backward";
+  UgkDrop d;
+  if (int e = drop_params(fn, p, seed, step, site, &d)) return e;
+  if (n == 0) return ok();
+  if (any_null({dx, dy, dout})) return bad(fn, "NULL pointer");
+  if (int e = launch_dropout(kDropSplit, dx, dy, dout, nullptr, n, d)) return e;
+  return ok();
+}
+
+int ugk_dropout_residual_layernorm_forward(float *res, float *out, float *mean, float *rstd, const float *x,
+                                           const float *y, const float *weight, const float *bias, int B, int T, int C,
+                                           float p, unsigned long long seed, int step, int site) {
+  const char *fn = "ugk_dropout_residual_layernorm_forward";
+  UgkDrop d;
+  if (int e = drop_params(fn, p, seed, step, site, &d)) return e;
+  if (int e = check_btc(fn, B, T, C)) return e;
+  if ((long long)B * T == 0) return ok();
+  if (C == 0) return bad(fn, "C must be > 0 when B*T > 0 (mean over an empty row)");
+  if (any_null({res, out, mean, rstd, x, y, weight, bias})) return bad(fn, "NULL pointer");
+  if (int e = launch_dropout_residual_layernorm_forward(res, out, mean, rstd, x, y, weight, bias, B * T, C, d)) return e;
+  return ok();
+}
+
+int ugk_layernorm_dropout_residual_backward(float *dinp, float *dweight, float *dbias, float *dx, float *dy,
+                                            const float *dout, const float *inp, const float *weight, const float *mean,
+                                            const float *rstd, int B, int T, int C, float p, unsigned long long seed,
+                                            int step, int site) {
+  const char *fn = "ugk_layernorm_dropout_residual_backward";
+  UgkDrop d;
+  if (int e = drop_params(fn, p, seed, step, site, &d)) return e;
+  if (int e = check_btc(fn, B, T, C)) return e;
+  if ((long long)B * T * C == 0) return ok();
+  if (any_null({dinp, dweight, dbias, dx, dy, dout, inp, weight, mean, rstd})) return bad(fn, "NULL pointer");
+  if (dinp == dx || dinp == dy) return bad(fn, "dinp must be distinct from dx and dy");
+  if (int e = launch_layernorm_backward(dinp, dweight, dbias, dout, inp, weight, mean, rstd, B * T, C)) return e;
+  if (int e = launch_dropout(kDropSplit, dx, dy, dinp, nullptr, (size_t)B * T * C, d)) return e;
+  return ok();
+}
+
+int ugk_attention_forward(float *out, float *lse, const float *q, const float *k, const float *v, ugk_attention a) {
+  return attention_forward("ugk_attention_forward", out, lse, q, k, v, a);
+}
+
+int ugk_attention_backward(float *dq, float *dk, float *dv, const float *dout, const float *q, const float *k,
+                           const float *v, const float *out, const float *lse, ugk_attention a) {
+  return attention_backward("ugk_attention_backward", dq, dk, dv, dout, q, k, v, out, lse, a, false);
+}
+
+int ugk_attention_backward_zeroed(float *dq, float *dk, float *dv, const float *dout, const float *q, const float *k,
+                                  const float *v, const float *out, const float *lse, ugk_attention a) {
+  return attention_backward("ugk_attention_backward_zeroed", dq, dk, dv, dout, q, k, v, out, lse, a, true);
+}
+
+int ugk_dense_attention_forward(void *, float *out, const float *qkv, int B, int T, int C, int NH) {
+  const char *fn = "ugk_dense_attention_forward";
+  ugk_attention a;
+  if (int e = dense_attention(fn, B, T, C, NH, &a)) return e;
+  if ((long long)B * T == 0) return ok();
+  if (any_null({out, qkv})) return bad(fn, "NULL pointer");
+  return attention_forward(fn, out, nullptr, qkv, qkv + C, qkv + 2 * (size_t)C, a);
+}
+
+int ugk_dense_attention_backward(void *, float *dqkv, const float *dout, const float *qkv, int B, int T, int C,
+                                 int NH) {
+  const char *fn = "ugk_dense_attention_backward";
+  ugk_attention a;
+  if (int e = dense_attention(fn, B, T, C, NH, &a)) return e;
+  const size_t rows = (size_t)B * T;
+  if (rows == 0) return ok();
+  if (any_null({dqkv, dout, qkv})) return bad(fn, "NULL pointer");
+  if (dqkv == qkv || dqkv == dout) return bad(fn, "dqkv must be distinct from qkv and dout");
+  const size_t parts = align_up(attention_parts_bytes(a)), stat = align_up(rows * NH * sizeof(float));
+  char *w = static_cast<char *>(workspace(kRegAttention, attention_scratch(rows, C, NH, parts)));
+  if (!w) return UGK_ENOMEM;
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  float *dsum = reinterpret_cast<float *>(w + parts), *lse = reinterpret_cast<float *>(w + parts + stat);
+  float *out = reinterpret_cast<float *>(w + parts + 2 * stat);
+  const float *k = qkv + C, *v = qkv + 2 * (size_t)C;
+  if (int e = launch_attention_forward(out, lse, qkv, k, v, reinterpret_cast<float *>(w), a, word)) return e;
+  if (int e = launch_attention_backward(dqkv, dqkv + C, dqkv + 2 * (size_t)C, dout, qkv, k, v, out, lse, dsum, a, false,
+                                        word))
+    return e;
+  return ok();
+}
+
 int ugk_set_gelu_exact(int exact) {
   set_gelu_exact(exact);
   return ok();
@@ -715,6 +945,8 @@ const char *ids_op_name(int code) {
     case UGK_IDS_ENCODER_LAYERNORM_FORWARD: return "encoder_layernorm_forward";
     case UGK_IDS_SOFTMAX_CROSSENTROPY: return "softmax_crossentropy";
     case UGK_IDS_CROSSENTROPY_BACKWARD: return "crossentropy_softmax_backward";
+    case UGK_IDS_ATTENTION_FORWARD: return "attention_forward";
+    case UGK_IDS_ATTENTION_BACKWARD: return "attention_backward";
     default: return "a guarded call";
   }
 }
@@ -748,6 +980,12 @@ int ugk_synchronize(void) {
       (void)hipGetLastError();
       return set_error(UGK_EHIP, "ugk_synchronize: clearing the id error word failed");
     }
+    if (code == UGK_IDS_ATTENTION_FORWARD || code == UGK_IDS_ATTENTION_BACKWARD)
+      return set_error(UGK_EINVAL,
+                       "ugk_synchronize: %s was given offsets outside its buffers, an end before its start or a "
+                       "sequence longer than max (found on the device; they were clamped, so its results are not "
+                       "meaningful)",
+                       ids_op_name(code));
     return set_error(UGK_EINVAL,
                      "ugk_synchronize: %s was given an id outside its table (found on the device by "
                      "ugk_ids_guard; the out-of-range ids were replaced, so its results are not meaningful)",

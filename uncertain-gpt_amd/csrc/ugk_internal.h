@@ -8,6 +8,8 @@
 
 #include "ugk.h"  // status codes
 
+struct UgkDrop;
+
 namespace ugk {
 
 constexpr int kWave = 64;      // CDNA wavefront width
@@ -21,8 +23,9 @@ int check_launch(const char *what);
 // Device workspace, one region per purpose, so that a kernel's scratch is
 // never another's: the LayerNorm-backward partial rows (one slot per call, or
 // 2L+1 slots for the step driver), the encoder backward's bucket state (kept
-// between calls), the KL total's partial sums and the long-row softmax's row
-// statistics. Each region is the library's own allocation, grown when a
+// between calls), the KL total's partial sums, the long-row softmax's row
+// statistics, and attention's (the backward's row sums, the recomputed forward
+// of the dense callback, the parts of a split key axis). Each region is the library's own allocation, grown when a
 // larger shape arrives (after waiting for the device), or a fixed part of a
 // workspace the caller handed over with ugk_set_workspace, which then never
 // grows. workspace() returns at least `bytes` of region r on the current
@@ -30,7 +33,7 @@ int check_launch(const char *what);
 // region's memory is new since its last use (its contents are undefined).
 // With keep_fresh the fresh mark is reported but left set (for a caller that
 // cannot prepare the memory now, e.g. under graph capture).
-enum Region { kRegLn = 0, kRegEncoder = 1, kRegKl = 2, kRegSoftmax = 3, kNumRegions = 4 };
+enum Region { kRegLn = 0, kRegEncoder = 1, kRegKl = 2, kRegSoftmax = 3, kRegAttention = 4, kNumRegions = 5 };
 void *workspace(Region r, size_t bytes, bool *fresh = nullptr, bool keep_fresh = false);
 // Whether the library stream is being captured into a graph (false if the
 // query fails).
@@ -337,6 +340,30 @@ int launch_ids_guard(int *ids, int n, int bound, int fill, int code);
 // Device address of the current device's id error word (nullptr with the
 // error set if its lookup failed).
 int *ids_error_word();
+
+// Dropout with the mask drawn where it is used (ugk_philox.h: UgkDrop).
+enum DropForm {
+  kDrop,         // a = drop(x)
+  kDropAcc,      // a += drop(x)
+  kDropAddTo,    // a = x + drop(y)
+  kDropSplit     // a += x; b += drop(x) (a == b: both, in that order)
+};
+int launch_dropout(DropForm form, float *a, float *b, const float *x, const float *y, size_t n, const UgkDrop &drop);
+int launch_dropout_residual_layernorm_forward(float *res, float *out, float *mean, float *rstd, const float *x,
+                                              const float *y, const float *weight, const float *bias, int rows, int C,
+                                              const UgkDrop &drop);
+constexpr int kMaxHead = 128;  // floats per head of the attention
+// Attention. `a` is checked and its strides are filled in; word: the id error
+// word. The forward's parts of a split key axis go to `parts`
+// (attention_parts_bytes(a); 0: not split), the backward's rows_q * NH row sums to
+// `dsum`. assign: dq, dk and dv are written, not added to.
+int launch_attention_forward(float *out, float *lse, const float *q, const float *k, const float *v, float *parts,
+                             const ugk_attention &a, int *word);
+int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout, const float *q, const float *k,
+                              const float *v, const float *out, const float *lse, float *dsum, const ugk_attention &a,
+                              bool assign, int *word);
+size_t attention_parts_bytes(const ugk_attention &a);
+size_t attention_parts_bound();  // over all calls
 
 // Workspace sizes.
 size_t layernorm_backward_scratch(int rows, int C);  // bytes of one call's partial rows

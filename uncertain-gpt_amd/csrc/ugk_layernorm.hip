@@ -34,12 +34,15 @@
 #include <mutex>
 
 #include "ugk_internal.h"
+#include "ugk_philox.h"
 
 namespace ugk {
 namespace {
 
 constexpr int kWavesPerBlock = kBlock / kWave;
 constexpr int kMaxV = 8;  // float4 per lane held in registers: C <= 2048
+// What a forward kernel normalises: inp, inp + inp2, or inp + dropout(inp2).
+enum FwdIn { kPlain = 0, kSum = 1, kDropSum = 2 };
 constexpr int kMaxWide = 8192;  // channels of the workgroup-per-row kernels
 
 __device__ __forceinline__ float4 add4(float4 a, float4 b) {
@@ -155,13 +158,15 @@ __device__ __forceinline__ void ln_row_out(const float4 (&xv)[V], const Cols<V, 
 // flight while it writes one.
 // kRes: the row is first formed as res = inp + inp2 (residual_forward,
 // train_bnn.c:182-186), stored to res, and normalised from the registers, the
-// pair gpt2_kernels.cuh:793-797 launches back to back.
-template <int V, bool kRes, int RPW, bool kRag, bool kEarly>
+// pair gpt2_kernels.cuh:793-797 launches back to back. kDropSum: inp2 goes
+// through dropout first (ugk_dropout_residual_forward), element i of the whole array.
+template <int V, int kIn, int RPW, bool kRag, bool kEarly>
 __global__ __launch_bounds__(kBlock) void k_ln_fwd_vec(float *__restrict__ out, float *__restrict__ mean,
                                                        float *__restrict__ rstd, const float *__restrict__ inp,
                                                        const float *__restrict__ weight,
                                                        const float *__restrict__ bias, int rows, int C,
-                                                       float *__restrict__ res, const float *__restrict__ inp2) {
+                                                       float *__restrict__ res, const float *__restrict__ inp2, UgkDrop drop) {
+  constexpr bool kRes = kIn != kPlain;
   const int lane = threadIdx.x & (kWave - 1);
   const int row0 = (blockIdx.x * kWavesPerBlock + (threadIdx.x >> 6)) * RPW;
   if (row0 >= rows) return;
@@ -193,7 +198,11 @@ __global__ __launch_bounds__(kBlock) void k_ln_fwd_vec(float *__restrict__ out, 
     for (int v = 0; v < V; v++) {
       xv[v] = xa[v];
       if (kRes) {
-        xv[v] = add4(xv[v], ya[kRes ? v : 0]);
+        float4 y = ya[kRes ? v : 0];
+        if (kIn == kDropSum)
+          y = kRag ? ugk_drop4_at(y, (uint64_t)row * C + cl.at[v], drop)
+                   : ugk_drop4(y, ((uint64_t)row * C + cl.at[v]) >> 2, drop);
+        xv[v] = add4(xv[v], y);
         cl.put(res + (size_t)row * C, v, xv[v]);
       }
     }
@@ -281,12 +290,13 @@ __global__ __launch_bounds__(kBlock) void k_enc_ln_fwd_vec(float *__restrict__ e
 // sum, a wavefront sum and the W wavefronts' sums added in order by every
 // thread, one barrier each. Memory-bound: 4,092 x 4,096 in 26.4 us (5.1 TB/s),
 // 83 us in the lane loop.
-template <int V, int W, bool kRes>
+template <int V, int W, int kIn>
 __global__ __launch_bounds__(W * kWave) void k_ln_fwd_wide(float *__restrict__ out, float *__restrict__ mean,
                                                            float *__restrict__ rstd, const float *__restrict__ inp,
                                                            const float *__restrict__ weight,
                                                            const float *__restrict__ bias, int C,
-                                                           float *__restrict__ res, const float *__restrict__ inp2) {
+                                                           float *__restrict__ res, const float *__restrict__ inp2, UgkDrop drop) {
+  constexpr bool kRes = kIn != kPlain;
   __shared__ float part[2][W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kWave - 1);
   const int row = blockIdx.x;
@@ -301,7 +311,9 @@ __global__ __launch_bounds__(W * kWave) void k_ln_fwd_wide(float *__restrict__ o
   if (kRes) {
 #pragma unroll
     for (int v = 0; v < V; v++) {
-      xv[v] = add4(xv[v], yv[kRes ? v : 0]);
+      float4 y = yv[kRes ? v : 0];
+      if (kIn == kDropSum) y = ugk_drop4_at(y, off + cl.at[v], drop);
+      xv[v] = add4(xv[v], y);
       cl.put(res + off, v, xv[v]);
     }
   }
@@ -1397,34 +1409,34 @@ size_t layernorm_backward_scratch(int rows, int C) {
 
 namespace {
 // Rows of 4 to 8,192 channels, at any alignment.
-template <bool kRes>
+template <int kIn>
 void launch_ln_fwd_rows(float *out, float *mean, float *rstd, const float *inp, const float *weight,
-                        const float *bias, int rows, int C, float *res, const float *inp2) {
+                        const float *bias, int rows, int C, float *res, const float *inp2, const UgkDrop &drop) {
   if (row_in_block(C)) {
     // 4 wavefronts with 3 or 4 float4 per lane up to 4,096 channels, 8 up to 8,192
     const bool w8 = C > 4 * kWave * 4 * 4;
     const int V = slots_of(C, (w8 ? 8 : 4) * kWave);
     const auto go = [&](auto k, int W) {
-      launch(k, dim3(rows), dim3(W * kWave), 0, out, mean, rstd, inp, weight, bias, C, res, inp2);
+      launch(k, dim3(rows), dim3(W * kWave), 0, out, mean, rstd, inp, weight, bias, C, res, inp2, drop);
     };
-    if (!w8 && V <= 3) go(k_ln_fwd_wide<3, 4, kRes>, 4);
-    else if (!w8) go(k_ln_fwd_wide<4, 4, kRes>, 4);
-    else if (V <= 3) go(k_ln_fwd_wide<3, 8, kRes>, 8);
-    else go(k_ln_fwd_wide<4, 8, kRes>, 8);
+    if (!w8 && V <= 3) go(k_ln_fwd_wide<3, 4, kIn>, 4);
+    else if (!w8) go(k_ln_fwd_wide<4, 4, kIn>, 4);
+    else if (V <= 3) go(k_ln_fwd_wide<3, 8, kIn>, 8);
+    else go(k_ln_fwd_wide<4, 8, kIn>, 8);
     return;
   }
   const bool rag = (C & 3) != 0, early = fwd_early(rows, C);
-  const int rpw = rag ? 1 : fwd_rpw(rows, C, kRes);
+  const int rpw = rag ? 1 : fwd_rpw(rows, C, kIn != kPlain);
   const dim3 grid(grid_for((size_t)rows, (size_t)kWavesPerBlock * rpw)), block(kBlock);
-  const auto go = [&](auto k) { launch(k, grid, block, 0, out, mean, rstd, inp, weight, bias, rows, C, res, inp2); };
+  const auto go = [&](auto k) { launch(k, grid, block, 0, out, mean, rstd, inp, weight, bias, rows, C, res, inp2, drop); };
   switch (slots_of(C, kWave)) {
 #define UGK_LN_FWD(v)                                                  \
   case v:                                                              \
-    if (rag && early) go(k_ln_fwd_vec<v, kRes, 1, true, true>);        \
-    else if (rag) go(k_ln_fwd_vec<v, kRes, 1, true, false>);           \
-    else if (early) go(k_ln_fwd_vec<v, kRes, 1, false, true>);         \
-    else if (rpw == 1) go(k_ln_fwd_vec<v, kRes, 1, false, false>);     \
-    else go(k_ln_fwd_vec<v, kRes, 2, false, false>);                   \
+    if (rag && early) go(k_ln_fwd_vec<v, kIn, 1, true, true>);        \
+    else if (rag) go(k_ln_fwd_vec<v, kIn, 1, true, false>);           \
+    else if (early) go(k_ln_fwd_vec<v, kIn, 1, false, true>);         \
+    else if (rpw == 1) go(k_ln_fwd_vec<v, kIn, 1, false, false>);     \
+    else go(k_ln_fwd_vec<v, kIn, 2, false, false>);                   \
     break;
     UGK_LN_FWD(1) UGK_LN_FWD(2) UGK_LN_FWD(3) UGK_LN_FWD(4)
     UGK_LN_FWD(5) UGK_LN_FWD(6) UGK_LN_FWD(7) UGK_LN_FWD(8)
@@ -1441,8 +1453,20 @@ int launch_residual_layernorm_forward(float *res, float *out, float *mean, float
     if (int e = launch_residual_forward(res, x, y, (size_t)rows * C)) return e;
     return launch_layernorm_forward(out, mean, rstd, res, weight, bias, rows, C);
   }
-  launch_ln_fwd_rows<true>(out, mean, rstd, x, weight, bias, rows, C, res, y);
+  launch_ln_fwd_rows<kSum>(out, mean, rstd, x, weight, bias, rows, C, res, y, UgkDrop{});
   return check_launch("residual_layernorm_forward");
+}
+
+int launch_dropout_residual_layernorm_forward(float *res, float *out, float *mean, float *rstd, const float *x,
+                                              const float *y, const float *weight, const float *bias, int rows, int C,
+                                              const UgkDrop &drop) {
+  if (rows == 0) return 0;
+  if (layernorm_exact() || !(row_in_wave(C) || row_in_block(C))) {
+    if (int e = launch_dropout(kDropAddTo, res, nullptr, x, y, (size_t)rows * C, drop)) return e;
+    return launch_layernorm_forward(out, mean, rstd, res, weight, bias, rows, C);
+  }
+  launch_ln_fwd_rows<kDropSum>(out, mean, rstd, x, weight, bias, rows, C, res, y, drop);
+  return check_launch("dropout_residual_layernorm_forward");
 }
 
 int launch_encoder_layernorm_forward(float *enc, float *out, float *mean, float *rstd, int *inp,
@@ -1947,7 +1971,7 @@ int launch_layernorm_forward(float *out, float *mean, float *rstd, const float *
   if (rows == 0) return 0;
   if (layernorm_exact()) return launch_layernorm_forward_exact(out, mean, rstd, inp, weight, bias, rows, C);
   if (row_in_wave(C) || row_in_block(C)) {
-    launch_ln_fwd_rows<false>(out, mean, rstd, inp, weight, bias, rows, C, nullptr, nullptr);
+    launch_ln_fwd_rows<kPlain>(out, mean, rstd, inp, weight, bias, rows, C, nullptr, nullptr, UgkDrop{});
   } else {
     const dim3 grid(grid_for((size_t)rows, kWavesPerBlock)), block(kBlock);
     launch(k_ln_fwd_scalar, grid, block, 0, out, mean, rstd, inp, weight, bias,

@@ -61,6 +61,18 @@ UGK_PHILOX_HD UgkPhilox4 ugk_philox_words(unsigned long long seed, int step, uin
 }
 
 #ifdef __HIPCC__
+// Dropout's parameters. Element i stays where word i % 4 of the Philox block i / 4
+// (counter {i / 4 low, high, step, stream}) is at least `below` = p 2^32, rounded;
+// it is then multiplied by `scale` = 1 / (1 - p). The block serves four elements,
+// so the draw costs a quarter of an eps draw's integer work per element, and the
+// probability is exact to 2^-33.
+struct UgkDrop {
+  unsigned long long seed;
+  int step;
+  uint32_t stream, below;
+  float scale;
+};
+
 // a ^ b ^ k in one v_bitop3_b32 (truth table 0x96), k in a scalar register.
 // Only for a k that is the same in every lane of the wavefront.
 __device__ __forceinline__ uint32_t ugk_xor3_uniform(uint32_t a, uint32_t b, uint32_t k) {
@@ -72,9 +84,10 @@ __device__ __forceinline__ uint32_t ugk_xor3_uniform(uint32_t a, uint32_t b, uin
 // ugk_philox_words for a (seed, step) shared by the whole wavefront (the
 // kernels draw eps(seed, step, i) for their own i): the same rounds, with each
 // round's two three-way xors as one instruction each, the round key scalar.
+// The fourth counter word (0 for eps) keeps streams of one seed and step apart.
 __device__ __forceinline__ UgkPhilox4 ugk_dev_philox_words_uniform(unsigned long long seed, int step,
-                                                                  uint64_t index) {
-  uint32_t c0 = (uint32_t)index, c1 = (uint32_t)(index >> 32), c2 = (uint32_t)step, c3 = 0u;
+                                                                  uint64_t index, uint32_t stream = 0u) {
+  uint32_t c0 = (uint32_t)index, c1 = (uint32_t)(index >> 32), c2 = (uint32_t)step, c3 = stream;
   uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
   for (int r = 0; r < 10; r++) {
@@ -129,5 +142,29 @@ __device__ __forceinline__ float ugk_dev_philox_normal(unsigned long long seed, 
 __device__ __forceinline__ float ugk_dev_philox_normal_fast(unsigned long long seed, int step, uint64_t index) {
   const UgkPhilox4 o = ugk_dev_philox_words_uniform(seed, step, index);
   return ugk_dev_box_muller_fast(o.w[0], o.w[1]);
+}
+
+// Elements 4 block .. 4 block + 3 that stay: v[j] scaled, else +0 (whatever v[j]
+// is, infinities and NaN too). The parameters must be the same across the wavefront.
+__device__ __forceinline__ float4 ugk_drop4(float4 v, uint64_t block, const UgkDrop &d) {
+  const UgkPhilox4 o = ugk_dev_philox_words_uniform(d.seed, d.step, block, d.stream);
+  return make_float4(o.w[0] >= d.below ? v.x * d.scale : 0.0f, o.w[1] >= d.below ? v.y * d.scale : 0.0f,
+                     o.w[2] >= d.below ? v.z * d.scale : 0.0f, o.w[3] >= d.below ? v.w * d.scale : 0.0f);
+}
+
+// The same for elements i .. i + 3, i any number: they lie in two blocks unless i is a multiple of 4.
+__device__ __forceinline__ float4 ugk_drop4_at(float4 v, uint64_t i, const UgkDrop &d) {
+  const unsigned sh = (unsigned)i & 3u;
+  const UgkPhilox4 a = ugk_dev_philox_words_uniform(d.seed, d.step, i >> 2, d.stream);
+  uint32_t w0 = a.w[0], w1 = a.w[1], w2 = a.w[2], w3 = a.w[3];
+  if (sh) {
+    const UgkPhilox4 b = ugk_dev_philox_words_uniform(d.seed, d.step, (i >> 2) + 1, d.stream);
+    w0 = sh == 1 ? a.w[1] : sh == 2 ? a.w[2] : a.w[3];
+    w1 = sh == 1 ? a.w[2] : sh == 2 ? a.w[3] : b.w[0];
+    w2 = sh == 1 ? a.w[3] : sh == 2 ? b.w[0] : b.w[1];
+    w3 = sh == 1 ? b.w[0] : sh == 2 ? b.w[1] : b.w[2];
+  }
+  return make_float4(w0 >= d.below ? v.x * d.scale : 0.0f, w1 >= d.below ? v.y * d.scale : 0.0f,
+                     w2 >= d.below ? v.z * d.scale : 0.0f, w3 >= d.below ? v.w * d.scale : 0.0f);
 }
 #endif

@@ -25,6 +25,10 @@ __all__ = [
     "gelu_forward", "gelu_backward", "residual_forward", "residual_backward",
     "bayes_materialize", "encoder_layernorm_forward", "residual_layernorm_forward", "layernorm_residual_backward",
     "softmax_crossentropy", "crossentropy_softmax_backward", "crossentropy_softmax_backward_zeroed",
+    "dropout_forward", "dropout_backward", "dropout_residual_forward", "dropout_residual_backward",
+    "dropout_residual_layernorm_forward", "layernorm_dropout_residual_backward",
+    "Attention", "attention_forward", "attention_backward", "attention_backward_zeroed", "dense_attention_forward",
+    "dense_attention_backward", "dense_attention_callbacks",
     "bayes_sample", "bayes_backward",
     "bayes_backward_philox", "kl_forward", "kl_backward", "adamw_update", "bbb_step_fused",
     "Loader", "loader_count", "ckpt_path", "ckpt_save", "ckpt_load",
@@ -54,6 +58,30 @@ _fl = ctypes.c_float
 class Config(ctypes.Structure):
     """``Config`` of gpt2_kernels.cuh:634 (ugk_config)."""
     _fields_ = [("B", _i), ("T", _i), ("C", _i), ("V", _i), ("NH", _i), ("maxT", _i), ("L", _i)]
+
+
+class Attention(ctypes.Structure):
+    """``ugk_attention``: the sequences, heads and row strides of an attention call.
+
+    ``q_start``, ``q_end``, ``k_start``, ``k_end`` are int32 device tensors of at least ``nseq`` elements (or
+    device addresses, or None): sequence b is the rows [q_start[b], q_end[b]) of q and [k_start[b], k_end[b]) of k
+    and v. Strides ``ldq``, ``ldk``, ``ldv``, ``ldo`` in floats, 0 for rows without gaps. ``scale`` defaults to
+    1/sqrt(HS). The structure keeps its tensors alive.
+    """
+    _OFFSETS = ("q_start", "q_end", "k_start", "k_end")
+    _fields_ = [(_n, _i) for _n in ("nseq", "NH", "NKV", "HS", "rows_q", "rows_k", "max_q", "max_k", "causal")] + \
+        [("scale", _fl)] + [(_n, _fp) for _n in _OFFSETS] + \
+        [(_n, ctypes.c_longlong) for _n in ("ldq", "ldk", "ldv", "ldo")]
+
+    def __init__(self, nseq: int, NH: int, NKV: int, HS: int, rows_q: int, rows_k: int, max_q: int, max_k: int,
+                 causal: bool = True, scale: Optional[float] = None, q_start=None, q_end=None, k_start=None, k_end=None,
+                 ldq: int = 0, ldk: int = 0, ldv: int = 0, ldo: int = 0):
+        if scale is None:
+            scale = HS ** -0.5 if HS > 0 else 0.0
+        tensors = (q_start, q_end, k_start, k_end)
+        super().__init__(nseq, NH, NKV, HS, rows_q, rows_k, max_q, max_k, 1 if causal else 0, scale,
+                         *(_ptr(t, n, nseq, "i32") for t, n in zip(tensors, self._OFFSETS)), ldq, ldk, ldv, ldo)
+        self._tensors = tensors
 
 
 _MATMUL_FWD = ctypes.CFUNCTYPE(_i, _fp, _fp, _fp, _fp, _fp, _i, _i, _i)
@@ -88,6 +116,17 @@ _SIGS = {
     "ugk_bayes_sample": [_fp, _fp, _fp, _fp, _sz, _u64, _i],
     "ugk_bayes_backward": [_fp, _fp, _fp, _fp, _fp, _sz],
     "ugk_bayes_backward_philox": [_fp, _fp, _fp, _fp, _sz, _u64, _i],
+    "ugk_dropout_forward": [_fp, _fp, _sz, _fl, _u64, _i, _i],
+    "ugk_dropout_backward": [_fp, _fp, _sz, _fl, _u64, _i, _i],
+    "ugk_dropout_residual_forward": [_fp, _fp, _fp, _sz, _fl, _u64, _i, _i],
+    "ugk_dropout_residual_backward": [_fp, _fp, _fp, _sz, _fl, _u64, _i, _i],
+    "ugk_dropout_residual_layernorm_forward": [_fp] * 8 + [_i, _i, _i, _fl, _u64, _i, _i],
+    "ugk_layernorm_dropout_residual_backward": [_fp] * 10 + [_i, _i, _i, _fl, _u64, _i, _i],
+    "ugk_attention_forward": [_fp] * 5 + [Attention],
+    "ugk_attention_backward": [_fp] * 9 + [Attention],
+    "ugk_attention_backward_zeroed": [_fp] * 9 + [Attention],
+    "ugk_dense_attention_forward": [_fp, _fp, _fp, _i, _i, _i, _i],
+    "ugk_dense_attention_backward": [_fp, _fp, _fp, _fp, _i, _i, _i, _i],
     "ugk_kl_forward": [ctypes.POINTER(ctypes.c_double), _fp, _fp, _sz, _fl],
     "ugk_kl_backward": [_fp, _fp, _fp, _fp, _sz, _fl, _fl],
     "ugk_adamw_update": [_fp, _fp, _fp, _fp, _sz, _i, _fl, _fl, _fl, _fl, _fl],
@@ -373,6 +412,122 @@ def _xent_backward(name, dlogits, probs, targets, B: int, T: int, V: int, zeroed
     args = (_ptr(dlogits, "dlogits", n, "f32"), _ptr(probs, "probs", n, "f32"), _ptr(targets, "targets", rows, "i32"),
             B, T, V)
     _check(lib.ugk_crossentropy_softmax_backward_checked(*args, zeroed) if checked else getattr(lib, "ugk_" + name)(*args))
+
+
+def dropout_forward(out, inp, n: int, p: float, seed: int, step: int, site: int = 0) -> None:
+    """``out = dropout(inp)``: element i is kept and multiplied by 1/(1-p) where word ``i % 4`` of Philox block
+    ``i // 4`` of (seed, step, site) is at least p * 2^32, else +0. The mask is drawn again by every call that
+    names the same (seed, step, site). No counterpart in the reference."""
+    _check(lib.ugk_dropout_forward(_ptr(out, "out", n, "f32"), _ptr(inp, "inp", n, "f32"), n, p, seed, step, site))
+
+
+def dropout_backward(dinp, dout, n: int, p: float, seed: int, step: int, site: int = 0) -> None:
+    """``dinp += dropout(dout)`` with the forward's mask."""
+    _check(lib.ugk_dropout_backward(_ptr(dinp, "dinp", n, "f32"), _ptr(dout, "dout", n, "f32"), n, p, seed, step, site))
+
+
+def dropout_residual_forward(out, x, y, n: int, p: float, seed: int, step: int, site: int = 0) -> None:
+    """``out = x + dropout(y)``."""
+    _check(lib.ugk_dropout_residual_forward(_ptr(out, "out", n, "f32"), _ptr(x, "x", n, "f32"), _ptr(y, "y", n, "f32"), n,
+                                            p, seed, step, site))
+
+
+def dropout_residual_backward(dx, dy, dout, n: int, p: float, seed: int, step: int, site: int = 0) -> None:
+    """``dx += dout``; ``dy += dropout(dout)``."""
+    _check(lib.ugk_dropout_residual_backward(_ptr(dx, "dx", n, "f32"), _ptr(dy, "dy", n, "f32"),
+                                             _ptr(dout, "dout", n, "f32"), n, p, seed, step, site))
+
+
+def dropout_residual_layernorm_forward(res, out, mean, rstd, x, y, weight, bias, B: int, T: int, C: int, p: float,
+                                       seed: int, step: int, site: int = 0) -> None:
+    """``dropout_residual_forward(res, x, y)`` then ``layernorm_forward(out, mean, rstd, res, ...)``, one pass."""
+    n, rows = B * T * C, B * T
+    _check(lib.ugk_dropout_residual_layernorm_forward(
+        _ptr(res, "res", n, "f32"), _ptr(out, "out", n, "f32"), _ptr(mean, "mean", rows, "f32"),
+        _ptr(rstd, "rstd", rows, "f32"), _ptr(x, "x", n, "f32"), _ptr(y, "y", n, "f32"),
+        _ptr(weight, "weight", C, "f32"), _ptr(bias, "bias", C, "f32"), B, T, C, p, seed, step, site))
+
+
+def layernorm_dropout_residual_backward(dinp, dweight, dbias, dx, dy, dout, inp, weight, mean, rstd, B: int, T: int,
+                                        C: int, p: float, seed: int, step: int, site: int = 0) -> None:
+    """``layernorm_backward`` then ``dropout_residual_backward(dx, dy, dinp)``."""
+    n, rows = B * T * C, B * T
+    _check(lib.ugk_layernorm_dropout_residual_backward(
+        _ptr(dinp, "dinp", n, "f32"), _ptr(dweight, "dweight", C, "f32"), _ptr(dbias, "dbias", C, "f32"),
+        _ptr(dx, "dx", n, "f32"), _ptr(dy, "dy", n, "f32"), _ptr(dout, "dout", n, "f32"),
+        _ptr(inp, "inp", n, "f32"), _ptr(weight, "weight", C, "f32"), _ptr(mean, "mean", rows, "f32"),
+        _ptr(rstd, "rstd", rows, "f32"), B, T, C, p, seed, step, site))
+
+
+def _rows_ptr(x, what: str, rows: int, ld: int, width: int):
+    """Device address of ``x``, the first of ``rows`` rows of ``width`` floats, ``ld`` (0: width) apart. A tensor may
+    be a view into the buffer that holds the rows: what counts is the memory behind its first element."""
+    if x is None or isinstance(x, int):
+        return x
+    torch = _torch or _import_torch()
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what}: expected a torch tensor or a device address, got {type(x)!r}")
+    if x.device.type != "cuda":
+        raise ValueError(f"{what}: tensor must be on the GPU, got {x.device}")
+    if x.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensor is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if x.dtype != torch.float32:
+        raise TypeError(f"{what}: dtype must be {torch.float32}, got {x.dtype}")
+    need = (rows - 1) * (ld or width) + width if rows > 0 else 0
+    has = x.untyped_storage().nbytes() // 4 - x.storage_offset()
+    if x.numel() == 0 and need or has < need:
+        raise ValueError(f"{what}: needs at least {need} elements from its first one on, has {has}")
+    return x.data_ptr()
+
+
+def _attention_ptrs(a: Attention, q, k, v, out):
+    q_w, k_w = a.NH * a.HS, a.NKV * a.HS
+    return ([_rows_ptr(x, n, a.rows_q, a.ldq, q_w) for n, x in q] + [_rows_ptr(x, n, a.rows_k, a.ldk, k_w) for n, x in k] +
+            [_rows_ptr(x, n, a.rows_k, a.ldv, k_w) for n, x in v] + [_rows_ptr(x, n, a.rows_q, a.ldo, q_w) for n, x in out])
+
+
+def attention_forward(out, lse, q, k, v, a: Attention) -> None:
+    """gpt2_kernels.cuh:416-498, for grouped heads, sequences of different lengths and a cache too: per query row and
+    head ``out = softmax(scale q.k) v`` over the allowed keys and ``lse = log sum exp`` (rows_q, NH), which may be
+    None. q, k, v and out may be views into rows that hold other things as well (strides in ``a``)."""
+    pq, pk, pv, po = _attention_ptrs(a, [("q", q)], [("k", k)], [("v", v)], [("out", out)])
+    _check(lib.ugk_attention_forward(po, _ptr(lse, "lse", a.rows_q * a.NH, "f32"), pq, pk, pv, a))
+
+
+def attention_backward(dq, dk, dv, dout, q, k, v, out, lse, a: Attention) -> None:
+    """gpt2_kernels.cuh:500-619: the gradients of attention_forward added to dq, dk and dv."""
+    _attention_backward(lib.ugk_attention_backward, dq, dk, dv, dout, q, k, v, out, lse, a)
+
+
+def attention_backward_zeroed(dq, dk, dv, dout, q, k, v, out, lse, a: Attention) -> None:
+    """attention_backward for dq, dk and dv that are zero before the call: they are written, not read."""
+    _attention_backward(lib.ugk_attention_backward_zeroed, dq, dk, dv, dout, q, k, v, out, lse, a)
+
+
+def _attention_backward(fn, dq, dk, dv, dout, q, k, v, out, lse, a: Attention) -> None:
+    pdq, pq, pdk, pk, pdv, pv, pdo, po = _attention_ptrs(a, [("dq", dq), ("q", q)], [("dk", dk), ("k", k)],
+                                                         [("dv", dv), ("v", v)], [("dout", dout), ("out", out)])
+    _check(fn(pdq, pdk, pdv, pdo, pq, pk, pv, po, _ptr(lse, "lse", a.rows_q * a.NH, "f32"), a))
+
+
+def dense_attention_forward(out, qkv, B: int, T: int, C: int, NH: int) -> None:
+    """attention_forward of qkv rows (3C), as the step driver's callback takes it (``dense_attention_callbacks``)."""
+    n = B * T * C
+    _check(lib.ugk_dense_attention_forward(None, _ptr(out, "out", n, "f32"), _ptr(qkv, "qkv", 3 * n, "f32"), B, T, C, NH))
+
+
+def dense_attention_backward(dqkv, dout, qkv, B: int, T: int, C: int, NH: int) -> None:
+    """``dqkv +=`` the gradient of dense_attention_forward, whose out and lse are computed again."""
+    n = B * T * C
+    _check(lib.ugk_dense_attention_backward(None, _ptr(dqkv, "dqkv", 3 * n, "f32"), _ptr(dout, "dout", n, "f32"),
+                                            _ptr(qkv, "qkv", 3 * n, "f32"), B, T, C, NH))
+
+
+def dense_attention_callbacks() -> dict:
+    """The library's own attention as DenseOps fields: ``DenseOps(matmul_forward=..., matmul_backward=...,
+    **dense_attention_callbacks())``. They run native code only."""
+    return {"attention_forward": ctypes.cast(lib.ugk_dense_attention_forward, _ATTN_FWD),
+            "attention_backward": ctypes.cast(lib.ugk_dense_attention_backward, _ATTN_BWD)}
 
 
 def bayes_sample(w, eps, mu, rho, n: int, seed: int, step: int) -> None:
