@@ -10,6 +10,7 @@
 #include <math.h>
 
 #include "ugk_internal.h"
+#include "ugk_split.h"
 
 namespace ugk {
 namespace {
@@ -89,18 +90,387 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
   if (lse && lane == 0) *lse = n ? m + logf(l) : -INFINITY;
 }
 
-__global__ __launch_bounds__(kBlock) void k_att_fwd_rows(float *out, float *lse, const float *q, const float *k,
-                                                         const float *v, ugk_attention a, int *word) {
-  const int per = (a.max_q + kBlock / kWave - 1) / (kBlock / kWave);
-  const int b = blockIdx.x / (a.NH * per), h = blockIdx.x / per % a.NH, part = blockIdx.x % per;
-  const Seq s = sequence(a, b, h == 0 && part == 0, word, UGK_IDS_ATTENTION_FORWARD);
-  const int i = part * (kBlock / kWave) + (threadIdx.x >> 6);
+// ---- forward, tiles on the matrix units -----------------------------------------
+//
+// The rows of a tile are (query row, head of the group) pairs, so that the heads
+// of a group share the key and value tiles: row r of a sequence and key/value
+// head is query row r / G, head r % G of the group. A wavefront holds 32 rows; a
+// workgroup of W wavefronts goes over the keys BK at a time.
+//
+// S^T = K Q^T: a lane then holds one row's scores of half of the keys (the other half
+// in lane ^ 32), so that the row's maximum, sum and factors are values of the
+// lane, and its 16 registers of a 32 x 32 block are, rounded to halves, the
+// operand of O^T += V^T P^T as they stand, with the keys in the order 16 c + 8
+// (j / 4) + 4 (lane / 32) + j % 4: V^T is laid out in that order. Nothing moves
+// between lanes but one exchange of halves per tile.
+//
+// Products are split (ugk_split.h). K and V are split while they are put into LDS, by the
+// exponent of the tile's largest magnitude (V: of all tiles so far, the
+// accumulators being rescaled when it grows); the maximum is taken over the
+// registers that the tile was loaded into, one tile ahead, and goes through LDS with
+// the barrier that the tile buffers need anyway: one barrier per tile. P lies
+// in (0, 1] and is scaled by 2^15 in its exponent.
+//
+// The workgroup's rows are taken one by one instead (row_forward), where a masked key
+// is not touched at all, if a tile holds an infinity or NaN; if not all rows see
+// all of a tile and its keys' magnitudes lie further apart than the halves'
+// digits allow (a row would lose its digits to keys that it must not see); or if
+// scores leave the range of the above (2^22 in base 2).
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+// One part of a split key axis: o normalised, and lse, per row.
+struct Parts {
+  float *o, *lse;    // null: not split
+  int splits, chunk; // keys per part
+};
+
+template <bool kFull>
+__device__ __forceinline__ float4 load4(const float *p, int nd) {
+  if (kFull || nd >= 4) return ld4(p);
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (nd > 0) v.x = p[0];
+  if (nd > 1) v.y = p[1];
+  if (nd > 2) v.z = p[2];
+  return v;
+}
+// Rows j .. j + 3 of [0, n): past it, zero (n > 0). tail: some of the tile's rows are.
+template <bool kFull>
+__device__ __forceinline__ Rows4 load_rows(const float *base, long long ld, int j, int n, bool tail, int nd) {
+  Rows4 t;
+  if (tail) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      t.r[r] = load4<kFull>(base + min(j + r, n - 1) * ld, nd);
+      if (j + r >= n) t.r[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+  } else {
+    const float *p = base + j * ld;
+#pragma unroll
+    for (int r = 0; r < 4; r++, p += ld) t.r[r] = load4<kFull>(p, nd);
+  }
+  return t;
+}
+__device__ __forceinline__ float part4(const float4 &v, int d) { return d == 0 ? v.x : d == 1 ? v.y : d == 2 ? v.z : v.w; }
+
+// The block's rows, scaled and split, to row-major halves (h, l: the two parts' arrays, `stride` halves a row).
+__device__ __forceinline__ void put_rows(const Rows4 &t, float scale, _Float16 *h, _Float16 *l, int stride) {
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    uint32_t h0, h1, l0, l1;
+    split2(t.r[r].x * scale, t.r[r].y * scale, h0, l0);
+    split2(t.r[r].z * scale, t.r[r].w * scale, h1, l1);
+    *reinterpret_cast<v2u *>(h + r * stride) = v2u{h0, h1};
+    *reinterpret_cast<v2u *>(l + r * stride) = v2u{l0, l1};
+  }
+}
+// The same transposed: row d of the arrays gets the block's column d.
+__device__ __forceinline__ void put_cols(const Rows4 &t, float scale, _Float16 *h, _Float16 *l, int stride) {
+#pragma unroll
+  for (int d = 0; d < 4; d++) {
+    uint32_t h0, h1, l0, l1;
+    split2(part4(t.r[0], d) * scale, part4(t.r[1], d) * scale, h0, l0);
+    split2(part4(t.r[2], d) * scale, part4(t.r[3], d) * scale, h1, l1);
+    *reinterpret_cast<v2u *>(h + d * stride) = v2u{h0, h1};
+    *reinterpret_cast<v2u *>(l + d * stride) = v2u{l0, l1};
+  }
+}
+// Where a group of four keys (key / 4) stands in a row of V^T.
+__device__ __forceinline__ int key_slot(int group) { return group / 4 * 16 + (group & 1) * 8 + (group >> 1 & 1) * 4; }
+
+__device__ __forceinline__ v8h frag(const _Float16 *p) { return *reinterpret_cast<const v8h *>(p); }
+
+// Eight floats from d on of a row, as operands.
+template <bool kFull>
+__device__ __forceinline__ void load8(const float *p, int d, int HS, bool live, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const float4 v = live ? load4<kFull>(p + d + 4 * j, HS - d - 4 * j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
+  }
+}
+__device__ __forceinline__ void split8(const float (&x)[8], float scale, v8h &h, v8h &l) {
+  v4u a, b;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    uint32_t hj, lj;
+    split2(x[2 * j] * scale, x[2 * j + 1] * scale, hj, lj);
+    a[j] = hj;
+    b[j] = lj;
+  }
+  h = __builtin_bit_cast(v8h, a);
+  l = __builtin_bit_cast(v8h, b);
+}
+
+template <int HSP, int BK, int W, bool kFull>
+__global__ __launch_bounds__(W * kWave, W == 1 ? 1 : 2) void k_att_fwd(float *out, float *lse, const float *q, const float *k,
+                                                       const float *v, ugk_attention a, Parts parts, unsigned pairs,
+                                                       int *word) {
+  constexpr int kThreads = W * kWave, KB = BK / 32, DC = HSP / 16, DB = HSP / 32, DG = HSP / 4;
+  constexpr int kBlocks = BK / 4 * DG, kPer = 2 * kBlocks / kThreads;  // 4 x 4 blocks: of K and of V, per thread
+  static_assert(kBlocks % kThreads == 0, "as many blocks of K and of V for each thread");
+  constexpr int kKs = HSP + 8, kVs = BK + 8;  // strides: odd multiples of 16 bytes, free of bank conflicts
+  __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kKs], lv[2][2][HSP * kVs];
+  __shared__ uint32_t slot[2][4][W];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
+  const unsigned pair = blockIdx.x % pairs;
+  const int tile = (int)(gridDim.x / pairs - 1 - blockIdx.x / pairs);  // the longest rows first
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
+  const Seq s = sequence(a, b, hk == 0 && tile == 0 && blockIdx.y == 0, word, UGK_IDS_ATTENTION_FORWARD);
+  const int rows = s.Lq * G, row0 = tile * (32 * W);
+  if (row0 >= rows) return;
+  const float *kb = k + (size_t)s.k0 * a.ldk + hk * a.HS, *vb = v + (size_t)s.k0 * a.ldv + hk * a.HS;
+  // this part's keys, and those that the workgroup's last row sees
+  const int first = parts.o ? min((int)blockIdx.y * parts.chunk, s.Lk) : 0;
+  const int stop = parts.o ? min(first + parts.chunk, s.Lk) : s.Lk;
+  const int n = max(first, min(stop, s.seen((min(row0 + 32 * W, rows) - 1) / G, a.causal)));
+  const int least = s.seen(row0 / G, a.causal);  // what every row of the workgroup sees
+
+  // this lane's row
+  const int r = row0 + wave * 32 + (lane & 31);
+  const bool live = r < rows;
+  const int i = r / G, h = hk * G + r % G;
+  const int lim = live ? min(n, s.seen(i, a.causal)) : 0;
+  int lo = live ? lim : n, hi = lim;  // least and most over the wavefront
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  const size_t grow = (size_t)s.q0 + (live ? i : 0);
+  const float *qr = q + grow * a.ldq + (live ? h : 0) * a.HS;
+  v8h qh[DC], ql[DC];
+  float cq;  // of the scores, to base 2
+  {
+    float x[DC][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int c = 0; c < DC; c++) {
+      load8<kFull>(qr, 16 * c + 8 * half, a.HS, live, x[c]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) m = max(m, abs_bits(x[c][j]));
+    }
+    const int e = split_exp(half_max_bits(m));
+    const float f = a.scale < 0.0f ? -split_scale(e) : split_scale(e);
+#pragma unroll
+    for (int c = 0; c < DC; c++) split8(x[c], f, qh[c], ql[c]);
+    cq = split_unscale(e) * (fabsf(a.scale) * kLog2e);
+  }
+
+  Rows4 t[kPer];
+  const auto is_v = [&](int u) { return u >= kPer / 2; };
+  const auto block = [&](int u) { return (tid + u * kThreads) % kBlocks; };
+  const auto load = [&](int k0) {
+    const bool tail = k0 + BK > n;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const int d = block(u) % DG * 4, j = k0 + block(u) / DG * 4;
+      t[u] = load_rows<kFull>((is_v(u) ? vb : kb) + d, is_v(u) ? a.ldv : a.ldk, j, n, tail, a.HS - d);
+    }
+  };
+  // The tile's largest magnitudes, of K and V, and where not all rows see all of it
+  // the least of the keys' largest.
+  const auto note = [&](int at, int k0) {
+    uint32_t m[4] = {};
+#pragma unroll
+    for (int u = 0; u < kPer; u++) m[is_v(u) ? 1 : 0] = max_abs(m[is_v(u) ? 1 : 0], t[u]);
+    if (k0 + BK > least) {
+#pragma unroll
+      for (int u = 0; u < kPer; u++) m[is_v(u) ? 3 : 2] = least_row<DG>(m[is_v(u) ? 3 : 2], t[u]);
+      m[2] = wave_max_bits(m[2]);
+      m[3] = wave_max_bits(m[3]);
+    }
+    m[0] = wave_max_bits(m[0]);
+    m[1] = wave_max_bits(m[1]);
+    if (lane == 0) {
+#pragma unroll
+      for (int x = 0; x < 4; x++) slot[at][x][wave] = m[x];
+    }
+  };
+  const auto noted = [&](int at, int which) {
+    uint32_t m = slot[at][which][0];
+#pragma unroll
+    for (int w = 1; w < W; w++) m = max(m, slot[at][which][w]);
+    return (uint32_t)__builtin_amdgcn_readfirstlane(m);
+  };
+  bool bad = false;
+  int ek = 0, ev = -100, ek_next = 0, ev_next = -100;
+  const auto stage = [&](int at) {
+    const uint32_t mk = noted(at, 0), mv = noted(at, 1);
+    bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted(at, 2)) || too_wide(mv, noted(at, 3));
+    ek_next = split_exp(mk);
+    ev_next = max(ev_next, split_exp(mv));
+    const float fk = split_scale(ek_next), fv = split_scale(ev_next);
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const int d = block(u) % DG * 4, g = block(u) / DG;
+      if (is_v(u)) put_cols(t[u], fv, lv[at][0] + d * kVs + key_slot(g), lv[at][1] + d * kVs + key_slot(g), kVs);
+      else put_rows(t[u], fk, lk[at][0] + 4 * g * kKs + d, lk[at][1] + 4 * g * kKs + d, kKs);
+    }
+  };
+
+  v16f o[DB] = {};
+  float l = 0.0f, bias = INFINITY;  // bias: 15 - the row's maximum so far
+  const auto compute = [&](int at, int k0, int ev_now) {
+    v16f sc[KB] = {};
+#pragma unroll
+    for (int c = 0; c < DC; c++)
+#pragma unroll
+      for (int x = 0; x < KB; x++) {
+        const int p = (32 * x + (lane & 31)) * kKs + 16 * c + 8 * half;
+        sc[x] = mfma3(frag(lk[at][0] + p), frag(lk[at][1] + p), qh[c], ql[c], sc[x]);
+      }
+    const float c2 = fmaxf(cq * split_unscale(ek), 0x1p-126f);
+    if (k0 + BK > lo) {  // some row does not see all of the tile
+      const int rel = lim - k0 - 4 * half;
+#pragma unroll
+      for (int x = 0; x < KB; x++)
+#pragma unroll
+        for (int y = 0; y < 16; y++)
+          if (32 * x + 8 * (y / 4) + y % 4 >= rel) sc[x][y] = -INFINITY;
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < KB; x++)
+#pragma unroll
+      for (int y = 0; y < 16; y++) m = fmaxf(m, sc[x][y]);
+    m = half_max(m) * c2;
+    bad = bad || (fabsf(m) >= 0x1p22f && m != -INFINITY) || c2 > 0x1p100f;
+    const float was = bias;
+    bias = fminf(bias, 15.0f - m);
+    const float b0 = bias == INFINITY ? 0.0f : bias;  // no key so far: every score is -inf
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < KB; x++)
+#pragma unroll
+      for (int y = 0; y < 16; y++) {
+        sc[x][y] = __builtin_amdgcn_exp2f(fmaf(sc[x][y], c2, b0));
+        sum += sc[x][y];
+      }
+    const float keep = was == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(b0 - was);
+    l = fmaf(l, keep, sum);
+    if (__any(keep != 1.0f) || ev != ev_now) {
+      const float f = keep * pow2(max(ev - ev_now, -126));
+      ev = ev_now;
+#pragma unroll
+      for (int x = 0; x < DB; x++)
+#pragma unroll
+        for (int y = 0; y < 16; y++) o[x][y] *= f;
+    }
+#pragma unroll
+    for (int c = 0; c < 2 * KB; c++) {
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[j] = sc[c / 2][8 * (c % 2) + j];
+      v8h ph, pl;
+      split8(p, 1.0f, ph, pl);
+#pragma unroll
+      for (int x = 0; x < DB; x++) {
+        const int at_v = (32 * x + (lane & 31)) * kVs + 16 * c + 8 * half;
+        o[x] = mfma3(frag(lv[at][0] + at_v), frag(lv[at][1] + at_v), ph, pl, o[x]);
+      }
+    }
+  };
+
+  const int tiles = (n - first + BK - 1) / BK;
+  if (tiles > 0) {
+    load(first);
+    note(0, first);
+    __syncthreads();
+    stage(0);
+    if (tiles > 1) {
+      load(first + BK);
+      note(1, first + BK);
+    }
+    __syncthreads();
+    for (int at = 0; at < tiles; at++) {
+      const int k0 = first + at * BK;
+      const int ev_now = ev_next;
+      ek = ek_next;
+      // tile at + 1: its maxima are noted, its buffer was read two barriers ago
+      if (at + 1 < tiles) stage((at + 1) & 1);
+      if (at + 2 < tiles) load(k0 + 2 * BK);
+      if (k0 < hi) compute(at & 1, k0, ev_now);
+      if (at + 2 < tiles) note(at & 1, k0 + 2 * BK);
+      __syncthreads();
+    }
+  }
+  // Any wavefront's trouble with a tile is every wavefront's; with its scores its own.
+  if (__any(bad)) {
+    for (int x = 0; x < 32; x++) {
+      const int rr = row0 + wave * 32 + x;
+      if (rr >= rows) break;
+      const int ii = rr / G, hh = hk * G + rr % G;
+      const size_t g = (size_t)s.q0 + ii;
+      const int upto = min(n, s.seen(ii, a.causal));
+      float *po = parts.o ? parts.o + (((size_t)blockIdx.y * a.nseq + b) * a.max_q + ii) * a.NH * a.HS + (size_t)hh * a.HS
+                          : out + g * a.ldo + hh * a.HS;
+      float *pl = parts.o ? parts.lse + (((size_t)blockIdx.y * a.nseq + b) * a.max_q + ii) * a.NH + hh
+                          : lse ? lse + g * a.NH + hh : nullptr;
+      row_forward(po, pl, q + g * a.ldq + hh * a.HS, kb + first * a.ldk, vb + first * a.ldv, max(upto - first, 0), a.HS,
+                  a.ldk, a.ldv, a.scale);
+    }
+    return;
+  }
+  if (!live) return;
+  l = half_sum(l);
+  const size_t prow = ((size_t)blockIdx.y * a.nseq + b) * a.max_q + i;
+  const bool some = lim > first;
+  const float f = some ? split_unscale(ev) / l : 0.0f;
+  float *po = parts.o ? parts.o + prow * a.NH * a.HS + (size_t)h * a.HS : out + grow * a.ldo + h * a.HS;
+#pragma unroll
+  for (int x = 0; x < DB; x++)
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+      const int d = 32 * x + 8 * y + 4 * half;
+      const float4 w = make_float4(o[x][4 * y] * f, o[x][4 * y + 1] * f, o[x][4 * y + 2] * f, o[x][4 * y + 3] * f);
+      if (kFull || d + 4 <= a.HS) {
+        st4(po + d, w);
+      } else {
+        if (d < a.HS) po[d] = w.x;
+        if (d + 1 < a.HS) po[d + 1] = w.y;
+        if (d + 2 < a.HS) po[d + 2] = w.z;
+      }
+    }
+  if (half == 0 && (parts.o || lse)) {
+    const float L = some ? (__builtin_amdgcn_logf(l) - bias) * kLn2 : -INFINITY;
+    if (parts.o) parts.lse[prow * a.NH + h] = L;
+    else lse[grow * a.NH + h] = L;
+  }
+}
+
+// The parts of a split key axis joined, one wavefront per row and head: out =
+// sum_x e^(lse_x - lse) o_x, in the parts' order.
+__global__ __launch_bounds__(kBlock) void k_att_join(float *out, float *lse, Parts parts, ugk_attention a) {
+  const size_t at = (size_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6), per = (size_t)a.nseq * a.max_q * a.NH;
+  if (at >= per) return;
+  const int lane = threadIdx.x & (kWave - 1), h = at % a.NH, i = at / a.NH % a.max_q, b = at / a.NH / a.max_q;
+  const Seq s = sequence(a, b, false, nullptr, 0);
   if (i >= s.Lq) return;
-  const size_t row = s.q0 + i;
-  const int hk = h / (a.NH / a.NKV);
-  row_forward(out + row * a.ldo + h * a.HS, lse ? lse + row * a.NH + h : nullptr, q + row * a.ldq + h * a.HS,
-              k + (size_t)s.k0 * a.ldk + hk * a.HS, v + (size_t)s.k0 * a.ldv + hk * a.HS, s.seen(i, a.causal), a.HS,
-              a.ldk, a.ldv, a.scale);
+  float m = -INFINITY;
+  for (int x = lane; x < parts.splits; x += kWave) {
+    const float y = parts.lse[x * per + at];
+    m = y != y ? INFINITY : fmaxf(m, y);  // NaN: every weight below is then NaN
+  }
+  m = wave_max(m);
+  float o0 = 0.0f, o1 = 0.0f, l = 0.0f;
+  const int d0 = min(lane, a.HS - 1), d1 = min(lane + kWave, a.HS - 1);
+  for (int x = 0; x < parts.splits; x++) {
+    const float y = parts.lse[x * per + at];
+    if (y == -INFINITY) continue;  // a part without a key of this row
+    const float w = expf(y - m), *o = parts.o + (x * per + at) * a.HS;
+    l += w;
+    o0 = fmaf(w, o[d0], o0);
+    o1 = fmaf(w, o[d1], o1);
+  }
+  const bool none = m == -INFINITY;
+  const float r = none ? 1.0f : l;
+  const size_t g = (size_t)s.q0 + i;
+  float *po = out + g * a.ldo + h * a.HS;
+  if (lane < a.HS) po[lane] = o0 / r;
+  if (lane + kWave < a.HS) po[lane + kWave] = o1 / r;
+  if (lse && lane == 0) lse[g * a.NH + h] = none ? -INFINITY : m + logf(l);
 }
 
 __device__ __forceinline__ void put(float *p, float x, bool assign) { *p = assign ? x : *p + x; }
@@ -198,14 +568,81 @@ __global__ __launch_bounds__(kBlock) void k_att_dkv_rows(float *dk, float *dv, c
 
 }  // namespace
 
-size_t attention_parts_bytes(const ugk_attention &) { return 0; }
-size_t attention_parts_bound() { return 0; }
+namespace {
+int cu_count() {
+  static const int n = [] {
+    int dev = 0, c = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) {
+      (void)hipGetLastError();
+      c = 0;
+    }
+    return c > 0 ? c : 256;
+  }();
+  return n;
+}
 
-int launch_attention_forward(float *out, float *lse, const float *q, const float *k, const float *v, float *,
+constexpr size_t kMaxParts = 1 << 15;  // rows of a head that the parts hold at most
+
+// How the forward of `a` is cut: wavefronts of a workgroup, key tile, parts of the key axis.
+struct FwdPlan {
+  int W, BK, tiles, splits, chunk;
+};
+FwdPlan fwd_plan(const ugk_attention &a) {
+  const long long pairs = (long long)a.nseq * a.NKV, rows = (long long)a.max_q * (a.NH / a.NKV);
+  const auto tiles = [&](int W) { return (rows + 32 * W - 1) / (32 * W); };
+  FwdPlan p{};
+  p.W = pairs * tiles(4) >= cu_count() ? 4 : 1;
+  p.BK = a.HS <= 64 && p.W == 4 ? 64 : 32;
+  p.tiles = (int)tiles(p.W);
+  p.splits = 1;
+  const long long wgs = pairs * p.tiles, prow = (long long)a.nseq * a.max_q * a.NH;
+  long long want = 2 * cu_count() / (wgs > 0 ? wgs : 1);
+  want = min(want, (long long)a.max_k / (4 * p.BK));
+  want = min(want, (long long)kMaxParts / (prow > 0 ? prow : 1));
+  if (want > 1) {
+    p.chunk = (int)((a.max_k + want - 1) / want + p.BK - 1) / p.BK * p.BK;
+    p.splits = (a.max_k + p.chunk - 1) / p.chunk;
+  }
+  return p;
+}
+size_t parts_lse(const ugk_attention &a, const FwdPlan &p) { return (size_t)p.splits * a.nseq * a.max_q * a.NH; }
+}  // namespace
+
+size_t attention_parts_bytes(const ugk_attention &a) {
+  const FwdPlan p = fwd_plan(a);
+  return p.splits > 1 ? parts_lse(a, p) * (a.HS + 1) * sizeof(float) : 0;
+}
+size_t attention_parts_bound() { return kMaxParts * (kMaxHead + 1) * sizeof(float); }
+
+int launch_attention_forward(float *out, float *lse, const float *q, const float *k, const float *v, float *mem,
                              const ugk_attention &a, int *word) {
-  const unsigned per = grid_for((size_t)a.max_q, kBlock / kWave);
-  launch(k_att_fwd_rows, dim3(per * a.NH * a.nseq), dim3(kBlock), 0, out, lse, q, k, v, a, word);
-  return check_launch("attention_forward");
+  const FwdPlan p = fwd_plan(a);
+  Parts parts{};
+  if (p.splits > 1) {
+    parts.lse = mem;
+    parts.o = mem + parts_lse(a, p);
+    parts.splits = p.splits;
+    parts.chunk = p.chunk;
+  }
+  const unsigned pairs = (unsigned)a.nseq * a.NKV;
+  const auto go = [&](auto kernel) {
+    launch(kernel, dim3(pairs * p.tiles, p.splits), dim3(p.W * kWave), 0, out, lse, q, k, v, a, parts, pairs, word);
+  };
+  if (a.HS <= 64) {
+    const bool full = a.HS == 64;
+    if (p.W == 4) full ? go(k_att_fwd<64, 64, 4, true>) : go(k_att_fwd<64, 64, 4, false>);
+    else full ? go(k_att_fwd<64, 32, 1, true>) : go(k_att_fwd<64, 32, 1, false>);
+  } else {
+    const bool full = a.HS == 128;
+    if (p.W == 4) full ? go(k_att_fwd<128, 32, 4, true>) : go(k_att_fwd<128, 32, 4, false>);
+    else full ? go(k_att_fwd<128, 32, 1, true>) : go(k_att_fwd<128, 32, 1, false>);
+  }
+  if (int e = check_launch("attention_forward")) return e;
+  if (p.splits > 1) {
+    launch(k_att_join, dim3(grid_for((size_t)a.nseq * a.max_q * a.NH, kBlock / kWave)), dim3(kBlock), 0, out, lse, parts, a);
+    return check_launch("attention_forward");
+  }
+  return UGK_OK;
 }
 
 int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout, const float *q, const float *k,

@@ -1,0 +1,130 @@
+// ugk_split.h - products of single-precision matrices on the half-precision
+// matrix units of gfx950.
+//
+// A float x, scaled by a power of two so that the largest of its row or tile
+// lies in [2^14, 2^15), is held as h + l with h = half(x), l = half(x - h), both
+// rounded to nearest. Each has 11 bits: |x - h| <= 2^-12 |x|, |x - h - l| <=
+// 2^-24 |x| as long as l is a normal half (|x| >= 2^-2, or 2^-16 of the largest);
+// below that the error stays under 2^-25, that is 2^-39 of the largest. A product x y is
+// taken as xh yh + xl yh + xh yl in single-precision accumulators; the part left
+// out, xl yl, is at most 2^-24 |x y|. So a product is within about three
+// roundings of single precision, for three times the half-precision units' work: they
+// do 16 times the operations of the single-precision ones (v_mfma_f32_32x32x16_f16
+// takes 32 cycles, v_mfma_f32_32x32x2_f32 64 for an eighth of the products), so
+// this has a ceiling of 5.3 times theirs. (Three bfloat16 parts would keep
+// the exponent range without scaling, but need six products.)
+#pragma once
+
+#include "ugk_internal.h"
+
+namespace ugk {
+namespace {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+// C += A B for a 32 x 32 tile over 16 products. Lane t holds row (of A) or column (of B)
+// t % 32, products 8 (t / 32) .. + 7; of C column t % 32 and in register r row
+// 8 (r / 4) + 4 (t / 32) + r % 4.
+__device__ __forceinline__ v16f mfma(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+// The same of two split operands.
+__device__ __forceinline__ v16f mfma3(v8h ah, v8h al, v8h bh, v8h bl, v16f c) {
+  return mfma(ah, bl, mfma(al, bh, mfma(ah, bh, c)));
+}
+
+// Two floats as halves: h, and l of what h leaves.
+__device__ __forceinline__ void split2(float x, float y, uint32_t &h, uint32_t &l) {
+  const v2f v = {x, y};
+  h = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
+  float rx, ry;  // x - h without a conversion of h: one instruction each
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rx) : "v"(h), "v"(x));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(ry) : "v"(h), "v"(y));
+  const v2f r = {rx, ry};
+  l = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
+}
+
+// The exponent that a largest magnitude (as its bits) is scaled by: x 2^(15 - e) is
+// below 2^15. Below 2^-100 (and at 0) the scale stays; infinite and NaN give some
+// exponent (the caller looks for them).
+__device__ __forceinline__ int split_exp(uint32_t bits) { return max((int)(bits >> 23) - 126, -100); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ float split_scale(int e) { return pow2(15 - e); }    // e in [-100, 129]
+__device__ __forceinline__ float split_unscale(int e) { return pow2(e - 15); }
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t max_abs(uint32_t m, float4 v) {
+  m = max(max(m, abs_bits(v.x)), abs_bits(v.y));
+  return max(max(m, abs_bits(v.z)), abs_bits(v.w));
+}
+
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp_bits(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, false);
+}
+// Largest of the wavefront's 64 lanes, in a scalar register.
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+  v = max(v, dpp_bits<kDppQuadSwap1>(v));
+  v = max(v, dpp_bits<kDppQuadSwap2>(v));
+  v = max(v, dpp_bits<kDppHalfMirror>(v));
+  v = max(v, dpp_bits<kDppMirror>(v));
+  const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  return max(max(a, b), max(c, d));
+}
+// Largest over the kLanes (16 or 32) lanes that share a row, in each of them.
+template <int kLanes>
+__device__ __forceinline__ uint32_t row_max_bits(uint32_t v) {
+  v = max(v, dpp_bits<kDppQuadSwap1>(v));
+  v = max(v, dpp_bits<kDppQuadSwap2>(v));
+  v = max(v, dpp_bits<kDppHalfMirror>(v));
+  v = max(v, dpp_bits<kDppMirror>(v));
+  if (kLanes == 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+  return v;
+}
+// x of this lane and of lane ^ 32, combined.
+__device__ __forceinline__ float half_max(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ uint32_t half_max_bits(uint32_t x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(s[0], s[1]);
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// A tile of 4 x 4 blocks, from rows of `ld` floats to registers.
+struct Rows4 {
+  float4 r[4];
+};
+__device__ __forceinline__ uint32_t max_abs(uint32_t m, const Rows4 &t) {
+#pragma unroll
+  for (int r = 0; r < 4; r++) m = max_abs(m, t.r[r]);
+  return m;
+}
+// For the least of the rows' largest magnitudes, rows of zeros left out: the
+// complement, so that it is a maximum too. kLanes lanes share the four rows.
+template <int kLanes>
+__device__ __forceinline__ uint32_t least_row(uint32_t m, const Rows4 &t) {
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const uint32_t x = row_max_bits<kLanes>(max_abs(0u, t.r[r]));
+    m = max(m, x ? ~x : 0u);
+  }
+  return m;
+}
+// Whether a row of the tile lies so far below the tile's largest that the tile's
+// scale would cost it digits (its elements from 2^-4 of its own largest on keep theirs).
+__device__ __forceinline__ bool too_wide(uint32_t largest, uint32_t least) {
+  return least && (largest >> 23) > (~least >> 23) + 12;
+}
+
+}  // namespace
+}  // namespace ugk
