@@ -501,21 +501,6 @@ __device__ void row_dq(float *dq, float *dsum, const float *dout, const float *q
   if (lane + kWave < HS) put(dq + lane + kWave, a1, assign);
 }
 
-__global__ __launch_bounds__(kBlock) void k_att_dq_rows(float *dq, float *dsum, const float *dout, const float *q,
-                                                        const float *k, const float *v, const float *out,
-                                                        const float *lse, ugk_attention a, bool assign, int *word) {
-  const int per = (a.max_q + kBlock / kWave - 1) / (kBlock / kWave);
-  const int b = blockIdx.x / (a.NH * per), h = blockIdx.x / per % a.NH, part = blockIdx.x % per;
-  const Seq s = sequence(a, b, h == 0 && part == 0, word, UGK_IDS_ATTENTION_BACKWARD);
-  const int i = part * (kBlock / kWave) + (threadIdx.x >> 6);
-  if (i >= s.Lq) return;
-  const size_t row = s.q0 + i;
-  const int hk = h / (a.NH / a.NKV);
-  row_dq(dq + row * a.ldq + h * a.HS, dsum + row * a.NH + h, dout + row * a.ldo + h * a.HS, q + row * a.ldq + h * a.HS,
-         k + (size_t)s.k0 * a.ldk + hk * a.HS, v + (size_t)s.k0 * a.ldv + hk * a.HS, out + row * a.ldo + h * a.HS,
-         lse[row * a.NH + h], s.seen(i, a.causal), a.HS, a.ldk, a.ldv, a.scale, assign);
-}
-
 // dk and dv of key row j of key/value head hk.
 __device__ void row_dkv(float *dk, float *dv, const float *dout, const float *q, const float *k, const float *v,
                         const float *lse, const float *dsum, const ugk_attention &a, const Seq &s, int j, int hk,
@@ -555,15 +540,499 @@ __device__ void row_dkv(float *dk, float *dv, const float *dout, const float *q,
   }
 }
 
-__global__ __launch_bounds__(kBlock) void k_att_dkv_rows(float *dk, float *dv, const float *dout, const float *q,
-                                                         const float *k, const float *v, const float *lse,
-                                                         const float *dsum, ugk_attention a, bool assign, int *word) {
-  const int per = (a.max_k + kBlock / kWave - 1) / (kBlock / kWave);
-  const int b = blockIdx.x / (a.NKV * per), hk = blockIdx.x / per % a.NKV, part = blockIdx.x % per;
-  const Seq s = sequence(a, b, hk == 0 && part == 0, word, UGK_IDS_ATTENTION_BACKWARD);
-  const int j = part * (kBlock / kWave) + (threadIdx.x >> 6);
-  if (j >= s.Lk) return;
-  row_dkv(dk, dv, dout, q, k, v, lse, dsum, a, s, j, hk, assign);
+// ---- backward, tiles on the matrix units ----------------------------------------
+//
+// Two passes, each of which computes the scores again: dq over the rows as the
+// forward holds them, then dk and dv over the keys, so that nothing is added by
+// two workgroups and the results do not depend on their order (one pass with
+// atomics would save the second S and dP, 4 of 14 HS operations per pair).
+// P = exp(S - lse) needs no running maximum. dS = P (dP - D) is scaled for its
+// halves by a bound: P <= 1 and |dP| <= HS max|dout| max|v|, so |dS| <= HS
+// max|dout| max|v| + |D|, which lies some 2^4 to 2^8 above its largest; a half and its
+// remainder reach 2^39 below the bound. The same tiles as in the forward fall
+// back to single rows.
+
+__device__ __forceinline__ void put4(float *p, float4 w, int nd, bool full, bool assign) {
+  if (full || nd >= 4) {
+    if (!assign) {
+      const float4 u = ld4(p);
+      w = make_float4(u.x + w.x, u.y + w.y, u.z + w.z, u.w + w.w);
+    }
+    st4(p, w);
+  } else {
+    if (nd > 0) put(p, w.x, assign);
+    if (nd > 1) put(p + 1, w.y, assign);
+    if (nd > 2) put(p + 2, w.z, assign);
+  }
+}
+// An accumulator's column (this lane's row of the result) to memory, times f.
+template <int DB, bool kFull>
+__device__ __forceinline__ void put_row(float *p, const v16f (&acc)[DB], float f, int half, int HS, bool assign) {
+#pragma unroll
+  for (int x = 0; x < DB; x++)
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+      const int d = 32 * x + 8 * y + 4 * half;
+      put4(p + d, make_float4(acc[x][4 * y] * f, acc[x][4 * y + 1] * f, acc[x][4 * y + 2] * f, acc[x][4 * y + 3] * f),
+           HS - d, kFull, assign);
+    }
+}
+
+// acc += A B for a 32-row block of B held in an accumulator's registers (C, scaled
+// to halves by f): A's rows in LDS, HSP of them, their columns in key_slot's order.
+template <int DB>
+__device__ __forceinline__ void mac_block(v16f (&acc)[DB], const v16f &c, float f, const _Float16 *ah, const _Float16 *al,
+                                          int stride, int lane) {
+#pragma unroll
+  for (int y = 0; y < 2; y++) {
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) p[j] = c[8 * y + j];
+    v8h bh, bl;
+    split8(p, f, bh, bl);
+#pragma unroll
+    for (int x = 0; x < DB; x++) {
+      const int at = (32 * x + (lane & 31)) * stride + 16 * y + 8 * (lane >> 5);
+      acc[x] = mfma3(frag(ah + at), frag(al + at), bh, bl, acc[x]);
+    }
+  }
+}
+// A 32 x 32 block of products of rows in LDS with the operands in registers.
+template <int DC>
+__device__ __forceinline__ v16f dot_block(const _Float16 *ah, const _Float16 *al, int stride, const v8h (&bh)[DC],
+                                          const v8h (&bl)[DC], int lane) {
+  v16f c = {};
+#pragma unroll
+  for (int x = 0; x < DC; x++) {
+    const int at = (lane & 31) * stride + 16 * x + 8 * (lane >> 5);
+    c = mfma3(frag(ah + at), frag(al + at), bh[x], bl[x], c);
+  }
+  return c;
+}
+
+// A lane's row (HS floats at p) as operands; *e: its exponent. Returns the bits of its largest magnitude.
+template <int DC, bool kFull>
+__device__ __forceinline__ uint32_t load_operand(const float *p, int HS, bool live, int half, v8h (&h)[DC], v8h (&l)[DC],
+                                                 int *e) {
+  float x[DC][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < DC; c++) {
+    load8<kFull>(p, 16 * c + 8 * half, HS, live, x[c]);
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = max(m, abs_bits(x[c][j]));
+  }
+  m = half_max_bits(m);
+  *e = split_exp(m);
+#pragma unroll
+  for (int c = 0; c < DC; c++) split8(x[c], split_scale(*e), h[c], l[c]);
+  return m;
+}
+
+// The largest of a noted quantity over the workgroup's wavefronts.
+template <int W>
+__device__ __forceinline__ uint32_t noted(const uint32_t (&slot)[W]) {
+  uint32_t m = slot[0];
+#pragma unroll
+  for (int w = 1; w < W; w++) m = max(m, slot[w]);
+  return (uint32_t)__builtin_amdgcn_readfirstlane(m);
+}
+
+template <int HSP, int W, bool kFull>
+__global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dq(
+    float *dq, float *dsum, const float *dout, const float *q, const float *k, const float *v, const float *out,
+    const float *lse, ugk_attention a, unsigned pairs, bool assign, int *word) {
+  constexpr int kThreads = W * kWave, BK = 32, DC = HSP / 16, DB = HSP / 32, DG = HSP / 4;
+  constexpr int kBlocks = BK / 4 * DG, kPer = 2 * kBlocks / kThreads;
+  static_assert(kPer >= 1 && kBlocks % kWave == 0, "whole wavefronts of K or V blocks");
+  constexpr int kRs = HSP + 8, kCs = BK + 8;
+  __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kRs], lv[2][2][BK * kRs], lt[2][2][HSP * kCs];
+  __shared__ uint32_t slot[2][4][W];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
+  const unsigned pair = blockIdx.x % pairs;
+  const int tile = (int)(gridDim.x / pairs - 1 - blockIdx.x / pairs);
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
+  const Seq s = sequence(a, b, hk == 0 && tile == 0, word, UGK_IDS_ATTENTION_BACKWARD);
+  const int rows = s.Lq * G, row0 = tile * (32 * W);
+  if (row0 >= rows) return;
+  const float *kb = k + (size_t)s.k0 * a.ldk + hk * a.HS, *vb = v + (size_t)s.k0 * a.ldv + hk * a.HS;
+  const int n = s.seen((min(row0 + 32 * W, rows) - 1) / G, a.causal), least = s.seen(row0 / G, a.causal);
+
+  const int r = row0 + wave * 32 + (lane & 31);
+  const bool live = r < rows;
+  const int i = live ? r / G : 0, h = hk * G + (live ? r % G : 0);
+  const int lim = live ? s.seen(i, a.causal) : 0;
+  int lo = live ? lim : n, hi = lim;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  const size_t grow = (size_t)s.q0 + i;
+  v8h qh[DC], ql[DC], gh[DC], gl[DC];
+  int eq, eg;
+  load_operand<DC, kFull>(q + grow * a.ldq + h * a.HS, a.HS, live, half, qh, ql, &eq);
+  const float *gr = dout + grow * a.ldo + h * a.HS;
+  const float gmax = __uint_as_float(load_operand<DC, kFull>(gr, a.HS, live, half, gh, gl, &eg));
+  float D = 0.0f;
+#pragma unroll
+  for (int c = 0; c < DC; c++) {
+    float x[8], y[8];
+    load8<kFull>(gr, 16 * c + 8 * half, a.HS, live, x);
+    load8<kFull>(out + grow * a.ldo + h * a.HS, 16 * c + 8 * half, a.HS, live, y);
+#pragma unroll
+    for (int j = 0; j < 8; j++) D = fmaf(x[j], y[j], D);
+  }
+  D = half_sum(D);
+  if (live && half == 0) dsum[grow * a.NH + h] = D;
+  const float L2 = live ? lse[grow * a.NH + h] * kLog2e : 0.0f;
+  const float cq = split_unscale(eq) * (a.scale * kLog2e), cg = split_unscale(eg);
+  bool bad = lim > 0 && !(fabsf(L2) < 0x1p22f);  // (the row's own q and dout reach its own results alone)
+
+  Rows4 t[kPer];
+  // K blocks by half of the wavefronts, V blocks by the others, in turn: K's are put twice
+  const auto is_v = [&](int u, int at) { return kPer == 1 ? ((wave >= W / 2) ^ (at & 1)) != 0 : u >= kPer / 2; };
+  const auto block = [&](int u) { return (tid + u * kThreads) % kBlocks; };
+  const auto load = [&](int at) {
+    const int k0 = at * BK;
+    const bool tail = k0 + BK > n;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const int d = block(u) % DG * 4, j = k0 + block(u) / DG * 4;
+      const bool w = is_v(u, at);
+      t[u] = load_rows<kFull>((w ? vb : kb) + d, w ? a.ldv : a.ldk, j, n, tail, a.HS - d);
+    }
+  };
+  const auto note = [&](int at) {
+    uint32_t m[4] = {};
+    const bool part = (at + 1) * BK > least;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const uint32_t x = max_abs(0u, t[u]), y = part ? least_row<DG>(0u, t[u]) : 0u;
+      if (is_v(u, at)) {
+        m[1] = max(m[1], x);
+        m[3] = max(m[3], y);
+      } else {
+        m[0] = max(m[0], x);
+        m[2] = max(m[2], y);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; x++) m[x] = wave_max_bits(m[x]);
+    if (lane == 0) {
+#pragma unroll
+      for (int x = 0; x < 4; x++) slot[at & 1][x][wave] = m[x];
+    }
+  };
+  int ek = -100, ev = -100;
+  const auto stage = [&](int at) {
+    const int z = at & 1;
+    const uint32_t mk = noted<W>(slot[z][0]), mv = noted<W>(slot[z][1]);
+    bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted<W>(slot[z][2])) || too_wide(mv, noted<W>(slot[z][3]));
+    ek = max(ek, split_exp(mk));
+    ev = max(ev, split_exp(mv));
+    const float fk = split_scale(ek), fv = split_scale(ev);
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const int d = block(u) % DG * 4, g = block(u) / DG;
+      if (is_v(u, at)) {
+        put_rows(t[u], fv, lv[z][0] + 4 * g * kRs + d, lv[z][1] + 4 * g * kRs + d, kRs);
+      } else {
+        put_rows(t[u], fk, lk[z][0] + 4 * g * kRs + d, lk[z][1] + 4 * g * kRs + d, kRs);
+        put_cols(t[u], fk, lt[z][0] + d * kCs + key_slot(g), lt[z][1] + d * kCs + key_slot(g), kCs);
+      }
+    }
+  };
+
+  v16f acc[DB] = {};
+  int ek_acc = -100, es = -100, ev_acc = -101;  // of the accumulators: K's, dS's and what dS's stands on
+  const auto compute = [&](int at, int ek_now, int ev_now) {
+    const int z = at & 1, k0 = at * BK;
+    if (ek_now != ek_acc || ev_now != ev_acc) {
+      const float bound = fmaf((float)a.HS * gmax, pow2(min(max(ev_now, -126), 127)), fabsf(D));
+      const int e = max(es, split_exp(__float_as_uint(bound)));
+      bad = bad || e > 120 || e + ek_now > 130;
+      const float f = pow2(max(ek_acc - ek_now, -126)) * pow2(max(es - e, -126));
+#pragma unroll
+      for (int x = 0; x < DB; x++)
+#pragma unroll
+        for (int y = 0; y < 16; y++) acc[x][y] *= f;
+      ek_acc = ek_now;
+      ev_acc = ev_now;
+      es = min(e, 120);
+    }
+    const float c2 = cq * split_unscale(ek_now), cd = cg * split_unscale(ev_now), f = split_scale(es);
+    bad = bad || fabsf(c2) > 0x1p100f || cd > 0x1p100f;
+    v16f p = dot_block<DC>(lk[z][0], lk[z][1], kRs, qh, ql, lane);
+    const v16f dp = dot_block<DC>(lv[z][0], lv[z][1], kRs, gh, gl, lane);
+#pragma unroll
+    for (int y = 0; y < 16; y++) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(p[y], c2, -L2));
+      p[y] = x * fmaf(dp[y], cd, -D);
+    }
+    if (k0 + BK > lo) {
+      const int rel = lim - k0 - 4 * half;
+#pragma unroll
+      for (int y = 0; y < 16; y++)
+        if (8 * (y / 4) + y % 4 >= rel) p[y] = 0.0f;
+    }
+    mac_block<DB>(acc, p, f, lt[z][0], lt[z][1], kCs, lane);
+  };
+
+  const int tiles = (n + BK - 1) / BK;
+  if (tiles > 0) {
+    load(0);
+    note(0);
+    __syncthreads();
+    stage(0);
+    if (tiles > 1) {
+      load(1);
+      note(1);
+    }
+    __syncthreads();
+    for (int at = 0; at < tiles; at++) {
+      const int ek_now = ek, ev_now = ev;
+      if (at + 1 < tiles) stage(at + 1);
+      if (at + 2 < tiles) load(at + 2);
+      if (at * BK < hi) compute(at, ek_now, ev_now);
+      if (at + 2 < tiles) note(at + 2);
+      __syncthreads();
+    }
+  }
+  if (__any(bad)) {
+    for (int x = 0; x < 32; x++) {
+      const int rr = row0 + wave * 32 + x;
+      if (rr >= rows) break;
+      const int ii = rr / G, hh = hk * G + rr % G;
+      const size_t g = (size_t)s.q0 + ii;
+      row_dq(dq + g * a.ldq + hh * a.HS, dsum + g * a.NH + hh, dout + g * a.ldo + hh * a.HS, q + g * a.ldq + hh * a.HS, kb, vb,
+             out + g * a.ldo + hh * a.HS, lse[g * a.NH + hh], s.seen(ii, a.causal), a.HS, a.ldk, a.ldv, a.scale, assign);
+    }
+    return;
+  }
+  if (live)
+    put_row<DB, kFull>(dq + grow * a.ldq + h * a.HS, acc, split_unscale(es) * split_unscale(ek_acc) * a.scale, half, a.HS,
+                       assign);
+}
+
+// Row r (query row r / G, head r % G of the group) of q or dout, from the row that
+// starts at `base`: rows `ld` floats apart, heads HS.
+struct GroupRows {
+  const float *base;
+  long long ld;
+  int HS, G;
+  __device__ __forceinline__ const float *at(int r) const {
+    if (G == 1) return base + r * ld;
+    const int i = r / G;
+    return base + i * ld + (r - i * G) * HS;
+  }
+};
+template <bool kFull>
+__device__ __forceinline__ Rows4 load_rows(const GroupRows &g, int d, int r, int n, int nd) {
+  Rows4 t;
+#pragma unroll
+  for (int x = 0; x < 4; x++) {
+    t.r[x] = load4<kFull>(g.at(min(r + x, n - 1)) + d, nd);
+    if (r + x >= n) t.r[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  return t;
+}
+
+template <int HSP, int W, bool kFull>
+__global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dkv(
+    float *dk, float *dv, const float *dout, const float *q, const float *k, const float *v, const float *lse,
+    const float *dsum, ugk_attention a, unsigned pairs, bool assign, int *word) {
+  constexpr int kThreads = W * kWave, BQ = 32, DC = HSP / 16, DB = HSP / 32, DG = HSP / 4;
+  constexpr int kBlocks = BQ / 4 * DG, kPer = 2 * kBlocks / kThreads;
+  static_assert(kPer >= 1 && kBlocks % kWave == 0, "whole wavefronts of Q or dout blocks");
+  constexpr int kRs = HSP + 8, kCs = BQ + 8;
+  __shared__ __attribute__((aligned(16))) _Float16 lq[2][2][BQ * kRs], lg[2][2][BQ * kRs], tq[2][2][HSP * kCs],
+      tg[2][2][HSP * kCs];
+  __shared__ __attribute__((aligned(16))) float lL[2][BQ], lD[2][BQ];
+  __shared__ uint32_t slot[2][6][W];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
+  const unsigned pair = blockIdx.x % pairs;
+  const int tile = (int)(blockIdx.x / pairs);  // the keys that the most rows see first
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
+  const Seq s = sequence(a, b, hk == 0 && tile == 0, word, UGK_IDS_ATTENTION_BACKWARD);
+  const int key0 = tile * (32 * W), rows = s.Lq * G;
+  if (key0 >= s.Lk) return;
+  // rows before `from` see none of the workgroup's keys, rows from `all` on all of them
+  const int from = min(s.first(key0, a.causal), s.Lq) * G / BQ * BQ;
+  const int all = min(s.first(min(key0 + 32 * W, s.Lk) - 1, a.causal), s.Lq) * G;
+
+  const int j = key0 + wave * 32 + (lane & 31);
+  const bool live = j < s.Lk;
+  const int lim = live ? min(s.first(j, a.causal), s.Lq) * G : rows;  // the first row that sees the key
+  int lo = lim, hi = live ? lim : 0;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  const size_t grow = (size_t)s.k0 + (live ? j : 0);
+  v8h kh[DC], kl[DC], vh[DC], vl[DC];
+  int ek, ev;
+  load_operand<DC, kFull>(k + grow * a.ldk + hk * a.HS, a.HS, live, half, kh, kl, &ek);
+  const float vmax = __uint_as_float(load_operand<DC, kFull>(v + grow * a.ldv + hk * a.HS, a.HS, live, half, vh, vl, &ev));
+  const float ck = split_unscale(ek) * (a.scale * kLog2e), cv = split_unscale(ev);
+  bool bad = false;
+
+  const GroupRows gq{q + (size_t)s.q0 * a.ldq + hk * G * a.HS, a.ldq, a.HS, G};
+  const GroupRows gg{dout + (size_t)s.q0 * a.ldo + hk * G * a.HS, a.ldo, a.HS, G};
+  const size_t stat = (size_t)s.q0 * a.NH + hk * G;
+  Rows4 t[kPer];
+  float tL = 0.0f, tD = 0.0f;
+  const auto is_g = [&](int u) { return kPer == 1 ? wave >= W / 2 : u >= kPer / 2; };
+  const auto block = [&](int u) { return (tid + u * kThreads) % kBlocks; };
+  const auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const int d = block(u) % DG * 4, r = r0 + block(u) / DG * 4;
+      t[u] = load_rows<kFull>(is_g(u) ? gg : gq, d, r, rows, a.HS - d);
+    }
+    if (tid < BQ) {
+      const int r = r0 + tid, i = min(r, rows - 1) / G, x = min(r, rows - 1) - i * G;
+      tL = lse[stat + (size_t)i * a.NH + x] * kLog2e;
+      tD = dsum[stat + (size_t)i * a.NH + x];
+      if (r >= rows) tL = tD = 0.0f;
+    }
+  };
+  const auto note = [&](int z, int r0) {
+    uint32_t m[6] = {};
+    const bool part = r0 < all;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const uint32_t x = max_abs(0u, t[u]), y = part ? least_row<DG>(0u, t[u]) : 0u;
+      if (is_g(u)) {
+        m[1] = max(m[1], x);
+        m[3] = max(m[3], y);
+      } else {
+        m[0] = max(m[0], x);
+        m[2] = max(m[2], y);
+      }
+    }
+    if (tid < BQ) {
+      m[4] = abs_bits(tD);
+      m[5] = tL == -INFINITY ? 0u : abs_bits(tL);  // (a row without keys)
+    }
+#pragma unroll
+    for (int x = 0; x < 6; x++) m[x] = wave_max_bits(m[x]);
+    if (lane == 0) {
+#pragma unroll
+      for (int x = 0; x < 6; x++) slot[z][x][wave] = m[x];
+    }
+  };
+  int eq = -100, eg = -100;
+  float dmax = 0.0f;
+  const auto stage = [&](int z) {
+    const uint32_t mq = noted<W>(slot[z][0]), mg = noted<W>(slot[z][1]), md = noted<W>(slot[z][4]);
+    bad = bad || mq >= kInfBits || mg >= kInfBits || md >= kInfBits || noted<W>(slot[z][5]) >= 0x4a800000u /* 2^22 */ ||
+          too_wide(mq, noted<W>(slot[z][2])) ||
+          too_wide(mg, noted<W>(slot[z][3]));
+    eq = max(eq, split_exp(mq));
+    eg = max(eg, split_exp(mg));
+    dmax = fmaxf(dmax, __uint_as_float(md));
+    const float fq = split_scale(eq), fg = split_scale(eg);
+#pragma unroll
+    for (int u = 0; u < kPer; u++) {
+      const int d = block(u) % DG * 4, g = block(u) / DG;
+      const float f = is_g(u) ? fg : fq;
+      _Float16 *rh = is_g(u) ? lg[z][0] : lq[z][0], *rl = is_g(u) ? lg[z][1] : lq[z][1];
+      _Float16 *ch = is_g(u) ? tg[z][0] : tq[z][0], *cl = is_g(u) ? tg[z][1] : tq[z][1];
+      put_rows(t[u], f, rh + 4 * g * kRs + d, rl + 4 * g * kRs + d, kRs);
+      put_cols(t[u], f, ch + d * kCs + key_slot(g), cl + d * kCs + key_slot(g), kCs);
+    }
+    if (tid < BQ) {
+      lL[z][tid] = tL;
+      lD[z][tid] = tD;
+    }
+  };
+
+  v16f ak[DB] = {}, av[DB] = {};
+  int eq_acc = -100, eg_acc = -100, es = -100;
+  float dmax_acc = -1.0f;
+  const auto compute = [&](int z, int r0, int eq_now, int eg_now, float dmax_now) {
+    if (eq_now != eq_acc || eg_now != eg_acc || dmax_now != dmax_acc) {
+      const float bound = fmaf((float)a.HS * vmax, pow2(min(max(eg_now, -126), 127)), dmax_now);
+      const int e = max(es, split_exp(__float_as_uint(bound)));
+      bad = bad || (live && (e > 120 || e + eq_now > 130));
+      const float fk = pow2(max(eq_acc - eq_now, -126)) * pow2(max(es - e, -126)), fv = pow2(max(eg_acc - eg_now, -126));
+      if (__any(fk != 1.0f || fv != 1.0f)) {
+#pragma unroll
+        for (int x = 0; x < DB; x++)
+#pragma unroll
+          for (int y = 0; y < 16; y++) {
+            ak[x][y] *= fk;
+            av[x][y] *= fv;
+          }
+      }
+      eq_acc = eq_now;
+      eg_acc = eg_now;
+      dmax_acc = dmax_now;
+      es = min(e, 120);
+    }
+    const float c2 = ck * split_unscale(eq_now), cd = cv * split_unscale(eg_now), f = pow2(-es);  // P is 2^15 up
+    bad = bad || (live && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
+    v16f p = dot_block<DC>(lq[z][0], lq[z][1], kRs, kh, kl, lane);
+    v16f ds = dot_block<DC>(lg[z][0], lg[z][1], kRs, vh, vl, lane);
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+      const float4 L = *reinterpret_cast<const float4 *>(&lL[z][8 * y + 4 * half]);
+      const float4 D = *reinterpret_cast<const float4 *>(&lD[z][8 * y + 4 * half]);
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const float Lx = part4(L, x);
+        p[4 * y + x] = __builtin_amdgcn_exp2f(fmaf(p[4 * y + x], c2, 15.0f - Lx));
+        ds[4 * y + x] = p[4 * y + x] * fmaf(ds[4 * y + x], cd, -part4(D, x));
+      }
+    }
+    if (r0 < hi || !live) {
+      const int rel = lim - r0 - 4 * half;
+#pragma unroll
+      for (int y = 0; y < 16; y++)
+        if (8 * (y / 4) + y % 4 < rel) p[y] = ds[y] = 0.0f;
+    }
+    mac_block<DB>(av, p, 1.0f, tg[z][0], tg[z][1], kCs, lane);
+    mac_block<DB>(ak, ds, f, tq[z][0], tq[z][1], kCs, lane);
+  };
+
+  const int tiles = rows > from ? (rows - from + BQ - 1) / BQ : 0;
+  if (tiles > 0) {
+    load(from);
+    note(0, from);
+    __syncthreads();
+    stage(0);
+    if (tiles > 1) {
+      load(from + BQ);
+      note(1, from + BQ);
+    }
+    __syncthreads();
+    for (int at = 0; at < tiles; at++) {
+      const int r0 = from + at * BQ, eq_now = eq, eg_now = eg;
+      const float dmax_now = dmax;
+      if (at + 1 < tiles) stage((at + 1) & 1);
+      if (at + 2 < tiles) load(r0 + 2 * BQ);
+      if (r0 + BQ > lo) compute(at & 1, r0, eq_now, eg_now, dmax_now);
+      if (at + 2 < tiles) note(at & 1, r0 + 2 * BQ);
+      __syncthreads();
+    }
+  }
+  if (__any(bad)) {
+    for (int x = 0; x < 32; x++) {
+      const int jj = key0 + wave * 32 + x;
+      if (jj >= s.Lk) break;
+      row_dkv(dk, dv, dout, q, k, v, lse, dsum, a, s, jj, hk, assign);
+    }
+    return;
+  }
+  if (!live) return;
+  put_row<DB, kFull>(dk + grow * a.ldk + hk * a.HS, ak, split_unscale(es) * split_unscale(eq_acc) * a.scale, half, a.HS, assign);
+  put_row<DB, kFull>(dv + grow * a.ldv + hk * a.HS, av, split_unscale(eg_acc) * 0x1p-15f, half, a.HS, assign);
 }
 
 }  // namespace
@@ -579,6 +1048,14 @@ int cu_count() {
     return c > 0 ? c : 256;
   }();
   return n;
+}
+
+// Wavefronts of a workgroup: four share a tile's staging while there are as many
+// workgroups as CUs, else fewer, down to one.
+int tile_waves(long long pairs, long long rows) {
+  for (int W = 4; W > 1; W /= 2)
+    if (pairs * ((rows + 32 * W - 1) / (32 * W)) >= cu_count()) return W;
+  return 1;
 }
 
 constexpr size_t kMaxParts = 1 << 15;  // rows of a head that the parts hold at most
@@ -648,14 +1125,30 @@ int launch_attention_forward(float *out, float *lse, const float *q, const float
 int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout, const float *q, const float *k,
                               const float *v, const float *out, const float *lse, float *dsum, const ugk_attention &a,
                               bool assign, int *word) {
-  if (a.max_q) {
-    const unsigned per = grid_for((size_t)a.max_q, kBlock / kWave);
-    launch(k_att_dq_rows, dim3(per * a.NH * a.nseq), dim3(kBlock), 0, dq, dsum, dout, q, k, v, out, lse, a, assign, word);
+  const unsigned pairs = (unsigned)a.nseq * a.NKV;
+  const bool wide = a.HS > 64, full = a.HS == (wide ? 128 : 64);
+  if (const long long rows = (long long)a.max_q * (a.NH / a.NKV)) {
+    const int W = wide ? 4 : tile_waves(pairs, rows);
+    const auto go = [&](auto kernel) {
+      launch(kernel, dim3(pairs * grid_for((size_t)rows, 32 * W)), dim3(W * kWave), 0, dq, dsum, dout, q, k, v, out, lse, a,
+             pairs, assign, word);
+    };
+#define UGK_ATT(kernel)                                                    \
+  if (wide) full ? go(kernel<128, 4, true>) : go(kernel<128, 4, false>);   \
+  else if (W == 4) full ? go(kernel<64, 4, true>) : go(kernel<64, 4, false>); \
+  else if (W == 2) full ? go(kernel<64, 2, true>) : go(kernel<64, 2, false>); \
+  else full ? go(kernel<64, 1, true>) : go(kernel<64, 1, false>);
+    UGK_ATT(k_att_dq)
     if (int e = check_launch("attention_backward")) return e;
   }
   if (a.max_k) {
-    const unsigned per = grid_for((size_t)a.max_k, kBlock / kWave);
-    launch(k_att_dkv_rows, dim3(per * a.NKV * a.nseq), dim3(kBlock), 0, dk, dv, dout, q, k, v, lse, dsum, a, assign, word);
+    const int W = wide ? 4 : tile_waves(pairs, a.max_k);
+    const auto go = [&](auto kernel) {
+      launch(kernel, dim3(pairs * grid_for((size_t)a.max_k, 32 * W)), dim3(W * kWave), 0, dk, dv, dout, q, k, v, lse, dsum, a,
+             pairs, assign, word);
+    };
+    UGK_ATT(k_att_dkv)
+#undef UGK_ATT
   }
   return check_launch("attention_backward");
 }
