@@ -9,6 +9,8 @@
 // the group.
 #include <math.h>
 
+#include <type_traits>
+
 #include "ugk_internal.h"
 #include "ugk_split.h"
 
@@ -63,6 +65,8 @@ __device__ __forceinline__ float dot(const float *x, const float *y, int n) {
   for (int d = 0; d < n; d++) s = fmaf(x[d], y[d], s);
   return s;
 }
+
+__device__ __forceinline__ void put(float *p, float x, bool assign) { *p = assign ? x : *p + x; }
 
 // One query row of one head by one wavefront: lanes over keys for the scores,
 // over channels for the sum.
@@ -440,6 +444,174 @@ __global__ __launch_bounds__(W * kWave, W == 1 ? 1 : 2) void k_att_fwd(float *ou
   }
 }
 
+__device__ __forceinline__ void put4(float *p, float4 w, int nd, bool full, bool assign) {
+  if (full || nd >= 4) {
+    if (!assign) {
+      const float4 u = ld4(p);
+      w = make_float4(u.x + w.x, u.y + w.y, u.z + w.z, u.w + w.w);
+    }
+    st4(p, w);
+  } else {
+    if (nd > 0) put(p, w.x, assign);
+    if (nd > 1) put(p + 1, w.y, assign);
+    if (nd > 2) put(p + 2, w.z, assign);
+  }
+}
+
+// ---- forward, few rows per key/value head ----------------------------------------
+//
+// With few (query row, head) pairs for a key/value head (a token's decode step), the
+// work is to read K and V once, and the products fit the vector units: 4 R
+// operations per byte pair against the matrix units' 32 rows that would stay
+// mostly empty. HSP / 4 lanes take a key, four floats each, so that a wavefront reads 64
+// / (HSP / 4) whole rows of K at a time, and then of V: U of them are in flight
+// per lane before the first is used. A group of lanes has its own running maximum,
+// sum and output (no exchange between groups until the end); its score sums go through
+// DPP. The groups, then the workgroup's NW wavefronts, are joined at the end
+// in their order, through LDS. Single precision throughout, and a key that
+// a row must not see is left out by selects, so nothing of it reaches the row.
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += dpp_lane<kDppQuadSwap1>(v);
+  v += dpp_lane<kDppQuadSwap2>(v);
+  v += dpp_lane<kDppHalfMirror>(v);
+  v += dpp_lane<kDppMirror>(v);
+  if (kLanes == 32) v += __shfl_xor(v, 16);
+  return v;
+}
+
+// Keys in flight per group of lanes, and wavefronts of a large workgroup: as many as the registers hold.
+constexpr int few_loads(int R) { return R == 1 ? 8 : 4; }
+constexpr int few_waves(int R) { return R <= 2 ? 16 : 8; }
+
+template <int HSP, int R, int NW, bool kFull>
+__global__ __launch_bounds__(NW * kWave) void k_att_few(float *out, float *lse, const float *q, const float *k,
+                                                        const float *v, ugk_attention a, Parts parts, unsigned pairs,
+                                                        int *word) {
+  constexpr int kLanes = HSP / 4, kKeys = kWave / kLanes, U = few_loads(R), kStep = kKeys * U;
+  __shared__ float4 lo[NW][R][kLanes];
+  __shared__ float lm[NW][R], ll[NW][R];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int group = lane / kLanes, d = lane % kLanes * 4, nd = a.HS - d;
+  const unsigned pair = blockIdx.x % pairs;
+  const int part = blockIdx.x / pairs;
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
+  const Seq s = sequence(a, b, hk == 0 && part == 0, word, UGK_IDS_ATTENTION_FORWARD);
+  const int rows = s.Lq * G;
+  if (rows <= 0) return;
+  const float *kb = k + (size_t)s.k0 * a.ldk + hk * a.HS + (nd > 0 ? d : 0);
+  const float *vb = v + (size_t)s.k0 * a.ldv + hk * a.HS + (nd > 0 ? d : 0);
+  const int first = parts.o ? min(part * parts.chunk, s.Lk) : 0;
+  const int stop = parts.o ? min(first + parts.chunk, s.Lk) : s.Lk;
+  float4 qv[R], o[R];
+  float m[R], l[R];
+  int lim[R], least = stop, n = first;
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int rr = min(r, rows - 1), i = rr / G, h = hk * G + rr % G;
+    qv[r] = load4<kFull>(q + ((size_t)s.q0 + i) * a.ldq + h * a.HS + (nd > 0 ? d : 0), nd);
+    const float f = a.scale * kLog2e;
+    qv[r] = make_float4(qv[r].x * f, qv[r].y * f, qv[r].z * f, qv[r].w * f);
+    lim[r] = r < rows ? min(stop, s.seen(i, a.causal)) : first;
+    if (r < rows) least = min(least, lim[r]);
+    n = max(n, lim[r]);
+    o[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+  }
+  for (int j0 = first + wave * kStep; j0 < n; j0 += NW * kStep) {
+    float4 kv[U], vv[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) kv[u] = load4<kFull>(kb + min(j0 + u * kKeys + group, n - 1) * a.ldk, nd);
+#pragma unroll
+    for (int u = 0; u < U; u++) vv[u] = load4<kFull>(vb + min(j0 + u * kKeys + group, n - 1) * a.ldv, nd);
+    const auto take = [&](auto masked) {  // masked: not every row sees all of these keys
+      constexpr bool kMasked = decltype(masked)::value;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        if (R > 1) __builtin_amdgcn_sched_barrier(0);  // row by row: the registers hold one row's scores
+        float p[U], top = m[r];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          p[u] = lanes_sum<kLanes>(fmaf(qv[r].w, kv[u].w, fmaf(qv[r].z, kv[u].z, fmaf(qv[r].y, kv[u].y, qv[r].x * kv[u].x))));
+          if (kMasked && j0 + u * kKeys + group >= lim[r]) p[u] = -INFINITY;
+          top = fmaxf(top, p[u]);
+        }
+        const float base = top == -INFINITY ? 0.0f : top, keep = __builtin_amdgcn_exp2f(m[r] - base);
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          p[u] = __builtin_amdgcn_exp2f(p[u] - base);
+          sum += p[u];
+        }
+        m[r] = top;
+        l[r] = fmaf(l[r], keep, sum);
+        o[r] = make_float4(o[r].x * keep, o[r].y * keep, o[r].z * keep, o[r].w * keep);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          float4 w = vv[u];
+          if (kMasked && j0 + u * kKeys + group >= lim[r]) w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          o[r].x = fmaf(p[u], w.x, o[r].x);
+          o[r].y = fmaf(p[u], w.y, o[r].y);
+          o[r].z = fmaf(p[u], w.z, o[r].z);
+          o[r].w = fmaf(p[u], w.w, o[r].w);
+        }
+      }
+    };
+    if (j0 + kStep > least) take(std::true_type{});
+    else take(std::false_type{});
+  }
+  // the wavefront's groups
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+#pragma unroll
+    for (int x = kLanes; x < kWave; x *= 2) {
+      __builtin_amdgcn_sched_barrier(0);
+      const float m2 = __shfl_xor(m[r], x), l2 = __shfl_xor(l[r], x);
+      const float4 o2 = make_float4(__shfl_xor(o[r].x, x), __shfl_xor(o[r].y, x), __shfl_xor(o[r].z, x), __shfl_xor(o[r].w, x));
+      const float top = fmaxf(m[r], m2), base = top == -INFINITY ? 0.0f : top;
+      const float f = __builtin_amdgcn_exp2f(m[r] - base), g = __builtin_amdgcn_exp2f(m2 - base);
+      l[r] = l[r] * f + l2 * g;
+      o[r] = make_float4(o[r].x * f + o2.x * g, o[r].y * f + o2.y * g, o[r].z * f + o2.z * g, o[r].w * f + o2.w * g);
+      m[r] = top;
+    }
+    if (group == 0) lo[wave][r][lane] = o[r];
+    if (lane == 0) {
+      lm[wave][r] = m[r];
+      ll[wave][r] = l[r];
+    }
+  }
+  __syncthreads();
+  // the wavefronts, kLanes threads per row
+  for (int x = threadIdx.x; x < min(R, rows) * kLanes; x += NW * kWave) {
+    const int r = x / kLanes, at = x % kLanes;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; w++) top = fmaxf(top, lm[w][r]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const float f = __builtin_amdgcn_exp2f(lm[w][r] - base);
+      const float4 y = lo[w][r][at];
+      sum = fmaf(ll[w][r], f, sum);
+      t = make_float4(fmaf(y.x, f, t.x), fmaf(y.y, f, t.y), fmaf(y.z, f, t.z), fmaf(y.w, f, t.w));
+    }
+    const int i = r / G, h = hk * G + r % G;
+    const bool any = min(stop, s.seen(i, a.causal)) > first;
+    const float f = any ? 1.0f / sum : 0.0f, L = any ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
+    t = any ? make_float4(t.x * f, t.y * f, t.z * f, t.w * f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const size_t prow = ((size_t)part * a.nseq + b) * a.max_q + i, grow = (size_t)s.q0 + i;
+    float *po = parts.o ? parts.o + prow * a.NH * a.HS + (size_t)h * a.HS : out + grow * a.ldo + h * a.HS;
+    put4(po + 4 * at, t, a.HS - 4 * at, kFull, true);
+    if (at == 0) {
+      if (parts.o) parts.lse[prow * a.NH + h] = L;
+      else if (lse) lse[grow * a.NH + h] = L;
+    }
+  }
+}
+
 // The parts of a split key axis joined, one wavefront per row and head: out =
 // sum_x e^(lse_x - lse) o_x, in the parts' order.
 __global__ __launch_bounds__(kBlock) void k_att_join(float *out, float *lse, Parts parts, ugk_attention a) {
@@ -473,7 +645,6 @@ __global__ __launch_bounds__(kBlock) void k_att_join(float *out, float *lse, Par
   if (lse && lane == 0) lse[g * a.NH + h] = none ? -INFINITY : m + logf(l);
 }
 
-__device__ __forceinline__ void put(float *p, float x, bool assign) { *p = assign ? x : *p + x; }
 
 // dq of one query row of one head, and D.
 __device__ void row_dq(float *dq, float *dsum, const float *dout, const float *q, const float *k, const float *v,
@@ -552,19 +723,6 @@ __device__ void row_dkv(float *dk, float *dv, const float *dout, const float *q,
 // remainder reach 2^39 below the bound. The same tiles as in the forward fall
 // back to single rows.
 
-__device__ __forceinline__ void put4(float *p, float4 w, int nd, bool full, bool assign) {
-  if (full || nd >= 4) {
-    if (!assign) {
-      const float4 u = ld4(p);
-      w = make_float4(u.x + w.x, u.y + w.y, u.z + w.z, u.w + w.w);
-    }
-    st4(p, w);
-  } else {
-    if (nd > 0) put(p, w.x, assign);
-    if (nd > 1) put(p + 1, w.y, assign);
-    if (nd > 2) put(p + 2, w.z, assign);
-  }
-}
 // An accumulator's column (this lane's row of the result) to memory, times f.
 template <int DB, bool kFull>
 __device__ __forceinline__ void put_row(float *p, const v16f (&acc)[DB], float f, int half, int HS, bool assign) {
@@ -1058,26 +1216,35 @@ int tile_waves(long long pairs, long long rows) {
   return 1;
 }
 
+constexpr int kFewRows = 4;
 constexpr size_t kMaxParts = 1 << 15;  // rows of a head that the parts hold at most
 
-// How the forward of `a` is cut: wavefronts of a workgroup, key tile, parts of the key axis.
+// How the forward of `a` is cut: rows per key/value head where they are few (k_att_few),
+// wavefronts of a workgroup, tiles of rows, parts of the key axis and keys per part.
 struct FwdPlan {
-  int W, BK, tiles, splits, chunk;
+  int few, W, tiles, splits, chunk;
 };
 FwdPlan fwd_plan(const ugk_attention &a) {
   const long long pairs = (long long)a.nseq * a.NKV, rows = (long long)a.max_q * (a.NH / a.NKV);
-  const auto tiles = [&](int W) { return (rows + 32 * W - 1) / (32 * W); };
   FwdPlan p{};
-  p.W = pairs * tiles(4) >= cu_count() ? 4 : 1;
-  p.BK = a.HS <= 64 && p.W == 4 ? 64 : 32;
-  p.tiles = (int)tiles(p.W);
+  int unit;  // keys that a workgroup takes at a time
+  if (rows <= kFewRows) {
+    p.few = rows <= 1 ? 1 : rows <= 2 ? 2 : 4;
+    p.tiles = 1;
+    p.W = pairs < 4 * cu_count() ? few_waves(p.few) : 4;
+    unit = p.W * (a.HS <= 64 ? 4 : 2) * few_loads(p.few);
+  } else {
+    p.W = pairs * ((rows + 127) / 128) >= cu_count() ? 4 : 1;
+    p.tiles = (int)((rows + 32 * p.W - 1) / (32 * p.W));
+    unit = a.HS <= 64 && p.W == 4 ? 64 : 32;
+  }
   p.splits = 1;
   const long long wgs = pairs * p.tiles, prow = (long long)a.nseq * a.max_q * a.NH;
-  long long want = 2 * cu_count() / (wgs > 0 ? wgs : 1);
-  want = min(want, (long long)a.max_k / (4 * p.BK));
+  long long want = (p.few ? 1 : 2) * cu_count() / (wgs > 0 ? wgs : 1);
+  want = min(want, (long long)a.max_k / (4 * unit));
   want = min(want, (long long)kMaxParts / (prow > 0 ? prow : 1));
   if (want > 1) {
-    p.chunk = (int)((a.max_k + want - 1) / want + p.BK - 1) / p.BK * p.BK;
+    p.chunk = (int)((a.max_k + want - 1) / want + unit - 1) / unit * unit;
     p.splits = (a.max_k + p.chunk - 1) / p.chunk;
   }
   return p;
@@ -1105,7 +1272,23 @@ int launch_attention_forward(float *out, float *lse, const float *q, const float
   const auto go = [&](auto kernel) {
     launch(kernel, dim3(pairs * p.tiles, p.splits), dim3(p.W * kWave), 0, out, lse, q, k, v, a, parts, pairs, word);
   };
-  if (a.HS <= 64) {
+  if (p.few) {
+    const auto few = [&](auto kernel) {
+      launch(kernel, dim3(pairs * p.splits), dim3(p.W * kWave), 0, out, lse, q, k, v, a, parts, pairs, word);
+    };
+#define UGK_FEW_HS(r, w)                                                             \
+  if (a.HS == 64) few(k_att_few<64, r, w, true>);                                    \
+  else if (a.HS < 64) few(k_att_few<64, r, w, false>);                               \
+  else if (a.HS == 128) few(k_att_few<128, r, w, true>);                             \
+  else few(k_att_few<128, r, w, false>);
+#define UGK_FEW(r)                                                                   \
+  case r:                                                                            \
+    if (p.W == 4) { UGK_FEW_HS(r, 4) } else { UGK_FEW_HS(r, few_waves(r)) }          \
+    break;
+    switch (p.few) { UGK_FEW(1) UGK_FEW(2) UGK_FEW(4) }
+#undef UGK_FEW
+#undef UGK_FEW_HS
+  } else if (a.HS <= 64) {
     const bool full = a.HS == 64;
     if (p.W == 4) full ? go(k_att_fwd<64, 64, 4, true>) : go(k_att_fwd<64, 64, 4, false>);
     else full ? go(k_att_fwd<64, 32, 1, true>) : go(k_att_fwd<64, 32, 1, false>);
