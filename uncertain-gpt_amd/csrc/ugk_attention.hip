@@ -120,6 +120,9 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
 // all of a tile and its keys' magnitudes lie further apart than the halves'
 // digits allow (a row would lose its digits to keys that it must not see); or if
 // scores leave the range of the above (2^22 in base 2).
+// A row's P are scaled to 2^kTop at the maximum that they stand on, which moves (and the accumulators with it) only
+// when a score lies 2^7 above it: P then stays below 2^(kTop + 7), the halves' range.
+constexpr float kTop = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 // One part of a split key axis: o normalised, and lse, per row.
@@ -137,51 +140,37 @@ __device__ __forceinline__ float4 load4(const float *p, int nd) {
   if (nd > 2) v.z = p[2];
   return v;
 }
-// Rows j .. j + 3 of [0, n): past it, zero (n > 0). tail: some of the tile's rows are.
-template <bool kFull>
+// Rows j, j + kStep, .. of [0, n): past it, zero (n > 0). tail: some of the tile's rows are.
+template <int kStep, bool kFull>
 __device__ __forceinline__ Rows4 load_rows(const float *base, long long ld, int j, int n, bool tail, int nd) {
   Rows4 t;
   if (tail) {
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      t.r[r] = load4<kFull>(base + min(j + r, n - 1) * ld, nd);
-      if (j + r >= n) t.r[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      t.r[r] = load4<kFull>(base + min(j + kStep * r, n - 1) * ld, nd);
+      if (j + kStep * r >= n) t.r[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
   } else {
     const float *p = base + j * ld;
 #pragma unroll
-    for (int r = 0; r < 4; r++, p += ld) t.r[r] = load4<kFull>(p, nd);
+    for (int r = 0; r < 4; r++, p += kStep * ld) t.r[r] = load4<kFull>(p, nd);
   }
   return t;
 }
 __device__ __forceinline__ float part4(const float4 &v, int d) { return d == 0 ? v.x : d == 1 ? v.y : d == 2 ? v.z : v.w; }
 
-// The block's rows, scaled and split, to row-major halves (h, l: the two parts' arrays, `stride` halves a row).
+// The block's rows, scaled and split, to rows of halves kStep apart (h, l: the two parts' arrays, `stride` halves a row).
+template <int kStep>
 __device__ __forceinline__ void put_rows(const Rows4 &t, float scale, _Float16 *h, _Float16 *l, int stride) {
 #pragma unroll
   for (int r = 0; r < 4; r++) {
     uint32_t h0, h1, l0, l1;
-    split2(t.r[r].x * scale, t.r[r].y * scale, h0, l0);
-    split2(t.r[r].z * scale, t.r[r].w * scale, h1, l1);
-    *reinterpret_cast<v2u *>(h + r * stride) = v2u{h0, h1};
-    *reinterpret_cast<v2u *>(l + r * stride) = v2u{l0, l1};
+    split2(t.r[r].x, t.r[r].y, scale, h0, l0);
+    split2(t.r[r].z, t.r[r].w, scale, h1, l1);
+    *reinterpret_cast<v2u *>(h + kStep * r * stride) = v2u{h0, h1};
+    *reinterpret_cast<v2u *>(l + kStep * r * stride) = v2u{l0, l1};
   }
 }
-// The same transposed: row d of the arrays gets the block's column d.
-__device__ __forceinline__ void put_cols(const Rows4 &t, float scale, _Float16 *h, _Float16 *l, int stride) {
-#pragma unroll
-  for (int d = 0; d < 4; d++) {
-    uint32_t h0, h1, l0, l1;
-    split2(part4(t.r[0], d) * scale, part4(t.r[1], d) * scale, h0, l0);
-    split2(part4(t.r[2], d) * scale, part4(t.r[3], d) * scale, h1, l1);
-    *reinterpret_cast<v2u *>(h + d * stride) = v2u{h0, h1};
-    *reinterpret_cast<v2u *>(l + d * stride) = v2u{l0, l1};
-  }
-}
-// Where a group of four keys (key / 4) stands in a row of V^T.
-__device__ __forceinline__ int key_slot(int group) { return group / 4 * 16 + (group & 1) * 8 + (group >> 1 & 1) * 4; }
-
-__device__ __forceinline__ v8h frag(const _Float16 *p) { return *reinterpret_cast<const v8h *>(p); }
 
 // Eight floats from d on of a row, as operands.
 template <bool kFull>
@@ -192,61 +181,80 @@ __device__ __forceinline__ void load8(const float *p, int d, int HS, bool live, 
     x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
   }
 }
-__device__ __forceinline__ void split8(const float (&x)[8], float scale, v8h &h, v8h &l) {
-  v4u a, b;
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    uint32_t hj, lj;
-    split2(x[2 * j] * scale, x[2 * j + 1] * scale, hj, lj);
-    a[j] = hj;
-    b[j] = lj;
+
+__device__ __forceinline__ void put4(float *p, float4 w, int nd, bool full, bool assign) {
+  if (full || nd >= 4) {
+    if (!assign) {
+      const float4 u = ld4(p);
+      w = make_float4(u.x + w.x, u.y + w.y, u.z + w.z, u.w + w.w);
+    }
+    st4(p, w);
+  } else {
+    if (nd > 0) put(p, w.x, assign);
+    if (nd > 1) put(p + 1, w.y, assign);
+    if (nd > 2) put(p + 2, w.z, assign);
   }
-  h = __builtin_bit_cast(v8h, a);
-  l = __builtin_bit_cast(v8h, b);
+}
+// An accumulator's column (this lane's row of the result) to memory, times f.
+template <int DB, bool kFull>
+__device__ __forceinline__ void put_row(float *p, const v16f (&acc)[DB], float f, int half, int HS, bool assign) {
+#pragma unroll
+  for (int x = 0; x < DB; x++)
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+      const int d = 32 * x + 8 * y + 4 * half;
+      put4(p + d, make_float4(acc[x][4 * y] * f, acc[x][4 * y + 1] * f, acc[x][4 * y + 2] * f, acc[x][4 * y + 3] * f),
+           HS - d, kFull, assign);
+    }
 }
 
-template <int HSP, int BK, int W, bool kFull>
+// The largest of a noted quantity over the workgroup's wavefronts.
+template <int W>
+__device__ __forceinline__ uint32_t noted(const uint32_t (&slot)[W]) {
+  uint32_t m = slot[0];
+#pragma unroll
+  for (int w = 1; w < W; w++) m = max(m, slot[w]);
+  return (uint32_t)__builtin_amdgcn_readfirstlane(m);
+}
+
+template <int HSP, int BK, int W, int QB, bool kFull>
 __global__ __launch_bounds__(W * kWave, W == 1 ? 1 : 2) void k_att_fwd(float *out, float *lse, const float *q, const float *k,
-                                                       const float *v, ugk_attention a, Parts parts, unsigned pairs,
-                                                       int *word) {
-  constexpr int kThreads = W * kWave, KB = BK / 32, DC = HSP / 16, DB = HSP / 32, DG = HSP / 4;
+                                                                       const float *v, ugk_attention a, Parts parts,
+                                                                       unsigned pairs, int *word) {
+  constexpr int kThreads = W * kWave, KB = BK / 32, DC = HSP / 16, DB = HSP / 32, DG = HSP / 4, kTile = 32 * W * QB;
   constexpr int kBlocks = BK / 4 * DG, kPer = 2 * kBlocks / kThreads;  // 4 x 4 blocks: of K and of V, per thread
-  static_assert(kBlocks % kThreads == 0, "as many blocks of K and of V for each thread");
-  constexpr int kKs = HSP + 8, kVs = BK + 8;  // strides: odd multiples of 16 bytes, free of bank conflicts
-  __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kKs], lv[2][2][HSP * kVs];
+  static_assert(kPer >= 1 && kBlocks % kWave == 0, "whole wavefronts of K or V blocks");
+  constexpr int kRs = HSP + 8, KG = BK / 4;  // halves a row: an odd multiple of 16 bytes, free of bank conflicts
+  __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kRs], lv[2][2][BK * kRs];
   __shared__ uint32_t slot[2][4][W];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
   const unsigned pair = blockIdx.x % pairs;
   const int tile = (int)(gridDim.x / pairs - 1 - blockIdx.x / pairs);  // the longest rows first
   const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
   const Seq s = sequence(a, b, hk == 0 && tile == 0 && blockIdx.y == 0, word, UGK_IDS_ATTENTION_FORWARD);
-  const int rows = s.Lq * G, row0 = tile * (32 * W);
+  const int rows = s.Lq * G, row0 = tile * kTile;
   if (row0 >= rows) return;
   const float *kb = k + (size_t)s.k0 * a.ldk + hk * a.HS, *vb = v + (size_t)s.k0 * a.ldv + hk * a.HS;
   // this part's keys, and those that the workgroup's last row sees
   const int first = parts.o ? min((int)blockIdx.y * parts.chunk, s.Lk) : 0;
   const int stop = parts.o ? min(first + parts.chunk, s.Lk) : s.Lk;
-  const int n = max(first, min(stop, s.seen((min(row0 + 32 * W, rows) - 1) / G, a.causal)));
+  const int n = max(first, min(stop, s.seen((min(row0 + kTile, rows) - 1) / G, a.causal)));
   const int least = s.seen(row0 / G, a.causal);  // what every row of the workgroup sees
 
-  // this lane's row
-  const int r = row0 + wave * 32 + (lane & 31);
-  const bool live = r < rows;
-  const int i = r / G, h = hk * G + r % G;
-  const int lim = live ? min(n, s.seen(i, a.causal)) : 0;
-  int lo = live ? lim : n, hi = lim;  // least and most over the wavefront
+  // this lane's rows
+  const int r0 = row0 + wave * (32 * QB) + (lane & 31);
+  int lim[QB], lo = n, hi = first;  // what they see; least and most over the wavefront
+  v8h qh[QB][DC], ql[QB][DC];
+  float cq[QB];  // of the scores, to base 2
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    lo = min(lo, __shfl_xor(lo, o));
-    hi = max(hi, __shfl_xor(hi, o));
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  const size_t grow = (size_t)s.q0 + (live ? i : 0);
-  const float *qr = q + grow * a.ldq + (live ? h : 0) * a.HS;
-  v8h qh[DC], ql[DC];
-  float cq;  // of the scores, to base 2
-  {
+  for (int u = 0; u < QB; u++) {
+    const int r = r0 + 32 * u;
+    const bool live = r < rows;
+    const int i = live ? r / G : 0, h = hk * G + (live ? r % G : 0);
+    lim[u] = live ? min(n, s.seen(i, a.causal)) : 0;
+    if (live) lo = min(lo, lim[u]);
+    hi = max(hi, lim[u]);
+    const float *qr = q + ((size_t)s.q0 + i) * a.ldq + h * a.HS;
     float x[DC][8];
     uint32_t m = 0;
 #pragma unroll
@@ -258,32 +266,43 @@ __global__ __launch_bounds__(W * kWave, W == 1 ? 1 : 2) void k_att_fwd(float *ou
     const int e = split_exp(half_max_bits(m));
     const float f = a.scale < 0.0f ? -split_scale(e) : split_scale(e);
 #pragma unroll
-    for (int c = 0; c < DC; c++) split8(x[c], f, qh[c], ql[c]);
-    cq = split_unscale(e) * (fabsf(a.scale) * kLog2e);
+    for (int c = 0; c < DC; c++) split8(x[c], f, qh[u][c], ql[u][c]);
+    cq[u] = split_unscale(e) * (fabsf(a.scale) * kLog2e);
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
 
   Rows4 t[kPer];
-  const auto is_v = [&](int u) { return u >= kPer / 2; };
+  const auto is_v = [&](int u) { return kPer == 1 ? wave >= W / 2 : u >= kPer / 2; };
   const auto block = [&](int u) { return (tid + u * kThreads) % kBlocks; };
   const auto load = [&](int k0) {
     const bool tail = k0 + BK > n;
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const int d = block(u) % DG * 4, j = k0 + block(u) / DG * 4;
-      t[u] = load_rows<kFull>((is_v(u) ? vb : kb) + d, is_v(u) ? a.ldv : a.ldk, j, n, tail, a.HS - d);
+      const int d = block(u) % DG * 4, j = k0 + block(u) / DG;
+      t[u] = load_rows<KG, kFull>((is_v(u) ? vb : kb) + d, is_v(u) ? a.ldv : a.ldk, j, n, tail, a.HS - d);
     }
   };
   // The tile's largest magnitudes, of K and V, and where not all rows see all of it
   // the least of the keys' largest.
   const auto note = [&](int at, int k0) {
     uint32_t m[4] = {};
-#pragma unroll
-    for (int u = 0; u < kPer; u++) m[is_v(u) ? 1 : 0] = max_abs(m[is_v(u) ? 1 : 0], t[u]);
     if (k0 + BK > least) {
 #pragma unroll
-      for (int u = 0; u < kPer; u++) m[is_v(u) ? 3 : 2] = least_row<DG>(m[is_v(u) ? 3 : 2], t[u]);
+      for (int u = 0; u < kPer; u++) {
+        m[is_v(u) ? 1 : 0] = max_abs<true>(m[is_v(u) ? 1 : 0], t[u]);
+        m[is_v(u) ? 3 : 2] = least_row<DG>(m[is_v(u) ? 3 : 2], t[u]);
+      }
       m[2] = wave_max_bits(m[2]);
       m[3] = wave_max_bits(m[3]);
+    } else {  // a NaN that every row sees is every row's result, as it comes
+#pragma unroll
+      for (int u = 0; u < kPer; u++) m[is_v(u) ? 1 : 0] = max_abs<false>(m[is_v(u) ? 1 : 0], t[u]);
     }
     m[0] = wave_max_bits(m[0]);
     m[1] = wave_max_bits(m[1]);
@@ -292,87 +311,116 @@ __global__ __launch_bounds__(W * kWave, W == 1 ? 1 : 2) void k_att_fwd(float *ou
       for (int x = 0; x < 4; x++) slot[at][x][wave] = m[x];
     }
   };
-  const auto noted = [&](int at, int which) {
-    uint32_t m = slot[at][which][0];
-#pragma unroll
-    for (int w = 1; w < W; w++) m = max(m, slot[at][which][w]);
-    return (uint32_t)__builtin_amdgcn_readfirstlane(m);
-  };
   bool bad = false;
-  int ek = 0, ev = -100, ek_next = 0, ev_next = -100;
+  int ek_next = 0, ev_next = -100;
   const auto stage = [&](int at) {
-    const uint32_t mk = noted(at, 0), mv = noted(at, 1);
-    bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted(at, 2)) || too_wide(mv, noted(at, 3));
+    const uint32_t mk = noted<W>(slot[at][0]), mv = noted<W>(slot[at][1]);
+    bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted<W>(slot[at][2])) || too_wide(mv, noted<W>(slot[at][3]));
     ek_next = split_exp(mk);
     ev_next = max(ev_next, split_exp(mv));
     const float fk = split_scale(ek_next), fv = split_scale(ev_next);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const int d = block(u) % DG * 4, g = block(u) / DG;
-      if (is_v(u)) put_cols(t[u], fv, lv[at][0] + d * kVs + key_slot(g), lv[at][1] + d * kVs + key_slot(g), kVs);
-      else put_rows(t[u], fk, lk[at][0] + 4 * g * kKs + d, lk[at][1] + 4 * g * kKs + d, kKs);
+      const int p = block(u) / DG * kRs + block(u) % DG * 4;
+      put_rows<KG>(t[u], is_v(u) ? fv : fk, (is_v(u) ? lv : lk)[at][0] + p, (is_v(u) ? lv : lk)[at][1] + p, kRs);
     }
   };
 
-  v16f o[DB] = {};
-  float l = 0.0f, bias = INFINITY;  // bias: 15 - the row's maximum so far
-  const auto compute = [&](int at, int k0, int ev_now) {
-    v16f sc[KB] = {};
+  v16f o[QB][DB] = {};
+  float l[QB] = {}, bias[QB];  // bias: kTop - the maximum that the row's P stand on
+  int ev = -100;
 #pragma unroll
-    for (int c = 0; c < DC; c++)
+  for (int u = 0; u < QB; u++) bias[u] = INFINITY;
+  const int vcols = cols_at(lane, kRs);
+  const auto compute = [&](int at, int k0, int ek, int ev_now) {
+    const float uk = split_unscale(ek);
+    float c2[QB];
 #pragma unroll
-      for (int x = 0; x < KB; x++) {
-        const int p = (32 * x + (lane & 31)) * kKs + 16 * c + 8 * half;
-        sc[x] = mfma3(frag(lk[at][0] + p), frag(lk[at][1] + p), qh[c], ql[c], sc[x]);
-      }
-    const float c2 = fmaxf(cq * split_unscale(ek), 0x1p-126f);
-    if (k0 + BK > lo) {  // some row does not see all of the tile
-      const int rel = lim - k0 - 4 * half;
-#pragma unroll
-      for (int x = 0; x < KB; x++)
-#pragma unroll
-        for (int y = 0; y < 16; y++)
-          if (32 * x + 8 * (y / 4) + y % 4 >= rel) sc[x][y] = -INFINITY;
+    for (int u = 0; u < QB; u++) {
+      c2[u] = fmaxf(cq[u] * uk, 0x1p-126f);
+      bad = bad || c2[u] > 0x1p100f;
     }
-    float m = -INFINITY;
+    if (ev != ev_now) {
+      const float f = pow2(max(ev - ev_now, -126));
 #pragma unroll
-    for (int x = 0; x < KB; x++)
+      for (int u = 0; u < QB; u++)
 #pragma unroll
-      for (int y = 0; y < 16; y++) m = fmaxf(m, sc[x][y]);
-    m = half_max(m) * c2;
-    bad = bad || (fabsf(m) >= 0x1p22f && m != -INFINITY) || c2 > 0x1p100f;
-    const float was = bias;
-    bias = fminf(bias, 15.0f - m);
-    const float b0 = bias == INFINITY ? 0.0f : bias;  // no key so far: every score is -inf
-    float sum = 0.0f;
+        for (int x = 0; x < DB; x++)
 #pragma unroll
-    for (int x = 0; x < KB; x++)
-#pragma unroll
-      for (int y = 0; y < 16; y++) {
-        sc[x][y] = __builtin_amdgcn_exp2f(fmaf(sc[x][y], c2, b0));
-        sum += sc[x][y];
-      }
-    const float keep = was == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(b0 - was);
-    l = fmaf(l, keep, sum);
-    if (__any(keep != 1.0f) || ev != ev_now) {
-      const float f = keep * pow2(max(ev - ev_now, -126));
+          for (int y = 0; y < 16; y++) o[u][x][y] *= f;
       ev = ev_now;
-#pragma unroll
-      for (int x = 0; x < DB; x++)
-#pragma unroll
-        for (int y = 0; y < 16; y++) o[x][y] *= f;
     }
 #pragma unroll
-    for (int c = 0; c < 2 * KB; c++) {
-      float p[8];
+    for (int w = 0; w < KB; w++) {  // 32 keys
+      v16f sc[QB] = {};
 #pragma unroll
-      for (int j = 0; j < 8; j++) p[j] = sc[c / 2][8 * (c % 2) + j];
-      v8h ph, pl;
-      split8(p, 1.0f, ph, pl);
+      for (int c = 0; c < DC; c++) {
+        const int p = (32 * w + (lane & 31)) * kRs + 16 * c + 8 * half;
+        const v8h fh = frag(lk[at][0] + p), fl = frag(lk[at][1] + p);
 #pragma unroll
-      for (int x = 0; x < DB; x++) {
-        const int at_v = (32 * x + (lane & 31)) * kVs + 16 * c + 8 * half;
-        o[x] = mfma3(frag(lv[at][0] + at_v), frag(lv[at][1] + at_v), ph, pl, o[x]);
+        for (int u = 0; u < QB; u++) sc[u] = mfma3(fh, fl, qh[u][c], ql[u][c], sc[u]);
+      }
+      if (k0 + 32 * w + 32 > lo) {  // some row does not see all of the keys
+#pragma unroll
+        for (int u = 0; u < QB; u++) {
+          const int rel = lim[u] - k0 - 32 * w - 4 * half;
+#pragma unroll
+          for (int y = 0; y < 16; y++)
+            if (8 * (y / 4) + y % 4 >= rel) sc[u][y] = -INFINITY;
+        }
+      }
+      float m[QB];
+      bool grown = false;
+#pragma unroll
+      for (int u = 0; u < QB; u++) {
+        m[u] = sc[u][0];
+#pragma unroll
+        for (int y = 1; y < 16; y++) m[u] = fmaxf(m[u], sc[u][y]);
+        m[u] = half_max(m[u]) * c2[u];
+        grown = grown || m[u] + bias[u] > kTop + 7.0f;
+      }
+      if (__any(grown)) {
+#pragma unroll
+        for (int u = 0; u < QB; u++) {
+          bad = bad || (fabsf(m[u]) >= 0x1p22f && m[u] != -INFINITY);
+          const float was = bias[u];
+          bias[u] = fminf(was, kTop - m[u]);
+          const float f = was == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(bias[u] - was);
+          l[u] *= f;
+#pragma unroll
+          for (int x = 0; x < DB; x++)
+#pragma unroll
+            for (int y = 0; y < 16; y++) o[u][x][y] *= f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < QB; u++) {
+        const float b0 = bias[u] == INFINITY ? 0.0f : bias[u];  // no key so far: every score is -inf
+        float sum = 0.0f;
+#pragma unroll
+        for (int y = 0; y < 16; y++) {
+          sc[u][y] = __builtin_amdgcn_exp2f(fmaf(sc[u][y], c2[u], b0));
+          sum += sc[u][y];
+        }
+        l[u] += sum;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        v8h ph[QB], pl[QB];
+#pragma unroll
+        for (int u = 0; u < QB; u++) {
+          float p[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) p[j] = sc[u][8 * c + j];
+          split8(p, ph[u], pl[u]);
+        }
+#pragma unroll
+        for (int x = 0; x < DB; x++) {
+          const int p = (32 * w + 16 * c) * kRs + 32 * x + vcols;
+          const v8h fh = frag_cols(lv[at][0] + p, kRs), fl = frag_cols(lv[at][1] + p, kRs);
+#pragma unroll
+          for (int u = 0; u < QB; u++) o[u][x] = mfma3(fh, fl, ph[u], pl[u], o[u][x]);
+        }
       }
     }
   };
@@ -389,72 +437,45 @@ __global__ __launch_bounds__(W * kWave, W == 1 ? 1 : 2) void k_att_fwd(float *ou
     }
     __syncthreads();
     for (int at = 0; at < tiles; at++) {
-      const int k0 = first + at * BK;
-      const int ev_now = ev_next;
-      ek = ek_next;
+      const int k0 = first + at * BK, ek = ek_next, ev_now = ev_next;
       // tile at + 1: its maxima are noted, its buffer was read two barriers ago
       if (at + 1 < tiles) stage((at + 1) & 1);
       if (at + 2 < tiles) load(k0 + 2 * BK);
-      if (k0 < hi) compute(at & 1, k0, ev_now);
+      if (k0 < hi) compute(at & 1, k0, ek, ev_now);
       if (at + 2 < tiles) note(at & 1, k0 + 2 * BK);
       __syncthreads();
     }
   }
   // Any wavefront's trouble with a tile is every wavefront's; with its scores its own.
   if (__any(bad)) {
-    for (int x = 0; x < 32; x++) {
-      const int rr = row0 + wave * 32 + x;
+    for (int x = 0; x < 32 * QB; x++) {
+      const int rr = row0 + wave * (32 * QB) + x;
       if (rr >= rows) break;
       const int ii = rr / G, hh = hk * G + rr % G;
       const size_t g = (size_t)s.q0 + ii;
       const int upto = min(n, s.seen(ii, a.causal));
-      float *po = parts.o ? parts.o + (((size_t)blockIdx.y * a.nseq + b) * a.max_q + ii) * a.NH * a.HS + (size_t)hh * a.HS
-                          : out + g * a.ldo + hh * a.HS;
-      float *pl = parts.o ? parts.lse + (((size_t)blockIdx.y * a.nseq + b) * a.max_q + ii) * a.NH + hh
-                          : lse ? lse + g * a.NH + hh : nullptr;
-      row_forward(po, pl, q + g * a.ldq + hh * a.HS, kb + first * a.ldk, vb + first * a.ldv, max(upto - first, 0), a.HS,
-                  a.ldk, a.ldv, a.scale);
+      const size_t prow = (((size_t)blockIdx.y * a.nseq + b) * a.max_q + ii) * a.NH + hh;
+      row_forward(parts.o ? parts.o + prow * a.HS : out + g * a.ldo + hh * a.HS,
+                  parts.o ? parts.lse + prow : lse ? lse + g * a.NH + hh : nullptr, q + g * a.ldq + hh * a.HS,
+                  kb + first * a.ldk, vb + first * a.ldv, max(upto - first, 0), a.HS, a.ldk, a.ldv, a.scale);
     }
     return;
   }
-  if (!live) return;
-  l = half_sum(l);
-  const size_t prow = ((size_t)blockIdx.y * a.nseq + b) * a.max_q + i;
-  const bool some = lim > first;
-  const float f = some ? split_unscale(ev) / l : 0.0f;
-  float *po = parts.o ? parts.o + prow * a.NH * a.HS + (size_t)h * a.HS : out + grow * a.ldo + h * a.HS;
 #pragma unroll
-  for (int x = 0; x < DB; x++)
-#pragma unroll
-    for (int y = 0; y < 4; y++) {
-      const int d = 32 * x + 8 * y + 4 * half;
-      const float4 w = make_float4(o[x][4 * y] * f, o[x][4 * y + 1] * f, o[x][4 * y + 2] * f, o[x][4 * y + 3] * f);
-      if (kFull || d + 4 <= a.HS) {
-        st4(po + d, w);
-      } else {
-        if (d < a.HS) po[d] = w.x;
-        if (d + 1 < a.HS) po[d + 1] = w.y;
-        if (d + 2 < a.HS) po[d + 2] = w.z;
-      }
+  for (int u = 0; u < QB; u++) {
+    const int r = r0 + 32 * u;
+    if (r >= rows) break;
+    const int i = r / G, h = hk * G + r % G;
+    const size_t grow = (size_t)s.q0 + i, prow = (((size_t)blockIdx.y * a.nseq + b) * a.max_q + i) * a.NH + h;
+    const float sum = half_sum(l[u]);
+    const bool some = lim[u] > first;
+    put_row<DB, kFull>(parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS, o[u],
+                       some ? split_unscale(ev) / sum : 0.0f, half, a.HS, true);
+    if (half == 0 && (parts.o || lse)) {
+      const float L = some ? (__builtin_amdgcn_logf(sum) - bias[u]) * kLn2 : -INFINITY;
+      if (parts.o) parts.lse[prow] = L;
+      else lse[grow * a.NH + h] = L;
     }
-  if (half == 0 && (parts.o || lse)) {
-    const float L = some ? (__builtin_amdgcn_logf(l) - bias) * kLn2 : -INFINITY;
-    if (parts.o) parts.lse[prow * a.NH + h] = L;
-    else lse[grow * a.NH + h] = L;
-  }
-}
-
-__device__ __forceinline__ void put4(float *p, float4 w, int nd, bool full, bool assign) {
-  if (full || nd >= 4) {
-    if (!assign) {
-      const float4 u = ld4(p);
-      w = make_float4(u.x + w.x, u.y + w.y, u.z + w.z, u.w + w.w);
-    }
-    st4(p, w);
-  } else {
-    if (nd > 0) put(p, w.x, assign);
-    if (nd > 1) put(p + 1, w.y, assign);
-    if (nd > 2) put(p + 2, w.z, assign);
   }
 }
 
@@ -723,24 +744,12 @@ __device__ void row_dkv(float *dk, float *dv, const float *dout, const float *q,
 // remainder reach 2^39 below the bound. The same tiles as in the forward fall
 // back to single rows.
 
-// An accumulator's column (this lane's row of the result) to memory, times f.
-template <int DB, bool kFull>
-__device__ __forceinline__ void put_row(float *p, const v16f (&acc)[DB], float f, int half, int HS, bool assign) {
-#pragma unroll
-  for (int x = 0; x < DB; x++)
-#pragma unroll
-    for (int y = 0; y < 4; y++) {
-      const int d = 32 * x + 8 * y + 4 * half;
-      put4(p + d, make_float4(acc[x][4 * y] * f, acc[x][4 * y + 1] * f, acc[x][4 * y + 2] * f, acc[x][4 * y + 3] * f),
-           HS - d, kFull, assign);
-    }
-}
 
-// acc += A B for a 32-row block of B held in an accumulator's registers (C, scaled
-// to halves by f): A's rows in LDS, HSP of them, their columns in key_slot's order.
+// acc += A^T B for a 32-row block of B held in an accumulator's registers (C, scaled
+// to halves by f): A's 32 rows in LDS, `cols` the lane's place in them (cols_at).
 template <int DB>
 __device__ __forceinline__ void mac_block(v16f (&acc)[DB], const v16f &c, float f, const _Float16 *ah, const _Float16 *al,
-                                          int stride, int lane) {
+                                          int stride, int cols) {
 #pragma unroll
   for (int y = 0; y < 2; y++) {
     float p[8];
@@ -750,8 +759,8 @@ __device__ __forceinline__ void mac_block(v16f (&acc)[DB], const v16f &c, float 
     split8(p, f, bh, bl);
 #pragma unroll
     for (int x = 0; x < DB; x++) {
-      const int at = (32 * x + (lane & 31)) * stride + 16 * y + 8 * (lane >> 5);
-      acc[x] = mfma3(frag(ah + at), frag(al + at), bh, bl, acc[x]);
+      const int at = 16 * y * stride + 32 * x + cols;
+      acc[x] = mfma3(frag_cols(ah + at, stride), frag_cols(al + at, stride), bh, bl, acc[x]);
     }
   }
 }
@@ -787,14 +796,6 @@ __device__ __forceinline__ uint32_t load_operand(const float *p, int HS, bool li
   return m;
 }
 
-// The largest of a noted quantity over the workgroup's wavefronts.
-template <int W>
-__device__ __forceinline__ uint32_t noted(const uint32_t (&slot)[W]) {
-  uint32_t m = slot[0];
-#pragma unroll
-  for (int w = 1; w < W; w++) m = max(m, slot[w]);
-  return (uint32_t)__builtin_amdgcn_readfirstlane(m);
-}
 
 template <int HSP, int W, bool kFull>
 __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dq(
@@ -803,8 +804,8 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dq
   constexpr int kThreads = W * kWave, BK = 32, DC = HSP / 16, DB = HSP / 32, DG = HSP / 4;
   constexpr int kBlocks = BK / 4 * DG, kPer = 2 * kBlocks / kThreads;
   static_assert(kPer >= 1 && kBlocks % kWave == 0, "whole wavefronts of K or V blocks");
-  constexpr int kRs = HSP + 8, kCs = BK + 8;
-  __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kRs], lv[2][2][BK * kRs], lt[2][2][HSP * kCs];
+  constexpr int kRs = HSP + 8, KG = BK / 4;
+  __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kRs], lv[2][2][BK * kRs];
   __shared__ uint32_t slot[2][4][W];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
   const unsigned pair = blockIdx.x % pairs;
@@ -850,17 +851,16 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dq
   bool bad = lim > 0 && !(fabsf(L2) < 0x1p22f);  // (the row's own q and dout reach its own results alone)
 
   Rows4 t[kPer];
-  // K blocks by half of the wavefronts, V blocks by the others, in turn: K's are put twice
-  const auto is_v = [&](int u, int at) { return kPer == 1 ? ((wave >= W / 2) ^ (at & 1)) != 0 : u >= kPer / 2; };
+  const auto is_v = [&](int u) { return kPer == 1 ? wave >= W / 2 : u >= kPer / 2; };
   const auto block = [&](int u) { return (tid + u * kThreads) % kBlocks; };
   const auto load = [&](int at) {
     const int k0 = at * BK;
     const bool tail = k0 + BK > n;
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const int d = block(u) % DG * 4, j = k0 + block(u) / DG * 4;
-      const bool w = is_v(u, at);
-      t[u] = load_rows<kFull>((w ? vb : kb) + d, w ? a.ldv : a.ldk, j, n, tail, a.HS - d);
+      const int d = block(u) % DG * 4, j = k0 + block(u) / DG;
+      const bool w = is_v(u);
+      t[u] = load_rows<KG, kFull>((w ? vb : kb) + d, w ? a.ldv : a.ldk, j, n, tail, a.HS - d);
     }
   };
   const auto note = [&](int at) {
@@ -868,8 +868,8 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dq
     const bool part = (at + 1) * BK > least;
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const uint32_t x = max_abs(0u, t[u]), y = part ? least_row<DG>(0u, t[u]) : 0u;
-      if (is_v(u, at)) {
+      const uint32_t x = max_abs<true>(0u, t[u]), y = part ? least_row<DG>(0u, t[u]) : 0u;
+      if (is_v(u)) {
         m[1] = max(m[1], x);
         m[3] = max(m[3], y);
       } else {
@@ -894,18 +894,15 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dq
     const float fk = split_scale(ek), fv = split_scale(ev);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const int d = block(u) % DG * 4, g = block(u) / DG;
-      if (is_v(u, at)) {
-        put_rows(t[u], fv, lv[z][0] + 4 * g * kRs + d, lv[z][1] + 4 * g * kRs + d, kRs);
-      } else {
-        put_rows(t[u], fk, lk[z][0] + 4 * g * kRs + d, lk[z][1] + 4 * g * kRs + d, kRs);
-        put_cols(t[u], fk, lt[z][0] + d * kCs + key_slot(g), lt[z][1] + d * kCs + key_slot(g), kCs);
-      }
+      const int p = block(u) / DG * kRs + block(u) % DG * 4;
+      const bool w = is_v(u);
+      put_rows<KG>(t[u], w ? fv : fk, (w ? lv : lk)[z][0] + p, (w ? lv : lk)[z][1] + p, kRs);
     }
   };
 
   v16f acc[DB] = {};
   int ek_acc = -100, es = -100, ev_acc = -101;  // of the accumulators: K's, dS's and what dS's stands on
+  const int cols = cols_at(lane, kRs);
   const auto compute = [&](int at, int ek_now, int ev_now) {
     const int z = at & 1, k0 = at * BK;
     if (ek_now != ek_acc || ev_now != ev_acc) {
@@ -936,7 +933,7 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dq
       for (int y = 0; y < 16; y++)
         if (8 * (y / 4) + y % 4 >= rel) p[y] = 0.0f;
     }
-    mac_block<DB>(acc, p, f, lt[z][0], lt[z][1], kCs, lane);
+    mac_block<DB>(acc, p, f, lk[z][0], lk[z][1], kRs, cols);
   };
 
   const int tiles = (n + BK - 1) / BK;
@@ -987,13 +984,13 @@ struct GroupRows {
     return base + i * ld + (r - i * G) * HS;
   }
 };
-template <bool kFull>
+template <int kStep, bool kFull>
 __device__ __forceinline__ Rows4 load_rows(const GroupRows &g, int d, int r, int n, int nd) {
   Rows4 t;
 #pragma unroll
   for (int x = 0; x < 4; x++) {
-    t.r[x] = load4<kFull>(g.at(min(r + x, n - 1)) + d, nd);
-    if (r + x >= n) t.r[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    t.r[x] = load4<kFull>(g.at(min(r + kStep * x, n - 1)) + d, nd);
+    if (r + kStep * x >= n) t.r[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   return t;
 }
@@ -1005,9 +1002,8 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dk
   constexpr int kThreads = W * kWave, BQ = 32, DC = HSP / 16, DB = HSP / 32, DG = HSP / 4;
   constexpr int kBlocks = BQ / 4 * DG, kPer = 2 * kBlocks / kThreads;
   static_assert(kPer >= 1 && kBlocks % kWave == 0, "whole wavefronts of Q or dout blocks");
-  constexpr int kRs = HSP + 8, kCs = BQ + 8;
-  __shared__ __attribute__((aligned(16))) _Float16 lq[2][2][BQ * kRs], lg[2][2][BQ * kRs], tq[2][2][HSP * kCs],
-      tg[2][2][HSP * kCs];
+  constexpr int kRs = HSP + 8, KG = BQ / 4;
+  __shared__ __attribute__((aligned(16))) _Float16 lq[2][2][BQ * kRs], lg[2][2][BQ * kRs];
   __shared__ __attribute__((aligned(16))) float lL[2][BQ], lD[2][BQ];
   __shared__ uint32_t slot[2][6][W];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
@@ -1050,8 +1046,8 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dk
   const auto load = [&](int r0) {
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const int d = block(u) % DG * 4, r = r0 + block(u) / DG * 4;
-      t[u] = load_rows<kFull>(is_g(u) ? gg : gq, d, r, rows, a.HS - d);
+      const int d = block(u) % DG * 4, r = r0 + block(u) / DG;
+      t[u] = load_rows<KG, kFull>(is_g(u) ? gg : gq, d, r, rows, a.HS - d);
     }
     if (tid < BQ) {
       const int r = r0 + tid, i = min(r, rows - 1) / G, x = min(r, rows - 1) - i * G;
@@ -1065,7 +1061,7 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dk
     const bool part = r0 < all;
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const uint32_t x = max_abs(0u, t[u]), y = part ? least_row<DG>(0u, t[u]) : 0u;
+      const uint32_t x = max_abs<true>(0u, t[u]), y = part ? least_row<DG>(0u, t[u]) : 0u;
       if (is_g(u)) {
         m[1] = max(m[1], x);
         m[3] = max(m[3], y);
@@ -1098,12 +1094,9 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dk
     const float fq = split_scale(eq), fg = split_scale(eg);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
-      const int d = block(u) % DG * 4, g = block(u) / DG;
-      const float f = is_g(u) ? fg : fq;
-      _Float16 *rh = is_g(u) ? lg[z][0] : lq[z][0], *rl = is_g(u) ? lg[z][1] : lq[z][1];
-      _Float16 *ch = is_g(u) ? tg[z][0] : tq[z][0], *cl = is_g(u) ? tg[z][1] : tq[z][1];
-      put_rows(t[u], f, rh + 4 * g * kRs + d, rl + 4 * g * kRs + d, kRs);
-      put_cols(t[u], f, ch + d * kCs + key_slot(g), cl + d * kCs + key_slot(g), kCs);
+      const int p = block(u) / DG * kRs + block(u) % DG * 4;
+      const bool w = is_g(u);
+      put_rows<KG>(t[u], w ? fg : fq, (w ? lg : lq)[z][0] + p, (w ? lg : lq)[z][1] + p, kRs);
     }
     if (tid < BQ) {
       lL[z][tid] = tL;
@@ -1114,6 +1107,7 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dk
   v16f ak[DB] = {}, av[DB] = {};
   int eq_acc = -100, eg_acc = -100, es = -100;
   float dmax_acc = -1.0f;
+  const int cols = cols_at(lane, kRs);
   const auto compute = [&](int z, int r0, int eq_now, int eg_now, float dmax_now) {
     if (eq_now != eq_acc || eg_now != eg_acc || dmax_now != dmax_acc) {
       const float bound = fmaf((float)a.HS * vmax, pow2(min(max(eg_now, -126), 127)), dmax_now);
@@ -1155,8 +1149,8 @@ __global__ __launch_bounds__(W * kWave, W < 4 || HSP > 64 ? 1 : 2) void k_att_dk
       for (int y = 0; y < 16; y++)
         if (8 * (y / 4) + y % 4 < rel) p[y] = ds[y] = 0.0f;
     }
-    mac_block<DB>(av, p, 1.0f, tg[z][0], tg[z][1], kCs, lane);
-    mac_block<DB>(ak, ds, f, tq[z][0], tq[z][1], kCs, lane);
+    mac_block<DB>(av, p, 1.0f, lg[z][0], lg[z][1], kRs, cols);
+    mac_block<DB>(ak, ds, f, lq[z][0], lq[z][1], kRs, cols);
   };
 
   const int tiles = rows > from ? (rows - from + BQ - 1) / BQ : 0;
@@ -1216,13 +1210,13 @@ int tile_waves(long long pairs, long long rows) {
   return 1;
 }
 
-constexpr int kFewRows = 4;
+constexpr int kFewRows = 4, kFewChunk = 1024;
 constexpr size_t kMaxParts = 1 << 15;  // rows of a head that the parts hold at most
 
 // How the forward of `a` is cut: rows per key/value head where they are few (k_att_few),
 // wavefronts of a workgroup, tiles of rows, parts of the key axis and keys per part.
 struct FwdPlan {
-  int few, W, tiles, splits, chunk;
+  int few, W, QB, tiles, splits, chunk;
 };
 FwdPlan fwd_plan(const ugk_attention &a) {
   const long long pairs = (long long)a.nseq * a.NKV, rows = (long long)a.max_q * (a.NH / a.NKV);
@@ -1231,16 +1225,22 @@ FwdPlan fwd_plan(const ugk_attention &a) {
   if (rows <= kFewRows) {
     p.few = rows <= 1 ? 1 : rows <= 2 ? 2 : 4;
     p.tiles = 1;
-    p.W = pairs < 4 * cu_count() ? few_waves(p.few) : 4;
+    p.W = pairs < 4 * cu_count() && a.max_k <= kFewChunk ? few_waves(p.few) : 4;
     unit = p.W * (a.HS <= 64 ? 4 : 2) * few_loads(p.few);
   } else {
+    // Two 32-row blocks per wavefront halve the staging and the reads of K and V per
+    // row, and pay while there are three workgroups per CU to balance the causal
+    // rows' lengths (16,384 rows of 12 heads 1,335 us against 1,453, 4 x 4,096
+    // 415 against 444; with one and a half 8 x 1,024 88 against 70).
     p.W = pairs * ((rows + 127) / 128) >= cu_count() ? 4 : 1;
-    p.tiles = (int)((rows + 32 * p.W - 1) / (32 * p.W));
-    unit = a.HS <= 64 && p.W == 4 ? 64 : 32;
+    p.QB = a.HS <= 64 && pairs * ((rows + 255) / 256) >= 3 * cu_count() ? 2 : 1;
+    p.tiles = (int)((rows + 32 * p.W * p.QB - 1) / (32 * p.W * p.QB));
+    unit = a.HS <= 64 && p.W == 4 && p.QB == 1 ? 64 : 32;
   }
   p.splits = 1;
   const long long wgs = pairs * p.tiles, prow = (long long)a.nseq * a.max_q * a.NH;
-  long long want = (p.few ? 1 : 2) * cu_count() / (wgs > 0 ? wgs : 1);
+  long long want = (p.few ? 1 : p.W == 4 ? 2 : 4) * cu_count() / (wgs > 0 ? wgs : 1);
+  if (p.few) want = max(want, (a.max_k + (long long)kFewChunk - 1) / kFewChunk);
   want = min(want, (long long)a.max_k / (4 * unit));
   want = min(want, (long long)kMaxParts / (prow > 0 ? prow : 1));
   if (want > 1) {
@@ -1290,12 +1290,13 @@ int launch_attention_forward(float *out, float *lse, const float *q, const float
 #undef UGK_FEW_HS
   } else if (a.HS <= 64) {
     const bool full = a.HS == 64;
-    if (p.W == 4) full ? go(k_att_fwd<64, 64, 4, true>) : go(k_att_fwd<64, 64, 4, false>);
-    else full ? go(k_att_fwd<64, 32, 1, true>) : go(k_att_fwd<64, 32, 1, false>);
+    if (p.QB == 2) full ? go(k_att_fwd<64, 32, 4, 2, true>) : go(k_att_fwd<64, 32, 4, 2, false>);
+    else if (p.W == 4) full ? go(k_att_fwd<64, 64, 4, 1, true>) : go(k_att_fwd<64, 64, 4, 1, false>);
+    else full ? go(k_att_fwd<64, 32, 1, 1, true>) : go(k_att_fwd<64, 32, 1, 1, false>);
   } else {
     const bool full = a.HS == 128;
-    if (p.W == 4) full ? go(k_att_fwd<128, 32, 4, true>) : go(k_att_fwd<128, 32, 4, false>);
-    else full ? go(k_att_fwd<128, 32, 1, true>) : go(k_att_fwd<128, 32, 1, false>);
+    if (p.W == 4) full ? go(k_att_fwd<128, 32, 4, 1, true>) : go(k_att_fwd<128, 32, 4, 1, false>);
+    else full ? go(k_att_fwd<128, 32, 1, 1, true>) : go(k_att_fwd<128, 32, 1, 1, false>);
   }
   if (int e = check_launch("attention_forward")) return e;
   if (p.splits > 1) {

@@ -36,15 +36,59 @@ __device__ __forceinline__ v16f mfma3(v8h ah, v8h al, v8h bh, v8h bl, v16f c) {
   return mfma(ah, bl, mfma(al, bh, mfma(ah, bh, c)));
 }
 
-// Two floats as halves: h, and l of what h leaves.
+// Two floats as halves: h, and l of what h leaves (x - h in one instruction, without
+// a conversion of h; v_fma_mixlo_f16, which would round as well, takes twice the cycles).
 __device__ __forceinline__ void split2(float x, float y, uint32_t &h, uint32_t &l) {
   const v2f v = {x, y};
   h = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
-  float rx, ry;  // x - h without a conversion of h: one instruction each
+  float rx, ry;
   asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rx) : "v"(h), "v"(x));
   asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(ry) : "v"(h), "v"(y));
   const v2f r = {rx, ry};
   l = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
+}
+__device__ __forceinline__ void split2(float x, float y, float f, uint32_t &h, uint32_t &l) { split2(x * f, y * f, h, l); }
+// Eight of either kind, as an operand.
+__device__ __forceinline__ void split8(const float (&x)[8], float f, v8h &h, v8h &l) {
+  v4u a, b;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    uint32_t hj, lj;
+    split2(x[2 * j], x[2 * j + 1], f, hj, lj);
+    a[j] = hj;
+    b[j] = lj;
+  }
+  h = __builtin_bit_cast(v8h, a);
+  l = __builtin_bit_cast(v8h, b);
+}
+__device__ __forceinline__ void split8(const float (&x)[8], v8h &h, v8h &l) {
+  v4u a, b;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    uint32_t hj, lj;
+    split2(x[2 * j], x[2 * j + 1], hj, lj);
+    a[j] = hj;
+    b[j] = lj;
+  }
+  h = __builtin_bit_cast(v8h, a);
+  l = __builtin_bit_cast(v8h, b);
+}
+
+// Operands from rows of halves in LDS, `stride` halves each. As rows: the lane's row t % 32, eight
+// of its columns. As columns: column t % 32 of a 32-column block, of the eight
+// rows 4 (t / 32) + j and 8 + 4 (t / 32) + j, j < 4, that lane t's accumulator registers 0..7 hold (8..15 of
+// the rows from 16 on): two transposing reads of four rows of 16 columns per 16 lanes.
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef __fp16 v4f16 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4f16 lds_v4f16;
+__device__ __forceinline__ v8h frag(const _Float16 *p) { return *reinterpret_cast<const v8h *>(p); }
+__device__ __forceinline__ int cols_at(int lane, int stride) {
+  return (4 * (lane >> 5) + (lane >> 2 & 3)) * stride + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+}
+__device__ __forceinline__ v8h frag_cols(const _Float16 *p, int stride) {
+  const v4h a = __builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4f16 *)p));
+  const v4h b = __builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4f16 *)(p + 8 * stride)));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // The exponent that a largest magnitude (as its bits) is scaled by: x 2^(15 - e) is
@@ -104,10 +148,31 @@ __device__ __forceinline__ float half_sum(float x) {
 struct Rows4 {
   float4 r[4];
 };
+// The largest magnitude's bits. With kNan, NaN counts as the largest (of the
+// non-negative floats the largest as signed integers, of the others as unsigned
+// ones); without, it is passed over, for half of the instructions.
+template <bool kNan>
 __device__ __forceinline__ uint32_t max_abs(uint32_t m, const Rows4 &t) {
+  if (kNan) {
+    int pos = (int)m;
+    uint32_t neg = 0;
 #pragma unroll
-  for (int r = 0; r < 4; r++) m = max_abs(m, t.r[r]);
-  return m;
+    for (int r = 0; r < 4; r++) {
+      const uint32_t x = __float_as_uint(t.r[r].x), y = __float_as_uint(t.r[r].y), z = __float_as_uint(t.r[r].z), w = __float_as_uint(t.r[r].w);
+      pos = max(max(pos, (int)x), (int)y);
+      pos = max(max(pos, (int)z), (int)w);
+      neg = max(max(neg, x), y);
+      neg = max(max(neg, z), w);
+    }
+    return max((uint32_t)pos, neg & 0x7fffffffu);
+  }
+  float f = __uint_as_float(m);
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    f = fmaxf(fmaxf(f, fabsf(t.r[r].x)), fabsf(t.r[r].y));
+    f = fmaxf(fmaxf(f, fabsf(t.r[r].z)), fabsf(t.r[r].w));
+  }
+  return __float_as_uint(f);
 }
 // For the least of the rows' largest magnitudes, rows of zeros left out: the
 // complement, so that it is a maximum too. kLanes lanes share the four rows.

@@ -211,13 +211,15 @@ def _check(status: int) -> None:
 # torch (plumbing only: device memory), imported when the first tensor arrives, and what _ptr's
 # first line asks of a tensor
 _torch = _Tensor = _DTYPES = None
+_one_device = False  # only one GPU is visible: a tensor cannot be on another than the current one
 
 
 def _import_torch():
-    global _torch, _Tensor, _DTYPES
+    global _torch, _Tensor, _DTYPES, _one_device
     if _torch is None:
         import torch
         _torch, _Tensor, _DTYPES = torch, torch.Tensor, {"f32": torch.float32, "i32": torch.int32}
+        _one_device = torch.cuda.device_count() == 1
     return _torch
 
 
@@ -459,9 +461,16 @@ def layernorm_dropout_residual_backward(dinp, dweight, dbias, dx, dy, dout, inp,
         _ptr(rstd, "rstd", rows, "f32"), B, T, C, p, seed, step, site))
 
 
-def _rows_ptr(x, what: str, rows: int, ld: int, width: int):
-    """Device address of ``x``, the first of ``rows`` rows of ``width`` floats, ``ld`` (0: width) apart. A tensor may
-    be a view into the buffer that holds the rows: what counts is the memory behind its first element."""
+def _rows_ptr(x, what: str, need: int):
+    """Device address of ``x``, the first of rows that end ``need`` floats behind it. A tensor may be a view into the
+    buffer that holds the rows: what counts is the memory behind its first element. What passes is decided in
+    one line, the rest by _rows_ptr_or_raise."""
+    if type(x) is _Tensor and _one_device and x.dtype is _DTYPES["f32"] and x.is_cuda and x.numel() >= need and x.is_contiguous():
+        return x.data_ptr()
+    return _rows_ptr_or_raise(x, what, need)
+
+
+def _rows_ptr_or_raise(x, what: str, need: int):
     if x is None or isinstance(x, int):
         return x
     torch = _torch or _import_torch()
@@ -473,24 +482,26 @@ def _rows_ptr(x, what: str, rows: int, ld: int, width: int):
         raise ValueError(f"{what}: tensor is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
     if x.dtype != torch.float32:
         raise TypeError(f"{what}: dtype must be {torch.float32}, got {x.dtype}")
-    need = (rows - 1) * (ld or width) + width if rows > 0 else 0
     has = x.untyped_storage().nbytes() // 4 - x.storage_offset()
-    if x.numel() == 0 and need or has < need:
+    if need > 0 and (x.numel() == 0 or has < need):
         raise ValueError(f"{what}: needs at least {need} elements from its first one on, has {has}")
     return x.data_ptr()
 
 
-def _attention_ptrs(a: Attention, q, k, v, out):
-    q_w, k_w = a.NH * a.HS, a.NKV * a.HS
-    return ([_rows_ptr(x, n, a.rows_q, a.ldq, q_w) for n, x in q] + [_rows_ptr(x, n, a.rows_k, a.ldk, k_w) for n, x in k] +
-            [_rows_ptr(x, n, a.rows_k, a.ldv, k_w) for n, x in v] + [_rows_ptr(x, n, a.rows_q, a.ldo, q_w) for n, x in out])
+def _attention_needs(a: Attention):
+    """The floats from the first element of q, k, v and out to the end of their last rows."""
+    rq, rk, HS = a.rows_q - 1, a.rows_k - 1, a.HS
+    wq, wk = a.NH * HS, a.NKV * HS
+    return (rq * (a.ldq or wq) + wq if rq >= 0 else 0, rk * (a.ldk or wk) + wk if rk >= 0 else 0,
+            rk * (a.ldv or wk) + wk if rk >= 0 else 0, rq * (a.ldo or wq) + wq if rq >= 0 else 0)
 
 
 def attention_forward(out, lse, q, k, v, a: Attention) -> None:
     """gpt2_kernels.cuh:416-498, for grouped heads, sequences of different lengths and a cache too: per query row and
     head ``out = softmax(scale q.k) v`` over the allowed keys and ``lse = log sum exp`` (rows_q, NH), which may be
     None. q, k, v and out may be views into rows that hold other things as well (strides in ``a``)."""
-    pq, pk, pv, po = _attention_ptrs(a, [("q", q)], [("k", k)], [("v", v)], [("out", out)])
+    nq, nk, nv, no = _attention_needs(a)
+    pq, pk, pv, po = _rows_ptr(q, "q", nq), _rows_ptr(k, "k", nk), _rows_ptr(v, "v", nv), _rows_ptr(out, "out", no)
     _check(lib.ugk_attention_forward(po, _ptr(lse, "lse", a.rows_q * a.NH, "f32"), pq, pk, pv, a))
 
 
@@ -505,9 +516,10 @@ def attention_backward_zeroed(dq, dk, dv, dout, q, k, v, out, lse, a: Attention)
 
 
 def _attention_backward(fn, dq, dk, dv, dout, q, k, v, out, lse, a: Attention) -> None:
-    pdq, pq, pdk, pk, pdv, pv, pdo, po = _attention_ptrs(a, [("dq", dq), ("q", q)], [("dk", dk), ("k", k)],
-                                                         [("dv", dv), ("v", v)], [("dout", dout), ("out", out)])
-    _check(fn(pdq, pdk, pdv, pdo, pq, pk, pv, po, _ptr(lse, "lse", a.rows_q * a.NH, "f32"), a))
+    nq, nk, nv, no = _attention_needs(a)
+    _check(fn(_rows_ptr(dq, "dq", nq), _rows_ptr(dk, "dk", nk), _rows_ptr(dv, "dv", nv), _rows_ptr(dout, "dout", no),
+              _rows_ptr(q, "q", nq), _rows_ptr(k, "k", nk), _rows_ptr(v, "v", nv), _rows_ptr(out, "out", no),
+              _ptr(lse, "lse", a.rows_q * a.NH, "f32"), a))
 
 
 def dense_attention_forward(out, qkv, B: int, T: int, C: int, NH: int) -> None:
