@@ -52,10 +52,11 @@ int current_device(const char *what) {
   return dev;
 }
 
-// Attention's region: parts of a split key axis, two floats per row and head
-// (row sums, lse), and out.
-size_t attention_scratch(size_t rows, size_t C, size_t NH, size_t parts) {
-  return align_up(parts) + 2 * align_up(rows * NH * sizeof(float)) + align_up(rows * C * sizeof(float));
+// Attention's region, in the dense callback's backward: the forward's parts of a
+// split key axis or the backward's own memory, then lse and out.
+size_t attention_scratch(size_t rows, size_t C, size_t NH, size_t parts, size_t backward) {
+  return align_up(parts > backward ? parts : backward) + align_up(rows * NH * sizeof(float)) +
+         align_up(rows * C * sizeof(float));
 }
 
 // Region sizes for every entry point at shapes up to cfg: the step driver's
@@ -69,7 +70,8 @@ void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
   out[kRegEncoder] = encoder_backward_scratch();
   out[kRegKl] = kl_forward_scratch();
   out[kRegSoftmax] = softmax_scratch(rows, cfg.V);
-  out[kRegAttention] = attention_scratch(rows, cfg.C, cfg.NH > 0 ? cfg.NH : 0, attention_parts_bound());
+  const size_t NH = cfg.NH > 0 ? cfg.NH : 0;
+  out[kRegAttention] = attention_scratch(rows, cfg.C, NH, attention_parts_bound(), attention_backward_bound(rows, cfg.C, NH));
 }
 
 // Grow the library-owned region r of device dev to `bytes` (lock held).
@@ -350,9 +352,12 @@ int check_attention(const char *fn, ugk_attention *a, bool *none) {
     return bad(fn, "rows * stride exceeds the address space");
   if ((long long)a->max_q * (a->NH / a->NKV) > INT_MAX / 2 || a->max_k > INT_MAX / 2)
     return bad(fn, "max_q * NH / NKV or max_k exceeds 2^30");
-  // a workgroup takes a few rows of q, or of k, at a time, for each sequence and key/value head
-  const long long blocks = ((long long)a->max_q * (a->NH / a->NKV) + a->max_k) / 4 + 1;
-  if ((long long)a->nseq * a->NKV > INT_MAX / 4 / blocks) return bad(fn, "nseq * heads * rows exceeds the grid");
+  // a workgroup of 256 threads takes up to 128 rows of q, or of k, of a sequence and key/value head, and a launch
+  // has fewer than 2^32 threads
+  const long long tq = ((long long)a->max_q * (a->NH / a->NKV) + 127) / 128, tk = ((long long)a->max_k + 127) / 128;
+  const long long blocks = tq > tk ? tq : tk;
+  if ((long long)a->nseq * a->NKV >= ((long long)1 << 24) / (blocks > 0 ? blocks : 1))
+    return bad(fn, "nseq * heads * rows exceeds the grid");
   *none = a->nseq == 0 || a->max_q == 0 || a->rows_q == 0;
   return UGK_OK;
 }
@@ -387,11 +392,11 @@ int attention_backward(const char *fn, float *dq, float *dk, float *dv, const fl
   for (const float *g : {dq, dk, dv})
     for (const float *x : {dout, q, k, v, out, lse})
       if (g && g == x) return bad(fn, "the gradients must be distinct from the inputs");
-  float *dsum = static_cast<float *>(workspace(kRegAttention, (size_t)a.rows_q * a.NH * sizeof(float) + kAlign));
-  if (!dsum) return UGK_ENOMEM;
+  float *mem = static_cast<float *>(workspace(kRegAttention, attention_backward_bytes(a) + kAlign));
+  if (!mem) return UGK_ENOMEM;
   int *word = ids_error_word();
   if (!word) return UGK_EHIP;
-  if (int e = launch_attention_backward(dq, dk, dv, dout, q, k, v, out, lse, dsum, a, assign, word)) return e;
+  if (int e = launch_attention_backward(dq, dk, dv, dout, q, k, v, out, lse, mem, a, assign, word)) return e;
   return ok();
 }
 
@@ -792,17 +797,16 @@ int ugk_dense_attention_backward(void *, float *dqkv, const float *dout, const f
   if (rows == 0) return ok();
   if (any_null({dqkv, dout, qkv})) return bad(fn, "NULL pointer");
   if (dqkv == qkv || dqkv == dout) return bad(fn, "dqkv must be distinct from qkv and dout");
-  const size_t parts = align_up(attention_parts_bytes(a)), stat = align_up(rows * NH * sizeof(float));
-  char *w = static_cast<char *>(workspace(kRegAttention, attention_scratch(rows, C, NH, parts)));
+  const size_t parts = attention_parts_bytes(a), backward = attention_backward_bytes(a);
+  char *w = static_cast<char *>(workspace(kRegAttention, attention_scratch(rows, C, NH, parts, backward)));
   if (!w) return UGK_ENOMEM;
   int *word = ids_error_word();
   if (!word) return UGK_EHIP;
-  float *dsum = reinterpret_cast<float *>(w + parts), *lse = reinterpret_cast<float *>(w + parts + stat);
-  float *out = reinterpret_cast<float *>(w + parts + 2 * stat);
+  float *mem = reinterpret_cast<float *>(w), *lse = reinterpret_cast<float *>(w + align_up(parts > backward ? parts : backward));
+  float *out = lse + align_up(rows * NH * sizeof(float)) / sizeof(float);
   const float *k = qkv + C, *v = qkv + 2 * (size_t)C;
-  if (int e = launch_attention_forward(out, lse, qkv, k, v, reinterpret_cast<float *>(w), a, word)) return e;
-  if (int e = launch_attention_backward(dqkv, dqkv + C, dqkv + 2 * (size_t)C, dout, qkv, k, v, out, lse, dsum, a, false,
-                                        word))
+  if (int e = launch_attention_forward(out, lse, qkv, k, v, mem, a, word)) return e;
+  if (int e = launch_attention_backward(dqkv, dqkv + C, dqkv + 2 * (size_t)C, dout, qkv, k, v, out, lse, mem, a, false, word))
     return e;
   return ok();
 }

@@ -355,15 +355,19 @@ int launch_dropout_residual_layernorm_forward(float *res, float *out, float *mea
 constexpr int kMaxHead = 128;  // floats per head of the attention
 // Attention. `a` is checked and its strides are filled in; word: the id error
 // word. The forward's parts of a split key axis go to `parts`
-// (attention_parts_bytes(a); 0: not split), the backward's rows_q * NH row sums to
-// `dsum`. assign: dq, dk and dv are written, not added to.
+// (attention_parts_bytes(a); 0: not split), the backward's rows_q * NH row sums
+// and parts of the rows' range to `mem` (attention_backward_bytes(a)). assign: dq,
+// dk and dv are written, not added to.
 int launch_attention_forward(float *out, float *lse, const float *q, const float *k, const float *v, float *parts,
                              const ugk_attention &a, int *word);
 int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout, const float *q, const float *k,
-                              const float *v, const float *out, const float *lse, float *dsum, const ugk_attention &a,
+                              const float *v, const float *out, const float *lse, float *mem, const ugk_attention &a,
                               bool assign, int *word);
 size_t attention_parts_bytes(const ugk_attention &a);
-size_t attention_parts_bound();  // over all calls
+size_t attention_backward_bytes(const ugk_attention &a);
+// over all calls, and over calls of one key/value head per query head with up to rows x C values
+size_t attention_parts_bound();
+size_t attention_backward_bound(size_t rows, size_t C, size_t NH);
 
 // Workspace sizes.
 size_t layernorm_backward_scratch(int rows, int C);  // bytes of one call's partial rows
