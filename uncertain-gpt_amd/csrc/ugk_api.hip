@@ -760,8 +760,9 @@ int ugk_layernorm_dropout_residual_backward(float *dinp, float *dweight, float *
   if ((long long)B * T * C == 0) return ok();
   if (any_null({dinp, dweight, dbias, dx, dy, dout, inp, weight, mean, rstd})) return bad(fn, "NULL pointer");
   if (dinp == dx || dinp == dy) return bad(fn, "dinp must be distinct from dx and dy");
-  if (int e = launch_layernorm_backward(dinp, dweight, dbias, dout, inp, weight, mean, rstd, B * T, C)) return e;
-  if (int e = launch_dropout(kDropSplit, dx, dy, dinp, nullptr, (size_t)B * T * C, d)) return e;
+  if (int e = launch_layernorm_dropout_residual_backward(dinp, dweight, dbias, dx, dy, dout, inp, weight, mean, rstd, B * T,
+                                                         C, d))
+    return e;
   return ok();
 }
 

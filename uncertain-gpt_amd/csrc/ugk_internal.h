@@ -352,6 +352,10 @@ int launch_dropout(DropForm form, float *a, float *b, const float *x, const floa
 int launch_dropout_residual_layernorm_forward(float *res, float *out, float *mean, float *rstd, const float *x,
                                               const float *y, const float *weight, const float *bias, int rows, int C,
                                               const UgkDrop &drop);
+int launch_layernorm_dropout_residual_backward(float *dinp, float *dweight, float *dbias, float *dx, float *dy,
+                                               const float *dout, const float *inp, const float *weight,
+                                               const float *mean, const float *rstd, int rows, int C,
+                                               const UgkDrop &drop);
 constexpr int kMaxHead = 128;  // floats per head of the attention
 // Attention. `a` is checked and its strides are filled in; word: the id error
 // word. The forward's parts of a split key axis go to `parts`

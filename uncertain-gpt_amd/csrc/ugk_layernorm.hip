@@ -43,6 +43,8 @@ constexpr int kWavesPerBlock = kBlock / kWave;
 constexpr int kMaxV = 8;  // float4 per lane held in registers: C <= 2048
 // What a forward kernel normalises: inp, inp + inp2, or inp + dropout(inp2).
 enum FwdIn { kPlain = 0, kSum = 1, kDropSum = 2 };
+// What a backward kernel does with its new dinp beyond it: nothing, residual_backward, dropout_residual_backward.
+enum BwdOut { kAlone = 0, kSplit = 1, kSplitDrop = 2 };
 constexpr int kMaxWide = 8192;  // channels of the workgroup-per-row kernels
 
 __device__ __forceinline__ float4 add4(float4 a, float4 b) {
@@ -515,12 +517,13 @@ __device__ __forceinline__ void ln_bwd_tail(float *partial, int nblk, int C, flo
 // an ordinary dinp store made it faster alone (35.7 against 37.2 us cold at
 // 8,192 x 768) but the step slower (3.02 against 2.93 ms), the dirty lines
 // of its 24 launches being written back during the kernels that follow.
-template <int V, int W, int R, bool kRes, int MINW, bool kNt, int kDinp, bool kAssign, bool kTail, bool kRag>
+// kRes = kSplitDrop: rdy takes dropout(dinp), element i of the whole array.
+template <int V, int W, int R, int kRes, int MINW, bool kNt, int kDinp, bool kAssign, bool kTail, bool kRag>
 __global__ __launch_bounds__(W * kWave, MINW) void k_ln_bwd_vec(
     float *__restrict__ dinp, float *__restrict__ partial, const float *__restrict__ dout,
     const float *__restrict__ inp, const float *__restrict__ weight, const float *__restrict__ mean,
     const float *__restrict__ rstd, int rows, int C, int rpw, float *__restrict__ rdx,
-    float *__restrict__ rdy, int same, float *dweight, float *dbias) {
+    float *__restrict__ rdy, int same, float *dweight, float *dbias, UgkDrop drop) {
   static_assert(!kRag || (kNt && !kTail), "ragged rows take the non-temporal stores and the second launch");
   __shared__ float4 red[W][2][V * kWave];
   const int lane = threadIdx.x & (kWave - 1);
@@ -631,11 +634,12 @@ __global__ __launch_bounds__(W * kWave, MINW) void k_ln_bwd_vec(
               st4(dinp + off[q] + cl.at[v], o);
           }
           if (kRes) {
-            float4 a = add4(ra[kRes ? q : 0][kRes ? v : 0], o);
+            float4 a = add4(ra[kRes ? q : 0][kRes ? v : 0], o), b = o;
+            if (kRes == kSplitDrop) b = ugk_drop4(o, (off[q] + cl.at[v]) >> 2, drop);
             if (same) {
-              a = add4(a, o);
+              a = add4(a, b);
             } else {
-              cl.put(rdy + off[q], v, add4(rb[kRes ? q : 0][kRes ? v : 0], o));
+              cl.put(rdy + off[q], v, add4(rb[kRes ? q : 0][kRes ? v : 0], b));
             }
             cl.put(rdx + off[q], v, a);
           }
@@ -693,12 +697,12 @@ __global__ __launch_bounds__(W * kWave, MINW) void k_ln_bwd_vec(
 // two-rows-per-wavefront kernel at 8,192 x 768, cold, with the same 512
 // partial rows. rpt and T fix the order of every addition; R does not, so the
 // plain backward (R = 2) and the fused pair (R = 4) give the same bits.
-template <int P, int T, int R, bool kRes, int MINW, bool kNt, int kDinp, bool kAssign, bool kTail>
+template <int P, int T, int R, int kRes, int MINW, bool kNt, int kDinp, bool kAssign, bool kTail>
 __global__ __launch_bounds__(P * T * kWave, MINW) void k_ln_bwd_team(
     float *__restrict__ dinp, float *__restrict__ partial, const float *__restrict__ dout,
     const float *__restrict__ inp, const float *__restrict__ weight, const float *__restrict__ mean,
     const float *__restrict__ rstd, int rows, int C, int rpt, float *__restrict__ rdx,
-    float *__restrict__ rdy, int same, float *dweight, float *dbias) {
+    float *__restrict__ rdy, int same, float *dweight, float *dbias, UgkDrop drop) {
   __shared__ float parts[2][T][R][P][2];  // a row's two sums by part, double-buffered by pass
   __shared__ float4 red[T][2][P * kWave];
   const int lane = threadIdx.x & (kWave - 1);
@@ -789,11 +793,12 @@ __global__ __launch_bounds__(P * T * kWave, MINW) void k_ln_bwd_team(
             st4(dinp + off[q], o);
         }
         if (kRes) {
-          float4 a = add4(ra[kRes ? q : 0], o);
+          float4 a = add4(ra[kRes ? q : 0], o), b = o;
+          if (kRes == kSplitDrop) b = ugk_drop4(o, off[q] >> 2, drop);
           if (same) {
-            a = add4(a, o);
+            a = add4(a, b);
           } else {
-            st_nt4(rdy + off[q], add4(rb[kRes ? q : 0], o));
+            st_nt4(rdy + off[q], add4(rb[kRes ? q : 0], b));
           }
           st_nt4(rdx + off[q], a);
         }
@@ -1984,13 +1989,13 @@ namespace {
 // tail: the workgroups finish the column sums into dweight/dbias themselves
 // (ln_bwd_tail); only for the per-op modes (dinp read and written, residual
 // targets read).
-template <bool kRes, int kDinp, bool kAssign>
+template <int kRes, int kDinp, bool kAssign>
 int launch_ln_bwd_vec(float *dinp, float *partial, const float *dout, const float *inp,
                       const float *weight, const float *mean, const float *rstd, int rows, int C,
                       float *rdx, float *rdy, int max_blocks, bool tail = false, float *dweight = nullptr,
-                      float *dbias = nullptr) {
-  static_assert(kRes || (kDinp == kDinpRw && !kAssign), "the plain backward reads and writes dinp");
-  constexpr bool kTailOk = kDinp == kDinpRw && !kAssign;
+                      float *dbias = nullptr, const UgkDrop &drop = UgkDrop{}) {
+  constexpr bool kPerOp = kDinp == kDinpRw && !kAssign, kTailOk = kPerOp && kRes != kSplitDrop;
+  static_assert(kPerOp || kRes == kSplit, "the plain backward and the pair with dropout read and write everything");
   int nblk, rpw;
   const int V = slots_of(C, kWave);
   const int same = rdx == rdy ? 1 : 0;
@@ -1999,45 +2004,45 @@ int launch_ln_bwd_vec(float *dinp, float *partial, const float *dout, const floa
   const auto both = [&](auto k_plain, auto k_tail, dim3 grid, dim3 block, int rp) {
     if (kTailOk && tail)
       launch(k_tail, grid, block, 0, dinp, partial, dout, inp, weight, mean, rstd, rows, C, rp, rdx, rdy, same,
-             dweight, dbias);
+             dweight, dbias, drop);
     else
       launch(k_plain, grid, block, 0, dinp, partial, dout, inp, weight, mean, rstd, rows, C, rp, rdx, rdy, same,
-             nullptr, nullptr);
+             nullptr, nullptr, drop);
   };
   if (team_path(rows, C)) {
     int rpt;
     team_shape(rows, max_blocks, &nblk, &rpt);
     const dim3 grid(nblk), block(kTeamParts * kTeams * kWave);
     if constexpr (kRes)
-      both(k_ln_bwd_team<kTeamParts, kTeams, 4, true, 3, true, kDinp, kAssign, false>,
-           k_ln_bwd_team<kTeamParts, kTeams, 4, true, 3, true, kDinp, kAssign, kTailOk>, grid, block, rpt);
+      both(k_ln_bwd_team<kTeamParts, kTeams, 4, kRes, 3, true, kDinp, kAssign, false>,
+           k_ln_bwd_team<kTeamParts, kTeams, 4, kRes, 3, true, kDinp, kAssign, kTailOk>, grid, block, rpt);
     else if (nt)
-      both(k_ln_bwd_team<kTeamParts, kTeams, 2, false, 1, true, kDinpRw, false, false>,
-           k_ln_bwd_team<kTeamParts, kTeams, 2, false, 1, true, kDinpRw, false, true>, grid, block, rpt);
+      both(k_ln_bwd_team<kTeamParts, kTeams, 2, kAlone, 1, true, kDinpRw, false, false>,
+           k_ln_bwd_team<kTeamParts, kTeams, 2, kAlone, 1, true, kDinpRw, false, true>, grid, block, rpt);
     else
-      both(k_ln_bwd_team<kTeamParts, kTeams, 2, false, 1, false, kDinpRw, false, false>,
-           k_ln_bwd_team<kTeamParts, kTeams, 2, false, 1, false, kDinpRw, false, true>, grid, block, rpt);
+      both(k_ln_bwd_team<kTeamParts, kTeams, 2, kAlone, 1, false, kDinpRw, false, false>,
+           k_ln_bwd_team<kTeamParts, kTeams, 2, kAlone, 1, false, kDinpRw, false, true>, grid, block, rpt);
     return nblk;
   }
-  const BwdCfg k = bwd_cfg(V, kRes);
+  const BwdCfg k = bwd_cfg(V, kRes != kAlone);
   bwd_shape_vec(rows, k, max_blocks, &nblk, &rpw);
   const dim3 grid(nblk), block(k.W * kWave);
   const bool rag = (C & 3) != 0;  // takes only the modes of the per-op calls (kTailOk)
   switch (V) {
 #define UGK_LN_BWD_K(v, ntv, tl)                                                                                    \
-  k_ln_bwd_vec<v, bwd_cfg(v, kRes).W, bwd_cfg(v, kRes).R, kRes, bwd_cfg(v, kRes).MINW, ntv, kDinp, kAssign, tl, false>
+  k_ln_bwd_vec<v, bwd_cfg(v, kRes != kAlone).W, bwd_cfg(v, kRes != kAlone).R, kRes, bwd_cfg(v, kRes != kAlone).MINW, ntv, kDinp, kAssign, tl, false>
 #define UGK_LN_BWD(v)                                                                                               \
   case v:                                                                                                           \
     if (rag) {                                                                                                      \
       if constexpr (kTailOk)                                                                                        \
-        launch(k_ln_bwd_vec<v, bwd_cfg(v, kRes).W, bwd_cfg(v, kRes).R, kRes, bwd_cfg(v, kRes).MINW, true, kDinpRw,   \
+        launch(k_ln_bwd_vec<v, bwd_cfg(v, kRes != kAlone).W, bwd_cfg(v, kRes != kAlone).R, kRes, bwd_cfg(v, kRes != kAlone).MINW, true, kDinpRw,   \
                             false, false, true>,                                                                    \
                grid, block, 0, dinp, partial, dout, inp, weight, mean, rstd, rows, C, rpw, rdx, rdy, same, nullptr, \
-               nullptr);                                                                                            \
+               nullptr, drop);                                                                                      \
     } else if (kRes || nt)                                                                                          \
       both(UGK_LN_BWD_K(v, true, false), UGK_LN_BWD_K(v, true, kTailOk), grid, block, rpw);                         \
     else                                                                                                            \
-      both(UGK_LN_BWD_K(v, kRes, false), UGK_LN_BWD_K(v, kRes, kTailOk), grid, block, rpw);                         \
+      both(UGK_LN_BWD_K(v, kRes != kAlone, false), UGK_LN_BWD_K(v, kRes != kAlone, kTailOk), grid, block, rpw);                         \
     break;
     UGK_LN_BWD(1) UGK_LN_BWD(2) UGK_LN_BWD(3) UGK_LN_BWD(4)
     UGK_LN_BWD(5) UGK_LN_BWD(6) UGK_LN_BWD(7) UGK_LN_BWD(8)
@@ -2125,9 +2130,9 @@ int launch_layernorm_backward_partials(float *dinp, float *partial, LnCols cols,
     const int mode = (C & 3) != 0 ? kDinpRw : dinp_mode;
     const bool assign = (C & 3) == 0 && assign_res;
 #define UGK_LN_BWD_MODE(d, a) \
-  launch_ln_bwd_vec<true, d, a>(dinp, partial, dout, inp, weight, mean, rstd, rows, C, dx, dy, max_blocks)
+  launch_ln_bwd_vec<kSplit, d, a>(dinp, partial, dout, inp, weight, mean, rstd, rows, C, dx, dy, max_blocks)
     if (!res)
-      *nblk = launch_ln_bwd_vec<false, kDinpRw, false>(dinp, partial, dout, inp, weight, mean, rstd, rows, C,
+      *nblk = launch_ln_bwd_vec<kAlone, kDinpRw, false>(dinp, partial, dout, inp, weight, mean, rstd, rows, C,
                                                        nullptr, nullptr, max_blocks);
     else if (mode == kDinpRw)
       *nblk = UGK_LN_BWD_MODE(kDinpRw, false);
@@ -2188,10 +2193,10 @@ int launch_layernorm_residual_backward_into(float *partial, int max_blocks, floa
   }
   if (layernorm_tail() && row_in_wave(C) && (C & 3) == 0 && !small_path(rows, C, dout, inp)) {
     if (res)
-      launch_ln_bwd_vec<true, kDinpRw, false>(dinp, partial, dout, inp, weight, mean, rstd, rows, C, dx, dy,
+      launch_ln_bwd_vec<kSplit, kDinpRw, false>(dinp, partial, dout, inp, weight, mean, rstd, rows, C, dx, dy,
                                               max_blocks, true, dweight, dbias);
     else
-      launch_ln_bwd_vec<false, kDinpRw, false>(dinp, partial, dout, inp, weight, mean, rstd, rows, C, nullptr,
+      launch_ln_bwd_vec<kAlone, kDinpRw, false>(dinp, partial, dout, inp, weight, mean, rstd, rows, C, nullptr,
                                                nullptr, max_blocks, true, dweight, dbias);
     return check_launch("layernorm_backward");
   }
@@ -2214,6 +2219,30 @@ int launch_layernorm_residual_backward(float *dinp, float *dweight, float *dbias
   // more workgroups than the cap it is given
   return launch_layernorm_residual_backward_into(partial, layernorm_backward_blocks_bound(rows, C), dinp, dweight,
                                                  dbias, dx, dy, dout, inp, weight, mean, rstd, rows, C);
+}
+
+// One pass where the rows take a wavefront or a team of them each (8,192 x 768 41.3 us
+// against 43.7 for the two ops, whose second reads dinp again, 4,096 x 1,600 48.3
+// against 54.9, 2,048 x 768 19.7 against 19.1), the two ops elsewhere: also for widths that
+// are no multiple of 4, whose slots lie in two Philox blocks each (three sequences of
+// 1,023 x 1,602 43.1 in one pass, 42.6 in two).
+int launch_layernorm_dropout_residual_backward(float *dinp, float *dweight, float *dbias, float *dx, float *dy,
+                                               const float *dout, const float *inp, const float *weight,
+                                               const float *mean, const float *rstd, int rows, int C,
+                                               const UgkDrop &drop) {
+  if (rows == 0) return 0;
+  if (layernorm_exact() || layernorm_tail() || !row_in_wave(C) || (C & 3) != 0 || small_path(rows, C, dout, inp)) {
+    if (int e = launch_layernorm_backward(dinp, dweight, dbias, dout, inp, weight, mean, rstd, rows, C)) return e;
+    return launch_dropout(kDropSplit, dx, dy, dinp, nullptr, (size_t)rows * C, drop);
+  }
+  float *partial = static_cast<float *>(workspace(kRegLn, layernorm_backward_scratch(rows, C)));
+  if (!partial) return UGK_ENOMEM;
+  const int nblk = launch_ln_bwd_vec<kSplitDrop, kDinpRw, false>(dinp, partial, dout, inp, weight, mean, rstd, rows, C, dx, dy,
+                                                                 layernorm_backward_blocks_bound(rows, C), false, nullptr,
+                                                                 nullptr, drop);
+  if (int e = check_launch("layernorm_dropout_residual_backward")) return e;
+  const LnReduceJob job{partial, dweight, dbias, nblk, dout, inp, mean, rstd};
+  return launch_layernorm_reduce(&job, 1, rows, C);
 }
 
 // ---- allocation-free variant ------------------------------------------------
