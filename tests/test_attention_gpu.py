@@ -409,3 +409,107 @@ def test_caller_owned_workspace(gpu):
 def attention_rows_beyond(gpu, cfg, n):
     """Rows whose 64 row sums each exceed any region of a workspace of n bytes."""
     return n // 256 + 1
+
+
+def own_size_bounds(s, q, k, v, out, lse, dout, scale):
+    """Bounds for one causal sequence from the sizes of what a row sees alone. An element is held to 2^-24 of itself
+    and 2^-27 of the largest of its own row (a tile that not all rows see holds no row more than 2^13 below its
+    largest) or 2^-40 of the largest that the row sees; the weights and dS to 2^-33 of the largest that it has seen."""
+    n, HS = q.shape[0], q.shape[2]
+    Q, K, V, O, G = (t[:, 0].double() for t in (q, k, v, out, dout))
+    ok = att_ref.allowed(n, n, True, DEV)
+    top = lambda t: t.abs().amax(1)  # noqa: E731
+    es = abs(scale) * (HS + 8) * 2.0 ** -23 * HS * top(Q)[:, None] * top(K)[None]
+    S = (Q @ K.T * scale).masked_fill(~ok, -math.inf)
+    P = torch.exp(S - lse.double())
+    rel = torch.where(ok, 2 * es + (S - lse.double()).abs().clamp(0, 90) * 2.0 ** -24, 0.0).amax(1, keepdim=True) * 2 + (2 * n + 32) * 2.0 ** -24
+    floor = n * 2.0 ** -33
+    seen_v = torch.cummax(top(V), 0).values
+    t_out = (P * rel) @ top(V)[:, None] + floor * seen_v[:, None]
+    D = (G.abs() * O.abs()).sum(1)
+    size = torch.where(ok, P * abs(scale) * (HS * top(G)[:, None] * top(V)[None] + D[:, None]), 0.0)
+    more = rel + (2 * HS + 32) * 2.0 ** -24
+    seen_k = torch.cummax(top(K), 0).values
+    worst = size.amax(1)
+    t_q = (size * more) @ top(K)[:, None] + floor * (worst * seen_k)[:, None]
+    back = lambda t: torch.cummax(t.flip(0), 0).values.flip(0)  # noqa: E731
+    t_k = (size * more).T @ top(Q)[:, None] + floor * (size.amax(0) * back(top(Q)))[:, None]
+    t_v = (P * more).T @ top(G)[:, None] + floor * back(top(G))[:, None]
+    return t_out, (t_q, t_k, t_v)
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("n", [65, 129, 300])
+def test_sizes_that_change_along_the_sequence(gpu, n, seed):
+    """Values and gradients whose size jumps by up to 2^40 from one block of rows to the next, or in the last row
+    alone: what a row does not see costs it no digits."""
+    c = Call(gpu, Seqs([n]), 1, 1, 64, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    step = (32, 64, n - 1, 7)[seed]
+    e = torch.randint(-20, 21, (n // step + 1,), generator=g).repeat_interleave(step)[:n].to(DEV)
+    e2 = torch.randint(-20, 21, (n // step + 1,), generator=g).repeat_interleave(step)[:n].to(DEV)
+    if seed == 2:
+        e[:], e2[:] = 0, 0
+        e[-1], e2[0] = 100, 60
+    c.v.copy_(torch.ldexp(c.v, e[:, None, None]))
+    c.dout.copy_(torch.ldexp(c.dout, e2[:, None, None]))
+    out, lse = c.forward()
+    w, wl, _, tol_l = att_ref.forward(c.s, c.q, c.k, c.v, c.scale, True)
+    t_out, tols = own_size_bounds(c.s, c.q, c.k, c.v, w.float(), wl.float(), c.dout, c.scale)
+    inside(out[:, 0], w[:, 0], t_out.expand(-1, 64), "out")
+    inside(lse, wl, tol_l, "lse")
+    gr = c.grads()
+    c.backward(out, lse, gr, zeroed=True)
+    want, _ = att_ref.backward(c.s, c.q, c.k, c.v, out, lse, c.dout, c.scale, True)
+    for name, x, y, t in zip(("dq", "dk", "dv"), gr, want, tols):
+        inside(x[:, 0], y[:, 0], t.expand(-1, 64), name)
+
+
+@pytest.mark.parametrize("n", [65, 130])
+def test_keys_whose_size_changes_along_the_sequence(gpu, n):
+    """Keys and queries whose size jumps, the scores staying of order one to a thousand."""
+    c = Call(gpu, Seqs([n]), 1, 1, 64)
+    e = (torch.arange(n, device=DEV) // 32 % 2) * 10
+    c.k.copy_(torch.ldexp(c.k, -e[:, None, None]))
+    c.q.copy_(torch.ldexp(c.q, (3 - e)[:, None, None]))
+    c.k[-1] *= 2.0 ** 20
+    c.q[0] *= 2.0 ** 15
+    out, lse = c.forward()
+    w, wl, _, _ = att_ref.forward(c.s, c.q, c.k, c.v, c.scale, True)
+    t_out, tols = own_size_bounds(c.s, c.q, c.k, c.v, w.float(), wl.float(), c.dout, c.scale)
+    inside(out[:, 0], w[:, 0], t_out.expand(-1, 64), "out")
+    gr = c.grads()
+    c.backward(out, lse, gr, zeroed=True)
+    want, _ = att_ref.backward(c.s, c.q, c.k, c.v, out, lse, c.dout, c.scale, True)
+    for name, x, y, t in zip(("dq", "dk", "dv"), gr, want, tols):
+        inside(x[:, 0], y[:, 0], t.expand(-1, 64), name)
+
+
+@pytest.mark.parametrize("lens,lk", [([70], None), ([2], [300]), ([1], [4000]), ([40], [1000])])
+def test_scores_of_minus_infinity(gpu, lens, lk):
+    """Keys whose scores are -infinity weigh nothing; a row that sees no others has out 0, lse -infinity, gradients 0.
+    The same in every kernel and in every part of a split key axis."""
+    c = Call(gpu, Seqs(lens, lk), 2, 1, 64)
+    c.q[:, :, 0] = c.q[:, :, 0].abs() + 0.1
+    nk = c.s.lk[0]
+    gone = slice(nk // 4, nk)
+    c.k[gone, :, 0] = -math.inf
+    out, lse = c.forward()
+    # the rows as if the sequence ended before those keys
+    q, k, v = c.q.double(), c.k[:nk // 4].double(), c.v[:nk // 4].double()
+    for h in range(2):
+        z = q[:, h] @ k[:, 0].T * c.scale
+        if lk is None:
+            z = z.masked_fill(~att_ref.allowed(lens[0], nk, True, DEV)[:, :nk // 4], -math.inf)
+        p = torch.softmax(z, 1)
+        assert torch.allclose(out[:, h].double(), p @ v[:, 0], rtol=1e-4, atol=1e-5)
+        assert torch.allclose(lse[:, h].double(), torch.logsumexp(z, 1), rtol=1e-5, atol=1e-5)
+    g = c.grads()
+    c.backward(out, lse, g)
+    assert g[2][gone].eq(0).all()
+    c.k[:, :, 0] = -math.inf
+    out, lse = c.forward()
+    assert out.eq(0).all() and (lse == -math.inf).all()
+    g = c.grads()
+    c.backward(out, lse, g)
+    assert g[2].eq(0).all()

@@ -68,6 +68,9 @@ __device__ __forceinline__ float dot(const float *x, const float *y, int n) {
 
 __device__ __forceinline__ void put(float *p, float x, bool assign) { *p = assign ? x : *p + x; }
 
+// exp(s - m); a score of -infinity weighs nothing, whatever m is.
+__device__ __forceinline__ float weight(float s, float m) { return s == -INFINITY ? 0.0f : expf(s - m); }
+
 // One query row of one head by one wavefront: lanes over keys for the scores,
 // over channels for the sum.
 __device__ void row_forward(float *out, float *lse, const float *q, const float *k, const float *v, int n, int HS,
@@ -80,7 +83,7 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
   const int d0 = min(lane, HS - 1), d1 = min(lane + kWave, HS - 1);
   for (int j0 = 0; j0 < n; j0 += kWave) {
     const int j = j0 + lane;
-    const float p = j < n ? expf(dot(q, k + j * ldk, HS) * scale - m) : 0.0f;
+    const float p = j < n ? weight(dot(q, k + j * ldk, HS) * scale, m) : 0.0f;
     l += wave_sum(p);
     for (int t = 0; t < min(kWave, n - j0); t++) {
       const float pt = __shfl(p, t);
@@ -88,10 +91,11 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
       o1 = fmaf(pt, v[(j0 + t) * ldv + d1], o1);
     }
   }
-  const float r = n ? l : 1.0f;
-  if (lane < HS) out[lane] = o0 / r;
-  if (lane + kWave < HS) out[lane + kWave] = o1 / r;
-  if (lse && lane == 0) *lse = n ? m + logf(l) : -INFINITY;
+  const bool none = l == 0.0f;  // no key, or every score -infinity
+  const float r = none ? 1.0f : l;
+  if (lane < HS) out[lane] = none ? 0.0f : o0 / r;
+  if (lane + kWave < HS) out[lane + kWave] = none ? 0.0f : o1 / r;
+  if (lse && lane == 0) *lse = none ? -INFINITY : m + logf(l);
 }
 
 // ---- forward, tiles on the matrix units -----------------------------------------
@@ -248,6 +252,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   const int least = s.seen(row0 / G, a.causal);  // what every row of the workgroup sees
 
   // this lane's rows
+  bool bad = false;
   const int r0 = row0 + wave * (32 * QB) + (lane & 31);
   int lim[QB], lo = n, hi = first;  // what they see; least and most over the wavefront
   v8h qh[QB][DC], ql[QB][DC];
@@ -269,7 +274,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 #pragma unroll
       for (int j = 0; j < 8; j++) m = max(m, abs_bits(x[c][j]));
     }
-    const int e = split_exp(half_max_bits(m));
+    m = half_max_bits(m);
+    bad = bad || m >= kInfBits;
+    const int e = split_exp(m);
     const float f = a.scale < 0.0f ? -split_scale(e) : split_scale(e);
 #pragma unroll
     for (int c = 0; c < DC; c++) split8(x[c], f, qh[u][c], ql[u][c]);
@@ -317,13 +324,12 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
       for (int x = 0; x < 4; x++) slot[at][x][wave] = m[x];
     }
   };
-  bool bad = false;
-  int ek_next = 0, ev_next = -100;
+  int ek_next = 0, ev_next = 0;  // of the tile staged last
   const auto stage = [&](int at) {
     const uint32_t mk = noted<W>(slot[at][0]), mv = noted<W>(slot[at][1]);
     bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted<W>(slot[at][2])) || too_wide(mv, noted<W>(slot[at][3]));
     ek_next = split_exp(mk);
-    ev_next = max(ev_next, split_exp(mv));
+    ev_next = split_exp(mv);
     const float fk = split_scale(ek_next), fv = split_scale(ev_next);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -334,27 +340,38 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 
   v16f o[QB][DB] = {};
   float l[QB] = {}, bias[QB];  // bias: kTop - the maximum that the row's P stand on
-  int ev = -100;
+  int ev[QB];  // the exponent that o stands on: the largest of the tiles that the row has seen
 #pragma unroll
-  for (int u = 0; u < QB; u++) bias[u] = INFINITY;
+  for (int u = 0; u < QB; u++) {
+    bias[u] = INFINITY;
+    ev[u] = -100;
+  }
   const int vcols = cols_at(lane, kRs);
   const auto compute = [&](int at, int k0, int ek, int ev_now) {
     const float uk = split_unscale(ek);
-    float c2[QB];
+    float c2[QB], up[QB], down[QB];  // P is taken times 2^up, up <= 0, where the row has seen larger values
+    int was[QB];
+    bool changed = false;
 #pragma unroll
     for (int u = 0; u < QB; u++) {
       c2[u] = fmaxf(cq[u] * uk, 0x1p-126f);
       bad = bad || c2[u] > 0x1p100f;
+      was[u] = ev[u];
+      if (lim[u] > k0) ev[u] = max(ev[u], ev_now);
+      changed = changed || ev[u] != was[u];
+      const int shift = max(min(ev_now - ev[u], 0), -100);
+      up[u] = (float)shift;
+      down[u] = pow2(-shift);
     }
-    if (ev != ev_now) {
-      const float f = pow2(max(ev - ev_now, -126));
+    if (__any(changed)) {
 #pragma unroll
-      for (int u = 0; u < QB; u++)
+      for (int u = 0; u < QB; u++) {
+        const float f = pow2(max(was[u] - ev[u], -126));
 #pragma unroll
         for (int x = 0; x < DB; x++)
 #pragma unroll
           for (int y = 0; y < 16; y++) o[u][x][y] *= f;
-      ev = ev_now;
+      }
     }
 #pragma unroll
     for (int w = 0; w < KB; w++) {  // 32 keys
@@ -389,9 +406,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 #pragma unroll
         for (int u = 0; u < QB; u++) {
           bad = bad || (fabsf(m[u]) >= 0x1p22f && m[u] != -INFINITY);
-          const float was = bias[u];
-          bias[u] = fminf(was, kTop - m[u]);
-          const float f = was == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(bias[u] - was);
+          const float old = bias[u];
+          bias[u] = fminf(old, kTop - m[u]);
+          const float f = old == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(bias[u] - old);
           l[u] *= f;
 #pragma unroll
           for (int x = 0; x < DB; x++)
@@ -401,14 +418,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
       }
 #pragma unroll
       for (int u = 0; u < QB; u++) {
-        const float b0 = bias[u] == INFINITY ? 0.0f : bias[u];  // no key so far: every score is -inf
+        const float b0 = (bias[u] == INFINITY ? 0.0f : bias[u]) + up[u];  // no key so far: every score is -inf
         float sum = 0.0f;
 #pragma unroll
         for (int y = 0; y < 16; y++) {
           sc[u][y] = __builtin_amdgcn_exp2f(fmaf(sc[u][y], c2[u], b0));
           sum += sc[u][y];
         }
-        l[u] += sum;
+        l[u] = fmaf(sum, down[u], l[u]);
       }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
@@ -476,7 +493,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     const float sum = half_sum(l[u]);
     const bool some = lim[u] > first;
     put_row<DB, kFull>(parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS, o[u],
-                       some ? split_unscale(ev) / sum : 0.0f, half, a.HS, true);
+                       some ? split_unscale(ev[u]) / sum : 0.0f, half, a.HS, true);
     if (half == 0 && (parts.o || lse)) {
       const float L = some ? (__builtin_amdgcn_logf(sum) - bias[u]) * kLn2 : -INFINITY;
       if (parts.o) parts.lse[prow] = L;
@@ -626,7 +643,7 @@ __global__ __launch_bounds__(NW * kWave) void k_att_few(float *out, float *lse, 
       t = make_float4(fmaf(y.x, f, t.x), fmaf(y.y, f, t.y), fmaf(y.z, f, t.z), fmaf(y.w, f, t.w));
     }
     const int i = r / G, h = hk * G + r % G;
-    const bool any = min(stop, s.seen(i, a.causal)) > first;
+    const bool any = sum != 0.0f;  // else no key, or every score -infinity
     const float f = any ? 1.0f / sum : 0.0f, L = any ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
     t = any ? make_float4(t.x * f, t.y * f, t.z * f, t.w * f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const size_t prow = ((size_t)part * a.nseq + b) * a.max_q + i, grow = (size_t)s.q0 + i;
@@ -688,7 +705,7 @@ __device__ void row_dq(float *dq, float *dsum, const float *dout, const float *q
   for (int j0 = 0; j0 < n; j0 += kWave) {
     const int j = j0 + lane;
     float ds = 0.0f;
-    if (j < n) ds = expf(dot(q, k + j * ldk, HS) * scale - lse) * (dot(dout, v + j * ldv, HS) - D) * scale;
+    if (j < n) ds = weight(dot(q, k + j * ldk, HS) * scale, lse) * (dot(dout, v + j * ldv, HS) - D) * scale;
     for (int t = 0; t < min(kWave, n - j0); t++) {
       const float x = __shfl(ds, t);
       a0 = fmaf(x, k[(j0 + t) * ldk + d0], a0);
@@ -716,7 +733,7 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
       float p = 0.0f, ds = 0.0f;
       if (i < end) {
         const size_t r = (size_t)s.q0 + i;
-        p = expf(dot(q + r * a.ldq + h * HS, kj, HS) * a.scale - lse[r * a.NH + h]);
+        p = weight(dot(q + r * a.ldq + h * HS, kj, HS) * a.scale, lse[r * a.NH + h]);
         ds = p * (dot(dout + r * a.ldo + h * HS, vj, HS) - dsum[r * a.NH + h]) * a.scale;
       }
       for (int t = 0; t < min(kWave, end - i0); t++) {
@@ -746,12 +763,22 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
 // forward holds them, then dk and dv over the keys, so that nothing is added by
 // two workgroups and the results do not depend on their order (one pass with
 // atomics would save the second S and dP, 4 of 14 HS operations per pair).
-// P = exp(S - lse) needs no running maximum. dS = P (dP - D) is scaled for its
-// halves by a bound: P <= 1 and |dP| <= HS max|dout| max|v|, so |dS| <= HS
-// max|dout| max|v| + |D|, which lies some 2^4 to 2^8 above its largest; a half and its
-// remainder reach 2^39 below the bound. The same tiles as in the forward fall
-// back to single rows.
+// P = exp(S - lse) needs no running maximum. The same tiles as in the forward
+// fall back to single rows.
 
+
+// The same times 2^e f, for any e.
+template <int DB, bool kFull>
+__device__ __forceinline__ void put_scaled(float *p, v16f (&acc)[DB], int e, float f, int half, int HS, bool assign) {
+  const int once = min(max(e, -126), 127), twice = min(max(e - once, -126), 127);
+  if (__any(twice != 0)) {
+#pragma unroll
+    for (int x = 0; x < DB; x++)
+#pragma unroll
+      for (int y = 0; y < 16; y++) acc[x][y] *= pow2(twice);
+  }
+  put_row<DB, kFull>(p, acc, pow2(once) * f, half, HS, assign);
+}
 
 // acc += A^T B for a 32-row block of B held in an accumulator's registers (C, scaled
 // to halves by f): A's 32 rows in LDS, `cols` the lane's place in them (cols_at).
@@ -783,6 +810,31 @@ __device__ __forceinline__ v16f dot_block(const _Float16 *ah, const _Float16 *al
     c = mfma3(frag(ah + at), frag(al + at), bh[x], bl[x], c);
   }
   return c;
+}
+
+// Before a block of dS (16 per lane, the row's or key's other half in lane ^ 32) is
+// accumulated with operands of exponent e: the accumulators stand on 2^ea, at least on the
+// largest of the block's dS times 2^e, so that dS 2^(15 + e - ea) is below 2^15. It moves
+// in steps of 2^2 or more, for it costs a pass over the accumulators. (dS's own
+// largest, not a bound from those of dout and v: P is small where there are many keys, and
+// the halves would lose its digits.) Returns whether the range does not do.
+constexpr int kNoScale = -250;
+template <int DB>
+__device__ __forceinline__ bool raise(int &ea, v16f (&acc)[DB], const v16f &ds, int e) {
+  float m = 0.0f;
+#pragma unroll
+  for (int y = 0; y < 16; y += 2) m = fmaxf(fmaxf(m, fabsf(ds[y])), fabsf(ds[y + 1]));
+  m = half_max(m);
+  const int need = split_exp(__float_as_uint(m)), was = ea;
+  if (m > 0.0f && need + e > ea) ea = need + e + 2;
+  if (__any(ea != was)) {
+    const float f = pow2(max(was - ea, -126));
+#pragma unroll
+    for (int x = 0; x < DB; x++)
+#pragma unroll
+      for (int y = 0; y < 16; y++) acc[x][y] *= f;
+  }
+  return m > 0x1p120f;
 }
 
 // A lane's row (HS floats at p) as operands; *e: its exponent. Returns the bits of its largest magnitude.
@@ -840,9 +892,9 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   const size_t grow = (size_t)s.q0 + i;
   v8h qh[DC], ql[DC], gh[DC], gl[DC];
   int eq, eg;
-  load_operand<DC, kFull>(q + grow * a.ldq + h * a.HS, a.HS, live, half, qh, ql, &eq);
+  const uint32_t qbits = load_operand<DC, kFull>(q + grow * a.ldq + h * a.HS, a.HS, live, half, qh, ql, &eq);
   const float *gr = dout + grow * a.ldo + h * a.HS;
-  const float gmax = __uint_as_float(load_operand<DC, kFull>(gr, a.HS, live, half, gh, gl, &eg));
+  const uint32_t gbits = load_operand<DC, kFull>(gr, a.HS, live, half, gh, gl, &eg);
   float D = 0.0f;
 #pragma unroll
   for (int c = 0; c < DC; c++) {
@@ -856,7 +908,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   if (live && half == 0) dsum[grow * a.NH + h] = D;
   const float L2 = live ? lse[grow * a.NH + h] * kLog2e : 0.0f;
   const float cq = split_unscale(eq) * (a.scale * kLog2e), cg = split_unscale(eg);
-  bool bad = lim > 0 && !(fabsf(L2) < 0x1p22f);  // (the row's own q and dout reach its own results alone)
+  bool bad = lim > 0 && (!(fabsf(L2) < 0x1p22f) || qbits >= kInfBits || gbits >= kInfBits);
 
   Rows4 t[kPer];
   const auto is_v = [&](int u) { return kPer == 1 ? wave >= W / 2 : u >= kPer / 2; };
@@ -895,13 +947,13 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
       for (int x = 0; x < 4; x++) slot[at & 1][x][wave] = m[x];
     }
   };
-  int ek = -100, ev = -100;
+  int ek = 0, ev = 0;  // of the tile staged last
   const auto stage = [&](int at) {
     const int z = at & 1;
     const uint32_t mk = noted<W>(slot[z][0]), mv = noted<W>(slot[z][1]);
     bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted<W>(slot[z][2])) || too_wide(mv, noted<W>(slot[z][3]));
-    ek = max(ek, split_exp(mk));
-    ev = max(ev, split_exp(mv));
+    ek = split_exp(mk);
+    ev = split_exp(mv);
     const float fk = split_scale(ek), fv = split_scale(ev);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -912,25 +964,12 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   };
 
   v16f acc[DB] = {};
-  int ek_acc = -100, es = -100, ev_acc = -101;  // of the accumulators: K's, dS's and what dS's stands on
+  int ea = kNoScale;  // the exponent that the accumulators stand on
   const int cols = cols_at(lane, kRs);
   const auto compute = [&](int at, int ek_now, int ev_now) {
     const int z = at & 1, k0 = at * BK;
-    if (ek_now != ek_acc || ev_now != ev_acc) {
-      const float bound = fmaf((float)a.HS * gmax, pow2(min(max(ev_now, -126), 127)), fabsf(D));
-      const int e = max(es, split_exp(__float_as_uint(bound)));
-      bad = bad || e > 120 || e + ek_now > 130;
-      const float f = pow2(max(ek_acc - ek_now, -126)) * pow2(max(es - e, -126));
-#pragma unroll
-      for (int x = 0; x < DB; x++)
-#pragma unroll
-        for (int y = 0; y < 16; y++) acc[x][y] *= f;
-      ek_acc = ek_now;
-      ev_acc = ev_now;
-      es = min(e, 120);
-    }
-    const float c2 = cq * split_unscale(ek_now), cd = cg * split_unscale(ev_now), f = split_scale(es);
-    bad = bad || fabsf(c2) > 0x1p100f || cd > 0x1p100f;
+    const float c2 = cq * split_unscale(ek_now), cd = cg * split_unscale(ev_now);
+    bad = bad || (lim > k0 && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
 #pragma unroll
     for (int w = 0; w < BK / 32; w++) {  // 32 keys
       const int o = 32 * w * kRs;
@@ -947,7 +986,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
         for (int y = 0; y < 16; y++)
           if (8 * (y / 4) + y % 4 >= rel) p[y] = 0.0f;
       }
-      mac_block<DB>(acc, p, f, lk[z][0] + o, lk[z][1] + o, kRs, cols);
+      bad = raise(ea, acc, p, ek_now) || bad;
+      mac_block<DB>(acc, p, pow2(max(min(15 + ek_now - ea, 127), -126)), lk[z][0] + o, lk[z][1] + o, kRs, cols);
     }
   };
 
@@ -982,9 +1022,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
     }
     return;
   }
-  if (live)
-    put_row<DB, kFull>(dq + grow * a.ldq + h * a.HS, acc, split_unscale(es) * split_unscale(ek_acc) * a.scale, half, a.HS,
-                       assign);
+  if (live) put_scaled<DB, kFull>(dq + grow * a.ldq + h * a.HS, acc, ea - 30, a.scale, half, a.HS, assign);
 }
 
 // Rows r = (query row r / G, head r % G of the group) of q or dout in tiles of kTile,
@@ -1036,7 +1074,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   constexpr int kRs = HSP + 8, KG = BQ / 4;
   __shared__ __attribute__((aligned(16))) _Float16 lq[2][2][BQ * kRs], lg[2][2][BQ * kRs];
   __shared__ __attribute__((aligned(16))) float lL[2][BQ], lD[2][BQ];
-  __shared__ uint32_t slot[2][6][W];
+  __shared__ uint32_t slot[2][5][W];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
   const unsigned pair = blockIdx.x % pairs;
   const int tile = (int)(blockIdx.x / pairs);  // the keys that the most rows see first
@@ -1067,10 +1105,10 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   const size_t grow = (size_t)s.k0 + (live ? j : 0);
   v8h kh[DC], kl[DC], vh[DC], vl[DC];
   int ek, ev;
-  load_operand<DC, kFull>(k + grow * a.ldk + hk * a.HS, a.HS, live, half, kh, kl, &ek);
-  const float vmax = __uint_as_float(load_operand<DC, kFull>(v + grow * a.ldv + hk * a.HS, a.HS, live, half, vh, vl, &ev));
+  const uint32_t kbits = load_operand<DC, kFull>(k + grow * a.ldk + hk * a.HS, a.HS, live, half, kh, kl, &ek);
+  const uint32_t vbits = load_operand<DC, kFull>(v + grow * a.ldv + hk * a.HS, a.HS, live, half, vh, vl, &ev);
   const float ck = split_unscale(ek) * (a.scale * kLog2e), cv = split_unscale(ev);
-  bool bad = false;
+  bool bad = kbits >= kInfBits || vbits >= kInfBits;
 
   const GroupRows<BQ, KG> gq{q + (size_t)s.q0 * a.ldq + hk * G * a.HS, a.ldq, a.HS, G};
   const GroupRows<BQ, KG> gg{dout + (size_t)s.q0 * a.ldo + hk * G * a.HS, a.ldo, a.HS, G};
@@ -1099,10 +1137,11 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       tL = lse[stat + (size_t)i * a.NH + x] * kLog2e;
       tD = dsum[stat + (size_t)i * a.NH + x];
       if (r >= rows) tL = tD = 0.0f;
+      if (s.seen(i, a.causal) == 0) tL = 0.0f;  // a row without keys
     }
   };
   const auto note = [&](int z, int r0) {
-    uint32_t m[6] = {};
+    uint32_t m[5] = {};
     const bool part = r0 < all;
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -1114,35 +1153,27 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
         m[w] = max_abs<false>(m[w], t[u]);
       }
     }
-    if (tid < BQ) {
-      m[4] = abs_bits(tD);
-      m[5] = tL == -INFINITY ? 0u : abs_bits(tL);  // (a row without keys)
-    }
+    if (tid < BQ) m[4] = abs_bits(tL);
     m[0] = wave_max_bits(m[0]);
     m[1] = wave_max_bits(m[1]);
     if (part) {
       m[2] = wave_max_bits(m[2]);
       m[3] = wave_max_bits(m[3]);
     }
-    if (wave == 0) {
-      m[4] = wave_max_bits(m[4]);
-      m[5] = wave_max_bits(m[5]);
-    }
+    if (wave == 0) m[4] = wave_max_bits(m[4]);
     if (lane == 0) {
 #pragma unroll
-      for (int x = 0; x < 6; x++) slot[z][x][wave] = m[x];
+      for (int x = 0; x < 5; x++) slot[z][x][wave] = m[x];
     }
   };
-  int eq = -100, eg = -100;
-  float dmax = 0.0f;
+  int eq = 0, eg = 0;  // of the tile staged last
   const auto stage = [&](int z) {
-    const uint32_t mq = noted<W>(slot[z][0]), mg = noted<W>(slot[z][1]), md = noted<W>(slot[z][4]);
-    bad = bad || mq >= kInfBits || mg >= kInfBits || md >= kInfBits || noted<W>(slot[z][5]) >= 0x4a800000u /* 2^22 */ ||
+    const uint32_t mq = noted<W>(slot[z][0]), mg = noted<W>(slot[z][1]);
+    bad = bad || mq >= kInfBits || mg >= kInfBits || noted<W>(slot[z][4]) >= 0x4a800000u /* 2^22 */ ||
           too_wide(mq, noted<W>(slot[z][2])) ||
           too_wide(mg, noted<W>(slot[z][3]));
-    eq = max(eq, split_exp(mq));
-    eg = max(eg, split_exp(mg));
-    dmax = fmaxf(dmax, __uint_as_float(md));
+    eq = split_exp(mq);
+    eg = split_exp(mg);
     const float fq = split_scale(eq), fg = split_scale(eg);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -1157,31 +1188,22 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   };
 
   v16f ak[DB] = {}, av[DB] = {};
-  int eq_acc = -100, eg_acc = -100, es = -100;
-  float dmax_acc = -1.0f;
+  int ea = kNoScale, eg_acc = -100;  // the exponents that dk's and dv's accumulators stand on
   const int cols = cols_at(lane, kRs);
-  const auto compute = [&](int z, int r0, int eq_now, int eg_now, float dmax_now) {
-    if (eq_now != eq_acc || eg_now != eg_acc || dmax_now != dmax_acc) {
-      const float bound = fmaf((float)a.HS * vmax, pow2(min(max(eg_now, -126), 127)), dmax_now);
-      const int e = max(es, split_exp(__float_as_uint(bound)));
-      bad = bad || (live && (e > 120 || e + eq_now > 130));
-      const float fk = pow2(max(eq_acc - eq_now, -126)) * pow2(max(es - e, -126)), fv = pow2(max(eg_acc - eg_now, -126));
-      if (__any(fk != 1.0f || fv != 1.0f)) {
+  const auto compute = [&](int z, int r0, int eq_now, int eg_now) {
+    const bool seen = live && lim < r0 + BQ;
+    const int eg_was = eg_acc;
+    if (seen) eg_acc = max(eg_acc, eg_now);
+    if (__any(eg_acc != eg_was)) {
+      const float f = pow2(max(eg_was - eg_acc, -126));
 #pragma unroll
-        for (int x = 0; x < DB; x++)
+      for (int x = 0; x < DB; x++)
 #pragma unroll
-          for (int y = 0; y < 16; y++) {
-            ak[x][y] *= fk;
-            av[x][y] *= fv;
-          }
-      }
-      eq_acc = eq_now;
-      eg_acc = eg_now;
-      dmax_acc = dmax_now;
-      es = min(e, 120);
+        for (int y = 0; y < 16; y++) av[x][y] *= f;
     }
-    const float c2 = ck * split_unscale(eq_now), cd = cv * split_unscale(eg_now), f = pow2(-es);  // P is 2^15 up
-    bad = bad || (live && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
+    const float c2 = ck * split_unscale(eq_now), cd = cv * split_unscale(eg_now);
+    const float fp = pow2(max(min(eg_now - eg_acc, 0), -126));
+    bad = bad || (seen && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
     v16f p = dot_block<DC>(lq[z][0], lq[z][1], kRs, kh, kl, lane);
     v16f ds = dot_block<DC>(lg[z][0], lg[z][1], kRs, vh, vl, lane);
 #pragma unroll
@@ -1200,8 +1222,9 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       for (int y = 0; y < 16; y++)
         if (8 * (y / 4) + y % 4 < rel) p[y] = ds[y] = 0.0f;
     }
-    mac_block<DB>(av, p, 1.0f, lg[z][0], lg[z][1], kRs, cols);
-    mac_block<DB>(ak, ds, f, lq[z][0], lq[z][1], kRs, cols);
+    mac_block<DB>(av, p, fp, lg[z][0], lg[z][1], kRs, cols);
+    bad = raise(ea, ak, ds, eq_now) || bad;
+    mac_block<DB>(ak, ds, pow2(max(min(15 + eq_now - ea, 127), -126)), lq[z][0], lq[z][1], kRs, cols);
   };
 
   const int tiles = rows > from ? (rows - from + BQ - 1) / BQ : 0;
@@ -1217,10 +1240,9 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     __syncthreads();
     for (int at = 0; at < tiles; at++) {
       const int r0 = from + at * BQ, eq_now = eq, eg_now = eg;
-      const float dmax_now = dmax;
       if (at + 1 < tiles) stage((at + 1) & 1);
       if (at + 2 < tiles) load(r0 + 2 * BQ);
-      if (r0 + BQ > lo) compute(at & 1, r0, eq_now, eg_now, dmax_now);
+      if (r0 + BQ > lo) compute(at & 1, r0, eq_now, eg_now);
       if (at + 2 < tiles) note(at & 1, r0 + 2 * BQ);
       __syncthreads();
     }
@@ -1239,8 +1261,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     return;
   }
   if (!live) return;
-  put_row<DB, kFull>(ok + grow * ldk, ak, split_unscale(es) * split_unscale(eq_acc) * a.scale, half, a.HS, assign);
-  put_row<DB, kFull>(ov + grow * ldv, av, split_unscale(eg_acc) * 0x1p-15f, half, a.HS, assign);
+  put_scaled<DB, kFull>(ok + grow * ldk, ak, ea - 45, a.scale, half, a.HS, assign);  // dS, like P, was 2^15 up
+  put_scaled<DB, kFull>(ov + grow * ldv, av, eg_acc - 30, 1.0f, half, a.HS, assign);
 }
 
 // The parts' dk and dv added, in the parts' order, a thread per element.
