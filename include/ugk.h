@@ -378,8 +378,13 @@ int ugk_layernorm_dropout_residual_backward(float *dinp, float *dweight,
  *                                 also j <= i + Lk - Lq (the last query row
  *                                 sees every key)
  *     out_i = sum_j softmax(s)_j v_j,   lse_i = log sum_j exp(s_j)
- * A row without an allowed key has out 0, lse -infinity and gradients 0.
- * What a row must not see does not reach it, infinities and NaN included.
+ * A row without an allowed key, or all of whose scores are -infinity, has out 0,
+ * lse -infinity and gradients 0. What a row must not see does not reach it,
+ * infinities and NaN included. Results are those of single precision: within the
+ * error of its sums; where one key, value, query or dout is over 2^12 times the
+ * others of the 32 to 64 rows around it, theirs are held to 2^-39 of it. (Infinities,
+ * NaN that only some rows see, magnitudes that far apart where only some rows see
+ * them, and scores beyond 2^21 are computed row by row, many times slower.)
  * Rows of the buffers outside every sequence are neither read nor written. */
 typedef struct {
   int nseq;           /* sequences */
@@ -412,7 +417,8 @@ int ugk_attention_forward(float *out, float *lse, const float *q, const float *k
  * gradients must not overlap each other's elements (they may lie side by side
  * in one buffer, as q, k and v do) or the inputs, and the sequences must not
  * share rows. Deterministic. Waits for nothing and allocates on first use like
- * the other entry points (rows_q * NH floats of workspace). */
+ * the other entry points: rows_q * NH floats of workspace and, where the keys alone
+ * would leave CUs idle, up to 8 partial dk and dv. */
 int ugk_attention_backward(float *dq, float *dk, float *dv, const float *dout,
                            const float *q, const float *k, const float *v,
                            const float *out, const float *lse, ugk_attention a);

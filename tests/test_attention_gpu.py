@@ -513,3 +513,39 @@ def test_scores_of_minus_infinity(gpu, lens, lk):
     g = c.grads()
     c.backward(out, lse, g)
     assert g[2].eq(0).all()
+
+
+@pytest.mark.parametrize("Q", [1, 12])
+def test_offsets_beyond_32_bits(gpu, Q):
+    """A cache of more than 2^31 floats, the sequences at its end."""
+    NH, HS, ld, n = 2, 64, 4096, 200
+    rows = 2 ** 31 // ld + 600
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    k = torch.empty(rows * ld, device=DEV)
+    starts = [rows - 500, rows - n]
+    tail = k[(rows - 500) * ld:]
+    tail.copy_(torch.randn(tail.numel(), generator=g, device=DEV))
+    q = rand(g, 2 * Q, NH * HS)
+    out, lse = torch.empty(2 * Q, NH * HS, device=DEV), torch.empty(2 * Q, NH, device=DEV)
+    a = gpu.Attention(nseq=2, NH=NH, NKV=NH, HS=HS, rows_q=2 * Q, rows_k=rows, max_q=Q, max_k=n, q_start=ints([0, Q]),
+                      q_end=ints([Q, 2 * Q]), k_start=ints(starts), k_end=ints([s + n for s in starts]), ldk=ld, ldv=ld)
+    gpu.attention_forward(out, lse, q, k, k[NH * HS:], a)
+    gpu.synchronize()
+    t = tail.view(-1, ld)
+    s = Seqs([Q, Q], [n, n])
+    s.k, s.rows_k = [0, 500 - n], 500
+    kk, vv = t[:, :NH * HS].unflatten(1, (NH, HS)), t[:, NH * HS:2 * NH * HS].unflatten(1, (NH, HS))
+    w, wl, tol, tol_l = att_ref.forward(s, q.view(2 * Q, NH, HS), kk, vv, HS ** -0.5, True)
+    inside(out.view(2 * Q, NH, HS), w, tol, "out")
+    inside(lse, wl, tol_l, "lse")
+
+
+def test_many_sequences(gpu):
+    """More (sequence, head) pairs than a launch has XCDs, CUs or parts for, of every length from 0 to 40."""
+    lens = [(7 * i) % 41 for i in range(700)]
+    for lq, lk in ((lens, None), ([1] * 700, lens)):
+        c = Call(gpu, Seqs(lq, lk), 2, 1, 8)
+        out, lse = c.forward()
+        check_forward(c, out, lse)
+        check_backward(c, out, lse)

@@ -102,30 +102,47 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
 //
 // The rows of a tile are (query row, head of the group) pairs, so that the heads
 // of a group share the key and value tiles: row r of a sequence and key/value
-// head is query row r / G, head r % G of the group. A wavefront holds 32 rows; a
-// workgroup of W wavefronts goes over the keys BK at a time.
+// head is query row r / G, head r % G of the group. A wavefront holds one or two
+// blocks of 32 rows; a workgroup of four goes over the keys BK at a time.
 //
 // S^T = K Q^T: a lane then holds one row's scores of half of the keys (the other half
 // in lane ^ 32), so that the row's maximum, sum and factors are values of the
 // lane, and its 16 registers of a 32 x 32 block are, rounded to halves, the
-// operand of O^T += V^T P^T as they stand, with the keys in the order 16 c + 8
-// (j / 4) + 4 (lane / 32) + j % 4: V^T is laid out in that order. Nothing moves
-// between lanes but one exchange of halves per tile.
+// operand of O^T += V^T P^T as they stand, with the keys in the order that
+// frag_cols reads V's columns in. Nothing moves between lanes but one exchange of
+// halves per block.
 //
 // Products are split (ugk_split.h). K and V are split while they are put into LDS, by the
-// exponent of the tile's largest magnitude (V: of all tiles so far, the
-// accumulators being rescaled when it grows); the maximum is taken over the
-// registers that the tile was loaded into, one tile ahead, and goes through LDS with
-// the barrier that the tile buffers need anyway: one barrier per tile. P lies
-// in (0, 1] and is scaled by 2^15 in its exponent.
+// exponent of the tile's largest magnitude; that is taken over the registers that
+// the tile was loaded into, one tile ahead, and goes through LDS with the barrier
+// that the tile buffers need anyway: one barrier per tile. A row's output stands on
+// the largest exponent of the tiles that it has seen, and its P are taken that much
+// lower where a tile lies below it (in the exponent, which costs nothing), so that what a row
+// must not see moves neither.
 //
 // The workgroup's rows are taken one by one instead (row_forward), where a masked key
-// is not touched at all, if a tile holds an infinity or NaN; if not all rows see
-// all of a tile and its keys' magnitudes lie further apart than the halves'
-// digits allow (a row would lose its digits to keys that it must not see); or if
-// scores leave the range of the above (2^22 in base 2).
-// A row's P are scaled to 2^kTop at the maximum that they stand on, which moves (and the accumulators with it) only
-// when a score lies 2^7 above it: P then stays below 2^(kTop + 7), the halves' range.
+// is not touched at all, if a tile holds an infinity, or NaN that not all rows see;
+// if not all rows see all of a tile and its keys' magnitudes lie further apart
+// than the halves' digits allow (too_wide); or if scores leave the range of the
+// above (2^22 in base 2).
+//
+// What bounds it: on gfx950 a wavefront's matrix instruction holds back the vector
+// instructions of every wavefront on its SIMD (8 x (mfma, 4 fma): 20.2 ns per pair with one
+// wavefront, 18.0 with two, of which the mfma alone takes 14.3), so the two
+// add up. 16,384 rows of 12 heads of 64 take 1,283 us: 321 TFLOP/s of products counted
+// once, 963 of halves. That is 1.67 us for a SIMD's block of 32 rows and 64 keys, of which
+// its 48 mfma take 0.69; the same products in single precision
+// (v_mfma_f32_32x32x2_f32, 128 of 64 cycles) would take 3.7. An earlier state of this kernel
+// took 1,530 us for 4 x 8,192 rows, and 1,122 without loading, splitting and storing the
+// tiles. Tried without gain: K and V read ahead from LDS during the softmax (72.0
+// against 71.2 us for 8 x 1,024 rows); workgroups of 8 wavefronts (1,445 against 1,528
+// us for 4 x 8,192 rows, but two blocks per wavefront 1,352); a pair's tiles on one XCD
+// (1,604 against 1,539); of those workgroups two per CU, with 128 registers a lane (spills:
+// 562 against 470 us for 8,192 rows).
+//
+// A row's P are scaled to 2^kTop at the maximum that they stand on, which moves
+// (and the accumulators with it) only when a score lies 2^7 above it: P then stays
+// below 2^(kTop + 7), the halves' range.
 constexpr float kTop = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -504,16 +521,24 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 
 // ---- forward, few rows per key/value head ----------------------------------------
 //
-// With few (query row, head) pairs for a key/value head (a token's decode step), the
-// work is to read K and V once, and the products fit the vector units: 4 R
-// operations per byte pair against the matrix units' 32 rows that would stay
-// mostly empty. HSP / 4 lanes take a key, four floats each, so that a wavefront reads 64
-// / (HSP / 4) whole rows of K at a time, and then of V: U of them are in flight
-// per lane before the first is used. A group of lanes has its own running maximum,
-// sum and output (no exchange between groups until the end); its score sums go through
-// DPP. The groups, then the workgroup's NW wavefronts, are joined at the end
-// in their order, through LDS. Single precision throughout, and a key that
-// a row must not see is left out by selects, so nothing of it reaches the row.
+// With up to four (query row, head) pairs for a key/value head (a token's decode
+// step), the work is to read K and V once: memory bounds it, and the products fit
+// the vector units, whose 32-row counterpart would stay mostly empty. HSP / 4 lanes take
+// a key, four floats each, so that a wavefront reads 64 / (HSP / 4) whole rows of
+// K at a time, and then of V: U of them are in flight per lane before the first is
+// used. A group of lanes has its own running maximum, sum and output (no exchange
+// between groups until the end); its score sums go through DPP. The groups, then the
+// workgroup's NW wavefronts, are joined at the end in their order, through LDS.
+// Single precision throughout, and a key that a row must not see is left out by
+// selects, so nothing of it reaches the row.
+//
+// 24 sequences of 8,192 keys, 8 key/value heads of 128: 271 us with one query head for
+// each, 277 with four (1,611 MB, 5.8 to 6.0 TB/s); 64 of 2,048, 12 heads of 64, 144 us (805
+// MB, 5.6 TB/s). On the 32-row tiles 24 of up to 16,384 keys took 993 us, here 413 and
+// 283 with the key axis split. Five to eight rows go to the tiles (24 x 4,096 keys, eight
+// query heads of 64 to each of 8: 91 us; four, here: 81), for here they would spill. Key axes
+// of more than kFewChunk are split also where the workgroups fill the CUs: the
+// lengths differ, and the longest would run alone; where they are equal it costs 1% to 4%.
 template <int kLanes>
 __device__ __forceinline__ float lanes_sum(float v) {
   v += dpp_lane<kDppQuadSwap1>(v);
@@ -763,9 +788,16 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
 // forward holds them, then dk and dv over the keys, so that nothing is added by
 // two workgroups and the results do not depend on their order (one pass with
 // atomics would save the second S and dP, 4 of 14 HS operations per pair).
-// P = exp(S - lse) needs no running maximum. The same tiles as in the forward
-// fall back to single rows.
-
+// P = exp(S - lse) needs no running maximum. A lane holds one row (dq) or one key (dk, dv)
+// as it holds a row in the forward, the other side goes through LDS in tiles, and
+// what its accumulators stand on follows what it has seen alone. The same tiles as
+// in the forward fall back to single rows.
+//
+// The same sum of matrix and vector instructions bounds them: of 858 (dk, dv) and 633 us
+// (dq) at 4 x 4,096 rows of 12 heads, 612 and 465 were left without loading,
+// splitting and storing the tiles. 8 x 1,024 rows of 12 heads: 128 and 100 us, 220
+// with the launches (146 TFLOP/s of 10 HS operations per pair). Workgroups of
+// one wavefront were slower at every size tried.
 
 // The same times 2^e f, for any e.
 template <int DB, bool kFull>
@@ -855,7 +887,6 @@ __device__ __forceinline__ uint32_t load_operand(const float *p, int HS, bool li
   for (int c = 0; c < DC; c++) split8(x[c], split_scale(*e), h[c], l[c]);
   return m;
 }
-
 
 template <int HSP, int BK, bool kFull>
 __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
