@@ -549,3 +549,26 @@ def test_many_sequences(gpu):
         out, lse = c.forward()
         check_forward(c, out, lse)
         check_backward(c, out, lse)
+
+
+def test_backward_workspace_of_a_large_cache(gpu):
+    """The parts of dk and dv hold all key rows: where the sequences are a small part of a cache, there are few."""
+    n, rows_k, NH, HS = 1100, 1 << 20, 2, 64
+    c = Call(gpu, Seqs([n], [n]), NH, 1, HS)
+    c.s.k, c.s.rows_k = [rows_k - n], rows_k
+    k, v = (torch.zeros(rows_k, 1, HS, device=DEV) for _ in range(2))
+    k[-n:], v[-n:] = c.k, c.v
+    c.k, c.v = k, v
+    out, lse = c.forward()
+    grads = c.grads()
+    gpu.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    c.backward(out, lse, grads)
+    gpu.synchronize()
+    # the bound: 2 * 8 parts of 2^20 rows would be 4.3 GB
+    assert free - torch.cuda.mem_get_info()[0] < 1 << 30
+    s = Seqs([n], [n])
+    want, tol = att_ref.backward(s, c.q, k[-n:], v[-n:], out, lse, c.dout, c.scale, True)
+    for got, w, t, name in zip((grads[0], grads[1][-n:], grads[2][-n:]), want, tol, ("dq", "dk", "dv")):
+        inside(got, w, t, name)
+    assert not grads[1][:-n].any() and not grads[2][:-n].any()

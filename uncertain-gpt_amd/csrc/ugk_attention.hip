@@ -1344,11 +1344,15 @@ long long filled(const ugk_attention &a, long long rows, long long most, int gro
 // dk and dv: parts of the rows' range where the keys make too few workgroups to fill
 // the CUs, which hold two workgroups for heads up to 64 and one for larger ones,
 // twice (the heads of a group share their keys: 4 x 2,048 rows of 16/4 heads 769 us
-// whole, 370 in four parts and 13 to add them). A part has four tiles or more.
+// whole, 370 in four parts and 13 to add them). A part has four tiles or more, and
+// the parts, which hold all key rows, stay below kSplitKeys
+// keys per CU (attention_backward_bound): a cache of which the sequences are a small part has fewer.
+constexpr long long kSplitKeys = 4 * kTileRows;  // per CU, over all parts and heads
 int dkv_splits(const ugk_attention &a) {
   const long long rows = (long long)a.max_q * (a.NH / a.NKV);
   const long long want = (a.HS > 64 ? 2LL : 4LL) * cu_count() / max(filled(a, a.rows_k, a.max_k, 1, kTileRows), 1LL);
-  return (int)max(1LL, min(min(want, (long long)kMaxSplits), rows / 128));
+  const long long keys = kSplitKeys * cu_count() / max((long long)a.rows_k * a.NKV, 1LL);
+  return (int)max(1LL, min(min(min(want, keys), (long long)kMaxSplits), rows / 128));
 }
 
 constexpr int kFewRows = 4, kFewChunk = 1024;
@@ -1448,9 +1452,7 @@ size_t attention_backward_bytes(const ugk_attention &a) {
   return (dsum + (splits > 1 ? 2 * splits * a.rows_k * a.NKV * a.HS : 0)) * sizeof(float);
 }
 size_t attention_backward_bound(size_t rows, size_t C, size_t NH) {
-  // splits times the workgroups, each of up to kTileRows keys of one head, are at most four per CU
-  const size_t keys = 4 * (size_t)cu_count() * kTileRows * kMaxHead;
-  const size_t split = min((size_t)kMaxSplits * rows * C, keys + rows * C);
+  const size_t split = min((size_t)kMaxSplits * rows * C, (size_t)kSplitKeys * cu_count() * kMaxHead);
   return ((rows * NH + 63) / 64 * 64 + 2 * split) * sizeof(float);
 }
 
