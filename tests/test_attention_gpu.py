@@ -572,3 +572,20 @@ def test_backward_workspace_of_a_large_cache(gpu):
     for got, w, t, name in zip((grads[0], grads[1][-n:], grads[2][-n:]), want, tol, ("dq", "dk", "dv")):
         inside(got, w, t, name)
     assert not grads[1][:-n].any() and not grads[2][:-n].any()
+
+
+@pytest.mark.parametrize("lens,lk", [([300, 41], None), ([1, 1], [700, 90]), ([2], [2000])])
+def test_limits_far_above_the_buffers(gpu, lens, lk):
+    """max_q and max_k of the longest sequence that there could be, not of this call's."""
+    c = Call(gpu, Seqs(lens, lk), 4, 2, 64)
+    out, lse = c.forward()
+    a = c.att()
+    a.max_q = a.max_k = 2 ** 31 - 1
+    out2, lse2, grads2 = torch.full_like(out, 7.0), torch.full_like(lse, 7.0), c.grads()
+    gpu.attention_forward(out2, lse2, c.q, c.k, c.v, a)
+    gpu.attention_backward(*grads2, c.dout, c.q, c.k, c.v, out2, lse2, a)
+    gpu.synchronize()
+    check_forward(c, out2, lse2)
+    want, tol = att_ref.backward(c.s, c.q, c.k, c.v, out2, lse2, c.dout, c.scale, True)
+    for got, w, t, name in zip(grads2, want, tol, ("dq", "dk", "dv")):
+        inside(got, w, t, name)

@@ -350,6 +350,9 @@ int check_attention(const char *fn, ugk_attention *a, bool *none) {
   const long long rows = (a->rows_q > a->rows_k ? a->rows_q : a->rows_k) + 1LL;
   if (a->ldq > most / rows || a->ldo > most / rows || a->ldk > most / rows || a->ldv > most / rows)
     return bad(fn, "rows * stride exceeds the address space");
+  // no sequence is longer than its buffer: a limit above that only makes empty workgroups and parts
+  a->max_q = a->max_q < a->rows_q ? a->max_q : a->rows_q;
+  a->max_k = a->max_k < a->rows_k ? a->max_k : a->rows_k;
   if ((long long)a->max_q * (a->NH / a->NKV) > INT_MAX / 2 || a->max_k > INT_MAX / 2)
     return bad(fn, "max_q * NH / NKV or max_k exceeds 2^30");
   // a workgroup of 256 threads takes up to 128 rows of q, or of k, of a sequence and key/value head, and a launch
@@ -358,7 +361,7 @@ int check_attention(const char *fn, ugk_attention *a, bool *none) {
   const long long blocks = tq > tk ? tq : tk;
   if ((long long)a->nseq * a->NKV >= ((long long)1 << 24) / (blocks > 0 ? blocks : 1))
     return bad(fn, "nseq * heads * rows exceeds the grid");
-  *none = a->nseq == 0 || a->max_q == 0 || a->rows_q == 0;
+  *none = a->nseq == 0 || a->max_q == 0;
   return UGK_OK;
 }
 
