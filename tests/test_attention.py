@@ -114,3 +114,17 @@ def test_reference_against_autograd():
     for x, t in zip(got, (q, k, v)):
         assert torch.allclose(x, t.grad, rtol=1e-9, atol=1e-9)
     assert (tol[~out.isnan()] < 1e-4).all() and tol_l[~lse.isnan()].isfinite().all()
+
+
+def test_more_sequences_than_the_offsets_hold():
+    import ugk
+    a = shape(ugk)
+    a.nseq = 1 << 20  # no offset tensors: the library's own checks apply
+    t = torch.zeros(10, 256)
+    with pytest.raises(ValueError, match="on the GPU"):
+        ugk.attention_forward(t, None, t, t, t, a)
+    a._most = 2
+    with pytest.raises(ValueError, match="the offsets hold 2"):
+        ugk.attention_forward(t, None, t, t, t, a)
+    with pytest.raises(ValueError, match="the offsets hold 2"):
+        ugk.attention_backward(t, t, t, t, t, t, t, t, t, a)

@@ -589,3 +589,29 @@ def test_limits_far_above_the_buffers(gpu, lens, lk):
     want, tol = att_ref.backward(c.s, c.q, c.k, c.v, out2, lse2, c.dout, c.scale, True)
     for got, w, t, name in zip(grads2, want, tol, ("dq", "dk", "dv")):
         inside(got, w, t, name)
+
+
+def test_tensors_that_the_binding_refuses(gpu, monkeypatch):
+    """Offsets for fewer sequences than asked for, rows whose elements are apart, tensors on another GPU."""
+    c = Call(gpu, Seqs([4, 3]), 2, 2, 64)
+    out, lse = c.forward()
+    a = c.att()
+    a.nseq = 3
+    with pytest.raises(ValueError, match="the offsets hold 2"):
+        gpu.attention_forward(out, lse, c.q, c.k, c.v, a)
+    with pytest.raises(ValueError, match="the offsets hold 2"):
+        c.gpu.attention_backward(*c.grads(), c.dout, c.q, c.k, c.v, out, lse, a)
+    wide = torch.zeros(128, 7, device=DEV).t()
+    with pytest.raises(ValueError, match="last stride"):
+        gpu.attention_forward(out, lse, wide, c.k, c.v, c.att())
+    a, x = c.att(), torch.zeros(64, device=DEV)
+    monkeypatch.setattr(gpu, "_one_device", False)
+    assert torch.cuda.current_device() == 0
+    gpu.attention_forward(out, lse, c.q, c.k, c.v, a)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: gpu.attention_forward(out, lse, c.q, c.k, c.v, a), lambda: gpu.dropout_forward(x, x, 64, 0.5, 1, 1),
+                 lambda: gpu.attention_forward(1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, a),
+                 lambda: gpu.attention_forward(1 << 20, lse, 1 << 20, 1 << 20, 1 << 20, gpu.Attention(1, 2, 2, 64, 7, 7, 7, 7)),
+                 lambda: gpu.dense_attention_forward(x, torch.zeros(192, device=DEV), 1, 1, 64, 1)):
+        with pytest.raises(ValueError, match="the current device is cuda:1"):
+            call()

@@ -66,8 +66,10 @@ class Attention(ctypes.Structure):
     ``q_start``, ``q_end``, ``k_start``, ``k_end`` are int32 device tensors of at least ``nseq`` elements (or
     device addresses, or None): sequence b is the rows [q_start[b], q_end[b]) of q and [k_start[b], k_end[b]) of k
     and v. Strides ``ldq``, ``ldk``, ``ldv``, ``ldo`` in floats, 0 for rows without gaps. ``scale`` defaults to
-    1/sqrt(HS). The structure keeps its tensors alive.
+    1/sqrt(HS). The structure keeps its tensors alive; a call refuses an ``nseq`` raised above what they hold.
     """
+    _tensors = ()
+    _most = 2 ** 31 - 1  # sequences that the offset tensors hold
     _OFFSETS = ("q_start", "q_end", "k_start", "k_end")
     _fields_ = [(_n, _i) for _n in ("nseq", "NH", "NKV", "HS", "rows_q", "rows_k", "max_q", "max_k", "causal")] + \
         [("scale", _fl)] + [(_n, _fp) for _n in _OFFSETS] + \
@@ -82,6 +84,7 @@ class Attention(ctypes.Structure):
         super().__init__(nseq, NH, NKV, HS, rows_q, rows_k, max_q, max_k, 1 if causal else 0, scale,
                          *(_ptr(t, n, nseq, "i32") for t, n in zip(tensors, self._OFFSETS)), ldq, ldk, ldv, ldo)
         self._tensors = tensors
+        self._most = min((t.numel() for t in tensors if t is not None and not isinstance(t, int)), default=Attention._most)
 
 
 _MATMUL_FWD = ctypes.CFUNCTYPE(_i, _fp, _fp, _fp, _fp, _fp, _i, _i, _i)
@@ -420,24 +423,24 @@ def dropout_forward(out, inp, n: int, p: float, seed: int, step: int, site: int 
     """``out = dropout(inp)``: element i is kept and multiplied by 1/(1-p) where word ``i % 4`` of Philox block
     ``i // 4`` of (seed, step, site) is at least p * 2^32, else +0. The mask is drawn again by every call that
     names the same (seed, step, site). No counterpart in the reference."""
-    _check(lib.ugk_dropout_forward(_ptr(out, "out", n, "f32"), _ptr(inp, "inp", n, "f32"), n, p, seed, step, site))
+    _check(lib.ugk_dropout_forward(_ptr_here(out, "out", n), _ptr_here(inp, "inp", n), n, p, seed, step, site))
 
 
 def dropout_backward(dinp, dout, n: int, p: float, seed: int, step: int, site: int = 0) -> None:
     """``dinp += dropout(dout)`` with the forward's mask."""
-    _check(lib.ugk_dropout_backward(_ptr(dinp, "dinp", n, "f32"), _ptr(dout, "dout", n, "f32"), n, p, seed, step, site))
+    _check(lib.ugk_dropout_backward(_ptr_here(dinp, "dinp", n), _ptr_here(dout, "dout", n), n, p, seed, step, site))
 
 
 def dropout_residual_forward(out, x, y, n: int, p: float, seed: int, step: int, site: int = 0) -> None:
     """``out = x + dropout(y)``."""
-    _check(lib.ugk_dropout_residual_forward(_ptr(out, "out", n, "f32"), _ptr(x, "x", n, "f32"), _ptr(y, "y", n, "f32"), n,
+    _check(lib.ugk_dropout_residual_forward(_ptr_here(out, "out", n), _ptr_here(x, "x", n), _ptr_here(y, "y", n), n,
                                             p, seed, step, site))
 
 
 def dropout_residual_backward(dx, dy, dout, n: int, p: float, seed: int, step: int, site: int = 0) -> None:
     """``dx += dout``; ``dy += dropout(dout)``."""
-    _check(lib.ugk_dropout_residual_backward(_ptr(dx, "dx", n, "f32"), _ptr(dy, "dy", n, "f32"),
-                                             _ptr(dout, "dout", n, "f32"), n, p, seed, step, site))
+    _check(lib.ugk_dropout_residual_backward(_ptr_here(dx, "dx", n), _ptr_here(dy, "dy", n),
+                                             _ptr_here(dout, "dout", n), n, p, seed, step, site))
 
 
 def dropout_residual_layernorm_forward(res, out, mean, rstd, x, y, weight, bias, B: int, T: int, C: int, p: float,
@@ -445,9 +448,9 @@ def dropout_residual_layernorm_forward(res, out, mean, rstd, x, y, weight, bias,
     """``dropout_residual_forward(res, x, y)`` then ``layernorm_forward(out, mean, rstd, res, ...)``, one pass."""
     n, rows = B * T * C, B * T
     _check(lib.ugk_dropout_residual_layernorm_forward(
-        _ptr(res, "res", n, "f32"), _ptr(out, "out", n, "f32"), _ptr(mean, "mean", rows, "f32"),
-        _ptr(rstd, "rstd", rows, "f32"), _ptr(x, "x", n, "f32"), _ptr(y, "y", n, "f32"),
-        _ptr(weight, "weight", C, "f32"), _ptr(bias, "bias", C, "f32"), B, T, C, p, seed, step, site))
+        _ptr_here(res, "res", n), _ptr_here(out, "out", n), _ptr_here(mean, "mean", rows),
+        _ptr_here(rstd, "rstd", rows), _ptr_here(x, "x", n), _ptr_here(y, "y", n),
+        _ptr_here(weight, "weight", C), _ptr_here(bias, "bias", C), B, T, C, p, seed, step, site))
 
 
 def layernorm_dropout_residual_backward(dinp, dweight, dbias, dx, dy, dout, inp, weight, mean, rstd, B: int, T: int,
@@ -455,10 +458,25 @@ def layernorm_dropout_residual_backward(dinp, dweight, dbias, dx, dy, dout, inp,
     """``layernorm_backward`` then ``dropout_residual_backward(dx, dy, dinp)``."""
     n, rows = B * T * C, B * T
     _check(lib.ugk_layernorm_dropout_residual_backward(
-        _ptr(dinp, "dinp", n, "f32"), _ptr(dweight, "dweight", C, "f32"), _ptr(dbias, "dbias", C, "f32"),
-        _ptr(dx, "dx", n, "f32"), _ptr(dy, "dy", n, "f32"), _ptr(dout, "dout", n, "f32"),
-        _ptr(inp, "inp", n, "f32"), _ptr(weight, "weight", C, "f32"), _ptr(mean, "mean", rows, "f32"),
-        _ptr(rstd, "rstd", rows, "f32"), B, T, C, p, seed, step, site))
+        _ptr_here(dinp, "dinp", n), _ptr_here(dweight, "dweight", C), _ptr_here(dbias, "dbias", C),
+        _ptr_here(dx, "dx", n), _ptr_here(dy, "dy", n), _ptr_here(dout, "dout", n),
+        _ptr_here(inp, "inp", n), _ptr_here(weight, "weight", C), _ptr_here(mean, "mean", rows),
+        _ptr_here(rstd, "rstd", rows), B, T, C, p, seed, step, site))
+
+
+def _here(x, what: str) -> None:
+    """Refuse a tensor on another GPU than the current one, whose kernels would read its address."""
+    if not _one_device and _torch is not None and isinstance(x, _torch.Tensor) and x.device.index != _torch.cuda.current_device():
+        raise ValueError(f"{what}: tensor is on {x.device}, the current device is cuda:{_torch.cuda.current_device()}")
+
+
+def _ptr_here(x, what: str, need: int):
+    """_ptr of floats that must be on the current GPU."""
+    if type(x) is _Tensor and _one_device and x.dtype is _DTYPES["f32"] and x.is_cuda and x.numel() >= need and x.is_contiguous():
+        return x.data_ptr()
+    p = _ptr(x, what, need, "f32")
+    _here(x, what)
+    return p
 
 
 def _rows_ptr(x, what: str, need: int):
@@ -478,10 +496,11 @@ def _rows_ptr_or_raise(x, what: str, need: int):
         raise TypeError(f"{what}: expected a torch tensor or a device address, got {type(x)!r}")
     if x.device.type != "cuda":
         raise ValueError(f"{what}: tensor must be on the GPU, got {x.device}")
-    if x.device.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: tensor is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    _here(x, what)
     if x.dtype != torch.float32:
         raise TypeError(f"{what}: dtype must be {torch.float32}, got {x.dtype}")
+    if x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{what}: the elements of a row must lie side by side, the last stride is {x.stride(-1)}")
     has = x.untyped_storage().nbytes() // 4 - x.storage_offset()
     if need > 0 and (x.numel() == 0 or has < need):
         raise ValueError(f"{what}: needs at least {need} elements from its first one on, has {has}")
@@ -490,6 +509,11 @@ def _rows_ptr_or_raise(x, what: str, need: int):
 
 def _attention_needs(a: Attention):
     """The floats from the first element of q, k, v and out to the end of their last rows."""
+    if a.nseq > a._most:
+        raise ValueError(f"nseq: {a.nseq} sequences, the offsets hold {a._most}")
+    if not _one_device:
+        for t, name in zip(a._tensors, a._OFFSETS):
+            _here(t, name)
     rq, rk, HS = a.rows_q - 1, a.rows_k - 1, a.HS
     wq, wk = a.NH * HS, a.NKV * HS
     return (rq * (a.ldq or wq) + wq if rq >= 0 else 0, rk * (a.ldk or wk) + wk if rk >= 0 else 0,
@@ -502,7 +526,7 @@ def attention_forward(out, lse, q, k, v, a: Attention) -> None:
     None. q, k, v and out may be views into rows that hold other things as well (strides in ``a``)."""
     nq, nk, nv, no = _attention_needs(a)
     pq, pk, pv, po = _rows_ptr(q, "q", nq), _rows_ptr(k, "k", nk), _rows_ptr(v, "v", nv), _rows_ptr(out, "out", no)
-    _check(lib.ugk_attention_forward(po, _ptr(lse, "lse", a.rows_q * a.NH, "f32"), pq, pk, pv, a))
+    _check(lib.ugk_attention_forward(po, _ptr_here(lse, "lse", a.rows_q * a.NH), pq, pk, pv, a))
 
 
 def attention_backward(dq, dk, dv, dout, q, k, v, out, lse, a: Attention) -> None:
@@ -519,20 +543,20 @@ def _attention_backward(fn, dq, dk, dv, dout, q, k, v, out, lse, a: Attention) -
     nq, nk, nv, no = _attention_needs(a)
     _check(fn(_rows_ptr(dq, "dq", nq), _rows_ptr(dk, "dk", nk), _rows_ptr(dv, "dv", nv), _rows_ptr(dout, "dout", no),
               _rows_ptr(q, "q", nq), _rows_ptr(k, "k", nk), _rows_ptr(v, "v", nv), _rows_ptr(out, "out", no),
-              _ptr(lse, "lse", a.rows_q * a.NH, "f32"), a))
+              _ptr_here(lse, "lse", a.rows_q * a.NH), a))
 
 
 def dense_attention_forward(out, qkv, B: int, T: int, C: int, NH: int) -> None:
     """attention_forward of qkv rows (3C), as the step driver's callback takes it (``dense_attention_callbacks``)."""
     n = B * T * C
-    _check(lib.ugk_dense_attention_forward(None, _ptr(out, "out", n, "f32"), _ptr(qkv, "qkv", 3 * n, "f32"), B, T, C, NH))
+    _check(lib.ugk_dense_attention_forward(None, _ptr_here(out, "out", n), _ptr_here(qkv, "qkv", 3 * n), B, T, C, NH))
 
 
 def dense_attention_backward(dqkv, dout, qkv, B: int, T: int, C: int, NH: int) -> None:
     """``dqkv +=`` the gradient of dense_attention_forward, whose out and lse are computed again."""
     n = B * T * C
-    _check(lib.ugk_dense_attention_backward(None, _ptr(dqkv, "dqkv", 3 * n, "f32"), _ptr(dout, "dout", n, "f32"),
-                                            _ptr(qkv, "qkv", 3 * n, "f32"), B, T, C, NH))
+    _check(lib.ugk_dense_attention_backward(None, _ptr_here(dqkv, "dqkv", 3 * n), _ptr_here(dout, "dout", n),
+                                            _ptr_here(qkv, "qkv", 3 * n), B, T, C, NH))
 
 
 def dense_attention_callbacks() -> dict:
