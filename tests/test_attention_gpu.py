@@ -615,3 +615,61 @@ def test_tensors_that_the_binding_refuses(gpu, monkeypatch):
                  lambda: gpu.dense_attention_forward(x, torch.zeros(192, device=DEV), 1, 1, 64, 1)):
         with pytest.raises(ValueError, match="the current device is cuda:1"):
             call()
+
+
+def test_a_graph_keeps_its_workspace_when_the_region_grows(gpu):
+    """A captured call, then a call that needs a larger workspace, then other memory written: the replay's results stay."""
+    cfg = gpu.Config(B=1, T=64, C=64, V=50, NH=1, maxT=64, L=1)
+    ws = torch.empty(gpu.workspace_bytes(cfg) + 256, dtype=torch.uint8, device=DEV)
+    at = (-ws.data_ptr()) % 256
+    gpu.set_workspace(ws[at:at + gpu.workspace_bytes(cfg)], cfg)
+    gpu.set_workspace(None, cfg)  # the library's own regions start again from nothing
+    c, big = Call(gpu, Seqs([1, 1], [3000, 2500]), 2, 2, 64), Call(gpu, Seqs([3000]), 40, 40, 8)
+    a = c.att()
+    want, want_lse = c.forward()
+    out, lse = torch.empty_like(want), torch.empty_like(want_lse)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gpu.set_stream(stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            gpu.attention_forward(out, lse, c.q, c.k, c.v, a)
+        before = gpu.lib.ugk_scratch_bytes()
+        with torch.cuda.stream(stream):
+            b_out, b_lse = big.forward()
+            big.backward(b_out, b_lse, big.grads())
+        stream.synchronize()
+        assert gpu.lib.ugk_scratch_bytes() > before
+        for _ in range(3):
+            out.fill_(3.0)
+            lse.fill_(3.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    finally:
+        gpu.set_stream(None)
+
+
+def test_capture_without_the_workspace_is_refused(gpu):
+    cfg = gpu.Config(B=1, T=64, C=64, V=50, NH=1, maxT=64, L=1)
+    ws = torch.empty(gpu.workspace_bytes(cfg) + 256, dtype=torch.uint8, device=DEV)
+    at = (-ws.data_ptr()) % 256
+    gpu.set_workspace(ws[at:at + gpu.workspace_bytes(cfg)], cfg)
+    gpu.set_workspace(None, cfg)
+    c = Call(gpu, Seqs([1, 1], [3000, 2500]), 2, 2, 64)
+    a, x, y = c.att(), torch.zeros(2, 2, 64, device=DEV), torch.zeros(2, 2, device=DEV)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gpu.set_stream(stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            with pytest.raises(gpu.UgkError) as err:
+                gpu.attention_forward(x, y, c.q, c.k, c.v, a)
+        assert err.value.status == 3 and "before graph capture" in str(err.value)
+    finally:
+        gpu.set_stream(None)
+    out, lse = c.forward()
+    check_forward(c, out, lse)

@@ -39,6 +39,7 @@ struct DevWorkspace {
   size_t user_bytes = 0;
   size_t off[kNumRegions] = {}, cap[kNumRegions] = {};
   bool fresh[kNumRegions] = {true, true, true, true, true};
+  bool captured[kNumRegions] = {};  // own[r] is in a graph, which may be replayed at any time: it is never freed
 };
 DevWorkspace g_ws[kMaxDevices];
 
@@ -80,9 +81,10 @@ void *own_region(DevWorkspace &w, Region r, size_t bytes) {
   if (w.own[r]) {
     // kernels queued earlier, on this or another stream, may still use the old buffer
     (void)hipDeviceSynchronize();
-    (void)hipFree(w.own[r]);
+    if (!w.captured[r]) (void)hipFree(w.own[r]);
     w.own[r] = nullptr;
     w.own_bytes[r] = 0;
+    w.captured[r] = false;
   }
   const size_t want = align_up(bytes < ((size_t)1 << 16) ? ((size_t)1 << 16) : bytes);
   if (hipMalloc(&w.own[r], want) != hipSuccess) {
@@ -125,9 +127,10 @@ void free_own(DevWorkspace &w) {
   if (!any) return;
   (void)hipDeviceSynchronize();
   for (int r = 0; r < kNumRegions; r++) {
-    if (w.own[r]) (void)hipFree(w.own[r]);
+    if (w.own[r] && !w.captured[r]) (void)hipFree(w.own[r]);
     w.own[r] = nullptr;
     w.own_bytes[r] = 0;
+    w.captured[r] = false;
     w.fresh[r] = true;
   }
 }
@@ -182,7 +185,8 @@ void *workspace(Region r, size_t bytes, bool *fresh, bool keep_fresh) {
     }
     p = w.user + w.off[r];
   } else {
-    if (!(w.own[r] && w.own_bytes[r] >= bytes) && stream_capturing()) {
+    const bool capturing = stream_capturing();
+    if (!(w.own[r] && w.own_bytes[r] >= bytes) && capturing) {
       // hipMalloc (and the wait before a regrowth) cannot be part of a graph
       set_error(UGK_ENOMEM,
                 "workspace: the %s need %zu bytes, which must be allocated before graph capture "
@@ -192,6 +196,7 @@ void *workspace(Region r, size_t bytes, bool *fresh, bool keep_fresh) {
     }
     p = own_region(w, r, bytes);
     if (!p) return nullptr;
+    w.captured[r] = w.captured[r] || capturing;
   }
   if (fresh) {  // the fresh mark is for the region's user, not for ugk_reserve*
     *fresh = w.fresh[r];
