@@ -129,7 +129,7 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
 // What bounds it: on gfx950 a wavefront's matrix instruction holds back the vector
 // instructions of every wavefront on its SIMD (8 x (mfma, 4 fma): 20.2 ns per pair with one
 // wavefront, 18.0 with two, of which the mfma alone takes 14.3), so the two
-// add up. 16,384 rows of 12 heads of 64 take 1,283 us: 321 TFLOP/s of products counted
+// add up. 16,384 rows of 12 heads of 64 take 1,283 us (1,248 to 1,325 from card to card): 321 TFLOP/s of products counted
 // once, 963 of halves. That is 1.67 us for a SIMD's block of 32 rows and 64 keys, of which
 // its 48 mfma take 0.69; the same products in single precision
 // (v_mfma_f32_32x32x2_f32, 128 of 64 cycles) would take 3.7. An earlier state of this kernel
@@ -1108,16 +1108,20 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   __shared__ uint32_t slot[2][5][W];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
   const unsigned pair = blockIdx.x % pairs;
-  const int tile = (int)(blockIdx.x / pairs);  // the keys that the most rows see first
+  // The keys that the most rows see first, their parts one after the other (with the parts
+  // as the slower index the last part's long ones came last: packed 4,095 rows of 16/4
+  // heads 205 us against 187, 4 x 2,048 600 against 548).
+  const int splits = parts.dk ? parts.splits : 1, unit = (int)(blockIdx.x / pairs);
+  const int tile = unit / splits, part_no = unit % splits;
   const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
-  const Seq s = sequence(a, b, hk == 0 && tile == 0 && blockIdx.y == 0, word, UGK_IDS_ATTENTION_BACKWARD);
+  const Seq s = sequence(a, b, hk == 0 && unit == 0, word, UGK_IDS_ATTENTION_BACKWARD);
   const int key0 = tile * (32 * W);
   if (key0 >= s.Lk) return;
   // rows before `from` see none of the workgroup's keys, rows from `all` on all of them
   int from = min(s.first(key0, a.causal), s.Lq) * G / BQ * BQ, rows = s.Lq * G;
   if (parts.dk) {  // this part's rows
     const int per = ((rows - from + parts.splits - 1) / parts.splits + BQ - 1) / BQ * BQ;
-    from = min(from + (int)blockIdx.y * per, rows);
+    from = min(from + part_no * per, rows);
     rows = min(from + per, rows);
   }
   const int all = min(s.first(min(key0 + 32 * W, s.Lk) - 1, a.causal), s.Lq) * G;
@@ -1278,7 +1282,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       __syncthreads();
     }
   }
-  const size_t wk = (size_t)a.NKV * a.HS, part = ((size_t)blockIdx.y * a.rows_k) * wk + hk * a.HS;
+  const size_t wk = (size_t)a.NKV * a.HS, part = (size_t)part_no * a.rows_k * wk + hk * a.HS;
   float *ok = parts.dk ? parts.dk + part : dk + hk * a.HS, *ov = parts.dk ? parts.dv + part : dv + hk * a.HS;
   const size_t ldk = parts.dk ? wk : (size_t)a.ldk, ldv = parts.dk ? wk : (size_t)a.ldv;
   assign = assign || parts.dk;
@@ -1344,9 +1348,11 @@ long long filled(const ugk_attention &a, long long rows, long long most, int gro
 // dk and dv: parts of the rows' range where the keys make too few workgroups to fill
 // the CUs, which hold two workgroups for heads up to 64 and one for larger ones,
 // twice (the heads of a group share their keys: 4 x 2,048 rows of 16/4 heads 769 us
-// whole, 370 in four parts and 13 to add them). A part has four tiles or more, and
-// the parts, which hold all key rows, stay below kSplitKeys
-// keys per CU (attention_backward_bound): a cache of which the sequences are a small part has fewer.
+// whole, 370 in four parts and 13 to add them; up to 16 parts for four times as
+// many workgroups took 203 against 187 us packed, 1,332 against 1,282 for 4 x 2,048 rows
+// of 16/4 heads of 128). A part has four tiles or more, and the parts, which hold all
+// key rows, stay below kSplitKeys keys per CU (attention_backward_bound): a cache of
+// which the sequences are a small part has fewer.
 constexpr long long kSplitKeys = 4 * kTileRows;  // per CU, over all parts and heads
 int dkv_splits(const ugk_attention &a) {
   const long long rows = (long long)a.max_q * (a.NH / a.NKV);
@@ -1480,7 +1486,7 @@ int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout
       parts.splits = splits;
     }
     const auto go = [&](auto kernel) {
-      launch(kernel, dim3(pairs * grid_for((size_t)a.max_k, kTileRows), splits), dim3(kTileThreads), 0, dk, dv, dout, q, k, v,
+      launch(kernel, dim3(pairs * grid_for((size_t)a.max_k, kTileRows) * splits), dim3(kTileThreads), 0, dk, dv, dout, q, k, v,
              lse, dsum, a, parts, pairs, assign, word);
     };
     if (wide) full ? go(k_att_dkv<128, true>) : go(k_att_dkv<128, false>);
