@@ -673,3 +673,11 @@ def test_capture_without_the_workspace_is_refused(gpu):
         gpu.set_stream(None)
     out, lse = c.forward()
     check_forward(c, out, lse)
+
+
+@pytest.mark.parametrize("HS", [65, 68, 80, 96, 100, 124, 126, 127])
+def test_head_sizes_above_64(gpu, HS):
+    c = Call(gpu, Seqs([150, 3, 0, 70], gap=1, tail=2), 4, 2, HS, pad=3, off=1)
+    out, lse = c.forward()
+    check_forward(c, out, lse)
+    check_backward(c, out, lse)

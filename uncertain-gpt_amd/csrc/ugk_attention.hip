@@ -158,9 +158,15 @@ struct Parts {
   int splits, chunk; // keys per part
 };
 
-template <bool kFull>
+// How a kernel reads rows of HS floats, four at a time with nd of them left (0 or less
+// behind the row): every slot is whole (HS is HSP), whole or behind the row (HS a multiple
+// of 4), any.
+enum Slots { kAny, kQuads, kWhole };
+
+template <Slots kSlots>
 __device__ __forceinline__ float4 load4(const float *p, int nd) {
-  if (kFull || nd >= 4) return ld4(p);
+  if (kSlots == kWhole || nd >= 4) return ld4(p);
+  if (kSlots == kQuads) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (nd > 0) v.x = p[0];
   if (nd > 1) v.y = p[1];
@@ -168,19 +174,19 @@ __device__ __forceinline__ float4 load4(const float *p, int nd) {
   return v;
 }
 // Rows j, j + kStep, .. of [0, n): past it, zero (n > 0). tail: some of the tile's rows are.
-template <int kStep, bool kFull>
+template <int kStep, Slots kSlots>
 __device__ __forceinline__ Rows4 load_rows(const float *base, long long ld, int j, int n, bool tail, int nd) {
   Rows4 t;
   if (tail) {
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      t.r[r] = load4<kFull>(base + min(j + kStep * r, n - 1) * ld, nd);
+      t.r[r] = load4<kSlots>(base + min(j + kStep * r, n - 1) * ld, nd);
       if (j + kStep * r >= n) t.r[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
   } else {
     const float *p = base + j * ld;
 #pragma unroll
-    for (int r = 0; r < 4; r++, p += kStep * ld) t.r[r] = load4<kFull>(p, nd);
+    for (int r = 0; r < 4; r++, p += kStep * ld) t.r[r] = load4<kSlots>(p, nd);
   }
   return t;
 }
@@ -200,11 +206,11 @@ __device__ __forceinline__ void put_rows(const Rows4 &t, float scale, _Float16 *
 }
 
 // Eight floats from d on of a row, as operands.
-template <bool kFull>
+template <Slots kSlots>
 __device__ __forceinline__ void load8(const float *p, int d, int HS, bool live, float (&x)[8]) {
 #pragma unroll
   for (int j = 0; j < 2; j++) {
-    const float4 v = live ? load4<kFull>(p + d + 4 * j, HS - d - 4 * j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 v = live ? load4<kSlots>(p + d + 4 * j, HS - d - 4 * j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
   }
 }
@@ -287,7 +293,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     uint32_t m = 0;
 #pragma unroll
     for (int c = 0; c < DC; c++) {
-      load8<kFull>(qr, 16 * c + 8 * half, a.HS, live, x[c]);
+      load8<kFull ? kWhole : kAny>(qr, 16 * c + 8 * half, a.HS, live, x[c]);
 #pragma unroll
       for (int j = 0; j < 8; j++) m = max(m, abs_bits(x[c][j]));
     }
@@ -315,7 +321,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
       const int d = block(u) % DG * 4, j = k0 + block(u) / DG;
-      t[u] = load_rows<KG, kFull>((is_v(u) ? vb : kb) + d, is_v(u) ? a.ldv : a.ldk, j, n, tail, a.HS - d);
+      t[u] = load_rows<KG, kFull ? kWhole : kAny>((is_v(u) ? vb : kb) + d, is_v(u) ? a.ldv : a.ldk, j, n, tail, a.HS - d);
     }
   };
   // The tile's largest magnitudes, of K and V, and where not all rows see all of it
@@ -578,7 +584,7 @@ __global__ __launch_bounds__(NW * kWave) void k_att_few(float *out, float *lse, 
 #pragma unroll
   for (int r = 0; r < R; r++) {
     const int rr = min(r, rows - 1), i = rr / G, h = hk * G + rr % G;
-    qv[r] = load4<kFull>(q + ((size_t)s.q0 + i) * a.ldq + h * a.HS + (nd > 0 ? d : 0), nd);
+    qv[r] = load4<kFull ? kWhole : kAny>(q + ((size_t)s.q0 + i) * a.ldq + h * a.HS + (nd > 0 ? d : 0), nd);
     const float f = a.scale * kLog2e;
     qv[r] = make_float4(qv[r].x * f, qv[r].y * f, qv[r].z * f, qv[r].w * f);
     lim[r] = r < rows ? min(stop, s.seen(i, a.causal)) : first;
@@ -591,9 +597,9 @@ __global__ __launch_bounds__(NW * kWave) void k_att_few(float *out, float *lse, 
   for (int j0 = first + wave * kStep; j0 < n; j0 += NW * kStep) {
     float4 kv[U], vv[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) kv[u] = load4<kFull>(kb + min(j0 + u * kKeys + group, n - 1) * a.ldk, nd);
+    for (int u = 0; u < U; u++) kv[u] = load4<kFull ? kWhole : kAny>(kb + min(j0 + u * kKeys + group, n - 1) * a.ldk, nd);
 #pragma unroll
-    for (int u = 0; u < U; u++) vv[u] = load4<kFull>(vb + min(j0 + u * kKeys + group, n - 1) * a.ldv, nd);
+    for (int u = 0; u < U; u++) vv[u] = load4<kFull ? kWhole : kAny>(vb + min(j0 + u * kKeys + group, n - 1) * a.ldv, nd);
     const auto take = [&](auto masked) {  // masked: not every row sees all of these keys
       constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
@@ -870,14 +876,14 @@ __device__ __forceinline__ bool raise(int &ea, v16f (&acc)[DB], const v16f &ds, 
 }
 
 // A lane's row (HS floats at p) as operands; *e: its exponent. Returns the bits of its largest magnitude.
-template <int DC, bool kFull>
+template <int DC, Slots kSlots>
 __device__ __forceinline__ uint32_t load_operand(const float *p, int HS, bool live, int half, v8h (&h)[DC], v8h (&l)[DC],
                                                  int *e) {
   float x[DC][8];
   uint32_t m = 0;
 #pragma unroll
   for (int c = 0; c < DC; c++) {
-    load8<kFull>(p, 16 * c + 8 * half, HS, live, x[c]);
+    load8<kSlots>(p, 16 * c + 8 * half, HS, live, x[c]);
 #pragma unroll
     for (int j = 0; j < 8; j++) m = max(m, abs_bits(x[c][j]));
   }
@@ -888,7 +894,7 @@ __device__ __forceinline__ uint32_t load_operand(const float *p, int HS, bool li
   return m;
 }
 
-template <int HSP, int BK, bool kFull>
+template <int HSP, int BK, Slots kSlots>
 __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
     float *dq, float *dsum, const float *dout, const float *q, const float *k, const float *v, const float *out,
     const float *lse, ugk_attention a, unsigned pairs, bool assign, int *word) {
@@ -923,15 +929,15 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   const size_t grow = (size_t)s.q0 + i;
   v8h qh[DC], ql[DC], gh[DC], gl[DC];
   int eq, eg;
-  const uint32_t qbits = load_operand<DC, kFull>(q + grow * a.ldq + h * a.HS, a.HS, live, half, qh, ql, &eq);
+  const uint32_t qbits = load_operand<DC, kSlots>(q + grow * a.ldq + h * a.HS, a.HS, live, half, qh, ql, &eq);
   const float *gr = dout + grow * a.ldo + h * a.HS;
-  const uint32_t gbits = load_operand<DC, kFull>(gr, a.HS, live, half, gh, gl, &eg);
+  const uint32_t gbits = load_operand<DC, kSlots>(gr, a.HS, live, half, gh, gl, &eg);
   float D = 0.0f;
 #pragma unroll
   for (int c = 0; c < DC; c++) {
     float x[8], y[8];
-    load8<kFull>(gr, 16 * c + 8 * half, a.HS, live, x);
-    load8<kFull>(out + grow * a.ldo + h * a.HS, 16 * c + 8 * half, a.HS, live, y);
+    load8<kSlots>(gr, 16 * c + 8 * half, a.HS, live, x);
+    load8<kSlots>(out + grow * a.ldo + h * a.HS, 16 * c + 8 * half, a.HS, live, y);
 #pragma unroll
     for (int j = 0; j < 8; j++) D = fmaf(x[j], y[j], D);
   }
@@ -951,7 +957,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
     for (int u = 0; u < kPer; u++) {
       const int d = block(u) % DG * 4, j = k0 + block(u) / DG;
       const bool w = is_v(u);
-      t[u] = load_rows<KG, kFull>((w ? vb : kb) + d, w ? a.ldv : a.ldk, j, n, tail, a.HS - d);
+      t[u] = load_rows<KG, kSlots>((w ? vb : kb) + d, w ? a.ldv : a.ldk, j, n, tail, a.HS - d);
     }
   };
   const auto note = [&](int at) {
@@ -1053,7 +1059,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
     }
     return;
   }
-  if (live) put_scaled<DB, kFull>(dq + grow * a.ldq + h * a.HS, acc, ea - 30, a.scale, half, a.HS, assign);
+  if (live) put_scaled<DB, kSlots == kWhole>(dq + grow * a.ldq + h * a.HS, acc, ea - 30, a.scale, half, a.HS, assign);
 }
 
 // Rows r = (query row r / G, head r % G of the group) of q or dout in tiles of kTile,
@@ -1069,18 +1075,18 @@ struct GroupRows {
     const int i = r / G;
     return base + i * ld + (r - i * G) * HS;
   }
-  template <bool kFull>
+  template <Slots kSlots>
   __device__ __forceinline__ Rows4 load(int r0, const long long (&off)[4], int x, int d, int n, int nd) const {
     Rows4 t;
     if (kTile % G == 0 && r0 + kTile <= n) {
       const float *p = base + r0 / G * ld + d;
 #pragma unroll
-      for (int y = 0; y < 4; y++) t.r[y] = load4<kFull>(p + off[y], nd);
+      for (int y = 0; y < 4; y++) t.r[y] = load4<kSlots>(p + off[y], nd);
     } else {
 #pragma unroll
       for (int y = 0; y < 4; y++) {
         const int r = r0 + x + kStep * y;
-        t.r[y] = load4<kFull>(at(min(r, n - 1)) + d, nd);
+        t.r[y] = load4<kSlots>(at(min(r, n - 1)) + d, nd);
         if (r >= n) t.r[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
     }
@@ -1095,7 +1101,7 @@ struct Halves {
   int splits;
 };
 
-template <int HSP, bool kFull>
+template <int HSP, Slots kSlots>
 __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     float *dk, float *dv, const float *dout, const float *q, const float *k, const float *v, const float *lse,
     const float *dsum, ugk_attention a, Halves parts, unsigned pairs, bool assign, int *word) {
@@ -1140,8 +1146,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   const size_t grow = (size_t)s.k0 + (live ? j : 0);
   v8h kh[DC], kl[DC], vh[DC], vl[DC];
   int ek, ev;
-  const uint32_t kbits = load_operand<DC, kFull>(k + grow * a.ldk + hk * a.HS, a.HS, live, half, kh, kl, &ek);
-  const uint32_t vbits = load_operand<DC, kFull>(v + grow * a.ldv + hk * a.HS, a.HS, live, half, vh, vl, &ev);
+  const uint32_t kbits = load_operand<DC, kSlots>(k + grow * a.ldk + hk * a.HS, a.HS, live, half, kh, kl, &ek);
+  const uint32_t vbits = load_operand<DC, kSlots>(v + grow * a.ldv + hk * a.HS, a.HS, live, half, vh, vl, &ev);
   const float ck = split_unscale(ek) * (a.scale * kLog2e), cv = split_unscale(ev);
   bool bad = kbits >= kInfBits || vbits >= kInfBits;
 
@@ -1164,8 +1170,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
       const int d = block(u) % DG * 4, x = block(u) / DG;
-      t[u] = is_g(u) ? gg.template load<kFull>(r0, off[u], x, d, rows, a.HS - d)
-                     : gq.template load<kFull>(r0, off[u], x, d, rows, a.HS - d);
+      t[u] = is_g(u) ? gg.template load<kSlots>(r0, off[u], x, d, rows, a.HS - d)
+                     : gq.template load<kSlots>(r0, off[u], x, d, rows, a.HS - d);
     }
     if (tid < BQ) {
       const int r = r0 + tid, i = min(r, rows - 1) / G, x = min(r, rows - 1) - i * G;
@@ -1296,8 +1302,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     return;
   }
   if (!live) return;
-  put_scaled<DB, kFull>(ok + grow * ldk, ak, ea - 45, a.scale, half, a.HS, assign);  // dS, like P, was 2^15 up
-  put_scaled<DB, kFull>(ov + grow * ldv, av, eg_acc - 30, 1.0f, half, a.HS, assign);
+  put_scaled<DB, kSlots == kWhole>(ok + grow * ldk, ak, ea - 45, a.scale, half, a.HS, assign);  // dS, like P, was 2^15 up
+  put_scaled<DB, kSlots == kWhole>(ov + grow * ldv, av, eg_acc - 30, 1.0f, half, a.HS, assign);
 }
 
 // The parts' dk and dv added, in the parts' order, a thread per element.
@@ -1467,14 +1473,17 @@ int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout
                               bool assign, int *word) {
   float *dsum = mem;
   const unsigned pairs = (unsigned)a.nseq * a.NKV;
-  const bool wide = a.HS > 64, full = a.HS == (wide ? 128 : 64);
+  // Head sizes of 65 to 127 that are multiples of 4 (80, 96, ..) have kernels of their own: reading
+  // the rows' ends float by float costs dk and dv 352 bytes a lane of spills (4 x 2,048 rows of
+  // 16/4 heads of 100: 1,229 us, 1,699 in the general form, which up to 64 spills nothing).
+  const bool wide = a.HS > 64, full = a.HS == (wide ? 128 : 64), quads = a.HS % 4 == 0;
   if (const long long rows = (long long)a.max_q * (a.NH / a.NKV)) {
     const auto go = [&](auto kernel) {
       launch(kernel, dim3(pairs * grid_for((size_t)rows, kTileRows)), dim3(kTileThreads), 0, dq, dsum, dout, q, k, v, out, lse,
              a, pairs, assign, word);
     };
-    if (wide) full ? go(k_att_dq<128, 32, true>) : go(k_att_dq<128, 32, false>);
-    else full ? go(k_att_dq<64, 64, true>) : go(k_att_dq<64, 64, false>);
+    if (wide) full ? go(k_att_dq<128, 32, kWhole>) : quads ? go(k_att_dq<128, 32, kQuads>) : go(k_att_dq<128, 32, kAny>);
+    else full ? go(k_att_dq<64, 64, kWhole>) : go(k_att_dq<64, 64, kAny>);
     if (int e = check_launch("attention_backward")) return e;
   }
   if (a.max_k) {
@@ -1489,8 +1498,8 @@ int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout
       launch(kernel, dim3(pairs * grid_for((size_t)a.max_k, kTileRows) * splits), dim3(kTileThreads), 0, dk, dv, dout, q, k, v,
              lse, dsum, a, parts, pairs, assign, word);
     };
-    if (wide) full ? go(k_att_dkv<128, true>) : go(k_att_dkv<128, false>);
-    else full ? go(k_att_dkv<64, true>) : go(k_att_dkv<64, false>);
+    if (wide) full ? go(k_att_dkv<128, kWhole>) : quads ? go(k_att_dkv<128, kQuads>) : go(k_att_dkv<128, kAny>);
+    else full ? go(k_att_dkv<64, kWhole>) : go(k_att_dkv<64, kAny>);
     if (splits > 1) {
       if (int e = check_launch("attention_backward")) return e;
       launch(k_att_dkv_join, dim3(a.max_k, grid_for((size_t)a.NKV * a.HS, kBlock), a.nseq), dim3(kBlock), 0, dk, dv, parts, a,
