@@ -681,3 +681,11 @@ def test_head_sizes_above_64(gpu, HS):
     out, lse = c.forward()
     check_forward(c, out, lse)
     check_backward(c, out, lse)
+
+
+@pytest.mark.parametrize("NH,NKV,HS,Q,lens", [(16, 2, 128, 1, [5000, 1, 0, 1025]), (8, 8, 64, 8, [4100, 1024, 7]), (12, 2, 40, 9, [3001, 2047])])
+def test_one_tile_of_rows_against_a_long_cache(gpu, NH, NKV, HS, Q, lens):
+    c = Call(gpu, Seqs([Q] * len(lens), lens, gap=1), NH, NKV, HS)
+    out, lse = c.forward()
+    check_forward(c, out, lse)
+    check_backward(c, out, lse)

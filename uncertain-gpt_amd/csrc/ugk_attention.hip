@@ -542,9 +542,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 // each, 277 with four (1,611 MB, 5.8 to 6.0 TB/s); 64 of 2,048, 12 heads of 64, 144 us (805
 // MB, 5.6 TB/s). On the 32-row tiles 24 of up to 16,384 keys took 993 us, here 413 and
 // 283 with the key axis split. Five to eight rows go to the tiles (24 x 4,096 keys, eight
-// query heads of 64 to each of 8: 91 us; four, here: 81), for here they would spill. Key axes
-// of more than kFewChunk are split also where the workgroups fill the CUs: the
-// lengths differ, and the longest would run alone; where they are equal it costs 1% to 4%.
+// query heads of 64 to each of 8: 102 us; four, here: 81), for here they would spill. The split
+// (fwd_plan) costs 1% to 4% where the lengths are equal.
 template <int kLanes>
 __device__ __forceinline__ float lanes_sum(float v) {
   v += dpp_lane<kDppQuadSwap1>(v);
@@ -1367,7 +1366,7 @@ int dkv_splits(const ugk_attention &a) {
   return (int)max(1LL, min(min(min(want, keys), (long long)kMaxSplits), rows / 128));
 }
 
-constexpr int kFewRows = 4, kFewChunk = 1024;
+constexpr int kFewRows = 4, kFewChunk = 1024;  // rows of k_att_few; keys per part
 constexpr size_t kMaxParts = 1 << 15;  // rows of a head that the parts hold at most
 
 // How the forward of `a` is cut: rows per key/value head where they are few and their
@@ -1396,7 +1395,14 @@ FwdPlan fwd_plan(const ugk_attention &a) {
   p.splits = 1;
   const long long wgs = pairs * p.tiles, prow = (long long)a.nseq * a.max_q * a.NH;
   long long want = (p.few ? 1 : 2) * cu_count() / (wgs > 0 ? wgs : 1);
-  if (p.few) want = max(want, (a.max_k + (long long)kFewChunk - 1) / kFewChunk);
+  // One tile of rows for all of a sequence's keys: parts of kFewChunk keys also where the
+  // workgroups fill the CUs, for a cache's lengths differ and the longest would run alone.
+  // On the 32-row tiles up to 8 of them (64/8 heads: 24 sequences of up to 16,384 keys of
+  // 128 324 us, 525 without and 333 without the limit; 48 of them, of 64, 403, 561 and 411; 24
+  // of 8,192 each 273, 309 and 273. Against it: 24 of 4,096 each, of 64, 102 and 92 without, 32
+  // of up to 4,096 88 and 83).
+  const long long chunks = (a.max_k + (long long)kFewChunk - 1) / kFewChunk;
+  if (p.tiles == 1) want = max(want, p.few ? chunks : min((long long)a.max_k / kFewChunk, 8LL));
   want = min(want, (long long)a.max_k / (4 * unit));
   want = min(want, (long long)kMaxParts / (prow > 0 ? prow : 1));
   if (want > 1) {
