@@ -1,0 +1,171 @@
+"""GPU: the digits of attention's results where the sizes of what goes into them differ: a large value of little weight,
+keys that hardly a row weighs, keys, values, queries and gradients whose size changes from row to row, scores of -infinity.
+
+The bounds, from 64 bits, with u = 2^-24. A row of q, k, v or dout of one head enters products to 2^-23 of each element
+(two 11-bit halves) and 2^-31 of its own largest (a tile is held at one scale only where its rows' largest are within
+2^6 of each other, so a row's largest is 2^7 or more in the halves' units, and 2^-25 the error of a half there); the
+omitted product of the two lower parts is 2^-22 of the product. Sums of HS such products are of 3 HS terms in 32 bits.
+So a score is off by
+
+    es = |scale| ((3 HS + 16) u sum |q k| + HS 2^-29 max|q| max|k|),
+
+its exponential by a factor of es and, for the rounding of the exponent, 4 u (|s| + |lse| + 4) more, and a row's sum of
+them by the mean of that over its weights; weights and results below 2^-126, the least number with 24 bits, by that (a
+product of 2^-105 and 2^-90 is 0 in 32 bits). Weights, and the
+score gradients of the backward, are held to two halves next to the largest contribution (weight times the row's
+largest) that the row or the key sees. In the forward that contribution is 2^14 or more in the halves' units (P of 2^7 or
+more times a value of 2^7 or more at the tile's scale), where another's P is off by 2^-25, times a value below
+2^15: 2^-24 of it for each term, here 2^-23. In the backward the largest P or dS is 2^12 or more, times 2^7: 2^-29, here 2^-28.
+"""
+import math
+
+import pytest
+import torch
+
+import att_ref
+from att_ref import Seqs
+from test_attention_gpu import DEV, Call, inside, rand
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def top(t):
+    return t.abs().amax(-1) if t.shape[0] else t.new_zeros(t.shape[:-1])
+
+
+def results(c, lse=None, out=None):
+    """out, lse, dq, dk, dv in 64 bits with their bounds; the gradients are those of the given out and lse."""
+    s, HS, G = c.s, c.HS, c.NH // c.NKV
+    w = {}
+    for name, t in (("out", c.q), ("lse", c.q[:, :, 0]), ("dq", c.q), ("dk", c.k), ("dv", c.k)):
+        w[name] = (torch.zeros(t.shape, dtype=torch.float64, device=DEV), torch.full(t.shape, 2.0 ** -126, dtype=torch.float64, device=DEV))
+    for b in range(len(s.lq)):
+        for h in range(c.NH):
+            rq, rk, q, k, v = att_ref._pieces(s, b, h, G, c.q, c.k, c.v)
+            n, g = k.shape[0], c.dout[rq, h].double()
+            ok = att_ref.allowed(q.shape[0], n, c.causal, DEV)
+            S = (q @ k.T * c.scale).masked_fill(~ok, -math.inf)
+            es = abs(c.scale) * ((3 * HS + 16) * U * (q.abs() @ k.abs().T) + HS * 2.0 ** -29 * top(q)[:, None] * top(k)[None])
+            L = torch.logsumexp(S, 1)
+            none = L == -math.inf
+            weigh = lambda L: torch.where(S == -math.inf, 0.0, torch.exp(S - torch.where(none, 0.0, L)[:, None]))  # noqa: E731
+            rel = lambda P: torch.where(P > 0, es + 4 * U * (S.abs() + L.abs()[:, None] + 4), 0.0)  # noqa: E731
+            P = weigh(L)
+            r, least = rel(P), 2.0 ** -126 * ok
+            mean = (P * r + least).sum(1)
+            w["out"][0][rq, h] = torch.where(P > 0, P, 0.0) @ torch.where(v.isfinite(), v, 0.0)
+            w["lse"][0][rq, h] = L
+            w["lse"][1][rq, h] += torch.where(none, 0.0, mean + (n + 16) * U + 4 * U * L.abs())
+            biggest = (P * top(v)[None]).amax(1, keepdim=True) if n else 0.0
+            w["out"][1][rq, h] += (P * (r + mean[:, None] + (2 * n + 32) * U) + least) @ v.abs() + \
+                (P @ top(v))[:, None] * 2.0 ** -30 + n * 2.0 ** -23 * biggest
+            if lse is None:
+                continue
+            o, L = out[rq, h].double(), lse[rq, h].double()
+            P = weigh(L)
+            r = rel(P)
+            D, Da = (g * o).sum(1, keepdim=True), (g * o).abs().sum(1, keepdim=True)
+            dP, dPa = g @ v.T, g.abs() @ v.abs().T
+            dS = P * (dP - D) * c.scale
+            eS = abs(c.scale) * least * (dPa + Da) + least + abs(c.scale) * P * ((dP - D).abs() * r + (3 * HS + 24) * U * (dPa + Da) + HS * 2.0 ** -29 * top(g)[:, None] * top(v)[None])
+            nq = q.shape[0] * G
+            for name, rows, X, eX, y in (("dq", (rq, h), dS, eS, k), ("dk", (rk, h // G), dS.T, eS.T, q),
+                                         ("dv", (rk, h // G), P.T, (P * r + least).T, g)):
+                terms = (2 * (n if name == "dq" else nq) + 32) * U
+                size = X.abs() * top(y)[None]
+                w[name][0][rows] += X @ y
+                w[name][1][rows] += (eX + X.abs() * terms) @ y.abs() + size.sum(1, keepdim=True) * 2.0 ** -30 + \
+                    (n if name == "dq" else nq) * 2.0 ** -28 * (size.amax(1, keepdim=True) if size.shape[1] else 0.0)
+    return w
+
+
+def check_forward(c):
+    out, lse = c.forward()
+    w = results(c)
+    inside(out, *w["out"], "out")
+    inside(lse, *w["lse"], "lse")
+
+
+# (query lengths, key lengths, NH, NKV, HS): tiles of 64 and 32 keys, ragged heads, groups, a split key axis, few rows
+SHAPES = [([40], [512], 2, 2, 64), ([300], None, 1, 1, 64), ([40], [512], 2, 1, 128), ([70, 33], None, 4, 1, 50), ([12], [3000], 2, 2, 64),
+          ([130], None, 2, 2, 100), ([1, 3], [512, 70], 2, 2, 64), ([50], [200], 3, 3, 4)]
+
+
+def large_value(gpu, size, lq, lk, NH, NKV, HS):
+    """Key 5 has a weight near e^-80 or less in every row, and a value `size` times the others."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)
+    c.q[:, :, 0] = 80.0 ** 0.5 / c.scale ** 0.5
+    for k0 in c.s.k:
+        c.k[k0 + 5, :, 0] = -(80.0 ** 0.5) / c.scale ** 0.5
+        c.v[k0 + 5] *= size
+    return c
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("size", [2.0 ** 12, 1e6, 1e10, 1e20])
+def test_a_large_value_of_little_weight(gpu, size, lq, lk, NH, NKV, HS):
+    check_forward(large_value(gpu, size, lq, lk, NH, NKV, HS))
+
+
+@pytest.mark.parametrize("first", [0, 5, 200])
+def test_a_large_value_of_little_weight_two_blocks_a_wavefront(gpu, first):
+    """As above where the call has so many rows that a wavefront takes two blocks of them."""
+    c = Call(gpu, Seqs([40], [300]), 768, 768, 64)
+    c.q[:, :, 0] = 80.0 ** 0.5 / c.scale ** 0.5
+    c.k[first, :, 0] = -(80.0 ** 0.5) / c.scale ** 0.5
+    c.v[first] *= 1e9
+    out, _ = c.forward()
+    c.NH = c.NKV = 8
+    c.q, c.k, c.v, c.dout = (t[:, :8] for t in (c.q, c.k, c.v, c.dout))
+    inside(out[:, :8], *results(c)["out"], "out")
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+def test_a_large_key_that_is_not_chosen(gpu, lq, lk, NH, NKV, HS):
+    """A key 1e12 times the others whose score is far below theirs."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)
+    c.q[:, :, 0] = 4.0
+    for k0 in c.s.k:
+        c.k[k0 + 7] *= 2.0
+        c.k[k0 + 7, :, 0] = -1e12
+    check_forward(c)
+
+
+def by_row(c, spread, seed, which):
+    """Rows of the tensors named in `which` times 2^e, e drawn from [-spread, spread] for each row."""
+    g = torch.Generator().manual_seed(seed)
+    for name in which:
+        t = getattr(c, name)
+        t.copy_(torch.ldexp(t, torch.randint(-spread, spread + 1, (t.shape[0], 1, 1), generator=g).to(DEV)))
+
+
+SPREADS = [(8, "q k"), (4, "v dout"), (8, "v dout"), (20, "v dout"), (45, "v"), (45, "dout"), (6, "k v dout")]
+
+
+def spread_rows(gpu, spread, which, lq, lk, NH, NKV, HS):
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS, scale=HS ** -0.5 * (2.0 ** -spread if "k" in which else 1.0))
+    by_row(c, spread, spread, which.split())
+    return c
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("spread,which", SPREADS)
+def test_sizes_that_change_from_row_to_row(gpu, spread, which, lq, lk, NH, NKV, HS):
+    check_forward(spread_rows(gpu, spread, which, lq, lk, NH, NKV, HS))
+
+
+def large_blocks(gpu, seed):
+    """Blocks of keys whose values, and scores, grow, shrink or alternate by large factors: what the sums stand on moves."""
+    c = Call(gpu, Seqs([37], [700]), 2, 1, 64)
+    at = torch.arange(700, device=DEV) // 32
+    e = ((at * 3) % 23 if seed == 0 else 40 - 2 * at if seed == 1 else 40 * (at % 2)).clamp(-60, 60)
+    c.v.copy_(torch.ldexp(c.v, e[:, None, None]))
+    c.q[:, :, 0] = 8.0
+    c.k[:, :, 0] = (at * (1, 3, 0)[seed] - 20).float()[:, None]
+    return c
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_largest_values_first_last_and_between(gpu, seed):
+    check_forward(large_blocks(gpu, seed))

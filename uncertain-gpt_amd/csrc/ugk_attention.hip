@@ -115,16 +115,18 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
 // Products are split (ugk_split.h). K and V are split while they are put into LDS, by the
 // exponent of the tile's largest magnitude; that is taken over the registers that
 // the tile was loaded into, one tile ahead, and goes through LDS with the barrier
-// that the tile buffers need anyway: one barrier per tile. A row's output stands on
-// the largest exponent of the tiles that it has seen, and its P are taken that much
-// lower where a tile lies below it (in the exponent, which costs nothing), so that what a row
-// must not see moves neither.
+// that the tile buffers need anyway: one barrier per tile. Where a tile's keys, or values, lie
+// further apart than 2^kSpread, each is split by its own exponent (lift_rows), and the
+// scores, or P, are taken that much lower: two passes over a lane's 16 registers more per block.
+//
+// A row's P go into the second product next to the largest contribution that the row
+// has seen, that is P times the largest of V's row (of its tile, where the tile has one
+// scale), not next to the largest P or the largest V: a large value of little weight
+// leaves the others their digits, and what a row must not see moves nothing.
 //
 // The workgroup's rows are taken one by one instead (row_forward), where a masked key
-// is not touched at all, if a tile holds an infinity, or NaN that not all rows see;
-// if not all rows see all of a tile and its keys' magnitudes lie further apart
-// than the halves' digits allow (too_wide); or if scores leave the range of the
-// above (2^22 in base 2).
+// is not touched at all, if a tile holds an infinity, or NaN that not all rows see,
+// or if scores leave the range of the above (2^22 in base 2).
 //
 // What bounds it: on gfx950 a wavefront's matrix instruction holds back the vector
 // instructions of every wavefront on its SIMD (8 x (mfma, 4 fma): 20.2 ns per pair with one
@@ -140,9 +142,13 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
 // (1,604 against 1,539); of those workgroups two per CU, with 128 registers a lane (spills:
 // 562 against 470 us for 8,192 rows).
 //
-// A row's P are scaled to 2^kTop at the maximum that they stand on, which moves
-// (and the accumulators with it) only when a score lies 2^7 above it: P then stays
+// A row's P are scaled to 2^kTop at the largest that they stand on, which moves
+// (and the accumulators with it) only when one lies 2^7 above it: P then stays
 // below 2^(kTop + 7), the halves' range.
+//
+// 8 x 1,024 rows of 12 heads of 64 whose values are of one size take 64 us, and 100 us where they are
+// times 2^-8 to 2^8 from row to row; 13 packed sequences of 16/4 heads of 128 121 and 183. (Looking for such rows costs
+// 1 to 2% where there are none; row by row the two took 25.9 and 54.5 ms.)
 constexpr float kTop = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -250,6 +256,54 @@ __device__ __forceinline__ uint32_t noted(const uint32_t (&slot)[W]) {
   return (uint32_t)__builtin_amdgcn_readfirstlane(m);
 }
 
+// Exponents that rows of the two tiles in LDS were lifted by (lift_rows), of two operands. All are zero but those of
+// wavefronts whose byte of `by` is set, which take back what they set.
+template <int kRows>
+struct Lifts {
+  static_assert(kTileWaves == 4, "one word of bytes");
+  __attribute__((aligned(16))) int d[2][2][kRows];
+  __attribute__((aligned(4))) uint8_t by[2][kTileWaves];
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < 4 * kRows; i += kTileThreads) d[i / (2 * kRows)][i / kRows % 2][i % kRows] = 0;
+    if (threadIdx.x < 2 * kTileWaves) by[threadIdx.x / kTileWaves][threadIdx.x % kTileWaves] = 0;
+  }
+  __device__ __forceinline__ uint32_t any(int z) const { return *reinterpret_cast<const uint32_t *>(by[z]); }
+  // those of rows 32 w + 8 x + 4 half .. + 3 of operand o
+  __device__ __forceinline__ int4 four(int z, int o, int w, int x, int half) const {
+    return *reinterpret_cast<const int4 *>(&d[z][o][32 * w + 8 * x + 4 * half]);
+  }
+};
+__device__ __forceinline__ int part4(const int4 &v, int d) { return d == 0 ? v.x : d == 1 ? v.y : d == 2 ? v.z : v.w; }
+// A block's scores (or what comes of them) times 2^d of their rows.
+template <int kRows>
+__device__ __forceinline__ void lower(v16f &c, const Lifts<kRows> &l, int z, int o, int w, int half, int more = 0) {
+#pragma unroll
+  for (int x = 0; x < 4; x++) {
+    const int4 d = l.four(z, o, w, x, half);
+#pragma unroll
+    for (int y = 0; y < 4; y++) c[4 * x + y] = ldexpf(c[4 * x + y], part4(d, y) + more);
+  }
+}
+
+// The rows of a wavefront's blocks lifted, and what they were lifted by noted for tile z, where one of them
+// lies far below its tile's largest; bit z of *lifted: this was so. operand(u), exponent(u) and first(u): a block's.
+template <int DG, int kStep, int kPer, int kRows, typename Operand, typename Exponent, typename First>
+__device__ __forceinline__ void lift_tile(Rows4 (&t)[kPer], Lifts<kRows> &l, int z, int lane, int wave, int *lifted,
+                                          Operand operand, Exponent exponent, First first) {
+  bool any = false;
+#pragma unroll
+  for (int u = 0; u < kPer; u++) {
+    int d[4];
+    any = lift_rows<DG>(t[u], exponent(u), d) || any;
+    if (lane % DG == 0) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) l.d[z][operand(u)][first(u) + kStep * r] = d[r];
+    }
+  }
+  if (lane == 0) l.by[z][wave] = any;
+  *lifted = (*lifted & ~(1 << z)) | (int)any << z;
+}
+
 template <int HSP, int BK, int QB, bool kFull>
 __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *lse, const float *q, const float *k,
                                                              const float *v, ugk_attention a, Parts parts, unsigned pairs,
@@ -259,8 +313,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   static_assert(kPer >= 1 && kBlocks % kWave == 0, "whole wavefronts of K or V blocks");
   constexpr int kRs = HSP + 8, KG = BK / 4;  // halves a row: an odd multiple of 16 bytes, free of bank conflicts
   __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kRs], lv[2][2][BK * kRs];
-  __shared__ uint32_t slot[2][4][W];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
+  __shared__ uint32_t slot[2][2][W];
+  __shared__ Lifts<BK> lifts;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const unsigned pair = blockIdx.x % pairs;
   const int tile = (int)(gridDim.x / pairs - 1 - blockIdx.x / pairs);  // the longest rows first
   const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
@@ -324,36 +379,38 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
       t[u] = load_rows<KG, kFull ? kWhole : kAny>((is_v(u) ? vb : kb) + d, is_v(u) ? a.ldv : a.ldk, j, n, tail, a.HS - d);
     }
   };
-  // The tile's largest magnitudes, of K and V, and where not all rows see all of it
-  // the least of the keys' largest.
+  // The tile's largest magnitudes, of K and V; where not all rows see all of it NaN counts as one.
+  uint32_t small[kPer];
   const auto note = [&](int at, int k0) {
-    uint32_t m[4] = {};
-    if (k0 + BK > least) {
+    uint32_t m[2] = {};
 #pragma unroll
-      for (int u = 0; u < kPer; u++) {
-        m[is_v(u) ? 1 : 0] = max_abs<true>(m[is_v(u) ? 1 : 0], t[u]);
-        m[is_v(u) ? 3 : 2] = least_row<DG>(m[is_v(u) ? 3 : 2], t[u]);
-      }
-      m[2] = wave_max_bits(m[2]);
-      m[3] = wave_max_bits(m[3]);
-    } else {  // a NaN that every row sees is every row's result, as it comes
-#pragma unroll
-      for (int u = 0; u < kPer; u++) m[is_v(u) ? 1 : 0] = max_abs<false>(m[is_v(u) ? 1 : 0], t[u]);
+    for (int u = 0; u < kPer; u++) {
+      const int w = is_v(u) ? 1 : 0;
+      m[w] = max_abs(m[w], t[u], &small[u]);
+      if (!kFull && a.HS <= block(u) % DG * 4) small[u] = kInfBits;  // behind the row
+      if (k0 + BK > least) m[w] = max_abs<true>(m[w], t[u]);  // else a NaN is every row's result, as it comes
     }
     m[0] = wave_max_bits(m[0]);
     m[1] = wave_max_bits(m[1]);
     if (lane == 0) {
-#pragma unroll
-      for (int x = 0; x < 4; x++) slot[at][x][wave] = m[x];
+      slot[at][0][wave] = m[0];
+      slot[at][1][wave] = m[1];
     }
   };
   int ek_next = 0, ev_next = 0;  // of the tile staged last
+  int lifted = 0;                // bit z: this wavefront's rows of tile z are
   const auto stage = [&](int at) {
     const uint32_t mk = noted<W>(slot[at][0]), mv = noted<W>(slot[at][1]);
-    bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted<W>(slot[at][2])) || too_wide(mv, noted<W>(slot[at][3]));
+    bad = bad || mk >= kInfBits || mv >= kInfBits;
     ek_next = split_exp(mk);
     ev_next = split_exp(mv);
     const float fk = split_scale(ek_next), fv = split_scale(ev_next);
+    bool spread = false;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) spread = spread || may_spread(small[u], is_v(u) ? mv : mk);
+    if (__builtin_expect(__any(spread) || (lifted >> at & 1), 0))
+      lift_tile<DG, KG>(t, lifts, at, lane, wave, &lifted, [&](int u) { return is_v(u) ? 1 : 0; },
+                        [&](int u) { return is_v(u) ? ev_next : ek_next; }, [&](int u) { return block(u) / DG; });
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
       const int p = block(u) / DG * kRs + block(u) % DG * 4;
@@ -361,40 +418,26 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     }
   };
 
+  // What the row's sums stand on, whole numbers: l on P 2^one, o on P V 2^all, V's scale included. Both are such that the
+  // largest that the row has seen (of its P; of P times the largest of V's row or tile) comes to 2^kTop, or
+  // up to 2^7 above. They only fall.
   v16f o[QB][DB] = {};
-  float l[QB] = {}, bias[QB];  // bias: kTop - the maximum that the row's P stand on
-  int ev[QB];  // the exponent that o stands on: the largest of the tiles that the row has seen
+  float l[QB] = {}, one[QB], all[QB];
 #pragma unroll
-  for (int u = 0; u < QB; u++) {
-    bias[u] = INFINITY;
-    ev[u] = -100;
-  }
+  for (int u = 0; u < QB; u++) one[u] = all[u] = 3.4028234663852886e38f;
   const int vcols = cols_at(lane, kRs);
   const auto compute = [&](int at, int k0, int ek, int ev_now) {
-    const float uk = split_unscale(ek);
-    float c2[QB], up[QB], down[QB];  // P is taken times 2^up, up <= 0, where the row has seen larger values
-    int was[QB];
-    bool changed = false;
+    const float uk = split_unscale(ek), ev = (float)ev_now;
+    const uint32_t lifted_by = lifts.any(at);
+    bool apart = false;
+    float c2[QB], b0[QB];  // P is taken times 2^b0 to be an operand
+    const auto stand = [&](int u) {
+      b0[u] = apart ? one[u] : fmaxf(all[u] + ev, one[u] - 100.0f);
+    };
 #pragma unroll
     for (int u = 0; u < QB; u++) {
       c2[u] = fmaxf(cq[u] * uk, 0x1p-126f);
       bad = bad || c2[u] > 0x1p100f;
-      was[u] = ev[u];
-      if (lim[u] > k0) ev[u] = max(ev[u], ev_now);
-      changed = changed || ev[u] != was[u];
-      const int shift = max(min(ev_now - ev[u], 0), -100);
-      up[u] = (float)shift;
-      down[u] = pow2(-shift);
-    }
-    if (__any(changed)) {
-#pragma unroll
-      for (int u = 0; u < QB; u++) {
-        const float f = pow2(max(was[u] - ev[u], -126));
-#pragma unroll
-        for (int x = 0; x < DB; x++)
-#pragma unroll
-          for (int y = 0; y < 16; y++) o[u][x][y] *= f;
-      }
     }
 #pragma unroll
     for (int w = 0; w < KB; w++) {  // 32 keys
@@ -406,6 +449,15 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 #pragma unroll
         for (int u = 0; u < QB; u++) sc[u] = mfma3(fh, fl, qh[u][c], ql[u][c], sc[u]);
       }
+      if (w == 0) {
+        apart = __builtin_amdgcn_readfirstlane(lifted_by) != 0;
+#pragma unroll
+        for (int u = 0; u < QB; u++) stand(u);
+      }
+      if (apart) {
+#pragma unroll
+        for (int u = 0; u < QB; u++) lower(sc[u], lifts, at, 0, w, half);
+      }
       if (k0 + 32 * w + 32 > lo) {  // some row does not see all of the keys
 #pragma unroll
         for (int u = 0; u < QB; u++) {
@@ -416,23 +468,36 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
         }
       }
       float m[QB];
-      bool grown = false;
+      bool grown = apart;
 #pragma unroll
       for (int u = 0; u < QB; u++) {
         m[u] = sc[u][0];
 #pragma unroll
         for (int y = 1; y < 16; y++) m[u] = fmaxf(m[u], sc[u][y]);
         m[u] = half_max(m[u]) * c2[u];
-        grown = grown || m[u] + bias[u] > kTop + 7.0f;
+        grown = grown || m[u] + fmaxf(one[u], b0[u]) > kTop + 7.0f;
       }
       if (__any(grown)) {
 #pragma unroll
         for (int u = 0; u < QB; u++) {
           bad = bad || (fabsf(m[u]) >= 0x1p22f && m[u] != -INFINITY);
-          const float old = bias[u];
-          bias[u] = fminf(old, kTop - m[u]);
-          const float f = old == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(bias[u] - old);
-          l[u] *= f;
+          float a = m[u];  // of P times V
+          if (apart) {
+            a = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+              const int4 d = lifts.four(at, 1, w, x, half);
+#pragma unroll
+              for (int y = 0; y < 4; y++) a = fmaxf(a, fmaf(sc[u][4 * x + y], c2[u], (float)part4(d, y)));
+            }
+            a = half_max(a);
+          }
+          const float was = one[u], before = all[u];
+          one[u] = fminf(was, kTop - ceilf(m[u]));
+          all[u] = fminf(before, kTop - ceilf(a) - ev);
+          stand(u);
+          l[u] *= __builtin_amdgcn_exp2f(one[u] - was);
+          const float f = __builtin_amdgcn_exp2f(all[u] - before);
 #pragma unroll
           for (int x = 0; x < DB; x++)
 #pragma unroll
@@ -441,14 +506,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
       }
 #pragma unroll
       for (int u = 0; u < QB; u++) {
-        const float b0 = (bias[u] == INFINITY ? 0.0f : bias[u]) + up[u];  // no key so far: every score is -inf
         float sum = 0.0f;
 #pragma unroll
         for (int y = 0; y < 16; y++) {
-          sc[u][y] = __builtin_amdgcn_exp2f(fmaf(sc[u][y], c2[u], b0));
+          sc[u][y] = __builtin_amdgcn_exp2f(fmaf(sc[u][y], c2[u], b0[u]));
           sum += sc[u][y];
         }
-        l[u] = fmaf(sum, down[u], l[u]);
+        l[u] += ldexpf(sum, (int)(one[u] - b0[u]));
+        if (apart) lower(sc[u], lifts, at, 1, w, half, (int)(all[u] + ev - one[u]));
       }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
@@ -472,6 +537,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   };
 
   const int tiles = (n - first + BK - 1) / BK;
+  lifts.clear();
   if (tiles > 0) {
     load(first);
     note(0, first);
@@ -516,9 +582,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     const float sum = half_sum(l[u]);
     const bool some = lim[u] > first;
     put_row<DB, kFull>(parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS, o[u],
-                       some ? split_unscale(ev[u]) / sum : 0.0f, half, a.HS, true);
+                       some ? pow2((int)(one[u] - all[u]) - 15) / sum : 0.0f, half, a.HS, true);
     if (half == 0 && (parts.o || lse)) {
-      const float L = some ? (__builtin_amdgcn_logf(sum) - bias[u]) * kLn2 : -INFINITY;
+      const float L = some ? (__builtin_amdgcn_logf(sum) - one[u]) * kLn2 : -INFINITY;
       if (parts.o) parts.lse[prow] = L;
       else lse[grow * a.NH + h] = L;
     }
@@ -795,8 +861,9 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
 // atomics would save the second S and dP, 4 of 14 HS operations per pair).
 // P = exp(S - lse) needs no running maximum. A lane holds one row (dq) or one key (dk, dv)
 // as it holds a row in the forward, the other side goes through LDS in tiles, and
-// what its accumulators stand on follows what it has seen alone. The same tiles as
-// in the forward fall back to single rows.
+// what its accumulators stand on follows what it has seen alone. Rows are taken one by one
+// instead for the reasons of the forward, and where not all rows (keys) see all of a tile and its
+// magnitudes lie further apart than the halves' digits allow (too_wide).
 //
 // The same sum of matrix and vector instructions bounds them: of 858 (dk, dv) and 633 us
 // (dq) at 4 x 4,096 rows of 12 heads, 612 and 465 were left without loading,

@@ -193,5 +193,38 @@ __device__ __forceinline__ bool too_wide(uint32_t largest, uint32_t least) {
   return least && (largest >> 23) > (~least >> 23) + 12;
 }
 
+// The largest magnitude's bits, NaN passed over, and in *least those of the smallest of the rows' four-element
+// largest: a row that lies far below the tile's largest has such four elements (others may have them too).
+__device__ __forceinline__ uint32_t max_abs(uint32_t m, const Rows4 &t, uint32_t *least) {
+  float f = __uint_as_float(m), q[4];
+#pragma unroll
+  for (int r = 0; r < 4; r++) q[r] = fmaxf(fmaxf(fabsf(t.r[r].x), fabsf(t.r[r].y)), fmaxf(fabsf(t.r[r].z), fabsf(t.r[r].w)));
+  f = fmaxf(fmaxf(f, q[0]), q[1]);
+  *least = __float_as_uint(fminf(fminf(q[0], q[1]), fminf(q[2], q[3])));
+  return __float_as_uint(fmaxf(fmaxf(f, q[2]), q[3]));
+}
+// A tile is held at the scale of its largest magnitude where its rows' largest are within 2^kSpread of that, else
+// rows are taken times 2^-d, d <= 0, to the largest's binade, and d goes along with the tile.
+constexpr int kSpread = 6;
+__device__ __forceinline__ bool may_spread(uint32_t least, uint32_t largest) { return least + ((uint32_t)kSpread << 23) < largest; }
+// The wavefront's rows, kLanes lanes to four of them, in a tile of exponent e; whether one of them lies that far below.
+template <int kLanes>
+__device__ __forceinline__ bool lift_rows(Rows4 &t, int e, int (&d)[4]) {
+  bool below = false;
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const uint32_t x = row_max_bits<kLanes>(max_abs(0u, t.r[r]));
+    d[r] = x ? min(split_exp(x) - e, 0) : 0;  // rows of zeros stay
+    below = below || d[r] < -kSpread;
+  }
+  below = __any(below);
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    if (!below) d[r] = 0;
+    t.r[r] = make_float4(ldexpf(t.r[r].x, -d[r]), ldexpf(t.r[r].y, -d[r]), ldexpf(t.r[r].z, -d[r]), ldexpf(t.r[r].w, -d[r]));
+  }
+  return below;
+}
+
 }  // namespace
 }  // namespace ugk
