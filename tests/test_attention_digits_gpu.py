@@ -169,3 +169,25 @@ def large_blocks(gpu, seed):
 @pytest.mark.parametrize("seed", range(3))
 def test_largest_values_first_last_and_between(gpu, seed):
     check_forward(large_blocks(gpu, seed))
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+def test_scores_that_overflow_to_minus_infinity(gpu, lq, lk, NH, NKV, HS):
+    """Finite queries and keys whose every product is beyond the range: out 0, lse -infinity, gradients 0."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)
+    c.q[:] = 2.0 ** 64
+    c.k[:] = -(2.0 ** 64)
+    out, lse = c.forward()
+    assert out.eq(0).all() and (lse == -math.inf).all()
+    g = c.grads(2.0)
+    c.backward(out, lse, g, zeroed=True)
+    assert all(x.eq(0).all() for x in g)
+    # from some key on: the rows hold what the keys before them give
+    n0 = min(c.s.lk) // 2
+    c.q[:], c.k[:] = 2.0 ** 60, -(2.0 ** 66)
+    for k0 in c.s.k:
+        c.k[k0:k0 + n0] = rand(torch.Generator(device=DEV).manual_seed(5), n0, NKV, HS) * 2.0 ** -62
+    out, lse = c.forward()
+    c.k.clamp_(min=-(2.0 ** 20))  # in 64 bits: scores far below
+    w = results(c)
+    inside(out, *w["out"], "out")

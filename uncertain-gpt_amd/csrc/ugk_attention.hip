@@ -558,6 +558,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
       __syncthreads();
     }
   }
+  // a row all of whose scores passed the range downwards: what it stands on never moved
+#pragma unroll
+  for (int u = 0; u < QB; u++) bad = bad || (lim[u] > first && one[u] > 1e38f);
   // Any wavefront's trouble with a tile is every wavefront's; with its scores its own.
   if (__any(bad)) {
     for (int x = 0; x < 32 * QB; x++) {
