@@ -191,3 +191,37 @@ def test_scores_that_overflow_to_minus_infinity(gpu, lq, lk, NH, NKV, HS):
     c.k.clamp_(min=-(2.0 ** 20))  # in 64 bits: scores far below
     w = results(c)
     inside(out, *w["out"], "out")
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("masked", ["all", "late"])
+def test_scores_of_the_lowest_value(gpu, masked, lq, lk, NH, NKV, HS):
+    """Keys masked by scores of the type's lowest value: they weigh nothing beside others, and among themselves the same
+    (what else a score holds is far below its last bit)."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS, scale=1.0)
+    c.q[:, :, 0] = 1.0
+    lowest = -3.4028234663852886e38
+    for k0, n in zip(c.s.k, c.s.lk):
+        c.k[k0 if masked == "all" else k0 + n // 2:k0 + n, :, 0] = lowest
+    out, lse = c.forward()
+    for b in range(len(c.s.lq)):
+        for h in range(NH):
+            rq, rk, q, k, v = att_ref._pieces(c.s, b, h, NH // NKV, c.q, c.k, c.v)
+            n = k.shape[0]
+            ok = att_ref.allowed(q.shape[0], n, True, DEV)
+            seen = ok.sum(1, keepdim=True)
+            if masked == "all":
+                # a mean of n values: n + 4 roundings of the sum of their sizes, the weights' 2^-22, and 2^-23 of the largest
+                want, size = ok.double() @ v / seen, ok.double() @ v.abs() / seen
+                inside(out[rq, h], want, size * (n + 64) * U + 2.0 ** -22 * v.abs().amax(), "out")
+                assert (lse[rq, h] == lowest).all()
+            else:
+                few = ok[:, :n // 2]
+                S = (q @ k[:n // 2].T).masked_fill(~few, -math.inf)
+                es = (3 * HS + 16) * U * (q.abs() @ k[:n // 2].abs().T) + HS * 2.0 ** -29 * top(q)[:, None] * top(k[:n // 2])[None]
+                P = torch.softmax(S, 1)
+                rel = 2 * es.amax(1, keepdim=True) + 16 * U * (S.masked_fill(~few, 0.0).abs().amax(1, keepdim=True) + 4)
+                want, size = P @ v[:n // 2], P @ v[:n // 2].abs()
+                # e^x - 1 for the relative error x of a weight, which may pass 1 where scores are in the hundreds
+                tol = size * (torch.expm1(rel) + (2 * n + 32) * U) + n * 2.0 ** -23 * (P * top(v[:n // 2])[None]).amax(1, keepdim=True)
+                inside(out[rq, h], want, tol + 2.0 ** -29 * v.abs().amax(), "out")

@@ -72,8 +72,8 @@ __device__ __forceinline__ void put(float *p, float x, bool assign) { *p = assig
 __device__ __forceinline__ float weight(float s, float m) { return s == -INFINITY ? 0.0f : expf(s - m); }
 
 // One query row of one head by one wavefront: lanes over keys for the scores,
-// over channels for the sum.
-__device__ void row_forward(float *out, float *lse, const float *q, const float *k, const float *v, int n, int HS,
+// over channels for the sum. To lse, or the maximum and the sum behind it to ml (if not null) and ml[ml_step].
+__device__ void row_forward(float *out, float *lse, float *ml, size_t ml_step, const float *q, const float *k, const float *v, int n, int HS,
                             long long ldk, long long ldv, float scale) {
   const int lane = threadIdx.x & (kWave - 1);
   float m = -INFINITY;
@@ -95,7 +95,12 @@ __device__ void row_forward(float *out, float *lse, const float *q, const float 
   const float r = none ? 1.0f : l;
   if (lane < HS) out[lane] = none ? 0.0f : o0 / r;
   if (lane + kWave < HS) out[lane + kWave] = none ? 0.0f : o1 / r;
-  if (lse && lane == 0) *lse = none ? -INFINITY : m + logf(l);
+  if (lane == 0 && ml) {
+    ml[0] = none ? -INFINITY : m;
+    ml[ml_step] = l;
+  } else if (lane == 0 && lse) {
+    *lse = none ? -INFINITY : m + logf(l);
+  }
 }
 
 // ---- forward, tiles on the matrix units -----------------------------------------
@@ -158,9 +163,10 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417
 // against 29.5, their backward 173 against 96).
 constexpr int kTileWaves = 4, kTileThreads = kTileWaves * kWave, kTileRows = 32 * kTileWaves;
 
-// One part of a split key axis: o normalised, and lse, per row.
+// One part of a split key axis: o normalised, its scores' maximum (or a number near it) m and the sum l of e^(s - m), per
+// row. (m + log l in one number would lose l where m is large: a mask's lowest value.)
 struct Parts {
-  float *o, *lse;    // null: not split
+  float *o, *m, *l;  // null: not split
   int splits, chunk; // keys per part
 };
 
@@ -570,8 +576,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
       const size_t g = (size_t)s.q0 + ii;
       const int upto = min(n, s.seen(ii, a.causal));
       const size_t prow = (((size_t)blockIdx.y * a.nseq + b) * a.max_q + ii) * a.NH + hh;
-      row_forward(parts.o ? parts.o + prow * a.HS : out + g * a.ldo + hh * a.HS,
-                  parts.o ? parts.lse + prow : lse ? lse + g * a.NH + hh : nullptr, q + g * a.ldq + hh * a.HS,
+      row_forward(parts.o ? parts.o + prow * a.HS : out + g * a.ldo + hh * a.HS, lse ? lse + g * a.NH + hh : nullptr,
+                  parts.o ? parts.m + prow : nullptr, parts.l - parts.m, q + g * a.ldq + hh * a.HS,
                   kb + first * a.ldk, vb + first * a.ldv, max(upto - first, 0), a.HS, a.ldk, a.ldv, a.scale);
     }
     return;
@@ -587,9 +593,12 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     put_row<DB, kFull>(parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS, o[u],
                        some ? pow2((int)(one[u] - all[u]) - 15) / sum : 0.0f, half, a.HS, true);
     if (half == 0 && (parts.o || lse)) {
-      const float L = some ? (__builtin_amdgcn_logf(sum) - one[u]) * kLn2 : -INFINITY;
-      if (parts.o) parts.lse[prow] = L;
-      else lse[grow * a.NH + h] = L;
+      if (parts.o) {
+        parts.m[prow] = some ? -one[u] * kLn2 : -INFINITY;
+        parts.l[prow] = some ? sum : 0.0f;
+      } else {
+        lse[grow * a.NH + h] = some ? (__builtin_amdgcn_logf(sum) - one[u]) * kLn2 : -INFINITY;
+      }
     }
   }
 }
@@ -605,7 +614,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 // between groups until the end); its score sums go through DPP. The groups, then the
 // workgroup's NW wavefronts, are joined at the end in their order, through LDS.
 // Single precision throughout, and a key that a row must not see is left out by
-// selects, so nothing of it reaches the row.
+// selects, so nothing of it reaches the row. A row whose scores all leave the range in base 2 (or hold a NaN, or an infinity)
+// is computed by row_forward.
 //
 // 24 sequences of 8,192 keys, 8 key/value heads of 128: 271 us with one query head for
 // each, 277 with four (1,611 MB, 5.8 to 6.0 TB/s); 64 of 2,048, 12 heads of 64, 144 us (805
@@ -726,8 +736,12 @@ __global__ __launch_bounds__(NW * kWave) void k_att_few(float *out, float *lse, 
   }
   __syncthreads();
   // the wavefronts, kLanes threads per row
-  for (int x = threadIdx.x; x < min(R, rows) * kLanes; x += NW * kWave) {
-    const int r = x / kLanes, at = x % kLanes;
+  static_assert(R * kLanes <= NW * kWave, "a thread has one row at most");
+  bool lost = false;  // scores beyond the range in base 2
+  const int r = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
+  const int i = r / G, h = hk * G + r % G;
+  const size_t prow = ((size_t)part * a.nseq + b) * a.max_q + i, grow = (size_t)s.q0 + i;
+  if (r < min(R, rows)) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; w++) top = fmaxf(top, lm[w][r]);
@@ -741,22 +755,33 @@ __global__ __launch_bounds__(NW * kWave) void k_att_few(float *out, float *lse, 
       sum = fmaf(ll[w][r], f, sum);
       t = make_float4(fmaf(y.x, f, t.x), fmaf(y.y, f, t.y), fmaf(y.z, f, t.z), fmaf(y.w, f, t.w));
     }
-    const int i = r / G, h = hk * G + r % G;
-    const bool any = sum != 0.0f;  // else no key, or every score -infinity
-    const float f = any ? 1.0f / sum : 0.0f, L = any ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
+    lost = !(sum > 0.0f) && min(stop, s.seen(i, a.causal)) > first;
+    const bool any = sum != 0.0f;  // else no key
+    const float f = any ? 1.0f / sum : 0.0f;
     t = any ? make_float4(t.x * f, t.y * f, t.z * f, t.w * f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const size_t prow = ((size_t)part * a.nseq + b) * a.max_q + i, grow = (size_t)s.q0 + i;
     float *po = parts.o ? parts.o + prow * a.NH * a.HS + (size_t)h * a.HS : out + grow * a.ldo + h * a.HS;
-    put4(po + 4 * at, t, a.HS - 4 * at, kFull, true);
-    if (at == 0) {
-      if (parts.o) parts.lse[prow * a.NH + h] = L;
-      else if (lse) lse[grow * a.NH + h] = L;
+    if (!lost) {
+      put4(po + 4 * at, t, a.HS - 4 * at, kFull, true);
+      if (at == 0 && parts.o) {
+        parts.m[prow * a.NH + h] = top * kLn2;
+        parts.l[prow * a.NH + h] = sum;
+      } else if (at == 0 && lse) {
+        lse[grow * a.NH + h] = any ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
+      }
     }
+  }
+  for (uint64_t rest = __ballot(lost && at == 0); rest; rest &= rest - 1) {
+    const int x = __builtin_ctzll(rest), rr = __shfl(r, x), ii = rr / G, hh = hk * G + rr % G;
+    const size_t p = (((size_t)part * a.nseq + b) * a.max_q + ii) * a.NH + hh, g = (size_t)s.q0 + ii;
+    row_forward(parts.o ? parts.o + p * a.HS : out + g * a.ldo + hh * a.HS, lse ? lse + g * a.NH + hh : nullptr,
+                parts.o ? parts.m + p : nullptr, parts.l - parts.m, q + g * a.ldq + hh * a.HS,
+                k + ((size_t)s.k0 + first) * a.ldk + hk * a.HS, v + ((size_t)s.k0 + first) * a.ldv + hk * a.HS,
+                min(stop, s.seen(ii, a.causal)) - first, a.HS, a.ldk, a.ldv, a.scale);
   }
 }
 
 // The parts of a split key axis joined, one wavefront per row and head: out =
-// sum_x e^(lse_x - lse) o_x, in the parts' order.
+// sum_x w_x o_x / sum_x w_x with w_x = l_x e^(m_x - max m), in the parts' order.
 __global__ __launch_bounds__(kBlock) void k_att_join(float *out, float *lse, Parts parts, ugk_attention a) {
   const size_t at = (size_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6), per = (size_t)a.nseq * a.max_q * a.NH;
   if (at >= per) return;
@@ -764,22 +789,22 @@ __global__ __launch_bounds__(kBlock) void k_att_join(float *out, float *lse, Par
   const Seq s = sequence(a, b, false, nullptr, 0);
   if (i >= s.Lq) return;
   float m = -INFINITY;
-  for (int x = lane; x < parts.splits; x += kWave) {
-    const float y = parts.lse[x * per + at];
-    m = y != y ? INFINITY : fmaxf(m, y);  // NaN: every weight below is then NaN
-  }
+  for (int x = lane; x < parts.splits; x += kWave) m = fmaxf(m, parts.m[x * per + at]);
   m = wave_max(m);
   float o0 = 0.0f, o1 = 0.0f, l = 0.0f;
   const int d0 = min(lane, a.HS - 1), d1 = min(lane + kWave, a.HS - 1);
-  for (int x = 0; x < parts.splits; x++) {
-    const float y = parts.lse[x * per + at];
-    if (y == -INFINITY) continue;  // a part without a key of this row
-    const float w = expf(y - m), *o = parts.o + (x * per + at) * a.HS;
-    l += w;
-    o0 = fmaf(w, o[d0], o0);
-    o1 = fmaf(w, o[d1], o1);
+  for (int x0 = 0; x0 < parts.splits; x0 += kWave) {
+    const int x = x0 + lane, n = min(kWave, parts.splits - x0);
+    const float lx = x < parts.splits ? parts.l[x * per + at] : 0.0f;
+    const float w = lx == 0.0f ? 0.0f : lx * expf(parts.m[x * per + at] - m);  // 0: a part without a key of this row, its o is 0
+    for (int t = 0; t < n; t++) {
+      const float wt = __shfl(w, t), *o = parts.o + ((x0 + t) * per + at) * a.HS;
+      l += wt;
+      o0 = fmaf(wt, o[d0], o0);
+      o1 = fmaf(wt, o[d1], o1);
+    }
   }
-  const bool none = m == -INFINITY;
+  const bool none = l == 0.0f;
   const float r = none ? 1.0f : l;
   const size_t g = (size_t)s.q0 + i;
   float *po = out + g * a.ldo + h * a.HS;
@@ -1481,22 +1506,23 @@ FwdPlan fwd_plan(const ugk_attention &a) {
   }
   return p;
 }
-size_t parts_lse(const ugk_attention &a, const FwdPlan &p) { return (size_t)p.splits * a.nseq * a.max_q * a.NH; }
+size_t parts_rows(const ugk_attention &a, const FwdPlan &p) { return (size_t)p.splits * a.nseq * a.max_q * a.NH; }
 }  // namespace
 
 size_t attention_parts_bytes(const ugk_attention &a) {
   const FwdPlan p = fwd_plan(a);
-  return p.splits > 1 ? parts_lse(a, p) * (a.HS + 1) * sizeof(float) : 0;
+  return p.splits > 1 ? parts_rows(a, p) * (a.HS + 2) * sizeof(float) : 0;
 }
-size_t attention_parts_bound() { return kMaxParts * (kMaxHead + 1) * sizeof(float); }
+size_t attention_parts_bound() { return kMaxParts * (kMaxHead + 2) * sizeof(float); }
 
 int launch_attention_forward(float *out, float *lse, const float *q, const float *k, const float *v, float *mem,
                              const ugk_attention &a, int *word) {
   const FwdPlan p = fwd_plan(a);
   Parts parts{};
   if (p.splits > 1) {
-    parts.lse = mem;
-    parts.o = mem + parts_lse(a, p);
+    parts.m = mem;
+    parts.l = parts.m + parts_rows(a, p);
+    parts.o = parts.l + parts_rows(a, p);
     parts.splits = p.splits;
     parts.chunk = p.chunk;
   }
