@@ -87,6 +87,16 @@ def check_forward(c):
     inside(lse, *w["lse"], "lse")
 
 
+def check_backward(c):
+    """Of the rounded results, which the kernels get as well."""
+    out, lse = c.forward()
+    w = results(c, lse, out)
+    g = c.grads(3.0)
+    c.backward(out, lse, g, zeroed=True)
+    for name, x in zip(("dq", "dk", "dv"), g):
+        inside(x, *w[name], name)
+
+
 # (query lengths, key lengths, NH, NKV, HS): tiles of 64 and 32 keys, ragged heads, groups, a split key axis, few rows
 SHAPES = [([40], [512], 2, 2, 64), ([300], None, 1, 1, 64), ([40], [512], 2, 1, 128), ([70, 33], None, 4, 1, 50), ([12], [3000], 2, 2, 64),
           ([130], None, 2, 2, 100), ([1, 3], [512, 70], 2, 2, 64), ([50], [200], 3, 3, 4)]
@@ -130,6 +140,20 @@ def test_a_large_key_that_is_not_chosen(gpu, lq, lk, NH, NKV, HS):
         c.k[k0 + 7] *= 2.0
         c.k[k0 + 7, :, 0] = -1e12
     check_forward(c)
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("bits", [16, 30, 45])
+def test_gradients_of_keys_of_little_weight(gpu, bits, lq, lk, NH, NKV, HS):
+    """One key takes nearly all the weight: the others weigh about 2^-bits in every row, and their dv and dk have
+    as many digits as the first one's."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)
+    x = (bits * math.log(2.0) / c.scale) ** 0.5
+    c.q[:, :, 0] = x
+    c.k[:, :, 0] = 0.0
+    for k0 in c.s.k:
+        c.k[k0, :, 0] = x
+    check_backward(c)
 
 
 def by_row(c, spread, seed, which):

@@ -944,12 +944,12 @@ __device__ __forceinline__ v16f dot_block(const _Float16 *ah, const _Float16 *al
   return c;
 }
 
-// Before a block of dS (16 per lane, the row's or key's other half in lane ^ 32) is
+// Before a block of dS or P (16 per lane, the row's or key's other half in lane ^ 32) is
 // accumulated with operands of exponent e: the accumulators stand on 2^ea, at least on the
-// largest of the block's dS times 2^e, so that dS 2^(15 + e - ea) is below 2^15. It moves
-// in steps of 2^2 or more, for it costs a pass over the accumulators. (dS's own
-// largest, not a bound from those of dout and v: P is small where there are many keys, and
-// the halves would lose its digits.) Returns whether the range does not do.
+// largest of the block times 2^e, so that dS 2^(15 + e - ea) is below 2^15. It moves
+// in steps of 2^2 or more, for it costs a pass over the accumulators. (The block's own
+// largest, not 1 for P or a bound from dout and v for dS: P is small where there are many keys or
+// another has the weight, and the halves would lose its digits.) Returns whether the range does not do.
 constexpr int kNoScale = -250;
 template <int DB>
 __device__ __forceinline__ bool raise(int &ea, v16f (&acc)[DB], const v16f &ds, int e) {
@@ -957,7 +957,7 @@ __device__ __forceinline__ bool raise(int &ea, v16f (&acc)[DB], const v16f &ds, 
 #pragma unroll
   for (int y = 0; y < 16; y += 2) m = fmaxf(fmaxf(m, fabsf(ds[y])), fabsf(ds[y + 1]));
   m = half_max(m);
-  const int need = split_exp(__float_as_uint(m)), was = ea;
+  const int need = max((int)(__float_as_uint(m) >> 23) - 126, -112), was = ea;
   if (m > 0.0f && need + e > ea) ea = need + e + 2;
   if (__any(ea != was)) {
     const float f = pow2(max(was - ea, -126));
@@ -1250,6 +1250,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   const size_t stat = (size_t)s.q0 * a.NH + hk * G;
   Rows4 t[kPer];
   float tL = 0.0f, tD = 0.0f;
+  bool past = false;  // this thread's row of the tile is behind the last one: its P are 0
   const auto is_g = [&](int u) { return kPer == 1 ? wave >= W / 2 : u >= kPer / 2; };
   const auto block = [&](int u) { return (tid + u * kThreads) % kBlocks; };
   long long off[kPer][4];  // a tile's rows from its first one
@@ -1271,7 +1272,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       const int r = r0 + tid, i = min(r, rows - 1) / G, x = min(r, rows - 1) - i * G;
       tL = lse[stat + (size_t)i * a.NH + x] * kLog2e;
       tD = dsum[stat + (size_t)i * a.NH + x];
-      if (r >= rows) tL = tD = 0.0f;
+      past = r >= rows;
+      if (past) tL = tD = 0.0f;
       if (s.seen(i, a.causal) == 0) tL = 0.0f;  // a row without keys
     }
   };
@@ -1317,47 +1319,45 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       put_rows<KG>(t[u], w ? fg : fq, (w ? lg : lq)[z][0] + p, (w ? lg : lq)[z][1] + p, kRs);
     }
     if (tid < BQ) {
-      lL[z][tid] = 15.0f - tL;
+      lL[z][tid] = past ? -INFINITY : 15.0f - tL;
       lD[z][tid] = tD;
     }
   };
 
   v16f ak[DB] = {}, av[DB] = {};
-  int ea = kNoScale, eg_acc = -100;  // the exponents that dk's and dv's accumulators stand on
+  int ea = kNoScale, ev_acc = kNoScale;  // the exponents that dk's and dv's accumulators stand on
   const int cols = cols_at(lane, kRs);
   const auto compute = [&](int z, int r0, int eq_now, int eg_now) {
     const bool seen = live && lim < r0 + BQ;
-    const int eg_was = eg_acc;
-    if (seen) eg_acc = max(eg_acc, eg_now);
-    if (__any(eg_acc != eg_was)) {
-      const float f = pow2(max(eg_was - eg_acc, -126));
-#pragma unroll
-      for (int x = 0; x < DB; x++)
-#pragma unroll
-        for (int y = 0; y < 16; y++) av[x][y] *= f;
-    }
     const float c2 = ck * split_unscale(eq_now), cd = cv * split_unscale(eg_now);
-    const float fp = pow2(max(min(eg_now - eg_acc, 0), -126));
     bad = bad || (seen && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
+    const int rel = r0 < hi || !live ? lim - r0 - 4 * half : 0;  // rows of the lane's half before rel do not see the key
     v16f p = dot_block<DC>(lq[z][0], lq[z][1], kRs, kh, kl, lane);
-    v16f ds = dot_block<DC>(lg[z][0], lg[z][1], kRs, vh, vl, lane);
 #pragma unroll
     for (int y = 0; y < 4; y++) {
       const float4 L = *reinterpret_cast<const float4 *>(&lL[z][8 * y + 4 * half]);
-      const float4 D = *reinterpret_cast<const float4 *>(&lD[z][8 * y + 4 * half]);
 #pragma unroll
-      for (int x = 0; x < 4; x++) {
-        p[4 * y + x] = __builtin_amdgcn_exp2f(fmaf(p[4 * y + x], c2, part4(L, x)));
-        ds[4 * y + x] = p[4 * y + x] * fmaf(ds[4 * y + x], cd, -part4(D, x));
-      }
+      for (int x = 0; x < 4; x++) p[4 * y + x] = __builtin_amdgcn_exp2f(fmaf(p[4 * y + x], c2, part4(L, x)));
     }
     if (r0 < hi || !live) {
-      const int rel = lim - r0 - 4 * half;
 #pragma unroll
       for (int y = 0; y < 16; y++)
-        if (8 * (y / 4) + y % 4 < rel) p[y] = ds[y] = 0.0f;
+        if (8 * (y / 4) + y % 4 < rel) p[y] = 0.0f;
     }
-    mac_block<DB>(av, p, fp, lg[z][0], lg[z][1], kRs, cols);
+    bad = raise(ev_acc, av, p, eg_now) || bad;
+    mac_block<DB>(av, p, pow2(max(min(15 + eg_now - ev_acc, 127), -126)), lg[z][0], lg[z][1], kRs, cols);
+    v16f ds = dot_block<DC>(lg[z][0], lg[z][1], kRs, vh, vl, lane);
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+      const float4 D = *reinterpret_cast<const float4 *>(&lD[z][8 * y + 4 * half]);
+#pragma unroll
+      for (int x = 0; x < 4; x++) ds[4 * y + x] = p[4 * y + x] * fmaf(ds[4 * y + x], cd, -part4(D, x));
+    }
+    if (r0 < hi || !live) {
+#pragma unroll
+      for (int y = 0; y < 16; y++)
+        if (8 * (y / 4) + y % 4 < rel) ds[y] = 0.0f;
+    }
     bad = raise(ea, ak, ds, eq_now) || bad;
     mac_block<DB>(ak, ds, pow2(max(min(15 + eq_now - ea, 127), -126)), lq[z][0], lq[z][1], kRs, cols);
   };
@@ -1396,8 +1396,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     return;
   }
   if (!live) return;
-  put_scaled<DB, kSlots == kWhole>(ok + grow * ldk, ak, ea - 45, a.scale, half, a.HS, assign);  // dS, like P, was 2^15 up
-  put_scaled<DB, kSlots == kWhole>(ov + grow * ldv, av, eg_acc - 30, 1.0f, half, a.HS, assign);
+  put_scaled<DB, kSlots == kWhole>(ok + grow * ldk, ak, ea - 45, a.scale, half, a.HS, assign);  // P, and so dS, was 2^15 up
+  put_scaled<DB, kSlots == kWhole>(ov + grow * ldv, av, ev_acc - 45, 1.0f, half, a.HS, assign);
 }
 
 // The parts' dk and dv added, in the parts' order, a thread per element.
