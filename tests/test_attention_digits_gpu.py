@@ -118,6 +118,12 @@ def test_a_large_value_of_little_weight(gpu, size, lq, lk, NH, NKV, HS):
     check_forward(large_value(gpu, size, lq, lk, NH, NKV, HS))
 
 
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("size", [2.0 ** 12, 1e6, 1e10])
+def test_gradients_beside_a_large_value_of_little_weight(gpu, size, lq, lk, NH, NKV, HS):
+    check_backward(large_value(gpu, size, lq, lk, NH, NKV, HS))
+
+
 @pytest.mark.parametrize("first", [0, 5, 200])
 def test_a_large_value_of_little_weight_two_blocks_a_wavefront(gpu, first):
     """As above where the call has so many rows that a wavefront takes two blocks of them."""
@@ -179,6 +185,12 @@ def test_sizes_that_change_from_row_to_row(gpu, spread, which, lq, lk, NH, NKV, 
     check_forward(spread_rows(gpu, spread, which, lq, lk, NH, NKV, HS))
 
 
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("spread,which", SPREADS)
+def test_gradients_where_sizes_change_from_row_to_row(gpu, spread, which, lq, lk, NH, NKV, HS):
+    check_backward(spread_rows(gpu, spread, which, lq, lk, NH, NKV, HS))
+
+
 def large_blocks(gpu, seed):
     """Blocks of keys whose values, and scores, grow, shrink or alternate by large factors: what the sums stand on moves."""
     c = Call(gpu, Seqs([37], [700]), 2, 1, 64)
@@ -193,6 +205,11 @@ def large_blocks(gpu, seed):
 @pytest.mark.parametrize("seed", range(3))
 def test_largest_values_first_last_and_between(gpu, seed):
     check_forward(large_blocks(gpu, seed))
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_gradients_of_largest_values_first_last_and_between(gpu, seed):
+    check_backward(large_blocks(gpu, seed))
 
 
 @pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
@@ -215,6 +232,25 @@ def test_scores_that_overflow_to_minus_infinity(gpu, lq, lk, NH, NKV, HS):
     c.k.clamp_(min=-(2.0 ** 20))  # in 64 bits: scores far below
     w = results(c)
     inside(out, *w["out"], "out")
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, 3e38])
+def test_rows_of_queries_that_cannot_be_used(gpu, value):
+    """Query and dout rows of NaN, infinities or the largest values: dk and dv of the keys that they do not see, and dq of the
+    other rows, have every digit."""
+    for HS, n, r in ((64, 150, 20), (128, 150, 40), (50, 300, 130)):
+        c = Call(gpu, Seqs([n]), 2, 1, HS)
+        out, lse = c.forward()
+        clean = Call(gpu, Seqs([n]), 2, 1, HS)
+        c.q[r], c.dout[r] = value, value
+        g = c.grads(5.0)
+        c.backward(out, lse, g, zeroed=True)
+        want = results(clean, lse, out)
+        keys = torch.arange(n, device=DEV) > r
+        others = torch.arange(n, device=DEV) != r
+        inside(g[0][others], want["dq"][0][others], want["dq"][1][others], "dq of the other rows")
+        inside(g[1][keys], want["dk"][0][keys], want["dk"][1][keys], "dk of the keys that the row does not see")
+        inside(g[2][keys], want["dv"][0][keys], want["dv"][1][keys], "dv of the keys that the row does not see")
 
 
 @pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)

@@ -889,9 +889,11 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
 // atomics would save the second S and dP, 4 of 14 HS operations per pair).
 // P = exp(S - lse) needs no running maximum. A lane holds one row (dq) or one key (dk, dv)
 // as it holds a row in the forward, the other side goes through LDS in tiles, and
-// what its accumulators stand on follows what it has seen alone. Rows are taken one by one
-// instead for the reasons of the forward, and where not all rows (keys) see all of a tile and its
-// magnitudes lie further apart than the halves' digits allow (too_wide).
+// what its accumulators stand on follows what it has seen alone: the largest P of a
+// key times the largest of dout's row, the largest dS times that of q's or k's. Rows that lie far
+// below their tile's largest are lifted, and others taken one by one, as in the forward: 8 x 1,024 rows of 12 heads
+// with dout's rows times 2^-8 to 2^8 take 250 us against 210, 4 x 2,048 of 16/4 heads of 128 1,430 against 1,140
+// (row by row 26 and 123 ms).
 //
 // The same sum of matrix and vector instructions bounds them: of 858 (dk, dv) and 633 us
 // (dq) at 4 x 4,096 rows of 12 heads, 612 and 465 were left without loading,
@@ -997,7 +999,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   static_assert(kPer >= 1 && kBlocks % kWave == 0, "whole wavefronts of K or V blocks");
   constexpr int kRs = HSP + 8, KG = BK / 4;
   __shared__ __attribute__((aligned(16))) _Float16 lk[2][2][BK * kRs], lv[2][2][BK * kRs];
-  __shared__ uint32_t slot[2][4][W];
+  __shared__ uint32_t slot[2][2][W];
+  __shared__ Lifts<BK> lifts;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
   const unsigned pair = blockIdx.x % pairs;
   const int tile = (int)(gridDim.x / pairs - 1 - blockIdx.x / pairs);
@@ -1054,37 +1057,37 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
       t[u] = load_rows<KG, kSlots>((w ? vb : kb) + d, w ? a.ldv : a.ldk, j, n, tail, a.HS - d);
     }
   };
+  uint32_t small[kPer];
   const auto note = [&](int at) {
-    uint32_t m[4] = {};
-    const bool part = (at + 1) * BK > least;
+    uint32_t m[2] = {};
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
       const int w = is_v(u) ? 1 : 0;
-      if (part) {
-        m[w] = max_abs<true>(m[w], t[u]);
-        m[w + 2] = least_row<DG>(m[w + 2], t[u]);
-      } else {
-        m[w] = max_abs<false>(m[w], t[u]);
-      }
-    }
-    if (part) {
-      m[2] = wave_max_bits(m[2]);
-      m[3] = wave_max_bits(m[3]);
+      m[w] = max_abs(m[w], t[u], &small[u]);
+      if (kSlots != kWhole && a.HS <= block(u) % DG * 4) small[u] = kInfBits;  // behind the row
+      if ((at + 1) * BK > least) m[w] = max_abs<true>(m[w], t[u]);
     }
     m[0] = wave_max_bits(m[0]);
     m[1] = wave_max_bits(m[1]);
     if (lane == 0) {
-#pragma unroll
-      for (int x = 0; x < 4; x++) slot[at & 1][x][wave] = m[x];
+      slot[at & 1][0][wave] = m[0];
+      slot[at & 1][1][wave] = m[1];
     }
   };
   int ek = 0, ev = 0;  // of the tile staged last
+  int lifted = 0;
   const auto stage = [&](int at) {
     const int z = at & 1;
     const uint32_t mk = noted<W>(slot[z][0]), mv = noted<W>(slot[z][1]);
-    bad = bad || mk >= kInfBits || mv >= kInfBits || too_wide(mk, noted<W>(slot[z][2])) || too_wide(mv, noted<W>(slot[z][3]));
+    bad = bad || mk >= kInfBits || mv >= kInfBits;
     ek = split_exp(mk);
     ev = split_exp(mv);
+    bool spread = false;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) spread = spread || may_spread(small[u], is_v(u) ? mv : mk);
+    if (__any(spread) || (lifted >> z & 1))
+      lift_tile<DG, KG>(t, lifts, z, lane, wave, &lifted, [&](int u) { return is_v(u) ? 1 : 0; },
+                        [&](int u) { return is_v(u) ? ev : ek; }, [&](int u) { return block(u) / DG; });
     const float fk = split_scale(ek), fv = split_scale(ev);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -1100,12 +1103,19 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   const auto compute = [&](int at, int ek_now, int ev_now) {
     const int z = at & 1, k0 = at * BK;
     const float c2 = cq * split_unscale(ek_now), cd = cg * split_unscale(ev_now);
+    const uint32_t lifted_by = lifts.any(z);
+    bool apart = false;
     bad = bad || (lim > k0 && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
 #pragma unroll
     for (int w = 0; w < BK / 32; w++) {  // 32 keys
       const int o = 32 * w * kRs;
       v16f p = dot_block<DC>(lk[z][0] + o, lk[z][1] + o, kRs, qh, ql, lane);
-      const v16f dp = dot_block<DC>(lv[z][0] + o, lv[z][1] + o, kRs, gh, gl, lane);
+      v16f dp = dot_block<DC>(lv[z][0] + o, lv[z][1] + o, kRs, gh, gl, lane);
+      if (w == 0) apart = __builtin_amdgcn_readfirstlane(lifted_by) != 0;
+      if (apart) {
+        lower(p, lifts, z, 0, w, half);
+        lower(dp, lifts, z, 1, w, half);
+      }
 #pragma unroll
       for (int y = 0; y < 16; y++) {
         const float x = __builtin_amdgcn_exp2f(fmaf(p[y], c2, -L2));
@@ -1117,12 +1127,14 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
         for (int y = 0; y < 16; y++)
           if (8 * (y / 4) + y % 4 >= rel) p[y] = 0.0f;
       }
+      if (apart) lower(p, lifts, z, 0, w, half);
       bad = raise(ea, acc, p, ek_now) || bad;
       mac_block<DB>(acc, p, pow2(max(min(15 + ek_now - ea, 127), -126)), lk[z][0] + o, lk[z][1] + o, kRs, cols);
     }
   };
 
   const int tiles = (n + BK - 1) / BK;
+  lifts.clear();
   if (tiles > 0) {
     load(0);
     note(0);
@@ -1205,7 +1217,8 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   constexpr int kRs = HSP + 8, KG = BQ / 4;
   __shared__ __attribute__((aligned(16))) _Float16 lq[2][2][BQ * kRs], lg[2][2][BQ * kRs];
   __shared__ __attribute__((aligned(16))) float lL[2][BQ], lD[2][BQ];
-  __shared__ uint32_t slot[2][5][W];
+  __shared__ uint32_t slot[2][3][W];
+  __shared__ Lifts<BQ> lifts;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, half = lane >> 5;
   const unsigned pair = blockIdx.x % pairs;
   // The keys that the most rows see first, their parts one after the other (with the parts
@@ -1277,40 +1290,38 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       if (s.seen(i, a.causal) == 0) tL = 0.0f;  // a row without keys
     }
   };
+  uint32_t small[kPer];
   const auto note = [&](int z, int r0) {
-    uint32_t m[5] = {};
-    const bool part = r0 < all;
+    uint32_t m[3] = {};
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
       const int w = is_g(u) ? 1 : 0;
-      if (part) {
-        m[w] = max_abs<true>(m[w], t[u]);
-        m[w + 2] = least_row<DG>(m[w + 2], t[u]);
-      } else {
-        m[w] = max_abs<false>(m[w], t[u]);
-      }
+      m[w] = max_abs(m[w], t[u], &small[u]);
+      if (kSlots != kWhole && a.HS <= block(u) % DG * 4) small[u] = kInfBits;  // behind the row
+      if (r0 < all) m[w] = max_abs<true>(m[w], t[u]);
     }
-    if (tid < BQ) m[4] = abs_bits(tL);
+    if (tid < BQ) m[2] = abs_bits(tL);
     m[0] = wave_max_bits(m[0]);
     m[1] = wave_max_bits(m[1]);
-    if (part) {
-      m[2] = wave_max_bits(m[2]);
-      m[3] = wave_max_bits(m[3]);
-    }
-    if (wave == 0) m[4] = wave_max_bits(m[4]);
+    if (wave == 0) m[2] = wave_max_bits(m[2]);
     if (lane == 0) {
 #pragma unroll
-      for (int x = 0; x < 5; x++) slot[z][x][wave] = m[x];
+      for (int x = 0; x < 3; x++) slot[z][x][wave] = m[x];
     }
   };
   int eq = 0, eg = 0;  // of the tile staged last
+  int lifted = 0;
   const auto stage = [&](int z) {
     const uint32_t mq = noted<W>(slot[z][0]), mg = noted<W>(slot[z][1]);
-    bad = bad || mq >= kInfBits || mg >= kInfBits || noted<W>(slot[z][4]) >= 0x4a800000u /* 2^22 */ ||
-          too_wide(mq, noted<W>(slot[z][2])) ||
-          too_wide(mg, noted<W>(slot[z][3]));
+    bad = bad || mq >= kInfBits || mg >= kInfBits || noted<W>(slot[z][2]) >= 0x4a800000u /* 2^22 */;
     eq = split_exp(mq);
     eg = split_exp(mg);
+    bool spread = false;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) spread = spread || may_spread(small[u], is_g(u) ? mg : mq);
+    if (__any(spread) || (lifted >> z & 1))
+      lift_tile<DG, KG>(t, lifts, z, lane, wave, &lifted, [&](int u) { return is_g(u) ? 1 : 0; },
+                        [&](int u) { return is_g(u) ? eg : eq; }, [&](int u) { return block(u) / DG; });
     const float fq = split_scale(eq), fg = split_scale(eg);
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -1331,8 +1342,11 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     const bool seen = live && lim < r0 + BQ;
     const float c2 = ck * split_unscale(eq_now), cd = cv * split_unscale(eg_now);
     bad = bad || (seen && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
+    const uint32_t lifted_by = lifts.any(z);
     const int rel = r0 < hi || !live ? lim - r0 - 4 * half : 0;  // rows of the lane's half before rel do not see the key
     v16f p = dot_block<DC>(lq[z][0], lq[z][1], kRs, kh, kl, lane);
+    const bool apart = __builtin_amdgcn_readfirstlane(lifted_by) != 0;
+    if (apart) lower(p, lifts, z, 0, 0, half);
 #pragma unroll
     for (int y = 0; y < 4; y++) {
       const float4 L = *reinterpret_cast<const float4 *>(&lL[z][8 * y + 4 * half]);
@@ -1344,12 +1358,18 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       for (int y = 0; y < 16; y++)
         if (8 * (y / 4) + y % 4 < rel) p[y] = 0.0f;
     }
+    if (apart) lower(p, lifts, z, 1, 0, half);
     bad = raise(ev_acc, av, p, eg_now) || bad;
     mac_block<DB>(av, p, pow2(max(min(15 + eg_now - ev_acc, 127), -126)), lg[z][0], lg[z][1], kRs, cols);
+    // dP of dout's lifted rows, and with it D; P is that much lower
     v16f ds = dot_block<DC>(lg[z][0], lg[z][1], kRs, vh, vl, lane);
 #pragma unroll
     for (int y = 0; y < 4; y++) {
-      const float4 D = *reinterpret_cast<const float4 *>(&lD[z][8 * y + 4 * half]);
+      float4 D = *reinterpret_cast<const float4 *>(&lD[z][8 * y + 4 * half]);
+      if (apart) {
+        const int4 d = lifts.four(z, 1, 0, y, half);
+        D = make_float4(ldexpf(D.x, -d.x), ldexpf(D.y, -d.y), ldexpf(D.z, -d.z), ldexpf(D.w, -d.w));
+      }
 #pragma unroll
       for (int x = 0; x < 4; x++) ds[4 * y + x] = p[4 * y + x] * fmaf(ds[4 * y + x], cd, -part4(D, x));
     }
@@ -1358,11 +1378,13 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
       for (int y = 0; y < 16; y++)
         if (8 * (y / 4) + y % 4 < rel) ds[y] = 0.0f;
     }
+    if (apart) lower(ds, lifts, z, 0, 0, half);
     bad = raise(ea, ak, ds, eq_now) || bad;
     mac_block<DB>(ak, ds, pow2(max(min(15 + eq_now - ea, 127), -126)), lq[z][0], lq[z][1], kRs, cols);
   };
 
   const int tiles = rows > from ? (rows - from + BQ - 1) / BQ : 0;
+  lifts.clear();
   if (tiles > 0) {
     load(from);
     note(0, from);

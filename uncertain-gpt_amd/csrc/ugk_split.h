@@ -176,23 +176,6 @@ __device__ __forceinline__ uint32_t max_abs(uint32_t m, const Rows4 &t) {
   }
   return __float_as_uint(f);
 }
-// For the least of the rows' largest magnitudes, rows of zeros left out: the
-// complement, so that it is a maximum too. kLanes lanes share the four rows.
-template <int kLanes>
-__device__ __forceinline__ uint32_t least_row(uint32_t m, const Rows4 &t) {
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    const uint32_t x = row_max_bits<kLanes>(max_abs(0u, t.r[r]));
-    m = max(m, x ? ~x : 0u);
-  }
-  return m;
-}
-// Whether a row of the tile lies so far below the tile's largest that the tile's
-// scale would cost it digits (its elements from 2^-4 of its own largest on keep theirs).
-__device__ __forceinline__ bool too_wide(uint32_t largest, uint32_t least) {
-  return least && (largest >> 23) > (~least >> 23) + 12;
-}
-
 // The largest magnitude's bits, NaN passed over, and in *least those of the smallest of the rows' four-element
 // largest: a row that lies far below the tile's largest has such four elements (others may have them too).
 __device__ __forceinline__ uint32_t max_abs(uint32_t m, const Rows4 &t, uint32_t *least) {
