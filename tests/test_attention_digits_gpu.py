@@ -213,6 +213,68 @@ def test_gradients_of_largest_values_first_last_and_between(gpu, seed):
 
 
 @pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+def test_keys_of_minus_infinity_in_the_backward(gpu, lq, lk, NH, NKV, HS):
+    """Keys whose scores are -infinity for an infinite element weigh nothing in the gradients either: dq is that of
+    the other keys, theirs are 0. A row without another key has gradients 0."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)
+    c.q[:, :, 0] = c.q[:, :, 0].abs() + 0.1
+    for k0, n in zip(c.s.k, c.s.lk):
+        c.k[k0 + n // 4:k0 + n, :, 0] = -math.inf
+    out, lse = c.forward()
+    finite = c.k.clone()
+    finite[c.k == -math.inf] = 0.0
+    short = Call(gpu, c.s, NH, NKV, HS)  # the same with those keys at a finite score far below
+    short.q, short.v, short.dout, short.k = c.q, c.v, c.dout, finite.clone()
+    short.k[:, :, 0][c.k[:, :, 0] == -math.inf] = -1e6
+    w = results(short, lse, out)
+    g, start = c.grads(3.0), 3.0
+    c.backward(out, lse, g, zeroed=True)
+    gone = c.k[:, :, 0] == -math.inf
+    # a row that sees finite keys: those of -infinity reach nothing; a row that sees none: zeros
+    for name, x in zip(("dq", "dk", "dv"), g):
+        want, tol = w[name]
+        if name == "dq":
+            empty = lse == -math.inf
+            assert x[empty].eq(0).all()
+            inside(x[~empty], want[~empty], tol[~empty], name)
+        else:
+            assert x[gone].eq(0).all(), name
+            keep = ~gone
+            inside(x[keep], want[keep], tol[keep], name)
+    # every key of -infinity: no gradients at all
+    c.k[:, :, 0] = -math.inf
+    out, lse = c.forward()
+    assert out.eq(0).all() and (lse == -math.inf).all()
+    g = c.grads(start)
+    c.backward(out, lse, g, zeroed=True)
+    assert all(x.eq(0).all() for x in g)
+
+
+def test_queries_of_minus_infinity_in_the_backward(gpu):
+    """A query row whose own infinite element makes all its scores -infinity: its gradients are 0 and it adds nothing
+    to those of the keys."""
+    c = Call(gpu, Seqs([70]), 2, 1, 64)
+    c.k[:, :, 0] = c.k[:, :, 0].abs() + 0.1
+    w = None
+    clean = Call(gpu, Seqs([70]), 2, 1, 64)
+    clean.k[:, :, 0] = clean.k[:, :, 0].abs() + 0.1
+    clean.dout[33] = 0.0
+    out, lse = clean.forward()
+    out[33] = 0.0
+    w = results(clean, lse, out)
+    c.q[33, :, 0] = -math.inf
+    out, lse = c.forward()
+    assert out[33].eq(0).all() and (lse[33] == -math.inf).all()
+    g = c.grads(2.0)
+    c.backward(out, lse, g, zeroed=True)
+    assert g[0][33].eq(0).all()
+    rows = torch.arange(70, device=DEV) != 33
+    inside(g[0][rows], w["dq"][0][rows], w["dq"][1][rows], "dq")
+    inside(g[1], *w["dk"], "dk")
+    inside(g[2], *w["dv"], "dv")
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
 def test_scores_that_overflow_to_minus_infinity(gpu, lq, lk, NH, NKV, HS):
     """Finite queries and keys whose every product is beyond the range: out 0, lse -infinity, gradients 0."""
     c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)

@@ -68,7 +68,8 @@ __device__ __forceinline__ float dot(const float *x, const float *y, int n) {
 
 __device__ __forceinline__ void put(float *p, float x, bool assign) { *p = assign ? x : *p + x; }
 
-// exp(s - m); a score of -infinity weighs nothing, whatever m is.
+// exp(s - m); a score of -infinity weighs nothing, whatever m is, and its key nothing in the gradients, whatever the infinite
+// element that it came from would make of a product with 0.
 __device__ __forceinline__ float weight(float s, float m) { return s == -INFINITY ? 0.0f : expf(s - m); }
 
 // One query row of one head by one wavefront: lanes over keys for the scores,
@@ -829,8 +830,15 @@ __device__ void row_dq(float *dq, float *dsum, const float *dout, const float *q
   for (int j0 = 0; j0 < n; j0 += kWave) {
     const int j = j0 + lane;
     float ds = 0.0f;
-    if (j < n) ds = weight(dot(q, k + j * ldk, HS) * scale, lse) * (dot(dout, v + j * ldv, HS) - D) * scale;
+    bool gone = false;
+    if (j < n) {
+      const float z = dot(q, k + j * ldk, HS) * scale;
+      gone = z == -INFINITY;
+      ds = weight(z, lse) * (dot(dout, v + j * ldv, HS) - D) * scale;
+    }
+    const uint64_t skip = __ballot(gone);
     for (int t = 0; t < min(kWave, n - j0); t++) {
+      if (skip >> t & 1) continue;
       const float x = __shfl(ds, t);
       a0 = fmaf(x, k[(j0 + t) * ldk + d0], a0);
       a1 = fmaf(x, k[(j0 + t) * ldk + d1], a1);
@@ -855,12 +863,17 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
     for (int i0 = max(s.first(j, a.causal), (max(ra - g, 0) + G - 1) / G); i0 < end; i0 += kWave) {
       const int i = i0 + lane;
       float p = 0.0f, ds = 0.0f;
+      bool gone = false;
       if (i < end) {
         const size_t r = (size_t)s.q0 + i;
-        p = weight(dot(q + r * a.ldq + h * HS, kj, HS) * a.scale, lse[r * a.NH + h]);
+        const float z = dot(q + r * a.ldq + h * HS, kj, HS) * a.scale;
+        gone = z == -INFINITY;
+        p = weight(z, lse[r * a.NH + h]);
         ds = p * (dot(dout + r * a.ldo + h * HS, vj, HS) - dsum[r * a.NH + h]) * a.scale;
       }
+      const uint64_t skip = __ballot(gone);
       for (int t = 0; t < min(kWave, end - i0); t++) {
+        if (skip >> t & 1) continue;
         const size_t r = (size_t)s.q0 + i0 + t;
         const float pt = __shfl(p, t), dt = __shfl(ds, t);
         const float *qr = q + r * a.ldq + h * HS, *gr = dout + r * a.ldo + h * HS;
