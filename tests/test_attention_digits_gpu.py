@@ -212,6 +212,30 @@ def test_gradients_of_largest_values_first_last_and_between(gpu, seed):
     check_backward(large_blocks(gpu, seed))
 
 
+def ends(gpu, sizes, scale, lq, lk, NH, NKV, HS):
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS, scale=HS ** -0.5 * 2.0 ** scale)
+    for name, e in zip(("q", "k", "v", "dout"), sizes):
+        t = getattr(c, name)
+        t.mul_(2.0 ** e)
+    return c
+
+
+ENDS = [((0, 0, -105, 0), 0), ((-105, 105, 0, -90), 0), ((-90, 100, 0, 0), -10), ((10, 10, 60, 40), -20)]
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("sizes,scale", ENDS)
+def test_the_ends_of_the_range(gpu, sizes, scale, lq, lk, NH, NKV, HS):
+    """Results near the least and the largest numbers have their digits."""
+    check_forward(ends(gpu, sizes, scale, lq, lk, NH, NKV, HS))
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("sizes,scale", ENDS)
+def test_gradients_at_the_ends_of_the_range(gpu, sizes, scale, lq, lk, NH, NKV, HS):
+    check_backward(ends(gpu, sizes, scale, lq, lk, NH, NKV, HS))
+
+
 @pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
 def test_keys_of_minus_infinity_in_the_backward(gpu, lq, lk, NH, NKV, HS):
     """Keys whose scores are -infinity for an infinite element weigh nothing in the gradients either: dq is that of

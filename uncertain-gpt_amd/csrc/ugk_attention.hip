@@ -254,6 +254,19 @@ __device__ __forceinline__ void put_row(float *p, const v16f (&acc)[DB], float f
     }
 }
 
+// The same times 2^e f, for any e; the factor stays far from the end of the range, where it would have few digits.
+template <int DB, bool kFull>
+__device__ __forceinline__ void put_scaled(float *p, v16f (&acc)[DB], int e, float f, int half, int HS, bool assign) {
+  const int once = min(max(e, -80), 80), twice = min(max(e - once, -126), 127);
+  if (__any(twice != 0)) {
+#pragma unroll
+    for (int x = 0; x < DB; x++)
+#pragma unroll
+      for (int y = 0; y < 16; y++) acc[x][y] *= pow2(twice);
+  }
+  put_row<DB, kFull>(p, acc, pow2(once) * f, half, HS, assign);
+}
+
 // The largest of a noted quantity over the workgroup's wavefronts.
 template <int W>
 __device__ __forceinline__ uint32_t noted(const uint32_t (&slot)[W]) {
@@ -341,7 +354,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   const int r0 = row0 + wave * (32 * QB) + (lane & 31);
   int lim[QB], lo = n, hi = first;  // what they see; least and most over the wavefront
   v8h qh[QB][DC], ql[QB][DC];
-  float cq[QB];  // of the scores, to base 2
+  int eq[QB];  // of q; the scores, to base 2, are products times 2^(eq + ek - 30) scale log2(e)
 #pragma unroll
   for (int u = 0; u < QB; u++) {
     const int r = r0 + 32 * u;
@@ -361,11 +374,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     }
     m = half_max_bits(m);
     bad = bad || m >= kInfBits;
-    const int e = split_exp(m);
-    const float f = a.scale < 0.0f ? -split_scale(e) : split_scale(e);
+    eq[u] = split_exp(m);
+    const float f = a.scale < 0.0f ? -split_scale(eq[u]) : split_scale(eq[u]);
 #pragma unroll
     for (int c = 0; c < DC; c++) split8(x[c], f, qh[u][c], ql[u][c]);
-    cq[u] = split_unscale(e) * (fabsf(a.scale) * kLog2e);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -434,7 +446,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   for (int u = 0; u < QB; u++) one[u] = all[u] = 3.4028234663852886e38f;
   const int vcols = cols_at(lane, kRs);
   const auto compute = [&](int at, int k0, int ek, int ev_now) {
-    const float uk = split_unscale(ek), ev = (float)ev_now;
+    const float ev = (float)ev_now;
     const uint32_t lifted_by = lifts.any(at);
     bool apart = false;
     float c2[QB], b0[QB];  // P is taken times 2^b0 to be an operand
@@ -443,7 +455,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     };
 #pragma unroll
     for (int u = 0; u < QB; u++) {
-      c2[u] = fmaxf(cq[u] * uk, 0x1p-126f);
+      c2[u] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, eq[u] + ek - 30), 0x1p-126f);
       bad = bad || c2[u] > 0x1p100f;
     }
 #pragma unroll
@@ -591,8 +603,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     const size_t grow = (size_t)s.q0 + i, prow = (((size_t)blockIdx.y * a.nseq + b) * a.max_q + i) * a.NH + h;
     const float sum = half_sum(l[u]);
     const bool some = lim[u] > first;
-    put_row<DB, kFull>(parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS, o[u],
-                       some ? pow2((int)(one[u] - all[u]) - 15) / sum : 0.0f, half, a.HS, true);
+    put_scaled<DB, kFull>(parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS, o[u], (int)(one[u] - all[u]) - 15,
+                          some ? 1.0f / sum : 0.0f, half, a.HS, true);
     if (half == 0 && (parts.o || lse)) {
       if (parts.o) {
         parts.m[prow] = some ? -one[u] * kLn2 : -INFINITY;
@@ -914,19 +926,6 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
 // with the launches (146 TFLOP/s of 10 HS operations per pair). Workgroups of
 // one wavefront were slower at every size tried.
 
-// The same times 2^e f, for any e.
-template <int DB, bool kFull>
-__device__ __forceinline__ void put_scaled(float *p, v16f (&acc)[DB], int e, float f, int half, int HS, bool assign) {
-  const int once = min(max(e, -126), 127), twice = min(max(e - once, -126), 127);
-  if (__any(twice != 0)) {
-#pragma unroll
-    for (int x = 0; x < DB; x++)
-#pragma unroll
-      for (int y = 0; y < 16; y++) acc[x][y] *= pow2(twice);
-  }
-  put_row<DB, kFull>(p, acc, pow2(once) * f, half, HS, assign);
-}
-
 // acc += A^T B for a 32-row block of B held in an accumulator's registers (C, scaled
 // to halves by f): A's 32 rows in LDS, `cols` the lane's place in them (cols_at).
 template <int DB>
@@ -1054,7 +1053,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   D = half_sum(D);
   if (live && half == 0) dsum[grow * a.NH + h] = D;
   const float L2 = live ? lse[grow * a.NH + h] * kLog2e : 0.0f;
-  const float cq = split_unscale(eq) * (a.scale * kLog2e), cg = split_unscale(eg);
+  const float cg = split_unscale(eg);
   bool bad = lim > 0 && (!(fabsf(L2) < 0x1p22f) || qbits >= kInfBits || gbits >= kInfBits);
 
   Rows4 t[kPer];
@@ -1115,7 +1114,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   const int cols = cols_at(lane, kRs);
   const auto compute = [&](int at, int ek_now, int ev_now) {
     const int z = at & 1, k0 = at * BK;
-    const float c2 = cq * split_unscale(ek_now), cd = cg * split_unscale(ev_now);
+    const float c2 = ldexpf(a.scale * kLog2e, eq + ek_now - 30), cd = cg * split_unscale(ev_now);
     const uint32_t lifted_by = lifts.any(z);
     bool apart = false;
     bad = bad || (lim > k0 && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
@@ -1268,7 +1267,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   int ek, ev;
   const uint32_t kbits = load_operand<DC, kSlots>(k + grow * a.ldk + hk * a.HS, a.HS, live, half, kh, kl, &ek);
   const uint32_t vbits = load_operand<DC, kSlots>(v + grow * a.ldv + hk * a.HS, a.HS, live, half, vh, vl, &ev);
-  const float ck = split_unscale(ek) * (a.scale * kLog2e), cv = split_unscale(ev);
+  const float cv = split_unscale(ev);
   bool bad = kbits >= kInfBits || vbits >= kInfBits;
 
   const GroupRows<BQ, KG> gq{q + (size_t)s.q0 * a.ldq + hk * G * a.HS, a.ldq, a.HS, G};
@@ -1353,7 +1352,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   const int cols = cols_at(lane, kRs);
   const auto compute = [&](int z, int r0, int eq_now, int eg_now) {
     const bool seen = live && lim < r0 + BQ;
-    const float c2 = ck * split_unscale(eq_now), cd = cv * split_unscale(eg_now);
+    const float c2 = ldexpf(a.scale * kLog2e, ek + eq_now - 30), cd = cv * split_unscale(eg_now);
     bad = bad || (seen && (fabsf(c2) > 0x1p100f || cd > 0x1p100f));
     const uint32_t lifted_by = lifts.any(z);
     const int rel = r0 < hi || !live ? lim - r0 - 4 * half : 0;  // rows of the lane's half before rel do not see the key
