@@ -380,12 +380,18 @@ int ugk_layernorm_dropout_residual_backward(float *dinp, float *dweight,
  *                                 sees every key)
  *     out_i = sum_j softmax(s)_j v_j,   lse_i = log sum_j exp(s_j)
  * A row without an allowed key, or all of whose scores are -infinity, has out 0,
- * lse -infinity and gradients 0. What a row must not see does not reach it,
- * infinities and NaN included. Results are those of single precision: within the
- * error of its sums; where one key, value, query or dout is over 2^12 times the
- * others of the 32 to 64 rows around it, theirs are held to 2^-39 of it. (Infinities,
- * NaN that only some rows see, magnitudes that far apart where only some rows see
- * them, and scores beyond 2^21 are computed row by row, many times slower.)
+ * lse -infinity and gradients 0; a key whose score is -infinity has no part in a
+ * row's gradients. What a row must not see does not reach it, infinities and NaN
+ * included. Sums, statistics and results are in single precision. A row (of one
+ * head) of q, k, v or dout enters products as two half-precision numbers per
+ * element, to 2^-23 of the element and 2^-31 of the row's largest, and a product
+ * is off by up to 2^-21 of its size; weights, and the gradients of the scores, are
+ * held to 2^-24, and 2^-29, of the largest contribution (weight times the value's
+ * largest element, and likewise) that the row or key sees. With up to four query
+ * rows times heads per key/value head the forward is in single precision
+ * throughout. Infinities, NaN that only some rows see, and scores beyond 2^21 are
+ * computed row by row, many times slower; keys, values, queries or dout whose
+ * sizes are over 2^6 apart within 32 to 64 rows take up to 1.6 times as long.
  * Rows of the buffers outside every sequence are neither read nor written. */
 typedef struct {
   int nseq;           /* sequences */

@@ -3,12 +3,13 @@
 //
 // A float x, scaled by a power of two so that the largest of its row or tile
 // lies in [2^14, 2^15), is held as h + l with h = half(x), l = half(x - h), both
-// rounded to nearest. Each has 11 bits: |x - h| <= 2^-12 |x|, |x - h - l| <=
-// 2^-24 |x| as long as l is a normal half (|x| >= 2^-2, or 2^-16 of the largest);
-// below that the error stays under 2^-25, that is 2^-39 of the largest. A product x y is
-// taken as xh yh + xl yh + xh yl in single-precision accumulators; the part left
-// out, xl yl, is at most 2^-24 |x y|. So a product is within about three
-// roundings of single precision, for three times the half-precision units' work: they
+// rounded to nearest (the splitting that Ootomo and Yokota, 2022, among others, use on such units). Each
+// has 11 bits: |x - h| <= 2^-11 |x|, |x - h - l| <= 2^-23 |x| as long as l is a
+// normal half (|x| >= 2^-2, or 2^-16 of the largest); below that the error stays
+// under 2^-25, that is 2^-39 of the largest. A product x y is taken as xh yh + xl yh +
+// xh yl in single-precision accumulators; the part left out, xl yl, is at most
+// 2^-22 |x y|. So a product is off by 2^-21 of its size at most, eight roundings of single
+// precision, and by a quarter of that in the mean, for three times the half-precision units' work: they
 // do 16 times the operations of the single-precision ones (v_mfma_f32_32x32x16_f16
 // takes 32 cycles, v_mfma_f32_32x32x2_f32 64 for an eighth of the products), so
 // this has a ceiling of 5.3 times theirs. (Three bfloat16 parts would keep
