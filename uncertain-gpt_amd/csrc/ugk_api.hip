@@ -63,7 +63,8 @@ size_t attention_scratch(size_t rows, size_t C, size_t NH, size_t parts, size_t 
 // Region sizes for every entry point at shapes up to cfg: the step driver's
 // 2L+1 LayerNorm slots (at least the one slot of a per-op call), the encoder
 // state, the KL partial sums, the softmax statistics of B*T rows, and attention
-// over B*T rows of C channels in NH heads (the dense callback's backward).
+// over B*T rows of C channels in NH heads (the dense callback's backward; none
+// where the callbacks take no such heads, or NH is 0).
 void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
   const int rows = cfg.B * cfg.T;
   const size_t slot = align_up(layernorm_backward_scratch(rows, cfg.C));
@@ -71,8 +72,10 @@ void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
   out[kRegEncoder] = encoder_backward_scratch();
   out[kRegKl] = kl_forward_scratch();
   out[kRegSoftmax] = softmax_scratch(rows, cfg.V);
-  const size_t NH = cfg.NH > 0 ? cfg.NH : 0;
-  out[kRegAttention] = attention_scratch(rows, cfg.C, NH, attention_parts_bound(), attention_backward_bound(rows, cfg.C, NH));
+  const int NH = cfg.NH, HS = NH > 0 ? cfg.C / NH : 0;
+  out[kRegAttention] = rows > 0 && HS >= 1 && HS <= kMaxHead && HS * NH == cfg.C
+                           ? attention_scratch(rows, cfg.C, NH, attention_parts_bound(HS), attention_backward_bound(rows, NH, HS))
+                           : 0;
 }
 
 // Grow the library-owned region r of device dev to `bytes` (lock held).
@@ -880,7 +883,7 @@ void *ugk_get_stream(void) { return g_stream.load(); }
 
 int ugk_reserve(int rows, int C) {
   if (rows < 0 || C < 0) return bad("ugk_reserve", "rows and C must be >= 0");
-  ugk_config cfg{1, rows, C, 1, 1, rows, 0};
+  ugk_config cfg{1, rows, C, 1, 0, rows, 0};  // no heads: attention's memory comes with its first call
   return ugk_reserve_config(cfg);
 }
 
@@ -900,6 +903,7 @@ int ugk_reserve_config(ugk_config cfg) {
   size_t sz[kNumRegions];
   region_sizes(cfg, sz);
   for (int r = 0; r < kNumRegions; r++) {
+    if (!sz[r]) continue;
     bool fresh = false;
     void *p = workspace(static_cast<Region>(r), sz[r], r == kRegEncoder ? &fresh : nullptr);
     if (!p) return UGK_ENOMEM;

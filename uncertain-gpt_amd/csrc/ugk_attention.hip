@@ -1547,7 +1547,7 @@ size_t attention_parts_bytes(const ugk_attention &a) {
   const FwdPlan p = fwd_plan(a);
   return p.splits > 1 ? parts_rows(a, p) * (a.HS + 2) * sizeof(float) : 0;
 }
-size_t attention_parts_bound() { return kMaxParts * (kMaxHead + 2) * sizeof(float); }
+size_t attention_parts_bound(size_t HS) { return kMaxParts * (HS + 2) * sizeof(float); }
 
 int launch_attention_forward(float *out, float *lse, const float *q, const float *k, const float *v, float *mem,
                              const ugk_attention &a, int *word) {
@@ -1599,8 +1599,11 @@ size_t attention_backward_bytes(const ugk_attention &a) {
   const size_t splits = dkv_splits(a), dsum = ((size_t)a.rows_q * a.NH + 63) / 64 * 64;
   return (dsum + (splits > 1 ? 2 * splits * a.rows_k * a.NKV * a.HS : 0)) * sizeof(float);
 }
-size_t attention_backward_bound(size_t rows, size_t C, size_t NH) {
-  const size_t split = min((size_t)kMaxSplits * rows * C, (size_t)kSplitKeys * cu_count() * kMaxHead);
+// dkv_splits: at most kMaxSplits, kSplitKeys keys per CU over all, and a part per 128 rows of q per key/value head, of
+// which a group has more in proportion to its fewer key/value heads.
+size_t attention_backward_bound(size_t rows, size_t NH, size_t HS) {
+  const size_t splits = min((size_t)kMaxSplits, (rows + 127) / 128);
+  const size_t split = min(splits * rows * NH, (size_t)kSplitKeys * cu_count()) * HS;
   return ((rows * NH + 63) / 64 * 64 + 2 * split) * sizeof(float);
 }
 

@@ -369,9 +369,9 @@ int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout
                               bool assign, int *word);
 size_t attention_parts_bytes(const ugk_attention &a);
 size_t attention_backward_bytes(const ugk_attention &a);
-// over all calls, and over calls of one key/value head per query head with up to rows x C values
-size_t attention_parts_bound();
-size_t attention_backward_bound(size_t rows, size_t C, size_t NH);
+// over all calls of heads of up to HS floats, and over those of up to `rows` rows of NH heads
+size_t attention_parts_bound(size_t HS);
+size_t attention_backward_bound(size_t rows, size_t NH, size_t HS);
 
 // Workspace sizes.
 size_t layernorm_backward_scratch(int rows, int C);  // bytes of one call's partial rows
