@@ -36,8 +36,10 @@
  * allocate nor wait. A call under HIP graph capture that would have to
  * allocate fails with UGK_ENOMEM before launching anything (reserve first, or
  * make one call at that shape outside the capture). Memory that a captured call
- * uses is kept for the graph's replays, also when the region grows later. A caller that owns all device memory (as the reference's
- * arms do) sizes a workspace with ugk_workspace_bytes and hands it over with
+ * uses is kept for the graph's replays, also when the region grows later (it then
+ * doubles at least), until ugk_release_graph_memory. Replays use the workspace as
+ * calls do: two graphs, or a graph and a call, must not run at the same time. A
+ * caller that owns all device memory (as the reference's arms do) sizes a workspace with ugk_workspace_bytes and hands it over with
  * ugk_set_workspace; the library then never allocates. The workspace is used
  * in stream order: ugk_set_stream waits for the work already queued on the
  * previous stream, so calls on two streams never share it at once. The
@@ -459,8 +461,14 @@ void *ugk_get_stream(void);
  * shapes up to (rows = B*T, C) now instead of on first use, but attention's,
  * which depends on the heads (ugk_reserve_config). */
 int ugk_reserve(int rows, int C);
-/* Bytes of workspace held on the current device (the caller's, if set). */
+/* Bytes of workspace held on the current device (the caller's, if set; else with
+ * what is kept for graphs). */
 size_t ugk_scratch_bytes(void);
+/* The caller's word that no graph with captured calls of this library on the
+ * current device will be replayed again: frees the memory kept for them, after
+ * waiting for the device, and no longer keeps what they used of the regions in
+ * use. UGK_EINVAL while the library's stream is being captured. */
+int ugk_release_graph_memory(void);
 /* Wait for all work queued on the library's stream. Then reports, as
  * UGK_EINVAL naming the op, an id that ugk_ids_guard found out of range since
  * the last report (and clears that record). */

@@ -69,3 +69,70 @@ def test_every_shape_up_to_the_config_fits(gpu, NH, C):
             gpu.dense_attention_backward(g, out, x, 1, T, C, NH)
     finally:
         gpu.set_workspace(None, cfg)
+
+
+def captured_backward(gpu, n, stream, graphs):
+    """A captured attention backward of n single rows of 64 heads: 256 n bytes of workspace. Returns it and its check."""
+    x = torch.randn(n, 64, device=DEV)
+    lse, g = torch.zeros(n, 64, device=DEV), [torch.zeros(n, 64, device=DEV) for _ in range(3)]
+    a = gpu.Attention(nseq=n, NH=64, NKV=64, HS=1, rows_q=n, rows_k=n, max_q=1, max_k=1, scale=0.0)
+    call = lambda: gpu.attention_backward_zeroed(*g, x, x, x, x, x, lse, a)  # noqa: E731
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        call()  # grows the region
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+    graphs.append(graph)
+
+    def check():
+        for t in g:
+            t.fill_(9.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        # one key of weight 1 (a score of 0, and the lse given): dv = dout, to the 2^-23 that two halves hold and a rounding; a
+        # scale of 0: dq = dk = 0
+        assert ((g[2] - x).abs() <= 2.0 ** -22 * x.abs()).all() and not g[0].any() and not g[1].any()
+    check.inputs = (x, lse, g)
+    return check
+
+
+@pytest.mark.gpu
+def test_memory_kept_for_graphs_is_counted_bounded_and_released(gpu):
+    gpu.set_workspace(None, gpu.Config(B=1, T=1, C=64, V=2, NH=0, maxT=1, L=0))
+    gpu.release_graph_memory()
+    assert gpu.scratch_bytes() == 0
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gpu.set_stream(stream.cuda_stream)
+    graphs, checks = [], []
+    try:
+        for i in range(9):
+            n = int(2000 * 1.3 ** i)
+            checks.append(captured_backward(gpu, n, stream, graphs))
+            # the region in use is at most twice what the largest call needs, what is kept for graphs below that again
+            assert 256 * n <= gpu.scratch_bytes() <= 4 * (256 * n + 4096)
+        held = gpu.scratch_bytes()
+        for c in checks + checks[::-1]:
+            c()
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            assert gpu.lib.ugk_release_graph_memory() == 1
+            torch.zeros(1, device=DEV).add_(1)
+        assert gpu.scratch_bytes() == held
+        del checks
+        graphs.clear()
+        gpu.release_graph_memory()
+        assert 256 * n <= gpu.scratch_bytes() <= 2 * (256 * n + 4096)
+        more = captured_backward(gpu, 4 * n, stream, graphs)  # the region in use was no graph's any more: freed
+        assert gpu.scratch_bytes() <= 256 * 4 * n + 4096
+        more()
+    finally:
+        gpu.set_stream(None)
+        graphs.clear()
+        gpu.release_graph_memory()
+
+
+def test_release_needs_no_gpu_to_be_declared():
+    import ugk
+    assert "release_graph_memory" in ugk.__all__ and callable(ugk.release_graph_memory)

@@ -12,6 +12,7 @@
 #include <atomic>
 #include <climits>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "../../include/ugk.h"
@@ -30,6 +31,12 @@ size_t align_up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 const char *const kRegionName[kNumRegions] = {"LayerNorm partial rows", "encoder bucket state", "KL partial sums",
                                               "softmax row statistics", "attention row sums and parts"};
 
+struct Kept {
+  void *p;
+  size_t bytes;
+  Kept *next;
+};
+
 // Per device: the library's own region allocations, or the caller's workspace
 // and the offset and capacity of each region in it.
 struct DevWorkspace {
@@ -39,7 +46,8 @@ struct DevWorkspace {
   size_t user_bytes = 0;
   size_t off[kNumRegions] = {}, cap[kNumRegions] = {};
   bool fresh[kNumRegions] = {true, true, true, true, true};
-  bool captured[kNumRegions] = {};  // own[r] is in a graph, which may be replayed at any time: it is never freed
+  bool captured[kNumRegions] = {};  // own[r] is in a graph, which may be replayed at any time
+  Kept *kept = nullptr;             // regions that only graphs use any more, until ugk_release_graph_memory
 };
 DevWorkspace g_ws[kMaxDevices];
 
@@ -78,19 +86,36 @@ void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
                            : 0;
 }
 
-// Grow the library-owned region r of device dev to `bytes` (lock held).
+// Give up the library-owned region r (lock held, the device has been waited for).
+void drop_region(DevWorkspace &w, int r) {
+  if (!w.captured[r]) {
+    (void)hipFree(w.own[r]);
+  } else if (Kept *k = new (std::nothrow) Kept{w.own[r], w.own_bytes[r], w.kept}) {
+    w.kept = k;
+  }  // without memory for the note it stays allocated all the same
+  w.own[r] = nullptr;
+  w.own_bytes[r] = 0;
+  w.captured[r] = false;
+}
+
+// Grow the library-owned region r of device dev to `bytes` (lock held). Where graphs keep the old one it
+// at least doubles, so that what they keep of growing shapes stays below what is in use.
 void *own_region(DevWorkspace &w, Region r, size_t bytes) {
   if (w.own[r] && w.own_bytes[r] >= bytes) return w.own[r];
+  const size_t least = align_up(bytes < ((size_t)1 << 16) ? ((size_t)1 << 16) : bytes);
+  size_t want = w.captured[r] && 2 * w.own_bytes[r] > least ? 2 * w.own_bytes[r] : least;
   if (w.own[r]) {
     // kernels queued earlier, on this or another stream, may still use the old buffer
     (void)hipDeviceSynchronize();
-    if (!w.captured[r]) (void)hipFree(w.own[r]);
-    w.own[r] = nullptr;
-    w.own_bytes[r] = 0;
-    w.captured[r] = false;
+    drop_region(w, r);
   }
-  const size_t want = align_up(bytes < ((size_t)1 << 16) ? ((size_t)1 << 16) : bytes);
-  if (hipMalloc(&w.own[r], want) != hipSuccess) {
+  hipError_t e = hipMalloc(&w.own[r], want);
+  if (e != hipSuccess && want > least) {
+    (void)hipGetLastError();
+    want = least;
+    e = hipMalloc(&w.own[r], want);
+  }
+  if (e != hipSuccess) {
     (void)hipGetLastError();
     w.own[r] = nullptr;
     set_error(UGK_ENOMEM, "workspace: cannot allocate %zu bytes for the %s", want, kRegionName[r]);
@@ -130,10 +155,7 @@ void free_own(DevWorkspace &w) {
   if (!any) return;
   (void)hipDeviceSynchronize();
   for (int r = 0; r < kNumRegions; r++) {
-    if (w.own[r] && !w.captured[r]) (void)hipFree(w.own[r]);
-    w.own[r] = nullptr;
-    w.own_bytes[r] = 0;
-    w.captured[r] = false;
+    if (w.own[r]) drop_region(w, r);
     w.fresh[r] = true;
   }
 }
@@ -216,6 +238,7 @@ size_t workspace_bytes_current() {
   if (w.user) return w.user_bytes;
   size_t t = 0;
   for (int r = 0; r < kNumRegions; r++) t += w.own_bytes[r];
+  for (const Kept *k = w.kept; k; k = k->next) t += k->bytes;
   return t;
 }
 
@@ -953,6 +976,26 @@ int ugk_set_workspace(void *ptr, size_t bytes, ugk_config cfg) {
 }
 
 size_t ugk_scratch_bytes(void) { return workspace_bytes_current(); }
+
+int ugk_release_graph_memory(void) {
+  const char *fn = "ugk_release_graph_memory";
+  const int dev = current_device(fn);
+  if (dev < 0) return set_error(UGK_EHIP, "%s: hipGetDevice failed", fn);
+  if (stream_capturing()) return bad(fn, "the library's stream is being captured");
+  std::lock_guard<std::mutex> lock(g_mu);
+  DevWorkspace &w = g_ws[dev];
+  if (w.kept && hipDeviceSynchronize() != hipSuccess) {  // a replay may be running
+    (void)hipGetLastError();
+    return set_error(UGK_EHIP, "%s: waiting for the device failed", fn);
+  }
+  while (Kept *k = w.kept) {
+    (void)hipFree(k->p);
+    w.kept = k->next;
+    delete k;
+  }
+  for (bool &c : w.captured) c = false;
+  return ok();
+}
 
 namespace {
 const char *ids_op_name(int code) {

@@ -32,7 +32,7 @@ __all__ = [
     "bayes_sample", "bayes_backward",
     "bayes_backward_philox", "kl_forward", "kl_backward", "adamw_update", "bbb_step_fused",
     "Loader", "loader_count", "ckpt_path", "ckpt_save", "ckpt_load",
-    "set_stream", "synchronize", "reserve", "scratch_bytes", "reserve_config", "workspace_bytes",
+    "set_stream", "synchronize", "reserve", "scratch_bytes", "release_graph_memory", "reserve_config", "workspace_bytes",
     "set_workspace", "set_sync_checks", "op_timer_start", "op_timer_read", "set_gelu_exact", "gelu_exact", "set_philox_exact", "philox_exact", "set_kl_exact", "kl_exact", "set_softmax_exact", "softmax_exact", "set_layernorm_exact", "layernorm_exact", "set_encoder_exact", "encoder_exact",
     "Config", "DenseOps", "param_count", "act_count", "gpt2_layers_forward",
     "gpt2_layers_backward", "gpt2_layers_backward_zeroed", "version",
@@ -143,6 +143,7 @@ _SIGS = {
     "ugk_op_timer_start": [_i],
     "ugk_op_timer_read": [_fp, _fp, _i, ctypes.POINTER(_i)],
     "ugk_scratch_bytes": [],
+    "ugk_release_graph_memory": [],
     "ugk_synchronize": [],
     "ugk_version": [],
     "ugk_set_gelu_exact": [_i],
@@ -637,6 +638,11 @@ def reserve(rows: int, C: int) -> None:
 
 def scratch_bytes() -> int:
     return int(lib.ugk_scratch_bytes())
+
+
+def release_graph_memory() -> None:
+    """Free the workspace kept for captured calls: no graph that holds one on this device is replayed again."""
+    _check(lib.ugk_release_graph_memory())
 
 
 def reserve_config(cfg: Config) -> None:
