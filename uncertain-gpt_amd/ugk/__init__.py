@@ -480,16 +480,18 @@ def _ptr_here(x, what: str, need: int):
     return p
 
 
-def _rows_ptr(x, what: str, need: int):
-    """Device address of ``x``, the first of rows that end ``need`` floats behind it. A tensor may be a view into the
-    buffer that holds the rows: what counts is the memory behind its first element. What passes is decided in
-    one line, the rest by _rows_ptr_or_raise."""
+def _rows_ptr(x, what: str, rows):
+    """Device address of ``x``, the first of rows that end ``need`` floats behind it, ``ld`` apart and ``w`` wide, of
+    ``heads`` heads (``rows``: these four). A tensor may be a view into the buffer that holds the rows, as long as its rows are
+    ``ld`` apart (of the filled part of caches, those of each cache): what counts is the memory behind its first
+    element. What passes is decided in one line, the rest by _rows_ptr_or_raise."""
+    need = rows[0]
     if type(x) is _Tensor and _one_device and x.dtype is _DTYPES["f32"] and x.is_cuda and x.numel() >= need and x.is_contiguous():
         return x.data_ptr()
-    return _rows_ptr_or_raise(x, what, need)
+    return _rows_ptr_or_raise(x, what, *rows)
 
 
-def _rows_ptr_or_raise(x, what: str, need: int):
+def _rows_ptr_or_raise(x, what: str, need: int, ld: int, w: int, heads: int):
     if x is None or isinstance(x, int):
         return x
     torch = _torch or _import_torch()
@@ -502,6 +504,20 @@ def _rows_ptr_or_raise(x, what: str, need: int):
         raise TypeError(f"{what}: dtype must be {torch.float32}, got {x.dtype}")
     if x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
         raise ValueError(f"{what}: the elements of a row must lie side by side, the last stride is {x.stride(-1)}")
+    if not x.is_contiguous():
+        run, outside = 1, False  # floats side by side so far; the dimensions from here on go from row to row
+        ones = 2 if heads == 1 else 1  # dimensions of 1 behind a row: its one head, one row
+        for size, stride in zip(reversed(x.shape), reversed(x.stride())):
+            if size == 1:
+                ones -= run >= w
+                outside = outside or ones == 0
+            elif not outside and stride == run and run < w:
+                run *= size
+            elif stride != ld if not outside else stride == 0 or ld > 0 and stride % ld:
+                raise ValueError(f"{what}: a tensor of shape {tuple(x.shape)} and strides {x.stride()} does not hold rows of {w} "
+                                 f"floats {ld} apart")
+            else:
+                outside = True
     has = x.untyped_storage().nbytes() // 4 - x.storage_offset()
     if need > 0 and (x.numel() == 0 or has < need):
         raise ValueError(f"{what}: needs at least {need} elements from its first one on, has {has}")
@@ -509,7 +525,8 @@ def _rows_ptr_or_raise(x, what: str, need: int):
 
 
 def _attention_needs(a: Attention):
-    """The floats from the first element of q, k, v and out to the end of their last rows."""
+    """Of q, k, v and out the floats from the first element to the end of the last row, from row to row and in a row, and
+    the heads."""
     if a.nseq > a._most:
         raise ValueError(f"nseq: {a.nseq} sequences, the offsets hold {a._most}")
     if not _one_device:
@@ -517,14 +534,16 @@ def _attention_needs(a: Attention):
             _here(t, name)
     rq, rk, HS = a.rows_q - 1, a.rows_k - 1, a.HS
     wq, wk = a.NH * HS, a.NKV * HS
-    return (rq * (a.ldq or wq) + wq if rq >= 0 else 0, rk * (a.ldk or wk) + wk if rk >= 0 else 0,
-            rk * (a.ldv or wk) + wk if rk >= 0 else 0, rq * (a.ldo or wq) + wq if rq >= 0 else 0)
+    return [(r * ld + w if r >= 0 else 0, ld, w, n)
+            for r, ld, w, n in ((rq, a.ldq or wq, wq, a.NH), (rk, a.ldk or wk, wk, a.NKV), (rk, a.ldv or wk, wk, a.NKV),
+                                (rq, a.ldo or wq, wq, a.NH))]
 
 
 def attention_forward(out, lse, q, k, v, a: Attention) -> None:
     """gpt2_kernels.cuh:416-498, for grouped heads, sequences of different lengths and a cache too: per query row and
     head ``out = softmax(scale q.k) v`` over the allowed keys and ``lse = log sum exp`` (rows_q, NH), which may be
-    None. q, k, v and out may be views into rows that hold other things as well (strides in ``a``)."""
+    None. q, k, v and out may be views into rows that hold other things as well, ``ldq``, ``ldk``, ``ldv`` and ``ldo`` of ``a``
+    apart; a view whose rows are not is refused."""
     nq, nk, nv, no = _attention_needs(a)
     pq, pk, pv, po = _rows_ptr(q, "q", nq), _rows_ptr(k, "k", nk), _rows_ptr(v, "v", nv), _rows_ptr(out, "out", no)
     _check(lib.ugk_attention_forward(po, _ptr_here(lse, "lse", a.rows_q * a.NH), pq, pk, pv, a))
