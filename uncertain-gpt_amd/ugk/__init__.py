@@ -532,11 +532,11 @@ def _attention_needs(a: Attention):
     if not _one_device:
         for t, name in zip(a._tensors, a._OFFSETS):
             _here(t, name)
-    rq, rk, HS = a.rows_q - 1, a.rows_k - 1, a.HS
-    wq, wk = a.NH * HS, a.NKV * HS
-    return [(r * ld + w if r >= 0 else 0, ld, w, n)
-            for r, ld, w, n in ((rq, a.ldq or wq, wq, a.NH), (rk, a.ldk or wk, wk, a.NKV), (rk, a.ldv or wk, wk, a.NKV),
-                                (rq, a.ldo or wq, wq, a.NH))]
+    rq, rk, HS, NH, NKV = a.rows_q - 1, a.rows_k - 1, a.HS, a.NH, a.NKV
+    wq, wk = NH * HS, NKV * HS
+    lq, lk, lv, lo = a.ldq or wq, a.ldk or wk, a.ldv or wk, a.ldo or wq
+    return ((rq * lq + wq if rq >= 0 else 0, lq, wq, NH), (rk * lk + wk if rk >= 0 else 0, lk, wk, NKV),
+            (rk * lv + wk if rk >= 0 else 0, lv, wk, NKV), (rq * lo + wq if rq >= 0 else 0, lo, wq, NH))
 
 
 def attention_forward(out, lse, q, k, v, a: Attention) -> None:
