@@ -1495,7 +1495,7 @@ int dkv_splits(const ugk_attention &a) {
   return (int)max(1LL, min(min(min(want, keys), (long long)kMaxSplits), rows / 128));
 }
 
-constexpr int kFewRows = 4, kFewChunk = 1024;  // rows of k_att_few; keys per part
+constexpr int kFewRows = 4, kFewChunk = 1024, kFewWide = 2048;  // rows of k_att_few; keys per part; keys of large workgroups
 constexpr size_t kMaxParts = 1 << 15;  // rows of a head that the parts hold at most
 
 // How the forward of `a` is cut: rows per key/value head where they are few and their
@@ -1510,7 +1510,10 @@ FwdPlan fwd_plan(const ugk_attention &a) {
   if (rows <= kFewRows) {
     p.few = rows <= 1 ? 1 : rows <= 2 ? 2 : 4;
     p.tiles = 1;
-    p.W = pairs < 4 * cu_count() && a.max_k <= kFewChunk ? few_waves(p.few) : 4;
+    // Large workgroups for short caches, which make few parts: 24 sequences, 32/8 heads of 128, of up to 512, 1,024,
+    // 1,536 and 2,048 keys 17, 28, 28 and 36 us, 23, 40, 37 and 46 in workgroups of four wavefronts; 16 of 12
+    // heads of 64 10, 13, 17 and 23, and 10, 14, 21 and 27. Of up to 4,096 49 and 44 (79 and 83 with 128).
+    p.W = pairs < 4 * cu_count() && a.max_k <= kFewWide ? few_waves(p.few) : 4;
     unit = p.W * (a.HS <= 64 ? 4 : 2) * few_loads(p.few);
   } else {
     // Two 32-row blocks per wavefront halve the staging and the reads of K and V per
