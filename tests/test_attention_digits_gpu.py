@@ -371,3 +371,38 @@ def test_scores_of_the_lowest_value(gpu, masked, lq, lk, NH, NKV, HS):
                 # e^x - 1 for the relative error x of a weight, which may pass 1 where scores are in the hundreds
                 tol = size * (torch.expm1(rel) + (2 * n + 32) * U) + n * 2.0 ** -23 * (P * top(v[:n // 2])[None]).amax(1, keepdim=True)
                 inside(out[rq, h], want, tol + 2.0 ** -29 * v.abs().amax(), "out")
+
+
+def zero_rows(gpu, name, lq, lk, NH, NKV, HS):
+    """Rows of zeros among the others, scores of up to hundreds: often all the weight falls on a value of zeros."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)
+    by_row(c, 3, 11, ["q", "k"])
+    t = getattr(c, name)
+    t[torch.rand(t.shape[0], generator=torch.Generator().manual_seed(5)).to(DEV) < 0.3] = 0.0
+    return c
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("name", ["k", "v"])
+def test_rows_of_zeros(gpu, name, lq, lk, NH, NKV, HS):
+    check_forward(zero_rows(gpu, name, lq, lk, NH, NKV, HS))
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+def test_gradients_of_rows_of_zeros(gpu, name, lq, lk, NH, NKV, HS):
+    check_backward(zero_rows(gpu, name, lq, lk, NH, NKV, HS))
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+@pytest.mark.parametrize("far", [30.0, 1000.0])
+def test_all_the_weight_on_a_value_of_zeros(gpu, far, lq, lk, NH, NKV, HS):
+    """The first key has a score `far` above the others and a value of zeros: what is left is the others', e^-far of them."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS)
+    c.q[:, :, 0] = (far / c.scale) ** 0.5
+    c.k[:, :, 0] = 0.0
+    for k0 in c.s.k:
+        c.k[k0, :, 0] = (far / c.scale) ** 0.5
+        c.v[k0] = 0.0
+    check_forward(c)
+    check_backward(c)

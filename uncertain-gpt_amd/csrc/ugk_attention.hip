@@ -306,15 +306,16 @@ __device__ __forceinline__ void lower(v16f &c, const Lifts<kRows> &l, int z, int
 }
 
 // The rows of a wavefront's blocks lifted, and what they were lifted by noted for tile z, where one of them
-// lies far below its tile's largest; bit z of *lifted: this was so. operand(u), exponent(u) and first(u): a block's.
+// lies far below its tile's largest; bit z of *lifted: this was so. The tile has `rows` rows. operand(u), exponent(u)
+// and first(u): a block's.
 template <int DG, int kStep, int kPer, int kRows, typename Operand, typename Exponent, typename First>
-__device__ __forceinline__ void lift_tile(Rows4 (&t)[kPer], Lifts<kRows> &l, int z, int lane, int wave, int *lifted,
+__device__ __forceinline__ void lift_tile(Rows4 (&t)[kPer], Lifts<kRows> &l, int z, int rows, int lane, int wave, int *lifted,
                                           Operand operand, Exponent exponent, First first) {
   bool any = false;
 #pragma unroll
   for (int u = 0; u < kPer; u++) {
     int d[4];
-    any = lift_rows<DG>(t[u], exponent(u), d) || any;
+    any = lift_rows<DG, kStep>(t[u], exponent(u), rows - first(u), d) || any;
     if (lane % DG == 0) {
 #pragma unroll
       for (int r = 0; r < 4; r++) l.d[z][operand(u)][first(u) + kStep * r] = d[r];
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   };
   int ek_next = 0, ev_next = 0;  // of the tile staged last
   int lifted = 0;                // bit z: this wavefront's rows of tile z are
-  const auto stage = [&](int at) {
+  const auto stage = [&](int at, int k0) {
     const uint32_t mk = noted<W>(slot[at][0]), mv = noted<W>(slot[at][1]);
     bad = bad || mk >= kInfBits || mv >= kInfBits;
     ek_next = split_exp(mk);
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 #pragma unroll
     for (int u = 0; u < kPer; u++) spread = spread || may_spread(small[u], is_v(u) ? mv : mk);
     if (__builtin_expect(__any(spread) || (lifted >> at & 1), 0))
-      lift_tile<DG, KG>(t, lifts, at, lane, wave, &lifted, [&](int u) { return is_v(u) ? 1 : 0; },
+      lift_tile<DG, KG>(t, lifts, at, n - k0, lane, wave, &lifted, [&](int u) { return is_v(u) ? 1 : 0; },
                         [&](int u) { return is_v(u) ? ev_next : ek_next; }, [&](int u) { return block(u) / DG; });
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
@@ -561,7 +562,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     load(first);
     note(0, first);
     __syncthreads();
-    stage(0);
+    stage(0, first);
     if (tiles > 1) {
       load(first + BK);
       note(1, first + BK);
@@ -570,7 +571,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
     for (int at = 0; at < tiles; at++) {
       const int k0 = first + at * BK, ek = ek_next, ev_now = ev_next;
       // tile at + 1: its maxima are noted, its buffer was read two barriers ago
-      if (at + 1 < tiles) stage((at + 1) & 1);
+      if (at + 1 < tiles) stage((at + 1) & 1, k0 + BK);
       if (at + 2 < tiles) load(k0 + 2 * BK);
       if (k0 < hi) compute(at & 1, k0, ek, ev_now);
       if (at + 2 < tiles) note(at & 1, k0 + 2 * BK);
@@ -1098,7 +1099,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
 #pragma unroll
     for (int u = 0; u < kPer; u++) spread = spread || may_spread(small[u], is_v(u) ? mv : mk);
     if (__any(spread) || (lifted >> z & 1))
-      lift_tile<DG, KG>(t, lifts, z, lane, wave, &lifted, [&](int u) { return is_v(u) ? 1 : 0; },
+      lift_tile<DG, KG>(t, lifts, z, n - at * BK, lane, wave, &lifted, [&](int u) { return is_v(u) ? 1 : 0; },
                         [&](int u) { return is_v(u) ? ev : ek; }, [&](int u) { return block(u) / DG; });
     const float fk = split_scale(ek), fv = split_scale(ev);
 #pragma unroll
@@ -1323,7 +1324,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   };
   int eq = 0, eg = 0;  // of the tile staged last
   int lifted = 0;
-  const auto stage = [&](int z) {
+  const auto stage = [&](int z, int r0) {
     const uint32_t mq = noted<W>(slot[z][0]), mg = noted<W>(slot[z][1]);
     bad = bad || mq >= kInfBits || mg >= kInfBits || noted<W>(slot[z][2]) >= 0x4a800000u /* 2^22 */;
     eq = split_exp(mq);
@@ -1332,7 +1333,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
 #pragma unroll
     for (int u = 0; u < kPer; u++) spread = spread || may_spread(small[u], is_g(u) ? mg : mq);
     if (__any(spread) || (lifted >> z & 1))
-      lift_tile<DG, KG>(t, lifts, z, lane, wave, &lifted, [&](int u) { return is_g(u) ? 1 : 0; },
+      lift_tile<DG, KG>(t, lifts, z, rows - r0, lane, wave, &lifted, [&](int u) { return is_g(u) ? 1 : 0; },
                         [&](int u) { return is_g(u) ? eg : eq; }, [&](int u) { return block(u) / DG; });
     const float fq = split_scale(eq), fg = split_scale(eg);
 #pragma unroll
@@ -1401,7 +1402,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     load(from);
     note(0, from);
     __syncthreads();
-    stage(0);
+    stage(0, from);
     if (tiles > 1) {
       load(from + BQ);
       note(1, from + BQ);
@@ -1409,7 +1410,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
     __syncthreads();
     for (int at = 0; at < tiles; at++) {
       const int r0 = from + at * BQ, eq_now = eq, eg_now = eg;
-      if (at + 1 < tiles) stage((at + 1) & 1);
+      if (at + 1 < tiles) stage((at + 1) & 1, r0 + BQ);
       if (at + 2 < tiles) load(r0 + 2 * BQ);
       if (r0 + BQ > lo) compute(at & 1, r0, eq_now, eg_now);
       if (at + 2 < tiles) note(at & 1, r0 + 2 * BQ);

@@ -188,17 +188,19 @@ __device__ __forceinline__ uint32_t max_abs(uint32_t m, const Rows4 &t, uint32_t
   return __float_as_uint(fmaxf(fmaxf(f, q[2]), q[3]));
 }
 // A tile is held at the scale of its largest magnitude where its rows' largest are within 2^kSpread of that, else
-// rows are taken times 2^-d, d <= 0, to the largest's binade, and d goes along with the tile.
-constexpr int kSpread = 6;
+// rows are taken times 2^-d, d <= 0, to the largest's binade, and d goes along with the tile. A row of zeros has a
+// d below all others: what it is multiplied by counts for nothing, however large.
+constexpr int kSpread = 6, kZeroRow = -(1 << 24);
 __device__ __forceinline__ bool may_spread(uint32_t least, uint32_t largest) { return least + ((uint32_t)kSpread << 23) < largest; }
-// The wavefront's rows, kLanes lanes to four of them, in a tile of exponent e; whether one of them lies that far below.
-template <int kLanes>
-__device__ __forceinline__ bool lift_rows(Rows4 &t, int e, int (&d)[4]) {
+// The wavefront's rows, kLanes lanes to four of them kStep apart, in a tile of exponent e; whether one of them lies that
+// far below. `rows`: the tile's rows from the first of the lane's four on (behind them are zeros that nothing reads).
+template <int kLanes, int kStep>
+__device__ __forceinline__ bool lift_rows(Rows4 &t, int e, int rows, int (&d)[4]) {
   bool below = false;
 #pragma unroll
   for (int r = 0; r < 4; r++) {
     const uint32_t x = row_max_bits<kLanes>(max_abs(0u, t.r[r]));
-    d[r] = x ? min(split_exp(x) - e, 0) : 0;  // rows of zeros stay
+    d[r] = x ? min(split_exp(x) - e, 0) : kStep * r < rows ? kZeroRow : 0;
     below = below || d[r] < -kSpread;
   }
   below = __any(below);
