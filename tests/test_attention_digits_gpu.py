@@ -406,3 +406,21 @@ def test_all_the_weight_on_a_value_of_zeros(gpu, far, lq, lk, NH, NKV, HS):
         c.v[k0] = 0.0
     check_forward(c)
     check_backward(c)
+
+
+@pytest.mark.parametrize("which,spread", [("k", 3), ("v", 12), ("zeros", 0)])
+def test_sizes_that_change_with_two_blocks_a_wavefront(gpu, which, spread):
+    """Keys and values of different sizes, and of zeros, where a wavefront takes two blocks of rows."""
+    c = Call(gpu, Seqs([70], [300]), 800, 800, 64)
+    if which == "zeros":
+        c.v[::3] = 0.0
+        c.q.mul_(8.0)
+    else:
+        by_row(c, spread, 3, [which])
+    out, lse = c.forward()
+    for heads in (slice(0, 3), slice(797, 800)):
+        d = Call(gpu, c.s, 3, 3, 64)
+        d.q, d.k, d.v = c.q[:, heads], c.k[:, heads], c.v[:, heads]
+        w = results(d)
+        inside(out[:, heads], *w["out"], "out")
+        inside(lse[:, heads], *w["lse"], "lse")

@@ -27,8 +27,9 @@ def test_a_config_without_heads_needs_none():
 @pytest.mark.gpu
 def test_reserve_without_heads_holds_none(gpu):
     gpu.set_workspace(None, gpu.Config(B=1, T=1, C=64, V=2, NH=0, maxT=1, L=0))
+    kept = gpu.scratch_bytes()  # for graphs of other tests
     gpu.reserve(8192, 768)
-    assert gpu.scratch_bytes() <= 22 << 20
+    assert gpu.scratch_bytes() - kept <= 22 << 20
     x = torch.randn(2 * 64, 3 * 128, device=DEV)
     g, out = torch.zeros_like(x), torch.empty(2 * 64, 128, device=DEV)
     gpu.dense_attention_forward(out, x, 2, 64, 128, 2)
