@@ -137,9 +137,9 @@ __device__ void row_forward(float *out, float *lse, float *ml, size_t ml_step, c
 // What bounds it: on gfx950 a wavefront's matrix instruction holds back the vector
 // instructions of every wavefront on its SIMD (8 x (mfma, 4 fma): 20.2 ns per pair with one
 // wavefront, 18.0 with two, of which the mfma alone takes 14.3), so the two
-// add up. 16,384 rows of 12 heads of 64 take 1,283 us (1,248 to 1,325 from card to card): 321 TFLOP/s of products counted
-// once, 963 of halves. That is 1.67 us for a SIMD's block of 32 rows and 64 keys, of which
-// its 48 mfma take 0.69; the same products in single precision
+// add up. 16,384 rows of 12 heads of 64 take 1,313 us (1,268 to 1,345 from card to card): 314 TFLOP/s of products counted
+// once, 942 of halves. That is 1.71 us for a SIMD's block of 32 rows and 64 keys, of which
+// its 48 mfma take 0.69 (by counters 42% of the time, vector instructions 55%); the same products in single precision
 // (v_mfma_f32_32x32x2_f32, 128 of 64 cycles) would take 3.7. An earlier state of this kernel
 // took 1,530 us for 4 x 8,192 rows, and 1,122 without loading, splitting and storing the
 // tiles. Tried without gain: K and V read ahead from LDS during the softmax (72.0
@@ -152,8 +152,8 @@ __device__ void row_forward(float *out, float *lse, float *ml, size_t ml_step, c
 // (and the accumulators with it) only when one lies 2^7 above it: P then stays
 // below 2^(kTop + 7), the halves' range.
 //
-// 8 x 1,024 rows of 12 heads of 64 whose values are of one size take 64 us, and 100 us where they are
-// times 2^-8 to 2^8 from row to row; 13 packed sequences of 16/4 heads of 128 121 and 183. (Looking for such rows costs
+// 8 x 1,024 rows of 12 heads of 64 whose values are of one size take 65 us, and 99 us where they are
+// times 2^-8 to 2^8 from row to row; 13 packed sequences of 16/4 heads of 128 122 and 192. (Looking for such rows costs
 // 1 to 2% where there are none; row by row the two took 25.9 and 54.5 ms.)
 constexpr float kTop = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
@@ -918,13 +918,13 @@ __device__ void row_dkv(float *dkj, float *dvj, const float *dout, const float *
 // what its accumulators stand on follows what it has seen alone: the largest P of a
 // key times the largest of dout's row, the largest dS times that of q's or k's. Rows that lie far
 // below their tile's largest are lifted, and others taken one by one, as in the forward: 8 x 1,024 rows of 12 heads
-// with dout's rows times 2^-8 to 2^8 take 250 us against 210, 4 x 2,048 of 16/4 heads of 128 1,430 against 1,140
+// with dout's rows times 2^-8 to 2^8 take 253 us against 210, 4 x 2,048 of 16/4 heads of 128 1,460 against 1,150
 // (row by row 26 and 123 ms).
 //
 // The same sum of matrix and vector instructions bounds them: of 858 (dk, dv) and 633 us
 // (dq) at 4 x 4,096 rows of 12 heads, 612 and 465 were left without loading,
-// splitting and storing the tiles. 8 x 1,024 rows of 12 heads: 128 and 100 us, 220
-// with the launches (146 TFLOP/s of 10 HS operations per pair). Workgroups of
+// splitting and storing the tiles. 8 x 1,024 rows of 12 heads: 137 and 103 us, 222
+// as calls among others (145 TFLOP/s of 10 HS operations per pair). Workgroups of
 // one wavefront were slower at every size tried.
 
 // acc += A^T B for a 32-row block of B held in an accumulator's registers (C, scaled
@@ -1617,8 +1617,8 @@ int launch_attention_backward(float *dq, float *dk, float *dv, const float *dout
   float *dsum = mem;
   const unsigned pairs = (unsigned)a.nseq * a.NKV;
   // Head sizes of 65 to 127 that are multiples of 4 (80, 96, ..) have kernels of their own: reading
-  // the rows' ends float by float costs dk and dv 352 bytes a lane of spills (4 x 2,048 rows of
-  // 16/4 heads of 100: 1,229 us, 1,699 in the general form, which up to 64 spills nothing).
+  // the rows' ends float by float costs dk and dv 288 bytes a lane of spills (4 x 2,048 rows of
+  // 16/4 heads of 100: 1,225 us, 1,705 in the general form, which up to 64 spills nothing).
   const bool wide = a.HS > 64, full = a.HS == (wide ? 128 : 64), quads = a.HS % 4 == 0;
   if (const long long rows = (long long)a.max_q * (a.NH / a.NKV)) {
     const auto go = [&](auto kernel) {
