@@ -130,9 +130,9 @@ __device__ void row_forward(float *out, float *lse, float *ml, size_t ml_step, c
 // scale), not next to the largest P or the largest V: a large value of little weight
 // leaves the others their digits, and what a row must not see moves nothing.
 //
-// The workgroup's rows are taken one by one instead (row_forward), where a masked key
-// is not touched at all, if a tile holds an infinity, or NaN that not all rows see,
-// or if scores leave the range of the above (2^22 in base 2).
+// A wavefront's rows are taken one by one instead (row_forward), where a masked key
+// is not touched at all, if a tile that some of them see holds an infinity, or NaN that not
+// all of the workgroup's see, or if scores leave the range of the above (2^22 in base 2).
 //
 // What bounds it: on gfx950 a wavefront's matrix instruction holds back the vector
 // instructions of every wavefront on its SIMD (8 x (mfma, 4 fma): 20.2 ns per pair with one
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   int lifted = 0;                // bit z: this wavefront's rows of tile z are
   const auto stage = [&](int at, int k0) {
     const uint32_t mk = noted<W>(slot[at][0]), mv = noted<W>(slot[at][1]);
-    bad = bad || mk >= kInfBits || mv >= kInfBits;
+    bad = bad || (k0 < hi && (mk >= kInfBits || mv >= kInfBits));
     ek_next = split_exp(mk);
     ev_next = split_exp(mv);
     const float fk = split_scale(ek_next), fv = split_scale(ev_next);
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
   // a row all of whose scores passed the range downwards: what it stands on never moved
 #pragma unroll
   for (int u = 0; u < QB; u++) bad = bad || (lim[u] > first && one[u] > 1e38f);
-  // Any wavefront's trouble with a tile is every wavefront's; with its scores its own.
+  // trouble with a tile that the wavefront's rows see, or with their scores
   if (__any(bad)) {
     for (int x = 0; x < 32 * QB; x++) {
       const int rr = row0 + wave * (32 * QB) + x;
@@ -1092,7 +1092,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dq(
   const auto stage = [&](int at) {
     const int z = at & 1;
     const uint32_t mk = noted<W>(slot[z][0]), mv = noted<W>(slot[z][1]);
-    bad = bad || mk >= kInfBits || mv >= kInfBits;
+    bad = bad || (at * BK < hi && (mk >= kInfBits || mv >= kInfBits));
     ek = split_exp(mk);
     ev = split_exp(mv);
     bool spread = false;
@@ -1326,7 +1326,7 @@ __global__ __launch_bounds__(kTileThreads, HSP > 64 ? 1 : 2) void k_att_dkv(
   int lifted = 0;
   const auto stage = [&](int z, int r0) {
     const uint32_t mq = noted<W>(slot[z][0]), mg = noted<W>(slot[z][1]);
-    bad = bad || mq >= kInfBits || mg >= kInfBits || noted<W>(slot[z][2]) >= 0x4a800000u /* 2^22 */;
+    bad = bad || (r0 + BQ > lo && (mq >= kInfBits || mg >= kInfBits || noted<W>(slot[z][2]) >= 0x4a800000u /* 2^22 */));
     eq = split_exp(mq);
     eg = split_exp(mg);
     bool spread = false;
