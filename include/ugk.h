@@ -29,17 +29,18 @@
  * sums (one slot per call, 2L+1 for the step driver), the encoder backward's
  * bucket state, the KL total's partial sums, the softmax's row
  * statistics (rows too long for one workgroup, and the exact mode's), and
- * attention's row sums and parts of a split axis, each in a region of its own. By default the library allocates
- * a region on the first call that needs it and grows it, after waiting for
- * the device, when a larger shape arrives; ugk_reserve / ugk_reserve_config
- * allocate everything up front, after which calls at those shapes neither
- * allocate nor wait. A call under HIP graph capture that would have to
- * allocate fails with UGK_ENOMEM before launching anything (reserve first, or
+ * attention's row sums and parts of a split axis, each in a region of its own. By
+ * default the library allocates a region on the first call that needs it and grows
+ * it, after waiting for the device, when a larger shape arrives; ugk_reserve /
+ * ugk_reserve_config allocate everything up front, after which calls at those
+ * shapes neither allocate nor wait. A call under HIP graph capture that would have
+ * to allocate fails with UGK_ENOMEM before launching anything (reserve first, or
  * make one call at that shape outside the capture). Memory that a captured call
  * uses is kept for the graph's replays, also when the region grows later (it then
  * doubles at least), until ugk_release_graph_memory. Replays use the workspace as
  * calls do: two graphs, or a graph and a call, must not run at the same time. A
- * caller that owns all device memory (as the reference's arms do) sizes a workspace with ugk_workspace_bytes and hands it over with
+ * caller that owns all device memory (as the reference's arms do) sizes a
+ * workspace with ugk_workspace_bytes and hands it over with
  * ugk_set_workspace; the library then never allocates. The workspace is used
  * in stream order: ugk_set_stream waits for the work already queued on the
  * previous stream, so calls on two streams never share it at once. The

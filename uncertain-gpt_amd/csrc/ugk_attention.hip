@@ -74,8 +74,8 @@ __device__ __forceinline__ float weight(float s, float m) { return s == -INFINIT
 
 // One query row of one head by one wavefront: lanes over keys for the scores,
 // over channels for the sum. To lse, or the maximum and the sum behind it to ml (if not null) and ml[ml_step].
-__device__ void row_forward(float *out, float *lse, float *ml, size_t ml_step, const float *q, const float *k, const float *v, int n, int HS,
-                            long long ldk, long long ldv, float scale) {
+__device__ void row_forward(float *out, float *lse, float *ml, size_t ml_step, const float *q, const float *k,
+                            const float *v, int n, int HS, long long ldk, long long ldv, float scale) {
   const int lane = threadIdx.x & (kWave - 1);
   float m = -INFINITY;
   for (int j = lane; j < n; j += kWave) m = fmaxf(m, dot(q, k + j * ldk, HS) * scale);
