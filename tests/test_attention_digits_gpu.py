@@ -424,3 +424,21 @@ def test_sizes_that_change_with_two_blocks_a_wavefront(gpu, which, spread):
         w = results(d)
         inside(out[:, heads], *w["out"], "out")
         inside(lse[:, heads], *w["lse"], "lse")
+
+
+@pytest.mark.parametrize("lq,lk,NH,NKV,HS", SHAPES)
+def test_scores_near_the_highest_value(gpu, lq, lk, NH, NKV, HS):
+    """One key at the highest score that is a number takes all the weight, NaN elsewhere stays NaN."""
+    c = Call(gpu, Seqs(lq, lk), NH, NKV, HS, scale=1.0)
+    c.q[:, :, 0] = 1.0
+    for k0 in c.s.k:
+        c.k[k0, :, 0] = 3.4028234663852886e38
+    out, lse = c.forward()
+    for b in range(len(c.s.lq)):
+        for h in range(NH):
+            rq, rk, q, k, v = att_ref._pieces(c.s, b, h, NH // NKV, c.q, c.k, c.v)
+            assert (out[rq, h].double() - v[0]).abs().max() <= 2.0 ** -22 * v[0].abs().max()
+            assert (lse[rq, h] == 3.4028234663852886e38).all()
+    c.k[c.s.k[0], :, 0] = math.nan
+    out, lse = c.forward()
+    assert out[c.s.q[0]:c.s.q[0] + c.s.lq[0]].isnan().all()

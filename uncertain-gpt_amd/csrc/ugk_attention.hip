@@ -578,9 +578,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
       __syncthreads();
     }
   }
-  // a row all of whose scores passed the range downwards: what it stands on never moved
+  // a row all of whose scores passed the range downwards (none is NaN): what it stands on never moved
 #pragma unroll
-  for (int u = 0; u < QB; u++) bad = bad || (lim[u] > first && one[u] > 1e38f);
+  for (int u = 0; u < QB; u++) bad = bad || (lim[u] > first && one[u] > 1e38f && l[u] == 0.0f);
   // trouble with a tile that the wavefront's rows see, or with their scores
   if (__any(bad)) {
     for (int x = 0; x < 32 * QB; x++) {
@@ -628,8 +628,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_att_fwd(float *out, float *
 // between groups until the end); its score sums go through DPP. The groups, then the
 // workgroup's NW wavefronts, are joined at the end in their order, through LDS.
 // Single precision throughout, and a key that a row must not see is left out by
-// selects, so nothing of it reaches the row. A row whose scores all leave the range in base 2 (or hold a NaN, or an infinity)
-// is computed by row_forward.
+// selects, so nothing of it reaches the row. A row whose scores all leave the range in base 2
+// downwards, or one upwards, is computed by row_forward.
 //
 // 24 sequences of 8,192 keys, 8 key/value heads of 128: 271 us with one query head for
 // each, 277 with four (1,611 MB, 5.8 to 6.0 TB/s); 64 of 2,048, 12 heads of 64, 144 us (805
@@ -769,7 +769,7 @@ __global__ __launch_bounds__(NW * kWave) void k_att_few(float *out, float *lse, 
       sum = fmaf(ll[w][r], f, sum);
       t = make_float4(fmaf(y.x, f, t.x), fmaf(y.y, f, t.y), fmaf(y.z, f, t.z), fmaf(y.w, f, t.w));
     }
-    lost = !(sum > 0.0f) && min(stop, s.seen(i, a.causal)) > first;
+    lost = (sum == 0.0f || top == INFINITY) && min(stop, s.seen(i, a.causal)) > first;
     const bool any = sum != 0.0f;  // else no key
     const float f = any ? 1.0f / sum : 0.0f;
     t = any ? make_float4(t.x * f, t.y * f, t.z * f, t.w * f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
