@@ -448,6 +448,101 @@ int ugk_dense_attention_forward(void *ctx, float *out, const float *qkv, int B,
 int ugk_dense_attention_backward(void *ctx, float *dqkv, const float *dout,
                                  const float *qkv, int B, int T, int C, int NH);
 
+/* ---- generation from a cache in 8 bits --------------------------------------
+ * No counterpart in the reference, which computes every position again for each
+ * token. A cache is `nblocks` blocks of UGK_CACHE8_BLOCK tokens, which a table deals
+ * out to the sequences in any order: k8 and v8 (ugk_cache8_bytes each, 16-byte
+ * aligned) hold the codes, ks and vs (nblocks, NKV) a scale per block and
+ * key/value head. A number is its code times the scale; codes are whole, -127 to 127, and
+ * scales powers of two (or 0, of zeros). With HP = HS rounded up to a
+ * multiple of 16, element d of key i of block n and head h has its code at
+ *     k8[((n NKV + h) 64 + i) HP + d]
+ *     v8[((n NKV + h) HP + d) 64 + 4 (i % 16) + i / 16]
+ * A pass over new tokens stores their keys and values, attends, and shortens k_len
+ * again by the tokens that it does not keep. */
+#define UGK_CACHE8_BLOCK 64
+typedef struct {
+  int nseq;           /* sequences */
+  int NH, NKV, HS;    /* as in ugk_attention */
+  int rows_q;         /* rows of q, out, lse and of store's and load's k and v */
+  int max_q, max_k;   /* the most of these rows and the most keys of a sequence */
+  int nblocks;        /* blocks of the cache */
+  int causal;         /* nonzero: row i of Lq sees the keys j <= i + Lk - Lq */
+  float scale;        /* of the scores */
+  /* DEVICE arrays. Sequence b has the rows [q_start[b], q_end[b]), its last
+   * positions, and k_len[b] keys with these; block table[b ld_table + j] holds its
+   * keys 64 j to 64 j + 63. NULL: rows [b max_q, (b + 1) max_q), and rows_q must be nseq *
+   * max_q; max_k keys; block b ld_table + j, and nblocks must be at least nseq * ld_table.
+   * Rows and lengths beyond the buffers and max are clamped, blocks beyond nblocks are left out, and the next
+   * ugk_synchronize reports either. */
+  const int *q_start, *q_end, *k_len, *table;
+  int ld_table;       /* 0: max_k / 64 rounded up, which is also the least */
+  /* floats from a row to the next of q, of store's and load's k and v, of out; 0:
+   * rows without gaps */
+  long long ldq, ldk, ldv, ldo;
+} ugk_cache8;
+
+/* Bytes of k8, and of v8. 0 where a size is out of range. */
+size_t ugk_cache8_bytes(int nblocks, int NKV, int HS);
+
+/* Stores the rows of k and v as the last keys of their sequences. A block's scale is
+ * the least power of two s with |x| <= 127 s for all its rows so far (2^-126 to
+ * 2^121; beyond, numbers are held as 127 2^121); a code is x / s rounded to the
+ * nearest, ties to even. A call that begins at a block's first key begins the block
+ * anew; one that continues a block keeps its scale or raises it, and then rounds
+ * its older codes again, in place: an element is off by half a step of its block's
+ * scale at most, or by less than a step once the scale has been raised. Two sequences
+ * must not share a block that the call writes. NaN is stored as 0; it and infinities are
+ * reported by the next ugk_synchronize, as are sequences of more rows than keys,
+ * whose first rows are not stored. */
+int ugk_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k,
+                     const float *v, ugk_cache8 a);
+/* What the cache holds in the store's place, to rows of k and v (exact). */
+int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks,
+                    const void *v8, const float *vs, ugk_cache8 a);
+
+/* ugk_attention_forward of q against the cache: out, and lse (rows_q, NH) if not
+ * NULL. A row without a key that it sees has out 0 and lse -infinity. A row of q (of one
+ * head) enters as whole numbers of 31 bits next to its largest element, or, with more than 32 query rows
+ * times heads per key/value head, as two half-precision numbers per element, to 2^-23 of the
+ * element and 2^-38 of the largest; weights to 2^-31, or to 2^-23 of the weight and 2^-38 of the largest of
+ * their block; statistics and sums are in single precision. A score of 2^127 or more, and a row of q
+ * with an infinity or NaN, has the row's out and lse NaN. out must not overlap q.
+ * weight, if not NULL, (nseq, ld_table): weight[b, j] += the sum of the weights, over
+ * sequence b's rows and heads and the keys of its block j. For up to 256 rows and heads per
+ * key/value head: tokens, drafts, or the last rows of a prompt. Deterministic. The
+ * workspace for it is 8 bytes per row, head and block. */
+int ugk_cache8_attention(float *out, float *lse, const float *q, const void *k8,
+                         const float *ks, const void *v8, const float *vs,
+                         float *weight, ugk_cache8 a);
+
+/* Takes all but `keep` blocks out of the rows of a table: of a sequence with n = k_len[b] /
+ * 64 rounded up blocks, n > keep, the d = n - keep of least weight (of equals the first) among those
+ * behind the `first` first and before the `recent` last, which always stay (first + recent
+ * <= keep, recent >= 1). In row b the n - d blocks that stay come first, in their
+ * order, then the entries from n on, then the d that went: those are free, and where the
+ * sequence grows into next if the row has no others. weight_out goes along (0 for all that are not in
+ * use), len_out[b] = k_len[b] - 64 d, dropped[b] = d. The cache itself is left alone. Outputs may be the inputs
+ * (table_out table, len_out k_len, weight_out weight). Weights order as numbers, NaN above all.
+ * ld, entries per row, up to 16,384 (1,048,576 tokens). */
+int ugk_cache8_evict(int *table_out, int *len_out, float *weight_out,
+                     int *dropped, const int *table, const int *k_len,
+                     const float *weight, int nseq, int ld, int keep, int first,
+                     int recent);
+
+/* Drafted tokens against the target. Sequence b has n = n_draft[b] (NULL: K) drafts draft[b, i],
+ * drawn with the probabilities q (nseq, K, V), or certain (q NULL: 1); p (nseq, K + 1, V) are the
+ * target's, row i before draft i. Draft i is accepted where u[b, i] q[b, i, t] < p[b, i, t], until the first that is not,
+ * a = accepted[b]; the next token is then drawn from max(p[b, a] - q[b, a], 0) (p where that is 0
+ * throughout), or, all accepted, from p[b, n]: the first whose cumulative sum passes u[b, K] times the
+ * whole. With u (nseq, K + 1) uniform in [0, 1) tokens are distributed as the target's. tokens (nseq, K + 1): the accepted
+ * drafts, that token, then -1. Products and sums are in 64 bits. p and q need not add up to 1; entries
+ * that are not positive finite numbers count as 0. A draft that is no token is not accepted, and a row of p without
+ * a probability gives token 0: either, and n_draft outside [0, K], the next ugk_synchronize reports. */
+int ugk_draft_verify(int *accepted, int *tokens, const float *p, const float *q,
+                     const int *draft, const int *n_draft, const float *u,
+                     int nseq, int K, int V);
+
 /* ---- library control (no counterpart in the reference: its kernels run on
  * the CUDA legacy default stream and abort on error, gpt2_kernels.cuh:88-101) */
 
@@ -489,6 +584,12 @@ int ugk_synchronize(void);
 #define UGK_IDS_CROSSENTROPY_BACKWARD 5
 #define UGK_IDS_ATTENTION_FORWARD 6 /* the offsets of the sequences */
 #define UGK_IDS_ATTENTION_BACKWARD 7
+#define UGK_IDS_CACHE8_STORE 8 /* rows, lengths or blocks, likewise below */
+#define UGK_IDS_CACHE8_LOAD 9
+#define UGK_IDS_CACHE8_ATTENTION 10
+#define UGK_IDS_CACHE8_EVICT 11
+#define UGK_IDS_CACHE8_VALUES 12 /* NaN or an infinity to store */
+#define UGK_IDS_DRAFT_VERIFY 13
 int ugk_ids_guard(int *ids, int n, int bound, int fill, int code);
 /* The ops that index a table by ids with that check inside their own kernels:
  * ugk_ids_guard over the B*T ids (bound V, the fill and code of the op; fill -1

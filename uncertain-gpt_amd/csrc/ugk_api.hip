@@ -396,6 +396,43 @@ int check_attention(const char *fn, ugk_attention *a, bool *none) {
   return UGK_OK;
 }
 
+// *a with its strides and ld_table filled in; *none: there is nothing to compute. k and v are
+// rows of the call (not for attention).
+int check_cache8(const char *fn, ugk_cache8 *a, bool *none) {
+  *none = false;
+  if (a->nseq < 0 || a->rows_q < 0 || a->max_q < 0 || a->max_k < 0 || a->nblocks < 0)
+    return bad(fn, "nseq, rows, max and nblocks must be >= 0");
+  if (a->NH < 1 || a->NKV < 1 || a->NH % a->NKV) return bad(fn, "NKV must be >= 1 and divide NH");
+  if (a->HS < 1 || a->HS > kMaxHead) return set_error(UGK_EINVAL, "%s: HS must be 1 to %d, got %d", fn, kMaxHead, a->HS);
+  if ((long long)a->NH * a->HS > INT_MAX) return bad(fn, "NH*HS exceeds INT_MAX");
+  if (isnan(a->scale) || isinf(a->scale)) return bad(fn, "scale must be finite");
+  if (!a->q_start != !a->q_end) return bad(fn, "start and end come together");
+  if (!a->q_start && (long long)a->nseq * a->max_q != a->rows_q) return bad(fn, "rows_q must be nseq * max_q without offsets");
+  if (a->max_k > INT_MAX / 2) return bad(fn, "max_k exceeds 2^30");
+  const int blocks = (a->max_k + kCacheBlock - 1) / kCacheBlock;
+  if (!a->ld_table) a->ld_table = blocks;
+  if (a->ld_table < blocks) return bad(fn, "ld_table is less than the blocks of max_k keys");
+  if (!a->table && (long long)a->nseq * a->ld_table > a->nblocks) return bad(fn, "nblocks must be nseq * ld_table without a table");
+  const long long wq = (long long)a->NH * a->HS, wk = (long long)a->NKV * a->HS;
+  if (!a->ldq) a->ldq = wq;
+  if (!a->ldo) a->ldo = wq;
+  if (!a->ldk) a->ldk = wk;
+  if (!a->ldv) a->ldv = wk;
+  if (a->ldq < wq || a->ldo < wq || a->ldk < wk || a->ldv < wk)
+    return bad(fn, "a row stride is less than its row (NH*HS, or NKV*HS for k and v)");
+  const long long most = (long long)1 << 60, rows = a->rows_q + 1LL;  // the addresses of the last rows, in bytes
+  if (a->ldq > most / rows || a->ldo > most / rows || a->ldk > most / rows || a->ldv > most / rows)
+    return bad(fn, "rows * stride exceeds the address space");
+  a->max_q = a->max_q < a->rows_q ? a->max_q : a->rows_q;
+  if ((long long)a->max_q * (a->NH / a->NKV) > INT_MAX / 2) return bad(fn, "max_q * NH / NKV exceeds 2^30");
+  // a launch has fewer than 2^32 threads: a workgroup of 256 for 64 keys of a sequence and key/value head, or 128 rows and heads
+  const long long tq = ((long long)a->max_q * (a->NH / a->NKV) + 127) / 128 + 1, tk = blocks + 1;
+  const long long per = (long long)a->nseq * a->NKV;
+  if (per >= ((long long)1 << 23) / (tq > tk ? tq : tk)) return bad(fn, "nseq * heads * rows exceeds the grid");
+  *none = a->nseq == 0 || a->max_q == 0;
+  return UGK_OK;
+}
+
 int attention_forward(const char *fn, float *out, float *lse, const float *q, const float *k, const float *v,
                       ugk_attention a) {
   bool none;
@@ -814,6 +851,97 @@ int ugk_attention_backward_zeroed(float *dq, float *dk, float *dv, const float *
   return attention_backward("ugk_attention_backward_zeroed", dq, dk, dv, dout, q, k, v, out, lse, a, true);
 }
 
+size_t ugk_cache8_bytes(int nblocks, int NKV, int HS) {
+  if (nblocks < 0 || NKV < 1 || HS < 1 || HS > kMaxHead || (long long)NKV * HS > INT_MAX) return 0;
+  return (size_t)nblocks * NKV * kCacheBlock * ((HS + 15) / 16 * 16);
+}
+
+int ugk_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, const float *v, ugk_cache8 a) {
+  const char *fn = "ugk_cache8_store";
+  bool none;
+  if (int e = check_cache8(fn, &a, &none)) return e;
+  if (none || a.max_k == 0) return ok();
+  if (any_null({k8, ks, v8, vs, k, v})) return bad(fn, "NULL pointer");
+  if (k8 == v8 || ks == vs) return bad(fn, "k8 and v8, and ks and vs, must be distinct buffers");
+  if (!aligned16(k8) || !aligned16(v8)) return bad(fn, "k8 and v8 must be 16-byte aligned");
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  if (int e = launch_cache8_store(k8, ks, v8, vs, k, v, a, word)) return e;
+  return ok();
+}
+
+int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks, const void *v8, const float *vs, ugk_cache8 a) {
+  const char *fn = "ugk_cache8_load";
+  bool none;
+  if (int e = check_cache8(fn, &a, &none)) return e;
+  if (none || a.max_k == 0) return ok();
+  if (any_null({k8, ks, v8, vs, k, v})) return bad(fn, "NULL pointer");
+  if (k == v) return bad(fn, "k and v must be distinct buffers");
+  if (!aligned16(k8) || !aligned16(v8)) return bad(fn, "k8 and v8 must be 16-byte aligned");
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  if (int e = launch_cache8_load(k, v, k8, ks, v8, vs, a, word)) return e;
+  return ok();
+}
+
+int ugk_cache8_attention(float *out, float *lse, const float *q, const void *k8, const float *ks, const void *v8,
+                         const float *vs, float *weight, ugk_cache8 a) {
+  const char *fn = "ugk_cache8_attention";
+  bool none;
+  if (int e = check_cache8(fn, &a, &none)) return e;
+  if (weight && (long long)a.max_q * (a.NH / a.NKV) > kWeighRows)
+    return set_error(UGK_EINVAL, "%s: weights are added up for up to %d rows and heads per key/value head", fn, kWeighRows);
+  if (none) return ok();
+  if (any_null({out, q})) return bad(fn, "NULL pointer");
+  if (a.max_k > 0 && any_null({k8, ks, v8, vs})) return bad(fn, "NULL pointer");
+  if (out == q) return bad(fn, "out must be distinct from q");
+  if (!aligned16(k8) || !aligned16(v8)) return bad(fn, "k8 and v8 must be 16-byte aligned");
+  float *mem = nullptr;
+  if (const size_t bytes = cache8_attention_bytes(a, weight)) {
+    mem = static_cast<float *>(workspace(kRegAttention, bytes));
+    if (!mem) return UGK_ENOMEM;
+  }
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  if (int e = launch_cache8_attention(out, lse, q, k8, ks, v8, vs, weight, mem, a, word)) return e;
+  return ok();
+}
+
+int ugk_cache8_evict(int *table_out, int *len_out, float *weight_out, int *dropped, const int *table, const int *k_len,
+                     const float *weight, int nseq, int ld, int keep, int first, int recent) {
+  const char *fn = "ugk_cache8_evict";
+  if (nseq < 0 || ld < 0) return bad(fn, "nseq and ld must be >= 0");
+  if (ld > kEvictBlocks) return set_error(UGK_EINVAL, "%s: ld must be at most %d, got %d", fn, kEvictBlocks, ld);
+  if (nseq > 1 << 21) return bad(fn, "nseq exceeds the grid");
+  if (first < 0 || recent < 1 || first > keep - recent) return bad(fn, "first >= 0, recent >= 1 and first + recent <= keep");
+  if (nseq == 0 || ld == 0) return ok();
+  if (any_null({table_out, len_out, weight_out, dropped, table, k_len, weight})) return bad(fn, "NULL pointer");
+  if (any_same({table_out, len_out, weight_out, dropped}) || any_same({table_out, k_len, weight}) ||
+      any_same({len_out, table, weight}) || any_same({weight_out, table, k_len}) || any_same({dropped, table, k_len, weight}))
+    return bad(fn, "the outputs must be distinct buffers, and may each be their own input only");
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  if (int e = launch_cache8_evict(table_out, len_out, weight_out, dropped, table, k_len, weight, nseq, ld, keep, first, recent, word))
+    return e;
+  return ok();
+}
+
+int ugk_draft_verify(int *accepted, int *tokens, const float *p, const float *q, const int *draft, const int *n_draft,
+                     const float *u, int nseq, int K, int V) {
+  const char *fn = "ugk_draft_verify";
+  if (nseq < 0 || K < 0 || V < 1) return bad(fn, "nseq and K must be >= 0, V > 0");
+  if (nseq > 1 << 21 || (long long)nseq * (K + 1LL) > INT_MAX) return bad(fn, "nseq * (K + 1) exceeds the grid");
+  if (V > 1 << 30) return bad(fn, "V exceeds 2^30");
+  if (nseq == 0) return ok();
+  if (any_null({accepted, tokens, p, u}) || (K > 0 && !draft)) return bad(fn, "NULL pointer");
+  if (any_same({accepted, tokens, draft}) || (n_draft && any_same({accepted, tokens, n_draft})))
+    return bad(fn, "accepted and tokens must be distinct from each other and from the inputs");
+  int *word = ids_error_word();
+  if (!word) return UGK_EHIP;
+  if (int e = launch_draft_verify(accepted, tokens, p, q, draft, n_draft, u, nseq, K, V, word)) return e;
+  return ok();
+}
+
 int ugk_dense_attention_forward(void *, float *out, const float *qkv, int B, int T, int C, int NH) {
   const char *fn = "ugk_dense_attention_forward";
   ugk_attention a;
@@ -1007,6 +1135,12 @@ const char *ids_op_name(int code) {
     case UGK_IDS_CROSSENTROPY_BACKWARD: return "crossentropy_softmax_backward";
     case UGK_IDS_ATTENTION_FORWARD: return "attention_forward";
     case UGK_IDS_ATTENTION_BACKWARD: return "attention_backward";
+    case UGK_IDS_CACHE8_STORE: return "cache8_store";
+    case UGK_IDS_CACHE8_LOAD: return "cache8_load";
+    case UGK_IDS_CACHE8_ATTENTION: return "cache8_attention";
+    case UGK_IDS_CACHE8_EVICT: return "cache8_evict";
+    case UGK_IDS_CACHE8_VALUES: return "cache8_store";
+    case UGK_IDS_DRAFT_VERIFY: return "draft_verify";
     default: return "a guarded call";
   }
 }
@@ -1046,6 +1180,18 @@ int ugk_synchronize(void) {
                        "sequence longer than max (found on the device; they were clamped, so its results are not "
                        "meaningful)",
                        ids_op_name(code));
+    if (code == UGK_IDS_CACHE8_VALUES)
+      return set_error(UGK_EINVAL, "ugk_synchronize: cache8_store was given NaN or an infinity, which 8 bits do not hold");
+    if (code >= UGK_IDS_CACHE8_STORE && code <= UGK_IDS_CACHE8_EVICT)
+      return set_error(UGK_EINVAL,
+                       "ugk_synchronize: %s was given rows or lengths outside its buffers or beyond max, more rows than "
+                       "keys to store, or a block outside the cache (found on the device; they were clamped or left "
+                       "out, so its results are not meaningful)",
+                       ids_op_name(code));
+    if (code == UGK_IDS_DRAFT_VERIFY)
+      return set_error(UGK_EINVAL,
+                       "ugk_synchronize: draft_verify was given a draft outside the vocabulary, a number of drafts "
+                       "outside [0, K] or a row without probabilities");
     return set_error(UGK_EINVAL,
                      "ugk_synchronize: %s was given an id outside its table (found on the device by "
                      "ugk_ids_guard; the out-of-range ids were replaced, so its results are not meaningful)",

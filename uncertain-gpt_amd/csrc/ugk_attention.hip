@@ -26,21 +26,6 @@ struct Seq {
   __device__ __forceinline__ int first(int j, int causal) const { return causal ? max(0, j - (Lk - Lq)) : 0; }
 };
 
-// Rows [begin, end) of `rows`, at most `most` of them; *bad: the arrays say otherwise.
-__device__ __forceinline__ int clamp_rows(const int *start, const int *end, int b, int rows, int most, int *begin,
-                                          bool *bad) {
-  if (!start) {
-    *begin = b * most;
-    return most;
-  }
-  const int s = start[b], e = end[b];
-  *begin = min(max(s, 0), rows);
-  const int stop = min(max(e, *begin), rows);
-  const int n = min(stop - *begin, most);
-  *bad = *bad || s != *begin || e != *begin + n;
-  return n;
-}
-
 // Sequence b; a workgroup with `tell` reports offsets that were clamped.
 __device__ __forceinline__ Seq sequence(const ugk_attention &a, int b, bool tell, int *word, int code) {
   Seq s;

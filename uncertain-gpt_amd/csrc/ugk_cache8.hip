@@ -1,0 +1,1058 @@
+// ugk_cache8.hip - a cache of keys and values in 8 bits: store, load, attention
+// over it, and the eviction of blocks that got little weight.
+//
+// A block of 64 tokens of one key/value head holds whole numbers c of up to 127
+// times a scale s. s is a power of two: x / s and c s are then exact, a code is one
+// rounding of one number (to half a step: 2^-7 to 2^-8 of the block's largest), and
+// the codes of a block whose scale grows with a later token are rounded again from
+// what they stand for, at most half a step of the new scale away. (A scale of
+// max / 127 would have steps up to twice as fine, and would round all older
+// codes again for every token that raises the maximum a little.)
+//
+// Keys lie as rows, values as columns: both are then the operands of
+// v_mfma_i32_16x16x64_i8 as they come from memory, 16 codes per lane, without a
+// conversion, a transposition or a trip through LDS. Rows are padded to a multiple
+// of 16 codes with zeros. Key i of a block stands at place 4 (i % 16) + i / 16 of a
+// column, the order in which the lanes hold the weights.
+#include <math.h>
+
+#include "ugk_internal.h"
+#include "ugk_split.h"
+
+namespace ugk {
+namespace {
+
+constexpr int kKeys = kCacheBlock;  // 64: a lane holds four scores of a block and row
+typedef int v4i __attribute__((ext_vector_type(4)));
+constexpr float kLog2e8 = 1.44269504088896340736f, kLn28 = 0.69314718055994530942f;
+
+// One sequence: its first row, its rows and its keys.
+struct Seq8 {
+  int q0, Lq, Lk;
+  // the keys that row i sees: [0, seen(i))
+  __device__ __forceinline__ int seen(int i, int causal) const { return causal ? max(0, min(Lk, i + 1 + Lk - Lq)) : Lk; }
+};
+
+// Sequence b; a workgroup with `tell` reports rows and lengths that were clamped.
+__device__ __forceinline__ Seq8 sequence8(const ugk_cache8 &a, int b, bool tell, int *word, int code) {
+  Seq8 s;
+  bool bad = false;
+  s.Lq = clamp_rows(a.q_start, a.q_end, b, a.rows_q, a.max_q, &s.q0, &bad);
+  const int n = a.k_len ? a.k_len[b] : a.max_k;
+  s.Lk = min(max(n, 0), a.max_k);
+  bad = bad || s.Lk != n;
+  if (bad && tell && threadIdx.x == 0) *word = code;
+  return s;
+}
+
+// Block j of sequence b, or -1 (reported) where the table names none.
+__device__ __forceinline__ int block_of(const ugk_cache8 &a, int b, int j, int *word, int code) {
+  if (!a.table) return b * a.ld_table + j;
+  const int id = a.table[(size_t)b * a.ld_table + j];
+  if ((unsigned)id < (unsigned)a.nblocks) return id;
+  *word = code;
+  return -1;
+}
+
+__host__ __device__ __forceinline__ int padded(int HS) { return (HS + 15) & ~15; }
+
+// ---- store and load -------------------------------------------------------------
+
+// The scale for numbers up to the one with these bits: the least power of two s, 2^-126 to
+// 2^121, with it <= 127 s (beyond 127 2^121 numbers are held as that); 0 for 0.
+__device__ __forceinline__ float scale_for(uint32_t bits) {
+  if (bits == 0) return 0.0f;
+  // 1.f 2^(x - 127) <= 127 2^e, that is 1.f <= (127 / 64) 2^(e + 133 - x) with 127 / 64 = 1 + 0x7e0000 / 2^23
+  const int e = (int)(bits >> 23) - 133 + ((bits & 0x7fffffu) > 0x7e0000u);
+  return __uint_as_float((uint32_t)(min(max(e, -126), 121) + 127) << 23);
+}
+__device__ __forceinline__ int code_of(float x, float inv) { return (int)fminf(fmaxf(rintf(x * inv), -127.0f), 127.0f); }
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
+}
+__device__ __forceinline__ int code_at(uint32_t w, int j) { return (int)(w << (24 - 8 * j)) >> 24; }
+// Four codes of the scale `was` as codes of the scale `now` (ratio = was / now, a power of two below 1).
+__device__ __forceinline__ uint32_t again4(uint32_t w, float ratio) {
+  return pack4(code_of((float)code_at(w, 0), ratio), code_of((float)code_at(w, 1), ratio), code_of((float)code_at(w, 2), ratio),
+               code_of((float)code_at(w, 3), ratio));
+}
+
+// What a workgroup of the store and the load has: a block of a sequence of which rows [r0, r1) are
+// the call's, those before r0 in the cache already.
+struct Touched {
+  int b, h, q, r0, r1, id;  // q: the buffer's row of r0
+};
+__device__ __forceinline__ bool touched(const ugk_cache8 &a, int per, int *word, int code, Touched *t) {
+  const unsigned x = blockIdx.x;
+  t->h = x % a.NKV;
+  const int nth = x / a.NKV % per;
+  t->b = x / a.NKV / per;
+  const bool tell = t->h == 0 && nth == 0 && blockIdx.y == 0;
+  const Seq8 s = sequence8(a, t->b, tell, word, code);
+  if (s.Lq > s.Lk && tell && threadIdx.x == 0) *word = code;  // rows before the first key
+  const int begin = max(s.Lk - s.Lq, 0), j = begin / kKeys + nth;
+  if (s.Lq == 0 || j * kKeys >= s.Lk) return false;
+  t->r0 = max(begin - j * kKeys, 0);
+  t->r1 = min(s.Lk - j * kKeys, kKeys);
+  t->q = s.q0 + s.Lq - s.Lk + j * kKeys + t->r0;
+  t->id = block_of(a, t->b, j, word, code);
+  return t->id >= 0;
+}
+
+// One block of one head and of k or v (blockIdx.y) by a workgroup. A thread has four columns of the rows
+// c, c + 16, c + 32, c + 48, whose codes are one word of each of the value's columns.
+//
+// Bound by memory: 4 bytes read and 1 written per number (what a token behind others costs is the launch).
+template <int CH>
+__global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, int8_t *v8, float *vs, const float *k, const float *v,
+                                                         ugk_cache8 a, int per, int *word) {
+  constexpr int HP = 16 * CH, G = HP / 4, kPer = (16 * G + kBlock - 1) / kBlock;
+  __shared__ uint32_t tile[HP * 17];  // the values' words, 17 to a column of 16: banks that differ
+  __shared__ uint32_t top[kBlock / kWave];
+  Touched t;
+  if (!touched(a, per, word, UGK_IDS_CACHE8_STORE, &t)) return;
+  const bool values = blockIdx.y;
+  const long long ld = values ? a.ldv : a.ldk;
+  const float *src = (values ? v : k) + (long long)(t.q - t.r0) * ld + t.h * a.HS;
+  float4 x[kPer][4];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    const int e = threadIdx.x + i * kBlock, g = e % G, c = e / G, nd = a.HS - 4 * g;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      x[i][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int row = c + 16 * r;
+      if (c >= 16 || row < t.r0 || row >= t.r1 || nd <= 0) continue;
+      const float *p = src + row * ld + 4 * g;
+      if (nd >= 4) {
+        x[i][r] = ld4(p);
+      } else {
+        x[i][r].x = p[0];
+        if (nd > 1) x[i][r].y = p[1];
+        if (nd > 2) x[i][r].z = p[2];
+      }
+    }
+  }
+  bool finite = true;
+  const auto look = [&](float &f) {
+    const uint32_t u = abs_bits(f);
+    finite = finite && u < kInfBits;
+    if (u > kInfBits) f = 0.0f;  // NaN
+    else most = max(most, u);
+  };
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      look(x[i][r].x);
+      look(x[i][r].y);
+      look(x[i][r].z);
+      look(x[i][r].w);
+    }
+  if (!finite) *word = UGK_IDS_CACHE8_VALUES;
+  most = wave_max_bits(most);
+  if ((threadIdx.x & (kWave - 1)) == 0) top[threadIdx.x / kWave] = most;
+  __syncthreads();
+  static_assert(kBlock / kWave == 4, "four wavefronts");
+  most = max(max(top[0], top[1]), max(top[2], top[3]));
+  const size_t at = (size_t)t.id * a.NKV + t.h;
+  float *sp = (values ? vs : ks) + at;
+  const float was = t.r0 > 0 ? *sp : 0.0f, need = scale_for(most), now = fmaxf(was, need);
+  const float inv = now > 0.0f ? 1.0f / now : 0.0f, ratio = was * inv;
+  const bool grown = t.r0 > 0 && now > was && was > 0.0f;
+  uint32_t *dst = reinterpret_cast<uint32_t *>((values ? v8 : k8) + at * kKeys * HP);
+  uint32_t w[kPer][4];
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      w[i][r] = pack4(code_of(x[i][r].x, inv), code_of(x[i][r].y, inv), code_of(x[i][r].z, inv), code_of(x[i][r].w, inv));
+  if (!values) {
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int e = threadIdx.x + i * kBlock, g = e % G, c = e / G;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int row = c + 16 * r;
+        if (c < 16 && row >= t.r0 && row < t.r1) dst[row * G + g] = w[i][r];
+      }
+    }
+    if (grown)
+      for (int e = threadIdx.x; e < t.r0 * G; e += kBlock) dst[e] = again4(dst[e], ratio);
+  } else {
+    // words of four keys of one column, from words of four columns of one key
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int e = threadIdx.x + i * kBlock, g = e % G, c = e / G;
+      if (c >= 16) continue;
+#pragma unroll
+      for (int d = 0; d < 4; d++)
+        tile[(4 * g + d) * 17 + c] = pack4(code_at(w[i][0], d), code_at(w[i][1], d), code_at(w[i][2], d), code_at(w[i][3], d));
+    }
+    __syncthreads();
+    const bool whole = t.r0 == 0 && t.r1 == kKeys;
+    for (int e = threadIdx.x; e < HP * 16; e += kBlock) {
+      const int d = e / 16, c = e % 16;
+      uint32_t word4 = tile[d * 17 + c];
+      if (!whole) {
+        uint32_t fresh = 0, older = 0;  // the bytes of the call's rows, of the rows before
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int row = c + 16 * r;
+          if (row < t.r0) older |= 0xffu << 8 * r;
+          else if (row < t.r1) fresh |= 0xffu << 8 * r;
+        }
+        if (!fresh && !(older && grown)) continue;
+        uint32_t held = dst[e];
+        if (grown) held = (again4(held, ratio) & older) | (held & ~older);
+        word4 = (word4 & fresh) | (held & ~fresh);
+      }
+      dst[e] = word4;
+    }
+  }
+  __syncthreads();  // every thread has read the scale that was
+  if (threadIdx.x == 0 && (now != was || t.r0 == 0)) *sp = now;
+}
+
+// The store's rows, read back.
+template <int CH>
+__global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, const int8_t *k8, const float *ks, const int8_t *v8,
+                                                        const float *vs, ugk_cache8 a, int per, int *word) {
+  constexpr int HP = 16 * CH, G = HP / 4;
+  __shared__ uint32_t tile[HP * 17];
+  Touched t;
+  if (!touched(a, per, word, UGK_IDS_CACHE8_LOAD, &t)) return;
+  const bool values = blockIdx.y;
+  const long long ld = values ? a.ldv : a.ldk;
+  float *to = (values ? v : k) + (long long)(t.q - t.r0) * ld + t.h * a.HS;
+  const size_t at = (size_t)t.id * a.NKV + t.h;
+  const float s = (values ? vs : ks)[at];
+  const uint32_t *src = reinterpret_cast<const uint32_t *>((values ? v8 : k8) + at * kKeys * HP);
+  if (values) {
+    for (int e = threadIdx.x; e < HP * 16; e += kBlock) tile[e / 16 * 17 + e % 16] = src[e];
+    __syncthreads();
+  }
+  for (int e = threadIdx.x + t.r0 * G; e < t.r1 * G; e += kBlock) {
+    const int row = e / G, g = e % G, nd = a.HS - 4 * g;
+    if (nd <= 0) continue;
+    uint32_t w;
+    if (values) {
+      const int c = row & 15, r = row >> 4;
+      w = pack4(code_at(tile[(4 * g) * 17 + c], r), code_at(tile[(4 * g + 1) * 17 + c], r), code_at(tile[(4 * g + 2) * 17 + c], r),
+                code_at(tile[(4 * g + 3) * 17 + c], r));
+    } else {
+      w = src[e];
+    }
+    float *p = to + row * ld + 4 * g;
+    const float4 x = make_float4((float)code_at(w, 0) * s, (float)code_at(w, 1) * s, (float)code_at(w, 2) * s, (float)code_at(w, 3) * s);
+    if (nd >= 4) {
+      st4(p, x);
+    } else {
+      p[0] = x.x;
+      if (nd > 1) p[1] = x.y;
+      if (nd > 2) p[2] = x.z;
+    }
+  }
+}
+
+// ---- attention --------------------------------------------------------------------
+
+// Parts of the key axis: o normalised, the maximum m of its scores in base 2 and the sum l of 2^(s - m), per row and head;
+// `block`: the same m and l of each block of 64 keys, and `stat` those of the whole axis (for the blocks' weights).
+struct Parts8 {
+  float *o, *m, *l;
+  float2 *block, *stat;
+  int splits;
+};
+
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float or0(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// Running sums of a row. l stands on m, the largest score so far; the output's sum on the block whose weight times
+// values was largest, 2^(mo + e): a block's values share a scale, so neither large values of little weight
+// nor small ones of much cost the others their digits, and nothing leaves the range before the division.
+struct Running {
+  float m = -INFINITY, l = 0.0f, mo = -INFINITY, e = 0.0f;
+  // A block with maximum mb, sum lb and values of the scale vs. Returns the factors of the sum so far and of the block's.
+  __device__ __forceinline__ float2 add(float mb, float lb, float vs) {
+    const float top = fmaxf(m, mb), base = or0(top);
+    l = fmaf(l, ex2(m - base), lb * ex2(mb - base));
+    m = top;
+    const float mant = __builtin_amdgcn_frexp_mantf(vs), ve = vs == 0.0f ? -4096.0f : (float)__builtin_amdgcn_frexp_expf(vs);
+    const bool more = mb + ve > mo + e;
+    const float mn = more ? mb : mo, en = more ? ve : e, on = or0(mn);
+    // a block of which the row sees nothing counts for nothing, whatever its scale
+    const float2 f = make_float2(ex2((mo - on) + (e - en)), mb == -INFINITY ? 0.0f : mant * ex2((mb - on) + (ve - en)));
+    mo = mn;
+    e = en;
+    return f;
+  }
+  // The factor that makes the output's sum the output, as a float and a power of two.
+  __device__ __forceinline__ float last(float sum, int *p) const {
+    const float x = (or0(mo) - or0(m)) + e, r = rintf(x);
+    *p = (int)fminf(fmaxf(r, -4096.0f), 4096.0f);
+    return sum != 0.0f ? ex2(x - r) / sum : 0.0f;
+  }
+};
+
+// f = scale log2(e) of the call, ks of a block and 2^x of a row's whole numbers, as one factor of its scores: below the largest float, so
+// that a score of 0 stays 0.
+__device__ __forceinline__ float score_factor(float f, float ks, int x) {
+  const float y = __builtin_amdgcn_ldexpf(__builtin_amdgcn_frexp_mantf(f) * __builtin_amdgcn_frexp_mantf(ks),
+                                          __builtin_amdgcn_frexp_expf(f) + __builtin_amdgcn_frexp_expf(ks) + x);
+  return fminf(fmaxf(y, -3.402823466e38f), 3.402823466e38f);
+}
+
+// Sum and maximum over the 16 lanes of a row.
+__device__ __forceinline__ float sum16(float v) {
+  v += dpp_lane<kDppQuadSwap1>(v);
+  v += dpp_lane<kDppQuadSwap2>(v);
+  v += dpp_lane<kDppHalfMirror>(v);
+  return v + dpp_lane<kDppMirror>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp_lane<kDppQuadSwap1>(v));
+  v = fmaxf(v, dpp_lane<kDppQuadSwap2>(v));
+  v = fmaxf(v, dpp_lane<kDppHalfMirror>(v));
+  return fmaxf(v, dpp_lane<kDppMirror>(v));
+}
+
+// A whole number of up to 2^30 as four digits of base 256 in [-128, 127], a byte each.
+__device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x00808080u) ^ 0x00808080u; }
+// The number whose digits' sums of products are d (each below 2^21): exact but for the roundings to float.
+__device__ __forceinline__ float undigits(v4i d) {
+  return fmaf((float)(d[3] * 256 + d[2]), 65536.0f, (float)(d[1] * 256 + d[0]));
+}
+
+constexpr int kFewWaves = 4;
+
+// Few rows (query rows times heads of the group): a token's step, drafts, an observation window.
+//
+// A row of q is held as whole numbers of 31 bits next to its largest element, and those as four digits, so that four
+// rows are one 16-row operand of the 8-bit matrix units: a block's scores take two instructions per 16 keys at 128 floats per
+// head, their sums are exact, and a lane finds the four digits of its score in its own four registers.
+// The weights, 31 bits next to the block's largest, go the same way into the product with the values.
+template <int DT, int R>
+__global__ __launch_bounds__(kFewWaves *kWave) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8,
+                                                                const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
+                                                                Parts8 parts, unsigned pairs, unsigned groups, int *word) {
+  constexpr int KS = (DT + 3) / 4, kStride = 20;
+  __shared__ alignas(16) uint32_t lp[kFewWaves][16 * kStride];
+  __shared__ float lo[kFewWaves][4][DT * 16];
+  __shared__ float lm[kFewWaves][4], ll[kFewWaves][4];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+  const unsigned pair = blockIdx.x % pairs, group = blockIdx.x / pairs % groups;
+  const int part = blockIdx.x / pairs / groups;
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV, HP = padded(a.HS), CH = HP / 16;
+  const Seq8 s = sequence8(a, b, hk == 0 && part == 0 && group == 0, word, UGK_IDS_CACHE8_ATTENTION);
+  const int rows = s.Lq * G, base_row = group * 4 * R;
+  if (base_row >= rows) return;
+  const int end = s.seen((min(base_row + 4 * R, rows) - 1) / G, a.causal);  // the last row sees most
+  const int nb = (end + kKeys - 1) / kKeys;
+  const int first = (int)((long long)nb * part / parts.splits), stop = (int)((long long)nb * (part + 1) / parts.splits);
+  const float f = a.scale * kLog2e8;
+
+  // q's digits: lane (row % 4 * 4 + digit, quad) holds dims 64 step + 16 quad + [0, 16)
+  v4i aq[R][KS];
+  int ex[R], lim[R], least = end;
+  bool nan[R];
+  Running run[R];
+  float o[R][DT];
+#pragma unroll
+  for (int rt = 0; rt < R; rt++) {
+    const int rr = min(base_row + 4 * rt + (col >> 2), rows - 1);
+    const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (hk * G + rr % G) * a.HS;
+    float x[KS][16];
+    uint32_t most = 0;
+#pragma unroll
+    for (int st = 0; st < KS; st++)
+#pragma unroll
+      for (int d = 0; d < 16; d++) {
+        const int at = 64 * st + 16 * quad + d;
+        x[st][d] = at < a.HS ? p[at] : 0.0f;
+        most = max(most, abs_bits(x[st][d]));
+      }
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+    const int e = (int)(most >> 23) - 127;  // below 2^(e + 1)
+#pragma unroll
+    for (int st = 0; st < KS; st++) {
+      v4i w = {0, 0, 0, 0};
+#pragma unroll
+      for (int d = 0; d < 16; d++) {
+        const uint32_t y = digits((int)rintf(__builtin_amdgcn_ldexpf(x[st][d], 29 - e)));
+        w[d / 4] |= (int)((y >> (8 * (lane & 3)) & 255u) << (8 * (d & 3)));
+      }
+      if (most >= kInfBits) w = v4i{0, 0, 0, 0};
+      aq[rt][st] = w;
+    }
+    // for the lanes that hold the row's scores: row quad of the four
+    ex[rt] = __shfl(e, 4 * quad) - 29;
+    nan[rt] = (uint32_t)__shfl((int)most, 4 * quad) >= kInfBits;
+    const int mine = base_row + 4 * rt + quad;
+    lim[rt] = mine < rows ? s.seen(mine / G, a.causal) : end;
+    least = min(least, lim[rt]);
+#pragma unroll
+    for (int t = 0; t < DT; t++) o[rt][t] = 0.0f;
+  }
+#pragma unroll
+  for (int x = 16; x < kWave; x *= 2) least = min(least, __shfl_xor(least, x));
+
+  int koff[KS], voff[DT];
+#pragma unroll
+  for (int st = 0; st < KS; st++) koff[st] = col * HP + 16 * min(4 * st + quad, CH - 1);  // behind the row q's digits are 0
+#pragma unroll
+  for (int t = 0; t < DT; t++) voff[t] = (16 * min(t, CH - 1) + col) * kKeys + 16 * quad;
+  uint32_t *mylp = lp[wave];
+
+  int next = first + wave < stop ? block_of(a, b, first + wave, word, UGK_IDS_CACHE8_ATTENTION) : 0;
+  for (int j = first + wave; j < stop; j += kFewWaves) {
+    const bool there = next >= 0;
+    const size_t at = (size_t)(there ? next : 0) * a.NKV + hk;
+    const int8_t *kb = k8 + at * kKeys * HP, *vb = v8 + at * kKeys * HP;
+    v4i kf[KS][4], vf[DT];
+#pragma unroll
+    for (int st = 0; st < KS; st++)
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++)
+        kf[st][kt] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(kb + koff[st] + kt * 16 * HP));
+#pragma unroll
+    for (int t = 0; t < DT; t++) vf[t] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(vb + voff[t]));
+    const float kscale = ks[at], vscale = vs[at];
+    if (j + kFewWaves < stop) next = block_of(a, b, j + kFewWaves, word, UGK_IDS_CACHE8_ATTENTION);
+    const bool masked = !there || (j + 1) * kKeys > least;
+#pragma unroll
+    for (int rt = 0; rt < R; rt++) {
+      if (R > 1) __builtin_amdgcn_sched_barrier(0);  // row by row: the registers hold one operand's scores
+      const float fac = nan[rt] ? NAN : score_factor(f, kscale, ex[rt]);
+      float p[4], mb = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++) {
+        v4i acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int st = 0; st < KS; st++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[rt][st], kf[st][kt], acc, 0, 0, 0);
+        p[kt] = undigits(acc) * fac;
+        if (masked && (!there || j * kKeys + kt * 16 + col >= lim[rt])) p[kt] = -INFINITY;
+        mb = fmaxf(mb, p[kt]);
+      }
+      mb = max16(mb);
+      const float zero = or0(mb);
+      uint32_t y[4];
+      float lb = 0.0f;
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++) {
+        p[kt] = ex2(p[kt] - zero);
+        lb += p[kt];
+        y[kt] = digits((int)rintf(p[kt] * 0x1p30f));
+      }
+      // the four keys' digits side by side: a word per digit
+      const uint32_t t0 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), t1 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u);
+      const uint32_t t2 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u), t3 = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
+      uint32_t *w = mylp + 4 * quad * kStride + col;
+      w[0] = __builtin_amdgcn_perm(t2, t0, 0x05040100u);
+      w[kStride] = __builtin_amdgcn_perm(t2, t0, 0x07060302u);
+      w[2 * kStride] = __builtin_amdgcn_perm(t3, t1, 0x05040100u);
+      w[3 * kStride] = __builtin_amdgcn_perm(t3, t1, 0x07060302u);
+      __builtin_amdgcn_wave_barrier();
+      const v4i ap = *reinterpret_cast<const v4i *>(mylp + col * kStride + 4 * quad);
+      __builtin_amdgcn_wave_barrier();
+      if (parts.block) {
+        const int mine = base_row + 4 * rt + quad;
+        const float sum = sum16(lb);
+        if (col == 0 && mine < rows)
+          parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + mine) * a.ld_table + j] = make_float2(mb, sum);
+      }
+      const float2 k = run[rt].add(mb, lb, vscale);
+#pragma unroll
+      for (int t = 0; t < DT; t++) {
+        const v4i acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap, vf[t], v4i{0, 0, 0, 0}, 0, 0, 0);
+        o[rt][t] = fmaf(undigits(acc), k.y, o[rt][t] * k.x);
+      }
+    }
+  }
+
+  // the wavefronts' sums, four rows at a time
+#pragma unroll
+  for (int rt = 0; rt < R; rt++) {
+    const float sum = sum16(run[rt].l);
+    int e;
+    const float g = run[rt].last(sum, &e);
+    e -= 30;  // of the weights' whole numbers
+    if (rt) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < DT; t++) lo[wave][quad][16 * t + col] = __builtin_amdgcn_ldexpf(o[rt][t] * g, e);
+    if (col == 0) {
+      lm[wave][quad] = run[rt].m;
+      ll[wave][quad] = sum;
+    }
+    __syncthreads();
+    const int r = threadIdx.x >> 6, mine = base_row + 4 * rt + r;
+    if (mine >= rows) continue;
+    float top = -INFINITY, total = 0.0f, wt[kFewWaves];
+#pragma unroll
+    for (int w = 0; w < kFewWaves; w++) top = fmaxf(top, lm[w][r]);
+#pragma unroll
+    for (int w = 0; w < kFewWaves; w++) {
+      wt[w] = ll[w][r] == 0.0f ? 0.0f : ll[w][r] * ex2(lm[w][r] - or0(top));
+      total += wt[w];
+    }
+    const int i = mine / G, h = hk * G + mine % G;
+    const size_t prow = (((size_t)part * a.nseq + b) * a.max_q + i) * a.NH + h, grow = (size_t)s.q0 + i;
+    float *po = parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    for (int d = lane; d < a.HS; d += kWave) {
+      float y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; w++) y = fmaf(wt[w] * inv, lo[w][r][d], y);
+      po[d] = y;
+    }
+    if (lane) continue;
+    if (parts.o) {
+      parts.m[prow] = top;
+      parts.l[prow] = total;
+    } else if (lse) {
+      lse[grow * a.NH + h] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn28;
+    }
+  }
+}
+
+// The parts of a split key axis joined, one wavefront per row and head, in the parts' order.
+__global__ __launch_bounds__(kBlock) void k_cache8_join(float *out, float *lse, Parts8 parts, ugk_cache8 a) {
+  const size_t at = (size_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6), per = (size_t)a.nseq * a.max_q * a.NH;
+  if (at >= per) return;
+  const int lane = threadIdx.x & (kWave - 1), h = at % a.NH, i = at / a.NH % a.max_q, b = at / a.NH / a.max_q;
+  const Seq8 s = sequence8(a, b, false, nullptr, 0);
+  if (i >= s.Lq) return;
+  float m = -INFINITY;
+  for (int x = lane; x < parts.splits; x += kWave) m = fmaxf(m, parts.m[x * per + at]);
+#pragma unroll
+  for (int x = 32; x; x /= 2) m = fmaxf(m, __shfl_xor(m, x));
+  float o0 = 0.0f, o1 = 0.0f, l = 0.0f;
+  const int d0 = min(lane, a.HS - 1), d1 = min(lane + kWave, a.HS - 1);
+  for (int x0 = 0; x0 < parts.splits; x0 += kWave) {
+    const int x = x0 + lane, n = min(kWave, parts.splits - x0);
+    const float lx = x < parts.splits ? parts.l[x * per + at] : 0.0f;
+    const float w = lx == 0.0f ? 0.0f : lx * ex2(parts.m[x * per + at] - or0(m));  // 0: a part without a key of this row, its o is 0
+    l += wave_sum(w);
+    for (int t = 0; t < n; t++) {
+      const float wt = __shfl(w, t), *o = parts.o + ((x0 + t) * per + at) * a.HS;
+      o0 = fmaf(wt, o[d0], o0);
+      o1 = fmaf(wt, o[d1], o1);
+    }
+  }
+  const bool none = l == 0.0f;
+  const float inv = none ? 1.0f : 1.0f / l;
+  const size_t g = (size_t)s.q0 + i;
+  float *po = out + g * a.ldo + h * a.HS;
+  if (lane < a.HS) po[lane] = o0 * inv;
+  if (lane + kWave < a.HS) po[lane + kWave] = o1 * inv;
+  if (lane) return;
+  if (lse) lse[g * a.NH + h] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn28;
+  if (parts.stat) parts.stat[at] = make_float2(m, l);
+}
+
+// weight[b, j] += the sum over rows and heads of what block j got: 16 blocks of a sequence per workgroup, 16 threads to each,
+// which take every sixteenth row and head; added in a fixed order.
+__global__ __launch_bounds__(kBlock) void k_cache8_weights(float *weight, Parts8 parts, ugk_cache8 a) {
+  __shared__ float part[16][17];
+  const int per = (a.ld_table + 15) / 16, b = blockIdx.x / per, j = blockIdx.x % per * 16 + (threadIdx.x & 15);
+  const int slice = threadIdx.x >> 4, G = a.NH / a.NKV;
+  const Seq8 s = sequence8(a, b, false, nullptr, 0);
+  const int nb = (s.Lk + kKeys - 1) / kKeys, rows = s.Lq * G;
+  float sum = 0.0f;
+  if (j < nb) {
+    for (int x = slice; x < rows * a.NKV; x += 16) {
+      const int hk = x / rows, rr = x % rows, i = rr / G, h = hk * G + rr % G;
+      if (j * kKeys >= s.seen(i, a.causal)) continue;
+      const float2 p = parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + rr) * a.ld_table + j];
+      const float2 all = parts.stat[((size_t)b * a.max_q + i) * a.NH + h];
+      if (p.y != 0.0f) sum += p.y * ex2(p.x - all.x) / all.y;
+    }
+  }
+  part[slice][threadIdx.x & 15] = sum;
+  __syncthreads();
+  if (slice || j >= nb) return;
+  float t = 0.0f;
+#pragma unroll
+  for (int x = 0; x < 16; x++) t += part[x][threadIdx.x];
+  weight[(size_t)b * a.ld_table + j] += t;
+}
+
+// Many rows: a prompt's. 128 rows of a sequence and key/value head per workgroup, 32 to a wavefront, over blocks whose codes go
+// through LDS as halves (which hold them exactly).
+//
+// The scores are computed transposed, so that a lane holds one row: its maximum and sum stay in the lane, and its weights are the second
+// product's operand as they stand. q and the weights are two halves each (ugk_split.h), so a product
+// is two of v_mfma_f32_32x32x16_f16, where fp32 keys and values need three.
+constexpr int kTileWaves8 = 4, kTileRows8 = 32 * kTileWaves8, kTileThreads8 = kTileWaves8 * kWave;
+
+// Four codes (bytes b0..b3 of w, with their signs turned over: c + 128) as halves.
+__device__ __forceinline__ v2u halves4(uint32_t w) {
+  const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};  // 0x6400 | byte is 1024 + byte
+  const v2h lo = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off;
+  const v2h hi = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off;
+  return v2u{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+template <int DT>
+__global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, float *lse, const float *q, const int8_t *k8,
+                                                                 const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
+                                                                 Parts8 parts, unsigned pairs, unsigned tiles, int *word) {
+  constexpr int KSTR = 16 * DT + 8, VSTR = kKeys + 8, D32 = DT / 2, NL = DT / 4;
+  __shared__ alignas(16) _Float16 kl[2][kKeys * KSTR];
+  __shared__ alignas(16) _Float16 vl[2][16 * DT * VSTR];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const unsigned pair = blockIdx.x % pairs;
+  const int tile = (int)(tiles - 1 - blockIdx.x / pairs), part = blockIdx.y;  // the longest first
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV, HP = padded(a.HS), CH = HP / 16;
+  const Seq8 s = sequence8(a, b, hk == 0 && part == 0 && tile == 0, word, UGK_IDS_CACHE8_ATTENTION);
+  const int rows = s.Lq * G, row0 = tile * kTileRows8;
+  if (row0 >= rows) return;
+  const int nb = (s.seen((min(row0 + kTileRows8, rows) - 1) / G, a.causal) + kKeys - 1) / kKeys;
+  const int first = (int)((long long)nb * part / parts.splits), stop = (int)((long long)nb * (part + 1) / parts.splits);
+  const int mine = row0 + 32 * wave + col, safe = min(mine, rows - 1), i = safe / G, h = hk * G + safe % G;
+  const int lim = s.seen(i, a.causal);
+  // what the wavefront's first and last rows see
+  const int wave_first = min(row0 + 32 * wave, rows - 1), wave_last = min(row0 + 32 * wave + 31, rows - 1);
+  const int least = s.seen(wave_first / G, a.causal), most_seen = s.seen(wave_last / G, a.causal);
+  const bool idle = row0 + 32 * wave >= rows;
+  const float f = a.scale * kLog2e8;
+
+  v8h qh[DT], ql[DT];
+  int e;
+  bool nan;
+  {
+    const float *p = q + ((size_t)s.q0 + i) * a.ldq + (size_t)h * a.HS;
+    float x[DT][8];
+    uint32_t most = 0;
+#pragma unroll
+    for (int st = 0; st < DT; st++)
+#pragma unroll
+      for (int d = 0; d < 8; d++) {
+        const int at = 16 * st + 8 * half + d;
+        x[st][d] = at < a.HS ? p[at] : 0.0f;
+        most = max(most, abs_bits(x[st][d]));
+      }
+    most = half_max_bits(most);
+    nan = most >= kInfBits;
+    e = (int)(most >> 23) - 126 - 15;  // below 2^15 2^e
+#pragma unroll
+    for (int st = 0; st < DT; st++) {
+#pragma unroll
+      for (int d = 0; d < 8; d++) x[st][d] = nan ? 0.0f : __builtin_amdgcn_ldexpf(x[st][d], -e);
+      split8(x[st], qh[st], ql[st]);
+    }
+  }
+
+  Running run;
+  v16f o[D32];
+#pragma unroll
+  for (int t = 0; t < D32; t++) o[t] = v16f{};
+
+  // staging: thread t has words of 16 codes t, t + 256 of the block's keys and of its values
+  int kdst[NL], vdst[NL];
+#pragma unroll
+  for (int n = 0; n < NL; n++) {
+    const int w = threadIdx.x + n * kTileThreads8, c = w & 3;
+    kdst[n] = w / CH * KSTR + w % CH * 16;
+    vdst[n] = (w >> 2) * VSTR + (c & 1) * 8 + (c >> 1) * 4;
+  }
+  v4u kr[NL], vr[NL];
+  float kscale = 0.0f, vscale = 0.0f;
+  bool there = true;
+  const auto fetch = [&](int j) {
+    const int id = block_of(a, b, j, word, UGK_IDS_CACHE8_ATTENTION);
+    there = id >= 0;
+    const size_t at = (size_t)(there ? id : 0) * a.NKV + hk;
+#pragma unroll
+    for (int n = 0; n < NL; n++) {
+      const int w = threadIdx.x + n * kTileThreads8;
+      if (w < 4 * HP) {
+        kr[n] = *reinterpret_cast<const v4u *>(k8 + at * kKeys * HP + 16 * w);
+        vr[n] = *reinterpret_cast<const v4u *>(v8 + at * kKeys * HP + 16 * w);
+      }
+    }
+    kscale = ks[at];
+    vscale = vs[at];
+  };
+  if (first < stop) fetch(first);
+  for (int j = first; j < stop; j++) {
+    _Float16 *kt = kl[(j - first) & 1], *vt = vl[(j - first) & 1];
+#pragma unroll
+    for (int n = 0; n < NL; n++) {
+      if (threadIdx.x + n * kTileThreads8 >= 4 * HP) continue;
+      const v4u kw = kr[n] ^ 0x80808080u, vw = vr[n] ^ 0x80808080u;
+      const v2u k0 = halves4(kw[0]), k1 = halves4(kw[1]), k2 = halves4(kw[2]), k3 = halves4(kw[3]);
+      *reinterpret_cast<v4u *>(kt + kdst[n]) = v4u{k0[0], k0[1], k1[0], k1[1]};
+      *reinterpret_cast<v4u *>(kt + kdst[n] + 8) = v4u{k2[0], k2[1], k3[0], k3[1]};
+      // a word of the values: keys c, c + 16, c + 32, c + 48; the words are c = 4 x .. 4 x + 3
+      const uint32_t t0 = __builtin_amdgcn_perm(vw[1], vw[0], 0x05010400u), t1 = __builtin_amdgcn_perm(vw[1], vw[0], 0x07030602u);
+      const uint32_t t2 = __builtin_amdgcn_perm(vw[3], vw[2], 0x05010400u), t3 = __builtin_amdgcn_perm(vw[3], vw[2], 0x07030602u);
+      *reinterpret_cast<v2u *>(vt + vdst[n]) = halves4(__builtin_amdgcn_perm(t2, t0, 0x05040100u));
+      *reinterpret_cast<v2u *>(vt + vdst[n] + 16) = halves4(__builtin_amdgcn_perm(t2, t0, 0x07060302u));
+      *reinterpret_cast<v2u *>(vt + vdst[n] + 32) = halves4(__builtin_amdgcn_perm(t3, t1, 0x05040100u));
+      *reinterpret_cast<v2u *>(vt + vdst[n] + 48) = halves4(__builtin_amdgcn_perm(t3, t1, 0x07060302u));
+    }
+    const float fac = nan ? NAN : score_factor(f, kscale, e), vnow = vscale;
+    const bool here = there;
+    __syncthreads();
+    if (j + 1 < stop) fetch(j + 1);
+    if (idle || j * kKeys >= most_seen) continue;
+    v16f sc[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      sc[x] = v16f{};
+#pragma unroll
+      for (int st = 0; st < DT; st++) {
+        if (st >= CH) continue;
+        const v8h kf = frag(kt + (32 * x + col) * KSTR + 16 * st + 8 * half);
+        sc[x] = mfma(kf, ql[st], sc[x]);
+        sc[x] = mfma(kf, qh[st], sc[x]);
+      }
+    }
+    float mb = -INFINITY;
+    const bool masked = !here || (j + 1) * kKeys > least;
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        float y = sc[x][r] * fac;
+        if (masked && (!here || j * kKeys + 32 * x + 8 * (r / 4) + 4 * half + r % 4 >= lim)) y = -INFINITY;
+        sc[x][r] = y;
+        mb = fmaxf(mb, y);
+      }
+    mb = half_max(mb);
+    const float zero = or0(mb);
+    float lb = 0.0f;
+    v8h ph[4], pl[4];
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      float p[8];
+#pragma unroll
+      for (int r = 0; r < 8; r++) {
+        p[r] = ex2(sc[g / 2][8 * (g % 2) + r] - zero);
+        lb += p[r];
+      }
+      split8(p, 0x1p14f, ph[g], pl[g]);
+    }
+    const float2 k = run.add(mb, lb, vnow);
+    const float ky = k.y * 0x1p-14f;
+#pragma unroll
+    for (int t = 0; t < D32; t++) {
+      if (2 * t >= CH) continue;
+      v16f acc = v16f{};
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const v8h vf = frag(vt + (32 * t + col) * VSTR + 16 * g + 8 * half);
+        acc = mfma(vf, pl[g], acc);
+        acc = mfma(vf, ph[g], acc);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) o[t][r] = fmaf(acc[r], ky, o[t][r] * k.x);
+    }
+  }
+  if (mine >= rows) return;
+  const float sum = half_sum(run.l);
+  int p;
+  const float g = run.last(sum, &p);
+  const size_t prow = (((size_t)part * a.nseq + b) * a.max_q + i) * a.NH + h, grow = (size_t)s.q0 + i;
+  float *po = parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + (size_t)h * a.HS;
+#pragma unroll
+  for (int t = 0; t < D32; t++)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * t + 8 * (r / 4) + 4 * half, nd = a.HS - d;
+      if (nd <= 0) continue;
+      float4 y;
+      y.x = __builtin_amdgcn_ldexpf(o[t][r] * g, p);
+      y.y = __builtin_amdgcn_ldexpf(o[t][r + 1] * g, p);
+      y.z = __builtin_amdgcn_ldexpf(o[t][r + 2] * g, p);
+      y.w = __builtin_amdgcn_ldexpf(o[t][r + 3] * g, p);
+      if (nd >= 4) {
+        st4(po + d, y);
+      } else {
+        po[d] = y.x;
+        if (nd > 1) po[d + 1] = y.y;
+        if (nd > 2) po[d + 2] = y.z;
+      }
+    }
+  if (half) return;
+  if (parts.o) {
+    parts.m[prow] = run.m;
+    parts.l[prow] = sum;
+  } else if (lse) {
+    lse[grow * a.NH + h] = sum == 0.0f ? -INFINITY : (run.m + __builtin_amdgcn_logf(sum)) * kLn28;
+  }
+}
+
+// ---- eviction ----------------------------------------------------------------------
+
+constexpr int kEvictThreads = 1024;
+
+// Sum over the workgroup's threads before this one, and in *all over all of them.
+__device__ __forceinline__ int before(int x, int *lds, int *all) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  int y = x;
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    const int z = __shfl_up(y, o);
+    if (lane >= o) y += z;
+  }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == kWave - 1) lds[wave] = y;
+  __syncthreads();
+  int sum = 0, total = 0;
+  for (int w = 0; w < kEvictThreads / kWave; w++) {
+    const int z = lds[w];
+    if (w < wave) sum += z;
+    total += z;
+  }
+  *all = total;
+  return sum + y - x;
+}
+
+// One sequence per workgroup, E entries of its table per thread, side by side in registers: the d lightest blocks by a search over the
+// weights' bits, eight at a time (counts in LDS), ties by their index; then each entry's place from counts of those
+// before it. Reading and writing 16 bytes per entry is nothing; what counts are the chain of
+// barriers (four counts and two sums).
+template <int E>
+__global__ __launch_bounds__(kEvictThreads) void k_cache8_evict(int *table_out, int *len_out, float *weight_out, int *dropped,
+                                                               const int *table, const int *k_len, const float *weight, int ld,
+                                                               int keep, int first, int recent, int *word) {
+  __shared__ int count[256], lds[kEvictThreads / kWave];
+  __shared__ int found, under;
+  const int b = blockIdx.x, len = k_len[b];
+  const int full = min(max(len, 0), (int)min((long long)ld * kKeys, (long long)0x7fffffff)), n = (full + kKeys - 1) / kKeys;
+  if (full != len && threadIdx.x == 0) *word = UGK_IDS_CACHE8_EVICT;
+  const int d = max(n - keep, 0), i0 = threadIdx.x * E;
+  const size_t row = (size_t)b * ld;
+  int id[E];
+  float w[E];
+  uint32_t key[E];
+#pragma unroll
+  for (int x = 0; x < E; x++) {
+    const int i = i0 + x;
+    id[x] = i < ld ? table[row + i] : 0;
+    w[x] = i < ld ? weight[row + i] : 0.0f;
+    // ascending in the weight; NaN, whatever its sign, above all
+    const uint32_t u = __float_as_uint(w[x] + 0.0f);
+    key[x] = w[x] != w[x] ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
+  }
+  // the value of the d-th lightest, eight bits at a time, and how many of its equals go
+  uint32_t value = 0;
+  int left = d;
+  if (d > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      __syncthreads();
+      if (threadIdx.x < 256) count[threadIdx.x] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < E; x++) {
+        const int i = i0 + x;
+        const bool may = i >= first && i < n - recent;
+        if (may && (shift == 24 || key[x] >> (shift + 8) == value >> (shift + 8))) atomicAdd(&count[key[x] >> shift & 255u], 1);
+      }
+      __syncthreads();
+      if (threadIdx.x < kWave) {  // four counts per lane
+        int c[4], sum = 0;
+#pragma unroll
+        for (int x = 0; x < 4; x++) sum += c[x] = count[4 * threadIdx.x + x];
+        int y = sum;
+#pragma unroll
+        for (int o = 1; o < kWave; o *= 2) {
+          const int z = __shfl_up(y, o);
+          if ((int)threadIdx.x >= o) y += z;
+        }
+        y -= sum;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          if (y < left && y + c[x] >= left) {
+            found = 4 * threadIdx.x + x;
+            under = y;
+          }
+          y += c[x];
+        }
+      }
+      __syncthreads();
+      value |= (uint32_t)found << shift;
+      left -= under;
+    }
+  }
+  int ties = 0, all;
+#pragma unroll
+  for (int x = 0; x < E; x++) ties += d > 0 && i0 + x >= first && i0 + x < n - recent && key[x] == value;
+  int tie = before(ties, lds, &all), gone = 0;
+  bool goes[E];
+#pragma unroll
+  for (int x = 0; x < E; x++) {
+    const bool may = d > 0 && i0 + x >= first && i0 + x < n - recent, same = may && key[x] == value;
+    goes[x] = may && (key[x] < value || (same && tie < left));
+    tie += same;
+    gone += goes[x];
+  }
+  int g = before(gone, lds, &all);  // behind its barriers everything has been read: the outputs may be the inputs
+#pragma unroll
+  for (int x = 0; x < E; x++) {
+    const int i = i0 + x;
+    if (i >= ld) break;
+    const int to = goes[x] ? ld - d + g : i - g;
+    g += goes[x];
+    table_out[row + to] = id[x];
+    weight_out[row + to] = goes[x] || i >= n ? 0.0f : w[x];
+  }
+  if (threadIdx.x == 0) {
+    len_out[b] = full - d * kKeys;
+    dropped[b] = d;
+  }
+}
+
+int cu_count8() {
+  static const int n = [] {
+    int dev = 0, c = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) {
+      (void)hipGetLastError();
+      c = 0;
+    }
+    return c > 0 ? c : 256;
+  }();
+  return n;
+}
+
+// How an attention call is cut: operands of four rows per workgroup of k_cache8_few (0: k_cache8_tile) and groups of them, tiles
+// of rows, parts of the key axis.
+struct Plan8 {
+  int few, groups, tiles, splits;
+};
+constexpr int kFewRows8 = 32;
+constexpr size_t kMaxParts8 = 1 << 15;  // rows of a head that the parts hold at most
+
+Plan8 plan8(const ugk_cache8 &a, bool weigh) {
+  Plan8 p{};
+  const long long pairs = (long long)a.nseq * a.NKV, rows = (long long)a.max_q * (a.NH / a.NKV);
+  const long long prow = (long long)a.nseq * a.max_q * a.NH, blocks = (a.max_k + kKeys - 1) / kKeys;
+  long long want;
+  if (rows <= kFewRows8 || weigh) {
+    p.few = rows <= 4 ? 1 : rows <= 8 ? 2 : rows <= 16 ? 4 : 8;
+    p.groups = (int)((rows + 4 * p.few - 1) / (4 * p.few));
+    want = max(8LL * cu_count8() / max(pairs * p.groups, 1LL), (blocks + 15) / 16);
+    want = min(want, blocks / 4);
+  } else {
+    p.tiles = (int)((rows + kTileRows8 - 1) / kTileRows8);
+    want = 2LL * cu_count8() / max(pairs * p.tiles, 1LL);
+    want = min(want, blocks / 4);
+  }
+  want = min(want, (long long)kMaxParts8 / max(prow, 1LL));
+  p.splits = (int)max(want, 1LL);
+  return p;
+}
+bool has_parts(const Plan8 &p, bool weigh) { return p.splits > 1 || weigh; }
+size_t parts_rows(const ugk_cache8 &a, const Plan8 &p) { return (size_t)p.splits * a.nseq * a.max_q * a.NH; }
+size_t even(size_t n) { return (n + 1) / 2 * 2; }
+}  // namespace
+
+size_t cache8_attention_bytes(const ugk_cache8 &a, bool weigh) {
+  const Plan8 p = plan8(a, weigh);
+  if (!has_parts(p, weigh)) return 0;
+  const size_t rows = (size_t)a.nseq * a.max_q * a.NH;
+  return (even(parts_rows(a, p) * (a.HS + 2)) + (weigh ? 2 * rows * (1 + (size_t)a.ld_table) : 0)) * sizeof(float);
+}
+
+int launch_cache8_attention(float *out, float *lse, const float *q, const void *k8, const float *ks, const void *v8,
+                            const float *vs, float *weight, float *mem, const ugk_cache8 &a, int *word) {
+  const Plan8 p = plan8(a, weight);
+  Parts8 parts{};
+  parts.splits = p.splits;
+  if (has_parts(p, weight)) {
+    parts.m = mem;
+    parts.l = parts.m + parts_rows(a, p);
+    parts.o = parts.l + parts_rows(a, p);
+    if (weight) {
+      parts.stat = reinterpret_cast<float2 *>(mem + even(parts_rows(a, p) * (a.HS + 2)));
+      parts.block = parts.stat + (size_t)a.nseq * a.max_q * a.NH;
+    }
+  }
+  const unsigned pairs = (unsigned)a.nseq * a.NKV;
+  const auto few = [&](auto kernel) {
+    launch(kernel, dim3(pairs * p.groups * p.splits), dim3(kFewWaves * kWave), 0, out, lse, q, (const int8_t *)k8, ks, (const int8_t *)v8,
+           vs, a, parts, pairs, (unsigned)p.groups, word);
+  };
+  const auto tile = [&](auto kernel) {
+    launch(kernel, dim3(pairs * p.tiles, p.splits), dim3(kTileThreads8), 0, out, lse, q, (const int8_t *)k8, ks, (const int8_t *)v8, vs, a,
+           parts, pairs, (unsigned)p.tiles, word);
+  };
+#define UGK_FEW8(r)                                                                                                    \
+  case r:                                                                                                              \
+    if (a.HS <= 32) few(k_cache8_few<2, r>);                                                                           \
+    else if (a.HS <= 64) few(k_cache8_few<4, r>);                                                                      \
+    else if (a.HS <= 96) few(k_cache8_few<6, r>);                                                                      \
+    else few(k_cache8_few<8, r>);                                                                                      \
+    break;
+  switch (p.few) {
+    UGK_FEW8(1) UGK_FEW8(2) UGK_FEW8(4) UGK_FEW8(8)
+    default: a.HS <= 64 ? tile(k_cache8_tile<4>) : tile(k_cache8_tile<8>);
+  }
+#undef UGK_FEW8
+  if (int e = check_launch("cache8_attention")) return e;
+  if (parts.o) {
+    launch(k_cache8_join, dim3(grid_for((size_t)a.nseq * a.max_q * a.NH, kBlock / kWave)), dim3(kBlock), 0, out, lse, parts, a);
+    if (int e = check_launch("cache8_attention")) return e;
+  }
+  if (weight) {
+    launch(k_cache8_weights, dim3((unsigned)a.nseq * ((a.ld_table + 15) / 16)), dim3(kBlock), 0, weight, parts, a);
+    return check_launch("cache8_attention");
+  }
+  return UGK_OK;
+}
+
+// Blocks that max_q rows of a sequence touch at most, wherever they begin.
+static int touched_blocks(const ugk_cache8 &a) {
+  const int n = a.max_q < a.max_k ? a.max_q : a.max_k;
+  const int by_rows = (int)(((long long)n + 2 * kKeys - 2) / kKeys), by_keys = (int)(((long long)a.max_k + kKeys - 1) / kKeys);
+  return by_rows < by_keys ? by_rows : by_keys;
+}
+#define UGK_CH8(kernel)                                                        \
+  switch (padded(a.HS) / 16) {                                                 \
+    case 1: go(kernel<1>); break;                                              \
+    case 2: go(kernel<2>); break;                                              \
+    case 3: go(kernel<3>); break;                                              \
+    case 4: go(kernel<4>); break;                                              \
+    case 5: go(kernel<5>); break;                                              \
+    case 6: go(kernel<6>); break;                                              \
+    case 7: go(kernel<7>); break;                                              \
+    default: go(kernel<8>);                                                    \
+  }
+int launch_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, const float *v, const ugk_cache8 &a, int *word) {
+  const int per = touched_blocks(a);
+  const auto go = [&](auto kernel) {
+    launch(kernel, dim3((unsigned)a.nseq * a.NKV * per, 2), dim3(kBlock), 0, (int8_t *)k8, ks, (int8_t *)v8, vs, k, v, a, per, word);
+  };
+  UGK_CH8(k_cache8_store)
+  return check_launch("cache8_store");
+}
+int launch_cache8_load(float *k, float *v, const void *k8, const float *ks, const void *v8, const float *vs, const ugk_cache8 &a,
+                       int *word) {
+  const int per = touched_blocks(a);
+  const auto go = [&](auto kernel) {
+    launch(kernel, dim3((unsigned)a.nseq * a.NKV * per, 2), dim3(kBlock), 0, k, v, (const int8_t *)k8, ks, (const int8_t *)v8, vs, a, per,
+           word);
+  };
+  UGK_CH8(k_cache8_load)
+  return check_launch("cache8_load");
+}
+#undef UGK_CH8
+
+int launch_cache8_evict(int *table_out, int *len_out, float *weight_out, int *dropped, const int *table, const int *k_len,
+                        const float *weight, int nseq, int ld, int keep, int first, int recent, int *word) {
+  const auto go = [&](auto kernel) {
+    launch(kernel, dim3(nseq), dim3(kEvictThreads), 0, table_out, len_out, weight_out, dropped, table, k_len, weight, ld, keep, first, recent,
+           word);
+  };
+  if (ld <= kEvictThreads) go(k_cache8_evict<1>);
+  else if (ld <= 4 * kEvictThreads) go(k_cache8_evict<4>);
+  else go(k_cache8_evict<16>);
+  static_assert(kEvictBlocks == 16 * kEvictThreads, "the longest row of a table");
+  return check_launch("cache8_evict");
+}
+
+}  // namespace ugk

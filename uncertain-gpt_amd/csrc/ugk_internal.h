@@ -191,6 +191,21 @@ __device__ __forceinline__ int check_id(int id, int *ids, size_t i, const IdChec
 }
 __device__ __forceinline__ int checked_id(int *ids, size_t i, const IdCheck &g) { return check_id(ids[i], ids, i, g); }
 
+// Rows [begin, end) of `rows`, at most `most` of them; *bad: the arrays say otherwise.
+__device__ __forceinline__ int clamp_rows(const int *start, const int *end, int b, int rows, int most, int *begin,
+                                          bool *bad) {
+  if (!start) {
+    *begin = b * most;
+    return most;
+  }
+  const int s = start[b], e = end[b];
+  *begin = min(max(s, 0), rows);
+  const int stop = min(max(e, *begin), rows);
+  const int n = min(stop - *begin, most);
+  *bad = *bad || s != *begin || e != *begin + n;
+  return n;
+}
+
 // Launchers, one per kernel family. Each validates nothing (ugk_api.hip does)
 // and returns the launch status through check_launch.
 int launch_residual_forward(float *out, const float *x, const float *y, size_t n);
@@ -372,6 +387,22 @@ size_t attention_backward_bytes(const ugk_attention &a);
 // over all calls of heads of up to HS floats, and over those of up to `rows` rows of NH heads
 size_t attention_parts_bound(size_t HS);
 size_t attention_backward_bound(size_t rows, size_t NH, size_t HS);
+
+// A cache in 8 bits. `a` is checked, its strides and ld_table are filled in; word: the id error word. Attention's parts of a
+// split key axis, and what the blocks' weights are computed from, go to `mem` (cache8_attention_bytes; 0: none).
+constexpr int kCacheBlock = 64;        // tokens per block
+constexpr int kEvictBlocks = 1 << 14;  // blocks per sequence that the eviction takes
+constexpr int kWeighRows = 256;        // rows and heads per key/value head whose weights attention adds up per block
+int launch_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, const float *v, const ugk_cache8 &a, int *word);
+int launch_cache8_load(float *k, float *v, const void *k8, const float *ks, const void *v8, const float *vs, const ugk_cache8 &a,
+                       int *word);
+int launch_cache8_attention(float *out, float *lse, const float *q, const void *k8, const float *ks, const void *v8, const float *vs,
+                            float *weight, float *mem, const ugk_cache8 &a, int *word);
+size_t cache8_attention_bytes(const ugk_cache8 &a, bool weigh);
+int launch_cache8_evict(int *table_out, int *len_out, float *weight_out, int *dropped, const int *table, const int *k_len,
+                        const float *weight, int nseq, int ld, int keep, int first, int recent, int *word);
+int launch_draft_verify(int *accepted, int *tokens, const float *p, const float *q, const int *draft, const int *n_draft,
+                        const float *u, int nseq, int K, int V, int *word);
 
 // Workspace sizes.
 size_t layernorm_backward_scratch(int rows, int C);  // bytes of one call's partial rows

@@ -29,6 +29,7 @@ __all__ = [
     "dropout_residual_layernorm_forward", "layernorm_dropout_residual_backward",
     "Attention", "attention_forward", "attention_backward", "attention_backward_zeroed", "dense_attention_forward",
     "dense_attention_backward", "dense_attention_callbacks",
+    "Cache8", "CACHE8_BLOCK", "cache8_bytes", "cache8_store", "cache8_load", "cache8_attention", "cache8_evict", "draft_verify",
     "bayes_sample", "bayes_backward",
     "bayes_backward_philox", "kl_forward", "kl_backward", "adamw_update", "bbb_step_fused",
     "Loader", "loader_count", "ckpt_path", "ckpt_save", "ckpt_load",
@@ -87,6 +88,43 @@ class Attention(ctypes.Structure):
         self._most = min((t.numel() for t in tensors if t is not None and not isinstance(t, int)), default=Attention._most)
 
 
+CACHE8_BLOCK = 64  # tokens per block of a cache in 8 bits
+
+
+class Cache8(ctypes.Structure):
+    """``ugk_cache8``: the sequences, heads and row strides of a call on a cache in 8 bits.
+
+    ``q_start``, ``q_end``, ``k_len`` are int32 device tensors of at least ``nseq`` elements and ``table`` one of
+    ``nseq * ld_table`` (or device addresses, or None): the call's rows of sequence b are [q_start[b], q_end[b]), its
+    last positions, it has k_len[b] keys with these, and block ``table[b, j]`` holds its keys 64 j to 64 j + 63.
+    ``ld_table`` defaults to the last dimension of a two-dimensional ``table``. Strides in floats, 0 for rows without gaps; ``scale``
+    defaults to 1/sqrt(HS). The structure keeps its tensors alive; a call refuses an ``nseq`` or ``ld_table`` raised above what
+    they hold.
+    """
+    _tensors = ()
+    _most = (2 ** 31 - 1, 2 ** 62)  # sequences that the offset tensors hold, entries of the table
+    _NAMES = ("q_start", "q_end", "k_len", "table")
+    _fields_ = [(_n, _i) for _n in ("nseq", "NH", "NKV", "HS", "rows_q", "max_q", "max_k", "nblocks", "causal")] + \
+        [("scale", _fl)] + [(_n, _fp) for _n in _NAMES] + [("ld_table", _i)] + \
+        [(_n, ctypes.c_longlong) for _n in ("ldq", "ldk", "ldv", "ldo")]
+
+    def __init__(self, nseq: int, NH: int, NKV: int, HS: int, rows_q: int, max_q: int, max_k: int, nblocks: int,
+                 causal: bool = True, scale: Optional[float] = None, q_start=None, q_end=None, k_len=None, table=None,
+                 ld_table: int = 0, ldq: int = 0, ldk: int = 0, ldv: int = 0, ldo: int = 0):
+        if scale is None:
+            scale = HS ** -0.5 if HS > 0 else 0.0
+        held = table is not None and not isinstance(table, int)
+        if held and not ld_table and table.dim() == 2:
+            ld_table = table.shape[1]
+        tensors = (q_start, q_end, k_len, table)
+        need = (nseq, nseq, nseq, max(nseq, 0) * (ld_table or -(-max_k // CACHE8_BLOCK)))
+        super().__init__(nseq, NH, NKV, HS, rows_q, max_q, max_k, nblocks, 1 if causal else 0, scale,
+                         *(_ptr(t, n, m, "i32") for t, n, m in zip(tensors, self._NAMES, need)), ld_table, ldq, ldk, ldv, ldo)
+        self._tensors = tensors
+        self._most = (min((t.numel() for t in tensors[:3] if t is not None and not isinstance(t, int)), default=Cache8._most[0]),
+                      table.numel() if held else Cache8._most[1])
+
+
 _MATMUL_FWD = ctypes.CFUNCTYPE(_i, _fp, _fp, _fp, _fp, _fp, _i, _i, _i)
 _MATMUL_BWD = ctypes.CFUNCTYPE(_i, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _i, _i, _i)
 _ATTN_FWD = ctypes.CFUNCTYPE(_i, _fp, _fp, _fp, _i, _i, _i, _i)
@@ -130,6 +168,12 @@ _SIGS = {
     "ugk_attention_backward_zeroed": [_fp] * 9 + [Attention],
     "ugk_dense_attention_forward": [_fp, _fp, _fp, _i, _i, _i, _i],
     "ugk_dense_attention_backward": [_fp, _fp, _fp, _fp, _i, _i, _i, _i],
+    "ugk_cache8_bytes": [_i, _i, _i],
+    "ugk_cache8_store": [_fp] * 6 + [Cache8],
+    "ugk_cache8_load": [_fp] * 6 + [Cache8],
+    "ugk_cache8_attention": [_fp] * 8 + [Cache8],
+    "ugk_cache8_evict": [_fp] * 7 + [_i] * 5,
+    "ugk_draft_verify": [_fp] * 7 + [_i] * 3,
     "ugk_kl_forward": [ctypes.POINTER(ctypes.c_double), _fp, _fp, _sz, _fl],
     "ugk_kl_backward": [_fp, _fp, _fp, _fp, _sz, _fl, _fl],
     "ugk_adamw_update": [_fp, _fp, _fp, _fp, _sz, _i, _fl, _fl, _fl, _fl, _fl],
@@ -190,7 +234,7 @@ _SIGS = {
     "ugk_ckpt_save": [ctypes.c_char_p, _fp, _sz, Config, _i],
     "ugk_ckpt_load": [ctypes.c_char_p, _fp, _sz, Config, ctypes.POINTER(_i)],
 }
-_RET = {"ugk_last_error": ctypes.c_char_p, "ugk_get_stream": _fp, "ugk_scratch_bytes": _sz, "ugk_workspace_bytes": _sz,
+_RET = {"ugk_last_error": ctypes.c_char_p, "ugk_get_stream": _fp, "ugk_scratch_bytes": _sz, "ugk_workspace_bytes": _sz, "ugk_cache8_bytes": _sz,
         "ugk_loader_tokens": ctypes.c_long, "ugk_loader_position": ctypes.c_long,
         "ugk_param_count": _sz, "ugk_act_count": _sz}
 for _name, _args in _SIGS.items():
@@ -222,7 +266,7 @@ def _import_torch():
     global _torch, _Tensor, _DTYPES, _one_device
     if _torch is None:
         import torch
-        _torch, _Tensor, _DTYPES = torch, torch.Tensor, {"f32": torch.float32, "i32": torch.int32}
+        _torch, _Tensor, _DTYPES = torch, torch.Tensor, {"f32": torch.float32, "i32": torch.int32, "i8": torch.int8}
         _one_device = torch.cuda.device_count() == 1
     return _torch
 
@@ -241,7 +285,7 @@ def _ptr_or_raise(x, what: str, need: int, dtype: str):
     if isinstance(x, int):
         return x
     torch = _import_torch()
-    want = {"f32": torch.float32, "i32": torch.int32}[dtype]
+    want = _DTYPES[dtype]
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: expected a torch tensor or a device address, got {type(x)!r}")
     if x.device.type != "cuda":
@@ -471,11 +515,11 @@ def _here(x, what: str) -> None:
         raise ValueError(f"{what}: tensor is on {x.device}, the current device is cuda:{_torch.cuda.current_device()}")
 
 
-def _ptr_here(x, what: str, need: int):
-    """_ptr of floats that must be on the current GPU."""
-    if type(x) is _Tensor and _one_device and x.dtype is _DTYPES["f32"] and x.is_cuda and x.numel() >= need and x.is_contiguous():
+def _ptr_here(x, what: str, need: int, dtype: str = "f32"):
+    """_ptr of a tensor that must be on the current GPU."""
+    if type(x) is _Tensor and _one_device and x.dtype is _DTYPES[dtype] and x.is_cuda and x.numel() >= need and x.is_contiguous():
         return x.data_ptr()
-    p = _ptr(x, what, need, "f32")
+    p = _ptr(x, what, need, dtype)
     _here(x, what)
     return p
 
@@ -564,6 +608,78 @@ def _attention_backward(fn, dq, dk, dv, dout, q, k, v, out, lse, a: Attention) -
     _check(fn(_rows_ptr(dq, "dq", nq), _rows_ptr(dk, "dk", nk), _rows_ptr(dv, "dv", nv), _rows_ptr(dout, "dout", no),
               _rows_ptr(q, "q", nq), _rows_ptr(k, "k", nk), _rows_ptr(v, "v", nv), _rows_ptr(out, "out", no),
               _ptr_here(lse, "lse", a.rows_q * a.NH), a))
+
+
+def cache8_bytes(nblocks: int, NKV: int, HS: int) -> int:
+    """Elements of k8, and of v8 (int8): ``nblocks * NKV * 64 * HP``, HP = HS rounded up to a multiple of 16."""
+    return int(lib.ugk_cache8_bytes(nblocks, NKV, HS))
+
+
+def _cache8(a: Cache8, k8, ks, v8, vs):
+    """The cache's addresses, after the checks of what a call's structure holds."""
+    if a.nseq > a._most[0]:
+        raise ValueError(f"nseq: {a.nseq} sequences, the offsets hold {a._most[0]}")
+    if a.nseq * (a.ld_table or -(-a.max_k // CACHE8_BLOCK)) > a._most[1]:
+        raise ValueError(f"table: {a.nseq} rows of {a.ld_table}, the tensor holds {a._most[1]} entries")
+    if not _one_device:
+        for t, name in zip(a._tensors, a._NAMES):
+            _here(t, name)
+    n, scales = lib.ugk_cache8_bytes(a.nblocks, a.NKV, a.HS), a.nblocks * a.NKV
+    return (_ptr_here(k8, "k8", n, "i8"), _ptr_here(ks, "ks", scales), _ptr_here(v8, "v8", n, "i8"), _ptr_here(vs, "vs", scales))
+
+
+def _cache8_rows(a: Cache8, ld: int, heads: int):
+    """Of rows of ``heads`` heads the floats from the first element to the end of the last row, from row to row and in a row, and
+    the heads."""
+    w = heads * a.HS
+    ld = ld or w
+    return ((a.rows_q - 1) * ld + w if a.rows_q > 0 else 0, ld, w, heads)
+
+
+def cache8_store(k8, ks, v8, vs, k, v, a: Cache8) -> None:
+    """Stores the rows of k and v, which may be views into rows that hold other things as well, as the last keys of their
+    sequences: int8 codes in k8 and v8 (``cache8_bytes`` each), a power of two per block and key/value head in ks and vs
+    (nblocks, NKV)."""
+    c = _cache8(a, k8, ks, v8, vs)
+    _check(lib.ugk_cache8_store(*c, _rows_ptr(k, "k", _cache8_rows(a, a.ldk, a.NKV)), _rows_ptr(v, "v", _cache8_rows(a, a.ldv, a.NKV)), a))
+
+
+def cache8_load(k, v, k8, ks, v8, vs, a: Cache8) -> None:
+    """What the cache holds where cache8_store of the same ``a`` puts it, to the rows of k and v."""
+    c = _cache8(a, k8, ks, v8, vs)
+    _check(lib.ugk_cache8_load(_rows_ptr(k, "k", _cache8_rows(a, a.ldk, a.NKV)), _rows_ptr(v, "v", _cache8_rows(a, a.ldv, a.NKV)), *c, a))
+
+
+def cache8_attention(out, lse, q, k8, ks, v8, vs, a: Cache8, weight=None) -> None:
+    """attention_forward of q against the cache; lse (rows_q, NH) may be None. ``weight`` (nseq, ld_table), if given, accumulates
+    what each block got over the rows and heads."""
+    c = _cache8(a, k8, ks, v8, vs)
+    w = None if weight is None else _ptr_here(weight, "weight", a.nseq * (a.ld_table or -(-a.max_k // CACHE8_BLOCK)))
+    _check(lib.ugk_cache8_attention(_rows_ptr(out, "out", _cache8_rows(a, a.ldo, a.NH)), _ptr_here(lse, "lse", a.rows_q * a.NH),
+                                    _rows_ptr(q, "q", _cache8_rows(a, a.ldq, a.NH)), *c, w, a))
+
+
+def cache8_evict(table_out, len_out, weight_out, dropped, table, k_len, weight, nseq: int, ld: int, keep: int, first: int = 0,
+                 recent: int = 1) -> None:
+    """All but ``keep`` blocks of each sequence leave its row of the table (nseq, ld): those of least weight behind the
+    ``first`` first and before the ``recent`` last. They move to the row's end; ``len_out`` and ``dropped`` (nseq) are the
+    keys left and the blocks gone. Outputs may be the inputs."""
+    n = nseq * ld
+    _check(lib.ugk_cache8_evict(
+        _ptr_here(table_out, "table_out", n, "i32"), _ptr_here(len_out, "len_out", nseq, "i32"), _ptr_here(weight_out, "weight_out", n),
+        _ptr_here(dropped, "dropped", nseq, "i32"), _ptr_here(table, "table", n, "i32"), _ptr_here(k_len, "k_len", nseq, "i32"),
+        _ptr_here(weight, "weight", n), nseq, ld, keep, first, recent))
+
+
+def draft_verify(accepted, tokens, p, q, draft, n_draft, u, nseq: int, K: int, V: int) -> None:
+    """Drafted tokens (nseq, K) of probabilities q (nseq, K, V; None: certain) against the target's p (nseq, K + 1, V), with the
+    random numbers u (nseq, K + 1): ``accepted`` (nseq) drafts, and ``tokens`` (nseq, K + 1), these, the next token and -1.
+    ``n_draft`` (nseq; None: K) are there."""
+    r = nseq * (K + 1)
+    _check(lib.ugk_draft_verify(
+        _ptr_here(accepted, "accepted", nseq, "i32"), _ptr_here(tokens, "tokens", r, "i32"), _ptr_here(p, "p", r * V),
+        _ptr_here(q, "q", nseq * K * V), _ptr_here(draft, "draft", nseq * K, "i32"), _ptr_here(n_draft, "n_draft", nseq, "i32"),
+        _ptr_here(u, "u", r), nseq, K, V))
 
 
 def dense_attention_forward(out, qkv, B: int, T: int, C: int, NH: int) -> None:
