@@ -29,7 +29,8 @@ constexpr int kMaxDevices = 64;
 constexpr size_t kAlign = 256;
 size_t align_up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 const char *const kRegionName[kNumRegions] = {"LayerNorm partial rows", "encoder bucket state", "KL partial sums",
-                                              "softmax row statistics", "attention row sums and parts"};
+                                              "softmax row statistics", "attention row sums and parts",
+                                              "sums of the drafts' rows"};
 
 struct Kept {
   void *p;
@@ -45,7 +46,7 @@ struct DevWorkspace {
   char *user = nullptr;
   size_t user_bytes = 0;
   size_t off[kNumRegions] = {}, cap[kNumRegions] = {};
-  bool fresh[kNumRegions] = {true, true, true, true, true};
+  bool fresh[kNumRegions] = {true, true, true, true, true, true};
   bool captured[kNumRegions] = {};  // own[r] is in a graph, which may be replayed at any time
   Kept *kept = nullptr;             // regions that only graphs use any more, until ugk_release_graph_memory
 };
@@ -70,7 +71,7 @@ size_t attention_scratch(size_t rows, size_t C, size_t NH, size_t parts, size_t 
 
 // Region sizes for every entry point at shapes up to cfg: the step driver's
 // 2L+1 LayerNorm slots (at least the one slot of a per-op call), the encoder
-// state, the KL partial sums, the softmax statistics of B*T rows, and attention
+// state, the KL partial sums, the softmax statistics of B*T rows, the sums of drafts over V tokens, and attention
 // over B*T rows of C channels in NH heads (the dense callback's backward; none
 // where the callbacks take no such heads, or NH is 0).
 void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
@@ -80,6 +81,7 @@ void region_sizes(const ugk_config &cfg, size_t out[kNumRegions]) {
   out[kRegEncoder] = encoder_backward_scratch();
   out[kRegKl] = kl_forward_scratch();
   out[kRegSoftmax] = softmax_scratch(rows, cfg.V);
+  out[kRegDraft] = draft_verify_bound(cfg.V);
   const int NH = cfg.NH, HS = NH > 0 ? cfg.C / NH : 0;
   out[kRegAttention] = rows > 0 && HS >= 1 && HS <= kMaxHead && HS * NH == cfg.C
                            ? attention_scratch(rows, cfg.C, NH, attention_parts_bound(HS), attention_backward_bound(rows, NH, HS))
@@ -938,7 +940,12 @@ int ugk_draft_verify(int *accepted, int *tokens, const float *p, const float *q,
     return bad(fn, "accepted and tokens must be distinct from each other and from the inputs");
   int *word = ids_error_word();
   if (!word) return UGK_EHIP;
-  if (int e = launch_draft_verify(accepted, tokens, p, q, draft, n_draft, u, nseq, K, V, word)) return e;
+  double *sums = nullptr;
+  if (const size_t bytes = draft_verify_bytes(nseq, V)) {
+    sums = static_cast<double *>(workspace(kRegDraft, bytes));
+    if (!sums) return UGK_ENOMEM;
+  }
+  if (int e = launch_draft_verify(accepted, tokens, p, q, draft, n_draft, u, sums, nseq, K, V, word)) return e;
   return ok();
 }
 

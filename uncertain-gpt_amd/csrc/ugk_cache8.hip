@@ -16,6 +16,8 @@
 // column, the order in which the lanes hold the weights.
 #include <math.h>
 
+#include <type_traits>
+
 #include "ugk_internal.h"
 #include "ugk_split.h"
 
@@ -45,13 +47,19 @@ __device__ __forceinline__ Seq8 sequence8(const ugk_cache8 &a, int b, bool tell,
   return s;
 }
 
-// Block j of sequence b, or -1 (reported) where the table names none.
-__device__ __forceinline__ int block_of(const ugk_cache8 &a, int b, int j, int *word, int code) {
-  if (!a.table) return b * a.ld_table + j;
-  const int id = a.table[(size_t)b * a.ld_table + j];
+// What the table says of block j of sequence b, and the block, or -1 (reported) where that is none. (Two steps: a loop reads the
+// table a turn before it needs the block.)
+__device__ __forceinline__ int table_at(const ugk_cache8 &a, int b, int j) {
+  const size_t at = (size_t)b * a.ld_table + j;
+  return a.table ? a.table[at] : (int)at;
+}
+__device__ __forceinline__ int checked_block(const ugk_cache8 &a, int id, int *word, int code) {
   if ((unsigned)id < (unsigned)a.nblocks) return id;
   *word = code;
   return -1;
+}
+__device__ __forceinline__ int block_of(const ugk_cache8 &a, int b, int j, int *word, int code) {
+  return checked_block(a, table_at(a, b, j), word, code);
 }
 
 __host__ __device__ __forceinline__ int padded(int HS) { return (HS + 15) & ~15; }
@@ -77,10 +85,10 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float ratio) {
                code_of((float)code_at(w, 3), ratio));
 }
 
-// What a workgroup of the store and the load has: a block of a sequence of which rows [r0, r1) are
+// What a workgroup of the store and the load has: block j of a sequence, of which rows [r0, r1) are
 // the call's, those before r0 in the cache already.
 struct Touched {
-  int b, h, q, r0, r1, id;  // q: the buffer's row of r0
+  int b, h, j, q, r0, r1;  // q: the buffer's row of r0
 };
 __device__ __forceinline__ bool touched(const ugk_cache8 &a, int per, int *word, int code, Touched *t) {
   const unsigned x = blockIdx.x;
@@ -90,13 +98,13 @@ __device__ __forceinline__ bool touched(const ugk_cache8 &a, int per, int *word,
   const bool tell = t->h == 0 && nth == 0 && blockIdx.y == 0;
   const Seq8 s = sequence8(a, t->b, tell, word, code);
   if (s.Lq > s.Lk && tell && threadIdx.x == 0) *word = code;  // rows before the first key
-  const int begin = max(s.Lk - s.Lq, 0), j = begin / kKeys + nth;
-  if (s.Lq == 0 || j * kKeys >= s.Lk) return false;
-  t->r0 = max(begin - j * kKeys, 0);
-  t->r1 = min(s.Lk - j * kKeys, kKeys);
-  t->q = s.q0 + s.Lq - s.Lk + j * kKeys + t->r0;
-  t->id = block_of(a, t->b, j, word, code);
-  return t->id >= 0;
+  const int begin = max(s.Lk - s.Lq, 0);
+  t->j = begin / kKeys + nth;
+  if (s.Lq == 0 || t->j * kKeys >= s.Lk) return false;
+  t->r0 = max(begin - t->j * kKeys, 0);
+  t->r1 = min(s.Lk - t->j * kKeys, kKeys);
+  t->q = s.q0 + s.Lq - s.Lk + t->j * kKeys + t->r0;
+  return true;
 }
 
 // One block of one head and of k or v (blockIdx.y) by a workgroup. A thread has four columns of the rows
@@ -114,6 +122,7 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
   const bool values = blockIdx.y;
   const long long ld = values ? a.ldv : a.ldk;
   const float *src = (values ? v : k) + (long long)(t.q - t.r0) * ld + t.h * a.HS;
+  const int id = block_of(a, t.b, t.j, word, UGK_IDS_CACHE8_STORE);  // on its way while the rows are
   float4 x[kPer][4];
   uint32_t most = 0;
 #pragma unroll
@@ -134,6 +143,10 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
       }
     }
   }
+  if (id < 0) return;
+  const size_t at = (size_t)id * a.NKV + t.h;
+  float *sp = (values ? vs : ks) + at;
+  const float was = t.r0 > 0 ? *sp : 0.0f;
   bool finite = true;
   const auto look = [&](float &f) {
     const uint32_t u = abs_bits(f);
@@ -156,9 +169,7 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
   __syncthreads();
   static_assert(kBlock / kWave == 4, "four wavefronts");
   most = max(max(top[0], top[1]), max(top[2], top[3]));
-  const size_t at = (size_t)t.id * a.NKV + t.h;
-  float *sp = (values ? vs : ks) + at;
-  const float was = t.r0 > 0 ? *sp : 0.0f, need = scale_for(most), now = fmaxf(was, need);
+  const float now = fmaxf(was, scale_for(most));
   const float inv = now > 0.0f ? 1.0f / now : 0.0f, ratio = was * inv;
   const bool grown = t.r0 > 0 && now > was && was > 0.0f;
   uint32_t *dst = reinterpret_cast<uint32_t *>((values ? v8 : k8) + at * kKeys * HP);
@@ -226,7 +237,9 @@ __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, cons
   const bool values = blockIdx.y;
   const long long ld = values ? a.ldv : a.ldk;
   float *to = (values ? v : k) + (long long)(t.q - t.r0) * ld + t.h * a.HS;
-  const size_t at = (size_t)t.id * a.NKV + t.h;
+  const int id = block_of(a, t.b, t.j, word, UGK_IDS_CACHE8_LOAD);
+  if (id < 0) return;
+  const size_t at = (size_t)id * a.NKV + t.h;
   const float s = (values ? vs : ks)[at];
   const uint32_t *src = reinterpret_cast<const uint32_t *>((values ? v8 : k8) + at * kKeys * HP);
   if (values) {
@@ -263,31 +276,37 @@ __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, cons
 struct Parts8 {
   float *o, *m, *l;
   float2 *block, *stat;
-  int splits;
+  int splits, chunk;  // blocks per part: a row has the parts up to its last key's
 };
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float or0(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// The exponent of a block's scale, a power of two; of 0 below all others.
+__device__ __forceinline__ float exponent(float scale) { return scale == 0.0f ? -4096.0f : (float)(__builtin_amdgcn_frexp_expf(scale) - 1); }
 
 // Running sums of a row. l stands on m, the largest score so far; the output's sum on the block whose weight times
 // values was largest, 2^(mo + e): a block's values share a scale, so neither large values of little weight
 // nor small ones of much cost the others their digits, and nothing leaves the range before the division.
 struct Running {
   float m = -INFINITY, l = 0.0f, mo = -INFINITY, e = 0.0f;
-  // A block with maximum mb, sum lb and values of the scale vs. Returns the factors of the sum so far and of the block's.
-  __device__ __forceinline__ float2 add(float mb, float lb, float vs) {
+  // A block's largest score, and its sum times 2^up on another score that is no larger than the largest so far.
+  __device__ __forceinline__ void sum(float mb, float lb, float on, float up) {
     const float top = fmaxf(m, mb), base = or0(top);
-    l = fmaf(l, ex2(m - base), lb * ex2(mb - base));
+    l = fmaf(l, ex2(m - base), lb * ex2((on - base) - up));
     m = top;
-    const float mant = __builtin_amdgcn_frexp_mantf(vs), ve = vs == 0.0f ? -4096.0f : (float)__builtin_amdgcn_frexp_expf(vs);
+  }
+  // A block with largest score mb and values of the scale 2^ve: the output's sum stands on it if it is the largest. Returns
+  // the factor of the sum so far.
+  __device__ __forceinline__ float stand(float mb, float ve) {
     const bool more = mb + ve > mo + e;
-    const float mn = more ? mb : mo, en = more ? ve : e, on = or0(mn);
-    // a block of which the row sees nothing counts for nothing, whatever its scale
-    const float2 f = make_float2(ex2((mo - on) + (e - en)), mb == -INFINITY ? 0.0f : mant * ex2((mb - on) + (ve - en)));
+    const float mn = more ? mb : mo, en = more ? ve : e, f = ex2((mo - or0(mn)) + (e - en));
     mo = mn;
     e = en;
     return f;
   }
+  // The factor of such a block's sum of values, of which its weights stand on mb; of a block of which the row sees nothing 0.
+  __device__ __forceinline__ float factor(float mb, float ve) const { return mb == -INFINITY ? 0.0f : ex2((mb - or0(mo)) + (ve - e)); }
   // The factor that makes the output's sum the output, as a float and a power of two.
   __device__ __forceinline__ float last(float sum, int *p) const {
     const float x = (or0(mo) - or0(m)) + e, r = rintf(x);
@@ -296,13 +315,45 @@ struct Running {
   }
 };
 
-// f = scale log2(e) of the call, ks of a block and 2^x of a row's whole numbers, as one factor of its scores: below the largest float, so
-// that a score of 0 stays 0.
+// N floats of a row of q from `at` on, 0 behind its HS, with the sign of the scores' scale; and the largest magnitude's bits.
+template <int N>
+__device__ __forceinline__ uint32_t load_q(const float *p, int at, const ugk_cache8 &a, float (&x)[N]) {
+  if (at + N <= a.HS) {
+#pragma unroll
+    for (int d = 0; d < N; d += 4) {
+      const float4 y = ld4(p + at + d);
+      x[d] = y.x;
+      x[d + 1] = y.y;
+      x[d + 2] = y.z;
+      x[d + 3] = y.w;
+    }
+  } else {
+#pragma unroll
+    for (int d = 0; d < N; d++) {
+      const float y = p[min(at + d, a.HS - 1)];
+      x[d] = at + d < a.HS ? y : 0.0f;
+    }
+  }
+  uint32_t most = 0;
+#pragma unroll
+  for (int d = 0; d < N; d++) {
+    most = max(most, abs_bits(x[d]));
+    if (a.scale < 0.0f) x[d] = -x[d];
+  }
+  return most;
+}
+
+// f = |scale| log2(e) of the call, ks of a block and 2^x of a row's whole numbers, as one factor of its scores: a normal
+// number, so that a score of 0 stays 0 and -infinity of a masked one itself.
 __device__ __forceinline__ float score_factor(float f, float ks, int x) {
   const float y = __builtin_amdgcn_ldexpf(__builtin_amdgcn_frexp_mantf(f) * __builtin_amdgcn_frexp_mantf(ks),
                                           __builtin_amdgcn_frexp_expf(f) + __builtin_amdgcn_frexp_expf(ks) + x);
-  return fminf(fmaxf(y, -3.402823466e38f), 3.402823466e38f);
+  return fmaxf(fminf(y, 3.402823466e38f), 0x1p-126f);
 }
+// The largest score of a block from the largest product, and what is added to a score times the factor so that 2^ of it is the weight times
+// 2^up: a score beyond the range makes it NaN.
+__device__ __forceinline__ float top_score(float product, float fac) { return product == -INFINITY ? product : product * fac; }
+__device__ __forceinline__ float less_top(float top, float up) { return top == INFINITY ? NAN : up - or0(top); }
 
 // Sum and maximum over the 16 lanes of a row.
 __device__ __forceinline__ float sum16(float v) {
@@ -327,223 +378,505 @@ __device__ __forceinline__ float undigits(v4i d) {
 
 constexpr int kFewWaves = 4;
 
-// Few rows (query rows times heads of the group): a token's step, drafts, an observation window.
+// The sequence and key/value head of workgroup x in a round of all of them, one further each time that all have had one: workgroups go to the chip's eight
+// dies in turn, and the long sequences would else be with the same ones throughout where the pairs are a multiple of eight.
+__device__ __forceinline__ unsigned turned(unsigned x, unsigned round, unsigned pairs) { return (x % pairs + round) % pairs; }
+
+// The codes of a block as the operands of the 8-bit matrix units: 16 bytes a lane of 16 keys' rows (kf) and of 16 columns (vf),
+// and the scales. A block that is not there is read as block 0, and its keys are masked.
+template <int DT>
+struct Codes {
+  static constexpr int KS = (DT + 3) / 4;
+  v4i kf[KS][4], vf[DT];
+  int koff[KS], voff, HP;
+  __device__ __forceinline__ Codes(int HP, int lane) : HP(HP) {
+    const int col = lane & 15, quad = lane >> 4;
+#pragma unroll
+    for (int st = 0; st < KS; st++) koff[st] = col * HP + 16 * min(4 * st + quad, HP / 16 - 1);  // behind the row q's digits are 0
+    voff = col * kKeys + 16 * quad;
+  }
+  __device__ __forceinline__ void keys(const int8_t *k8, size_t at) {
+    const int8_t *p = k8 + at * kKeys * HP;
+#pragma unroll
+    for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+      for (int st = 0; st < KS; st++) kf[st][kt] = *reinterpret_cast<const v4i *>(p + kt * 16 * HP + koff[st]);
+  }
+  __device__ __forceinline__ void values(const int8_t *v8, size_t at) {
+    const int8_t *p = v8 + at * kKeys * HP;
+#pragma unroll
+    for (int t = 0; t < DT; t++) vf[t] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(p + min(t, HP / 16 - 1) * 16 * kKeys + voff));
+  }
+};
+
+// x is computed here, in this branch: the compiler otherwise moves what only the next step of a loop uses behind the branches in between, and holds all
+// that it is computed from until there.
+template <typename T>
+__device__ __forceinline__ T here(T x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A 4 x 4 transposition of bytes: the words' bytes 0, then 1, 2 and 3.
+__device__ __forceinline__ v4i turn4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t t0 = __builtin_amdgcn_perm(b, a, 0x05010400u), t1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+  const uint32_t t2 = __builtin_amdgcn_perm(d, c, 0x05010400u), t3 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+  return v4i{(int)__builtin_amdgcn_perm(t2, t0, 0x05040100u), (int)__builtin_amdgcn_perm(t2, t0, 0x07060302u),
+             (int)__builtin_amdgcn_perm(t3, t1, 0x05040100u), (int)__builtin_amdgcn_perm(t3, t1, 0x07060302u)};
+}
+
+// Where a row's results go: of this part of the key axis, or of the whole.
+struct Place8 {
+  float *o, *m, *l, *lse;
+  __device__ __forceinline__ Place8(float *out, float *lse_, const Parts8 &parts, const ugk_cache8 &a, int part, size_t row, int h) {
+    const size_t p = ((size_t)part * a.rows_q + row) * a.NH + h;
+    o = parts.o ? parts.o + p * a.HS : out + row * a.ldo + (size_t)h * a.HS;
+    m = parts.o ? parts.m + p : nullptr;
+    l = parts.o ? parts.l + p : nullptr;
+    lse = parts.o || !lse_ ? nullptr : lse_ + row * a.NH + h;
+  }
+  __device__ __forceinline__ void put(float top, float sum) const {
+    if (m) {
+      *m = top;
+      *l = sum;
+    } else if (lse) {
+      *lse = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn28;
+    }
+  }
+};
+
+// A wavefront's blocks from the first, `by` apart, with what the next one needs on its way: the keys from where the
+// scores are computed, the values from where the output is, the table a turn before.
+struct Walk {
+  int j, stop, by, id, next;  // next: what the table says of j + by
+  __device__ __forceinline__ Walk(const ugk_cache8 &a, int b, int first, int stop, int by, int *word) : j(first), stop(stop), by(by) {
+    id = next = 0;
+    if (j < stop) {
+      const int t = table_at(a, b, j);
+      next = table_at(a, b, min(j + by, stop - 1));
+      id = checked_block(a, t, word, UGK_IDS_CACHE8_ATTENTION);
+    }
+  }
+  __device__ __forceinline__ bool there() const { return id >= 0; }
+  __device__ __forceinline__ bool more() const { return j + by < stop; }
+  // The next block, while this one is computed; the table's word on the one behind it is on its way then.
+  __device__ __forceinline__ int ahead(const ugk_cache8 &a, int b, int *word) {
+    const int i = checked_block(a, __builtin_amdgcn_readfirstlane(next), word, UGK_IDS_CACHE8_ATTENTION);
+    next = table_at(a, b, min(j + 2 * by, stop - 1));
+    return i;
+  }
+  __device__ __forceinline__ void step(int i) {
+    j += by;
+    id = i;
+  }
+};
+__device__ __forceinline__ size_t block_head(int id, int NKV, int hk) { return (size_t)max(id, 0) * NKV + hk; }
+
+// Up to four rows (query rows times heads of the group) of a sequence and key/value head.
 //
 // A row of q is held as whole numbers of 31 bits next to its largest element, and those as four digits, so that four
 // rows are one 16-row operand of the 8-bit matrix units: a block's scores take two instructions per 16 keys at 128 floats per
 // head, their sums are exact, and a lane finds the four digits of its score in its own four registers.
 // The weights, 31 bits next to the block's largest, go the same way into the product with the values.
-template <int DT, int R>
-__global__ __launch_bounds__(kFewWaves *kWave) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8,
-                                                                const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
-                                                                Parts8 parts, unsigned pairs, unsigned groups, int *word) {
+template <int DT>
+__global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8,
+                                                                   const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
+                                                                   Parts8 parts, unsigned pairs, int *word) {
   constexpr int KS = (DT + 3) / 4, kStride = 20;
   __shared__ alignas(16) uint32_t lp[kFewWaves][16 * kStride];
   __shared__ float lo[kFewWaves][4][DT * 16];
   __shared__ float lm[kFewWaves][4], ll[kFewWaves][4];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-  const unsigned pair = blockIdx.x % pairs, group = blockIdx.x / pairs % groups;
-  const int part = blockIdx.x / pairs / groups;
-  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV, HP = padded(a.HS), CH = HP / 16;
-  const Seq8 s = sequence8(a, b, hk == 0 && part == 0 && group == 0, word, UGK_IDS_CACHE8_ATTENTION);
-  const int rows = s.Lq * G, base_row = group * 4 * R;
-  if (base_row >= rows) return;
-  const int end = s.seen((min(base_row + 4 * R, rows) - 1) / G, a.causal);  // the last row sees most
-  const int nb = (end + kKeys - 1) / kKeys;
-  const int first = (int)((long long)nb * part / parts.splits), stop = (int)((long long)nb * (part + 1) / parts.splits);
-  const float f = a.scale * kLog2e8;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const unsigned pair = turned(blockIdx.x, blockIdx.x / pairs, pairs);
+  const int part = blockIdx.x / pairs;
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
+  const Seq8 s = sequence8(a, b, hk == 0 && part == 0, word, UGK_IDS_CACHE8_ATTENTION);
+  const int rows = s.Lq * G;
+  if (rows == 0) return;
+  const int end = s.seen(s.Lq - 1, a.causal), nb = (end + kKeys - 1) / kKeys;  // the last row sees most
+  const int first = part * parts.chunk, stop = min(first + parts.chunk, nb);
+  if (part > 0 && first >= nb) return;  // no row of the workgroup has this part
+  const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
 
-  // q's digits: lane (row % 4 * 4 + digit, quad) holds dims 64 step + 16 quad + [0, 16)
-  v4i aq[R][KS];
-  int ex[R], lim[R], least = end;
-  bool nan[R];
-  Running run[R];
-  float o[R][DT];
-#pragma unroll
-  for (int rt = 0; rt < R; rt++) {
-    const int rr = min(base_row + 4 * rt + (col >> 2), rows - 1);
-    const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (hk * G + rr % G) * a.HS;
+  Codes<DT> c(padded(a.HS), lane);
+  Walk walk(a, b, first + wave, stop, kFewWaves, word);
+  float kscale = 0.0f, vscale = 0.0f;
+  if (walk.j < stop) {
+    const size_t at = block_head(walk.id, a.NKV, hk);
+    c.keys(k8, at);
+    c.values(v8, at);
+    kscale = ks[at];
+    vscale = vs[at];
+  }
+
+  // q's digits: lane (4 row + digit, quad) holds dims 64 step + 16 quad + [0, 16)
+  v4i aq[KS];
+  int ex;
+  bool nan;
+  {
+    const int rr = min(col >> 2, rows - 1);
+    const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (size_t)(hk * G + rr % G) * a.HS;
     float x[KS][16];
     uint32_t most = 0;
 #pragma unroll
-    for (int st = 0; st < KS; st++)
-#pragma unroll
-      for (int d = 0; d < 16; d++) {
-        const int at = 64 * st + 16 * quad + d;
-        x[st][d] = at < a.HS ? p[at] : 0.0f;
-        most = max(most, abs_bits(x[st][d]));
-      }
+    for (int st = 0; st < KS; st++) most = max(most, load_q(p, 64 * st + 16 * quad, a, x[st]));
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
     most = max(most, (uint32_t)__shfl_xor((int)most, 32));
     const int e = (int)(most >> 23) - 127;  // below 2^(e + 1)
 #pragma unroll
     for (int st = 0; st < KS; st++) {
-      v4i w = {0, 0, 0, 0};
+      aq[st] = v4i{0, 0, 0, 0};
 #pragma unroll
       for (int d = 0; d < 16; d++) {
         const uint32_t y = digits((int)rintf(__builtin_amdgcn_ldexpf(x[st][d], 29 - e)));
-        w[d / 4] |= (int)((y >> (8 * (lane & 3)) & 255u) << (8 * (d & 3)));
+        aq[st][d / 4] |= (int)((y >> (8 * (lane & 3)) & 255u) << (8 * (d & 3)));
       }
-      if (most >= kInfBits) w = v4i{0, 0, 0, 0};
-      aq[rt][st] = w;
+      if (most >= kInfBits) aq[st] = v4i{0, 0, 0, 0};
     }
-    // for the lanes that hold the row's scores: row quad of the four
-    ex[rt] = __shfl(e, 4 * quad) - 29;
-    nan[rt] = (uint32_t)__shfl((int)most, 4 * quad) >= kInfBits;
-    const int mine = base_row + 4 * rt + quad;
-    lim[rt] = mine < rows ? s.seen(mine / G, a.causal) : end;
-    least = min(least, lim[rt]);
-#pragma unroll
-    for (int t = 0; t < DT; t++) o[rt][t] = 0.0f;
+    // for the lanes that hold the row's scores: row quad
+    ex = __shfl(e, 4 * quad) - 29;
+    nan = (uint32_t)__shfl((int)most, 4 * quad) >= kInfBits;
   }
+  const int lim = quad < rows ? s.seen(quad / G, a.causal) : end;
+  Running run;
+  float o[DT];
 #pragma unroll
-  for (int x = 16; x < kWave; x *= 2) least = min(least, __shfl_xor(least, x));
-
-  int koff[KS], voff[DT];
-#pragma unroll
-  for (int st = 0; st < KS; st++) koff[st] = col * HP + 16 * min(4 * st + quad, CH - 1);  // behind the row q's digits are 0
-#pragma unroll
-  for (int t = 0; t < DT; t++) voff[t] = (16 * min(t, CH - 1) + col) * kKeys + 16 * quad;
+  for (int t = 0; t < DT; t++) o[t] = 0.0f;
   uint32_t *mylp = lp[wave];
 
-  int next = first + wave < stop ? block_of(a, b, first + wave, word, UGK_IDS_CACHE8_ATTENTION) : 0;
-  for (int j = first + wave; j < stop; j += kFewWaves) {
-    const bool there = next >= 0;
-    const size_t at = (size_t)(there ? next : 0) * a.NKV + hk;
-    const int8_t *kb = k8 + at * kKeys * HP, *vb = v8 + at * kKeys * HP;
-    v4i kf[KS][4], vf[DT];
+  const auto block = [&](auto next) {  // next: another block follows
+    constexpr bool kNext = decltype(next)::value;
+    const int id = kNext ? walk.ahead(a, b, word) : 0;
+    const size_t ahead = block_head(id, a.NKV, hk);
+    const int seen = walk.there() ? lim - walk.j * kKeys : 0;  // of this block's keys
+    const float fac = nan ? NAN : score_factor(f, kscale, ex), vnow = exponent(vscale);
+    float p[4], mb = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 4; kt++) {
+      v4i acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int st = 0; st < KS; st++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[st], c.kf[st][kt], acc, 0, 0, 0);
+      p[kt] = kt * 16 + col < seen ? undigits(acc) : -INFINITY;
+      mb = fmaxf(mb, p[kt]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // into the registers that the products have read
+    if (kNext) {
+      c.keys(k8, ahead);
+      kscale = ks[ahead];
+      vscale = vs[ahead];
+    }
+    mb = top_score(max16(mb), fac);
+    const float less = less_top(mb, 30.0f);  // weights times 2^30
+    uint32_t y[4];
+    float lb = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < 4; kt++) {
+      p[kt] = ex2(fmaf(p[kt], fac, less));
+      lb += p[kt];
+      y[kt] = digits((int)p[kt]);
+    }
+    const v4i t = turn4(y[0], y[1], y[2], y[3]);  // the four keys' digits side by side: a word per digit
+    uint32_t *w = mylp + 4 * quad * kStride + col;
+#pragma unroll
+    for (int d = 0; d < 4; d++) w[d * kStride] = (uint32_t)t[d];
+    __builtin_amdgcn_wave_barrier();
+    const v4i ap = *reinterpret_cast<const v4i *>(mylp + col * kStride + 4 * quad);
+    __builtin_amdgcn_wave_barrier();
+    lb *= 0x1p-30f;
+    if (parts.block) {
+      const float sum = sum16(lb);
+      if (col == 0 && quad < rows)
+        parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + quad) * a.ld_table + walk.j] = make_float2(mb, sum);
+    }
+    run.sum(mb, lb, mb, 0.0f);
+    const float fo = run.stand(mb, vnow), fb = run.factor(mb, vnow);
+#pragma unroll
+    for (int t = 0; t < DT; t++) {
+      const v4i acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap, c.vf[t], v4i{0, 0, 0, 0}, 0, 0, 0);
+      o[t] = here(fmaf(undigits(acc), fb, o[t] * fo));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (kNext) c.values(v8, ahead);
+    if (kNext) walk.step(id);
+  };
+  while (walk.more()) block(std::true_type{});
+  if (walk.j < stop) block(std::false_type{});
+
+  // the wavefronts' sums
+  const float sum = sum16(run.l);
+  int e;
+  const float g = run.last(sum, &e);
+  e -= 30;  // of the weights' whole numbers
+#pragma unroll
+  for (int t = 0; t < DT; t++) lo[wave][quad][16 * t + col] = __builtin_amdgcn_ldexpf(o[t] * g, e);
+  if (col == 0) {
+    lm[wave][quad] = run.m;
+    ll[wave][quad] = sum;
+  }
+  __syncthreads();
+  const int r = threadIdx.x >> 6;
+  if (r >= rows) return;
+  float top = -INFINITY, total = 0.0f, wt[kFewWaves];
+#pragma unroll
+  for (int w = 0; w < kFewWaves; w++) top = fmaxf(top, lm[w][r]);
+#pragma unroll
+  for (int w = 0; w < kFewWaves; w++) {
+    wt[w] = ll[w][r] == 0.0f ? 0.0f : ll[w][r] * ex2(lm[w][r] - or0(top));
+    total += wt[w];
+  }
+  const Place8 to(out, lse, parts, a, part, (size_t)s.q0 + r / G, hk * G + r % G);
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  for (int d = lane; d < a.HS; d += kWave) {
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; w++) y = fmaf(wt[w] * inv, lo[w][r][d], y);
+    to.o[d] = y;
+  }
+  if (lane == 0) to.put(top, total);
+}
+
+// x of the lanes that hold the same row in the four quarters of a wavefront, combined.
+__device__ __forceinline__ float quarters_max(float x) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_max(fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
+}
+
+// Up to 16 RW rows: drafts, large groups, an observation window (in `groups` of them). The same products transposed, with an operand per digit:
+// a lane holds 16 scores of one row, and its weights are the second product's operand as they stand, for a column of
+// the values' codes has its keys in the order in which the lanes hold them. A wavefront has 16 rows; with RW 2 two of them take the
+// same blocks, which the second finds in a cache.
+template <int DT, int RW>
+__global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out, float *lse, const float *q, const int8_t *k8,
+                                                                    const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
+                                                                    Parts8 parts, unsigned pairs, unsigned groups, int *word) {
+  constexpr int KS = (DT + 3) / 4, kStride = 16 * DT + 4, KW = kFewWaves / RW;
+  __shared__ alignas(16) float lo[kFewWaves][16 * kStride];
+  __shared__ float lm[kFewWaves][16], ll[kFewWaves][16];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const unsigned pair = turned(blockIdx.x, blockIdx.x / pairs, pairs), group = blockIdx.x / pairs % groups;
+  const int part = blockIdx.x / pairs / groups;
+  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
+  const Seq8 s = sequence8(a, b, hk == 0 && part == 0 && group == 0, word, UGK_IDS_CACHE8_ATTENTION);
+  const int rows = s.Lq * G, row0 = group * 16 * RW;
+  if (row0 >= rows) return;
+  const int end = s.seen((min(row0 + 16 * RW, rows) - 1) / G, a.causal), nb = (end + kKeys - 1) / kKeys;
+  const int first = part * parts.chunk, stop = min(first + parts.chunk, nb);
+  if (part > 0 && first >= nb) return;  // no row of the workgroup has this part
+  const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
+
+  Codes<DT> c(padded(a.HS), lane);
+  Walk walk(a, b, first + wave % KW, stop, KW, word);
+  float kscale = 0.0f, vscale = 0.0f;
+  if (walk.j < stop) {
+    const size_t at = block_head(walk.id, a.NKV, hk);
+    c.keys(k8, at);
+    c.values(v8, at);
+    kscale = ks[at];
+    vscale = vs[at];
+  }
+
+  v4i aq[KS][4];
+  const int mine = row0 + 16 * (wave / KW) + col, lim = mine < rows ? s.seen(mine / G, a.causal) : end;
+  int ex;
+  bool nan;
+  Running run;
+  float o[DT][4];
+  {
+    const int rr = min(mine, rows - 1);
+    const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (size_t)(hk * G + rr % G) * a.HS;
+    float x[KS][16];
+    uint32_t most = 0;
+#pragma unroll
+    for (int st = 0; st < KS; st++) most = max(most, load_q(p, 64 * st + 16 * quad, a, x[st]));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+    nan = most >= kInfBits;
+    ex = (int)(most >> 23) - 127 - 29;
 #pragma unroll
     for (int st = 0; st < KS; st++)
 #pragma unroll
-      for (int kt = 0; kt < 4; kt++)
-        kf[st][kt] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(kb + koff[st] + kt * 16 * HP));
+      for (int d = 0; d < 16; d += 4) {
+        uint32_t y[4];
 #pragma unroll
-    for (int t = 0; t < DT; t++) vf[t] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(vb + voff[t]));
-    const float kscale = ks[at], vscale = vs[at];
-    if (j + kFewWaves < stop) next = block_of(a, b, j + kFewWaves, word, UGK_IDS_CACHE8_ATTENTION);
-    const bool masked = !there || (j + 1) * kKeys > least;
+        for (int r = 0; r < 4; r++) y[r] = digits((int)rintf(__builtin_amdgcn_ldexpf(nan ? 0.0f : x[st][d + r], -ex)));
+        const v4i t = turn4(y[0], y[1], y[2], y[3]);
 #pragma unroll
-    for (int rt = 0; rt < R; rt++) {
-      if (R > 1) __builtin_amdgcn_sched_barrier(0);  // row by row: the registers hold one operand's scores
-      const float fac = nan[rt] ? NAN : score_factor(f, kscale, ex[rt]);
-      float p[4], mb = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < 4; kt++) {
-        v4i acc = {0, 0, 0, 0};
-#pragma unroll
-        for (int st = 0; st < KS; st++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[rt][st], kf[st][kt], acc, 0, 0, 0);
-        p[kt] = undigits(acc) * fac;
-        if (masked && (!there || j * kKeys + kt * 16 + col >= lim[rt])) p[kt] = -INFINITY;
-        mb = fmaxf(mb, p[kt]);
+        for (int r = 0; r < 4; r++) aq[st][r][d / 4] = t[r];
       }
-      mb = max16(mb);
-      const float zero = or0(mb);
-      uint32_t y[4];
-      float lb = 0.0f;
 #pragma unroll
-      for (int kt = 0; kt < 4; kt++) {
-        p[kt] = ex2(p[kt] - zero);
-        lb += p[kt];
-        y[kt] = digits((int)rintf(p[kt] * 0x1p30f));
-      }
-      // the four keys' digits side by side: a word per digit
-      const uint32_t t0 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), t1 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u);
-      const uint32_t t2 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u), t3 = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
-      uint32_t *w = mylp + 4 * quad * kStride + col;
-      w[0] = __builtin_amdgcn_perm(t2, t0, 0x05040100u);
-      w[kStride] = __builtin_amdgcn_perm(t2, t0, 0x07060302u);
-      w[2 * kStride] = __builtin_amdgcn_perm(t3, t1, 0x05040100u);
-      w[3 * kStride] = __builtin_amdgcn_perm(t3, t1, 0x07060302u);
-      __builtin_amdgcn_wave_barrier();
-      const v4i ap = *reinterpret_cast<const v4i *>(mylp + col * kStride + 4 * quad);
-      __builtin_amdgcn_wave_barrier();
-      if (parts.block) {
-        const int mine = base_row + 4 * rt + quad;
-        const float sum = sum16(lb);
-        if (col == 0 && mine < rows)
-          parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + mine) * a.ld_table + j] = make_float2(mb, sum);
-      }
-      const float2 k = run[rt].add(mb, lb, vscale);
+    for (int t = 0; t < DT; t++)
 #pragma unroll
-      for (int t = 0; t < DT; t++) {
-        const v4i acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap, vf[t], v4i{0, 0, 0, 0}, 0, 0, 0);
-        o[rt][t] = fmaf(undigits(acc), k.y, o[rt][t] * k.x);
-      }
-    }
+      for (int r = 0; r < 4; r++) o[t][r] = 0.0f;
   }
+  const int least = s.seen(row0 / G, a.causal);
 
-  // the wavefronts' sums, four rows at a time
+  const auto block = [&](auto next) {  // next: another block follows
+    constexpr bool kNext = decltype(next)::value;
+    const int id = kNext ? walk.ahead(a, b, word) : 0;
+    const size_t ahead = block_head(id, a.NKV, hk);
+    const bool masked = !walk.there() || (walk.j + 1) * kKeys > least;
+    const int seen = walk.there() ? lim - walk.j * kKeys - 4 * quad : 0;  // of this block's keys from the lane's first on
+    const float vnow = exponent(vscale);
+    const float fac = nan ? NAN : score_factor(f, kscale, ex);
+    float p[4][4], mb = -INFINITY;
 #pragma unroll
-  for (int rt = 0; rt < R; rt++) {
-    const float sum = sum16(run[rt].l);
-    int e;
-    const float g = run[rt].last(sum, &e);
-    e -= 30;  // of the weights' whole numbers
-    if (rt) __syncthreads();
+    for (int kt = 0; kt < 4; kt++) {
+      __builtin_amdgcn_sched_barrier(0);  // tile by tile: the registers hold one tile's digits
+      v4i acc[4];
 #pragma unroll
-    for (int t = 0; t < DT; t++) lo[wave][quad][16 * t + col] = __builtin_amdgcn_ldexpf(o[rt][t] * g, e);
-    if (col == 0) {
-      lm[wave][quad] = run[rt].m;
-      ll[wave][quad] = sum;
+      for (int d = 0; d < 4; d++) {
+        acc[d] = v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int st = 0; st < KS; st++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.kf[st][kt], aq[st][d], acc[d], 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[kt][r] = here(undigits(v4i{acc[0][r], acc[1][r], acc[2][r], acc[3][r]}));
+      }
     }
-    __syncthreads();
-    const int r = threadIdx.x >> 6, mine = base_row + 4 * rt + r;
-    if (mine >= rows) continue;
-    float top = -INFINITY, total = 0.0f, wt[kFewWaves];
+    if (masked) {
+      const int n = here(seen);
 #pragma unroll
-    for (int w = 0; w < kFewWaves; w++) top = fmaxf(top, lm[w][r]);
+      for (int kt = 0; kt < 4; kt++)
 #pragma unroll
-    for (int w = 0; w < kFewWaves; w++) {
-      wt[w] = ll[w][r] == 0.0f ? 0.0f : ll[w][r] * ex2(lm[w][r] - or0(top));
+        for (int r = 0; r < 4; r++) p[kt][r] = kt * 16 + r < n ? p[kt][r] : -INFINITY;
+    }
+#pragma unroll
+    for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) mb = fmaxf(mb, p[kt][r]);
+    __builtin_amdgcn_sched_barrier(0);  // into the registers that the products have read
+    if (kNext) {
+      c.keys(k8, ahead);
+      kscale = ks[ahead];
+      vscale = vs[ahead];
+    }
+    mb = top_score(quarters_max(mb), fac);
+    const float less = less_top(mb, 30.0f);
+    float lb = 0.0f;
+    v4i bp[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      uint32_t y[4];
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++) {
+        const float x = ex2(fmaf(p[kt][r], fac, less));
+        lb += x;
+        y[kt] = digits((int)x);
+      }
+      const v4i t = turn4(y[0], y[1], y[2], y[3]);
+#pragma unroll
+      for (int d = 0; d < 4; d++) bp[d][r] = t[d];
+    }
+    lb *= 0x1p-30f;
+    if (parts.block) {
+      const float sum = quarters_sum(lb);
+      if (quad == 0 && mine < rows)
+        parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + mine) * a.ld_table + walk.j] = make_float2(mb, sum);
+    }
+    run.sum(mb, lb, mb, 0.0f);
+    const float fo = run.stand(mb, vnow), fb = run.factor(mb, vnow);
+#pragma unroll
+    for (int t = 0; t < DT; t++) {
+      if (t % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+      v4i acc[4];
+#pragma unroll
+      for (int d = 0; d < 4; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.vf[t], bp[d], v4i{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        o[t][r] = here(fmaf(undigits(v4i{acc[0][r], acc[1][r], acc[2][r], acc[3][r]}), fb, o[t][r] * fo));
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (kNext) c.values(v8, ahead);
+    if (kNext) walk.step(id);
+  };
+  while (walk.more()) block(std::true_type{});
+  if (walk.j < stop) block(std::false_type{});
+
+  // the sums of the wavefronts that share rows
+  const float sum = quarters_sum(run.l);
+  int e;
+  const float g = run.last(sum, &e);
+  e -= 30;  // of the weights' whole numbers
+#pragma unroll
+  for (int t = 0; t < DT; t++)
+    *reinterpret_cast<float4 *>(&lo[wave][col * kStride + 16 * t + 4 * quad]) =
+        make_float4(__builtin_amdgcn_ldexpf(o[t][0] * g, e), __builtin_amdgcn_ldexpf(o[t][1] * g, e),
+                    __builtin_amdgcn_ldexpf(o[t][2] * g, e), __builtin_amdgcn_ldexpf(o[t][3] * g, e));
+  if (quad == 0) {
+    lm[wave][col] = run.m;
+    ll[wave][col] = sum;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int x = wave; x < 16 * RW; x += kFewWaves) {
+    const int r = x & 15, w0 = x / 16 * KW, row = row0 + x;
+    if (row >= rows) break;
+    float top = -INFINITY, total = 0.0f, wt[KW];
+#pragma unroll
+    for (int w = 0; w < KW; w++) top = fmaxf(top, lm[w0 + w][r]);
+#pragma unroll
+    for (int w = 0; w < KW; w++) {
+      wt[w] = ll[w0 + w][r] == 0.0f ? 0.0f : ll[w0 + w][r] * ex2(lm[w0 + w][r] - or0(top));
       total += wt[w];
     }
-    const int i = mine / G, h = hk * G + mine % G;
-    const size_t prow = (((size_t)part * a.nseq + b) * a.max_q + i) * a.NH + h, grow = (size_t)s.q0 + i;
-    float *po = parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + h * a.HS;
+    const Place8 to(out, lse, parts, a, part, (size_t)s.q0 + row / G, hk * G + row % G);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     for (int d = lane; d < a.HS; d += kWave) {
       float y = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kFewWaves; w++) y = fmaf(wt[w] * inv, lo[w][r][d], y);
-      po[d] = y;
+      for (int w = 0; w < KW; w++) y = fmaf(wt[w] * inv, lo[w0 + w][r * kStride + d], y);
+      to.o[d] = y;
     }
-    if (lane) continue;
-    if (parts.o) {
-      parts.m[prow] = top;
-      parts.l[prow] = total;
-    } else if (lse) {
-      lse[grow * a.NH + h] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn28;
-    }
+    if (lane == 0) to.put(top, total);
   }
 }
 
 // The parts of a split key axis joined, one wavefront per row and head, in the parts' order.
 __global__ __launch_bounds__(kBlock) void k_cache8_join(float *out, float *lse, Parts8 parts, ugk_cache8 a) {
-  const size_t at = (size_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6), per = (size_t)a.nseq * a.max_q * a.NH;
-  if (at >= per) return;
-  const int lane = threadIdx.x & (kWave - 1), h = at % a.NH, i = at / a.NH % a.max_q, b = at / a.NH / a.max_q;
+  const size_t nth = (size_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6), per = (size_t)a.rows_q * a.NH;
+  if (nth >= (size_t)a.nseq * a.max_q * a.NH) return;
+  const int lane = threadIdx.x & (kWave - 1), h = nth % a.NH, i = nth / a.NH % a.max_q, b = nth / a.NH / a.max_q;
   const Seq8 s = sequence8(a, b, false, nullptr, 0);
   if (i >= s.Lq) return;
+  const size_t g = (size_t)s.q0 + i, at = g * a.NH + h;
+  const int splits = max(1, (s.seen(i, a.causal) + kKeys * parts.chunk - 1) / (kKeys * parts.chunk));
   float m = -INFINITY;
-  for (int x = lane; x < parts.splits; x += kWave) m = fmaxf(m, parts.m[x * per + at]);
+  for (int x = lane; x < splits; x += kWave) m = fmaxf(m, parts.m[x * per + at]);
 #pragma unroll
   for (int x = 32; x; x /= 2) m = fmaxf(m, __shfl_xor(m, x));
   float o0 = 0.0f, o1 = 0.0f, l = 0.0f;
   const int d0 = min(lane, a.HS - 1), d1 = min(lane + kWave, a.HS - 1);
-  for (int x0 = 0; x0 < parts.splits; x0 += kWave) {
-    const int x = x0 + lane, n = min(kWave, parts.splits - x0);
-    const float lx = x < parts.splits ? parts.l[x * per + at] : 0.0f;
+  for (int x0 = 0; x0 < splits; x0 += kWave) {
+    const int x = x0 + lane, n = min(kWave, splits - x0);
+    const float lx = x < splits ? parts.l[x * per + at] : 0.0f;
     const float w = lx == 0.0f ? 0.0f : lx * ex2(parts.m[x * per + at] - or0(m));  // 0: a part without a key of this row, its o is 0
     l += wave_sum(w);
-    for (int t = 0; t < n; t++) {
-      const float wt = __shfl(w, t), *o = parts.o + ((x0 + t) * per + at) * a.HS;
-      o0 = fmaf(wt, o[d0], o0);
-      o1 = fmaf(wt, o[d1], o1);
+    for (int t = 0; t < n; t += 8) {  // eight parts' loads at a time
+      float y0[8], y1[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float *o = parts.o + ((x0 + min(t + u, n - 1)) * per + at) * a.HS;
+        y0[u] = o[d0];
+        y1[u] = o[d1];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float wt = __shfl(w, (t + u) & (kWave - 1));
+        o0 = t + u < n ? fmaf(wt, y0[u], o0) : o0;
+        o1 = t + u < n ? fmaf(wt, y1[u], o1) : o1;
+      }
     }
   }
   const bool none = l == 0.0f;
   const float inv = none ? 1.0f : 1.0f / l;
-  const size_t g = (size_t)s.q0 + i;
   float *po = out + g * a.ldo + h * a.HS;
   if (lane < a.HS) po[lane] = o0 * inv;
   if (lane + kWave < a.HS) po[lane + kWave] = o1 * inv;
@@ -566,7 +899,7 @@ __global__ __launch_bounds__(kBlock) void k_cache8_weights(float *weight, Parts8
       const int hk = x / rows, rr = x % rows, i = rr / G, h = hk * G + rr % G;
       if (j * kKeys >= s.seen(i, a.causal)) continue;
       const float2 p = parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + rr) * a.ld_table + j];
-      const float2 all = parts.stat[((size_t)b * a.max_q + i) * a.NH + h];
+      const float2 all = parts.stat[((size_t)s.q0 + i) * a.NH + h];
       if (p.y != 0.0f) sum += p.y * ex2(p.x - all.x) / all.y;
     }
   }
@@ -596,28 +929,30 @@ __device__ __forceinline__ v2u halves4(uint32_t w) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, float *lse, const float *q, const int8_t *k8,
+__global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(float *out, float *lse, const float *q, const int8_t *k8,
                                                                  const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
                                                                  Parts8 parts, unsigned pairs, unsigned tiles, int *word) {
-  constexpr int KSTR = 16 * DT + 8, VSTR = kKeys + 8, D32 = DT / 2, NL = DT / 4;
+  constexpr int KSTR = 16 * DT + 8, VSTR = kKeys + 8, D32 = DT / 2, NL = (DT + 3) / 4;
   __shared__ alignas(16) _Float16 kl[2][kKeys * KSTR];
   __shared__ alignas(16) _Float16 vl[2][16 * DT * VSTR];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-  const unsigned pair = blockIdx.x % pairs;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const unsigned pair = turned(blockIdx.x, blockIdx.x / pairs + blockIdx.y, pairs);
   const int tile = (int)(tiles - 1 - blockIdx.x / pairs), part = blockIdx.y;  // the longest first
   const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV, HP = padded(a.HS), CH = HP / 16;
   const Seq8 s = sequence8(a, b, hk == 0 && part == 0 && tile == 0, word, UGK_IDS_CACHE8_ATTENTION);
   const int rows = s.Lq * G, row0 = tile * kTileRows8;
   if (row0 >= rows) return;
   const int nb = (s.seen((min(row0 + kTileRows8, rows) - 1) / G, a.causal) + kKeys - 1) / kKeys;
-  const int first = (int)((long long)nb * part / parts.splits), stop = (int)((long long)nb * (part + 1) / parts.splits);
+  const int first = part * parts.chunk, stop = min(first + parts.chunk, nb);
+  if (part > 0 && first >= nb) return;  // no row of the workgroup has this part
   const int mine = row0 + 32 * wave + col, safe = min(mine, rows - 1), i = safe / G, h = hk * G + safe % G;
   const int lim = s.seen(i, a.causal);
   // what the wavefront's first and last rows see
   const int wave_first = min(row0 + 32 * wave, rows - 1), wave_last = min(row0 + 32 * wave + 31, rows - 1);
   const int least = s.seen(wave_first / G, a.causal), most_seen = s.seen(wave_last / G, a.causal);
   const bool idle = row0 + 32 * wave >= rows;
-  const float f = a.scale * kLog2e8;
+  const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
 
   v8h qh[DT], ql[DT];
   int e;
@@ -627,13 +962,7 @@ __global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, fl
     float x[DT][8];
     uint32_t most = 0;
 #pragma unroll
-    for (int st = 0; st < DT; st++)
-#pragma unroll
-      for (int d = 0; d < 8; d++) {
-        const int at = 16 * st + 8 * half + d;
-        x[st][d] = at < a.HS ? p[at] : 0.0f;
-        most = max(most, abs_bits(x[st][d]));
-      }
+    for (int st = 0; st < DT; st++) most = max(most, load_q(p, 16 * st + 8 * half, a, x[st]));
     most = half_max_bits(most);
     nan = most >= kInfBits;
     e = (int)(most >> 23) - 126 - 15;  // below 2^15 2^e
@@ -661,10 +990,12 @@ __global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, fl
   v4u kr[NL], vr[NL];
   float kscale = 0.0f, vscale = 0.0f;
   bool there = true;
+  int next = first < stop ? table_at(a, b, first) : 0;
   const auto fetch = [&](int j) {
-    const int id = block_of(a, b, j, word, UGK_IDS_CACHE8_ATTENTION);
+    const int id = checked_block(a, __builtin_amdgcn_readfirstlane(next), word, UGK_IDS_CACHE8_ATTENTION);
+    next = table_at(a, b, min(j + 1, stop - 1));
     there = id >= 0;
-    const size_t at = (size_t)(there ? id : 0) * a.NKV + hk;
+    const size_t at = block_head(id, a.NKV, hk);
 #pragma unroll
     for (int n = 0; n < NL; n++) {
       const int w = threadIdx.x + n * kTileThreads8;
@@ -676,6 +1007,10 @@ __global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, fl
     kscale = ks[at];
     vscale = vs[at];
   };
+  if (CH < DT) {  // behind the keys' rows q is 0, and what is there has to be a number
+    for (int x = threadIdx.x; x < 2 * kKeys * KSTR / 2; x += kTileThreads8) reinterpret_cast<uint32_t *>(kl[0])[x] = 0u;
+    __syncthreads();
+  }
   if (first < stop) fetch(first);
   for (int j = first; j < stop; j++) {
     _Float16 *kt = kl[(j - first) & 1], *vt = vl[(j - first) & 1];
@@ -694,8 +1029,8 @@ __global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, fl
       *reinterpret_cast<v2u *>(vt + vdst[n] + 32) = halves4(__builtin_amdgcn_perm(t3, t1, 0x05040100u));
       *reinterpret_cast<v2u *>(vt + vdst[n] + 48) = halves4(__builtin_amdgcn_perm(t3, t1, 0x07060302u));
     }
-    const float fac = nan ? NAN : score_factor(f, kscale, e), vnow = vscale;
-    const bool here = there;
+    const float fac = nan ? NAN : score_factor(f, kscale, e), vnow = exponent(vscale);
+    const bool held = there;
     __syncthreads();
     if (j + 1 < stop) fetch(j + 1);
     if (idle || j * kKeys >= most_seen) continue;
@@ -705,59 +1040,70 @@ __global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, fl
       sc[x] = v16f{};
 #pragma unroll
       for (int st = 0; st < DT; st++) {
-        if (st >= CH) continue;
         const v8h kf = frag(kt + (32 * x + col) * KSTR + 16 * st + 8 * half);
         sc[x] = mfma(kf, ql[st], sc[x]);
         sc[x] = mfma(kf, qh[st], sc[x]);
       }
     }
     float mb = -INFINITY;
-    const bool masked = !here || (j + 1) * kKeys > least;
+    const bool masked = !held || (j + 1) * kKeys > least;
+    const int seen = held ? lim - j * kKeys - 4 * half : 0;  // of this block's keys from the lane's first on
+    if (masked) {
+      const int n = here(seen);
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) sc[x][r] = 32 * x + 8 * (r / 4) + r % 4 < n ? sc[x][r] : -INFINITY;
+    }
 #pragma unroll
     for (int x = 0; x < 2; x++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        float y = sc[x][r] * fac;
-        if (masked && (!here || j * kKeys + 32 * x + 8 * (r / 4) + 4 * half + r % 4 >= lim)) y = -INFINITY;
-        sc[x][r] = y;
-        mb = fmaxf(mb, y);
-      }
-    mb = half_max(mb);
-    const float zero = or0(mb);
+      for (int r = 0; r < 16; r++) mb = fmaxf(mb, sc[x][r]);
+    mb = top_score(half_max(mb), fac);
+    const float fo = run.stand(mb, vnow);
+    if (__any(fo != 1.0f)) {
+      const float x = here(fo);
+#pragma unroll
+      for (int t = 0; t < D32; t++) o[t] *= x;
+    }
+    // The weights stand on what the output's sum stands on, times 2^14: the products add up in its registers.
+    const float up = 14.0f + (vnow - run.e), less = mb == INFINITY ? NAN : up - or0(run.mo);
     float lb = 0.0f;
-    v8h ph[4], pl[4];
+    const bool apart = __any(run.e - vnow > 64.0f);  // weights that the row's sum needs may vanish next to another block's values
+    if (apart) {
+      const float own = here(less_top(mb, 0.0f));  // on the block's own largest
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) lb += ex2(fmaf(sc[x][r], fac, own));
+      run.sum(mb, lb, mb, 0.0f);
+    }
 #pragma unroll
     for (int g = 0; g < 4; g++) {
       float p[8];
+      v8h ph, pl;
 #pragma unroll
       for (int r = 0; r < 8; r++) {
-        p[r] = ex2(sc[g / 2][8 * (g % 2) + r] - zero);
+        p[r] = ex2(fmaf(sc[g / 2][8 * (g % 2) + r], fac, less));
         lb += p[r];
       }
-      split8(p, 0x1p14f, ph[g], pl[g]);
-    }
-    const float2 k = run.add(mb, lb, vnow);
-    const float ky = k.y * 0x1p-14f;
+      split8(p, ph, pl);
 #pragma unroll
-    for (int t = 0; t < D32; t++) {
-      if (2 * t >= CH) continue;
-      v16f acc = v16f{};
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
+      for (int t = 0; t < D32; t++) {
         const v8h vf = frag(vt + (32 * t + col) * VSTR + 16 * g + 8 * half);
-        acc = mfma(vf, pl[g], acc);
-        acc = mfma(vf, ph[g], acc);
+        o[t] = mfma(vf, pl, o[t]);
+        o[t] = mfma(vf, ph, o[t]);
       }
-#pragma unroll
-      for (int r = 0; r < 16; r++) o[t][r] = fmaf(acc[r], ky, o[t][r] * k.x);
     }
+    if (!apart) run.sum(mb, lb, run.mo, up);
   }
   if (mine >= rows) return;
   const float sum = half_sum(run.l);
   int p;
   const float g = run.last(sum, &p);
-  const size_t prow = (((size_t)part * a.nseq + b) * a.max_q + i) * a.NH + h, grow = (size_t)s.q0 + i;
-  float *po = parts.o ? parts.o + prow * a.HS : out + grow * a.ldo + (size_t)h * a.HS;
+  p -= 14;  // of the weights
+  const Place8 to(out, lse, parts, a, part, (size_t)s.q0 + i, h);
+  float *po = to.o;
 #pragma unroll
   for (int t = 0; t < D32; t++)
 #pragma unroll
@@ -777,13 +1123,7 @@ __global__ __launch_bounds__(kTileThreads8, 2) void k_cache8_tile(float *out, fl
         if (nd > 2) po[d + 2] = y.z;
       }
     }
-  if (half) return;
-  if (parts.o) {
-    parts.m[prow] = run.m;
-    parts.l[prow] = sum;
-  } else if (lse) {
-    lse[grow * a.NH + h] = sum == 0.0f ? -INFINITY : (run.m + __builtin_amdgcn_logf(sum)) * kLn28;
-  }
+  if (half == 0) to.put(run.m, sum);
 }
 
 // ---- eviction ----------------------------------------------------------------------
@@ -919,43 +1259,44 @@ int cu_count8() {
   return n;
 }
 
-// How an attention call is cut: operands of four rows per workgroup of k_cache8_few (0: k_cache8_tile) and groups of them, tiles
-// of rows, parts of the key axis.
+// How an attention call is cut: k_cache8_few (few 1), k_cache8_some with 16 or 32 rows per workgroup (4, 8) in so many groups, or
+// tiles of rows of k_cache8_tile (0); parts of the key axis of `chunk` blocks.
 struct Plan8 {
-  int few, groups, tiles, splits;
+  int few, groups, tiles, splits, chunk;
 };
 constexpr int kFewRows8 = 32;
-constexpr size_t kMaxParts8 = 1 << 15;  // rows of a head that the parts hold at most
 
 Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   Plan8 p{};
-  const long long pairs = (long long)a.nseq * a.NKV, rows = (long long)a.max_q * (a.NH / a.NKV);
-  const long long prow = (long long)a.nseq * a.max_q * a.NH, blocks = (a.max_k + kKeys - 1) / kKeys;
-  long long want;
+  const long long pairs = (long long)a.nseq * a.NKV, G = a.NH / a.NKV, rows = a.max_q * G, blocks = (a.max_k + kKeys - 1) / kKeys;
+  long long chunk;
   if (rows <= kFewRows8 || weigh) {
-    p.few = rows <= 4 ? 1 : rows <= 8 ? 2 : rows <= 16 ? 4 : 8;
+    p.few = rows <= 4 ? 1 : rows <= 16 ? 4 : 8;
     p.groups = (int)((rows + 4 * p.few - 1) / (4 * p.few));
-    want = max(8LL * cu_count8() / max(pairs * p.groups, 1LL), (blocks + 15) / 16);
-    want = min(want, blocks / 4);
+    chunk = blocks * pairs * p.groups / ((p.few == 1 ? 4 : 2) * cu_count8());
+    chunk = max(min(chunk, (long long)32), (long long)4);
   } else {
     p.tiles = (int)((rows + kTileRows8 - 1) / kTileRows8);
-    want = 2LL * cu_count8() / max(pairs * p.tiles, 1LL);
-    want = min(want, blocks / 4);
+    const long long filled = min(pairs * p.tiles, (a.rows_q * G / kTileRows8 + a.nseq) * a.NKV);
+    chunk = filled >= 2 * cu_count8() ? blocks : max(blocks * filled / (8 * cu_count8()), (long long)8);
   }
-  want = min(want, (long long)kMaxParts8 / max(prow, 1LL));
-  p.splits = (int)max(want, 1LL);
+  // what a workspace of the same rows and heads has for the fp32 attention
+  const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / ((a.HS + 2) * sizeof(float));
+  const long long fit = max((long long)(most / max((size_t)a.rows_q * a.NH, (size_t)1)), 1LL);
+  p.chunk = (int)max(max(chunk, (blocks + fit - 1) / fit), 1LL);
+  p.splits = (int)max((blocks + p.chunk - 1) / p.chunk, 1LL);
   return p;
 }
 bool has_parts(const Plan8 &p, bool weigh) { return p.splits > 1 || weigh; }
-size_t parts_rows(const ugk_cache8 &a, const Plan8 &p) { return (size_t)p.splits * a.nseq * a.max_q * a.NH; }
+size_t parts_rows(const ugk_cache8 &a, const Plan8 &p) { return (size_t)p.splits * a.rows_q * a.NH; }
 size_t even(size_t n) { return (n + 1) / 2 * 2; }
 }  // namespace
 
 size_t cache8_attention_bytes(const ugk_cache8 &a, bool weigh) {
   const Plan8 p = plan8(a, weigh);
   if (!has_parts(p, weigh)) return 0;
-  const size_t rows = (size_t)a.nseq * a.max_q * a.NH;
-  return (even(parts_rows(a, p) * (a.HS + 2)) + (weigh ? 2 * rows * (1 + (size_t)a.ld_table) : 0)) * sizeof(float);
+  const size_t stat = (size_t)a.rows_q * a.NH, block = (size_t)a.nseq * a.max_q * a.NH * a.ld_table;
+  return (even(parts_rows(a, p) * (a.HS + 2)) + (weigh ? 2 * (stat + block) : 0)) * sizeof(float);
 }
 
 int launch_cache8_attention(float *out, float *lse, const float *q, const void *k8, const float *ks, const void *v8,
@@ -963,36 +1304,40 @@ int launch_cache8_attention(float *out, float *lse, const float *q, const void *
   const Plan8 p = plan8(a, weight);
   Parts8 parts{};
   parts.splits = p.splits;
+  parts.chunk = p.chunk;
   if (has_parts(p, weight)) {
     parts.m = mem;
     parts.l = parts.m + parts_rows(a, p);
     parts.o = parts.l + parts_rows(a, p);
     if (weight) {
       parts.stat = reinterpret_cast<float2 *>(mem + even(parts_rows(a, p) * (a.HS + 2)));
-      parts.block = parts.stat + (size_t)a.nseq * a.max_q * a.NH;
+      parts.block = parts.stat + (size_t)a.rows_q * a.NH;
     }
   }
   const unsigned pairs = (unsigned)a.nseq * a.NKV;
+  const int8_t *kc = static_cast<const int8_t *>(k8), *vc = static_cast<const int8_t *>(v8);
   const auto few = [&](auto kernel) {
-    launch(kernel, dim3(pairs * p.groups * p.splits), dim3(kFewWaves * kWave), 0, out, lse, q, (const int8_t *)k8, ks, (const int8_t *)v8,
-           vs, a, parts, pairs, (unsigned)p.groups, word);
+    launch(kernel, dim3(pairs * p.splits), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, word);
+  };
+  const auto some = [&](auto kernel) {
+    launch(kernel, dim3(pairs * p.groups * p.splits), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs,
+           (unsigned)p.groups, word);
   };
   const auto tile = [&](auto kernel) {
-    launch(kernel, dim3(pairs * p.tiles, p.splits), dim3(kTileThreads8), 0, out, lse, q, (const int8_t *)k8, ks, (const int8_t *)v8, vs, a,
-           parts, pairs, (unsigned)p.tiles, word);
+    launch(kernel, dim3(pairs * p.tiles, p.splits), dim3(kTileThreads8), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, (unsigned)p.tiles,
+           word);
   };
-#define UGK_FEW8(r)                                                                                                    \
-  case r:                                                                                                              \
-    if (a.HS <= 32) few(k_cache8_few<2, r>);                                                                           \
-    else if (a.HS <= 64) few(k_cache8_few<4, r>);                                                                      \
-    else if (a.HS <= 96) few(k_cache8_few<6, r>);                                                                      \
-    else few(k_cache8_few<8, r>);                                                                                      \
-    break;
+  const int d = a.HS <= 32 ? 2 : a.HS <= 64 ? 4 : a.HS <= 96 ? 6 : 8;
   switch (p.few) {
-    UGK_FEW8(1) UGK_FEW8(2) UGK_FEW8(4) UGK_FEW8(8)
-    default: a.HS <= 64 ? tile(k_cache8_tile<4>) : tile(k_cache8_tile<8>);
+    case 1: d == 2 ? few(k_cache8_few<2>) : d == 4 ? few(k_cache8_few<4>) : d == 6 ? few(k_cache8_few<6>) : few(k_cache8_few<8>); break;
+    case 4:
+      d == 2 ? some(k_cache8_some<2, 1>) : d == 4 ? some(k_cache8_some<4, 1>) : d == 6 ? some(k_cache8_some<6, 1>) : some(k_cache8_some<8, 1>);
+      break;
+    case 8:
+      d == 2 ? some(k_cache8_some<2, 2>) : d == 4 ? some(k_cache8_some<4, 2>) : d == 6 ? some(k_cache8_some<6, 2>) : some(k_cache8_some<8, 2>);
+      break;
+    default: d == 2 ? tile(k_cache8_tile<2>) : d == 4 ? tile(k_cache8_tile<4>) : d == 6 ? tile(k_cache8_tile<6>) : tile(k_cache8_tile<8>);
   }
-#undef UGK_FEW8
   if (int e = check_launch("cache8_attention")) return e;
   if (parts.o) {
     launch(k_cache8_join, dim3(grid_for((size_t)a.nseq * a.max_q * a.NH, kBlock / kWave)), dim3(kBlock), 0, out, lse, parts, a);

@@ -5,134 +5,283 @@
 // that does not, the token comes from max(p_i - q_i, 0), and behind all drafts from p_n: the tokens are then distributed as
 // the target's own. The comparison and the cumulative sums are in 64 bits: the products of two floats are exact there, and a sum of a
 // vocabulary of floats is off by 2^-35 of itself at most, so that the token hardly depends on the order of additions.
+#include <climits>
+
 #include "ugk_internal.h"
 
 namespace ugk {
 namespace {
 
-constexpr int kDraftThreads = 1024, kDraftWaves = kDraftThreads / kWave;
+constexpr int kDraftThreads = 1024, kDraftWaves = kDraftThreads / kWave, kSumThreads = 256;
+constexpr int kStep = 4 * kDraftThreads;  // floats that a workgroup takes at a time
+constexpr int kMaxSegs = 1024;            // segments of a row
 
 __device__ __forceinline__ double wave_sum64(double x) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
   return x;
 }
-
-// What token v of a row may be drawn with. less: the drafts' probabilities of the row, or null; gone: the token that
-// is not drawn (its draft was certain), or -1.
-__device__ __forceinline__ double mass(const float *p, const float *less, int gone, int v) {
-  const double x = less ? (double)p[v] - (double)less[v] : (double)p[v];
-  return v != gone && x > 0.0 && x <= 3.402823466e38 ? x : 0.0;
-}
-
-// The token at the fraction u of the cumulative sum of [0, V), or -1 where the sum is 0: the sixteen wavefronts sum a
-// sixteenth each, then a sixteenth of the one in which the sum passes, then one wavefront walks that 256th.
-__device__ int draw(const float *p, const float *less, int gone, int V, double u, double *lds) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  int begin = 0, end = V;
-  double target = 0.0;
-  bool any = true;
-#pragma unroll 1
-  for (int level = 0; level < 2; level++) {
-    const int per = (end - begin + kDraftWaves - 1) / kDraftWaves;
-    const int from = min(begin + wave * per, end), to = min(from + per, end);
-    double s0 = 0.0, s1 = 0.0, s2 = 0.0, s3 = 0.0;
-    int v = from + lane;
-    for (; v + 3 * kWave < to; v += 4 * kWave) {
-      s0 += mass(p, less, gone, v);
-      s1 += mass(p, less, gone, v + kWave);
-      s2 += mass(p, less, gone, v + 2 * kWave);
-      s3 += mass(p, less, gone, v + 3 * kWave);
-    }
-    for (; v < to; v += kWave) s0 += mass(p, less, gone, v);
-    const double sum = wave_sum64((s0 + s1) + (s2 + s3));
-    __syncthreads();  // the last level's sums have been read
-    if (lane == 0) lds[wave] = sum;
-    __syncthreads();
-    double total = 0.0;
-    for (int w = 0; w < kDraftWaves; w++) total += lds[w];
-    if (level == 0) {
-      any = total > 0.0;
-      target = u * total;
-    }
-    // the first part that the sum passes the target in, or else the last that has any mass
-    double sofar = 0.0, at = 0.0;
-    int part = 0;
-    for (int w = 0; w < kDraftWaves; w++) {
-      const double x = lds[w];
-      if (x > 0.0) {
-        part = w;
-        at = sofar;
-      }
-      sofar += x;
-      if (x > 0.0 && sofar > target) break;
-    }
-    target -= at;
-    const int lo = min(begin + part * per, end);
-    end = min(lo + per, end);
-    begin = lo;
-  }
-  int token = -1;
-  double sofar = 0.0;
-  for (int v0 = begin; v0 < end; v0 += kWave) {  // by each wavefront alike
-    const double x = v0 + lane < end ? mass(p, less, gone, v0 + lane) : 0.0;
-    double y = x;
+// The sum over the lanes up to this one.
+__device__ __forceinline__ double wave_scan64(double x) {
+  const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
-    for (int o = 1; o < kWave; o *= 2) {
-      const double z = __shfl_up(y, o);
-      if (lane >= o) y += z;
-    }
-    const unsigned long long some = __ballot(x > 0.0), past = __ballot(x > 0.0 && sofar + y > target);
-    if (past) {
-      token = v0 + __builtin_ctzll(past);
-      break;
-    }
-    if (some) token = v0 + 63 - __builtin_clzll(some);
-    sofar += __shfl(y, kWave - 1);
+  for (int o = 1; o < kWave; o *= 2) {
+    const double z = __shfl_up(x, o);
+    if (lane >= o) x += z;
   }
-  return any ? token : -1;
+  return x;
 }
 
-// One sequence per workgroup. Bound by the two rows of V floats that it reads (the second level reads a sixteenth of them
-// again, from a cache), at a CU's share of the memory's rate.
-__global__ __launch_bounds__(kDraftThreads) void k_draft_verify(int *accepted, int *tokens, const float *p, const float *q,
-                                                               const int *draft, const int *n_draft, const float *u, int K, int V,
-                                                               int *word) {
-  __shared__ double lds[kDraftWaves];
-  const int b = blockIdx.x, given = n_draft ? n_draft[b] : K, n = min(max(given, 0), K);
+// One sequence's row that its next token is drawn from: p, less the drafts' probabilities of the row (or null) or without the
+// one token (or -1) whose draft was certain; what is not positive and finite counts as 0.
+struct Row {
+  const float *p, *less;
+  int gone, a, n;  // accepted drafts, drafts
+  bool bad;
+  __device__ __forceinline__ double one(float x, float y, int v) const {
+    const double d = (double)x - (double)y;
+    return v != gone && d > 0.0 && d <= 3.402823466e38 ? d : 0.0;
+  }
+  // tokens v .. v + 3, those from `end` on 0
+  __device__ __forceinline__ void four(int v, int end, double (&x)[4]) const {
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f), g = f;
+    if (v + 4 <= end) {
+      f = ld4(p + v);
+      if (less) g = ld4(less + v);
+    } else if (v < end) {
+      f.x = p[v];
+      if (v + 1 < end) f.y = p[v + 1];
+      if (v + 2 < end) f.z = p[v + 2];
+      if (less) {
+        g.x = less[v];
+        if (v + 1 < end) g.y = less[v + 1];
+        if (v + 2 < end) g.z = less[v + 2];
+      }
+    }
+    x[0] = one(f.x, g.x, v);
+    x[1] = one(f.y, g.y, v + 1);
+    x[2] = one(f.z, g.z, v + 2);
+    x[3] = one(f.w, g.w, v + 3);
+  }
+};
+
+// Sequence b's drafts, a lane of every wavefront to each, until one is not accepted.
+__device__ Row verify(const float *p, const float *q, const int *draft, const int *n_draft, const float *u, int b, int K, int V) {
+  const int given = n_draft ? n_draft[b] : K, n = min(max(given, 0), K), lane = threadIdx.x & (kWave - 1);
   p += (size_t)b * (K + 1) * V;
   if (q) q += (size_t)b * K * V;
   draft += (size_t)b * K;
   u += (size_t)b * (K + 1);
+  Row r;
+  r.bad = given != n;
+  r.n = n;
   int a = 0;
-  bool bad = given != n;
-  for (; a < n; a++) {
-    const int t = draft[a];
-    if ((unsigned)t >= (unsigned)V) {  // no token: not accepted
-      bad = true;
+  for (; a < n; a += kWave) {
+    const int i = a + lane;
+    bool no = i < n;
+    if (no) {
+      const int t = draft[i];
+      if ((unsigned)t < (unsigned)V) {  // else no token: not accepted
+        const double pt = p[(size_t)i * V + t], qt = q ? q[(size_t)i * V + t] : 1.0;
+        no = !((double)u[i] * qt < pt);
+      }
+    }
+    const unsigned long long first = __ballot(no);
+    if (first) {
+      a += __builtin_ctzll(first);
       break;
     }
-    const double pt = p[(size_t)a * V + t], qt = q ? q[(size_t)a * V + t] : 1.0;
-    if (!((double)u[a] * qt < pt)) break;
   }
-  const float *row = p + (size_t)a * V, *less = a < n && q ? q + (size_t)a * V : nullptr;
-  int token = draw(row, less, a < n && !q ? draft[a] : -1, V, (double)u[K], lds);
-  if (token < 0 && a < n) token = draw(row, nullptr, -1, V, (double)u[K], lds);  // p and q are the same
-  if (token < 0) {
-    token = 0;
-    bad = true;
-  }
-  if (bad && threadIdx.x == 0) *word = UGK_IDS_DRAFT_VERIFY;
-  tokens += (size_t)b * (K + 1);
-  for (int i = threadIdx.x; i <= K; i += kDraftThreads) tokens[i] = i < a ? draft[i] : i == a ? token : -1;
-  if (threadIdx.x == 0) accepted[b] = a;
+  r.a = min(a, n);
+  const int t = r.a < n ? draft[r.a] : -1;
+  r.bad = r.bad || (r.a < n && (unsigned)t >= (unsigned)V);
+  r.p = p + (size_t)r.a * V;
+  r.less = r.a < n && q ? q + (size_t)r.a * V : nullptr;
+  r.gone = q ? -1 : t;
+  return r;
 }
 
+// The sums of the segments of every sequence's row, one per workgroup, where one workgroup per sequence would leave most CUs idle.
+__global__ __launch_bounds__(kSumThreads) void k_draft_sums(double *sums, const float *p, const float *q, const int *draft,
+                                                           const int *n_draft, const float *u, int K, int V, int segs, int seg) {
+  __shared__ double part[kSumThreads / kWave];
+  const int b = blockIdx.x / segs, s = blockIdx.x % segs;
+  const Row r = verify(p, q, draft, n_draft, u, b, K, V);
+  const int from = s * seg, to = min(from + seg, V);
+  double t[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 1
+  for (int v0 = from; v0 < to; v0 += kStep) {
+    double x[kStep / (4 * kSumThreads)][4];
+#pragma unroll
+    for (int i = 0; i < kStep / (4 * kSumThreads); i++) r.four(v0 + 4 * ((int)threadIdx.x + i * kSumThreads), to, x[i]);
+#pragma unroll
+    for (int i = 0; i < kStep / (4 * kSumThreads); i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) t[j] += x[i][j];
+  }
+  const double sum = wave_sum64((t[0] + t[1]) + (t[2] + t[3]));
+  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+struct DrawLds {
+  double seg[kMaxSegs], wave[kDraftWaves];
+  int first, last;
+};
+
+// The token of row r at the fraction u of its cumulative sum, or -1 where that is 0. `sums`: the segments', or null; a wavefront sums a
+// segment then. The segment in which the sum passes is walked with four tokens per thread.
+__device__ int draw(const Row &r, int V, int segs, int seg, double u, const double *sums, DrawLds &lds) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  int begin = 0;
+  double target = 0.0, sofar = 0.0;
+  bool any = true;
+  if (segs > 1) {
+    __syncthreads();  // what a draw before this one had there has been read
+    if (sums) {
+      for (int s = threadIdx.x; s < segs; s += kDraftThreads) lds.seg[s] = sums[s];
+    } else {
+#pragma unroll 1
+      for (int s = wave; s < segs; s += kDraftWaves) {
+        const int from = s * seg, to = min(from + seg, V);
+        double t[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 1
+        for (int v0 = from; v0 < to; v0 += 16 * kWave) {
+          double x[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) r.four(v0 + 4 * (lane + i * kWave), to, x[i]);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[j] += x[i][j];
+        }
+        const double sum = wave_sum64((t[0] + t[1]) + (t[2] + t[3]));
+        if (lane == 0) lds.seg[s] = sum;
+      }
+    }
+    __syncthreads();
+    // by each wavefront alike, a run of segments per lane
+    const int per = (segs + kWave - 1) / kWave, s0 = min(lane * per, segs), s1 = min(s0 + per, segs);
+    double mine = 0.0;
+    for (int s = s0; s < s1; s++) mine += lds.seg[s];
+    const double to = wave_scan64(mine), total = __shfl(to, kWave - 1);
+    any = total > 0.0;
+    target = u * total;
+    // the first segment that the sum passes the target in, or else the last that has any mass
+    const unsigned long long over = __ballot(mine > 0.0 && to > target), some = __ballot(mine > 0.0);
+    const int x = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
+    double at = to - mine, held = at;
+    int s = s0;
+    for (int w = s0; w < s1; w++) {
+      const double y = lds.seg[w];
+      if (y > 0.0) {
+        s = w;
+        held = at;
+      }
+      at += y;
+      if (y > 0.0 && at > target) break;
+    }
+    begin = __shfl(s, x) * seg;
+    sofar = __shfl(held, x);
+  }
+  const int end = segs > 1 ? min(begin + seg, V) : V;
+  int token = -1;
+  for (int v0 = begin; v0 < end; v0 += kStep) {
+    const int v = v0 + 4 * (int)threadIdx.x;
+    double x[4];
+    r.four(v, end, x);
+    const double mine = (x[0] + x[1]) + (x[2] + x[3]), up = wave_scan64(mine);
+    __syncthreads();  // the last step's have been read
+    if (lane == kWave - 1) lds.wave[wave] = up;
+    if (threadIdx.x == 0) {
+      lds.first = INT_MAX;
+      lds.last = -1;
+    }
+    __syncthreads();
+    double before = 0.0, all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kDraftWaves; w++) {
+      before += w < wave ? lds.wave[w] : 0.0;
+      all += lds.wave[w];
+    }
+    if (segs == 1 && v0 == begin) {  // V is at most kStep then: this is the whole row
+      any = all > 0.0;
+      target = u * all;
+    }
+    double sum = sofar + (before + (up - mine));
+    int past = INT_MAX, last = -1;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      sum += x[i];
+      if (x[i] > 0.0) {
+        last = v + i;
+        if (past == INT_MAX && sum > target) past = v + i;
+      }
+    }
+    const unsigned long long over = __ballot(past != INT_MAX), some = __ballot(last >= 0);
+    if (over && lane == __builtin_ctzll(over)) atomicMin(&lds.first, past);
+    if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&lds.last, last);
+    __syncthreads();
+    if (lds.first != INT_MAX) {
+      token = lds.first;
+      break;
+    }
+    token = max(token, lds.last);
+    sofar += all;
+  }
+  return any ? token : -1;
+}
+
+// One sequence per workgroup. Bound by the row (or two) of V floats that it reads without `sums`, at a CU's share of the memory's rate,
+// and by the chain from the drafts to their probabilities, the row and the walk.
+__global__ __launch_bounds__(kDraftThreads) void k_draft_verify(int *accepted, int *tokens, const float *p, const float *q, const int *draft,
+                                                               const int *n_draft, const float *u, const double *sums, int K, int V,
+                                                               int segs, int seg, int *word) {
+  __shared__ DrawLds lds;
+  const int b = blockIdx.x;
+  Row r = verify(p, q, draft, n_draft, u, b, K, V);
+  const double x = u[(size_t)b * (K + 1) + K];
+  int token = draw(r, V, segs, seg, x, sums ? sums + (size_t)b * segs : nullptr, lds);
+  if (token < 0 && r.a < r.n) {  // p and q are the same
+    r.less = nullptr;
+    r.gone = -1;
+    token = draw(r, V, segs, seg, x, nullptr, lds);
+  }
+  if (token < 0) {
+    token = 0;
+    r.bad = true;
+  }
+  if (r.bad && threadIdx.x == 0) *word = UGK_IDS_DRAFT_VERIFY;
+  tokens += (size_t)b * (K + 1);
+  draft += (size_t)b * K;
+  for (int i = threadIdx.x; i <= K; i += kDraftThreads) tokens[i] = i < r.a ? draft[i] : i == r.a ? token : -1;
+  if (threadIdx.x == 0) accepted[b] = r.a;
+}
+
+// Segments of a row: whole steps, at most kMaxSegs.
+int seg_floats(int V) { return (int)(((long long)V + (long long)kMaxSegs * kStep - 1) / ((long long)kMaxSegs * kStep)) * kStep; }
+// Sums in a launch of their own while one workgroup per sequence would leave CUs idle.
+bool separate(int nseq, int V) { return V > 2 * kStep && nseq < 256; }
 }  // namespace
 
+size_t draft_verify_bytes(int nseq, int V) {
+  return separate(nseq, V) ? (size_t)nseq * (((size_t)V + seg_floats(V) - 1) / seg_floats(V)) * sizeof(double) : 0;
+}
+// over all vocabularies of up to V
+size_t draft_verify_bound(int V) {
+  const size_t segs = ((size_t)V + kStep - 1) / kStep;
+  return segs > 2 ? 255 * (segs < (size_t)kMaxSegs ? segs : (size_t)kMaxSegs) * sizeof(double) : 0;
+}
+
 int launch_draft_verify(int *accepted, int *tokens, const float *p, const float *q, const int *draft, const int *n_draft,
-                        const float *u, int nseq, int K, int V, int *word) {
-  launch(k_draft_verify, dim3(nseq), dim3(kDraftThreads), 0, accepted, tokens, p, q, draft, n_draft, u, K, V, word);
+                        const float *u, double *sums, int nseq, int K, int V, int *word) {
+  const int seg = seg_floats(V), segs = (int)(((long long)V + seg - 1) / seg);
+  if (sums) {
+    launch(k_draft_sums, dim3((unsigned)nseq * segs), dim3(kSumThreads), 0, sums, p, q, draft, n_draft, u, K, V, segs, seg);
+    if (int e = check_launch("draft_verify")) return e;
+  }
+  launch(k_draft_verify, dim3(nseq), dim3(kDraftThreads), 0, accepted, tokens, p, q, draft, n_draft, u, sums, K, V, segs, seg, word);
   return check_launch("draft_verify");
 }
 

@@ -24,7 +24,7 @@ int check_launch(const char *what);
 // never another's: the LayerNorm-backward partial rows (one slot per call, or
 // 2L+1 slots for the step driver), the encoder backward's bucket state (kept
 // between calls), the KL total's partial sums, the long-row softmax's row
-// statistics, and attention's (the backward's row sums, the recomputed forward
+// statistics, attention's (the backward's row sums, the recomputed forward
 // of the dense callback, the parts of a split key axis). Each region is the library's own allocation, grown when a
 // larger shape arrives (after waiting for the device), or a fixed part of a
 // workspace the caller handed over with ugk_set_workspace, which then never
@@ -33,7 +33,7 @@ int check_launch(const char *what);
 // region's memory is new since its last use (its contents are undefined).
 // With keep_fresh the fresh mark is reported but left set (for a caller that
 // cannot prepare the memory now, e.g. under graph capture).
-enum Region { kRegLn = 0, kRegEncoder = 1, kRegKl = 2, kRegSoftmax = 3, kRegAttention = 4, kNumRegions = 5 };
+enum Region { kRegLn = 0, kRegEncoder = 1, kRegKl = 2, kRegSoftmax = 3, kRegAttention = 4, kRegDraft = 5, kNumRegions = 6 };
 void *workspace(Region r, size_t bytes, bool *fresh = nullptr, bool keep_fresh = false);
 // Whether the library stream is being captured into a graph (false if the
 // query fails).
@@ -402,7 +402,9 @@ size_t cache8_attention_bytes(const ugk_cache8 &a, bool weigh);
 int launch_cache8_evict(int *table_out, int *len_out, float *weight_out, int *dropped, const int *table, const int *k_len,
                         const float *weight, int nseq, int ld, int keep, int first, int recent, int *word);
 int launch_draft_verify(int *accepted, int *tokens, const float *p, const float *q, const int *draft, const int *n_draft,
-                        const float *u, int nseq, int K, int V, int *word);
+                        const float *u, double *sums, int nseq, int K, int V, int *word);
+size_t draft_verify_bytes(int nseq, int V);  // of sums; 0: none
+size_t draft_verify_bound(int V);            // over all calls of up to V tokens
 
 // Workspace sizes.
 size_t layernorm_backward_scratch(int rows, int C);  // bytes of one call's partial rows
