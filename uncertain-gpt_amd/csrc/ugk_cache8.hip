@@ -35,7 +35,7 @@ struct Seq8 {
   __device__ __forceinline__ int seen(int i, int causal) const { return causal ? max(0, min(Lk, i + 1 + Lk - Lq)) : Lk; }
 };
 
-// Sequence b; a workgroup with `tell` reports rows and lengths that were clamped.
+// Sequence b; threads with `tell` report rows and lengths that were clamped.
 __device__ __forceinline__ Seq8 sequence8(const ugk_cache8 &a, int b, bool tell, int *word, int code) {
   Seq8 s;
   bool bad = false;
@@ -43,7 +43,7 @@ __device__ __forceinline__ Seq8 sequence8(const ugk_cache8 &a, int b, bool tell,
   const int n = a.k_len ? a.k_len[b] : a.max_k;
   s.Lk = min(max(n, 0), a.max_k);
   bad = bad || s.Lk != n;
-  if (bad && tell && threadIdx.x == 0) *word = code;
+  if (bad && tell) *word = code;
   return s;
 }
 
@@ -146,6 +146,14 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
   if (id < 0) return;
   const size_t at = (size_t)id * a.NKV + t.h;
   float *sp = (values ? vs : ks) + at;
+  uint32_t *dst = reinterpret_cast<uint32_t *>((values ? v8 : k8) + at * kKeys * HP);
+  // words of the values hold four keys: of a block that is not all new what they hold is on its way with the scale
+  const bool whole = t.r0 == 0 && t.r1 == kKeys;
+  uint32_t held[CH];
+  if (values && !whole) {
+#pragma unroll
+    for (int i = 0; i < CH; i++) held[i] = dst[threadIdx.x + i * kBlock];
+  }
   const float was = t.r0 > 0 ? *sp : 0.0f;
   bool finite = true;
   const auto look = [&](float &f) {
@@ -172,7 +180,6 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
   const float now = fmaxf(was, scale_for(most));
   const float inv = now > 0.0f ? 1.0f / now : 0.0f, ratio = was * inv;
   const bool grown = t.r0 > 0 && now > was && was > 0.0f;
-  uint32_t *dst = reinterpret_cast<uint32_t *>((values ? v8 : k8) + at * kKeys * HP);
   uint32_t w[kPer][4];
 #pragma unroll
   for (int i = 0; i < kPer; i++)
@@ -202,9 +209,10 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
         tile[(4 * g + d) * 17 + c] = pack4(code_at(w[i][0], d), code_at(w[i][1], d), code_at(w[i][2], d), code_at(w[i][3], d));
     }
     __syncthreads();
-    const bool whole = t.r0 == 0 && t.r1 == kKeys;
-    for (int e = threadIdx.x; e < HP * 16; e += kBlock) {
-      const int d = e / 16, c = e % 16;
+    static_assert(HP * 16 == CH * kBlock, "a word of each turn for every thread");
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int e = threadIdx.x + i * kBlock, d = e / 16, c = e % 16;
       uint32_t word4 = tile[d * 17 + c];
       if (!whole) {
         uint32_t fresh = 0, older = 0;  // the bytes of the call's rows, of the rows before
@@ -215,9 +223,9 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
           else if (row < t.r1) fresh |= 0xffu << 8 * r;
         }
         if (!fresh && !(older && grown)) continue;
-        uint32_t held = dst[e];
-        if (grown) held = (again4(held, ratio) & older) | (held & ~older);
-        word4 = (word4 & fresh) | (held & ~fresh);
+        uint32_t old = held[i];
+        if (grown) old = (again4(old, ratio) & older) | (old & ~older);
+        word4 = (word4 & fresh) | (old & ~fresh);
       }
       dst[e] = word4;
     }
@@ -272,11 +280,12 @@ __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, cons
 // ---- attention --------------------------------------------------------------------
 
 // Parts of the key axis: o normalised, the maximum m of its scores in base 2 and the sum l of 2^(s - m), per row and head;
-// `block`: the same m and l of each block of 64 keys, and `stat` those of the whole axis (for the blocks' weights).
+// `block`: the same m and l of each block of 64 keys, and `stat` of rows that have no parts (for the blocks' weights).
 struct Parts8 {
   float *o, *m, *l;
   float2 *block, *stat;
-  int splits, chunk;  // blocks per part: a row has the parts up to its last key's
+  int *used;                 // the blocks per part of this call
+  int splits, least, slots;  // parts of the longest axis, the fewest blocks per part, workgroups that the CUs hold (0: `least` it is)
 };
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -378,10 +387,6 @@ __device__ __forceinline__ float undigits(v4i d) {
 
 constexpr int kFewWaves = 4;
 
-// The sequence and key/value head of workgroup x in a round of all of them, one further each time that all have had one: workgroups go to the chip's eight
-// dies in turn, and the long sequences would else be with the same ones throughout where the pairs are a multiple of eight.
-__device__ __forceinline__ unsigned turned(unsigned x, unsigned round, unsigned pairs) { return (x % pairs + round) % pairs; }
-
 // The codes of a block as the operands of the 8-bit matrix units: 16 bytes a lane of 16 keys' rows (kf) and of 16 columns (vf),
 // and the scales. A block that is not there is read as block 0, and its keys are masked.
 template <int DT>
@@ -428,20 +433,24 @@ __device__ __forceinline__ v4i turn4(uint32_t a, uint32_t b, uint32_t c, uint32_
 // Where a row's results go: of this part of the key axis, or of the whole.
 struct Place8 {
   float *o, *m, *l, *lse;
-  __device__ __forceinline__ Place8(float *out, float *lse_, const Parts8 &parts, const ugk_cache8 &a, int part, size_t row, int h) {
-    const size_t p = ((size_t)part * a.rows_q + row) * a.NH + h;
-    o = parts.o ? parts.o + p * a.HS : out + row * a.ldo + (size_t)h * a.HS;
-    m = parts.o ? parts.m + p : nullptr;
-    l = parts.o ? parts.l + p : nullptr;
-    lse = parts.o || !lse_ ? nullptr : lse_ + row * a.NH + h;
+  float2 *stat;
+  // whole: no other part has keys of the row
+  __device__ __forceinline__ Place8(float *out, float *lse_, const Parts8 &parts, const ugk_cache8 &a, int part, bool whole, size_t row,
+                                    int h) {
+    const size_t at = row * a.NH + h, p = (size_t)part * a.rows_q * a.NH + at;
+    o = whole ? out + row * a.ldo + (size_t)h * a.HS : parts.o + p * a.HS;
+    m = whole ? nullptr : parts.m + p;
+    l = whole ? nullptr : parts.l + p;
+    lse = whole && lse_ ? lse_ + at : nullptr;
+    stat = whole && parts.stat ? parts.stat + at : nullptr;
   }
   __device__ __forceinline__ void put(float top, float sum) const {
     if (m) {
       *m = top;
       *l = sum;
-    } else if (lse) {
-      *lse = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn28;
     }
+    if (lse) *lse = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn28;
+    if (stat) *stat = make_float2(top, sum);
   }
 };
 
@@ -472,6 +481,118 @@ struct Walk {
 };
 __device__ __forceinline__ size_t block_head(int id, int NKV, int hk) { return (size_t)max(id, 0) * NKV + hk; }
 
+__device__ __forceinline__ int wave_sum_int(int x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ int wave_scan_int(int x) {
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// What a workgroup has: group `group` of R rows of a sequence and key/value head, and of their blocks a part.
+struct Job8 {
+  Seq8 s;
+  int b, hk, group, part, rows, first, stop;
+  bool none, whole;  // nothing; all blocks
+};
+// Blocks that group t of R rows sees: its last row sees most.
+__device__ __forceinline__ int blocks_of(const Seq8 &s, const ugk_cache8 &a, int G, int R, int t) {
+  return (s.seen((min((t + 1) * R, s.Lq * G) - 1) / G, a.causal) + kKeys - 1) / kKeys;
+}
+// The parts of nb blocks, of at most `chunk` each and as equal as they can be.
+__device__ __forceinline__ int parts_for(int nb, int chunk) { return max(1, (nb + chunk - 1) / chunk); }
+// Workgroup blockIdx.x's. Where the key axis is cut (parts.slots), the parts follow one another without a gap for the shorter
+// sequences, whose workgroups, empty, would still be dealt out to the CUs in turn and leave some with two and others with none; and a
+// part has so many blocks, from what the sequences really hold, that the workgroups are about as many as the CUs take, or, where the rows alone make
+// that many, that none has more than its share of all blocks. Every wavefront finds its place alike: a lane to a sequence, then to
+// a group. Else workgroups are of pairs, groups (the longest first) and parts in turn.
+template <int R>
+__device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts, unsigned pairs, unsigned groups, int *word) {
+  Job8 w;
+  const int lane = threadIdx.x & (kWave - 1), G = a.NH / a.NKV;
+  int chunk = parts.least;
+  w.none = true;
+  if (parts.slots) {
+    int blocks = 0, jobs = 0;
+    Seq8 s{0, 0, 0};  // the lane's of the last 64 sequences, which are mostly all
+    for (int b = lane; b < a.nseq; b += kWave) {
+      s = sequence8(a, b, blockIdx.x == 0, word, UGK_IDS_CACHE8_ATTENTION);
+      const int n = (s.Lq * G + R - 1) / R;
+      jobs += n;
+      for (int t = 0; t < n; t++) blocks += blocks_of(s, a, G, R, t);
+    }
+    jobs = wave_sum_int(jobs) * a.NKV;
+    blocks = wave_sum_int(blocks) * a.NKV;
+    const int left = 2 * jobs < parts.slots ? parts.slots - jobs : parts.slots;
+    chunk = __builtin_amdgcn_readfirstlane(max(chunk, (blocks + left - 1) / left));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *parts.used = chunk;
+    // the sequence, then the group and the part that are number x of all
+    int x = blockIdx.x, b = -1;
+    for (int b0 = 0; b0 < a.nseq && b < 0; b0 += kWave) {
+      int mine = 0;
+      if (a.nseq > kWave && b0 + lane < a.nseq) s = sequence8(a, b0 + lane, false, nullptr, 0);
+      if (b0 + lane < a.nseq) {
+        const int n = (s.Lq * G + R - 1) / R;
+        for (int t = 0; t < n; t++) mine += parts_for(blocks_of(s, a, G, R, t), chunk);
+        mine *= a.NKV;
+      }
+      const int to = wave_scan_int(mine), all = __shfl(to, kWave - 1);
+      const uint64_t over = __ballot(to > x);
+      if (over) {
+        const int l = __builtin_ctzll(over);
+        b = b0 + l;
+        x -= __shfl(to - mine, l);
+        w.s.q0 = __builtin_amdgcn_readfirstlane(__shfl(s.q0, l));
+        w.s.Lq = __builtin_amdgcn_readfirstlane(__shfl(s.Lq, l));
+        w.s.Lk = __builtin_amdgcn_readfirstlane(__shfl(s.Lk, l));
+      } else {
+        x -= all;
+      }
+    }
+    if (b < 0) return w;
+    w.b = __builtin_amdgcn_readfirstlane(b);
+    const int n = (w.s.Lq * G + R - 1) / R;
+    for (int t0 = 0; t0 < n; t0 += kWave) {
+      const int t = n - 1 - t0 - lane, mine = t < 0 ? 0 : parts_for(blocks_of(w.s, a, G, R, t), chunk) * a.NKV;
+      const int to = wave_scan_int(mine), all = __shfl(to, kWave - 1);
+      const uint64_t over = __ballot(to > x);
+      if (over) {
+        const int l = __builtin_ctzll(over);
+        w.group = __builtin_amdgcn_readfirstlane(n - 1 - t0 - l);
+        x -= __shfl(to - mine, l);
+        break;
+      }
+      x -= all;
+    }
+    x = __builtin_amdgcn_readfirstlane(x);
+    w.part = x / a.NKV;
+    w.hk = x % a.NKV;
+  } else {
+    const unsigned round = blockIdx.x / pairs, pair = (blockIdx.x % pairs + round) % pairs;
+    w.b = pair / a.NKV;
+    w.hk = pair % a.NKV;
+    w.part = round / groups;
+    w.group = groups - 1 - round % groups;
+    w.s = sequence8(a, w.b, w.hk == 0 && round == 0, word, UGK_IDS_CACHE8_ATTENTION);
+    if (parts.o && blockIdx.x == 0 && threadIdx.x == 0) *parts.used = chunk;
+    if (w.group * R >= w.s.Lq * G) return w;
+  }
+  w.rows = w.s.Lq * G;
+  const int nb = blocks_of(w.s, a, G, R, w.group), n = parts.o ? parts_for(nb, chunk) : 1;
+  w.whole = n == 1;
+  w.none = w.part >= n;
+  w.first = (int)((long long)nb * w.part / n);
+  w.stop = (int)((long long)nb * (w.part + 1) / n);
+  return w;
+}
+
 // Up to four rows (query rows times heads of the group) of a sequence and key/value head.
 //
 // A row of q is held as whole numbers of 31 bits next to its largest element, and those as four digits, so that four
@@ -488,15 +609,10 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_fe
   __shared__ float lm[kFewWaves][4], ll[kFewWaves][4];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const unsigned pair = turned(blockIdx.x, blockIdx.x / pairs, pairs);
-  const int part = blockIdx.x / pairs;
-  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
-  const Seq8 s = sequence8(a, b, hk == 0 && part == 0, word, UGK_IDS_CACHE8_ATTENTION);
-  const int rows = s.Lq * G;
-  if (rows == 0) return;
-  const int end = s.seen(s.Lq - 1, a.causal), nb = (end + kKeys - 1) / kKeys;  // the last row sees most
-  const int first = part * parts.chunk, stop = min(first + parts.chunk, nb);
-  if (part > 0 && first >= nb) return;  // no row of the workgroup has this part
+  const Job8 job = job_of<4>(a, parts, pairs, 1, word);
+  if (job.none) return;
+  const Seq8 &s = job.s;
+  const int b = job.b, hk = job.hk, G = a.NH / a.NKV, rows = job.rows, first = job.first, stop = job.stop;
   const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
 
   Codes<DT> c(padded(a.HS), lane);
@@ -538,7 +654,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_fe
     ex = __shfl(e, 4 * quad) - 29;
     nan = (uint32_t)__shfl((int)most, 4 * quad) >= kInfBits;
   }
-  const int lim = quad < rows ? s.seen(quad / G, a.causal) : end;
+  const int lim = quad < rows ? s.seen(quad / G, a.causal) : 0;
   Running run;
   float o[DT];
 #pragma unroll
@@ -625,7 +741,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_fe
     wt[w] = ll[w][r] == 0.0f ? 0.0f : ll[w][r] * ex2(lm[w][r] - or0(top));
     total += wt[w];
   }
-  const Place8 to(out, lse, parts, a, part, (size_t)s.q0 + r / G, hk * G + r % G);
+  const Place8 to(out, lse, parts, a, job.part, job.whole, (size_t)s.q0 + r / G, hk * G + r % G);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   for (int d = lane; d < a.HS; d += kWave) {
     float y = 0.0f;
@@ -659,15 +775,10 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
   __shared__ float lm[kFewWaves][16], ll[kFewWaves][16];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const unsigned pair = turned(blockIdx.x, blockIdx.x / pairs, pairs), group = blockIdx.x / pairs % groups;
-  const int part = blockIdx.x / pairs / groups;
-  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV;
-  const Seq8 s = sequence8(a, b, hk == 0 && part == 0 && group == 0, word, UGK_IDS_CACHE8_ATTENTION);
-  const int rows = s.Lq * G, row0 = group * 16 * RW;
-  if (row0 >= rows) return;
-  const int end = s.seen((min(row0 + 16 * RW, rows) - 1) / G, a.causal), nb = (end + kKeys - 1) / kKeys;
-  const int first = part * parts.chunk, stop = min(first + parts.chunk, nb);
-  if (part > 0 && first >= nb) return;  // no row of the workgroup has this part
+  const Job8 job = job_of<16 * RW>(a, parts, pairs, groups, word);
+  if (job.none) return;
+  const Seq8 &s = job.s;
+  const int b = job.b, hk = job.hk, G = a.NH / a.NKV, rows = job.rows, row0 = job.group * 16 * RW, first = job.first, stop = job.stop;
   const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
 
   Codes<DT> c(padded(a.HS), lane);
@@ -682,7 +793,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
   }
 
   v4i aq[KS][4];
-  const int mine = row0 + 16 * (wave / KW) + col, lim = mine < rows ? s.seen(mine / G, a.causal) : end;
+  const int mine = row0 + 16 * (wave / KW) + col, lim = mine < rows ? s.seen(mine / G, a.causal) : 0;
   int ex;
   bool nan;
   Running run;
@@ -827,7 +938,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
       wt[w] = ll[w0 + w][r] == 0.0f ? 0.0f : ll[w0 + w][r] * ex2(lm[w0 + w][r] - or0(top));
       total += wt[w];
     }
-    const Place8 to(out, lse, parts, a, part, (size_t)s.q0 + row / G, hk * G + row % G);
+    const Place8 to(out, lse, parts, a, job.part, job.whole, (size_t)s.q0 + row / G, hk * G + row % G);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     for (int d = lane; d < a.HS; d += kWave) {
       float y = 0.0f;
@@ -839,77 +950,112 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
   }
 }
 
-// The parts of a split key axis joined, one wavefront per row and head, in the parts' order.
-__global__ __launch_bounds__(kBlock) void k_cache8_join(float *out, float *lse, Parts8 parts, ugk_cache8 a) {
-  const size_t nth = (size_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6), per = (size_t)a.rows_q * a.NH;
-  if (nth >= (size_t)a.nseq * a.max_q * a.NH) return;
-  const int lane = threadIdx.x & (kWave - 1), h = nth % a.NH, i = nth / a.NH % a.max_q, b = nth / a.NH / a.max_q;
+// What m and l of the parts of row `at` say of the whole.
+__device__ __forceinline__ float2 joined(const Parts8 &parts, size_t per, size_t at, int n) {
+  float m = -INFINITY, l = 0.0f;
+  for (int p0 = 0; p0 < n; p0 += 8) {
+    float lp[8], mp[8], top = m;
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const size_t p = min(p0 + u, n - 1) * per + at;
+      mp[u] = parts.m[p];
+      lp[u] = p0 + u < n ? parts.l[p] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++) top = fmaxf(top, lp[u] == 0.0f ? -INFINITY : mp[u]);
+    l *= ex2(m - or0(top));
+    m = top;
+#pragma unroll
+    for (int u = 0; u < 8; u++) l += lp[u] == 0.0f ? 0.0f : lp[u] * ex2(mp[u] - or0(top));
+  }
+  return make_float2(m, l);
+}
+
+// Behind the attention, workgroups of two kinds. The first `joins` join the parts of a split key axis, one wavefront per row and head, in the
+// parts' order, where a workgroup of `rows` rows had more than one. The others add up the weights of 16 blocks of a sequence, 16
+// threads to each, which take every sixteenth row and head, in a fixed order: weight[b, j] += sum of l_j 2^(m_j - m) / l.
+__global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse, float *weight, Parts8 parts, ugk_cache8 a, int rows,
+                                                         unsigned joins) {
+  constexpr int kAtOnce = 8;  // parts whose loads are on their way together
+  const int G = a.NH / a.NKV;
+  const size_t per = (size_t)a.rows_q * a.NH;
+  if (blockIdx.x >= joins) {
+    __shared__ float part[16][17];
+    __shared__ float2 whole[kBlock];
+    const unsigned x = blockIdx.x - joins;
+    const int of = (a.ld_table + 15) / 16, b = x / of, j = x % of * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+    const Seq8 s = sequence8(a, b, false, nullptr, 0);
+    const int nb = (s.Lk + kKeys - 1) / kKeys, n = s.Lq * G, chunk = joins ? *parts.used : 0;
+    if (x % of * 16 >= nb) return;
+    float sum = 0.0f;
+    for (int y0 = 0; y0 < n * a.NKV; y0 += kBlock) {  // a row and head per thread, then a block per thread
+      const int mine = y0 + (int)threadIdx.x;
+      if (mine < n * a.NKV) {
+        const int hk = mine / n, rr = mine % n;
+        const size_t at = ((size_t)s.q0 + rr / G) * a.NH + hk * G + rr % G;
+        const int all = joins ? parts_for(blocks_of(s, a, G, rows, rr / rows), chunk) : 1;
+        whole[threadIdx.x] = all > 1 ? joined(parts, per, at, all) : parts.stat[at];
+      }
+      __syncthreads();
+      for (int y = y0 + slice; y < min(y0 + kBlock, n * a.NKV); y += 16) {
+        const int hk = y / n, rr = y % n;
+        if (j * kKeys >= s.seen(rr / G, a.causal)) continue;
+        const float2 p = parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + rr) * a.ld_table + j], w = whole[y - y0];
+        if (p.y != 0.0f) sum += p.y * ex2(p.x - w.x) / w.y;
+      }
+      __syncthreads();
+    }
+    part[slice][threadIdx.x & 15] = sum;
+    __syncthreads();
+    if (slice || j >= nb) return;
+    float t = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 16; y++) t += part[y][threadIdx.x];
+    weight[(size_t)b * a.ld_table + j] += t;
+    return;
+  }
+  const int per_seq = (a.max_q * G + 3) / 4, b = blockIdx.x / per_seq / a.NKV, hk = blockIdx.x / per_seq % a.NKV;
+  const int lane = threadIdx.x & (kWave - 1), rr = blockIdx.x % per_seq * 4 + (threadIdx.x >> 6);
   const Seq8 s = sequence8(a, b, false, nullptr, 0);
-  if (i >= s.Lq) return;
+  const int chunk = *parts.used;
+  if (rr >= s.Lq * G) return;
+  const int n = parts_for(blocks_of(s, a, G, rows, rr / rows), chunk);
+  if (n == 1) return;  // one workgroup had the row whole
+  const int i = rr / G, h = hk * G + rr % G;
   const size_t g = (size_t)s.q0 + i, at = g * a.NH + h;
-  const int splits = max(1, (s.seen(i, a.causal) + kKeys * parts.chunk - 1) / (kKeys * parts.chunk));
-  float m = -INFINITY;
-  for (int x = lane; x < splits; x += kWave) m = fmaxf(m, parts.m[x * per + at]);
-#pragma unroll
-  for (int x = 32; x; x /= 2) m = fmaxf(m, __shfl_xor(m, x));
-  float o0 = 0.0f, o1 = 0.0f, l = 0.0f;
+  float m = -INFINITY, o0 = 0.0f, o1 = 0.0f, l = 0.0f;
   const int d0 = min(lane, a.HS - 1), d1 = min(lane + kWave, a.HS - 1);
-  for (int x0 = 0; x0 < splits; x0 += kWave) {
-    const int x = x0 + lane, n = min(kWave, splits - x0);
-    const float lx = x < splits ? parts.l[x * per + at] : 0.0f;
-    const float w = lx == 0.0f ? 0.0f : lx * ex2(parts.m[x * per + at] - or0(m));  // 0: a part without a key of this row, its o is 0
-    l += wave_sum(w);
-    for (int t = 0; t < n; t += 8) {  // eight parts' loads at a time
-      float y0[8], y1[8];
+  for (int t = 0; t < n; t += kAtOnce) {
+    float y0[kAtOnce], y1[kAtOnce], mt[kAtOnce], lt[kAtOnce], top = m;
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const float *o = parts.o + ((x0 + min(t + u, n - 1)) * per + at) * a.HS;
-        y0[u] = o[d0];
-        y1[u] = o[d1];
-      }
+    for (int u = 0; u < kAtOnce; u++) {
+      const size_t p = min(t + u, n - 1) * per + at;
+      y0[u] = parts.o[p * a.HS + d0];
+      y1[u] = parts.o[p * a.HS + d1];
+      mt[u] = parts.m[p];
+      lt[u] = t + u < n ? parts.l[p] : 0.0f;
+    }
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const float wt = __shfl(w, (t + u) & (kWave - 1));
-        o0 = t + u < n ? fmaf(wt, y0[u], o0) : o0;
-        o1 = t + u < n ? fmaf(wt, y1[u], o1) : o1;
-      }
+    for (int u = 0; u < kAtOnce; u++) top = fmaxf(top, lt[u] == 0.0f ? -INFINITY : mt[u]);
+    const float keep = ex2(m - or0(top));
+    m = top;
+    l *= keep;
+    o0 *= keep;
+    o1 *= keep;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++) {
+      const float w = lt[u] == 0.0f ? 0.0f : lt[u] * ex2(mt[u] - or0(top));  // 0: a part without a key of this row, its o is 0
+      l += w;
+      o0 = fmaf(w, y0[u], o0);
+      o1 = fmaf(w, y1[u], o1);
     }
   }
   const bool none = l == 0.0f;
   const float inv = none ? 1.0f : 1.0f / l;
-  float *po = out + g * a.ldo + h * a.HS;
+  float *po = out + g * a.ldo + (size_t)h * a.HS;
   if (lane < a.HS) po[lane] = o0 * inv;
   if (lane + kWave < a.HS) po[lane + kWave] = o1 * inv;
-  if (lane) return;
-  if (lse) lse[g * a.NH + h] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn28;
-  if (parts.stat) parts.stat[at] = make_float2(m, l);
-}
-
-// weight[b, j] += the sum over rows and heads of what block j got: 16 blocks of a sequence per workgroup, 16 threads to each,
-// which take every sixteenth row and head; added in a fixed order.
-__global__ __launch_bounds__(kBlock) void k_cache8_weights(float *weight, Parts8 parts, ugk_cache8 a) {
-  __shared__ float part[16][17];
-  const int per = (a.ld_table + 15) / 16, b = blockIdx.x / per, j = blockIdx.x % per * 16 + (threadIdx.x & 15);
-  const int slice = threadIdx.x >> 4, G = a.NH / a.NKV;
-  const Seq8 s = sequence8(a, b, false, nullptr, 0);
-  const int nb = (s.Lk + kKeys - 1) / kKeys, rows = s.Lq * G;
-  float sum = 0.0f;
-  if (j < nb) {
-    for (int x = slice; x < rows * a.NKV; x += 16) {
-      const int hk = x / rows, rr = x % rows, i = rr / G, h = hk * G + rr % G;
-      if (j * kKeys >= s.seen(i, a.causal)) continue;
-      const float2 p = parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + rr) * a.ld_table + j];
-      const float2 all = parts.stat[((size_t)s.q0 + i) * a.NH + h];
-      if (p.y != 0.0f) sum += p.y * ex2(p.x - all.x) / all.y;
-    }
-  }
-  part[slice][threadIdx.x & 15] = sum;
-  __syncthreads();
-  if (slice || j >= nb) return;
-  float t = 0.0f;
-#pragma unroll
-  for (int x = 0; x < 16; x++) t += part[x][threadIdx.x];
-  weight[(size_t)b * a.ld_table + j] += t;
+  if (lse && lane == 0) lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn28;
 }
 
 // Many rows: a prompt's. 128 rows of a sequence and key/value head per workgroup, 32 to a wavefront, over blocks whose codes go
@@ -931,21 +1077,17 @@ __device__ __forceinline__ v2u halves4(uint32_t w) {
 template <int DT>
 __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(float *out, float *lse, const float *q, const int8_t *k8,
                                                                  const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
-                                                                 Parts8 parts, unsigned pairs, unsigned tiles, int *word) {
+                                                                 Parts8 parts, unsigned pairs, unsigned groups, int *word) {
   constexpr int KSTR = 16 * DT + 8, VSTR = kKeys + 8, D32 = DT / 2, NL = (DT + 3) / 4;
   __shared__ alignas(16) _Float16 kl[2][kKeys * KSTR];
   __shared__ alignas(16) _Float16 vl[2][16 * DT * VSTR];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const unsigned pair = turned(blockIdx.x, blockIdx.x / pairs + blockIdx.y, pairs);
-  const int tile = (int)(tiles - 1 - blockIdx.x / pairs), part = blockIdx.y;  // the longest first
-  const int b = pair / a.NKV, hk = pair % a.NKV, G = a.NH / a.NKV, HP = padded(a.HS), CH = HP / 16;
-  const Seq8 s = sequence8(a, b, hk == 0 && part == 0 && tile == 0, word, UGK_IDS_CACHE8_ATTENTION);
-  const int rows = s.Lq * G, row0 = tile * kTileRows8;
-  if (row0 >= rows) return;
-  const int nb = (s.seen((min(row0 + kTileRows8, rows) - 1) / G, a.causal) + kKeys - 1) / kKeys;
-  const int first = part * parts.chunk, stop = min(first + parts.chunk, nb);
-  if (part > 0 && first >= nb) return;  // no row of the workgroup has this part
+  const Job8 job = job_of<kTileRows8>(a, parts, pairs, groups, word);
+  if (job.none) return;
+  const Seq8 &s = job.s;
+  const int b = job.b, hk = job.hk, G = a.NH / a.NKV, HP = padded(a.HS), CH = HP / 16;
+  const int rows = job.rows, row0 = job.group * kTileRows8, first = job.first, stop = job.stop;
   const int mine = row0 + 32 * wave + col, safe = min(mine, rows - 1), i = safe / G, h = hk * G + safe % G;
   const int lim = s.seen(i, a.causal);
   // what the wavefront's first and last rows see
@@ -1102,7 +1244,7 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
   int p;
   const float g = run.last(sum, &p);
   p -= 14;  // of the weights
-  const Place8 to(out, lse, parts, a, part, (size_t)s.q0 + i, h);
+  const Place8 to(out, lse, parts, a, job.part, job.whole, (size_t)s.q0 + i, h);
   float *po = to.o;
 #pragma unroll
   for (int t = 0; t < D32; t++)
@@ -1128,7 +1270,7 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
 
 // ---- eviction ----------------------------------------------------------------------
 
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictThreads = 1024, kBins = 2 * kEvictThreads;
 
 // Sum over the workgroup's threads before this one, and in *all over all of them.
 __device__ __forceinline__ int before(int x, int *lds, int *all) {
@@ -1153,14 +1295,14 @@ __device__ __forceinline__ int before(int x, int *lds, int *all) {
 }
 
 // One sequence per workgroup, E entries of its table per thread, side by side in registers: the d lightest blocks by a search over the
-// weights' bits, eight at a time (counts in LDS), ties by their index; then each entry's place from counts of those
-// before it. Reading and writing 16 bytes per entry is nothing; what counts are the chain of
-// barriers (four counts and two sums).
+// weights' bits, eleven at a time (counts in LDS: eight at a time took a turn more, and the exponents of many weights met in the same
+// counter), ties by their index; then each entry's place from counts of those before it. Reading and writing 16 bytes
+// per entry is nothing; what counts are the chain of barriers (three counts and two sums).
 template <int E>
 __global__ __launch_bounds__(kEvictThreads) void k_cache8_evict(int *table_out, int *len_out, float *weight_out, int *dropped,
                                                                const int *table, const int *k_len, const float *weight, int ld,
                                                                int keep, int first, int recent, int *word) {
-  __shared__ int count[256], lds[kEvictThreads / kWave];
+  __shared__ int count[kBins], lds[kEvictThreads / kWave];
   __shared__ int found, under;
   const int b = blockIdx.x, len = k_len[b];
   const int full = min(max(len, 0), (int)min((long long)ld * kKeys, (long long)0x7fffffff)), n = (full + kKeys - 1) / kKeys;
@@ -1179,47 +1321,36 @@ __global__ __launch_bounds__(kEvictThreads) void k_cache8_evict(int *table_out, 
     const uint32_t u = __float_as_uint(w[x] + 0.0f);
     key[x] = w[x] != w[x] ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
   }
-  // the value of the d-th lightest, eight bits at a time, and how many of its equals go
+  // the value of the d-th lightest, eleven bits at a time (the last ten), and how many of its equals go
   uint32_t value = 0;
-  int left = d;
+  int left = d, all;
   if (d > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (threadIdx.x < 256) count[threadIdx.x] = 0;
+#pragma unroll 1
+    for (int turn = 0; turn < 3; turn++) {
+      const int shift = turn == 0 ? 21 : turn == 1 ? 10 : 0, above = turn == 0 ? 31 : turn == 1 ? 21 : 10;  // the bits found so far
+      for (int i = threadIdx.x; i < kBins; i += kEvictThreads) count[i] = 0;
       __syncthreads();
 #pragma unroll
       for (int x = 0; x < E; x++) {
         const int i = i0 + x;
         const bool may = i >= first && i < n - recent;
-        if (may && (shift == 24 || key[x] >> (shift + 8) == value >> (shift + 8))) atomicAdd(&count[key[x] >> shift & 255u], 1);
+        const bool same = turn == 0 || key[x] >> above == value >> above;
+        if (may && same) atomicAdd(&count[key[x] >> shift & (turn == 2 ? 1023u : 2047u)], 1);
       }
       __syncthreads();
-      if (threadIdx.x < kWave) {  // four counts per lane
-        int c[4], sum = 0;
-#pragma unroll
-        for (int x = 0; x < 4; x++) sum += c[x] = count[4 * threadIdx.x + x];
-        int y = sum;
-#pragma unroll
-        for (int o = 1; o < kWave; o *= 2) {
-          const int z = __shfl_up(y, o);
-          if ((int)threadIdx.x >= o) y += z;
-        }
-        y -= sum;
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-          if (y < left && y + c[x] >= left) {
-            found = 4 * threadIdx.x + x;
-            under = y;
-          }
-          y += c[x];
-        }
+      const int c0 = count[2 * threadIdx.x], c1 = count[2 * threadIdx.x + 1];
+      const int y = before(c0 + c1, lds, &all);
+      if (y < left && y + c0 + c1 >= left) {
+        const bool second = y + c0 < left;
+        found = 2 * threadIdx.x + second;
+        under = y + (second ? c0 : 0);
       }
       __syncthreads();
       value |= (uint32_t)found << shift;
       left -= under;
     }
   }
-  int ties = 0, all;
+  int ties = 0;
 #pragma unroll
   for (int x = 0; x < E; x++) ties += d > 0 && i0 + x >= first && i0 + x < n - recent && key[x] == value;
   int tie = before(ties, lds, &all), gone = 0;
@@ -1259,44 +1390,45 @@ int cu_count8() {
   return n;
 }
 
-// How an attention call is cut: k_cache8_few (few 1), k_cache8_some with 16 or 32 rows per workgroup (4, 8) in so many groups, or
-// tiles of rows of k_cache8_tile (0); parts of the key axis of `chunk` blocks.
+// How an attention call is cut: k_cache8_few (rows 4), k_cache8_some (16, 32) in so many groups, or k_cache8_tile (128) in so many
+// tiles; parts of the key axis of at least `least` blocks; and workgroups that the CUs hold at once.
 struct Plan8 {
-  int few, groups, tiles, splits, chunk;
+  int rows, groups, splits, least, slots;
 };
 constexpr int kFewRows8 = 32;
 
 Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   Plan8 p{};
   const long long pairs = (long long)a.nseq * a.NKV, G = a.NH / a.NKV, rows = a.max_q * G, blocks = (a.max_k + kKeys - 1) / kKeys;
-  long long chunk;
-  if (rows <= kFewRows8 || weigh) {
-    p.few = rows <= 4 ? 1 : rows <= 16 ? 4 : 8;
-    p.groups = (int)((rows + 4 * p.few - 1) / (4 * p.few));
-    chunk = blocks * pairs * p.groups / ((p.few == 1 ? 4 : 2) * cu_count8());
-    chunk = max(min(chunk, (long long)32), (long long)4);
-  } else {
-    p.tiles = (int)((rows + kTileRows8 - 1) / kTileRows8);
-    const long long filled = min(pairs * p.tiles, (a.rows_q * G / kTileRows8 + a.nseq) * a.NKV);
-    chunk = filled >= 2 * cu_count8() ? blocks : max(blocks * filled / (8 * cu_count8()), (long long)8);
+  p.rows = rows <= 4 ? 4 : rows <= 16 ? 16 : rows <= kFewRows8 || weigh ? 32 : kTileRows8;
+  p.groups = (int)((rows + p.rows - 1) / p.rows);
+  const bool narrow = a.HS <= 64;
+  p.slots = cu_count8() * (p.rows == 4 ? 4 : p.rows == kTileRows8 ? (narrow ? 3 : 2) : (narrow ? 4 : 2));
+  // the shares of so many blocks, were all sequences full
+  const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / p.slots;
+  long long least = max(min(share / 2, blocks / 2), 4LL);
+  // few blocks are not worth a look at all sequences, nor are many groups, which fill the CUs
+  if (blocks <= 32 || jobs > 4LL * p.slots || blocks * pairs * p.groups > 1 << 30) {
+    p.slots = 0;
+    least = max(share, 4LL);
   }
   // what a workspace of the same rows and heads has for the fp32 attention
-  const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / ((a.HS + 2) * sizeof(float));
+  const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / ((a.HS + 2) * sizeof(float)) - 1;
   const long long fit = max((long long)(most / max((size_t)a.rows_q * a.NH, (size_t)1)), 1LL);
-  p.chunk = (int)max(max(chunk, (blocks + fit - 1) / fit), 1LL);
-  p.splits = (int)max((blocks + p.chunk - 1) / p.chunk, 1LL);
+  p.least = (int)max(max(least, (blocks + fit - 1) / fit), 1LL);
+  p.splits = (int)max((blocks + p.least - 1) / p.least, 1LL);
+  if (p.splits == 1) p.slots = 0;
   return p;
 }
-bool has_parts(const Plan8 &p, bool weigh) { return p.splits > 1 || weigh; }
 size_t parts_rows(const ugk_cache8 &a, const Plan8 &p) { return (size_t)p.splits * a.rows_q * a.NH; }
 size_t even(size_t n) { return (n + 1) / 2 * 2; }
 }  // namespace
 
 size_t cache8_attention_bytes(const ugk_cache8 &a, bool weigh) {
   const Plan8 p = plan8(a, weigh);
-  if (!has_parts(p, weigh)) return 0;
+  const size_t parts = p.splits > 1 ? even(parts_rows(a, p) * (a.HS + 2)) + 2 : 0;
   const size_t stat = (size_t)a.rows_q * a.NH, block = (size_t)a.nseq * a.max_q * a.NH * a.ld_table;
-  return (even(parts_rows(a, p) * (a.HS + 2)) + (weigh ? 2 * (stat + block) : 0)) * sizeof(float);
+  return (parts + (weigh ? 2 * (stat + block) : 0)) * sizeof(float);
 }
 
 int launch_cache8_attention(float *out, float *lse, const float *q, const void *k8, const float *ks, const void *v8,
@@ -1304,50 +1436,51 @@ int launch_cache8_attention(float *out, float *lse, const float *q, const void *
   const Plan8 p = plan8(a, weight);
   Parts8 parts{};
   parts.splits = p.splits;
-  parts.chunk = p.chunk;
-  if (has_parts(p, weight)) {
-    parts.m = mem;
+  parts.least = p.least;
+  parts.slots = p.slots;
+  if (p.splits > 1) {
+    parts.used = reinterpret_cast<int *>(mem);
+    parts.m = mem + 2;
     parts.l = parts.m + parts_rows(a, p);
     parts.o = parts.l + parts_rows(a, p);
-    if (weight) {
-      parts.stat = reinterpret_cast<float2 *>(mem + even(parts_rows(a, p) * (a.HS + 2)));
-      parts.block = parts.stat + (size_t)a.rows_q * a.NH;
-    }
+    mem += 2 + even(parts_rows(a, p) * (a.HS + 2));
+  }
+  if (weight) {
+    parts.stat = reinterpret_cast<float2 *>(mem);
+    parts.block = parts.stat + (size_t)a.rows_q * a.NH;
   }
   const unsigned pairs = (unsigned)a.nseq * a.NKV;
+  // as many parts in all as CUs, and one more for each group of rows, or all that there may be of each
+  const unsigned wgs = p.slots ? p.slots + pairs * p.groups : pairs * p.groups * p.splits;
   const int8_t *kc = static_cast<const int8_t *>(k8), *vc = static_cast<const int8_t *>(v8);
   const auto few = [&](auto kernel) {
-    launch(kernel, dim3(pairs * p.splits), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, word);
+    launch(kernel, dim3(wgs), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, word);
   };
   const auto some = [&](auto kernel) {
-    launch(kernel, dim3(pairs * p.groups * p.splits), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs,
+    launch(kernel, dim3(wgs), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs,
            (unsigned)p.groups, word);
   };
   const auto tile = [&](auto kernel) {
-    launch(kernel, dim3(pairs * p.tiles, p.splits), dim3(kTileThreads8), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, (unsigned)p.tiles,
+    launch(kernel, dim3(wgs), dim3(kTileThreads8), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, (unsigned)p.groups,
            word);
   };
   const int d = a.HS <= 32 ? 2 : a.HS <= 64 ? 4 : a.HS <= 96 ? 6 : 8;
-  switch (p.few) {
-    case 1: d == 2 ? few(k_cache8_few<2>) : d == 4 ? few(k_cache8_few<4>) : d == 6 ? few(k_cache8_few<6>) : few(k_cache8_few<8>); break;
-    case 4:
+  switch (p.rows) {
+    case 4: d == 2 ? few(k_cache8_few<2>) : d == 4 ? few(k_cache8_few<4>) : d == 6 ? few(k_cache8_few<6>) : few(k_cache8_few<8>); break;
+    case 16:
       d == 2 ? some(k_cache8_some<2, 1>) : d == 4 ? some(k_cache8_some<4, 1>) : d == 6 ? some(k_cache8_some<6, 1>) : some(k_cache8_some<8, 1>);
       break;
-    case 8:
+    case 32:
       d == 2 ? some(k_cache8_some<2, 2>) : d == 4 ? some(k_cache8_some<4, 2>) : d == 6 ? some(k_cache8_some<6, 2>) : some(k_cache8_some<8, 2>);
       break;
     default: d == 2 ? tile(k_cache8_tile<2>) : d == 4 ? tile(k_cache8_tile<4>) : d == 6 ? tile(k_cache8_tile<6>) : tile(k_cache8_tile<8>);
   }
   if (int e = check_launch("cache8_attention")) return e;
-  if (parts.o) {
-    launch(k_cache8_join, dim3(grid_for((size_t)a.nseq * a.max_q * a.NH, kBlock / kWave)), dim3(kBlock), 0, out, lse, parts, a);
-    if (int e = check_launch("cache8_attention")) return e;
-  }
-  if (weight) {
-    launch(k_cache8_weights, dim3((unsigned)a.nseq * ((a.ld_table + 15) / 16)), dim3(kBlock), 0, weight, parts, a);
-    return check_launch("cache8_attention");
-  }
-  return UGK_OK;
+  const unsigned joins = parts.o ? pairs * grid_for((size_t)a.max_q * (a.NH / a.NKV), 4) : 0;
+  const unsigned weighs = weight ? (unsigned)a.nseq * ((a.ld_table + 15) / 16) : 0;
+  if (joins + weighs == 0) return UGK_OK;
+  launch(k_cache8_finish, dim3(joins + weighs), dim3(kBlock), 0, out, lse, weight, parts, a, p.rows, joins);
+  return check_launch("cache8_attention");
 }
 
 // Blocks that max_q rows of a sequence touch at most, wherever they begin.

@@ -65,8 +65,9 @@ struct Row {
   }
 };
 
-// Sequence b's drafts, a lane of every wavefront to each, until one is not accepted.
-__device__ Row verify(const float *p, const float *q, const int *draft, const int *n_draft, const float *u, int b, int K, int V) {
+// Sequence b's drafts, a lane of every wavefront to each, until one is not accepted; or, if `accepted`, as many as that says.
+__device__ Row verify(const float *p, const float *q, const int *draft, const int *n_draft, const float *u, const int *accepted, int b,
+                      int K, int V) {
   const int given = n_draft ? n_draft[b] : K, n = min(max(given, 0), K), lane = threadIdx.x & (kWave - 1);
   p += (size_t)b * (K + 1) * V;
   if (q) q += (size_t)b * K * V;
@@ -75,8 +76,8 @@ __device__ Row verify(const float *p, const float *q, const int *draft, const in
   Row r;
   r.bad = given != n;
   r.n = n;
-  int a = 0;
-  for (; a < n; a += kWave) {
+  int a = accepted ? accepted[b] : 0;
+  for (; a < n && !accepted; a += kWave) {
     const int i = a + lane;
     bool no = i < n;
     if (no) {
@@ -101,12 +102,13 @@ __device__ Row verify(const float *p, const float *q, const int *draft, const in
   return r;
 }
 
-// The sums of the segments of every sequence's row, one per workgroup, where one workgroup per sequence would leave most CUs idle.
-__global__ __launch_bounds__(kSumThreads) void k_draft_sums(double *sums, const float *p, const float *q, const int *draft,
+// The sums of the segments of every sequence's row, one per workgroup, where one workgroup per sequence would leave most CUs idle; and the
+// accepted drafts, for the launch behind this one.
+__global__ __launch_bounds__(kSumThreads) void k_draft_sums(double *sums, int *accepted, const float *p, const float *q, const int *draft,
                                                            const int *n_draft, const float *u, int K, int V, int segs, int seg) {
   __shared__ double part[kSumThreads / kWave];
   const int b = blockIdx.x / segs, s = blockIdx.x % segs;
-  const Row r = verify(p, q, draft, n_draft, u, b, K, V);
+  const Row r = verify(p, q, draft, n_draft, u, nullptr, b, K, V);
   const int from = s * seg, to = min(from + seg, V);
   double t[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 1
@@ -122,7 +124,10 @@ __global__ __launch_bounds__(kSumThreads) void k_draft_sums(double *sums, const 
   const double sum = wave_sum64((t[0] + t[1]) + (t[2] + t[3]));
   if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+  if (threadIdx.x == 0) {
+    sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+    if (s == 0) accepted[b] = r.a;
+  }
 }
 
 struct DrawLds {
@@ -240,7 +245,7 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_verify(int *accepted, i
                                                                int segs, int seg, int *word) {
   __shared__ DrawLds lds;
   const int b = blockIdx.x;
-  Row r = verify(p, q, draft, n_draft, u, b, K, V);
+  Row r = verify(p, q, draft, n_draft, u, sums ? accepted : nullptr, b, K, V);
   const double x = u[(size_t)b * (K + 1) + K];
   int token = draw(r, V, segs, seg, x, sums ? sums + (size_t)b * segs : nullptr, lds);
   if (token < 0 && r.a < r.n) {  // p and q are the same
@@ -278,7 +283,7 @@ int launch_draft_verify(int *accepted, int *tokens, const float *p, const float 
                         const float *u, double *sums, int nseq, int K, int V, int *word) {
   const int seg = seg_floats(V), segs = (int)(((long long)V + seg - 1) / seg);
   if (sums) {
-    launch(k_draft_sums, dim3((unsigned)nseq * segs), dim3(kSumThreads), 0, sums, p, q, draft, n_draft, u, K, V, segs, seg);
+    launch(k_draft_sums, dim3((unsigned)nseq * segs), dim3(kSumThreads), 0, sums, accepted, p, q, draft, n_draft, u, K, V, segs, seg);
     if (int e = check_launch("draft_verify")) return e;
   }
   launch(k_draft_verify, dim3(nseq), dim3(kDraftThreads), 0, accepted, tokens, p, q, draft, n_draft, u, sums, K, V, segs, seg, word);

@@ -624,7 +624,8 @@ def _cache8(a: Cache8, k8, ks, v8, vs):
     if not _one_device:
         for t, name in zip(a._tensors, a._NAMES):
             _here(t, name)
-    n, scales = lib.ugk_cache8_bytes(a.nblocks, a.NKV, a.HS), a.nblocks * a.NKV
+    scales = a.nblocks * a.NKV
+    n = scales * CACHE8_BLOCK * ((a.HS + 15) & ~15)
     return (_ptr_here(k8, "k8", n, "i8"), _ptr_here(ks, "ks", scales), _ptr_here(v8, "v8", n, "i8"), _ptr_here(vs, "vs", scales))
 
 
