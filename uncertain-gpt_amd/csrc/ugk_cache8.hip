@@ -285,7 +285,8 @@ struct Parts8 {
   float *o, *m, *l;
   float2 *block, *stat;
   int *used;                 // the blocks per part of this call
-  int splits, least, slots;  // parts of the longest axis, the fewest blocks per part, workgroups that the CUs hold (0: `least` it is)
+  int splits, least;         // parts of the longest axis, the fewest blocks per part
+  int slots, cus;            // workgroups that the CUs hold (0: parts of `least` blocks), CUs
 };
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -324,31 +325,40 @@ struct Running {
   }
 };
 
-// N floats of a row of q from `at` on, 0 behind its HS, with the sign of the scores' scale; and the largest magnitude's bits.
-template <int N>
-__device__ __forceinline__ uint32_t load_q(const float *p, int at, const ugk_cache8 &a, float (&x)[N]) {
-  if (at + N <= a.HS) {
+// S times N floats of a row of q from `first` on, `step` apart, 0 behind its HS, with the sign of the scores' scale; and the largest
+// magnitude's bits. (One branch for all: a branch for each N would wait for its loads.)
+template <int S, int N>
+__device__ __forceinline__ uint32_t load_q(const float *p, int first, int step, const ugk_cache8 &a, float (&x)[S][N]) {
+  if (a.HS % 4 == 0) {
 #pragma unroll
-    for (int d = 0; d < N; d += 4) {
-      const float4 y = ld4(p + at + d);
-      x[d] = y.x;
-      x[d + 1] = y.y;
-      x[d + 2] = y.z;
-      x[d + 3] = y.w;
-    }
+    for (int s = 0; s < S; s++)
+#pragma unroll
+      for (int d = 0; d < N; d += 4) {
+        const int at = first + s * step + d;
+        const float4 y = ld4(p + min(at, a.HS - 4));
+        x[s][d] = at < a.HS ? y.x : 0.0f;
+        x[s][d + 1] = at < a.HS ? y.y : 0.0f;
+        x[s][d + 2] = at < a.HS ? y.z : 0.0f;
+        x[s][d + 3] = at < a.HS ? y.w : 0.0f;
+      }
   } else {
 #pragma unroll
-    for (int d = 0; d < N; d++) {
-      const float y = p[min(at + d, a.HS - 1)];
-      x[d] = at + d < a.HS ? y : 0.0f;
-    }
+    for (int s = 0; s < S; s++)
+#pragma unroll
+      for (int d = 0; d < N; d++) {
+        const int at = first + s * step + d;
+        const float y = p[min(at, a.HS - 1)];
+        x[s][d] = at < a.HS ? y : 0.0f;
+      }
   }
   uint32_t most = 0;
 #pragma unroll
-  for (int d = 0; d < N; d++) {
-    most = max(most, abs_bits(x[d]));
-    if (a.scale < 0.0f) x[d] = -x[d];
-  }
+  for (int s = 0; s < S; s++)
+#pragma unroll
+    for (int d = 0; d < N; d++) {
+      most = max(most, abs_bits(x[s][d]));
+      if (a.scale < 0.0f) x[s][d] = -x[s][d];
+    }
   return most;
 }
 
@@ -378,6 +388,10 @@ __device__ __forceinline__ float max16(float v) {
   return fmaxf(v, dpp_lane<kDppMirror>(v));
 }
 
+// x 2^p, at most 2^30 but for infinities and NaN, as a whole number.
+__device__ __forceinline__ int whole(float x, int p) {
+  return (int)rintf(fminf(fmaxf(__builtin_amdgcn_ldexpf(x, p), -0x1p30f), 0x1p30f));
+}
 // A whole number of up to 2^30 as four digits of base 256 in [-128, 127], a byte each.
 __device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x00808080u) ^ 0x00808080u; }
 // The number whose digits' sums of products are d (each below 2^21): exact but for the roundings to float.
@@ -520,18 +534,25 @@ __device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts,
   int chunk = parts.least;
   w.none = true;
   if (parts.slots) {
-    int blocks = 0, jobs = 0;
+    int blocks = 0, jobs = 0, longest = 0;
     Seq8 s{0, 0, 0};  // the lane's of the last 64 sequences, which are mostly all
     for (int b = lane; b < a.nseq; b += kWave) {
       s = sequence8(a, b, blockIdx.x == 0, word, UGK_IDS_CACHE8_ATTENTION);
       const int n = (s.Lq * G + R - 1) / R;
       jobs += n;
-      for (int t = 0; t < n; t++) blocks += blocks_of(s, a, G, R, t);
+      for (int t = 0; t < n; t++) {
+        const int nb = blocks_of(s, a, G, R, t);
+        blocks += nb;
+        longest = max(longest, nb);
+      }
     }
+    longest = (int)wave_max_bits((uint32_t)longest);
     jobs = wave_sum_int(jobs) * a.NKV;
     blocks = wave_sum_int(blocks) * a.NKV;
     const int left = 2 * jobs < parts.slots ? parts.slots - jobs : parts.slots;
     chunk = __builtin_amdgcn_readfirstlane(max(chunk, (blocks + left - 1) / left));
+    // no group has much more than a CU's share: the parts' way through memory would cost more than they save
+    if ((long long)2 * longest * parts.cus <= 3LL * blocks) chunk = max(chunk, longest);
     if (blockIdx.x == 0 && threadIdx.x == 0) *parts.used = chunk;
     // the sequence, then the group and the part that are number x of all
     int x = blockIdx.x, b = -1;
@@ -588,8 +609,9 @@ __device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts,
   const int nb = blocks_of(w.s, a, G, R, w.group), n = parts.o ? parts_for(nb, chunk) : 1;
   w.whole = n == 1;
   w.none = w.part >= n;
-  w.first = (int)((long long)nb * w.part / n);
-  w.stop = (int)((long long)nb * (w.part + 1) / n);
+  const int each = nb / n, longer = nb - each * n;  // the first ones are one longer
+  w.first = w.part * each + min(w.part, longer);
+  w.stop = w.first + each + (w.part < longer);
   return w;
 }
 
@@ -600,7 +622,7 @@ __device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts,
 // head, their sums are exact, and a lane finds the four digits of its score in its own four registers.
 // The weights, 31 bits next to the block's largest, go the same way into the product with the values.
 template <int DT>
-__global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8,
+__global__ __launch_bounds__(kFewWaves *kWave, DT >= 6 ? 3 : 4) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8,
                                                                    const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
                                                                    Parts8 parts, unsigned pairs, int *word) {
   constexpr int KS = (DT + 3) / 4, kStride = 20;
@@ -634,9 +656,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_fe
     const int rr = min(col >> 2, rows - 1);
     const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (size_t)(hk * G + rr % G) * a.HS;
     float x[KS][16];
-    uint32_t most = 0;
-#pragma unroll
-    for (int st = 0; st < KS; st++) most = max(most, load_q(p, 64 * st + 16 * quad, a, x[st]));
+    uint32_t most = load_q(p, 16 * quad, 64, a, x);
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
     most = max(most, (uint32_t)__shfl_xor((int)most, 32));
     const int e = (int)(most >> 23) - 127;  // below 2^(e + 1)
@@ -645,10 +665,9 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_fe
       aq[st] = v4i{0, 0, 0, 0};
 #pragma unroll
       for (int d = 0; d < 16; d++) {
-        const uint32_t y = digits((int)rintf(__builtin_amdgcn_ldexpf(x[st][d], 29 - e)));
+        const uint32_t y = digits(whole(x[st][d], 29 - e));
         aq[st][d / 4] |= (int)((y >> (8 * (lane & 3)) & 255u) << (8 * (d & 3)));
       }
-      if (most >= kInfBits) aq[st] = v4i{0, 0, 0, 0};
     }
     // for the lanes that hold the row's scores: row quad
     ex = __shfl(e, 4 * quad) - 29;
@@ -683,14 +702,14 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_fe
       vscale = vs[ahead];
     }
     mb = top_score(max16(mb), fac);
-    const float less = less_top(mb, 30.0f);  // weights times 2^30
+    const float less = less_top(mb, 0.0f);
     uint32_t y[4];
     float lb = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < 4; kt++) {
       p[kt] = ex2(fmaf(p[kt], fac, less));
       lb += p[kt];
-      y[kt] = digits((int)p[kt]);
+      y[kt] = digits((int)(p[kt] * 0x1p30f));  // (2^30 in the exponent would cost the weights four bits)
     }
     const v4i t = turn4(y[0], y[1], y[2], y[3]);  // the four keys' digits side by side: a word per digit
     uint32_t *w = mylp + 4 * quad * kStride + col;
@@ -699,7 +718,6 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT == 6 ? 3 : 4) void k_cache8_fe
     __builtin_amdgcn_wave_barrier();
     const v4i ap = *reinterpret_cast<const v4i *>(mylp + col * kStride + 4 * quad);
     __builtin_amdgcn_wave_barrier();
-    lb *= 0x1p-30f;
     if (parts.block) {
       const float sum = sum16(lb);
       if (col == 0 && quad < rows)
@@ -802,9 +820,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
     const int rr = min(mine, rows - 1);
     const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (size_t)(hk * G + rr % G) * a.HS;
     float x[KS][16];
-    uint32_t most = 0;
-#pragma unroll
-    for (int st = 0; st < KS; st++) most = max(most, load_q(p, 64 * st + 16 * quad, a, x[st]));
+    uint32_t most = load_q(p, 16 * quad, 64, a, x);
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
     most = max(most, (uint32_t)__shfl_xor((int)most, 32));
     nan = most >= kInfBits;
@@ -815,7 +831,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
       for (int d = 0; d < 16; d += 4) {
         uint32_t y[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) y[r] = digits((int)rintf(__builtin_amdgcn_ldexpf(nan ? 0.0f : x[st][d + r], -ex)));
+        for (int r = 0; r < 4; r++) y[r] = digits(whole(x[st][d + r], -ex));
         const v4i t = turn4(y[0], y[1], y[2], y[3]);
 #pragma unroll
         for (int r = 0; r < 4; r++) aq[st][r][d / 4] = t[r];
@@ -869,7 +885,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
       vscale = vs[ahead];
     }
     mb = top_score(quarters_max(mb), fac);
-    const float less = less_top(mb, 30.0f);
+    const float less = less_top(mb, 0.0f);
     float lb = 0.0f;
     v4i bp[4];
 #pragma unroll
@@ -879,13 +895,12 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
       for (int kt = 0; kt < 4; kt++) {
         const float x = ex2(fmaf(p[kt][r], fac, less));
         lb += x;
-        y[kt] = digits((int)x);
+        y[kt] = digits((int)(x * 0x1p30f));
       }
       const v4i t = turn4(y[0], y[1], y[2], y[3]);
 #pragma unroll
       for (int d = 0; d < 4; d++) bp[d][r] = t[d];
     }
-    lb *= 0x1p-30f;
     if (parts.block) {
       const float sum = quarters_sum(lb);
       if (quad == 0 && mine < rows)
@@ -1102,10 +1117,7 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
   {
     const float *p = q + ((size_t)s.q0 + i) * a.ldq + (size_t)h * a.HS;
     float x[DT][8];
-    uint32_t most = 0;
-#pragma unroll
-    for (int st = 0; st < DT; st++) most = max(most, load_q(p, 16 * st + 8 * half, a, x[st]));
-    most = half_max_bits(most);
+    const uint32_t most = half_max_bits(load_q(p, 8 * half, 16, a, x));
     nan = most >= kInfBits;
     e = (int)(most >> 23) - 126 - 15;  // below 2^15 2^e
 #pragma unroll
@@ -1403,14 +1415,15 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   p.rows = rows <= 4 ? 4 : rows <= 16 ? 16 : rows <= kFewRows8 || weigh ? 32 : kTileRows8;
   p.groups = (int)((rows + p.rows - 1) / p.rows);
   const bool narrow = a.HS <= 64;
-  p.slots = cu_count8() * (p.rows == 4 ? 4 : p.rows == kTileRows8 ? (narrow ? 3 : 2) : (narrow ? 4 : 2));
+  p.slots = cu_count8() * (p.rows == 4 ? (narrow ? 4 : 3) : p.rows == kTileRows8 ? (narrow ? 3 : 2) : (narrow ? 4 : 2));
   // the shares of so many blocks, were all sequences full
   const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / p.slots;
   long long least = max(min(share / 2, blocks / 2), 4LL);
   // few blocks are not worth a look at all sequences, nor are many groups, which fill the CUs
   if (blocks <= 32 || jobs > 4LL * p.slots || blocks * pairs * p.groups > 1 << 30) {
     p.slots = 0;
-    least = max(share, 4LL);
+    // with weights to add up, the launch that joins parts is there anyway
+    least = 3 * jobs >= 2LL * cu_count8() && !weigh ? blocks : max(share, 4LL);
   }
   // what a workspace of the same rows and heads has for the fp32 attention
   const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / ((a.HS + 2) * sizeof(float)) - 1;
@@ -1438,6 +1451,7 @@ int launch_cache8_attention(float *out, float *lse, const float *q, const void *
   parts.splits = p.splits;
   parts.least = p.least;
   parts.slots = p.slots;
+  parts.cus = cu_count8();
   if (p.splits > 1) {
     parts.used = reinterpret_cast<int *>(mem);
     parts.m = mem + 2;
