@@ -28,8 +28,9 @@
  * workspace beyond their arguments: the LayerNorm backward's partial column
  * sums (one slot per call, 2L+1 for the step driver), the encoder backward's
  * bucket state, the KL total's partial sums, the softmax's row
- * statistics (rows too long for one workgroup, and the exact mode's), and
- * attention's row sums and parts of a split axis, each in a region of its own. By
+ * statistics (rows too long for one workgroup, and the exact mode's),
+ * attention's row sums and parts of a split axis, and the sums of the rows that
+ * drafts are verified against, each in a region of its own. By
  * default the library allocates a region on the first call that needs it and grows
  * it, after waiting for the device, when a larger shape arrives; ugk_reserve /
  * ugk_reserve_config allocate everything up front, after which calls at those
@@ -503,15 +504,21 @@ int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks,
 
 /* ugk_attention_forward of q against the cache: out, and lse (rows_q, NH) if not
  * NULL. A row without a key that it sees has out 0 and lse -infinity. A row of q (of one
- * head) enters as whole numbers of 31 bits next to its largest element, or, with more than 32 query rows
- * times heads per key/value head, as two half-precision numbers per element, to 2^-23 of the
- * element and 2^-38 of the largest; weights to 2^-31, or to 2^-23 of the weight and 2^-38 of the largest of
- * their block; statistics and sums are in single precision. A score of 2^127 or more, and a row of q
- * with an infinity or NaN, has the row's out and lse NaN. out must not overlap q.
- * weight, if not NULL, (nseq, ld_table): weight[b, j] += the sum of the weights, over
- * sequence b's rows and heads and the keys of its block j. For up to 256 rows and heads per
- * key/value head: tokens, drafts, or the last rows of a prompt. Deterministic. The
- * workspace for it is 8 bytes per row, head and block. */
+ * head) enters as whole numbers of 31 bits next to its largest element and the
+ * weights as such next to the largest of their block; or, with more than 32 query
+ * rows times heads per key/value head and no `weight`, both as two half-precision
+ * numbers, q to 2^-23 of the element and 2^-38 of the largest, weights to 2^-23
+ * of the weight and 2^-38 of the largest contribution (weight times the values'
+ * scale) that the row sees. Products with the codes are exact, statistics and sums
+ * in single precision. A score of about 2^127 or more, or an infinity or NaN in its row
+ * of q, makes a row's out and lse NaN; one of about -2^127 or less weighs nothing. out
+ * must not overlap q.
+ * weight, if not NULL, (nseq, ld_table): weight[b, j] += the sum of the weights over
+ * sequence b's rows and heads and the keys of its block j. For up to 256 query rows
+ * times heads per key/value head: tokens, drafts, or the last rows of a prompt. It
+ * takes 8 bytes of workspace per row, head and block. Deterministic: the same call
+ * gives the same bits. The workspace is attention's: a config's of as many rows and
+ * heads has what calls without `weight` need. */
 int ugk_cache8_attention(float *out, float *lse, const float *q, const void *k8,
                          const float *ks, const void *v8, const float *vs,
                          float *weight, ugk_cache8 a);

@@ -469,6 +469,47 @@ def test_split_key_axes(gpu, nseq, lq, NH, NKV, HS, cap):
         check(gpu, c, NH, q, starts, [lq] * nseq, keys, rows, weigh=True)
 
 
+@pytest.mark.parametrize("lq,NH,NKV,HS", [(1, 2, 2, 16), (3, 4, 1, 64), (7, 4, 2, 33), (40, 2, 1, 64)])
+@pytest.mark.parametrize("nseq", [5, 64, 131])
+def test_many_sequences_of_very_different_lengths(gpu, nseq, lq, NH, NKV, HS):
+    """Parts dealt out by what the sequences hold: some have no rows, some no keys, few have almost all of them."""
+    g = torch.Generator().manual_seed(nseq + lq)
+    cap = 2500
+    keys = [0 if r < 0.1 else int(cap ** r) for r in torch.rand(nseq, generator=g).tolist()]
+    keys[-1] = cap
+    lens = [0 if r < 0.2 else max(1, int(lq * r)) for r in torch.rand(nseq, generator=g).tolist()]
+    lens[-1] = lens[0] = lq
+    c, gg = filled(gpu, nseq, cap, NKV, HS, keys, seed=nseq)
+    starts, rows = place_rows(lens)
+    q = rand(gg, rows, NH, HS)
+    out, L, _ = check(gpu, c, NH, q, starts, lens, keys, rows, max_q=lq)
+    again, L2, _ = check(gpu, c, NH, q, starts, lens, keys, rows, max_q=lq)
+    assert torch.equal(out, again) and torch.equal(L, L2)
+    check(gpu, c, NH, q, starts, lens, keys, rows, causal=False, max_q=lq)
+    if lq * NH // NKV <= 256:
+        check(gpu, c, NH, q, starts, lens, keys, rows, weigh=True, max_q=lq)
+
+
+def test_many_groups_of_rows_in_a_sequence(gpu):
+    """More than 64 workgroups' rows in one sequence, whose key axis is cut all the same."""
+    NH, NKV, HS, lq, n = 8, 1, 16, 1100, 2400
+    c, g = filled(gpu, 2, n, NKV, HS, [n, 70])
+    starts, rows = place_rows([lq, 3])
+    q = rand(g, rows, NH, HS)
+    check(gpu, c, NH, q, starts, [lq, 3], [n, 70], rows)
+
+
+@pytest.mark.parametrize("lq", [1, 5, 40])
+def test_scores_far_below_zero(gpu, lq):
+    """Blocks of which a row sees nothing, next to scores of -1,000 and less."""
+    NH, NKV, HS, n = 2, 1, 64, 450  # the rows lie on both sides of the border at 448
+    c, g = filled(gpu, 1, n, NKV, HS, [n], size=lambda k, v: k.abs_().add_(1.0))
+    q = -rand(g, lq, NH, HS).abs() - 2.0
+    check(gpu, c, NH, q, [0], [lq], [n], lq, scale=8.0)
+    check(gpu, c, NH, q, [0], [lq], [n], lq, scale=8.0, weigh=True)
+    check(gpu, c, NH, -q, [0], [lq], [n], lq, scale=-8.0)
+
+
 def test_captured_and_on_another_stream(gpu):
     """Store, attention with weights and eviction in a graph, replayed between eager calls on another stream."""
     NH, NKV, HS, cap, nseq = 4, 2, 64, 500, 3

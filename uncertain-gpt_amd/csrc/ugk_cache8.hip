@@ -123,26 +123,35 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
   const long long ld = values ? a.ldv : a.ldk;
   const float *src = (values ? v : k) + (long long)(t.q - t.r0) * ld + t.h * a.HS;
   const int id = block_of(a, t.b, t.j, word, UGK_IDS_CACHE8_STORE);  // on its way while the rows are
+  // What lies outside the call's rows and the head is read from the nearest that does not, and taken as 0: a branch would wait
+  // for each of these loads.
   float4 x[kPer][4];
-  uint32_t most = 0;
+  const auto mine = [&](int i, int r, auto &&take) {
+    const int e = threadIdx.x + i * kBlock, d = e % G * 4, row = e / G + 16 * r;
+    take(src + min(max(row, t.r0), t.r1 - 1) * ld, d, e / G < 16 && row >= t.r0 && row < t.r1, x[i][r]);
+  };
+  if (a.HS % 4 == 0) {
 #pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    const int e = threadIdx.x + i * kBlock, g = e % G, c = e / G, nd = a.HS - 4 * g;
+    for (int i = 0; i < kPer; i++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      x[i][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const int row = c + 16 * r;
-      if (c >= 16 || row < t.r0 || row >= t.r1 || nd <= 0) continue;
-      const float *p = src + row * ld + 4 * g;
-      if (nd >= 4) {
-        x[i][r] = ld4(p);
-      } else {
-        x[i][r].x = p[0];
-        if (nd > 1) x[i][r].y = p[1];
-        if (nd > 2) x[i][r].z = p[2];
-      }
-    }
+      for (int r = 0; r < 4; r++)
+        mine(i, r, [&](const float *p, int d, bool in, float4 &y) {
+          const float4 z = ld4(p + min(d, a.HS - 4));
+          in = in && d < a.HS;
+          y = make_float4(in ? z.x : 0.0f, in ? z.y : 0.0f, in ? z.z : 0.0f, in ? z.w : 0.0f);
+        });
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        mine(i, r, [&](const float *p, int d, bool in, float4 &y) {
+          const float z0 = p[min(d, a.HS - 1)], z1 = p[min(d + 1, a.HS - 1)], z2 = p[min(d + 2, a.HS - 1)], z3 = p[min(d + 3, a.HS - 1)];
+          y = make_float4(in && d < a.HS ? z0 : 0.0f, in && d + 1 < a.HS ? z1 : 0.0f, in && d + 2 < a.HS ? z2 : 0.0f,
+                          in && d + 3 < a.HS ? z3 : 0.0f);
+        });
   }
+  uint32_t most = 0;
   if (id < 0) return;
   const size_t at = (size_t)id * a.NKV + t.h;
   float *sp = (values ? vs : ks) + at;
@@ -250,23 +259,29 @@ __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, cons
   const size_t at = (size_t)id * a.NKV + t.h;
   const float s = (values ? vs : ks)[at];
   const uint32_t *src = reinterpret_cast<const uint32_t *>((values ? v8 : k8) + at * kKeys * HP);
+  uint32_t w[CH];
+#pragma unroll
+  for (int i = 0; i < CH; i++) w[i] = src[threadIdx.x + i * kBlock];
   if (values) {
-    for (int e = threadIdx.x; e < HP * 16; e += kBlock) tile[e / 16 * 17 + e % 16] = src[e];
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int e = threadIdx.x + i * kBlock;
+      tile[e / 16 * 17 + e % 16] = w[i];
+    }
     __syncthreads();
   }
-  for (int e = threadIdx.x + t.r0 * G; e < t.r1 * G; e += kBlock) {
-    const int row = e / G, g = e % G, nd = a.HS - 4 * g;
-    if (nd <= 0) continue;
-    uint32_t w;
+#pragma unroll
+  for (int i = 0; i < CH; i++) {
+    const int e = threadIdx.x + i * kBlock, row = e / G, g = e % G, nd = a.HS - 4 * g;
+    if (row < t.r0 || row >= t.r1 || nd <= 0) continue;
     if (values) {
-      const int c = row & 15, r = row >> 4;
-      w = pack4(code_at(tile[(4 * g) * 17 + c], r), code_at(tile[(4 * g + 1) * 17 + c], r), code_at(tile[(4 * g + 2) * 17 + c], r),
-                code_at(tile[(4 * g + 3) * 17 + c], r));
-    } else {
-      w = src[e];
+      const uint32_t *p = tile + 4 * g * 17 + (row & 15);
+      const int r = row >> 4;
+      w[i] = pack4(code_at(p[0], r), code_at(p[17], r), code_at(p[34], r), code_at(p[51], r));
     }
     float *p = to + row * ld + 4 * g;
-    const float4 x = make_float4((float)code_at(w, 0) * s, (float)code_at(w, 1) * s, (float)code_at(w, 2) * s, (float)code_at(w, 3) * s);
+    const float4 x = make_float4((float)code_at(w[i], 0) * s, (float)code_at(w[i], 1) * s, (float)code_at(w[i], 2) * s,
+                                 (float)code_at(w[i], 3) * s);
     if (nd >= 4) {
       st4(p, x);
     } else {
@@ -596,7 +611,12 @@ __device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts,
     w.part = x / a.NKV;
     w.hk = x % a.NKV;
   } else {
-    const unsigned round = blockIdx.x / pairs, pair = (blockIdx.x % pairs + round) % pairs;
+    // Each CU gets one workgroup of every `cus`: of the first the longest, of the second the shortest first, and so on, so that all
+    // have much the same to do (8 x 1,024 rows of 12 heads of 64 in turn 49 us, the longest first throughout).
+    unsigned x = blockIdx.x;
+    const unsigned cus = (unsigned)parts.cus, lap = x / cus;
+    if (lap % 2 && (lap + 1) * cus <= gridDim.x) x = lap * cus + (cus - 1 - x % cus);
+    const unsigned round = x / pairs, pair = (x % pairs + round) % pairs;
     w.b = pair / a.NKV;
     w.hk = pair % a.NKV;
     w.part = round / groups;
@@ -1327,8 +1347,8 @@ __global__ __launch_bounds__(kEvictThreads) void k_cache8_evict(int *table_out, 
 #pragma unroll
   for (int x = 0; x < E; x++) {
     const int i = i0 + x;
-    id[x] = i < ld ? table[row + i] : 0;
-    w[x] = i < ld ? weight[row + i] : 0.0f;
+    id[x] = table[row + min(i, ld - 1)];  // without a branch, which would wait for each load
+    w[x] = weight[row + min(i, ld - 1)];
     // ascending in the weight; NaN, whatever its sign, above all
     const uint32_t u = __float_as_uint(w[x] + 0.0f);
     key[x] = w[x] != w[x] ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;

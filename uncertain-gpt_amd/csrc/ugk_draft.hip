@@ -42,26 +42,51 @@ struct Row {
     const double d = (double)x - (double)y;
     return v != gone && d > 0.0 && d <= 3.402823466e38 ? d : 0.0;
   }
-  // tokens v .. v + 3, those from `end` on 0
-  __device__ __forceinline__ void four(int v, int end, double (&x)[4]) const {
-    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f), g = f;
-    if (v + 4 <= end) {
-      f = ld4(p + v);
-      if (less) g = ld4(less + v);
-    } else if (v < end) {
-      f.x = p[v];
-      if (v + 1 < end) f.y = p[v + 1];
-      if (v + 2 < end) f.z = p[v + 2];
+  // N times four tokens, v0 .. v0 + 3, `step` apart, those from `end` on 0. whole: all of the wavefront's are before it. (All loads
+  // before the first use: a branch around each would wait for it.)
+  template <int N>
+  __device__ __forceinline__ void quads(int v0, int step, int end, bool whole, double (&x)[N][4]) const {
+    float4 f[N], g[N];
+    if (whole && less) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        f[i] = ld4(p + v0 + i * step);
+        g[i] = ld4(less + v0 + i * step);
+      }
+    } else if (whole) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        f[i] = ld4(p + v0 + i * step);
+        g[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+    } else {
+      const int last = end - 1;
+      const auto at = [&](const float *q, int v) {
+        return make_float4(q[min(v, last)], q[min(v + 1, last)], q[min(v + 2, last)], q[min(v + 3, last)]);
+      };
+#pragma unroll
+      for (int i = 0; i < N; i++) f[i] = at(p, v0 + i * step);
+#pragma unroll
+      for (int i = 0; i < N; i++) g[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (less) {
-        g.x = less[v];
-        if (v + 1 < end) g.y = less[v + 1];
-        if (v + 2 < end) g.z = less[v + 2];
+#pragma unroll
+        for (int i = 0; i < N; i++) g[i] = at(less, v0 + i * step);
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int v = v0 + i * step;
+        f[i] = make_float4(v < end ? f[i].x : 0.0f, v + 1 < end ? f[i].y : 0.0f, v + 2 < end ? f[i].z : 0.0f, v + 3 < end ? f[i].w : 0.0f);
+        g[i] = make_float4(v < end ? g[i].x : 0.0f, v + 1 < end ? g[i].y : 0.0f, v + 2 < end ? g[i].z : 0.0f, v + 3 < end ? g[i].w : 0.0f);
       }
     }
-    x[0] = one(f.x, g.x, v);
-    x[1] = one(f.y, g.y, v + 1);
-    x[2] = one(f.z, g.z, v + 2);
-    x[3] = one(f.w, g.w, v + 3);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int v = v0 + i * step;
+      x[i][0] = one(f[i].x, g[i].x, v);
+      x[i][1] = one(f[i].y, g[i].y, v + 1);
+      x[i][2] = one(f[i].z, g[i].z, v + 2);
+      x[i][3] = one(f[i].w, g[i].w, v + 3);
+    }
   }
 };
 
@@ -114,8 +139,7 @@ __global__ __launch_bounds__(kSumThreads) void k_draft_sums(double *sums, int *a
 #pragma unroll 1
   for (int v0 = from; v0 < to; v0 += kStep) {
     double x[kStep / (4 * kSumThreads)][4];
-#pragma unroll
-    for (int i = 0; i < kStep / (4 * kSumThreads); i++) r.four(v0 + 4 * ((int)threadIdx.x + i * kSumThreads), to, x[i]);
+    r.quads(v0 + 4 * (int)threadIdx.x, 4 * kSumThreads, to, v0 + kStep <= to, x);
 #pragma unroll
     for (int i = 0; i < kStep / (4 * kSumThreads); i++)
 #pragma unroll
@@ -154,8 +178,7 @@ __device__ int draw(const Row &r, int V, int segs, int seg, double u, const doub
 #pragma unroll 1
         for (int v0 = from; v0 < to; v0 += 16 * kWave) {
           double x[4][4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) r.four(v0 + 4 * (lane + i * kWave), to, x[i]);
+          r.quads(v0 + 4 * lane, 4 * kWave, to, v0 + 16 * kWave <= to, x);
 #pragma unroll
           for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -194,8 +217,9 @@ __device__ int draw(const Row &r, int V, int segs, int seg, double u, const doub
   int token = -1;
   for (int v0 = begin; v0 < end; v0 += kStep) {
     const int v = v0 + 4 * (int)threadIdx.x;
-    double x[4];
-    r.four(v, end, x);
+    double y[1][4];
+    r.quads(v, 0, end, v0 + kStep <= end, y);
+    const double (&x)[4] = y[0];
     const double mine = (x[0] + x[1]) + (x[2] + x[3]), up = wave_scan64(mine);
     __syncthreads();  // the last step's have been read
     if (lane == kWave - 1) lds.wave[wave] = up;
