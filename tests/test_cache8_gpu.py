@@ -490,6 +490,25 @@ def test_many_sequences_of_very_different_lengths(gpu, nseq, lq, NH, NKV, HS):
         check(gpu, c, NH, q, starts, lens, keys, rows, weigh=True, max_q=lq)
 
 
+@pytest.mark.parametrize("nseq,lq,NH,NKV,HS,cap,equal", [(100, 1, 16, 16, 16, 2200, False), (40, 1, 16, 16, 16, 2600, True),
+                                                         (3, 300, 3, 1, 80, 3000, False), (20, 9, 14, 2, 33, 2100, False),
+                                                         (6, 130, 5, 1, 128, 4500, False), (1, 4, 1, 1, 64, 2113, True)])
+def test_blocks_dealt_out_in_equal_shares(gpu, nseq, lq, NH, NKV, HS, cap, equal):
+    """More groups of rows than workgroups, groups that are each a workgroup's, heads of groups that are no power of two, rows
+    before the first key, many short sequences in one workgroup."""
+    g = torch.Generator().manual_seed(cap + nseq)
+    keys = [cap if equal else max(1, int(cap ** r)) for r in torch.rand(nseq, generator=g).tolist()]
+    keys[-1] = cap
+    lens = [max(1, lq - b % 3) for b in range(nseq)]
+    c, gg = filled(gpu, nseq, cap, NKV, HS, keys, seed=nseq)
+    starts, rows = place_rows(lens)
+    q = rand(gg, rows, NH, HS)
+    check(gpu, c, NH, q, starts, lens, keys, rows, max_q=lq)
+    check(gpu, c, NH, q, starts, lens, keys, rows, causal=False, max_q=lq)
+    if lq * NH // NKV <= 256:
+        check(gpu, c, NH, q, starts, lens, keys, rows, weigh=True, max_q=lq)
+
+
 def test_many_groups_of_rows_in_a_sequence(gpu):
     """More than 64 workgroups' rows in one sequence, whose key axis is cut all the same."""
     NH, NKV, HS, lq, n = 8, 1, 16, 1100, 2400

@@ -294,15 +294,23 @@ __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, cons
 
 // ---- attention --------------------------------------------------------------------
 
-// Parts of the key axis: o normalised, the maximum m of its scores in base 2 and the sum l of 2^(s - m), per row and head;
+// Parts of the key axis: o normalised, the maximum m of its scores in base 2 and the sum l of 2^(s - m), per slot and row of a group;
 // `block`: the same m and l of each block of 64 keys, and `stat` of rows that have no parts (for the blocks' weights).
 struct Parts8 {
-  float *o, *m, *l;
-  float2 *block, *stat;
-  int *used;                 // the blocks per part of this call
-  int splits, least;         // parts of the longest axis, the fewest blocks per part
-  int slots, cus;            // workgroups that the CUs hold (0: parts of `least` blocks), CUs
+  float *o;
+  float2 *ml, *block, *stat;
+  int2 *job;           // of a sequence, key/value head and group: the slot of its first part, and its parts
+  int rows, step;      // of a slot; 1 where a job's parts lie in slots side by side, 2 where those behind the first are at 2 x workgroup
+  int splits, least;   // most parts of a job where workgroups are of one, blocks per part at least
+  int wgs, cus;        // workgroups that share all blocks (0: a workgroup has one job's part), CUs
+  unsigned inverse;    // ceil(2^32 / heads of a group), 0 for one head
 };
+__host__ __device__ __forceinline__ int part_floats(int HS) { return (HS + 3) & ~3; }
+// Where a row of part p is, whose job's first part is in slot `first`.
+__device__ __forceinline__ size_t part_row(const Parts8 &parts, int first, int p, int r) {
+  const int slot = p ? (first & -parts.step) + parts.step * p : first;
+  return (size_t)slot * parts.rows + r;
+}
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float or0(float m) { return m == -INFINITY ? 0.0f : m; }
@@ -461,23 +469,19 @@ __device__ __forceinline__ v4i turn4(uint32_t a, uint32_t b, uint32_t c, uint32_
 
 // Where a row's results go: of this part of the key axis, or of the whole.
 struct Place8 {
-  float *o, *m, *l, *lse;
-  float2 *stat;
-  // whole: no other part has keys of the row
-  __device__ __forceinline__ Place8(float *out, float *lse_, const Parts8 &parts, const ugk_cache8 &a, int part, bool whole, size_t row,
-                                    int h) {
-    const size_t at = row * a.NH + h, p = (size_t)part * a.rows_q * a.NH + at;
-    o = whole ? out + row * a.ldo + (size_t)h * a.HS : parts.o + p * a.HS;
-    m = whole ? nullptr : parts.m + p;
-    l = whole ? nullptr : parts.l + p;
+  float *o, *lse;
+  float2 *ml, *stat;
+  // whole: no other part has keys of the row, number r of the group
+  __device__ __forceinline__ Place8(float *out, float *lse_, const Parts8 &parts, const ugk_cache8 &a, int slot, bool whole, int r,
+                                    size_t row, int h) {
+    const size_t at = row * a.NH + h, p = (size_t)slot * parts.rows + r;
+    o = whole ? out + row * a.ldo + (size_t)h * a.HS : parts.o + p * part_floats(a.HS);
+    ml = whole ? nullptr : parts.ml + p;
     lse = whole && lse_ ? lse_ + at : nullptr;
     stat = whole && parts.stat ? parts.stat + at : nullptr;
   }
   __device__ __forceinline__ void put(float top, float sum) const {
-    if (m) {
-      *m = top;
-      *l = sum;
-    }
+    if (ml) *ml = make_float2(top, sum);
     if (lse) *lse = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn28;
     if (stat) *stat = make_float2(top, sum);
   }
@@ -525,92 +529,159 @@ __device__ __forceinline__ int wave_scan_int(int x) {
   return x;
 }
 
-// What a workgroup has: group `group` of R rows of a sequence and key/value head, and of their blocks a part.
+// What a workgroup has at a time: of group `group` of R rows of a sequence and key/value head blocks [first, stop).
 struct Job8 {
   Seq8 s;
-  int b, hk, group, part, rows, first, stop;
-  bool none, whole;  // nothing; all blocks
+  int b, hk, group, rows, first, stop, slot;
+  bool whole;  // all blocks
 };
-// Blocks that group t of R rows sees: its last row sees most.
-__device__ __forceinline__ int blocks_of(const Seq8 &s, const ugk_cache8 &a, int G, int R, int t) {
-  return (s.seen((min((t + 1) * R, s.Lq * G) - 1) / G, a.causal) + kKeys - 1) / kKeys;
-}
+// Blocks that a row at position i sees.
+__device__ __forceinline__ int blocks_at(const Seq8 &s, const ugk_cache8 &a, int i) { return (s.seen(i, a.causal) + kKeys - 1) / kKeys; }
 // The parts of nb blocks, of at most `chunk` each and as equal as they can be.
 __device__ __forceinline__ int parts_for(int nb, int chunk) { return max(1, (nb + chunk - 1) / chunk); }
-// Workgroup blockIdx.x's. Where the key axis is cut (parts.slots), the parts follow one another without a gap for the shorter
-// sequences, whose workgroups, empty, would still be dealt out to the CUs in turn and leave some with two and others with none; and a
-// part has so many blocks, from what the sequences really hold, that the workgroups are about as many as the CUs take, or, where the rows alone make
-// that many, that none has more than its share of all blocks. Every wavefront finds its place alike: a lane to a sequence, then to
-// a group. Else workgroups are of pairs, groups (the longest first) and parts in turn.
-template <int R>
-__device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts, unsigned pairs, unsigned groups, int *word) {
-  Job8 w;
-  const int lane = threadIdx.x & (kWave - 1), G = a.NH / a.NKV;
-  int chunk = parts.least;
-  w.none = true;
-  if (parts.slots) {
-    int blocks = 0, jobs = 0, longest = 0;
-    Seq8 s{0, 0, 0};  // the lane's of the last 64 sequences, which are mostly all
-    for (int b = lane; b < a.nseq; b += kWave) {
-      s = sequence8(a, b, blockIdx.x == 0, word, UGK_IDS_CACHE8_ATTENTION);
-      const int n = (s.Lq * G + R - 1) / R;
-      jobs += n;
-      for (int t = 0; t < n; t++) {
-        const int nb = blocks_of(s, a, G, R, t);
-        blocks += nb;
-        longest = max(longest, nb);
-      }
+
+// The workgroup's jobs, one after another.
+//
+// Where the key axis is cut over all CUs (parts.wgs), the blocks of all sequences, groups (the last rows first) and key/value heads are one long row,
+// from what the sequences really hold, of which every workgroup has the same share: it may begin and end within a job. Equal shares are what
+// counts: the CUs' time is their matrix units' or their part of the memory's, and a CU that holds two workgroups
+// is done no sooner than one that holds one of twice their blocks. A job's beginning (its rows, their results) counts as kBegin blocks.
+// Every wavefront finds its place alike, a lane to a sequence, then to a group.
+// Else workgroups are of pairs, groups (the longest first) and parts in turn.
+template <int R, int kBegin, bool kShared>
+struct Jobs {
+  // the lane's sequence, its groups and their units: blocks, and kBegin of each (a group without a block has one: its rows' results are written, too)
+  struct Held {
+    Seq8 s;
+    int n, units;
+  };
+  const ugk_cache8 &a;
+  const Parts8 &parts;
+  const unsigned pairs, groups;
+  const int G, lane;
+  int *const word;
+  int at, end, share, j;  // units; the number of the job
+  bool whole;             // workgroups have whole groups
+
+  __device__ __forceinline__ Jobs(const ugk_cache8 &a, const Parts8 &parts, unsigned pairs, unsigned groups, int *word)
+      : a(a), parts(parts), pairs(pairs), groups(groups), G(a.NH / a.NKV), lane(threadIdx.x & (kWave - 1)), word(word), at(0), end(1), share(1),
+        j(0), whole(false) {}
+  __device__ __forceinline__ int blocks_of(const Seq8 &s, int t) const {  // its last row sees most
+    const int row = min((t + 1) * R, s.Lq * G) - 1;
+    return blocks_at(s, a, parts.inverse ? (int)__umulhi((unsigned)row, parts.inverse) : row);
+  }
+  __device__ __forceinline__ int units(int nb) const { return whole ? 1 : kBegin + max(nb, 1); }
+  __device__ __forceinline__ Held held(int b, bool tell, int *longest) const {
+    Held h{{0, 0, 0}, 0, 0};
+    if (b >= a.nseq) return h;
+    h.s = sequence8(a, b, tell, word, UGK_IDS_CACHE8_ATTENTION);
+    h.n = (h.s.Lq * G + R - 1) / R;
+    if (whole) h.units = h.n;
+    for (int t = 0; !whole && t < h.n; t++) {
+      const int nb = blocks_of(h.s, t);
+      h.units += kBegin + max(nb, 1);
+      *longest = max(*longest, nb);
+    }
+    return h;
+  }
+
+  // The first job; false: none.
+  __device__ __forceinline__ bool first(Job8 &w) {
+    if (!kShared) return only(w);
+    Held h{{0, 0, 0}, 0, 0}, one = h;  // the first 64 sequences', which are mostly all
+    int all = 0, jobs = 0, longest = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += kWave) {
+      h = held(b0 + lane, blockIdx.x == 0, &longest);
+      jobs += h.n;
+      all += h.units;
+      if (b0 == 0) one = h;
     }
     longest = (int)wave_max_bits((uint32_t)longest);
-    jobs = wave_sum_int(jobs) * a.NKV;
-    blocks = wave_sum_int(blocks) * a.NKV;
-    const int left = 2 * jobs < parts.slots ? parts.slots - jobs : parts.slots;
-    chunk = __builtin_amdgcn_readfirstlane(max(chunk, (blocks + left - 1) / left));
+    jobs = __builtin_amdgcn_readfirstlane(wave_sum_int(jobs) * a.NKV);
+    all = __builtin_amdgcn_readfirstlane(wave_sum_int(all) * a.NKV);
     // no group has much more than a CU's share: the parts' way through memory would cost more than they save
-    if ((long long)2 * longest * parts.cus <= 3LL * blocks) chunk = max(chunk, longest);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *parts.used = chunk;
-    // the sequence, then the group and the part that are number x of all
-    int x = blockIdx.x, b = -1;
-    for (int b0 = 0; b0 < a.nseq && b < 0; b0 += kWave) {
-      int mine = 0;
-      if (a.nseq > kWave && b0 + lane < a.nseq) s = sequence8(a, b0 + lane, false, nullptr, 0);
-      if (b0 + lane < a.nseq) {
-        const int n = (s.Lq * G + R - 1) / R;
-        for (int t = 0; t < n; t++) mine += parts_for(blocks_of(s, a, G, R, t), chunk);
-        mine *= a.NKV;
-      }
-      const int to = wave_scan_int(mine), all = __shfl(to, kWave - 1);
+    whole = __builtin_amdgcn_readfirstlane((long long)2 * longest * parts.cus <= 3LL * (all - kBegin * jobs));
+    share = whole ? 1 : max(parts.least, (all + parts.wgs - 1) / parts.wgs);
+    all = whole ? jobs : all;
+    end = (int)min((long long)(blockIdx.x + 1) * share, (long long)all);
+    at = (int)min((long long)blockIdx.x * share, (long long)all);
+    if (at >= end) return false;
+    if (whole) one.units = one.n;
+
+    int x = at, n = 0;
+    for (int b0 = 0; b0 < a.nseq; b0 += kWave) {
+      h = b0 ? held(b0 + lane, false, &longest) : one;
+      const int mine = h.units * a.NKV, to = wave_scan_int(mine);
       const uint64_t over = __ballot(to > x);
       if (over) {
         const int l = __builtin_ctzll(over);
-        b = b0 + l;
-        x -= __shfl(to - mine, l);
-        w.s.q0 = __builtin_amdgcn_readfirstlane(__shfl(s.q0, l));
-        w.s.Lq = __builtin_amdgcn_readfirstlane(__shfl(s.Lq, l));
-        w.s.Lk = __builtin_amdgcn_readfirstlane(__shfl(s.Lk, l));
-      } else {
-        x -= all;
-      }
-    }
-    if (b < 0) return w;
-    w.b = __builtin_amdgcn_readfirstlane(b);
-    const int n = (w.s.Lq * G + R - 1) / R;
-    for (int t0 = 0; t0 < n; t0 += kWave) {
-      const int t = n - 1 - t0 - lane, mine = t < 0 ? 0 : parts_for(blocks_of(w.s, a, G, R, t), chunk) * a.NKV;
-      const int to = wave_scan_int(mine), all = __shfl(to, kWave - 1);
-      const uint64_t over = __ballot(to > x);
-      if (over) {
-        const int l = __builtin_ctzll(over);
-        w.group = __builtin_amdgcn_readfirstlane(n - 1 - t0 - l);
-        x -= __shfl(to - mine, l);
+        x = __builtin_amdgcn_readfirstlane(x - __shfl(to - mine, l));
+        j += wave_sum_int(lane < l ? h.n : 0);
+        n = __builtin_amdgcn_readfirstlane(__shfl(h.n, l));
+        w.b = b0 + l;
+        w.s.q0 = __builtin_amdgcn_readfirstlane(__shfl(h.s.q0, l));
+        w.s.Lq = __builtin_amdgcn_readfirstlane(__shfl(h.s.Lq, l));
+        w.s.Lk = __builtin_amdgcn_readfirstlane(__shfl(h.s.Lk, l));
         break;
       }
-      x -= all;
+      x -= __shfl(to, kWave - 1);
+      j += wave_sum_int(h.n);
+    }
+    w.group = 0;
+    for (int t0 = 0; t0 < n; t0 += kWave) {
+      const int t = n - 1 - t0 - lane, mine = t < 0 ? 0 : units(blocks_of(w.s, t)) * a.NKV, to = wave_scan_int(mine);
+      const uint64_t over = __ballot(to > x);
+      if (over) {
+        const int l = __builtin_ctzll(over);
+        x -= __shfl(to - mine, l);
+        w.group = n - 1 - t0 - l;
+        break;
+      }
+      x -= __shfl(to, kWave - 1);
     }
     x = __builtin_amdgcn_readfirstlane(x);
-    w.part = x / a.NKV;
-    w.hk = x % a.NKV;
-  } else {
+    w.group = __builtin_amdgcn_readfirstlane(w.group);
+    const int u = units(blocks_of(w.s, w.group));
+    w.hk = x / u;
+    j = __builtin_amdgcn_readfirstlane((j + n - 1 - w.group) * a.NKV + w.hk);
+    return take(w, x % u);
+  }
+  // The one behind w; false: none.
+  __device__ __forceinline__ bool next(Job8 &w) {
+    if (!kShared || at >= end) return false;
+    j++;
+    if (++w.hk == a.NKV) {
+      w.hk = 0;
+      if (--w.group < 0) {
+        do {
+          if (++w.b == a.nseq) return false;
+          const Seq8 s = sequence8(a, w.b, false, word, 0);
+          w.s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
+          w.s.Lq = __builtin_amdgcn_readfirstlane(s.Lq);
+          w.s.Lk = __builtin_amdgcn_readfirstlane(s.Lk);
+        } while (w.s.Lq == 0);
+        w.group = (w.s.Lq * G + R - 1) / R - 1;
+      }
+    }
+    return take(w, 0);
+  }
+  // This workgroup's blocks of job w, of which `at` is unit `off`; false: it has only of the job's beginning.
+  __device__ __forceinline__ bool take(Job8 &w, int off) {
+    const int nb = blocks_of(w.s, w.group), begin = whole ? 0 : kBegin, u = units(nb), stop = min(off + end - at, u) - begin;
+    w.rows = w.s.Lq * G;
+    w.first = max(off - begin, 0);
+    if (stop <= w.first) return false;
+    w.whole = w.first == 0 && stop == u - begin;
+    w.slot = blockIdx.x + (parts.step == 1 ? j : (int)blockIdx.x + (at != (int)blockIdx.x * share));
+    if (w.first == 0 && threadIdx.x == 0) tell(w, whole ? 1 : (at - off + u - 1) / share - (int)blockIdx.x + 1);
+    w.stop = whole ? nb : min(stop, nb);
+    at += u - off;
+    return true;
+  }
+  __device__ __forceinline__ void tell(const Job8 &w, int n) const {
+    if (parts.job) parts.job[((size_t)w.b * a.NKV + w.hk) * groups + w.group] = make_int2(w.slot, n);
+  }
+  __device__ __forceinline__ bool only(Job8 &w) {
     // Each CU gets one workgroup of every `cus`: of the first the longest, of the second the shortest first, and so on, so that all
     // have much the same to do (8 x 1,024 rows of 12 heads of 64 in turn 49 us, the longest first throughout).
     unsigned x = blockIdx.x;
@@ -619,21 +690,22 @@ __device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts,
     const unsigned round = x / pairs, pair = (x % pairs + round) % pairs;
     w.b = pair / a.NKV;
     w.hk = pair % a.NKV;
-    w.part = round / groups;
     w.group = groups - 1 - round % groups;
     w.s = sequence8(a, w.b, w.hk == 0 && round == 0, word, UGK_IDS_CACHE8_ATTENTION);
-    if (parts.o && blockIdx.x == 0 && threadIdx.x == 0) *parts.used = chunk;
-    if (w.group * R >= w.s.Lq * G) return w;
+    w.rows = w.s.Lq * G;
+    if (w.group * R >= w.rows) return false;
+    const int part = round / groups, nb = blocks_at(w.s, a, (min((w.group + 1) * R, w.rows) - 1) / G);
+    const int n = parts.o ? parts_for(nb, parts.least) : 1;
+    if (part >= n) return false;
+    const int each = nb / n, longer = nb - each * n;  // the first ones are one longer
+    w.whole = n == 1;
+    w.first = part * each + min(part, longer);
+    w.stop = w.first + each + (part < longer);
+    w.slot = (int)((pair * groups + w.group) * parts.splits) + part;
+    if (part == 0 && threadIdx.x == 0) tell(w, n);
+    return true;
   }
-  w.rows = w.s.Lq * G;
-  const int nb = blocks_of(w.s, a, G, R, w.group), n = parts.o ? parts_for(nb, chunk) : 1;
-  w.whole = n == 1;
-  w.none = w.part >= n;
-  const int each = nb / n, longer = nb - each * n;  // the first ones are one longer
-  w.first = w.part * each + min(w.part, longer);
-  w.stop = w.first + each + (w.part < longer);
-  return w;
-}
+};
 
 // Up to four rows (query rows times heads of the group) of a sequence and key/value head.
 //
@@ -642,17 +714,15 @@ __device__ __forceinline__ Job8 job_of(const ugk_cache8 &a, const Parts8 &parts,
 // head, their sums are exact, and a lane finds the four digits of its score in its own four registers.
 // The weights, 31 bits next to the block's largest, go the same way into the product with the values.
 template <int DT>
-__global__ __launch_bounds__(kFewWaves *kWave, DT >= 6 ? 3 : 4) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8,
-                                                                   const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
-                                                                   Parts8 parts, unsigned pairs, int *word) {
+__device__ __forceinline__ void few_job(float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8,
+                                        const float *vs, const ugk_cache8 &a, const Parts8 &parts, const Job8 &job, int *word) {
   constexpr int KS = (DT + 3) / 4, kStride = 20;
   __shared__ alignas(16) uint32_t lp[kFewWaves][16 * kStride];
   __shared__ float lo[kFewWaves][4][DT * 16];
   __shared__ float lm[kFewWaves][4], ll[kFewWaves][4];
-  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int thread = here((int)threadIdx.x);  // what is computed from it is not kept from job to job
+  const int lane = thread & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(thread >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const Job8 job = job_of<4>(a, parts, pairs, 1, word);
-  if (job.none) return;
   const Seq8 &s = job.s;
   const int b = job.b, hk = job.hk, G = a.NH / a.NKV, rows = job.rows, first = job.first, stop = job.stop;
   const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
@@ -779,7 +849,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT >= 6 ? 3 : 4) void k_cache8_fe
     wt[w] = ll[w][r] == 0.0f ? 0.0f : ll[w][r] * ex2(lm[w][r] - or0(top));
     total += wt[w];
   }
-  const Place8 to(out, lse, parts, a, job.part, job.whole, (size_t)s.q0 + r / G, hk * G + r % G);
+  const Place8 to(out, lse, parts, a, job.slot, job.whole, r, (size_t)s.q0 + r / G, hk * G + r % G);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   for (int d = lane; d < a.HS; d += kWave) {
     float y = 0.0f;
@@ -788,6 +858,18 @@ __global__ __launch_bounds__(kFewWaves *kWave, DT >= 6 ? 3 : 4) void k_cache8_fe
     to.o[d] = y;
   }
   if (lane == 0) to.put(top, total);
+}
+
+template <int DT, bool kShared>
+__global__ __launch_bounds__(kFewWaves *kWave, DT >= 6 ? 3 : 4) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8, const float *ks,
+                               const int8_t *v8, const float *vs, ugk_cache8 a, Parts8 parts, unsigned pairs,
+                               unsigned groups, int *word) {
+  Jobs<4, 4, kShared> jobs(a, parts, pairs, groups, word);
+  Job8 job;
+  for (bool more = jobs.first(job); more; more = jobs.next(job)) {
+    few_job<DT>(out, lse, q, k8, ks, v8, vs, a, parts, job, word);
+    __syncthreads();  // LDS is read until here
+  }
 }
 
 // x of the lanes that hold the same row in the four quarters of a wavefront, combined.
@@ -805,16 +887,14 @@ __device__ __forceinline__ float quarters_sum(float x) {
 // the values' codes has its keys in the order in which the lanes hold them. A wavefront has 16 rows; with RW 2 two of them take the
 // same blocks, which the second finds in a cache.
 template <int DT, int RW>
-__global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out, float *lse, const float *q, const int8_t *k8,
-                                                                    const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
-                                                                    Parts8 parts, unsigned pairs, unsigned groups, int *word) {
+__device__ __forceinline__ void some_job(float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8,
+                                         const float *vs, const ugk_cache8 &a, const Parts8 &parts, const Job8 &job, int *word) {
   constexpr int KS = (DT + 3) / 4, kStride = 16 * DT + 4, KW = kFewWaves / RW;
   __shared__ alignas(16) float lo[kFewWaves][16 * kStride];
   __shared__ float lm[kFewWaves][16], ll[kFewWaves][16];
-  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int thread = here((int)threadIdx.x);  // what is computed from it is not kept from job to job
+  const int lane = thread & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(thread >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const Job8 job = job_of<16 * RW>(a, parts, pairs, groups, word);
-  if (job.none) return;
   const Seq8 &s = job.s;
   const int b = job.b, hk = job.hk, G = a.NH / a.NKV, rows = job.rows, row0 = job.group * 16 * RW, first = job.first, stop = job.stop;
   const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
@@ -973,7 +1053,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
       wt[w] = ll[w0 + w][r] == 0.0f ? 0.0f : ll[w0 + w][r] * ex2(lm[w0 + w][r] - or0(top));
       total += wt[w];
     }
-    const Place8 to(out, lse, parts, a, job.part, job.whole, (size_t)s.q0 + row / G, hk * G + row % G);
+    const Place8 to(out, lse, parts, a, job.slot, job.whole, x, (size_t)s.q0 + row / G, hk * G + row % G);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     for (int d = lane; d < a.HS; d += kWave) {
       float y = 0.0f;
@@ -985,51 +1065,63 @@ __global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out,
   }
 }
 
-// What m and l of the parts of row `at` say of the whole.
-__device__ __forceinline__ float2 joined(const Parts8 &parts, size_t per, size_t at, int n) {
+template <int DT, int RW, bool kShared>
+__global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out, float *lse, const float *q, const int8_t *k8, const float *ks,
+                               const int8_t *v8, const float *vs, ugk_cache8 a, Parts8 parts, unsigned pairs,
+                               unsigned groups, int *word) {
+  Jobs<16 * RW, 4, kShared> jobs(a, parts, pairs, groups, word);
+  Job8 job;
+  for (bool more = jobs.first(job); more; more = jobs.next(job)) {
+    some_job<DT, RW>(out, lse, q, k8, ks, v8, vs, a, parts, job, word);
+    __syncthreads();  // LDS is read until here
+  }
+}
+
+// What m and l of the n parts of row r of a group say of the whole.
+__device__ __forceinline__ float2 joined(const Parts8 &parts, int first, int n, int r) {
   float m = -INFINITY, l = 0.0f;
-  for (int p0 = 0; p0 < n; p0 += 8) {
-    float lp[8], mp[8], top = m;
+  for (int p0 = 0; p0 < n; p0 += 4) {
+    float2 x[4];
+    float top = m;
 #pragma unroll
-    for (int u = 0; u < 8; u++) {
-      const size_t p = min(p0 + u, n - 1) * per + at;
-      mp[u] = parts.m[p];
-      lp[u] = p0 + u < n ? parts.l[p] : 0.0f;
+    for (int u = 0; u < 4; u++) {
+      x[u] = parts.ml[part_row(parts, first, min(p0 + u, n - 1), r)];
+      if (p0 + u >= n) x[u].y = 0.0f;
     }
 #pragma unroll
-    for (int u = 0; u < 8; u++) top = fmaxf(top, lp[u] == 0.0f ? -INFINITY : mp[u]);
+    for (int u = 0; u < 4; u++) top = fmaxf(top, x[u].y == 0.0f ? -INFINITY : x[u].x);
     l *= ex2(m - or0(top));
     m = top;
 #pragma unroll
-    for (int u = 0; u < 8; u++) l += lp[u] == 0.0f ? 0.0f : lp[u] * ex2(mp[u] - or0(top));
+    for (int u = 0; u < 4; u++) l += x[u].y == 0.0f ? 0.0f : x[u].y * ex2(x[u].x - or0(top));
   }
   return make_float2(m, l);
 }
 
-// Behind the attention, workgroups of two kinds. The first `joins` join the parts of a split key axis, one wavefront per row and head, in the
-// parts' order, where a workgroup of `rows` rows had more than one. The others add up the weights of 16 blocks of a sequence, 16
+// Behind the attention, workgroups of two kinds. The first `joins` join the parts of a split key axis, half a wavefront per row and head, in the
+// parts' order, where a group of `rows` rows had more than one. The others add up the weights of 16 blocks of a sequence, 16
 // threads to each, which take every sixteenth row and head, in a fixed order: weight[b, j] += sum of l_j 2^(m_j - m) / l.
 __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse, float *weight, Parts8 parts, ugk_cache8 a, int rows,
-                                                         unsigned joins) {
-  constexpr int kAtOnce = 8;  // parts whose loads are on their way together
+                                                         int groups, unsigned joins) {
+  constexpr int kAtOnce = 4;  // parts whose loads are on their way together
+  constexpr int kJoinRows = 2 * kBlock / kWave;
   const int G = a.NH / a.NKV;
-  const size_t per = (size_t)a.rows_q * a.NH;
   if (blockIdx.x >= joins) {
     __shared__ float part[16][17];
     __shared__ float2 whole[kBlock];
     const unsigned x = blockIdx.x - joins;
     const int of = (a.ld_table + 15) / 16, b = x / of, j = x % of * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
     const Seq8 s = sequence8(a, b, false, nullptr, 0);
-    const int nb = (s.Lk + kKeys - 1) / kKeys, n = s.Lq * G, chunk = joins ? *parts.used : 0;
+    const int nb = (s.Lk + kKeys - 1) / kKeys, n = s.Lq * G;
     if (x % of * 16 >= nb) return;
     float sum = 0.0f;
     for (int y0 = 0; y0 < n * a.NKV; y0 += kBlock) {  // a row and head per thread, then a block per thread
       const int mine = y0 + (int)threadIdx.x;
       if (mine < n * a.NKV) {
         const int hk = mine / n, rr = mine % n;
-        const size_t at = ((size_t)s.q0 + rr / G) * a.NH + hk * G + rr % G;
-        const int all = joins ? parts_for(blocks_of(s, a, G, rows, rr / rows), chunk) : 1;
-        whole[threadIdx.x] = all > 1 ? joined(parts, per, at, all) : parts.stat[at];
+        const int2 job = parts.job ? parts.job[((size_t)b * a.NKV + hk) * groups + rr / rows] : make_int2(0, 1);
+        whole[threadIdx.x] =
+            job.y > 1 ? joined(parts, job.x, job.y, rr % rows) : parts.stat[((size_t)s.q0 + rr / G) * a.NH + hk * G + rr % G];
       }
       __syncthreads();
       for (int y = y0 + slice; y < min(y0 + kBlock, n * a.NKV); y += 16) {
@@ -1049,48 +1141,52 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
     weight[(size_t)b * a.ld_table + j] += t;
     return;
   }
-  const int per_seq = (a.max_q * G + 3) / 4, b = blockIdx.x / per_seq / a.NKV, hk = blockIdx.x / per_seq % a.NKV;
-  const int lane = threadIdx.x & (kWave - 1), rr = blockIdx.x % per_seq * 4 + (threadIdx.x >> 6);
+  const int per_seq = (a.max_q * G + kJoinRows - 1) / kJoinRows, pair = blockIdx.x / per_seq, b = pair / a.NKV, hk = pair % a.NKV;
+  const int rr = blockIdx.x % per_seq * kJoinRows + (threadIdx.x >> 5), r = rr % rows, d = 4 * (threadIdx.x & 31);
+  const int2 job = parts.job[(size_t)pair * groups + min(rr / rows, groups - 1)];
   const Seq8 s = sequence8(a, b, false, nullptr, 0);
-  const int chunk = *parts.used;
-  if (rr >= s.Lq * G) return;
-  const int n = parts_for(blocks_of(s, a, G, rows, rr / rows), chunk);
-  if (n == 1) return;  // one workgroup had the row whole
-  const int i = rr / G, h = hk * G + rr % G;
-  const size_t g = (size_t)s.q0 + i, at = g * a.NH + h;
-  float m = -INFINITY, o0 = 0.0f, o1 = 0.0f, l = 0.0f;
-  const int d0 = min(lane, a.HS - 1), d1 = min(lane + kWave, a.HS - 1);
+  if (rr >= s.Lq * G || job.y == 1) return;  // no row, or one workgroup had it whole
+  const int n = job.y, floats = part_floats(a.HS), h = hk * G + rr % G;
+  const size_t g = (size_t)s.q0 + rr / G;
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int t = 0; t < n; t += kAtOnce) {
-    float y0[kAtOnce], y1[kAtOnce], mt[kAtOnce], lt[kAtOnce], top = m;
+    float4 y[kAtOnce];
+    float2 x[kAtOnce];
+    float top = m;
 #pragma unroll
     for (int u = 0; u < kAtOnce; u++) {
-      const size_t p = min(t + u, n - 1) * per + at;
-      y0[u] = parts.o[p * a.HS + d0];
-      y1[u] = parts.o[p * a.HS + d1];
-      mt[u] = parts.m[p];
-      lt[u] = t + u < n ? parts.l[p] : 0.0f;
+      const size_t p = part_row(parts, job.x, min(t + u, n - 1), r);
+      y[u] = ld4(parts.o + p * floats + min(d, floats - 4));
+      x[u] = parts.ml[p];
+      if (t + u >= n) x[u].y = 0.0f;
     }
 #pragma unroll
-    for (int u = 0; u < kAtOnce; u++) top = fmaxf(top, lt[u] == 0.0f ? -INFINITY : mt[u]);
+    for (int u = 0; u < kAtOnce; u++) top = fmaxf(top, x[u].y == 0.0f ? -INFINITY : x[u].x);
     const float keep = ex2(m - or0(top));
     m = top;
     l *= keep;
-    o0 *= keep;
-    o1 *= keep;
+    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
 #pragma unroll
     for (int u = 0; u < kAtOnce; u++) {
-      const float w = lt[u] == 0.0f ? 0.0f : lt[u] * ex2(mt[u] - or0(top));  // 0: a part without a key of this row, its o is 0
+      const float w = x[u].y == 0.0f ? 0.0f : x[u].y * ex2(x[u].x - or0(top));  // 0: a part without a key of this row, its o is 0
       l += w;
-      o0 = fmaf(w, y0[u], o0);
-      o1 = fmaf(w, y1[u], o1);
+      o = make_float4(fmaf(w, y[u].x, o.x), fmaf(w, y[u].y, o.y), fmaf(w, y[u].z, o.z), fmaf(w, y[u].w, o.w));
     }
   }
   const bool none = l == 0.0f;
   const float inv = none ? 1.0f : 1.0f / l;
-  float *po = out + g * a.ldo + (size_t)h * a.HS;
-  if (lane < a.HS) po[lane] = o0 * inv;
-  if (lane + kWave < a.HS) po[lane + kWave] = o1 * inv;
-  if (lse && lane == 0) lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn28;
+  float *po = out + g * a.ldo + (size_t)h * a.HS + d;
+  const int nd = a.HS - d;
+  const float4 y = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (nd >= 4) {
+    st4(po, y);
+  } else if (nd > 0) {
+    po[0] = y.x;
+    if (nd > 1) po[1] = y.y;
+    if (nd > 2) po[2] = y.z;
+  }
+  if (lse && d == 0) lse[g * a.NH + h] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn28;
 }
 
 // Many rows: a prompt's. 128 rows of a sequence and key/value head per workgroup, 32 to a wavefront, over blocks whose codes go
@@ -1110,16 +1206,14 @@ __device__ __forceinline__ v2u halves4(uint32_t w) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(float *out, float *lse, const float *q, const int8_t *k8,
-                                                                 const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a,
-                                                                 Parts8 parts, unsigned pairs, unsigned groups, int *word) {
+__device__ __forceinline__ void tile_job(float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8,
+                                         const float *vs, const ugk_cache8 &a, const Parts8 &parts, const Job8 &job, int *word) {
   constexpr int KSTR = 16 * DT + 8, VSTR = kKeys + 8, D32 = DT / 2, NL = (DT + 3) / 4;
   __shared__ alignas(16) _Float16 kl[2][kKeys * KSTR];
   __shared__ alignas(16) _Float16 vl[2][16 * DT * VSTR];
-  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int thread = here((int)threadIdx.x);  // what is computed from it is not kept from job to job
+  const int lane = thread & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(thread >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const Job8 job = job_of<kTileRows8>(a, parts, pairs, groups, word);
-  if (job.none) return;
   const Seq8 &s = job.s;
   const int b = job.b, hk = job.hk, G = a.NH / a.NKV, HP = padded(a.HS), CH = HP / 16;
   const int rows = job.rows, row0 = job.group * kTileRows8, first = job.first, stop = job.stop;
@@ -1130,6 +1224,36 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
   const int least = s.seen(wave_first / G, a.causal), most_seen = s.seen(wave_last / G, a.causal);
   const bool idle = row0 + 32 * wave >= rows;
   const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
+
+  // staging: thread t has words of 16 codes t, t + 256 of the block's keys and of its values
+  int kdst[NL], vdst[NL];
+#pragma unroll
+  for (int n = 0; n < NL; n++) {
+    const int w = thread + n * kTileThreads8, c = w & 3;
+    kdst[n] = w / CH * KSTR + w % CH * 16;
+    vdst[n] = (w >> 2) * VSTR + (c & 1) * 8 + (c >> 1) * 4;
+  }
+  v4u kr[NL], vr[NL];
+  float kscale = 0.0f, vscale = 0.0f;
+  bool there = true;
+  int next = first < stop ? table_at(a, b, first) : 0;
+  const auto fetch = [&](int j) {
+    const int id = checked_block(a, __builtin_amdgcn_readfirstlane(next), word, UGK_IDS_CACHE8_ATTENTION);
+    next = table_at(a, b, min(j + 1, stop - 1));
+    there = id >= 0;
+    const size_t at = block_head(id, a.NKV, hk);
+#pragma unroll
+    for (int n = 0; n < NL; n++) {
+      const int w = thread + n * kTileThreads8;
+      if (w < 4 * HP) {
+        kr[n] = *reinterpret_cast<const v4u *>(k8 + at * kKeys * HP + 16 * w);
+        vr[n] = *reinterpret_cast<const v4u *>(v8 + at * kKeys * HP + 16 * w);
+      }
+    }
+    kscale = ks[at];
+    vscale = vs[at];
+  };
+  if (first < stop) fetch(first);
 
   v8h qh[DT], ql[DT];
   int e;
@@ -1153,44 +1277,15 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
 #pragma unroll
   for (int t = 0; t < D32; t++) o[t] = v16f{};
 
-  // staging: thread t has words of 16 codes t, t + 256 of the block's keys and of its values
-  int kdst[NL], vdst[NL];
-#pragma unroll
-  for (int n = 0; n < NL; n++) {
-    const int w = threadIdx.x + n * kTileThreads8, c = w & 3;
-    kdst[n] = w / CH * KSTR + w % CH * 16;
-    vdst[n] = (w >> 2) * VSTR + (c & 1) * 8 + (c >> 1) * 4;
-  }
-  v4u kr[NL], vr[NL];
-  float kscale = 0.0f, vscale = 0.0f;
-  bool there = true;
-  int next = first < stop ? table_at(a, b, first) : 0;
-  const auto fetch = [&](int j) {
-    const int id = checked_block(a, __builtin_amdgcn_readfirstlane(next), word, UGK_IDS_CACHE8_ATTENTION);
-    next = table_at(a, b, min(j + 1, stop - 1));
-    there = id >= 0;
-    const size_t at = block_head(id, a.NKV, hk);
-#pragma unroll
-    for (int n = 0; n < NL; n++) {
-      const int w = threadIdx.x + n * kTileThreads8;
-      if (w < 4 * HP) {
-        kr[n] = *reinterpret_cast<const v4u *>(k8 + at * kKeys * HP + 16 * w);
-        vr[n] = *reinterpret_cast<const v4u *>(v8 + at * kKeys * HP + 16 * w);
-      }
-    }
-    kscale = ks[at];
-    vscale = vs[at];
-  };
   if (CH < DT) {  // behind the keys' rows q is 0, and what is there has to be a number
-    for (int x = threadIdx.x; x < 2 * kKeys * KSTR / 2; x += kTileThreads8) reinterpret_cast<uint32_t *>(kl[0])[x] = 0u;
+    for (int x = thread; x < 2 * kKeys * KSTR / 2; x += kTileThreads8) reinterpret_cast<uint32_t *>(kl[0])[x] = 0u;
     __syncthreads();
   }
-  if (first < stop) fetch(first);
   for (int j = first; j < stop; j++) {
     _Float16 *kt = kl[(j - first) & 1], *vt = vl[(j - first) & 1];
 #pragma unroll
     for (int n = 0; n < NL; n++) {
-      if (threadIdx.x + n * kTileThreads8 >= 4 * HP) continue;
+      if (thread + n * kTileThreads8 >= 4 * HP) continue;
       const v4u kw = kr[n] ^ 0x80808080u, vw = vr[n] ^ 0x80808080u;
       const v2u k0 = halves4(kw[0]), k1 = halves4(kw[1]), k2 = halves4(kw[2]), k3 = halves4(kw[3]);
       *reinterpret_cast<v4u *>(kt + kdst[n]) = v4u{k0[0], k0[1], k1[0], k1[1]};
@@ -1208,17 +1303,29 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
     __syncthreads();
     if (j + 1 < stop) fetch(j + 1);
     if (idle || j * kKeys >= most_seen) continue;
-    v16f sc[2];
+    // The operands of two steps on their way, and of two products in a row no sum is the same.
+    const _Float16 *kp = kt + col * KSTR + 8 * half, *vp = vt + col * VSTR + 8 * half;
+    v8h kf[2][2], vf[D32];
+    v16f sc[2] = {v16f{}, v16f{}};
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-      sc[x] = v16f{};
+    for (int st = 0; st < 2; st++)
 #pragma unroll
-      for (int st = 0; st < DT; st++) {
-        const v8h kf = frag(kt + (32 * x + col) * KSTR + 16 * st + 8 * half);
-        sc[x] = mfma(kf, ql[st], sc[x]);
-        sc[x] = mfma(kf, qh[st], sc[x]);
-      }
+      for (int x = 0; x < 2; x++) kf[st][x] = frag(kp + 32 * x * KSTR + 16 * st);
+#pragma unroll
+    for (int st = 0; st < DT; st++) {
+      __builtin_amdgcn_sched_barrier(0);
+      sc[0] = mfma(kf[st % 2][0], ql[st], sc[0]);
+      sc[1] = mfma(kf[st % 2][1], ql[st], sc[1]);
+      sc[0] = mfma(kf[st % 2][0], qh[st], sc[0]);
+      sc[1] = mfma(kf[st % 2][1], qh[st], sc[1]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (st + 2 < DT)
+#pragma unroll
+        for (int x = 0; x < 2; x++) kf[st % 2][x] = frag(kp + 32 * x * KSTR + 16 * (st + 2));
     }
+#pragma unroll
+    for (int t = 0; t < D32; t++) vf[t] = frag(vp + 32 * t * VSTR);
+    __builtin_amdgcn_sched_barrier(0);
     float mb = -INFINITY;
     const bool masked = !held || (j + 1) * kKeys > least;
     const int seen = held ? lim - j * kKeys - 4 * half : 0;  // of this block's keys from the lane's first on
@@ -1263,10 +1370,11 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
       }
       split8(p, ph, pl);
 #pragma unroll
+      for (int t = 0; t < D32; t++) o[t] = mfma(vf[t], pl, o[t]);
+#pragma unroll
       for (int t = 0; t < D32; t++) {
-        const v8h vf = frag(vt + (32 * t + col) * VSTR + 16 * g + 8 * half);
-        o[t] = mfma(vf, pl, o[t]);
-        o[t] = mfma(vf, ph, o[t]);
+        o[t] = mfma(vf[t], ph, o[t]);
+        if (g < 3) vf[t] = frag(vp + 32 * t * VSTR + 16 * (g + 1));
       }
     }
     if (!apart) run.sum(mb, lb, run.mo, up);
@@ -1276,7 +1384,7 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
   int p;
   const float g = run.last(sum, &p);
   p -= 14;  // of the weights
-  const Place8 to(out, lse, parts, a, job.part, job.whole, (size_t)s.q0 + i, h);
+  const Place8 to(out, lse, parts, a, job.slot, job.whole, mine - row0, (size_t)s.q0 + i, h);
   float *po = to.o;
 #pragma unroll
   for (int t = 0; t < D32; t++)
@@ -1298,6 +1406,18 @@ __global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(
       }
     }
   if (half == 0) to.put(run.m, sum);
+}
+
+template <int DT, bool kShared>
+__global__ __launch_bounds__(kTileThreads8, DT <= 4 ? 3 : 2) void k_cache8_tile(float *out, float *lse, const float *q, const int8_t *k8, const float *ks,
+                               const int8_t *v8, const float *vs, ugk_cache8 a, Parts8 parts, unsigned pairs,
+                               unsigned groups, int *word) {
+  Jobs<kTileRows8, 2, kShared> jobs(a, parts, pairs, groups, word);
+  Job8 job;
+  for (bool more = jobs.first(job); more; more = jobs.next(job)) {
+    tile_job<DT>(out, lse, q, k8, ks, v8, vs, a, parts, job, word);
+    __syncthreads();  // LDS is read until here
+  }
 }
 
 // ---- eviction ----------------------------------------------------------------------
@@ -1423,9 +1543,11 @@ int cu_count8() {
 }
 
 // How an attention call is cut: k_cache8_few (rows 4), k_cache8_some (16, 32) in so many groups, or k_cache8_tile (128) in so many
-// tiles; parts of the key axis of at least `least` blocks; and workgroups that the CUs hold at once.
+// tiles; `wgs` workgroups that share all blocks, or up to `splits` parts of `least` blocks or more of each; the rows of a slot of
+// parts, the slots, and where a job's are.
 struct Plan8 {
-  int rows, groups, splits, least, slots;
+  int rows, groups, splits, least, wgs, grid, held, step;
+  size_t slots;
 };
 constexpr int kFewRows8 = 32;
 
@@ -1434,86 +1556,103 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   const long long pairs = (long long)a.nseq * a.NKV, G = a.NH / a.NKV, rows = a.max_q * G, blocks = (a.max_k + kKeys - 1) / kKeys;
   p.rows = rows <= 4 ? 4 : rows <= 16 ? 16 : rows <= kFewRows8 || weigh ? 32 : kTileRows8;
   p.groups = (int)((rows + p.rows - 1) / p.rows);
+  p.held = (int)min((long long)p.rows, rows);
+  p.step = 1;
+  p.splits = 1;
   const bool narrow = a.HS <= 64;
-  p.slots = cu_count8() * (p.rows == 4 ? (narrow ? 4 : 3) : p.rows == kTileRows8 ? (narrow ? 3 : 2) : (narrow ? 4 : 2));
-  // the shares of so many blocks, were all sequences full
-  const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / p.slots;
-  long long least = max(min(share / 2, blocks / 2), 4LL);
-  // few blocks are not worth a look at all sequences, nor are many groups, which fill the CUs
-  if (blocks <= 32 || jobs > 4LL * p.slots || blocks * pairs * p.groups > 1 << 30) {
-    p.slots = 0;
-    // with weights to add up, the launch that joins parts is there anyway
-    least = 3 * jobs >= 2LL * cu_count8() && !weigh ? blocks : max(share, 4LL);
-  }
+  const int cus = cu_count8(), at_once = cus * (p.rows == 4 ? (narrow ? 4 : 3) : p.rows == kTileRows8 ? (narrow ? 3 : 2) : (narrow ? 4 : 2));
+  // at most so many jobs, and the shares of so many blocks, were all sequences full
+  const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / at_once;
   // what a workspace of the same rows and heads has for the fp32 attention
-  const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / ((a.HS + 2) * sizeof(float)) - 1;
-  const long long fit = max((long long)(most / max((size_t)a.rows_q * a.NH, (size_t)1)), 1LL);
-  p.least = (int)max(max(least, (blocks + fit - 1) / fit), 1LL);
-  p.splits = (int)max((blocks + p.least - 1) / p.least, 1LL);
-  if (p.splits == 1) p.slots = 0;
+  const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / sizeof(float) - 4;
+  const long long told = 2 * pairs * p.groups, fit = ((long long)most - told) / ((part_floats(a.HS) + 2) * (long long)p.held);
+  // few blocks are not worth a look at all sequences, nor are many groups, which fill the CUs
+  if (blocks > 32 && jobs <= 4LL * at_once && blocks * pairs * p.groups <= 1 << 30 && (rows + p.rows) * G >> 32 == 0) {
+    // a job has one part more than workgroups' borders, and a workgroup two at most that are not whole
+    p.step = jobs <= at_once && fit >= 2 * jobs ? 1 : 2;
+    p.wgs = (int)max(min((long long)at_once, p.step == 1 ? fit - jobs : fit / 2), 0LL);
+  }
+  if (p.wgs) {
+    p.least = 4;
+    p.slots = p.step == 1 ? p.wgs + jobs : 2LL * p.wgs;
+    p.grid = max(p.wgs, (int)jobs);
+  } else {
+    // with weights to add up, the launch that joins parts is there anyway
+    const long long least = max(3 * jobs >= 2LL * cus && !weigh ? blocks : max(share, 4LL), 1LL);
+    p.step = 1;
+    p.splits = (int)max(min((blocks + least - 1) / least, fit / (pairs * p.groups)), 1LL);
+    p.least = (int)max((blocks + p.splits - 1) / p.splits, 1LL);
+    p.grid = (int)(pairs * p.groups * p.splits);
+    p.slots = p.splits > 1 ? p.grid : 0;
+  }
   return p;
 }
-size_t parts_rows(const ugk_cache8 &a, const Plan8 &p) { return (size_t)p.splits * a.rows_q * a.NH; }
-size_t even(size_t n) { return (n + 1) / 2 * 2; }
+size_t slot_floats(const ugk_cache8 &a, const Plan8 &p) { return p.slots * p.held * part_floats(a.HS); }
+size_t parts_floats(const ugk_cache8 &a, const Plan8 &p) {
+  return p.slots ? slot_floats(a, p) + 2 * (p.slots * p.held + (size_t)a.nseq * a.NKV * p.groups) : 0;
+}
 }  // namespace
 
 size_t cache8_attention_bytes(const ugk_cache8 &a, bool weigh) {
-  const Plan8 p = plan8(a, weigh);
-  const size_t parts = p.splits > 1 ? even(parts_rows(a, p) * (a.HS + 2)) + 2 : 0;
   const size_t stat = (size_t)a.rows_q * a.NH, block = (size_t)a.nseq * a.max_q * a.NH * a.ld_table;
-  return (parts + (weigh ? 2 * (stat + block) : 0)) * sizeof(float);
+  return (parts_floats(a, plan8(a, weigh)) + (weigh ? 2 * (stat + block) : 0)) * sizeof(float);
 }
 
 int launch_cache8_attention(float *out, float *lse, const float *q, const void *k8, const float *ks, const void *v8,
                             const float *vs, float *weight, float *mem, const ugk_cache8 &a, int *word) {
   const Plan8 p = plan8(a, weight);
+  const unsigned pairs = (unsigned)a.nseq * a.NKV, G = a.NH / a.NKV;
   Parts8 parts{};
+  parts.rows = p.held;
+  parts.step = p.step;
   parts.splits = p.splits;
   parts.least = p.least;
-  parts.slots = p.slots;
+  parts.wgs = p.wgs;
   parts.cus = cu_count8();
-  if (p.splits > 1) {
-    parts.used = reinterpret_cast<int *>(mem);
-    parts.m = mem + 2;
-    parts.l = parts.m + parts_rows(a, p);
-    parts.o = parts.l + parts_rows(a, p);
-    mem += 2 + even(parts_rows(a, p) * (a.HS + 2));
+  parts.inverse = G == 1 ? 0u : (unsigned)((1ULL << 32) / G + 1);
+  if (p.slots) {
+    parts.o = mem;
+    parts.ml = reinterpret_cast<float2 *>(mem + slot_floats(a, p));
+    parts.job = reinterpret_cast<int2 *>(parts.ml + p.slots * p.held);
+    mem += parts_floats(a, p);
   }
   if (weight) {
     parts.stat = reinterpret_cast<float2 *>(mem);
     parts.block = parts.stat + (size_t)a.rows_q * a.NH;
   }
-  const unsigned pairs = (unsigned)a.nseq * a.NKV;
-  // as many parts in all as CUs, and one more for each group of rows, or all that there may be of each
-  const unsigned wgs = p.slots ? p.slots + pairs * p.groups : pairs * p.groups * p.splits;
   const int8_t *kc = static_cast<const int8_t *>(k8), *vc = static_cast<const int8_t *>(v8);
-  const auto few = [&](auto kernel) {
-    launch(kernel, dim3(wgs), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, word);
+  const auto go = [&](auto kernel) {
+    launch(kernel, dim3(p.grid), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, (unsigned)p.groups, word);
   };
-  const auto some = [&](auto kernel) {
-    launch(kernel, dim3(wgs), dim3(kFewWaves * kWave), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs,
-           (unsigned)p.groups, word);
+  const auto of = [&](auto shared) {
+    constexpr bool kS = decltype(shared)::value;
+    const int d = a.HS <= 32 ? 2 : a.HS <= 64 ? 4 : a.HS <= 96 ? 6 : 8;
+    switch (p.rows) {
+      case 4:
+        d == 2 ? go(k_cache8_few<2, kS>) : d == 4 ? go(k_cache8_few<4, kS>) : d == 6 ? go(k_cache8_few<6, kS>) : go(k_cache8_few<8, kS>);
+        break;
+      case 16:
+        d == 2   ? go(k_cache8_some<2, 1, kS>)
+        : d == 4 ? go(k_cache8_some<4, 1, kS>)
+        : d == 6 ? go(k_cache8_some<6, 1, kS>)
+                 : go(k_cache8_some<8, 1, kS>);
+        break;
+      case 32:
+        d == 2   ? go(k_cache8_some<2, 2, kS>)
+        : d == 4 ? go(k_cache8_some<4, 2, kS>)
+        : d == 6 ? go(k_cache8_some<6, 2, kS>)
+                 : go(k_cache8_some<8, 2, kS>);
+        break;
+      default:
+        d == 2 ? go(k_cache8_tile<2, kS>) : d == 4 ? go(k_cache8_tile<4, kS>) : d == 6 ? go(k_cache8_tile<6, kS>) : go(k_cache8_tile<8, kS>);
+    }
   };
-  const auto tile = [&](auto kernel) {
-    launch(kernel, dim3(wgs), dim3(kTileThreads8), 0, out, lse, q, kc, ks, vc, vs, a, parts, pairs, (unsigned)p.groups,
-           word);
-  };
-  const int d = a.HS <= 32 ? 2 : a.HS <= 64 ? 4 : a.HS <= 96 ? 6 : 8;
-  switch (p.rows) {
-    case 4: d == 2 ? few(k_cache8_few<2>) : d == 4 ? few(k_cache8_few<4>) : d == 6 ? few(k_cache8_few<6>) : few(k_cache8_few<8>); break;
-    case 16:
-      d == 2 ? some(k_cache8_some<2, 1>) : d == 4 ? some(k_cache8_some<4, 1>) : d == 6 ? some(k_cache8_some<6, 1>) : some(k_cache8_some<8, 1>);
-      break;
-    case 32:
-      d == 2 ? some(k_cache8_some<2, 2>) : d == 4 ? some(k_cache8_some<4, 2>) : d == 6 ? some(k_cache8_some<6, 2>) : some(k_cache8_some<8, 2>);
-      break;
-    default: d == 2 ? tile(k_cache8_tile<2>) : d == 4 ? tile(k_cache8_tile<4>) : d == 6 ? tile(k_cache8_tile<6>) : tile(k_cache8_tile<8>);
-  }
+  p.wgs ? of(std::true_type{}) : of(std::false_type{});
   if (int e = check_launch("cache8_attention")) return e;
-  const unsigned joins = parts.o ? pairs * grid_for((size_t)a.max_q * (a.NH / a.NKV), 4) : 0;
+  const unsigned joins = p.slots ? pairs * grid_for((size_t)a.max_q * G, 2 * kBlock / kWave) : 0;
   const unsigned weighs = weight ? (unsigned)a.nseq * ((a.ld_table + 15) / 16) : 0;
   if (joins + weighs == 0) return UGK_OK;
-  launch(k_cache8_finish, dim3(joins + weighs), dim3(kBlock), 0, out, lse, weight, parts, a, p.rows, joins);
+  launch(k_cache8_finish, dim3(joins + weighs), dim3(kBlock), 0, out, lse, weight, parts, a, p.rows, p.groups, joins);
   return check_launch("cache8_attention");
 }
 
