@@ -1109,6 +1109,8 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
   if (blockIdx.x >= joins) {
     __shared__ float part[16][17];
     __shared__ float2 whole[kBlock];
+    __shared__ size_t from[kBlock];
+    __shared__ int end[kBlock];
     const unsigned x = blockIdx.x - joins;
     const int of = (a.ld_table + 15) / 16, b = x / of, j = x % of * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
     const Seq8 s = sequence8(a, b, false, nullptr, 0);
@@ -1120,15 +1122,26 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
       if (mine < n * a.NKV) {
         const int hk = mine / n, rr = mine % n;
         const int2 job = parts.job ? parts.job[((size_t)b * a.NKV + hk) * groups + rr / rows] : make_int2(0, 1);
+        from[threadIdx.x] = (((size_t)b * a.NKV + hk) * a.max_q * G + rr) * a.ld_table;
+        end[threadIdx.x] = s.seen(rr / G, a.causal);
         whole[threadIdx.x] =
             job.y > 1 ? joined(parts, job.x, job.y, rr % rows) : parts.stat[((size_t)s.q0 + rr / G) * a.NH + hk * G + rr % G];
       }
       __syncthreads();
-      for (int y = y0 + slice; y < min(y0 + kBlock, n * a.NKV); y += 16) {
-        const int hk = y / n, rr = y % n;
-        if (j * kKeys >= s.seen(rr / G, a.causal)) continue;
-        const float2 p = parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + rr) * a.ld_table + j], w = whole[y - y0];
-        if (p.y != 0.0f) sum += p.y * ex2(p.x - w.x) / w.y;
+      const int stop = min(n * a.NKV - y0, kBlock);
+      for (int y = slice; y < stop; y += 16 * kAtOnce) {
+        float2 p[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+          const int z = min(y + 16 * u, stop - 1);
+          const bool sees = y + 16 * u < stop && j * kKeys < end[z];
+          p[u] = sees ? parts.block[from[z] + j] : make_float2(0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+          const float2 w = whole[min(y + 16 * u, stop - 1)];
+          if (p[u].y != 0.0f) sum += p[u].y * ex2(p[u].x - w.x) / w.y;
+        }
       }
       __syncthreads();
     }

@@ -116,13 +116,16 @@ class Cache8(ctypes.Structure):
         held = table is not None and not isinstance(table, int)
         if held and not ld_table and table.dim() == 2:
             ld_table = table.shape[1]
-        tensors = (q_start, q_end, k_len, table)
-        need = (nseq, nseq, nseq, max(nseq, 0) * (ld_table or -(-max_k // CACHE8_BLOCK)))
+        entries = max(nseq, 0) * (ld_table or -(-max_k // CACHE8_BLOCK))
         super().__init__(nseq, NH, NKV, HS, rows_q, max_q, max_k, nblocks, 1 if causal else 0, scale,
-                         *(_ptr(t, n, m, "i32") for t, n, m in zip(tensors, self._NAMES, need)), ld_table, ldq, ldk, ldv, ldo)
-        self._tensors = tensors
-        self._most = (min((t.numel() for t in tensors[:3] if t is not None and not isinstance(t, int)), default=Cache8._most[0]),
-                      table.numel() if held else Cache8._most[1])
+                         _ptr(q_start, "q_start", nseq, "i32"), _ptr(q_end, "q_end", nseq, "i32"), _ptr(k_len, "k_len", nseq, "i32"),
+                         _ptr(table, "table", entries, "i32"), ld_table, ldq, ldk, ldv, ldo)
+        self._tensors = (q_start, q_end, k_len, table)
+        most, held_most = Cache8._most
+        for t in (q_start, q_end, k_len):
+            if t is not None and not isinstance(t, int):
+                most = min(most, t.numel())
+        self._most = (most, table.numel() if held else held_most)
 
 
 _MATMUL_FWD = ctypes.CFUNCTYPE(_i, _fp, _fp, _fp, _fp, _fp, _i, _i, _i)
