@@ -509,6 +509,19 @@ def test_blocks_dealt_out_in_equal_shares(gpu, nseq, lq, NH, NKV, HS, cap, equal
         check(gpu, c, NH, q, starts, lens, keys, rows, weigh=True, max_q=lq)
 
 
+@pytest.mark.parametrize("lq,NH,NKV,HS", [(5, 4, 1, 128), (17, 1, 1, 64), (19, 2, 2, 33), (6, 3, 1, 96), (20, 2, 1, 64), (35, 1, 1, 16), (33, 2, 1, 80)])
+@pytest.mark.parametrize("cap", [200, 2500])
+def test_groups_of_rows_that_end_in_a_few(gpu, cap, lq, NH, NKV, HS):
+    """A few rows and heads more than 16, and with weights than 32."""
+    keys, lens = [cap, 3, cap // 2, 64], [lq, lq, lq - 1, 1]
+    c, g = filled(gpu, 4, cap, NKV, HS, keys, seed=cap + lq)
+    starts, rows = place_rows(lens)
+    q = rand(g, rows, NH, HS)
+    for causal in (True, False):
+        check(gpu, c, NH, q, starts, lens, keys, rows, causal=causal)
+        check(gpu, c, NH, q, starts, lens, keys, rows, causal=causal, weigh=True)
+
+
 def test_many_groups_of_rows_in_a_sequence(gpu):
     """More than 64 workgroups' rows in one sequence, whose key axis is cut all the same."""
     NH, NKV, HS, lq, n = 8, 1, 16, 1100, 2400

@@ -467,6 +467,17 @@ __device__ __forceinline__ v4i turn4(uint32_t a, uint32_t b, uint32_t c, uint32_
              (int)__builtin_amdgcn_perm(t3, t1, 0x05040100u), (int)__builtin_amdgcn_perm(t3, t1, 0x07060302u)};
 }
 
+// The first n of four floats.
+__device__ __forceinline__ void put4(float *p, float4 y, int n) {
+  if (n >= 4) {
+    st4(p, y);
+  } else if (n > 0) {
+    p[0] = y.x;
+    if (n > 1) p[1] = y.y;
+    if (n > 2) p[2] = y.z;
+  }
+}
+
 // Where a row's results go: of this part of the key axis, or of the whole.
 struct Place8 {
   float *o, *lse;
@@ -514,20 +525,16 @@ struct Walk {
 };
 __device__ __forceinline__ size_t block_head(int id, int NKV, int hk) { return (size_t)max(id, 0) * NKV + hk; }
 
-__device__ __forceinline__ int wave_sum_int(int x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
-}
+// The sum over the lanes up to this one (a shuffle through LDS for each step took a microsecond more).
 __device__ __forceinline__ int wave_scan_int(int x) {
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int o = 1; o < kWave; o *= 2) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes below in a row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of the row before, of the first two rows
+  return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
 }
+__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, kWave - 1); }
 
 // What a workgroup has at a time: of group `group` of R rows of a sequence and key/value head blocks [first, stop).
 struct Job8 {
@@ -597,10 +604,10 @@ struct Jobs {
       if (b0 == 0) one = h;
     }
     longest = (int)wave_max_bits((uint32_t)longest);
-    jobs = __builtin_amdgcn_readfirstlane(wave_sum_int(jobs) * a.NKV);
-    all = __builtin_amdgcn_readfirstlane(wave_sum_int(all) * a.NKV);
+    jobs = last_lane(wave_scan_int(jobs)) * a.NKV;
+    all = last_lane(wave_scan_int(all)) * a.NKV;
     // no group has much more than a CU's share: the parts' way through memory would cost more than they save
-    whole = __builtin_amdgcn_readfirstlane((long long)2 * longest * parts.cus <= 3LL * (all - kBegin * jobs));
+    whole = (long long)2 * longest * parts.cus <= 3LL * (all - kBegin * jobs);
     share = whole ? 1 : max(parts.least, (all + parts.wgs - 1) / parts.wgs);
     all = whole ? jobs : all;
     end = (int)min((long long)(blockIdx.x + 1) * share, (long long)all);
@@ -611,21 +618,21 @@ struct Jobs {
     int x = at, n = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += kWave) {
       h = b0 ? held(b0 + lane, false, &longest) : one;
-      const int mine = h.units * a.NKV, to = wave_scan_int(mine);
+      const int to = wave_scan_int(h.units) * a.NKV, before = wave_scan_int(h.n);
       const uint64_t over = __ballot(to > x);
       if (over) {
         const int l = __builtin_ctzll(over);
-        x = __builtin_amdgcn_readfirstlane(x - __shfl(to - mine, l));
-        j += wave_sum_int(lane < l ? h.n : 0);
-        n = __builtin_amdgcn_readfirstlane(__shfl(h.n, l));
+        n = __builtin_amdgcn_readlane(h.n, l);
+        x -= __builtin_amdgcn_readlane(to - h.units * a.NKV, l);
+        j += __builtin_amdgcn_readlane(before, l) - n;
         w.b = b0 + l;
-        w.s.q0 = __builtin_amdgcn_readfirstlane(__shfl(h.s.q0, l));
-        w.s.Lq = __builtin_amdgcn_readfirstlane(__shfl(h.s.Lq, l));
-        w.s.Lk = __builtin_amdgcn_readfirstlane(__shfl(h.s.Lk, l));
+        w.s.q0 = __builtin_amdgcn_readlane(h.s.q0, l);
+        w.s.Lq = __builtin_amdgcn_readlane(h.s.Lq, l);
+        w.s.Lk = __builtin_amdgcn_readlane(h.s.Lk, l);
         break;
       }
-      x -= __shfl(to, kWave - 1);
-      j += wave_sum_int(h.n);
+      x -= last_lane(to);
+      j += last_lane(before);
     }
     w.group = 0;
     for (int t0 = 0; t0 < n; t0 += kWave) {
@@ -633,17 +640,15 @@ struct Jobs {
       const uint64_t over = __ballot(to > x);
       if (over) {
         const int l = __builtin_ctzll(over);
-        x -= __shfl(to - mine, l);
+        x -= __builtin_amdgcn_readlane(to - mine, l);
         w.group = n - 1 - t0 - l;
         break;
       }
-      x -= __shfl(to, kWave - 1);
+      x -= last_lane(to);
     }
-    x = __builtin_amdgcn_readfirstlane(x);
-    w.group = __builtin_amdgcn_readfirstlane(w.group);
     const int u = units(blocks_of(w.s, w.group));
     w.hk = x / u;
-    j = __builtin_amdgcn_readfirstlane((j + n - 1 - w.group) * a.NKV + w.hk);
+    j = (j + n - 1 - w.group) * a.NKV + w.hk;
     return take(w, x % u);
   }
   // The one behind w; false: none.
@@ -707,44 +712,42 @@ struct Jobs {
   }
 };
 
-// Up to four rows (query rows times heads of the group) of a sequence and key/value head.
+// ---- up to 32 rows (query rows times heads of the group) ----
 //
-// A row of q is held as whole numbers of 31 bits next to its largest element, and those as four digits, so that four
-// rows are one 16-row operand of the 8-bit matrix units: a block's scores take two instructions per 16 keys at 128 floats per
-// head, their sums are exact, and a lane finds the four digits of its score in its own four registers.
-// The weights, 31 bits next to the block's largest, go the same way into the product with the values.
-template <int DT>
-__device__ __forceinline__ void few_job(float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8,
-                                        const float *vs, const ugk_cache8 &a, const Parts8 &parts, const Job8 &job, int *word) {
-  constexpr int KS = (DT + 3) / 4, kStride = 20;
-  __shared__ alignas(16) uint32_t lp[kFewWaves][16 * kStride];
-  __shared__ float lo[kFewWaves][4][DT * 16];
-  __shared__ float lm[kFewWaves][4], ll[kFewWaves][4];
-  const int thread = here((int)threadIdx.x);  // what is computed from it is not kept from job to job
-  const int lane = thread & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(thread >> 6);
-  const int col = lane & 15, quad = lane >> 4;
-  const Seq8 &s = job.s;
-  const int b = job.b, hk = job.hk, G = a.NH / a.NKV, rows = job.rows, first = job.first, stop = job.stop;
-  const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
+// A row of q is held as whole numbers of 31 bits next to its largest element, and those as four digits of base 256; its products with the codes
+// are exact on the 8-bit matrix units, and so are the weights', 31 bits next to the block's largest, with the values' codes.
 
-  Codes<DT> c(padded(a.HS), lane);
-  Walk walk(a, b, first + wave, stop, kFewWaves, word);
-  float kscale = 0.0f, vscale = 0.0f;
-  if (walk.j < stop) {
-    const size_t at = block_head(walk.id, a.NKV, hk);
-    c.keys(k8, at);
-    c.values(v8, at);
-    kscale = ks[at];
-    vscale = vs[at];
+// What all rows of a wavefront need of a call and a block.
+struct Block8 {
+  const ugk_cache8 &a;
+  const Parts8 &parts;
+  const Job8 &job;
+  int lane, j;
+  bool there;
+  float f, kscale, vexp;  // f: |scale| log2(e) (its sign goes with q)
+  // where the block's m and l of a row go
+  __device__ __forceinline__ float2 *stat(int row) const {
+    return parts.block + (((size_t)job.b * a.NKV + job.hk) * a.max_q * (a.NH / a.NKV) + row) * a.ld_table + j;
   }
+};
 
-  // q's digits: lane (4 row + digit, quad) holds dims 64 step + 16 quad + [0, 16)
+// Four rows: their four digits are one operand of 16 rows, so that a block's scores take two instructions per 16 keys at 128 floats per
+// head, and a lane finds the four digits of its score in its own four registers. A lane has a score of row lane / 16 for each 16 keys.
+template <int DT>
+struct Four {
+  static constexpr int KS = (DT + 3) / 4, kStride = 20, kLds = 16 * kStride;  // kLds words of LDS per wavefront
+  using Scores = float[4];
+  using Weights = v4i;
   v4i aq[KS];
-  int ex;
+  int row, lim, ex;
   bool nan;
-  {
-    const int rr = min(col >> 2, rows - 1);
-    const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (size_t)(hk * G + rr % G) * a.HS;
+  Running run;
+  float o[DT];
+
+  // Rows from row0 on. Lane (4 row + digit, quad) holds dims 64 step + 16 quad + [0, 16) of q.
+  __device__ __forceinline__ void load(const float *q, const ugk_cache8 &a, const Job8 &job, int row0, int lane) {
+    const int col = lane & 15, quad = lane >> 4, G = a.NH / a.NKV, rr = min(row0 + (col >> 2), job.rows - 1);
+    const float *p = q + ((size_t)job.s.q0 + rr / G) * a.ldq + (size_t)(job.hk * G + rr % G) * a.HS;
     float x[KS][16];
     uint32_t most = load_q(p, 16 * quad, 64, a, x);
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
@@ -762,21 +765,15 @@ __device__ __forceinline__ void few_job(float *out, float *lse, const float *q, 
     // for the lanes that hold the row's scores: row quad
     ex = __shfl(e, 4 * quad) - 29;
     nan = (uint32_t)__shfl((int)most, 4 * quad) >= kInfBits;
-  }
-  const int lim = quad < rows ? s.seen(quad / G, a.causal) : 0;
-  Running run;
-  float o[DT];
+    row = row0 + quad;
+    lim = row < job.rows ? job.s.seen(row / G, a.causal) : 0;
 #pragma unroll
-  for (int t = 0; t < DT; t++) o[t] = 0.0f;
-  uint32_t *mylp = lp[wave];
-
-  const auto block = [&](auto next) {  // next: another block follows
-    constexpr bool kNext = decltype(next)::value;
-    const int id = kNext ? walk.ahead(a, b, word) : 0;
-    const size_t ahead = block_head(id, a.NKV, hk);
-    const int seen = walk.there() ? lim - walk.j * kKeys : 0;  // of this block's keys
-    const float fac = nan ? NAN : score_factor(f, kscale, ex), vnow = exponent(vscale);
-    float p[4], mb = -INFINITY;
+    for (int t = 0; t < DT; t++) o[t] = 0.0f;
+  }
+  // The scores' products; the largest.
+  __device__ __forceinline__ float products(const Codes<DT> &c, const Block8 &k, Scores &p) const {
+    const int seen = k.there ? lim - k.j * kKeys : 0, col = k.lane & 15;  // of this block's keys
+    float mb = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 4; kt++) {
       v4i acc = {0, 0, 0, 0};
@@ -785,12 +782,12 @@ __device__ __forceinline__ void few_job(float *out, float *lse, const float *q, 
       p[kt] = kt * 16 + col < seen ? undigits(acc) : -INFINITY;
       mb = fmaxf(mb, p[kt]);
     }
-    __builtin_amdgcn_sched_barrier(0);  // into the registers that the products have read
-    if (kNext) {
-      c.keys(k8, ahead);
-      kscale = ks[ahead];
-      vscale = vs[ahead];
-    }
+    return mb;
+  }
+  // The weights as an operand.
+  __device__ __forceinline__ void weights(Scores &p, float mb, const Block8 &k, uint32_t *lp, Weights &ap, float &fo, float &fb) {
+    const int col = k.lane & 15, quad = k.lane >> 4;
+    const float fac = nan ? NAN : score_factor(k.f, k.kscale, ex);
     mb = top_score(max16(mb), fac);
     const float less = less_top(mb, 0.0f);
     uint32_t y[4];
@@ -802,75 +799,42 @@ __device__ __forceinline__ void few_job(float *out, float *lse, const float *q, 
       y[kt] = digits((int)(p[kt] * 0x1p30f));  // (2^30 in the exponent would cost the weights four bits)
     }
     const v4i t = turn4(y[0], y[1], y[2], y[3]);  // the four keys' digits side by side: a word per digit
-    uint32_t *w = mylp + 4 * quad * kStride + col;
+    uint32_t *w = lp + 4 * quad * kStride + col;
 #pragma unroll
     for (int d = 0; d < 4; d++) w[d * kStride] = (uint32_t)t[d];
     __builtin_amdgcn_wave_barrier();
-    const v4i ap = *reinterpret_cast<const v4i *>(mylp + col * kStride + 4 * quad);
+    ap = *reinterpret_cast<const v4i *>(lp + col * kStride + 4 * quad);
     __builtin_amdgcn_wave_barrier();
-    if (parts.block) {
+    if (k.parts.block) {
       const float sum = sum16(lb);
-      if (col == 0 && quad < rows)
-        parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + quad) * a.ld_table + walk.j] = make_float2(mb, sum);
+      if (col == 0 && row < k.job.rows) *k.stat(row) = make_float2(mb, sum);
     }
     run.sum(mb, lb, mb, 0.0f);
-    const float fo = run.stand(mb, vnow), fb = run.factor(mb, vnow);
+    fo = run.stand(mb, k.vexp);
+    fb = run.factor(mb, k.vexp);
+  }
+  __device__ __forceinline__ void add(const Codes<DT> &c, const Weights &ap, float fo, float fb) {
 #pragma unroll
     for (int t = 0; t < DT; t++) {
       const v4i acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap, c.vf[t], v4i{0, 0, 0, 0}, 0, 0, 0);
       o[t] = here(fmaf(undigits(acc), fb, o[t] * fo));
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if (kNext) c.values(v8, ahead);
-    if (kNext) walk.step(id);
-  };
-  while (walk.more()) block(std::true_type{});
-  if (walk.j < stop) block(std::false_type{});
-
-  // the wavefronts' sums
-  const float sum = sum16(run.l);
-  int e;
-  const float g = run.last(sum, &e);
-  e -= 30;  // of the weights' whole numbers
-#pragma unroll
-  for (int t = 0; t < DT; t++) lo[wave][quad][16 * t + col] = __builtin_amdgcn_ldexpf(o[t] * g, e);
-  if (col == 0) {
-    lm[wave][quad] = run.m;
-    ll[wave][quad] = sum;
   }
-  __syncthreads();
-  const int r = threadIdx.x >> 6;
-  if (r >= rows) return;
-  float top = -INFINITY, total = 0.0f, wt[kFewWaves];
+  // Outputs, maxima and sums to LDS.
+  __device__ __forceinline__ void put(float *lo, int stride, float *lm, float *ll, int lane) const {
+    const int col = lane & 15, quad = lane >> 4;
+    const float sum = sum16(run.l);
+    int e;
+    const float g = run.last(sum, &e);
+    e -= 30;  // of the weights' whole numbers
 #pragma unroll
-  for (int w = 0; w < kFewWaves; w++) top = fmaxf(top, lm[w][r]);
-#pragma unroll
-  for (int w = 0; w < kFewWaves; w++) {
-    wt[w] = ll[w][r] == 0.0f ? 0.0f : ll[w][r] * ex2(lm[w][r] - or0(top));
-    total += wt[w];
+    for (int t = 0; t < DT; t++) lo[quad * stride + 16 * t + col] = __builtin_amdgcn_ldexpf(o[t] * g, e);
+    if (col == 0) {
+      lm[quad] = run.m;
+      ll[quad] = sum;
+    }
   }
-  const Place8 to(out, lse, parts, a, job.slot, job.whole, r, (size_t)s.q0 + r / G, hk * G + r % G);
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  for (int d = lane; d < a.HS; d += kWave) {
-    float y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; w++) y = fmaf(wt[w] * inv, lo[w][r][d], y);
-    to.o[d] = y;
-  }
-  if (lane == 0) to.put(top, total);
-}
-
-template <int DT, bool kShared>
-__global__ __launch_bounds__(kFewWaves *kWave, DT >= 6 ? 3 : 4) void k_cache8_few(float *out, float *lse, const float *q, const int8_t *k8, const float *ks,
-                               const int8_t *v8, const float *vs, ugk_cache8 a, Parts8 parts, unsigned pairs,
-                               unsigned groups, int *word) {
-  Jobs<4, 4, kShared> jobs(a, parts, pairs, groups, word);
-  Job8 job;
-  for (bool more = jobs.first(job); more; more = jobs.next(job)) {
-    few_job<DT>(out, lse, q, k8, ks, v8, vs, a, parts, job, word);
-    __syncthreads();  // LDS is read until here
-  }
-}
+};
 
 // x of the lanes that hold the same row in the four quarters of a wavefront, combined.
 __device__ __forceinline__ float quarters_max(float x) {
@@ -882,43 +846,26 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// Up to 16 RW rows: drafts, large groups, an observation window (in `groups` of them). The same products transposed, with an operand per digit:
-// a lane holds 16 scores of one row, and its weights are the second product's operand as they stand, for a column of
-// the values' codes has its keys in the order in which the lanes hold them. A wavefront has 16 rows; with RW 2 two of them take the
-// same blocks, which the second finds in a cache.
-template <int DT, int RW>
-__device__ __forceinline__ void some_job(float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8,
-                                         const float *vs, const ugk_cache8 &a, const Parts8 &parts, const Job8 &job, int *word) {
-  constexpr int KS = (DT + 3) / 4, kStride = 16 * DT + 4, KW = kFewWaves / RW;
-  __shared__ alignas(16) float lo[kFewWaves][16 * kStride];
-  __shared__ float lm[kFewWaves][16], ll[kFewWaves][16];
-  const int thread = here((int)threadIdx.x);  // what is computed from it is not kept from job to job
-  const int lane = thread & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(thread >> 6);
-  const int col = lane & 15, quad = lane >> 4;
-  const Seq8 &s = job.s;
-  const int b = job.b, hk = job.hk, G = a.NH / a.NKV, rows = job.rows, row0 = job.group * 16 * RW, first = job.first, stop = job.stop;
-  const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
-
-  Codes<DT> c(padded(a.HS), lane);
-  Walk walk(a, b, first + wave % KW, stop, KW, word);
-  float kscale = 0.0f, vscale = 0.0f;
-  if (walk.j < stop) {
-    const size_t at = block_head(walk.id, a.NKV, hk);
-    c.keys(k8, at);
-    c.values(v8, at);
-    kscale = ks[at];
-    vscale = vs[at];
-  }
-
+// Sixteen rows: the same products transposed, with an operand per digit. A lane holds 16 scores of one row, lane % 16, and its weights are
+// the second product's operand as they stand, for a column of the values' codes has its keys in the order in which the lanes hold them.
+template <int DT>
+struct Sixteen {
+  static constexpr int KS = (DT + 3) / 4, kLds = 4;  // (none)
+  using Scores = float[4][4];
+  using Weights = v4i[4];
   v4i aq[KS][4];
-  const int mine = row0 + 16 * (wave / KW) + col, lim = mine < rows ? s.seen(mine / G, a.causal) : 0;
-  int ex;
+  int row, lim, least, ex;  // least: what the first row sees
   bool nan;
   Running run;
   float o[DT][4];
-  {
-    const int rr = min(mine, rows - 1);
-    const float *p = q + ((size_t)s.q0 + rr / G) * a.ldq + (size_t)(hk * G + rr % G) * a.HS;
+
+  __device__ __forceinline__ void load(const float *q, const ugk_cache8 &a, const Job8 &job, int row0, int lane) {
+    const int quad = lane >> 4, G = a.NH / a.NKV;
+    row = row0 + (lane & 15);
+    lim = row < job.rows ? job.s.seen(row / G, a.causal) : 0;
+    least = job.s.seen(min(row0, job.rows - 1) / G, a.causal);
+    const int rr = min(row, job.rows - 1);
+    const float *p = q + ((size_t)job.s.q0 + rr / G) * a.ldq + (size_t)(job.hk * G + rr % G) * a.HS;
     float x[KS][16];
     uint32_t most = load_q(p, 16 * quad, 64, a, x);
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
@@ -941,17 +888,8 @@ __device__ __forceinline__ void some_job(float *out, float *lse, const float *q,
 #pragma unroll
       for (int r = 0; r < 4; r++) o[t][r] = 0.0f;
   }
-  const int least = s.seen(row0 / G, a.causal);
-
-  const auto block = [&](auto next) {  // next: another block follows
-    constexpr bool kNext = decltype(next)::value;
-    const int id = kNext ? walk.ahead(a, b, word) : 0;
-    const size_t ahead = block_head(id, a.NKV, hk);
-    const bool masked = !walk.there() || (walk.j + 1) * kKeys > least;
-    const int seen = walk.there() ? lim - walk.j * kKeys - 4 * quad : 0;  // of this block's keys from the lane's first on
-    const float vnow = exponent(vscale);
-    const float fac = nan ? NAN : score_factor(f, kscale, ex);
-    float p[4][4], mb = -INFINITY;
+  __device__ __forceinline__ float products(const Codes<DT> &c, const Block8 &k, Scores &p) const {
+    float mb = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 4; kt++) {
       __builtin_amdgcn_sched_barrier(0);  // tile by tile: the registers hold one tile's digits
@@ -963,12 +901,10 @@ __device__ __forceinline__ void some_job(float *out, float *lse, const float *q,
         for (int st = 0; st < KS; st++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.kf[st][kt], aq[st][d], acc[d], 0, 0, 0);
       }
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        p[kt][r] = here(undigits(v4i{acc[0][r], acc[1][r], acc[2][r], acc[3][r]}));
-      }
+      for (int r = 0; r < 4; r++) p[kt][r] = here(undigits(v4i{acc[0][r], acc[1][r], acc[2][r], acc[3][r]}));
     }
-    if (masked) {
-      const int n = here(seen);
+    if (!k.there || (k.j + 1) * kKeys > least) {
+      const int n = here(k.there ? lim - k.j * kKeys - 4 * (k.lane >> 4) : 0);  // seen of this block's keys from the lane's first on
 #pragma unroll
       for (int kt = 0; kt < 4; kt++)
 #pragma unroll
@@ -978,16 +914,13 @@ __device__ __forceinline__ void some_job(float *out, float *lse, const float *q,
     for (int kt = 0; kt < 4; kt++)
 #pragma unroll
       for (int r = 0; r < 4; r++) mb = fmaxf(mb, p[kt][r]);
-    __builtin_amdgcn_sched_barrier(0);  // into the registers that the products have read
-    if (kNext) {
-      c.keys(k8, ahead);
-      kscale = ks[ahead];
-      vscale = vs[ahead];
-    }
+    return mb;
+  }
+  __device__ __forceinline__ void weights(const Scores &p, float mb, const Block8 &k, uint32_t *, Weights &bp, float &fo, float &fb) {
+    const float fac = nan ? NAN : score_factor(k.f, k.kscale, ex);
     mb = top_score(quarters_max(mb), fac);
     const float less = less_top(mb, 0.0f);
     float lb = 0.0f;
-    v4i bp[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       uint32_t y[4];
@@ -1001,13 +934,15 @@ __device__ __forceinline__ void some_job(float *out, float *lse, const float *q,
 #pragma unroll
       for (int d = 0; d < 4; d++) bp[d][r] = t[d];
     }
-    if (parts.block) {
+    if (k.parts.block) {
       const float sum = quarters_sum(lb);
-      if (quad == 0 && mine < rows)
-        parts.block[(((size_t)b * a.NKV + hk) * a.max_q * G + mine) * a.ld_table + walk.j] = make_float2(mb, sum);
+      if (k.lane < 16 && row < k.job.rows) *k.stat(row) = make_float2(mb, sum);
     }
     run.sum(mb, lb, mb, 0.0f);
-    const float fo = run.stand(mb, vnow), fb = run.factor(mb, vnow);
+    fo = run.stand(mb, k.vexp);
+    fb = run.factor(mb, k.vexp);
+  }
+  __device__ __forceinline__ void add(const Codes<DT> &c, const Weights &bp, float fo, float fb) {
 #pragma unroll
     for (int t = 0; t < DT; t++) {
       if (t % 2 == 0) __builtin_amdgcn_sched_barrier(0);
@@ -1015,10 +950,71 @@ __device__ __forceinline__ void some_job(float *out, float *lse, const float *q,
 #pragma unroll
       for (int d = 0; d < 4; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.vf[t], bp[d], v4i{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        o[t][r] = here(fmaf(undigits(v4i{acc[0][r], acc[1][r], acc[2][r], acc[3][r]}), fb, o[t][r] * fo));
-      }
+      for (int r = 0; r < 4; r++) o[t][r] = here(fmaf(undigits(v4i{acc[0][r], acc[1][r], acc[2][r], acc[3][r]}), fb, o[t][r] * fo));
     }
+  }
+  __device__ __forceinline__ void put(float *lo, int stride, float *lm, float *ll, int lane) const {
+    const int col = lane & 15, quad = lane >> 4;
+    const float sum = quarters_sum(run.l);
+    int e;
+    const float g = run.last(sum, &e);
+    e -= 30;  // of the weights' whole numbers
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+      *reinterpret_cast<float4 *>(&lo[col * stride + 16 * t + 4 * quad]) =
+          make_float4(__builtin_amdgcn_ldexpf(o[t][0] * g, e), __builtin_amdgcn_ldexpf(o[t][1] * g, e),
+                      __builtin_amdgcn_ldexpf(o[t][2] * g, e), __builtin_amdgcn_ldexpf(o[t][3] * g, e));
+    if (quad == 0) {
+      lm[col] = run.m;
+      ll[col] = sum;
+    }
+  }
+};
+
+// Up to R rows: a token's, drafts, large groups, an observation window (in `groups` of them). The wavefronts share the blocks, and a wavefront has all
+// rows, 4 or 16. Of 32 it has half, and two take the same blocks, the second from a cache.
+template <int DT, int R>
+__device__ __forceinline__ void rows_job(float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8,
+                                         const float *vs, const ugk_cache8 &a, const Parts8 &parts, const Job8 &job, int *word) {
+  using Rows = std::conditional_t<R == 4, Four<DT>, Sixteen<DT>>;
+  constexpr int kRow = 16 * DT + 4, kRows = R == 4 ? 4 : 16, KW = R == 32 ? 2 : kFewWaves;
+  __shared__ alignas(16) float lo[kFewWaves][kRows * kRow];
+  __shared__ float lm[kFewWaves][kRows], ll[kFewWaves][kRows];
+  __shared__ alignas(16) uint32_t lp[kFewWaves][Rows::kLds];
+  const int thread = here((int)threadIdx.x);  // what is computed from it is not kept from job to job
+  const int lane = thread & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+  const int stop = job.stop, row0 = job.group * R, hk = job.hk;
+
+  Codes<DT> c(padded(a.HS), lane);
+  Walk walk(a, job.b, job.first + wave % KW, stop, KW, word);
+  float kscale = 0.0f, vscale = 0.0f;
+  if (walk.j < stop) {
+    const size_t at = block_head(walk.id, a.NKV, hk);
+    c.keys(k8, at);
+    c.values(v8, at);
+    kscale = ks[at];
+    vscale = vs[at];
+  }
+  Rows rows;
+  rows.load(q, a, job, row0 + wave / KW * 16, lane);
+
+  const auto block = [&](auto next) {  // next: another block follows
+    constexpr bool kNext = decltype(next)::value;
+    const int id = kNext ? walk.ahead(a, job.b, word) : 0;
+    const size_t ahead = block_head(id, a.NKV, hk);
+    const Block8 k{a, parts, job, lane, walk.j, walk.there(), fabsf(a.scale) * kLog2e8, kscale, exponent(vscale)};
+    typename Rows::Scores p;
+    typename Rows::Weights w;
+    float fo, fb;
+    const float mb = rows.products(c, k, p);
+    __builtin_amdgcn_sched_barrier(0);  // into the registers that the products have read
+    if (kNext) {
+      c.keys(k8, ahead);
+      kscale = ks[ahead];
+      vscale = vs[ahead];
+    }
+    rows.weights(p, mb, k, lp[wave], w, fo, fb);
+    rows.add(c, w, fo, fb);
     __builtin_amdgcn_sched_barrier(0);
     if (kNext) c.values(v8, ahead);
     if (kNext) walk.step(id);
@@ -1026,25 +1022,14 @@ __device__ __forceinline__ void some_job(float *out, float *lse, const float *q,
   while (walk.more()) block(std::true_type{});
   if (walk.j < stop) block(std::false_type{});
 
-  // the sums of the wavefronts that share rows
-  const float sum = quarters_sum(run.l);
-  int e;
-  const float g = run.last(sum, &e);
-  e -= 30;  // of the weights' whole numbers
-#pragma unroll
-  for (int t = 0; t < DT; t++)
-    *reinterpret_cast<float4 *>(&lo[wave][col * kStride + 16 * t + 4 * quad]) =
-        make_float4(__builtin_amdgcn_ldexpf(o[t][0] * g, e), __builtin_amdgcn_ldexpf(o[t][1] * g, e),
-                    __builtin_amdgcn_ldexpf(o[t][2] * g, e), __builtin_amdgcn_ldexpf(o[t][3] * g, e));
-  if (quad == 0) {
-    lm[wave][col] = run.m;
-    ll[wave][col] = sum;
-  }
+  rows.put(lo[wave], kRow, lm[wave], ll[wave], lane);
   __syncthreads();
-#pragma unroll 1
-  for (int x = wave; x < 16 * RW; x += kFewWaves) {
-    const int r = x & 15, w0 = x / 16 * KW, row = row0 + x;
-    if (row >= rows) break;
+  // a row's sums of the wavefronts that have it; 16 lanes to a row, or a wavefront
+  constexpr int kLanes = R == 4 ? kWave : 16, kAtOnce = kWave / kLanes;
+  const int G = a.NH / a.NKV, d0 = 4 * (lane & (kLanes - 1));
+  for (int n0 = kAtOnce * wave; n0 < R; n0 += kAtOnce * kFewWaves) {
+    const int n = n0 + lane / kLanes, r = n % kRows, w0 = n / kRows * KW, row = row0 + n;
+    if (row >= job.rows) break;
     float top = -INFINITY, total = 0.0f, wt[KW];
 #pragma unroll
     for (int w = 0; w < KW; w++) top = fmaxf(top, lm[w0 + w][r]);
@@ -1053,26 +1038,32 @@ __device__ __forceinline__ void some_job(float *out, float *lse, const float *q,
       wt[w] = ll[w0 + w][r] == 0.0f ? 0.0f : ll[w0 + w][r] * ex2(lm[w0 + w][r] - or0(top));
       total += wt[w];
     }
-    const Place8 to(out, lse, parts, a, job.slot, job.whole, x, (size_t)s.q0 + row / G, hk * G + row % G);
+    const int i = parts.inverse ? (int)__umulhi((unsigned)row, parts.inverse) : row;
+    const Place8 to(out, lse, parts, a, job.slot, job.whole, n, (size_t)job.s.q0 + i, hk * G + row - i * G);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    for (int d = lane; d < a.HS; d += kWave) {
-      float y = 0.0f;
 #pragma unroll
-      for (int w = 0; w < KW; w++) y = fmaf(wt[w] * inv, lo[w0 + w][r * kStride + d], y);
-      to.o[d] = y;
+    for (int d = d0; d < 16 * DT; d += 4 * kLanes) {
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < KW; w++) {
+        const float4 z = ld4(&lo[w0 + w][r * kRow + d]);
+        const float f = wt[w] * inv;
+        y = make_float4(fmaf(f, z.x, y.x), fmaf(f, z.y, y.y), fmaf(f, z.z, y.z), fmaf(f, z.w, y.w));
+      }
+      put4(to.o + d, y, a.HS - d);
     }
-    if (lane == 0) to.put(top, total);
+    if (d0 == 0) to.put(top, total);
   }
 }
 
-template <int DT, int RW, bool kShared>
-__global__ __launch_bounds__(kFewWaves *kWave, 2) void k_cache8_some(float *out, float *lse, const float *q, const int8_t *k8, const float *ks,
-                               const int8_t *v8, const float *vs, ugk_cache8 a, Parts8 parts, unsigned pairs,
-                               unsigned groups, int *word) {
-  Jobs<16 * RW, 4, kShared> jobs(a, parts, pairs, groups, word);
+template <int DT, int R, bool kShared>
+__global__ __launch_bounds__(kFewWaves *kWave, R > 4 ? 2 : DT >= 6 ? 3 : 4) void k_cache8_rows(
+    float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8, const float *vs, ugk_cache8 a, Parts8 parts,
+    unsigned pairs, unsigned groups, int *word) {
+  Jobs<R, 6, kShared> jobs(a, parts, pairs, groups, word);
   Job8 job;
   for (bool more = jobs.first(job); more; more = jobs.next(job)) {
-    some_job<DT, RW>(out, lse, q, k8, ks, v8, vs, a, parts, job, word);
+    rows_job<DT, R>(out, lse, q, k8, ks, v8, vs, a, parts, job, word);
     __syncthreads();  // LDS is read until here
   }
 }
@@ -1189,16 +1180,7 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
   }
   const bool none = l == 0.0f;
   const float inv = none ? 1.0f : 1.0f / l;
-  float *po = out + g * a.ldo + (size_t)h * a.HS + d;
-  const int nd = a.HS - d;
-  const float4 y = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-  if (nd >= 4) {
-    st4(po, y);
-  } else if (nd > 0) {
-    po[0] = y.x;
-    if (nd > 1) po[1] = y.y;
-    if (nd > 2) po[2] = y.z;
-  }
+  put4(out + g * a.ldo + (size_t)h * a.HS + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.HS - d);
   if (lse && d == 0) lse[g * a.NH + h] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn28;
 }
 
@@ -1398,25 +1380,15 @@ __device__ __forceinline__ void tile_job(float *out, float *lse, const float *q,
   const float g = run.last(sum, &p);
   p -= 14;  // of the weights
   const Place8 to(out, lse, parts, a, job.slot, job.whole, mine - row0, (size_t)s.q0 + i, h);
-  float *po = to.o;
 #pragma unroll
   for (int t = 0; t < D32; t++)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const int d = 32 * t + 8 * (r / 4) + 4 * half, nd = a.HS - d;
-      if (nd <= 0) continue;
-      float4 y;
-      y.x = __builtin_amdgcn_ldexpf(o[t][r] * g, p);
-      y.y = __builtin_amdgcn_ldexpf(o[t][r + 1] * g, p);
-      y.z = __builtin_amdgcn_ldexpf(o[t][r + 2] * g, p);
-      y.w = __builtin_amdgcn_ldexpf(o[t][r + 3] * g, p);
-      if (nd >= 4) {
-        st4(po + d, y);
-      } else {
-        po[d] = y.x;
-        if (nd > 1) po[d + 1] = y.y;
-        if (nd > 2) po[d + 2] = y.z;
-      }
+      const int d = 32 * t + 8 * (r / 4) + 4 * half;
+      put4(to.o + d,
+           make_float4(__builtin_amdgcn_ldexpf(o[t][r] * g, p), __builtin_amdgcn_ldexpf(o[t][r + 1] * g, p),
+                       __builtin_amdgcn_ldexpf(o[t][r + 2] * g, p), __builtin_amdgcn_ldexpf(o[t][r + 3] * g, p)),
+           a.HS - d);
     }
   if (half == 0) to.put(run.m, sum);
 }
@@ -1555,7 +1527,7 @@ int cu_count8() {
   return n;
 }
 
-// How an attention call is cut: k_cache8_few (rows 4), k_cache8_some (16, 32) in so many groups, or k_cache8_tile (128) in so many
+// How an attention call is cut: k_cache8_rows (4, 16, 32 rows) in so many groups, or k_cache8_tile (128) in so many
 // tiles; `wgs` workgroups that share all blocks, or up to `splits` parts of `least` blocks or more of each; the rows of a slot of
 // parts, the slots, and where a job's are.
 struct Plan8 {
@@ -1573,7 +1545,7 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   p.step = 1;
   p.splits = 1;
   const bool narrow = a.HS <= 64;
-  const int cus = cu_count8(), at_once = cus * (p.rows == 4 ? (narrow ? 4 : 3) : p.rows == kTileRows8 ? (narrow ? 3 : 2) : (narrow ? 4 : 2));
+  const int cus = cu_count8(), at_once = cus * (p.rows == 4 ? (narrow ? 4 : 3) : narrow ? 3 : 2);
   // at most so many jobs, and the shares of so many blocks, were all sequences full
   const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / at_once;
   // what a workspace of the same rows and heads has for the fp32 attention
@@ -1642,19 +1614,22 @@ int launch_cache8_attention(float *out, float *lse, const float *q, const void *
     const int d = a.HS <= 32 ? 2 : a.HS <= 64 ? 4 : a.HS <= 96 ? 6 : 8;
     switch (p.rows) {
       case 4:
-        d == 2 ? go(k_cache8_few<2, kS>) : d == 4 ? go(k_cache8_few<4, kS>) : d == 6 ? go(k_cache8_few<6, kS>) : go(k_cache8_few<8, kS>);
+        d == 2   ? go(k_cache8_rows<2, 4, kS>)
+        : d == 4 ? go(k_cache8_rows<4, 4, kS>)
+        : d == 6 ? go(k_cache8_rows<6, 4, kS>)
+                 : go(k_cache8_rows<8, 4, kS>);
         break;
       case 16:
-        d == 2   ? go(k_cache8_some<2, 1, kS>)
-        : d == 4 ? go(k_cache8_some<4, 1, kS>)
-        : d == 6 ? go(k_cache8_some<6, 1, kS>)
-                 : go(k_cache8_some<8, 1, kS>);
+        d == 2   ? go(k_cache8_rows<2, 16, kS>)
+        : d == 4 ? go(k_cache8_rows<4, 16, kS>)
+        : d == 6 ? go(k_cache8_rows<6, 16, kS>)
+                 : go(k_cache8_rows<8, 16, kS>);
         break;
       case 32:
-        d == 2   ? go(k_cache8_some<2, 2, kS>)
-        : d == 4 ? go(k_cache8_some<4, 2, kS>)
-        : d == 6 ? go(k_cache8_some<6, 2, kS>)
-                 : go(k_cache8_some<8, 2, kS>);
+        d == 2   ? go(k_cache8_rows<2, 32, kS>)
+        : d == 4 ? go(k_cache8_rows<4, 32, kS>)
+        : d == 6 ? go(k_cache8_rows<6, 32, kS>)
+                 : go(k_cache8_rows<8, 32, kS>);
         break;
       default:
         d == 2 ? go(k_cache8_tile<2, kS>) : d == 4 ? go(k_cache8_tile<4, kS>) : d == 6 ? go(k_cache8_tile<6, kS>) : go(k_cache8_tile<8, kS>);
