@@ -525,15 +525,6 @@ struct Walk {
 };
 __device__ __forceinline__ size_t block_head(int id, int NKV, int hk) { return (size_t)max(id, 0) * NKV + hk; }
 
-// The sum over the lanes up to this one (a shuffle through LDS for each step took a microsecond more).
-__device__ __forceinline__ int wave_scan_int(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes below in a row of 16
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of the row before, of the first two rows
-  return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-}
 __device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, kWave - 1); }
 
 // What a workgroup has at a time: of group `group` of R rows of a sequence and key/value head blocks [first, stop).
@@ -604,8 +595,8 @@ struct Jobs {
       if (b0 == 0) one = h;
     }
     longest = (int)wave_max_bits((uint32_t)longest);
-    jobs = last_lane(wave_scan_int(jobs)) * a.NKV;
-    all = last_lane(wave_scan_int(all)) * a.NKV;
+    jobs = last_lane(wave_scan(jobs)) * a.NKV;
+    all = last_lane(wave_scan(all)) * a.NKV;
     // no group has much more than a CU's share: the parts' way through memory would cost more than they save
     whole = (long long)2 * longest * parts.cus <= 3LL * (all - kBegin * jobs);
     share = whole ? 1 : max(parts.least, (all + parts.wgs - 1) / parts.wgs);
@@ -618,7 +609,7 @@ struct Jobs {
     int x = at, n = 0;
     for (int b0 = 0; b0 < a.nseq; b0 += kWave) {
       h = b0 ? held(b0 + lane, false, &longest) : one;
-      const int to = wave_scan_int(h.units) * a.NKV, before = wave_scan_int(h.n);
+      const int to = wave_scan(h.units) * a.NKV, before = wave_scan(h.n);
       const uint64_t over = __ballot(to > x);
       if (over) {
         const int l = __builtin_ctzll(over);
@@ -636,7 +627,7 @@ struct Jobs {
     }
     w.group = 0;
     for (int t0 = 0; t0 < n; t0 += kWave) {
-      const int t = n - 1 - t0 - lane, mine = t < 0 ? 0 : units(blocks_of(w.s, t)) * a.NKV, to = wave_scan_int(mine);
+      const int t = n - 1 - t0 - lane, mine = t < 0 ? 0 : units(blocks_of(w.s, t)) * a.NKV, to = wave_scan(mine);
       const uint64_t over = __ballot(to > x);
       if (over) {
         const int l = __builtin_ctzll(over);
@@ -1412,12 +1403,7 @@ constexpr int kEvictThreads = 1024, kBins = 2 * kEvictThreads;
 // Sum over the workgroup's threads before this one, and in *all over all of them.
 __device__ __forceinline__ int before(int x, int *lds, int *all) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  int y = x;
-#pragma unroll
-  for (int o = 1; o < kWave; o *= 2) {
-    const int z = __shfl_up(y, o);
-    if (lane >= o) y += z;
-  }
+  const int y = wave_scan(x);
   __syncthreads();  // the last call's sums have been read
   if (lane == kWave - 1) lds[wave] = y;
   __syncthreads();

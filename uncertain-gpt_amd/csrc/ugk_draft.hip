@@ -16,22 +16,6 @@ constexpr int kDraftThreads = 1024, kDraftWaves = kDraftThreads / kWave, kSumThr
 constexpr int kStep = 4 * kDraftThreads;  // floats that a workgroup takes at a time
 constexpr int kMaxSegs = 1024;            // segments of a row
 
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
-}
-// The sum over the lanes up to this one.
-__device__ __forceinline__ double wave_scan64(double x) {
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int o = 1; o < kWave; o *= 2) {
-    const double z = __shfl_up(x, o);
-    if (lane >= o) x += z;
-  }
-  return x;
-}
-
 // One sequence's row that its next token is drawn from: p, less the drafts' probabilities of the row (or null) or without the
 // one token (or -1) whose draft was certain; what is not positive and finite counts as 0.
 struct Row {
@@ -145,8 +129,8 @@ __global__ __launch_bounds__(kSumThreads) void k_draft_sums(double *sums, int *a
 #pragma unroll
       for (int j = 0; j < 4; j++) t[j] += x[i][j];
   }
-  const double sum = wave_sum64((t[0] + t[1]) + (t[2] + t[3]));
-  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = sum;
+  const double sum = wave_scan((t[0] + t[1]) + (t[2] + t[3]));
+  if ((threadIdx.x & (kWave - 1)) == kWave - 1) part[threadIdx.x / kWave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
@@ -184,8 +168,8 @@ __device__ int draw(const Row &r, int V, int segs, int seg, double u, const doub
 #pragma unroll
             for (int j = 0; j < 4; j++) t[j] += x[i][j];
         }
-        const double sum = wave_sum64((t[0] + t[1]) + (t[2] + t[3]));
-        if (lane == 0) lds.seg[s] = sum;
+        const double sum = wave_scan((t[0] + t[1]) + (t[2] + t[3]));
+        if (lane == kWave - 1) lds.seg[s] = sum;
       }
     }
     __syncthreads();
@@ -193,7 +177,7 @@ __device__ int draw(const Row &r, int V, int segs, int seg, double u, const doub
     const int per = (segs + kWave - 1) / kWave, s0 = min(lane * per, segs), s1 = min(s0 + per, segs);
     double mine = 0.0;
     for (int s = s0; s < s1; s++) mine += lds.seg[s];
-    const double to = wave_scan64(mine), total = __shfl(to, kWave - 1);
+    const double to = wave_scan(mine), total = __shfl(to, kWave - 1);
     any = total > 0.0;
     target = u * total;
     // the first segment that the sum passes the target in, or else the last that has any mass
@@ -220,7 +204,7 @@ __device__ int draw(const Row &r, int V, int segs, int seg, double u, const doub
     double y[1][4];
     r.quads(v, 0, end, v0 + kStep <= end, y);
     const double (&x)[4] = y[0];
-    const double mine = (x[0] + x[1]) + (x[2] + x[3]), up = wave_scan64(mine);
+    const double mine = (x[0] + x[1]) + (x[2] + x[3]), up = wave_scan(mine);
     __syncthreads();  // the last step's have been read
     if (lane == kWave - 1) lds.wave[wave] = up;
     if (threadIdx.x == 0) {

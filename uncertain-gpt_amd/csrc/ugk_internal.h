@@ -113,6 +113,30 @@ constexpr int kDppQuadSwap2 = 0x4e;   // quad_perm [2,3,0,1]
 constexpr int kDppHalfMirror = 0x141; // row_half_mirror: lane i <-> 7 - i within 8
 constexpr int kDppMirror = 0x140;     // row_mirror: lane i <-> 15 - i within 16
 
+// Sum over the lanes of a wavefront up to this one, all lanes active: from 1, 2, 4 and 8
+// lanes below within a row of 16, then the last lane of row 0 (2) to row 1 (3), and of row 1
+// to rows 2 and 3. (With shuffles, six round trips through LDS, k_draft_verify of 27 tokens
+// took 5.2 us and not 4.5, k_cache8_evict of 16 blocks of each sequence 6.5 and not 5.4.)
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int scan_step(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false);
+}
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double scan_step(double x) {
+  const long long b = __double_as_longlong(x);
+  const unsigned lo = (unsigned)scan_step<kCtrl, kRows>((int)b), hi = (unsigned)scan_step<kCtrl, kRows>((int)(b >> 32));
+  return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T x) {
+  x += scan_step<0x111, 0xf>(x);
+  x += scan_step<0x112, 0xf>(x);
+  x += scan_step<0x114, 0xf>(x);
+  x += scan_step<0x118, 0xf>(x);
+  x += scan_step<0x142, 0xa>(x);
+  return x + scan_step<0x143, 0xc>(x);
+}
+
 // Sum over the 64 lanes of a wavefront, all lanes active; every lane gets the
 // same bits. Within each row of 16 lanes, four DPP steps each add the value
 // of a partner lane (partners then hold the same two operands, so the same
