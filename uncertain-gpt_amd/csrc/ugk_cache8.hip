@@ -392,10 +392,18 @@ __device__ __forceinline__ float score_factor(float f, float ks, int x) {
                                           __builtin_amdgcn_frexp_expf(f) + __builtin_amdgcn_frexp_expf(ks) + x);
   return fmaxf(fminf(y, 3.402823466e38f), 0x1p-126f);
 }
+// x is computed here, in this branch: the compiler otherwise moves what only the next step of a loop uses behind the branches in between, and holds all
+// that it is computed from until there; and a choice between a number and NaN, made once, it makes again for all that is computed with it.
+template <typename T>
+__device__ __forceinline__ T here(T x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // The largest score of a block from the largest product, and what is added to a score times the factor so that 2^ of it is the weight times
 // 2^up: a score beyond the range makes it NaN.
 __device__ __forceinline__ float top_score(float product, float fac) { return product == -INFINITY ? product : product * fac; }
-__device__ __forceinline__ float less_top(float top, float up) { return top == INFINITY ? NAN : up - or0(top); }
+__device__ __forceinline__ float less_top(float top, float up) { return here(top == INFINITY ? NAN : up - or0(top)); }
 
 // Sum and maximum over the 16 lanes of a row.
 __device__ __forceinline__ float sum16(float v) {
@@ -450,14 +458,6 @@ struct Codes {
     for (int t = 0; t < DT; t++) vf[t] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(p + min(t, HP / 16 - 1) * 16 * kKeys + voff));
   }
 };
-
-// x is computed here, in this branch: the compiler otherwise moves what only the next step of a loop uses behind the branches in between, and holds all
-// that it is computed from until there.
-template <typename T>
-__device__ __forceinline__ T here(T x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
 
 // A 4 x 4 transposition of bytes: the words' bytes 0, then 1, 2 and 3.
 __device__ __forceinline__ v4i turn4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -778,7 +778,7 @@ struct Four {
   // The weights as an operand.
   __device__ __forceinline__ void weights(Scores &p, float mb, const Block8 &k, uint32_t *lp, Weights &ap, float &fo, float &fb) {
     const int col = k.lane & 15, quad = k.lane >> 4;
-    const float fac = nan ? NAN : score_factor(k.f, k.kscale, ex);
+    const float fac = here(nan ? NAN : score_factor(k.f, k.kscale, ex));
     mb = top_score(max16(mb), fac);
     const float less = less_top(mb, 0.0f);
     uint32_t y[4];
@@ -908,7 +908,7 @@ struct Sixteen {
     return mb;
   }
   __device__ __forceinline__ void weights(const Scores &p, float mb, const Block8 &k, uint32_t *, Weights &bp, float &fo, float &fb) {
-    const float fac = nan ? NAN : score_factor(k.f, k.kscale, ex);
+    const float fac = here(nan ? NAN : score_factor(k.f, k.kscale, ex));
     mb = top_score(quarters_max(mb), fac);
     const float less = less_top(mb, 0.0f);
     float lb = 0.0f;
@@ -1284,7 +1284,7 @@ __device__ __forceinline__ void tile_job(float *out, float *lse, const float *q,
       *reinterpret_cast<v2u *>(vt + vdst[n] + 32) = halves4(__builtin_amdgcn_perm(t3, t1, 0x05040100u));
       *reinterpret_cast<v2u *>(vt + vdst[n] + 48) = halves4(__builtin_amdgcn_perm(t3, t1, 0x07060302u));
     }
-    const float fac = nan ? NAN : score_factor(f, kscale, e), vnow = exponent(vscale);
+    const float fac = here(nan ? NAN : score_factor(f, kscale, e)), vnow = exponent(vscale);
     const bool held = there;
     __syncthreads();
     if (j + 1 < stop) fetch(j + 1);
@@ -1334,7 +1334,7 @@ __device__ __forceinline__ void tile_job(float *out, float *lse, const float *q,
       for (int t = 0; t < D32; t++) o[t] *= x;
     }
     // The weights stand on what the output's sum stands on, times 2^14: the products add up in its registers.
-    const float up = 14.0f + (vnow - run.e), less = mb == INFINITY ? NAN : up - or0(run.mo);
+    const float up = 14.0f + (vnow - run.e), less = here(mb == INFINITY ? NAN : up - or0(run.mo));
     float lb = 0.0f;
     const bool apart = __any(run.e - vnow > 64.0f);  // weights that the row's sum needs may vanish next to another block's values
     if (apart) {
