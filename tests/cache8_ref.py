@@ -6,7 +6,8 @@ Error bounds of the attention (u = 2^-24). A row of q is off by 2^-30 of its lar
 roundings in the second, and up to 8 roundings of the parts' sum and the factor: off by e_s = ((2 HS + 8) u + 2^-23) scale sum |q k|
 + 2^-30 scale max|q| sum |k| at most. p = 2^(s - m) is off by a factor of e^(2 e_s) (its own score's error and the
 maximum's), the rounding of its exponent (|s - m| u, and as much for the block's maximum against the row's) and of three exponentials (4 u each).
-A weight is held to 2^-31 of the block's largest, or 2^-23 of itself and 2^-38 of that, and a block's largest is at most the row's. A sum of n
+A weight is held to 2^-31 of the block's largest, or 2^-23 of itself and 2^-38 of that (of two halves, as seen through the
+values' scales: of the largest contribution), and a block's largest is at most the row's. A sum of n
 products adds n u (2 n for two halves), the blocks' and parts' factors 16 u.
 """
 import math

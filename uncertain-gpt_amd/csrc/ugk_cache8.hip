@@ -47,8 +47,8 @@ __device__ __forceinline__ Seq8 sequence8(const ugk_cache8 &a, int b, bool tell,
   return s;
 }
 
-// What the table says of block j of sequence b, and the block, or -1 (reported) where that is none. (Two steps: a loop reads the
-// table a turn before it needs the block.)
+// What the table says of block j of sequence b, and the block, or -1 (reported) where that is none. (Two steps: a loop reads
+// the table a turn before it needs the block.)
 __device__ __forceinline__ int table_at(const ugk_cache8 &a, int b, int j) {
   const size_t at = (size_t)b * a.ld_table + j;
   return a.table ? a.table[at] : (int)at;
@@ -110,7 +110,9 @@ __device__ __forceinline__ bool touched(const ugk_cache8 &a, int per, int *word,
 // One block of one head and of k or v (blockIdx.y) by a workgroup. A thread has four columns of the rows
 // c, c + 16, c + 32, c + 48, whose codes are one word of each of the value's columns.
 //
-// Bound by memory: 4 bytes read and 1 written per number (what a token behind others costs is the launch).
+// Bound by memory: 4 bytes read and 1 written per number, 4.4 TB/s of 8 x 1,024 keys and values of 12 heads of 64 (14.2 us),
+// 5.4 the way back (k_cache8_load, 11.7 us). A token behind others costs the launch and three loads that depend on
+// each other: 4.4 us of 4 sequences, 6.4 of 24 with 8 heads of 128.
 template <int CH>
 __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, int8_t *v8, float *vs, const float *k, const float *v,
                                                          ugk_cache8 a, int per, int *word) {
@@ -294,8 +296,9 @@ __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, cons
 
 // ---- attention --------------------------------------------------------------------
 
-// Parts of the key axis: o normalised, the maximum m of its scores in base 2 and the sum l of 2^(s - m), per slot and row of a group;
-// `block`: the same m and l of each block of 64 keys, and `stat` of rows that have no parts (for the blocks' weights).
+// Parts of the key axis: o normalised, the maximum m of its scores in base 2 and the sum l of 2^(s - m), per slot and row of
+// a group; `block`: the same m and l of each block of 64 keys, and `stat` of rows that have no parts (for the blocks'
+// weights).
 struct Parts8 {
   float *o;
   float2 *ml, *block, *stat;
@@ -348,8 +351,8 @@ struct Running {
   }
 };
 
-// S times N floats of a row of q from `first` on, `step` apart, 0 behind its HS, with the sign of the scores' scale; and the largest
-// magnitude's bits. (One branch for all: a branch for each N would wait for its loads.)
+// S times N floats of a row of q from `first` on, `step` apart, 0 behind its HS, with the sign of the scores' scale; and the
+// largest magnitude's bits. (One branch for all: a branch for each N would wait for its loads.)
 template <int S, int N>
 __device__ __forceinline__ uint32_t load_q(const float *p, int first, int step, const ugk_cache8 &a, float (&x)[S][N]) {
   if (a.HS % 4 == 0) {
@@ -392,16 +395,17 @@ __device__ __forceinline__ float score_factor(float f, float ks, int x) {
                                           __builtin_amdgcn_frexp_expf(f) + __builtin_amdgcn_frexp_expf(ks) + x);
   return fmaxf(fminf(y, 3.402823466e38f), 0x1p-126f);
 }
-// x is computed here, in this branch: the compiler otherwise moves what only the next step of a loop uses behind the branches in between, and holds all
-// that it is computed from until there; and a choice between a number and NaN, made once, it makes again for all that is computed with it.
+// x is computed here, in this branch: the compiler otherwise moves what only the next step of a loop uses behind the branches
+// in between, and holds all that it is computed from until there; and a choice between a number and NaN, made once, it makes
+// again for all that is computed with it.
 template <typename T>
 __device__ __forceinline__ T here(T x) {
   asm volatile("" : "+v"(x));
   return x;
 }
 
-// The largest score of a block from the largest product, and what is added to a score times the factor so that 2^ of it is the weight times
-// 2^up: a score beyond the range makes it NaN.
+// The largest score of a block from the largest product, and what is added to a score times the factor so that 2^ of it is
+// the weight times 2^up: a score beyond the range makes it NaN.
 __device__ __forceinline__ float top_score(float product, float fac) { return product == -INFINITY ? product : product * fac; }
 __device__ __forceinline__ float less_top(float top, float up) { return here(top == INFINITY ? NAN : up - or0(top)); }
 
@@ -540,15 +544,18 @@ __device__ __forceinline__ int parts_for(int nb, int chunk) { return max(1, (nb 
 
 // The workgroup's jobs, one after another.
 //
-// Where the key axis is cut over all CUs (parts.wgs), the blocks of all sequences, groups (the last rows first) and key/value heads are one long row,
-// from what the sequences really hold, of which every workgroup has the same share: it may begin and end within a job. Equal shares are what
-// counts: the CUs' time is their matrix units' or their part of the memory's, and a CU that holds two workgroups
-// is done no sooner than one that holds one of twice their blocks. A job's beginning (its rows, their results) counts as kBegin blocks.
-// Every wavefront finds its place alike, a lane to a sequence, then to a group.
-// Else workgroups are of pairs, groups (the longest first) and parts in turn.
+// Shared: the blocks of all sequences, groups (the last rows first) and key/value heads are one long row, from what the
+// sequences really hold, of which every workgroup has the same share: it may begin and end within a job. Equal shares are
+// what counts, for the CUs' time is their matrix and vector units' or their part of the memory's, and a CU that holds two
+// workgroups is done no sooner than one that holds one of twice their blocks. (Parts of each job alone, about as many as the
+// CUs hold: prompts behind long conversations, 16/4 heads of 128, 74 us, not 61; drafts 37, not 32.) A job's beginning (its
+// rows, their results) counts as kBegin blocks: 6 of k_cache8_rows (4: 5% slower where a workgroup has some 20 blocks), 2 of
+// tiles (1 and 3: 3%). Every wavefront finds its place alike, a lane to a sequence, then to a group, 2.7 us in all. Else
+// workgroups are of pairs, groups (the longest first) and parts in turn.
 template <int R, int kBegin, bool kShared>
 struct Jobs {
-  // the lane's sequence, its groups and their units: blocks, and kBegin of each (a group without a block has one: its rows' results are written, too)
+  // the lane's sequence, its groups and their units: blocks, and kBegin of each (a group without a block has one: its rows'
+  // results are written, too)
   struct Held {
     Seq8 s;
     int n, units;
@@ -678,8 +685,8 @@ struct Jobs {
     if (parts.job) parts.job[((size_t)w.b * a.NKV + w.hk) * groups + w.group] = make_int2(w.slot, n);
   }
   __device__ __forceinline__ bool only(Job8 &w) {
-    // Each CU gets one workgroup of every `cus`: of the first the longest, of the second the shortest first, and so on, so that all
-    // have much the same to do (8 x 1,024 rows of 12 heads of 64 in turn 49 us, the longest first throughout).
+    // Each CU gets one workgroup of every `cus`: of the first the longest, of the second the shortest first, and so on, so
+    // that all have much the same to do (8 x 1,024 rows of 12 heads of 64: 46 us, and 49 with the longest first throughout).
     unsigned x = blockIdx.x;
     const unsigned cus = (unsigned)parts.cus, lap = x / cus;
     if (lap % 2 && (lap + 1) * cus <= gridDim.x) x = lap * cus + (cus - 1 - x % cus);
@@ -703,11 +710,11 @@ struct Jobs {
   }
 };
 
-// ---- up to 32 rows (query rows times heads of the group) ----
+// ---- up to 32 rows (query rows times heads of the group) at a time ----
 //
-// A row of q is held as whole numbers of 31 bits next to its largest element, and those as four digits of base 256; its products with the codes
-// are exact on the 8-bit matrix units, and so are the weights', 31 bits next to the block's largest, with the values' codes.
-
+// A row of q is held as whole numbers of 31 bits next to its largest element, and those as four digits of base 256; its
+// products with the codes are exact on the 8-bit matrix units, and so are the weights', 31 bits next to the block's
+// largest, with the values' codes. So no code is converted, and a score is rounded where its digits' sums are added up.
 // What all rows of a wavefront need of a call and a block.
 struct Block8 {
   const ugk_cache8 &a;
@@ -722,8 +729,9 @@ struct Block8 {
   }
 };
 
-// Four rows: their four digits are one operand of 16 rows, so that a block's scores take two instructions per 16 keys at 128 floats per
-// head, and a lane finds the four digits of its score in its own four registers. A lane has a score of row lane / 16 for each 16 keys.
+// Four rows: their four digits are one operand of 16 rows, so that a block's scores take two instructions per 16 keys at 128
+// floats per head, and a lane finds the four digits of its score in its own four registers. A lane has a score of row lane /
+// 16 for each 16 keys.
 template <int DT>
 struct Four {
   static constexpr int KS = (DT + 3) / 4, kStride = 20, kLds = 16 * kStride;  // kLds words of LDS per wavefront
@@ -837,8 +845,9 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// Sixteen rows: the same products transposed, with an operand per digit. A lane holds 16 scores of one row, lane % 16, and its weights are
-// the second product's operand as they stand, for a column of the values' codes has its keys in the order in which the lanes hold them.
+// Sixteen rows: the same products transposed, with an operand per digit. A lane holds 16 scores of one row, lane % 16, and
+// its weights are the second product's operand as they stand, for a column of the values' codes has its keys in the order in
+// which the lanes hold them.
 template <int DT>
 struct Sixteen {
   static constexpr int KS = (DT + 3) / 4, kLds = 4;  // (none)
@@ -962,8 +971,16 @@ struct Sixteen {
   }
 };
 
-// Up to R rows: a token's, drafts, large groups, an observation window (in `groups` of them). The wavefronts share the blocks, and a wavefront has all
-// rows, 4 or 16. Of 32 it has half, and two take the same blocks, the second from a cache.
+// Up to R rows: a token's, drafts, large groups, an observation window (in `groups` of them). The wavefronts share the blocks,
+// and a wavefront has all rows, 4 or 16. Of 32 it has half, and two take the same blocks, the second from a cache. Keys are
+// loaded into the registers that the scores have left, values into those that the output has, while the other half of the
+// block is computed.
+//
+// Four rows are bound by memory: 346 MB of 24 conversations in 62 us, 5.5 TB/s, with three wavefronts on a SIMD (two:
+// 70 us). Sixteen are bound by the digits' vector instructions, four of five of a block's, beside the loads: 86 MB of 16
+// conversations, 20 rows each, 32 us. (20 rows as 16 and 4 of the same wavefront: 38 us, for it has all blocks' time in a
+// row.) What is left of short calls is the way there: 16 x 12 heads of 64, up to 16 blocks each, 8.8 us, of which the
+// blocks take 1.2.
 template <int DT, int R>
 __device__ __forceinline__ void rows_job(float *out, float *lse, const float *q, const int8_t *k8, const float *ks, const int8_t *v8,
                                          const float *vs, const ugk_cache8 &a, const Parts8 &parts, const Job8 &job, int *word) {
@@ -1080,9 +1097,11 @@ __device__ __forceinline__ float2 joined(const Parts8 &parts, int first, int n, 
   return make_float2(m, l);
 }
 
-// Behind the attention, workgroups of two kinds. The first `joins` join the parts of a split key axis, half a wavefront per row and head, in the
-// parts' order, where a group of `rows` rows had more than one. The others add up the weights of 16 blocks of a sequence, 16
-// threads to each, which take every sixteenth row and head, in a fixed order: weight[b, j] += sum of l_j 2^(m_j - m) / l.
+// Behind the attention, workgroups of two kinds. The first `joins` join the parts of a split key axis, half a wavefront per
+// row and head, in the parts' order, where a group of `rows` rows had more than one. The others add up the weights of 16
+// blocks of a sequence, 16 threads to each, which take every sixteenth row and head, in a fixed order:
+// weight[b, j] += sum of l_j 2^(m_j - m) / l. Two launches in one: 4 to 6 us of rows that are a token's or drafts, a launch and
+// three dependent loads; 10 us of prompts (35 MB of parts, and workgroups of rows that are not there).
 __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse, float *weight, Parts8 parts, ugk_cache8 a, int rows,
                                                          int groups, unsigned joins) {
   constexpr int kAtOnce = 4;  // parts whose loads are on their way together
@@ -1175,12 +1194,17 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
   if (lse && d == 0) lse[g * a.NH + h] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn28;
 }
 
-// Many rows: a prompt's. 128 rows of a sequence and key/value head per workgroup, 32 to a wavefront, over blocks whose codes go
-// through LDS as halves (which hold them exactly).
+// Many rows: a prompt's. 128 rows of a sequence and key/value head per workgroup, 32 to a wavefront, over blocks whose codes
+// go through LDS as halves (which hold them exactly).
 //
-// The scores are computed transposed, so that a lane holds one row: its maximum and sum stay in the lane, and its weights are the second
-// product's operand as they stand. q and the weights are two halves each (ugk_split.h), so a product
-// is two of v_mfma_f32_32x32x16_f16, where fp32 keys and values need three.
+// The scores are computed transposed, so that a lane holds one row: its maximum and sum stay in the lane, and its weights are
+// the second product's operand as they stand. q and the weights are two halves each (ugk_split.h), so a product is two of
+// v_mfma_f32_32x32x16_f16, where fp32 keys and values need three.
+//
+// Bound by matrix and vector instructions, which add up on a SIMD: 64 of the first and some 540 of the others per block and
+// wavefront at heads of 128. 8 x 1,024 rows of 12 heads of 64 42 us, 4 x 2,048 of 16/4 of 128 171 (of fp32 keys and values 67
+// and 192). Products of one sum never follow one another, and their operands are two steps ahead (62 us, not 64, of prompts
+// behind long conversations); wavefront priorities changed nothing.
 constexpr int kTileWaves8 = 4, kTileRows8 = 32 * kTileWaves8, kTileThreads8 = kTileWaves8 * kWave;
 
 // Four codes (bytes b0..b3 of w, with their signs turned over: c + 128) as halves.
@@ -1417,10 +1441,11 @@ __device__ __forceinline__ int before(int x, int *lds, int *all) {
   return sum + y - x;
 }
 
-// One sequence per workgroup, E entries of its table per thread, side by side in registers: the d lightest blocks by a search over the
-// weights' bits, eleven at a time (counts in LDS: eight at a time took a turn more, and the exponents of many weights met in the same
-// counter), ties by their index; then each entry's place from counts of those before it. Reading and writing 16 bytes
-// per entry is nothing; what counts are the chain of barriers (three counts and two sums).
+// One sequence per workgroup, E entries of its table per thread, side by side in registers: the d lightest blocks by a search
+// over the weights' bits, eleven at a time (counts in LDS: eight at a time took a turn more, and the exponents of many
+// weights met in the same counter), ties by their index; then each entry's place from counts of those before it. Reading and
+// writing 16 bytes per entry is nothing; what counts are the chain of barriers (three counts and two sums): 5.4 us of up to 16
+// blocks of 16 sequences, 9.7 of up to 4,096 of 64.
 template <int E>
 __global__ __launch_bounds__(kEvictThreads) void k_cache8_evict(int *table_out, int *len_out, float *weight_out, int *dropped,
                                                                const int *table, const int *k_len, const float *weight, int ld,
@@ -1514,30 +1539,40 @@ int cu_count8() {
 }
 
 // How an attention call is cut: k_cache8_rows (4, 16, 32 rows) in so many groups, or k_cache8_tile (128) in so many
-// tiles; `wgs` workgroups that share all blocks, or up to `splits` parts of `least` blocks or more of each; the rows of a slot of
-// parts, the slots, and where a job's are.
+// tiles; `wgs` workgroups that share all blocks, or up to `splits` parts of `least` blocks or more of each; the rows of a
+// slot of parts, the slots, and where a job's are.
+//
+// By rows (query rows times heads of the group; times in us, 24 sequences of up to 8,192 keys, heads of 128, by the
+// smaller and the next larger form): 4 rows 36 and 39; 16 rows 27 and 33; 32 rows 37 and 49; 64 rows in two groups of 32
+// or a tile 63 and 71. Where tiles fill the CUs, two groups are the slower (64 x 12 heads of 64, 64 rows each: 36
+// and 31). Weights are added up by groups of 32 whatever the rows.
 struct Plan8 {
   int rows, groups, splits, least, wgs, grid, held, step;
   size_t slots;
 };
-constexpr int kFewRows8 = 32;
 
 Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   Plan8 p{};
+  const int cus = cu_count8();
   const long long pairs = (long long)a.nseq * a.NKV, G = a.NH / a.NKV, rows = a.max_q * G, blocks = (a.max_k + kKeys - 1) / kKeys;
-  p.rows = rows <= 4 ? 4 : rows <= 16 ? 16 : rows <= kFewRows8 || weigh ? 32 : kTileRows8;
+  const bool groups = weigh || rows <= 32 || (rows <= 64 && pairs <= cus);
+  p.rows = rows <= 4 ? 4 : rows <= 16 ? 16 : groups ? 32 : kTileRows8;
   p.groups = (int)((rows + p.rows - 1) / p.rows);
   p.held = (int)min((long long)p.rows, rows);
   p.step = 1;
   p.splits = 1;
-  const bool narrow = a.HS <= 64;
-  const int cus = cu_count8(), at_once = cus * (p.rows == 4 ? (narrow ? 4 : 3) : narrow ? 3 : 2);
+  // Workgroups that the CUs hold at once. Fewer leave a SIMD's wavefront alone with its loads' and products' latency (heads
+  // of 128, one to a CU: tiles 81 us, not 64, 32 rows 46, not 36); with more, some CUs have a second round (32 rows of heads
+  // of 64, four: 29, not 24).
+  const int at_once = cus * (a.HS > 64 ? (p.rows == 4 ? 3 : 2) : (p.rows == 4 ? 4 : 3));
   // at most so many jobs, and the shares of so many blocks, were all sequences full
   const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / at_once;
   // what a workspace of the same rows and heads has for the fp32 attention
   const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / sizeof(float) - 4;
   const long long told = 2 * pairs * p.groups, fit = ((long long)most - told) / ((part_floats(a.HS) + 2) * (long long)p.held);
-  // few blocks are not worth a look at all sequences, nor are many groups, which fill the CUs
+  // Few blocks are not worth a look at all sequences and a second launch (16 x 12 heads of 64, one row, up to 1,024 keys 8.4
+  // us, in shares 9.5 and 3.6; up to 4,096 keys 18.5, and 15 and 4; 24 x 8 heads of 128, up to 8,192 keys 50, and 36 and
+  // 4.7), nor are many groups, which fill the CUs.
   if (blocks > 32 && jobs <= 4LL * at_once && blocks * pairs * p.groups <= 1 << 30 && (rows + p.rows) * G >> 32 == 0) {
     // a job has one part more than workgroups' borders, and a workgroup two at most that are not whole
     p.step = jobs <= at_once && fit >= 2 * jobs ? 1 : 2;
@@ -1548,7 +1583,8 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
     p.slots = p.step == 1 ? p.wgs + jobs : 2LL * p.wgs;
     p.grid = max(p.wgs, (int)jobs);
   } else {
-    // with weights to add up, the launch that joins parts is there anyway
+    // Whole where that fills two thirds of the CUs (192 workgroups of up to 16 blocks 8.4 us; in parts 8.1, and 4 to join
+    // them); with weights to add up, the launch that joins parts is there anyway.
     const long long least = max(3 * jobs >= 2LL * cus && !weigh ? blocks : max(share, 4LL), 1LL);
     p.step = 1;
     p.splits = (int)max(min((blocks + least - 1) / least, fit / (pairs * p.groups)), 1LL);
