@@ -505,9 +505,9 @@ int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks,
 /* ugk_attention_forward of q against the cache: out, and lse (rows_q, NH) if not
  * NULL. A row without a key that it sees has out 0 and lse -infinity. A row of q (of one
  * head) enters as whole numbers of 31 bits next to its largest element and the
- * weights as such next to the largest of their block; or, with more than 32 query
- * rows times heads per key/value head and no `weight`, both as two half-precision
- * numbers, q to 2^-23 of the element and 2^-38 of the largest, weights to 2^-23
+ * weights as such next to the largest of their block; or, with more than 64 query
+ * rows times heads per key/value head (more than 32, where sequences times key/value heads
+ * outnumber the CUs) and no `weight`, both as two half-precision numbers, q to 2^-23 of the element and 2^-38 of the largest, weights to 2^-23
  * of the weight and 2^-38 of the largest contribution (weight times the values'
  * scale) that the row sees. Products with the codes are exact, statistics and sums
  * in single precision. A score of about 2^127 or more, or an infinity or NaN in its row

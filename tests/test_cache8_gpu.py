@@ -209,7 +209,7 @@ def attend(gpu, c, NH, q, starts, lens, keys, rows, causal=True, weight=None, ls
 
 def check(gpu, c, NH, q, starts, lens, keys, rows, causal=True, weigh=False, pad=0, scale=None, **kw):
     weight = torch.full(c.table.shape, 0.5, device=DEV) if weigh else None
-    few = weigh or max(lens) * (NH // c.NKV) <= 32
+    few = weigh or max(lens) * (NH // c.NKV) <= 64  # the rows whose weights may be whole numbers
     out, L = attend(gpu, c, NH, q, starts, lens, keys, rows, causal, weight, pad=pad, scale=scale, **kw)
     gpu.synchronize()
     s = c.HS ** -0.5 if scale is None else scale
