@@ -475,7 +475,8 @@ typedef struct {
    * keys 64 j to 64 j + 63. NULL: rows [b max_q, (b + 1) max_q), and rows_q must be nseq *
    * max_q; max_k keys; block b ld_table + j, and nblocks must be at least nseq * ld_table.
    * Rows and lengths beyond the buffers and max are clamped, blocks beyond nblocks are left out, and the next
-   * ugk_synchronize reports either. */
+   * ugk_synchronize reports either. A row belongs to one sequence: what a call with
+   * rows in several leaves in out or the cache is undefined, and it may be reported. */
   const int *q_start, *q_end, *k_len, *table;
   int ld_table;       /* 0: max_k / 64 rounded up, which is also the least */
   /* floats from a row to the next of q, of store's and load's k and v, of out; 0:

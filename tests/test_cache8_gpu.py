@@ -121,6 +121,55 @@ def test_store_and_load(gpu, steps, NKV, HS):
             assert torch.equal(c.v8[i][..., behind], before[2][i][..., behind])
 
 
+@pytest.mark.parametrize("nseq,lq,NKV,HS", [(40, 640, 8, 16), (100, 300, 8, 64), (70, 1000, 9, 33)])
+def test_store_of_one_sequence_of_many_rows_among_many_of_one(gpu, nseq, lq, NKV, HS):
+    """max_q is one sequence's: a call for all leaves what calls for each do."""
+    cap = lq + 100
+    lens, keys = [1 + b % 2 for b in range(nseq)], [2 + 11 * b % cap for b in range(nseq)]
+    lens[nseq - 3], keys[nseq - 3], lens[3], lens[5], keys[5] = lq, cap, 0, 0, 0
+    starts, rows = place_rows(lens)
+    g = gen(nseq)
+    k, v = rand(g, rows, NKV, HS), rand(g, rows, NKV, HS)
+    c, d = (Cache(gpu, nseq, cap, NKV, HS, seed=5) for _ in "cd")
+    gpu.cache8_store(*c.parts(), k, v, c.call(NKV, starts, lens, keys, rows))
+    for b in range(nseq):
+        a = d.gpu.Cache8(nseq=1, NH=NKV, NKV=NKV, HS=HS, rows_q=rows, max_q=lq, max_k=cap, nblocks=d.nblocks, q_start=ints([starts[b]]),
+                         q_end=ints([starts[b] + lens[b]]), k_len=ints([keys[b]]), table=d.table[b:b + 1])
+        gpu.cache8_store(*d.parts(), k, v, a)
+    assert all(torch.equal(x, y) for x, y in zip(c.parts(), d.parts()))
+    k2, v2 = torch.full_like(k, 9.0), torch.full_like(v, 9.0)
+    gpu.cache8_load(k2, v2, *c.parts(), c.call(NKV, starts, lens, keys, rows))
+    gpu.synchronize()
+    for b in range(nseq):
+        at = slice(starts[b], starts[b] + lens[b])
+        for got, name in ((k2, "k"), (v2, "v")):
+            assert torch.equal(got[at].double(), c.values(b, keys[b], name)[keys[b] - lens[b]:])
+    used = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    for b in range(nseq):
+        used[starts[b]:starts[b] + lens[b]] = True
+    assert (k2[~used] == 9.0).all() and (v2[~used] == 9.0).all()
+
+
+def test_store_reports_rows_in_several_sequences(gpu):
+    """As many blocks as a buffer of so many rows cannot touch: none is written outside its place."""
+    nseq, lq, NKV, HS = 64, 640, 8, 16
+    c = Cache(gpu, nseq, lq, NKV, HS)
+    k = rand(gen(1), lq, NKV, HS)
+    gpu.cache8_store(*c.parts(), k, k.clone(), c.call(NKV, [0] * nseq, [lq] * nseq, [lq] * nseq))
+    with pytest.raises(gpu.UgkError, match="cache8_store"):
+        gpu.synchronize()
+    bad = Cache(gpu, nseq, lq, NKV, HS)
+    keys = [lq] * nseq
+    keys[50] = lq + 1
+    lens = [1] * nseq
+    lens[2] = lq
+    starts, rows = place_rows(lens)
+    k = rand(gen(1), rows, NKV, HS)
+    gpu.cache8_store(*bad.parts(), k, k.clone(), bad.call(NKV, starts, lens, keys, rows))
+    with pytest.raises(gpu.UgkError, match="cache8_store"):
+        gpu.synchronize()
+
+
 def one_block(gpu, values, NKV=1):
     """values: a list of rows of numbers, stored one call each; the codes and the scale of K and V."""
     HS = len(values[0])
@@ -520,6 +569,34 @@ def test_groups_of_rows_that_end_in_a_few(gpu, cap, lq, NH, NKV, HS):
     for causal in (True, False):
         check(gpu, c, NH, q, starts, lens, keys, rows, causal=causal)
         check(gpu, c, NH, q, starts, lens, keys, rows, causal=causal, weigh=True)
+
+
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("lq,NH,NKV,HS,cap", [(640, 1, 1, 64, 500), (200, 3, 1, 33, 2300), (36, 14, 2, 16, 300), (9, 4, 1, 128, 2500), (5000, 2, 1, 16, 5100)])
+def test_one_sequence_of_many_rows_among_many_of_one(gpu, lq, NH, NKV, HS, cap, weigh):
+    """max_q is one sequence's: most groups of rows are not there."""
+    if weigh and lq * NH // NKV > 256:
+        return
+    nseq = 40
+    lens, keys = [1] * nseq, [1 + 7 * b % cap for b in range(nseq)]
+    lens[17], keys[17], lens[3], keys[3], lens[39] = lq, cap, 0, 0, 0
+    c, g = filled(gpu, nseq, cap, NKV, HS, keys)
+    starts, rows = place_rows(lens)
+    q = rand(g, rows, NH, HS)
+    check(gpu, c, NH, q, starts, lens, keys, rows, weigh=weigh)
+
+
+@pytest.mark.parametrize("lq,weigh", [(320, False), (48, False), (48, True)])
+def test_rows_in_several_sequences_are_reported(gpu, lq, weigh):
+    """64 sequences of the same rows, whose groups are more than a buffer of so many rows has: nothing is computed."""
+    nseq, cap, HS = 64, 2200, 16
+    c, g = filled(gpu, nseq, cap, 1, HS, [cap] * nseq)
+    q, out = rand(g, lq, 1, HS), torch.full((lq, 1, HS), 7.0, device=DEV)
+    weight = torch.zeros(nseq, c.table.shape[1], device=DEV) if weigh else None
+    gpu.cache8_attention(out, None, q, *c.parts(), c.call(1, [0] * nseq, [lq] * nseq, [cap] * nseq), weight=weight)
+    with pytest.raises(gpu.UgkError, match="cache8_attention"):
+        gpu.synchronize()
+    assert (out == 7.0).all() and (not weigh or not weight.any())
 
 
 def test_many_groups_of_rows_in_a_sequence(gpu):

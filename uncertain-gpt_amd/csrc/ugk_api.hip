@@ -893,6 +893,9 @@ int ugk_cache8_attention(float *out, float *lse, const float *q, const void *k8,
   if (int e = check_cache8(fn, &a, &none)) return e;
   if (weight && (long long)a.max_q * (a.NH / a.NKV) > kWeighRows)
     return set_error(UGK_EINVAL, "%s: weights are added up for up to %d rows and heads per key/value head", fn, kWeighRows);
+  // a workgroup of 256 for 32 rows and heads then
+  if (weight && (long long)a.nseq * a.NKV >= ((long long)1 << 24) / (((long long)a.max_q * (a.NH / a.NKV) + 31) / 32 + 1))
+    return bad(fn, "nseq * heads * rows exceeds the grid");
   if (none) return ok();
   if (any_null({out, q})) return bad(fn, "NULL pointer");
   if (a.max_k > 0 && any_null({k8, ks, v8, vs})) return bad(fn, "NULL pointer");

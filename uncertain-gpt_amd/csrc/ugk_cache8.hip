@@ -85,19 +85,52 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float ratio) {
                code_of((float)code_at(w, 3), ratio));
 }
 
+__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, kWave - 1); }
+
 // What a workgroup of the store and the load has: block j of a sequence, of which rows [r0, r1) are
 // the call's, those before r0 in the cache already.
 struct Touched {
   int b, h, j, q, r0, r1;  // q: the buffer's row of r0
 };
-__device__ __forceinline__ bool touched(const ugk_cache8 &a, int per, int *word, int code, Touched *t) {
-  const unsigned x = blockIdx.x;
-  t->h = x % a.NKV;
-  const int nth = x / a.NKV % per;
-  t->b = x / a.NKV / per;
-  const bool tell = t->h == 0 && nth == 0 && blockIdx.y == 0;
-  const Seq8 s = sequence8(a, t->b, tell, word, code);
-  if (s.Lq > s.Lk && tell && threadIdx.x == 0) *word = code;  // rows before the first key
+// Workgroups are of heads, and of `per` blocks of each sequence; or (per 0) of the `all` blocks that there are, a lane to a
+// sequence finds which.
+__device__ __forceinline__ bool touched(const ugk_cache8 &a, int per, int all, int *word, int code, Touched *t) {
+  const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+  int nth = blockIdx.x / a.NKV;
+  Seq8 s;
+  t->h = blockIdx.x % a.NKV;
+  if (per) {
+    t->b = nth / per;
+    nth %= per;
+    const bool tell = t->h == 0 && nth == 0 && blockIdx.y == 0;
+    s = sequence8(a, t->b, tell, word, code);
+    if (s.Lq > s.Lk && tell && threadIdx.x == 0) *word = code;  // rows before the first key
+  } else {
+    const int lane = threadIdx.x & (kWave - 1);
+    t->b = -1;
+    for (int b0 = 0; b0 < a.nseq && (t->b < 0 || first); b0 += kWave) {
+      Seq8 own{0, 0, 0};
+      int n = 0;
+      if (b0 + lane < a.nseq) {
+        own = sequence8(a, b0 + lane, first, word, code);
+        if (own.Lq > own.Lk && first) *word = code;
+        if (own.Lq > 0) n = (own.Lk + kKeys - 1) / kKeys - max(own.Lk - own.Lq, 0) / kKeys;
+      }
+      const int to = wave_scan(n);
+      const uint64_t over = __ballot(to > nth);
+      if (over && t->b < 0) {
+        const int l = __builtin_ctzll(over);
+        t->b = b0 + l;
+        s = Seq8{__builtin_amdgcn_readlane(own.q0, l), __builtin_amdgcn_readlane(own.Lq, l), __builtin_amdgcn_readlane(own.Lk, l)};
+        nth -= __builtin_amdgcn_readlane(to - n, l);
+      } else if (t->b < 0) {
+        nth -= last_lane(to);
+      }
+      all -= last_lane(to);
+    }
+    if (first && all < 0 && threadIdx.x == 0) *word = code;  // rows in several sequences: there is no workgroup for some
+    if (t->b < 0) return false;
+  }
   const int begin = max(s.Lk - s.Lq, 0);
   t->j = begin / kKeys + nth;
   if (s.Lq == 0 || t->j * kKeys >= s.Lk) return false;
@@ -115,12 +148,12 @@ __device__ __forceinline__ bool touched(const ugk_cache8 &a, int per, int *word,
 // each other: 4.4 us of 4 sequences, 6.4 of 24 with 8 heads of 128.
 template <int CH>
 __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, int8_t *v8, float *vs, const float *k, const float *v,
-                                                         ugk_cache8 a, int per, int *word) {
+                                                         ugk_cache8 a, int per, int all, int *word) {
   constexpr int HP = 16 * CH, G = HP / 4, kPer = (16 * G + kBlock - 1) / kBlock;
   __shared__ uint32_t tile[HP * 17];  // the values' words, 17 to a column of 16: banks that differ
   __shared__ uint32_t top[kBlock / kWave];
   Touched t;
-  if (!touched(a, per, word, UGK_IDS_CACHE8_STORE, &t)) return;
+  if (!touched(a, per, all, word, UGK_IDS_CACHE8_STORE, &t)) return;
   const bool values = blockIdx.y;
   const long long ld = values ? a.ldv : a.ldk;
   const float *src = (values ? v : k) + (long long)(t.q - t.r0) * ld + t.h * a.HS;
@@ -248,11 +281,11 @@ __global__ __launch_bounds__(kBlock) void k_cache8_store(int8_t *k8, float *ks, 
 // The store's rows, read back.
 template <int CH>
 __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, const int8_t *k8, const float *ks, const int8_t *v8,
-                                                        const float *vs, ugk_cache8 a, int per, int *word) {
+                                                        const float *vs, ugk_cache8 a, int per, int all, int *word) {
   constexpr int HP = 16 * CH, G = HP / 4;
   __shared__ uint32_t tile[HP * 17];
   Touched t;
-  if (!touched(a, per, word, UGK_IDS_CACHE8_LOAD, &t)) return;
+  if (!touched(a, per, all, word, UGK_IDS_CACHE8_LOAD, &t)) return;
   const bool values = blockIdx.y;
   const long long ld = values ? a.ldv : a.ldk;
   float *to = (values ? v : k) + (long long)(t.q - t.r0) * ld + t.h * a.HS;
@@ -302,9 +335,14 @@ __global__ __launch_bounds__(kBlock) void k_cache8_load(float *k, float *v, cons
 struct Parts8 {
   float *o;
   float2 *ml, *block, *stat;
-  int2 *job;           // of a sequence, key/value head and group: the slot of its first part, and its parts
+  // What the launch behind has to know: the jobs that there are (one of every sequence, head and group where workgroups have
+  // one), four words; eight words for each, in their order: the sequence's first row and its rows, the head, the group, the
+  // slot of the first part, the parts (0: no such job); and, for the blocks' weights, of every sequence, head and group the
+  // two last again where workgroups have many.
+  int *told;
   int rows, step;      // of a slot; 1 where a job's parts lie in slots side by side, 2 where those behind the first are at 2 x workgroup
   int splits, least;   // most parts of a job where workgroups are of one, blocks per part at least
+  int ld, most;        // blocks of max_k keys; jobs where they are counted
   int wgs, cus;        // workgroups that share all blocks (0: a workgroup has one job's part), CUs
   unsigned inverse;    // ceil(2^32 / heads of a group), 0 for one head
 };
@@ -529,8 +567,6 @@ struct Walk {
 };
 __device__ __forceinline__ size_t block_head(int id, int NKV, int hk) { return (size_t)max(id, 0) * NKV + hk; }
 
-__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, kWave - 1); }
-
 // What a workgroup has at a time: of group `group` of R rows of a sequence and key/value head blocks [first, stop).
 struct Job8 {
   Seq8 s;
@@ -577,16 +613,34 @@ struct Jobs {
   }
   __device__ __forceinline__ int units(int nb) const { return whole ? 1 : kBegin + max(nb, 1); }
   __device__ __forceinline__ Held held(int b, bool tell, int *longest) const {
+    constexpr int kOwn = 64;  // groups that a lane adds up by itself; of sequences of more all lanes do
     Held h{{0, 0, 0}, 0, 0};
-    if (b >= a.nseq) return h;
-    h.s = sequence8(a, b, tell, word, UGK_IDS_CACHE8_ATTENTION);
-    h.n = (h.s.Lq * G + R - 1) / R;
-    if (whole) h.units = h.n;
-    for (int t = 0; !whole && t < h.n; t++) {
+    if (b < a.nseq) {
+      h.s = sequence8(a, b, tell, word, UGK_IDS_CACHE8_ATTENTION);
+      h.n = (h.s.Lq * G + R - 1) / R;
+    }
+    if (whole) {
+      h.units = h.n;
+      return h;
+    }
+    for (int t = 0; t < h.n && h.n <= kOwn; t++) {
       const int nb = blocks_of(h.s, t);
       h.units += kBegin + max(nb, 1);
       *longest = max(*longest, nb);
     }
+    for (uint64_t many = __ballot(h.n > kOwn); many; many &= many - 1) {
+      const int l = __builtin_ctzll(many), n = __builtin_amdgcn_readlane(h.n, l);
+      const Seq8 s{__builtin_amdgcn_readlane(h.s.q0, l), __builtin_amdgcn_readlane(h.s.Lq, l), __builtin_amdgcn_readlane(h.s.Lk, l)};
+      int sum = 0;
+      for (int t = lane; t < n; t += kWave) {
+        const int nb = blocks_of(s, t);
+        sum += kBegin + max(nb, 1);
+        *longest = max(*longest, nb);
+      }
+      sum = last_lane(wave_scan(sum));
+      if (lane == l) h.units = sum;
+    }
+    return h;
     return h;
   }
 
@@ -607,7 +661,12 @@ struct Jobs {
     // no group has much more than a CU's share: the parts' way through memory would cost more than they save
     whole = (long long)2 * longest * parts.cus <= 3LL * (all - kBegin * jobs);
     share = whole ? 1 : max(parts.least, (all + parts.wgs - 1) / parts.wgs);
-    all = whole ? jobs : all;
+    const bool over = jobs > parts.most;  // rows in more than one sequence: there is no place for so many
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      *parts.told = over ? 0 : jobs;
+      if (over) *word = UGK_IDS_CACHE8_ATTENTION;
+    }
+    all = __builtin_amdgcn_readfirstlane(over ? 0 : whole ? jobs : all);  // (or the job, and 25 more registers, are per lane)
     end = (int)min((long long)(blockIdx.x + 1) * share, (long long)all);
     at = (int)min((long long)blockIdx.x * share, (long long)all);
     if (at >= end) return false;
@@ -676,13 +735,18 @@ struct Jobs {
     if (stop <= w.first) return false;
     w.whole = w.first == 0 && stop == u - begin;
     w.slot = blockIdx.x + (parts.step == 1 ? j : (int)blockIdx.x + (at != (int)blockIdx.x * share));
-    if (w.first == 0 && threadIdx.x == 0) tell(w, whole ? 1 : (at - off + u - 1) / share - (int)blockIdx.x + 1);
+    if (w.first == 0) tell(w, whole ? 1 : (at - off + u - 1) / share - (int)blockIdx.x + 1);
     w.stop = whole ? nb : min(stop, nb);
     at += u - off;
     return true;
   }
   __device__ __forceinline__ void tell(const Job8 &w, int n) const {
-    if (parts.job) parts.job[((size_t)w.b * a.NKV + w.hk) * groups + w.group] = make_int2(w.slot, n);
+    if (!parts.told || threadIdx.x) return;
+    const size_t at = ((size_t)w.b * a.NKV + w.hk) * groups + w.group;
+    int4 *to = reinterpret_cast<int4 *>(parts.told + 4) + 2 * (kShared ? (size_t)j : at);
+    to[0] = make_int4(w.s.q0, w.rows, w.hk, w.group);
+    to[1] = make_int4(w.slot, n, 0, 0);
+    if (kShared && parts.block) reinterpret_cast<int2 *>(parts.told + 4 + 8 * (size_t)parts.most)[at] = make_int2(w.slot, n);
   }
   __device__ __forceinline__ bool only(Job8 &w) {
     // Each CU gets one workgroup of every `cus`: of the first the longest, of the second the shortest first, and so on, so
@@ -696,8 +760,12 @@ struct Jobs {
     w.group = groups - 1 - round % groups;
     w.s = sequence8(a, w.b, w.hk == 0 && round == 0, word, UGK_IDS_CACHE8_ATTENTION);
     w.rows = w.s.Lq * G;
-    if (w.group * R >= w.rows) return false;
-    const int part = round / groups, nb = blocks_at(w.s, a, (min((w.group + 1) * R, w.rows) - 1) / G);
+    const int part = round / groups;
+    if (w.group * R >= w.rows) {
+      if (part == 0) tell(w, 0);
+      return false;
+    }
+    const int nb = blocks_at(w.s, a, (min((w.group + 1) * R, w.rows) - 1) / G);
     const int n = parts.o ? parts_for(nb, parts.least) : 1;
     if (part >= n) return false;
     const int each = nb / n, longer = nb - each * n;  // the first ones are one longer
@@ -705,7 +773,7 @@ struct Jobs {
     w.first = part * each + min(part, longer);
     w.stop = w.first + each + (part < longer);
     w.slot = (int)((pair * groups + w.group) * parts.splits) + part;
-    if (part == 0 && threadIdx.x == 0) tell(w, n);
+    if (part == 0) tell(w, n);
     return true;
   }
 };
@@ -725,7 +793,7 @@ struct Block8 {
   float f, kscale, vexp;  // f: |scale| log2(e) (its sign goes with q)
   // where the block's m and l of a row go
   __device__ __forceinline__ float2 *stat(int row) const {
-    return parts.block + (((size_t)job.b * a.NKV + job.hk) * a.max_q * (a.NH / a.NKV) + row) * a.ld_table + j;
+    return parts.block + (((size_t)job.b * a.NKV + job.hk) * a.max_q * (a.NH / a.NKV) + row) * parts.ld + j;
   }
 };
 
@@ -1097,15 +1165,16 @@ __device__ __forceinline__ float2 joined(const Parts8 &parts, int first, int n, 
   return make_float2(m, l);
 }
 
+constexpr int kJoinRows8 = 2 * kBlock / kWave;  // rows that a workgroup joins
+
 // Behind the attention, workgroups of two kinds. The first `joins` join the parts of a split key axis, half a wavefront per
 // row and head, in the parts' order, where a group of `rows` rows had more than one. The others add up the weights of 16
 // blocks of a sequence, 16 threads to each, which take every sixteenth row and head, in a fixed order:
 // weight[b, j] += sum of l_j 2^(m_j - m) / l. Two launches in one: 4 to 6 us of rows that are a token's or drafts, a launch and
-// three dependent loads; 10 us of prompts (35 MB of parts, and workgroups of rows that are not there).
+// three dependent loads; 9 us of prompts behind long conversations (35 MB of parts).
 __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse, float *weight, Parts8 parts, ugk_cache8 a, int rows,
-                                                         int groups, unsigned joins) {
+                                                         int groups, int per_job, unsigned joins) {
   constexpr int kAtOnce = 4;  // parts whose loads are on their way together
-  constexpr int kJoinRows = 2 * kBlock / kWave;
   const int G = a.NH / a.NKV;
   if (blockIdx.x >= joins) {
     __shared__ float part[16][17];
@@ -1113,17 +1182,22 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
     __shared__ size_t from[kBlock];
     __shared__ int end[kBlock];
     const unsigned x = blockIdx.x - joins;
-    const int of = (a.ld_table + 15) / 16, b = x / of, j = x % of * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
+    const int of = (parts.ld + 15) / 16, b = x / of, j = x % of * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
     const Seq8 s = sequence8(a, b, false, nullptr, 0);
     const int nb = (s.Lk + kKeys - 1) / kKeys, n = s.Lq * G;
-    if (x % of * 16 >= nb) return;
+    if (x % of * 16 >= nb || (parts.wgs && *parts.told == 0)) return;
     float sum = 0.0f;
     for (int y0 = 0; y0 < n * a.NKV; y0 += kBlock) {  // a row and head per thread, then a block per thread
       const int mine = y0 + (int)threadIdx.x;
       if (mine < n * a.NKV) {
         const int hk = mine / n, rr = mine % n;
-        const int2 job = parts.job ? parts.job[((size_t)b * a.NKV + hk) * groups + rr / rows] : make_int2(0, 1);
-        from[threadIdx.x] = (((size_t)b * a.NKV + hk) * a.max_q * G + rr) * a.ld_table;
+        int2 job = make_int2(0, 1);
+        if (parts.told) {
+          const size_t at = ((size_t)b * a.NKV + hk) * groups + rr / rows;
+          const int *t = parts.told + 4 + (parts.wgs ? 8 * (size_t)parts.most + 2 * at : 8 * at + 4);
+          job = make_int2(t[0], t[1]);
+        }
+        from[threadIdx.x] = (((size_t)b * a.NKV + hk) * a.max_q * G + rr) * parts.ld;
         end[threadIdx.x] = s.seen(rr / G, a.causal);
         whole[threadIdx.x] =
             job.y > 1 ? joined(parts, job.x, job.y, rr % rows) : parts.stat[((size_t)s.q0 + rr / G) * a.NH + hk * G + rr % G];
@@ -1155,13 +1229,15 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
     weight[(size_t)b * a.ld_table + j] += t;
     return;
   }
-  const int per_seq = (a.max_q * G + kJoinRows - 1) / kJoinRows, pair = blockIdx.x / per_seq, b = pair / a.NKV, hk = pair % a.NKV;
-  const int rr = blockIdx.x % per_seq * kJoinRows + (threadIdx.x >> 5), r = rr % rows, d = 4 * (threadIdx.x & 31);
-  const int2 job = parts.job[(size_t)pair * groups + min(rr / rows, groups - 1)];
-  const Seq8 s = sequence8(a, b, false, nullptr, 0);
-  if (rr >= s.Lq * G || job.y == 1) return;  // no row, or one workgroup had it whole
-  const int n = job.y, floats = part_floats(a.HS), h = hk * G + rr % G;
-  const size_t g = (size_t)s.q0 + rr / G;
+  const unsigned x = blockIdx.x / per_job;
+  const int r = blockIdx.x % per_job * kJoinRows8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+  const int4 *told = reinterpret_cast<const int4 *>(parts.told + 4) + 2 * (size_t)x;
+  const int4 from = told[0], job = told[1];
+  if (parts.wgs && x >= (unsigned)*parts.told) return;
+  const int n = job.y, rr = from.w * rows + r;
+  if (n < 2 || r >= rows || rr >= from.y) return;  // one workgroup had it whole; no row
+  const int floats = part_floats(a.HS), h = from.z * G + rr % G;
+  const size_t g = (size_t)from.x + rr / G;
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int t = 0; t < n; t += kAtOnce) {
@@ -1202,9 +1278,9 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
 // v_mfma_f32_32x32x16_f16, where fp32 keys and values need three.
 //
 // Bound by matrix and vector instructions, which add up on a SIMD: 64 of the first and some 540 of the others per block and
-// wavefront at heads of 128. 8 x 1,024 rows of 12 heads of 64 42 us, 4 x 2,048 of them 72, of 16/4 heads of 128 160 to 178 (of
-// fp32 keys and values 67, 107 and 191). Products of one sum never follow one another, and their operands are two steps ahead (62 us, not 64, of prompts
-// behind long conversations); wavefront priorities changed nothing.
+// wavefront at heads of 128. 8 x 1,024 rows of 12 heads of 64 42 us, 4 x 2,048 of them 72, of 16/4 heads of 128 160 to 178
+// (of fp32 keys and values 67, 107 and 191). Products of one sum never follow one another, and their operands are two steps
+// ahead (62 us, not 64, of prompts behind long conversations); wavefront priorities changed nothing.
 constexpr int kTileWaves8 = 4, kTileRows8 = 32 * kTileWaves8, kTileThreads8 = kTileWaves8 * kWave;
 
 // Four codes (bytes b0..b3 of w, with their signs turned over: c + 128) as halves.
@@ -1540,15 +1616,16 @@ int cu_count8() {
 
 // How an attention call is cut: k_cache8_rows (4, 16, 32 rows) in so many groups, or k_cache8_tile (128) in so many
 // tiles; `wgs` workgroups that share all blocks, or up to `splits` parts of `least` blocks or more of each; the rows of a
-// slot of parts, the slots, and where a job's are.
+// slot of parts, the slots and jobs, and where a job's are.
 //
 // By rows (query rows times heads of the group; times in us, 24 sequences of up to 8,192 keys, heads of 128, by the
 // smaller and the next larger form): 4 rows 36 and 39; 16 rows 27 and 33; 32 rows 37 and 49; 64 rows in two groups of 32
 // or a tile 63 and 71. Where tiles fill the CUs, two groups are the slower (64 x 12 heads of 64, 64 rows each: 36
 // and 31). Weights are added up by groups of 32 whatever the rows.
+constexpr int kJobInts = 8;
 struct Plan8 {
-  int rows, groups, splits, least, wgs, grid, held, step;
-  size_t slots;
+  int rows, groups, splits, least, wgs, grid, held, per_job, step;
+  size_t slots, jobs;
 };
 
 Plan8 plan8(const ugk_cache8 &a, bool weigh) {
@@ -1559,6 +1636,7 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   p.rows = rows <= 4 ? 4 : rows <= 16 ? 16 : groups ? 32 : kTileRows8;
   p.groups = (int)((rows + p.rows - 1) / p.rows);
   p.held = (int)min((long long)p.rows, rows);
+  p.per_job = (p.held + kJoinRows8 - 1) / kJoinRows8;
   p.step = 1;
   p.splits = 1;
   // Workgroups that the CUs hold at once. Fewer leave a SIMD's wavefront alone with its loads' and products' latency (heads
@@ -1569,40 +1647,53 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / at_once;
   // what a workspace of the same rows and heads has for the fp32 attention
   const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / sizeof(float) - 4;
-  const long long told = 2 * pairs * p.groups, fit = ((long long)most - told) / ((part_floats(a.HS) + 2) * (long long)p.held);
+  const long long every = pairs * p.groups;
+  const auto fit = [&](long long jobs, bool shared) {  // slots
+    return ((long long)most - kJobInts * jobs - (shared && weigh ? 2 * every : 0)) / ((part_floats(a.HS) + 2) * (long long)p.held);
+  };
   // Few blocks are not worth a look at all sequences and a second launch (16 x 12 heads of 64, one row, up to 1,024 keys 8.4
   // us, in shares 9.5 and 3.6; up to 4,096 keys 18.5, and 15 and 4; 24 x 8 heads of 128, up to 8,192 keys 50, and 36 and
-  // 4.7), nor are many groups, which fill the CUs.
-  if (blocks > 32 && jobs <= 4LL * at_once && blocks * pairs * p.groups <= 1 << 30 && (rows + p.rows) * G >> 32 == 0) {
+  // 4.7), nor are many groups, which fill the CUs. But where most groups are not there, for max_q is a few sequences', the
+  // workgroups that find none would take the time (64 sequences of 12 heads of 64,
+  // 2,048 rows of one and one of the others: 78 and 9 us in shares, 101 else).
+  if (((blocks > 32 && jobs <= 4LL * at_once) || every > 4 * jobs) && (blocks + 8) * jobs <= 1 << 30 &&
+      jobs * p.per_job < 1 << 24 && (rows + p.rows) * G >> 32 == 0) {
     // a job has one part more than workgroups' borders, and a workgroup two at most that are not whole
-    p.step = jobs <= at_once && fit >= 2 * jobs ? 1 : 2;
-    p.wgs = (int)max(min((long long)at_once, p.step == 1 ? fit - jobs : fit / 2), 0LL);
+    const long long slots = fit(jobs, true);
+    p.step = jobs <= at_once && slots >= 2 * jobs ? 1 : 2;
+    p.wgs = (int)max(min((long long)at_once, p.step == 1 ? slots - jobs : slots / 2), 0LL);
   }
   if (p.wgs) {
     p.least = 4;
     p.slots = p.step == 1 ? p.wgs + jobs : 2LL * p.wgs;
     p.grid = max(p.wgs, (int)jobs);
+    p.jobs = jobs;
   } else {
     // Whole where that fills two thirds of the CUs (192 workgroups of up to 16 blocks 8.4 us; in parts 8.1, and 4 to join
     // them); with weights to add up, the launch that joins parts is there anyway.
     const long long least = max(3 * jobs >= 2LL * cus && !weigh ? blocks : max(share, 4LL), 1LL);
     p.step = 1;
-    p.splits = (int)max(min((blocks + least - 1) / least, fit / (pairs * p.groups)), 1LL);
+    p.splits = (int)max(min(min((blocks + least - 1) / least, fit(every, false) / every), ((1LL << 24) - 1) / every), 1LL);
     p.least = (int)max((blocks + p.splits - 1) / p.splits, 1LL);
-    p.grid = (int)(pairs * p.groups * p.splits);
+    p.grid = (int)(every * p.splits);
     p.slots = p.splits > 1 ? p.grid : 0;
+    p.jobs = every;
   }
   return p;
 }
 size_t slot_floats(const ugk_cache8 &a, const Plan8 &p) { return p.slots * p.held * part_floats(a.HS); }
-size_t parts_floats(const ugk_cache8 &a, const Plan8 &p) {
-  return p.slots ? slot_floats(a, p) + 2 * (p.slots * p.held + (size_t)a.nseq * a.NKV * p.groups) : 0;
+size_t told_ints(const ugk_cache8 &a, const Plan8 &p, bool weigh) {
+  return 4 + kJobInts * p.jobs + (p.wgs && weigh ? 2 * (size_t)a.nseq * a.NKV * p.groups : 0);
 }
+size_t parts_floats(const ugk_cache8 &a, const Plan8 &p, bool weigh) {
+  return p.slots ? slot_floats(a, p) + told_ints(a, p, weigh) + 2 * p.slots * p.held : 0;
+}
+int blocks_of_keys(const ugk_cache8 &a) { return (a.max_k + kKeys - 1) / kKeys; }
 }  // namespace
 
 size_t cache8_attention_bytes(const ugk_cache8 &a, bool weigh) {
-  const size_t stat = (size_t)a.rows_q * a.NH, block = (size_t)a.nseq * a.max_q * a.NH * a.ld_table;
-  return (parts_floats(a, plan8(a, weigh)) + (weigh ? 2 * (stat + block) : 0)) * sizeof(float);
+  const size_t stat = (size_t)a.rows_q * a.NH, block = (size_t)a.nseq * a.max_q * a.NH * blocks_of_keys(a);
+  return (parts_floats(a, plan8(a, weigh), weigh) + (weigh ? 2 * (stat + block) : 0)) * sizeof(float);
 }
 
 int launch_cache8_attention(float *out, float *lse, const float *q, const void *k8, const float *ks, const void *v8,
@@ -1616,12 +1707,14 @@ int launch_cache8_attention(float *out, float *lse, const float *q, const void *
   parts.least = p.least;
   parts.wgs = p.wgs;
   parts.cus = cu_count8();
+  parts.ld = blocks_of_keys(a);
+  parts.most = (int)p.jobs;
   parts.inverse = G == 1 ? 0u : (unsigned)((1ULL << 32) / G + 1);
   if (p.slots) {
     parts.o = mem;
-    parts.ml = reinterpret_cast<float2 *>(mem + slot_floats(a, p));
-    parts.job = reinterpret_cast<int2 *>(parts.ml + p.slots * p.held);
-    mem += parts_floats(a, p);
+    parts.told = reinterpret_cast<int *>(mem + slot_floats(a, p));
+    parts.ml = reinterpret_cast<float2 *>(mem + slot_floats(a, p) + told_ints(a, p, weight));
+    mem += parts_floats(a, p, weight);
   }
   if (weight) {
     parts.stat = reinterpret_cast<float2 *>(mem);
@@ -1659,10 +1752,10 @@ int launch_cache8_attention(float *out, float *lse, const float *q, const void *
   };
   p.wgs ? of(std::true_type{}) : of(std::false_type{});
   if (int e = check_launch("cache8_attention")) return e;
-  const unsigned joins = p.slots ? pairs * grid_for((size_t)a.max_q * G, 2 * kBlock / kWave) : 0;
-  const unsigned weighs = weight ? (unsigned)a.nseq * ((a.ld_table + 15) / 16) : 0;
+  const unsigned joins = p.slots ? (unsigned)(p.jobs * p.per_job) : 0;
+  const unsigned weighs = weight ? (unsigned)a.nseq * grid_for(parts.ld, 16) : 0;
   if (joins + weighs == 0) return UGK_OK;
-  launch(k_cache8_finish, dim3(joins + weighs), dim3(kBlock), 0, out, lse, weight, parts, a, p.rows, p.groups, joins);
+  launch(k_cache8_finish, dim3(joins + weighs), dim3(kBlock), 0, out, lse, weight, parts, a, p.rows, p.groups, p.per_job, joins);
   return check_launch("cache8_attention");
 }
 
@@ -1683,19 +1776,30 @@ static int touched_blocks(const ugk_cache8 &a) {
     case 7: go(kernel<7>); break;                                              \
     default: go(kernel<8>);                                                    \
   }
+// Workgroups of a head by blocks: `per` of each sequence, or, where that is more than twice as many as there can be (max_q is
+// a few sequences'; 64 of 12 heads of 64, 2,048 rows of one and one of the others: 12 us, 41 else) and the CUs would have
+// rounds of them, `all` that there can be. Rows of a sequence touch one block more than they fill, and another where they
+// begin.
+struct Store8 {
+  int per, all;
+};
+static Store8 store8(const ugk_cache8 &a) {
+  const long long per = touched_blocks(a), most = a.nseq * per, all = a.rows_q / kKeys + 2LL * a.nseq;
+  return most > 2 * all && 2 * most * a.NKV > 16LL * cu_count8() ? Store8{0, (int)all} : Store8{(int)per, (int)most};
+}
 int launch_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, const float *v, const ugk_cache8 &a, int *word) {
-  const int per = touched_blocks(a);
+  const Store8 n = store8(a);
   const auto go = [&](auto kernel) {
-    launch(kernel, dim3((unsigned)a.nseq * a.NKV * per, 2), dim3(kBlock), 0, (int8_t *)k8, ks, (int8_t *)v8, vs, k, v, a, per, word);
+    launch(kernel, dim3((unsigned)n.all * a.NKV, 2), dim3(kBlock), 0, (int8_t *)k8, ks, (int8_t *)v8, vs, k, v, a, n.per, n.all, word);
   };
   UGK_CH8(k_cache8_store)
   return check_launch("cache8_store");
 }
 int launch_cache8_load(float *k, float *v, const void *k8, const float *ks, const void *v8, const float *vs, const ugk_cache8 &a,
                        int *word) {
-  const int per = touched_blocks(a);
+  const Store8 n = store8(a);
   const auto go = [&](auto kernel) {
-    launch(kernel, dim3((unsigned)a.nseq * a.NKV * per, 2), dim3(kBlock), 0, k, v, (const int8_t *)k8, ks, (const int8_t *)v8, vs, a, per,
+    launch(kernel, dim3((unsigned)n.all * a.NKV, 2), dim3(kBlock), 0, k, v, (const int8_t *)k8, ks, (const int8_t *)v8, vs, a, n.per, n.all,
            word);
   };
   UGK_CH8(k_cache8_load)
