@@ -512,8 +512,8 @@ int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks,
  * of the weight and 2^-38 of the largest contribution (weight times the values'
  * scale) that the row sees. Products with the codes are exact, statistics and sums
  * in single precision. A score of about 2^127 or more, or an infinity or NaN in its row
- * of q, makes a row's out and lse NaN; one of about -2^127 or less weighs nothing. out
- * must not overlap q.
+ * of q, makes a row's out, lse and what it adds to `weight` NaN; one of about -2^127 or
+ * less weighs nothing. out must not overlap q.
  * weight, if not NULL, (nseq, ld_table): weight[b, j] += the sum of the weights over
  * sequence b's rows and heads and the keys of its block j. For up to 256 query rows
  * times heads per key/value head: tokens, drafts, or the last rows of a prompt. It

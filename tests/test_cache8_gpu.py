@@ -399,6 +399,25 @@ def test_rows_that_are_no_numbers(gpu, lq):
     gpu.synchronize()
 
 
+@pytest.mark.parametrize("cap", [300, 2500])
+@pytest.mark.parametrize("lq", [1, 6, 20])
+def test_weights_of_a_row_that_is_no_number(gpu, lq, cap):
+    """The blocks that it sees get NaN; other sequences' get what they would."""
+    NH, NKV, HS = 4, 2, 64
+    keys = [cap - 70, cap, 90]
+    c, g = filled(gpu, 3, cap, NKV, HS, keys)
+    starts, rows = place_rows([lq] * 3)
+    q = rand(g, rows, NH, HS)
+    want, got = (torch.zeros(c.table.shape, device=DEV) for _ in "wg")
+    attend(gpu, c, NH, q, starts, [lq] * 3, keys, rows, weight=want)
+    q[starts[1], 3, 9] = math.nan
+    attend(gpu, c, NH, q, starts, [lq] * 3, keys, rows, weight=got)
+    gpu.synchronize()
+    seen = -(-(keys[1] - lq + 1) // 64)  # of the sequence's first row
+    assert got[1, :seen].isnan().all() and not got[1, seen:].isnan().any()
+    assert torch.equal(got[[0, 2]], want[[0, 2]])
+
+
 @pytest.mark.parametrize("lq", [1, 3, 40])
 def test_what_lies_outside_does_not_matter(gpu, lq):
     """Codes behind the last key, blocks of others, scales of others, q rows of nobody: the same bits whatever they are."""
