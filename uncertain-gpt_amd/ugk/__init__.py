@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional
 
 __all__ = [
@@ -101,31 +102,35 @@ class Cache8(ctypes.Structure):
     defaults to 1/sqrt(HS). The structure keeps its tensors alive; a call refuses an ``nseq`` or ``ld_table`` raised above what
     they hold.
     """
-    _tensors = ()
-    _most = (2 ** 31 - 1, 2 ** 62)  # sequences that the offset tensors hold, entries of the table
+    _tensors = (None,) * 4
+    _checked = (0, 0)  # sequences, and entries of the table, that the tensors were seen to hold
     _NAMES = ("q_start", "q_end", "k_len", "table")
     _fields_ = [(_n, _i) for _n in ("nseq", "NH", "NKV", "HS", "rows_q", "max_q", "max_k", "nblocks", "causal")] + \
         [("scale", _fl)] + [(_n, _fp) for _n in _NAMES] + [("ld_table", _i)] + \
         [(_n, ctypes.c_longlong) for _n in ("ldq", "ldk", "ldv", "ldo")]
+    _PACK = struct.Struct("@9if4Pi4q")  # the fields at once, a third of the time that ctypes takes for them
 
     def __init__(self, nseq: int, NH: int, NKV: int, HS: int, rows_q: int, max_q: int, max_k: int, nblocks: int,
                  causal: bool = True, scale: Optional[float] = None, q_start=None, q_end=None, k_len=None, table=None,
                  ld_table: int = 0, ldq: int = 0, ldk: int = 0, ldv: int = 0, ldo: int = 0):
         if scale is None:
             scale = HS ** -0.5 if HS > 0 else 0.0
-        held = table is not None and not isinstance(table, int)
-        if held and not ld_table and table.dim() == 2:
+        if not ld_table and table is not None and not isinstance(table, int) and table.dim() == 2:
             ld_table = table.shape[1]
         entries = max(nseq, 0) * (ld_table or -(-max_k // CACHE8_BLOCK))
-        super().__init__(nseq, NH, NKV, HS, rows_q, max_q, max_k, nblocks, 1 if causal else 0, scale,
-                         _ptr(q_start, "q_start", nseq, "i32"), _ptr(q_end, "q_end", nseq, "i32"), _ptr(k_len, "k_len", nseq, "i32"),
-                         _ptr(table, "table", entries, "i32"), ld_table, ldq, ldk, ldv, ldo)
+        p0, p1, p2 = _ptr(q_start, "q_start", nseq, "i32"), _ptr(q_end, "q_end", nseq, "i32"), _ptr(k_len, "k_len", nseq, "i32")
+        p3 = _ptr(table, "table", entries, "i32")
+        try:
+            self._PACK.pack_into(self, 0, nseq, NH, NKV, HS, rows_q, max_q, max_k, nblocks, 1 if causal else 0, scale,
+                                 p0 or 0, p1 or 0, p2 or 0, p3 or 0, ld_table, ldq, ldk, ldv, ldo)
+        except struct.error:  # something else than numbers in their ranges: as ctypes takes or refuses it
+            super().__init__(nseq, NH, NKV, HS, rows_q, max_q, max_k, nblocks, 1 if causal else 0, scale, p0, p1, p2, p3, ld_table,
+                             ldq, ldk, ldv, ldo)
         self._tensors = (q_start, q_end, k_len, table)
-        most, held_most = Cache8._most
-        for t in (q_start, q_end, k_len):
-            if t is not None and not isinstance(t, int):
-                most = min(most, t.numel())
-        self._most = (most, table.numel() if held else held_most)
+        self._checked = (nseq, entries)
+
+
+assert Cache8._PACK.size == ctypes.sizeof(Cache8)
 
 
 _MATMUL_FWD = ctypes.CFUNCTYPE(_i, _fp, _fp, _fp, _fp, _fp, _i, _i, _i)
@@ -620,10 +625,13 @@ def cache8_bytes(nblocks: int, NKV: int, HS: int) -> int:
 
 def _cache8(a: Cache8, k8, ks, v8, vs):
     """The cache's addresses, after the checks of what a call's structure holds."""
-    if a.nseq > a._most[0]:
-        raise ValueError(f"nseq: {a.nseq} sequences, the offsets hold {a._most[0]}")
-    if a.nseq * (a.ld_table or -(-a.max_k // CACHE8_BLOCK)) > a._most[1]:
-        raise ValueError(f"table: {a.nseq} rows of {a.ld_table}, the tensor holds {a._most[1]} entries")
+    nseq = a.nseq
+    entries = nseq * (a.ld_table or -(-a.max_k // CACHE8_BLOCK))
+    if nseq > a._checked[0] or entries > a._checked[1]:  # raised since
+        for t, name, need in zip(a._tensors, a._NAMES, (nseq, nseq, nseq, entries)):
+            if t is not None and not isinstance(t, int) and t.numel() < need:
+                raise ValueError(f"{'table' if t is a._tensors[3] else 'nseq'}: {nseq} sequences and {entries} entries of their table, "
+                                 f"{name} holds {t.numel()}")
     if not _one_device:
         for t, name in zip(a._tensors, a._NAMES):
             _here(t, name)
@@ -632,12 +640,15 @@ def _cache8(a: Cache8, k8, ks, v8, vs):
     return (_ptr_here(k8, "k8", n, "i8"), _ptr_here(ks, "ks", scales), _ptr_here(v8, "v8", n, "i8"), _ptr_here(vs, "vs", scales))
 
 
-def _cache8_rows(a: Cache8, ld: int, heads: int):
-    """Of rows of ``heads`` heads the floats from the first element to the end of the last row, from row to row and in a row, and
-    the heads."""
-    w = heads * a.HS
+def _cache8_rows(x, what: str, a: Cache8, ld: int, heads: int):
+    """Device address of a call's rows of ``heads`` heads, ``ld`` floats apart (0: without gaps); _rows_ptr's line here, for a
+    small call is mostly this."""
+    rows, w = a.rows_q, heads * a.HS
     ld = ld or w
-    return ((a.rows_q - 1) * ld + w if a.rows_q > 0 else 0, ld, w, heads)
+    need = (rows - 1) * ld + w if rows > 0 else 0
+    if type(x) is _Tensor and _one_device and x.dtype is _DTYPES["f32"] and x.is_cuda and x.numel() >= need and x.is_contiguous():
+        return x.data_ptr()
+    return _rows_ptr_or_raise(x, what, need, ld, w, heads)
 
 
 def cache8_store(k8, ks, v8, vs, k, v, a: Cache8) -> None:
@@ -645,13 +656,13 @@ def cache8_store(k8, ks, v8, vs, k, v, a: Cache8) -> None:
     sequences: int8 codes in k8 and v8 (``cache8_bytes`` each), a power of two per block and key/value head in ks and vs
     (nblocks, NKV)."""
     c = _cache8(a, k8, ks, v8, vs)
-    _check(lib.ugk_cache8_store(*c, _rows_ptr(k, "k", _cache8_rows(a, a.ldk, a.NKV)), _rows_ptr(v, "v", _cache8_rows(a, a.ldv, a.NKV)), a))
+    _check(lib.ugk_cache8_store(*c, _cache8_rows(k, "k", a, a.ldk, a.NKV), _cache8_rows(v, "v", a, a.ldv, a.NKV), a))
 
 
 def cache8_load(k, v, k8, ks, v8, vs, a: Cache8) -> None:
     """What the cache holds where cache8_store of the same ``a`` puts it, to the rows of k and v."""
     c = _cache8(a, k8, ks, v8, vs)
-    _check(lib.ugk_cache8_load(_rows_ptr(k, "k", _cache8_rows(a, a.ldk, a.NKV)), _rows_ptr(v, "v", _cache8_rows(a, a.ldv, a.NKV)), *c, a))
+    _check(lib.ugk_cache8_load(_cache8_rows(k, "k", a, a.ldk, a.NKV), _cache8_rows(v, "v", a, a.ldv, a.NKV), *c, a))
 
 
 def cache8_attention(out, lse, q, k8, ks, v8, vs, a: Cache8, weight=None) -> None:
@@ -659,8 +670,8 @@ def cache8_attention(out, lse, q, k8, ks, v8, vs, a: Cache8, weight=None) -> Non
     what each block got over the rows and heads."""
     c = _cache8(a, k8, ks, v8, vs)
     w = None if weight is None else _ptr_here(weight, "weight", a.nseq * (a.ld_table or -(-a.max_k // CACHE8_BLOCK)))
-    _check(lib.ugk_cache8_attention(_rows_ptr(out, "out", _cache8_rows(a, a.ldo, a.NH)), _ptr_here(lse, "lse", a.rows_q * a.NH),
-                                    _rows_ptr(q, "q", _cache8_rows(a, a.ldq, a.NH)), *c, w, a))
+    _check(lib.ugk_cache8_attention(_cache8_rows(out, "out", a, a.ldo, a.NH), _ptr_here(lse, "lse", a.rows_q * a.NH),
+                                    _cache8_rows(q, "q", a, a.ldq, a.NH), *c, w, a))
 
 
 def cache8_evict(table_out, len_out, weight_out, dropped, table, k_len, weight, nseq: int, ld: int, keep: int, first: int = 0,
