@@ -690,6 +690,51 @@ def test_captured_and_on_another_stream(gpu):
     assert dropped.tolist() == [0, 0, 2]
 
 
+@pytest.mark.parametrize("lq,NH,weigh", [(1, 2, True), (6, 8, True), (70, 4, False)])
+def test_captured_with_lengths_that_change(gpu, lq, NH, weigh):
+    """A graph's replays take the lengths, rows and blocks that the tensors hold then, and share out the work anew."""
+    NKV, HS, cap, nseq = 2, 64, 2600, 5
+    c, g = filled(gpu, nseq, cap, NKV, HS, [cap] * nseq)
+    starts, rows = place_rows([lq] * nseq)
+    q = rand(g, rows, NH, HS)
+    out, lse = torch.empty(rows, NH, HS, device=DEV), torch.empty(rows, NH, device=DEV)
+    weight = torch.zeros(c.table.shape, device=DEV) if weigh else None
+    lens, end = ints([cap] * nseq), ints([a + lq for a in starts])
+    a = c.call(NH, starts, [lq] * nseq, [cap] * nseq, rows, k_len=lens, q_end=end)
+
+    def step():
+        if weigh:
+            weight.zero_()
+        gpu.cache8_attention(out, lse, q, *c.parts(), a, weight=weight)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        gpu.set_stream(s.cuda_stream)
+        try:
+            step()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                step()
+            for n, keys in enumerate(([cap, 1, 700, 64, 0], [lq] * nseq, [2048, 2049, cap, 3, 1], [cap] * nseq)):
+                lens.copy_(ints(keys))
+                end.copy_(ints([x + lq - (b + n) % 2 * (lq // 2) for b, x in enumerate(starts)]))
+                c.table.copy_(c.table.roll(n, 0))
+                for t in (out, lse):
+                    t.fill_(5.0)
+                step()
+                want = [t.clone() for t in (out, lse, weight) if t is not None]
+                for t in (out, lse):
+                    t.fill_(5.0)
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert all(torch.equal(t, w) for t, w in zip([t for t in (out, lse, weight) if t is not None], want)), n
+        finally:
+            s.synchronize()
+            gpu.set_stream(None)
+    check(gpu, c, NH, q, starts, [lq] * nseq, [cap] * nseq, rows, weigh=weigh)
+
+
 def test_tensors_too_small_are_refused(gpu):
     c, g = filled(gpu, 2, 200, 2, 64, [150, 200])
     q, out = rand(g, 2, 4, 64), torch.empty(2, 4, 64, device=DEV)
