@@ -618,6 +618,21 @@ def test_rows_in_several_sequences_are_reported(gpu, lq, weigh):
     assert (out == 7.0).all() and (not weigh or not weight.any())
 
 
+@pytest.mark.parametrize("lq,NH,NKV,HS", [(1, 2, 1, 64), (7, 6, 3, 33), (50, 3, 1, 16)])
+def test_a_padded_batch(gpu, lq, NH, NKV, HS):
+    """Few of many sequences have rows."""
+    nseq, cap = 333, 2200
+    lens, keys = [0] * nseq, [0] * nseq
+    for b, n in ((2, 2200), (3, 40), (66, 1), (67, 700), (68, 64), (200, 2100), (331, 1500)):
+        lens[b], keys[b] = lq, n
+    c, g = filled(gpu, nseq, cap, NKV, HS, keys)
+    starts, rows = place_rows(lens, gap=0)
+    q = rand(g, rows, NH, HS)
+    check(gpu, c, NH, q, starts, lens, keys, rows)
+    if lq * NH // NKV <= 256:
+        check(gpu, c, NH, q, starts, lens, keys, rows, weigh=True)
+
+
 def test_many_groups_of_rows_in_a_sequence(gpu):
     """More than 64 workgroups' rows in one sequence, whose key axis is cut all the same."""
     NH, NKV, HS, lq, n = 8, 1, 16, 1100, 2400

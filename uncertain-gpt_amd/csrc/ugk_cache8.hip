@@ -641,7 +641,6 @@ struct Jobs {
       if (lane == l) h.units = sum;
     }
     return h;
-    return h;
   }
 
   // The first job; false: none.
@@ -715,13 +714,18 @@ struct Jobs {
     if (++w.hk == a.NKV) {
       w.hk = 0;
       if (--w.group < 0) {
-        do {
-          if (++w.b == a.nseq) return false;
-          const Seq8 s = sequence8(a, w.b, false, word, 0);
-          w.s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
-          w.s.Lq = __builtin_amdgcn_readfirstlane(s.Lq);
-          w.s.Lk = __builtin_amdgcn_readfirstlane(s.Lk);
-        } while (w.s.Lq == 0);
+        // the next sequence that has rows: a lane to each, for many may have none
+        for (uint64_t some = 0; !some;) {
+          if (++w.b >= a.nseq) return false;
+          Seq8 s{0, 0, 0};
+          if (w.b + lane < a.nseq) s = sequence8(a, w.b + lane, false, word, 0);
+          some = __ballot(s.Lq > 0);
+          const int l = some ? __builtin_ctzll(some) : kWave - 1;
+          w.b += l;
+          w.s.q0 = __builtin_amdgcn_readlane(s.q0, l);
+          w.s.Lq = __builtin_amdgcn_readlane(s.Lq, l);
+          w.s.Lk = __builtin_amdgcn_readlane(s.Lk, l);
+        }
         w.group = (w.s.Lq * G + R - 1) / R - 1;
       }
     }
@@ -1643,8 +1647,8 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   // of 128, one to a CU: tiles 81 us, not 64, 32 rows 46, not 36); with more, some CUs have a second round (32 rows of heads
   // of 64, four: 29, not 24).
   const int at_once = cus * (a.HS > 64 ? (p.rows == 4 ? 3 : 2) : (p.rows == 4 ? 4 : 3));
-  // at most so many jobs, and the shares of so many blocks, were all sequences full
-  const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + a.nseq) * a.NKV), share = blocks * jobs / at_once;
+  // at most so many jobs (a sequence that has one has a row), and the shares of so many blocks, were all sequences full
+  const long long jobs = min(pairs * p.groups, (a.rows_q * G / p.rows + min(a.nseq, a.rows_q)) * a.NKV), share = blocks * jobs / at_once;
   // what a workspace of the same rows and heads has for the fp32 attention
   const size_t most = max(attention_parts_bound(a.HS), attention_backward_bound(a.rows_q, a.NH, a.HS)) / sizeof(float) - 4;
   const long long every = pairs * p.groups;
@@ -1654,10 +1658,11 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   // Few blocks are not worth a look at all sequences and a second launch (16 x 12 heads of 64, one row, up to 1,024 keys 8.4
   // us, in shares 9.5 and 3.6; up to 4,096 keys 18.5, and 15 and 4; 24 x 8 heads of 128, up to 8,192 keys 50, and 36 and
   // 4.7), nor are many groups, which fill the CUs. But where most groups are not there, for max_q is a few sequences', the
-  // workgroups that find none would take the time (64 sequences of 12 heads of 64,
-  // 2,048 rows of one and one of the others: 78 and 9 us in shares, 101 else).
-  if (((blocks > 32 && jobs <= 4LL * at_once) || every > 4 * jobs) && (blocks + 8) * jobs <= 1 << 30 &&
-      jobs * p.per_job < 1 << 24 && (rows + p.rows) * G >> 32 == 0) {
+  // workgroups that find none would take the time (64 sequences of 12 heads of 64, 2,048 rows of one and one of the others:
+  // 78 and 9 us in shares, 101 else; where they are few it is nothing: a row of each of 10 of 400 sequences of up to 1,024
+  // keys 12.6 and 3.8, 11.0 else).
+  const bool few = blocks > 32 && jobs <= 4LL * at_once, empty = every > 4 * jobs && every > 8LL * at_once;
+  if ((few || empty) && (blocks + 8) * jobs <= 1 << 30 && jobs * p.per_job < 1 << 24 && (rows + p.rows) * G >> 32 == 0) {
     // a job has one part more than workgroups' borders, and a workgroup two at most that are not whole
     const long long slots = fit(jobs, true);
     p.step = jobs <= at_once && slots >= 2 * jobs ? 1 : 2;
@@ -1784,7 +1789,7 @@ struct Store8 {
   int per, all;
 };
 static Store8 store8(const ugk_cache8 &a) {
-  const long long per = touched_blocks(a), most = a.nseq * per, all = a.rows_q / kKeys + 2LL * a.nseq;
+  const long long per = touched_blocks(a), most = a.nseq * per, all = a.rows_q / kKeys + 2LL * min(a.nseq, a.rows_q);
   return most > 2 * all && 2 * most * a.NKV > 16LL * cu_count8() ? Store8{0, (int)all} : Store8{(int)per, (int)most};
 }
 int launch_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, const float *v, const ugk_cache8 &a, int *word) {
