@@ -64,6 +64,26 @@ def test_pointers_refused_on_the_host():
     assert lib.ugk_cache8_attention(*P[:8], many) == 1 and b"256 rows" in lib.ugk_last_error()
 
 
+def test_weights_of_more_workgroups_than_a_grid_has():
+    import ugk
+    a = shape(ugk, nseq=2000000, NH=1, NKV=1, rows_q=256, max_q=256, max_k=64, nblocks=8, q_start=64, q_end=128, table=256, ld_table=1)
+    x = list(P[:8])
+    assert ugk.lib.ugk_cache8_attention(*x, a) == 1 and b"grid" in ugk.lib.ugk_last_error()
+
+
+def test_the_structure_holds_what_it_was_given():
+    import ugk
+    given = dict(nseq=3, NH=8, NKV=2, HS=50, rows_q=11, max_q=7, max_k=130, nblocks=9, causal=False, scale=0.5, q_start=64, q_end=128,
+                 k_len=192, table=256, ld_table=5, ldq=400, ldk=1 << 40, ldv=101, ldo=402)
+    a = ugk.Cache8(**given)
+    for name, value in given.items():
+        assert getattr(a, name) == value, name
+    b = ugk.Cache8(1, 1, 1, 64, 1, 1, 64, 1)
+    assert (b.q_start, b.q_end, b.k_len, b.table, b.ld_table, b.ldq, b.causal, b.scale) == (None, None, None, None, 0, 0, 1, 0.125)
+    with pytest.raises(TypeError):
+        ugk.Cache8(1, 1, 1, 64, 1, 1, 64, 1.5)
+
+
 def test_nothing_to_do_is_done_without_a_gpu():
     import ugk
     lib = ugk.lib
