@@ -494,10 +494,17 @@ struct Codes {
 #pragma unroll
       for (int st = 0; st < KS; st++) kf[st][kt] = *reinterpret_cast<const v4i *>(p + kt * 16 * HP + koff[st]);
   }
+  // kOnce: no other wavefront loads them, and they pass the caches by (24 conversations of one token 62 us, else 70; of 32
+  // rows, of which two wavefronts take each block, 32, and past the caches 33. Keys past the caches: 41, for a block's 64
+  // bytes of a row are half of what a load brings).
+  template <bool kOnce>
   __device__ __forceinline__ void values(const int8_t *v8, size_t at) {
     const int8_t *p = v8 + at * kKeys * HP;
 #pragma unroll
-    for (int t = 0; t < DT; t++) vf[t] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(p + min(t, HP / 16 - 1) * 16 * kKeys + voff));
+    for (int t = 0; t < DT; t++) {
+      const v4i *x = reinterpret_cast<const v4i *>(p + min(t, HP / 16 - 1) * 16 * kKeys + voff);
+      vf[t] = kOnce ? __builtin_nontemporal_load(x) : *x;
+    }
   }
 };
 
@@ -1071,7 +1078,7 @@ __device__ __forceinline__ void rows_job(float *out, float *lse, const float *q,
   if (walk.j < stop) {
     const size_t at = block_head(walk.id, a.NKV, hk);
     c.keys(k8, at);
-    c.values(v8, at);
+    c.template values<R != 32>(v8, at);
     kscale = ks[at];
     vscale = vs[at];
   }
@@ -1096,7 +1103,7 @@ __device__ __forceinline__ void rows_job(float *out, float *lse, const float *q,
     rows.weights(p, mb, k, lp[wave], w, fo, fb);
     rows.add(c, w, fo, fb);
     __builtin_amdgcn_sched_barrier(0);
-    if (kNext) c.values(v8, ahead);
+    if (kNext) c.template values<R != 32>(v8, ahead);
     if (kNext) walk.step(id);
   };
   while (walk.more()) block(std::true_type{});
@@ -1178,7 +1185,7 @@ constexpr int kJoinRows8 = 2 * kBlock / kWave;  // rows that a workgroup joins
 // three dependent loads; 9 us of prompts behind long conversations (35 MB of parts).
 __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse, float *weight, Parts8 parts, ugk_cache8 a, int rows,
                                                          int groups, int per_job, unsigned joins) {
-  constexpr int kAtOnce = 4;  // parts whose loads are on their way together
+  constexpr int kAtOnce = 4;  // of blocks
   const int G = a.NH / a.NKV;
   if (blockIdx.x >= joins) {
     __shared__ float part[16][17];
@@ -1244,30 +1251,36 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
   const size_t g = (size_t)from.x + rr / G;
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int t = 0; t < n; t += kAtOnce) {
-    float4 y[kAtOnce];
-    float2 x[kAtOnce];
+  // So many parts' loads are on their way together (four throughout: one conversation's 64 parts 6.6 us, not 6.1; twelve:
+  // prompts behind long conversations 10.4, not 9.1).
+  const auto join = [&](auto many, int t) {
+    constexpr int kParts = decltype(many)::value;
+    float4 y[kParts];
+    float2 x[kParts];
     float top = m;
 #pragma unroll
-    for (int u = 0; u < kAtOnce; u++) {
+    for (int u = 0; u < kParts; u++) {
       const size_t p = part_row(parts, job.x, min(t + u, n - 1), r);
       y[u] = ld4(parts.o + p * floats + min(d, floats - 4));
       x[u] = parts.ml[p];
       if (t + u >= n) x[u].y = 0.0f;
     }
 #pragma unroll
-    for (int u = 0; u < kAtOnce; u++) top = fmaxf(top, x[u].y == 0.0f ? -INFINITY : x[u].x);
+    for (int u = 0; u < kParts; u++) top = fmaxf(top, x[u].y == 0.0f ? -INFINITY : x[u].x);
     const float keep = ex2(m - or0(top));
     m = top;
     l *= keep;
     o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
 #pragma unroll
-    for (int u = 0; u < kAtOnce; u++) {
+    for (int u = 0; u < kParts; u++) {
       const float w = x[u].y == 0.0f ? 0.0f : x[u].y * ex2(x[u].x - or0(top));  // 0: a part without a key of this row, its o is 0
       l += w;
       o = make_float4(fmaf(w, y[u].x, o.x), fmaf(w, y[u].y, o.y), fmaf(w, y[u].z, o.z), fmaf(w, y[u].w, o.w));
     }
-  }
+  };
+  int t = 0;
+  for (; t + 4 < n; t += 8) join(std::integral_constant<int, 8>{}, t);
+  if (t < n) join(std::integral_constant<int, 4>{}, t);
   const bool none = l == 0.0f;
   const float inv = none ? 1.0f : 1.0f / l;
   put4(out + g * a.ldo + (size_t)h * a.HS + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.HS - d);
