@@ -870,7 +870,8 @@ struct Four {
   // The weights as an operand.
   __device__ __forceinline__ void weights(Scores &p, float mb, const Block8 &k, uint32_t *lp, Weights &ap, float &fo, float &fb) {
     const int col = k.lane & 15, quad = k.lane >> 4;
-    const float fac = here(nan ? NAN : score_factor(k.f, k.kscale, ex)), most = max16(mb);
+    // a number where the row sees nothing: the result of one without any key is 0 whatever it holds
+    const float most = max16(mb), fac = here(nan && most != -INFINITY ? NAN : score_factor(k.f, k.kscale, ex));
     mb = top_score(most, fac);
     float less = less_top(mb, 0.0f);
     if (__any(far_score(mb))) {
@@ -1007,7 +1008,7 @@ struct Sixteen {
     return mb;
   }
   __device__ __forceinline__ void weights(Scores &p, float mb, const Block8 &k, uint32_t *, Weights &bp, float &fo, float &fb) {
-    const float fac = here(nan ? NAN : score_factor(k.f, k.kscale, ex)), most = quarters_max(mb);
+    const float most = quarters_max(mb), fac = here(nan && most != -INFINITY ? NAN : score_factor(k.f, k.kscale, ex));
     mb = top_score(most, fac);
     float less = less_top(mb, 0.0f);
     if (__any(far_score(mb))) {
@@ -1420,8 +1421,8 @@ __device__ __forceinline__ void tile_job(float *out, float *lse, const float *q,
       *reinterpret_cast<v2u *>(vt + vdst[n] + 32) = halves4(__builtin_amdgcn_perm(t3, t1, 0x05040100u));
       *reinterpret_cast<v2u *>(vt + vdst[n] + 48) = halves4(__builtin_amdgcn_perm(t3, t1, 0x07060302u));
     }
-    const float fac = here(nan ? NAN : score_factor(f, kscale, e)), vnow = exponent(vscale);
     const bool held = there;
+    const float fac = here(score_factor(f, kscale, e)), vnow = exponent(vscale);
     __syncthreads();
     if (j + 1 < stop) fetch(j + 1);
     if (idle || j * kKeys >= most_seen) continue;
@@ -1511,7 +1512,8 @@ __device__ __forceinline__ void tile_job(float *out, float *lse, const float *q,
     if (!apart) run.sum(mb, lb, run.mo, up);
   }
   if (mine >= rows) return;
-  const float sum = half_sum(run.l);
+  float sum = half_sum(run.l);
+  if (nan && sum != 0.0f) sum = NAN;  // (its q is 0 here: all keys that it sees have the weight 1)
   int p;
   const float g = run.last(sum, &p);
   p -= 14;  // of the weights
