@@ -467,7 +467,7 @@ typedef struct {
   int NH, NKV, HS;    /* as in ugk_attention */
   int rows_q;         /* rows of q, out, lse and of store's and load's k and v */
   int max_q, max_k;   /* the most of these rows and the most keys of a sequence */
-  int nblocks;        /* blocks of the cache */
+  int nblocks;        /* blocks of the cache; attention takes 0 only with max_k 0 */
   int causal;         /* nonzero: row i of Lq sees the keys j <= i + Lk - Lq */
   float scale;        /* of the scores */
   /* DEVICE arrays. Sequence b has the rows [q_start[b], q_end[b]), its last

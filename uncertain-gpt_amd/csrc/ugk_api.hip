@@ -898,6 +898,7 @@ int ugk_cache8_attention(float *out, float *lse, const float *q, const void *k8,
     return bad(fn, "nseq * heads * rows exceeds the grid");
   if (none) return ok();
   if (any_null({out, q})) return bad(fn, "NULL pointer");
+  if (a.max_k > 0 && a.nblocks == 0) return bad(fn, "nblocks must be >= 1 where max_k is");  // a masked block is read as block 0
   if (a.max_k > 0 && any_null({k8, ks, v8, vs})) return bad(fn, "NULL pointer");
   if (out == q) return bad(fn, "out must be distinct from q");
   if (!aligned16(k8) || !aligned16(v8)) return bad(fn, "k8 and v8 must be 16-byte aligned");
