@@ -545,7 +545,7 @@ int ugk_cache8_evict(int *table_out, int *len_out, float *weight_out,
  * throughout), or, all accepted, from p[b, n]: the first whose cumulative sum passes u[b, K] times the
  * whole. With u (nseq, K + 1) uniform in [0, 1) tokens are distributed as the target's. tokens (nseq, K + 1): the accepted
  * drafts, that token, then -1. Products and sums are in 64 bits. p and q need not add up to 1; entries
- * that are not positive finite numbers count as 0. A draft that is no token is not accepted, and a row of p without
+ * of either that are not positive finite numbers count as 0. A draft that is no token is not accepted, and a row of p without
  * a probability gives token 0: either, and n_draft outside [0, K], the next ugk_synchronize reports. */
 int ugk_draft_verify(int *accepted, int *tokens, const float *p, const float *q,
                      const int *draft, const int *n_draft, const float *u,

@@ -15,15 +15,17 @@ constexpr int kDraftThreads = 1024, kDraftWaves = kDraftThreads / kWave, kSumThr
 constexpr int kStep = 4 * kDraftThreads;  // floats that a workgroup takes at a time
 constexpr int kMaxSegs = 1024;            // segments of a row
 
+// x, or 0 where it is no probability: neither a positive normal (class 8) nor a positive subnormal (7) number.
+__device__ __forceinline__ float probability(float x) { return __builtin_amdgcn_classf(x, 1 << 7 | 1 << 8) ? x : 0.0f; }
+
 // One sequence's row that its next token is drawn from: p, less the drafts' probabilities of the row (or null) or without the
-// one token (or -1) whose draft was certain; what is not positive and finite counts as 0.
+// one token (or -1) whose draft was certain.
 struct Row {
   const float *p, *less;
   int gone, a, n;  // accepted drafts, drafts
   bool bad;
   __device__ __forceinline__ double one(float x, float y, int v) const {
-    const double d = (double)x - (double)y;
-    return v != gone && d > 0.0 && d <= 3.402823466e38 ? d : 0.0;
+    return fmax((double)(v == gone ? 0.0f : probability(x)) - (double)probability(y), 0.0);
   }
   // N times four tokens, v0 .. v0 + 3, `step` apart, those from `end` on 0. whole: all of the wavefront's are before it. (All
   // loads before the first use: a branch around each would wait for it.)
@@ -91,7 +93,7 @@ __device__ Row verify(const float *p, const float *q, const int *draft, const in
     if (no) {
       const int t = draft[i];
       if ((unsigned)t < (unsigned)V) {  // else no token: not accepted
-        const double pt = p[(size_t)i * V + t], qt = q ? q[(size_t)i * V + t] : 1.0;
+        const double pt = probability(p[(size_t)i * V + t]), qt = q ? probability(q[(size_t)i * V + t]) : 1.0;
         no = !((double)u[i] * qt < pt);
       }
     }
