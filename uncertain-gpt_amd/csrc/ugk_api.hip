@@ -940,8 +940,9 @@ int ugk_draft_verify(int *accepted, int *tokens, const float *p, const float *q,
   if (V > 1 << 30) return bad(fn, "V exceeds 2^30");
   if (nseq == 0) return ok();
   if (any_null({accepted, tokens, p, u}) || (K > 0 && !draft)) return bad(fn, "NULL pointer");
-  if (any_same({accepted, tokens, draft}) || (n_draft && any_same({accepted, tokens, n_draft})))
-    return bad(fn, "accepted and tokens must be distinct from each other and from the inputs");
+  for (const void *in : {(const void *)p, (const void *)q, (const void *)draft, (const void *)n_draft, (const void *)u})
+    if (any_same({accepted, tokens, in}))  // (neither is NULL)
+      return bad(fn, "accepted and tokens must be distinct from each other and from the inputs");
   int *word = ids_error_word();
   if (!word) return UGK_EHIP;
   double *sums = nullptr;
