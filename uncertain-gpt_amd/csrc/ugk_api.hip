@@ -427,10 +427,9 @@ int check_cache8(const char *fn, ugk_cache8 *a, bool *none) {
     return bad(fn, "rows * stride exceeds the address space");
   a->max_q = a->max_q < a->rows_q ? a->max_q : a->rows_q;
   if ((long long)a->max_q * (a->NH / a->NKV) > INT_MAX / 2) return bad(fn, "max_q * NH / NKV exceeds 2^30");
-  // a launch has fewer than 2^32 threads: a workgroup of 256 for 64 keys of a sequence and key/value head, or 128 rows and heads
-  const long long tq = ((long long)a->max_q * (a->NH / a->NKV) + 127) / 128 + 1, tk = blocks + 1;
-  const long long per = (long long)a->nseq * a->NKV;
-  if (per >= ((long long)1 << 23) / (tq > tk ? tq : tk)) return bad(fn, "nseq * heads * rows exceeds the grid");
+  // a launch has fewer than 2^32 threads: a workgroup of 256 for 128 rows and heads of a sequence and key/value head
+  const long long tq = ((long long)a->max_q * (a->NH / a->NKV) + 127) / 128 + 1;
+  if ((long long)a->nseq * a->NKV >= ((long long)1 << 23) / tq) return bad(fn, "nseq * heads * rows exceeds the grid");
   *none = a->nseq == 0 || a->max_q == 0;
   return UGK_OK;
 }
@@ -863,6 +862,7 @@ int ugk_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, c
   bool none;
   if (int e = check_cache8(fn, &a, &none)) return e;
   if (none || a.max_k == 0) return ok();
+  if (cache8_store_workgroups(a) >= 1 << 23) return bad(fn, "blocks * heads exceeds the grid");
   if (any_null({k8, ks, v8, vs, k, v})) return bad(fn, "NULL pointer");
   if (k8 == v8 || ks == vs) return bad(fn, "k8 and v8, and ks and vs, must be distinct buffers");
   if (!aligned16(k8) || !aligned16(v8)) return bad(fn, "k8 and v8 must be 16-byte aligned");
@@ -877,6 +877,7 @@ int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks, const v
   bool none;
   if (int e = check_cache8(fn, &a, &none)) return e;
   if (none || a.max_k == 0) return ok();
+  if (cache8_store_workgroups(a) >= 1 << 23) return bad(fn, "blocks * heads exceeds the grid");
   if (any_null({k8, ks, v8, vs, k, v})) return bad(fn, "NULL pointer");
   if (k == v) return bad(fn, "k and v must be distinct buffers");
   if (!aligned16(k8) || !aligned16(v8)) return bad(fn, "k8 and v8 must be 16-byte aligned");
@@ -896,6 +897,9 @@ int ugk_cache8_attention(float *out, float *lse, const float *q, const void *k8,
   // a workgroup of 256 for 32 rows and heads then
   if (weight && (long long)a.nseq * a.NKV >= ((long long)1 << 24) / (((long long)a.max_q * (a.NH / a.NKV) + 31) / 32 + 1))
     return bad(fn, "nseq * heads * rows exceeds the grid");
+  // and one for 16 blocks of a sequence
+  if (weight && a.nseq * (((long long)a.max_k + kCacheBlock - 1) / kCacheBlock / 16 + 1) >= (long long)1 << 23)
+    return bad(fn, "nseq * blocks exceeds the grid of their weights");
   if (none) return ok();
   if (any_null({out, q})) return bad(fn, "NULL pointer");
   if (a.max_k > 0 && a.nblocks == 0) return bad(fn, "nblocks must be >= 1 where max_k is");  // a masked block is read as block 0

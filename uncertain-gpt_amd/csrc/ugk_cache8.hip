@@ -1705,7 +1705,7 @@ Plan8 plan8(const ugk_cache8 &a, bool weigh) {
   // 78 and 9 us in shares, 101 else; where they are few it is nothing: a row of each of 10 of 400 sequences of up to 1,024
   // keys 12.6 and 3.8, 11.0 else).
   const bool few = blocks > 32 && jobs <= 4LL * at_once, empty = every > 4 * jobs && every > 8LL * at_once;
-  if ((few || empty) && (blocks + 8) * jobs <= 1 << 30 && jobs * p.per_job < 1 << 24 && (rows + p.rows) * G >> 32 == 0) {
+  if ((few || empty) && (blocks + 8) * jobs <= 1 << 30 && jobs * p.per_job < 1 << 23 && (rows + p.rows) * G >> 32 == 0) {
     // a job has one part more than workgroups' borders, and a workgroup two at most that are not whole
     const long long slots = fit(jobs, true);
     p.step = jobs <= at_once && slots >= 2 * jobs ? 1 : 2;
@@ -1835,6 +1835,7 @@ static Store8 store8(const ugk_cache8 &a) {
   const long long per = touched_blocks(a), most = a.nseq * per, all = a.rows_q / kKeys + 2LL * min(a.nseq, a.rows_q);
   return most > 2 * all && 2 * most * a.NKV > 16LL * cu_count8() ? Store8{0, (int)all} : Store8{(int)per, (int)most};
 }
+long long cache8_store_workgroups(const ugk_cache8 &a) { return (long long)store8(a).all * a.NKV; }
 int launch_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, const float *v, const ugk_cache8 &a, int *word) {
   const Store8 n = store8(a);
   const auto go = [&](auto kernel) {

@@ -417,6 +417,7 @@ size_t attention_backward_bound(size_t rows, size_t NH, size_t HS);
 constexpr int kCacheBlock = 64;        // tokens per block
 constexpr int kEvictBlocks = 1 << 14;  // blocks per sequence that the eviction takes
 constexpr int kWeighRows = 256;        // rows and heads per key/value head whose weights attention adds up per block
+long long cache8_store_workgroups(const ugk_cache8 &a);  // of k, and as many of v; of the load likewise
 int launch_cache8_store(void *k8, float *ks, void *v8, float *vs, const float *k, const float *v, const ugk_cache8 &a, int *word);
 int launch_cache8_load(float *k, float *v, const void *k8, const float *ks, const void *v8, const float *vs, const ugk_cache8 &a,
                        int *word);
