@@ -345,6 +345,8 @@ struct Parts8 {
   int ld, most;        // blocks of max_k keys; jobs where they are counted
   int wgs, cus;        // workgroups that share all blocks (0: a workgroup has one job's part), CUs
   unsigned inverse;    // ceil(2^32 / heads of a group), 0 for one head
+  float factor;        // |scale| log2(e) is this, 0 or 1/2 to 1, times 2^power: the product itself may leave a float's range
+  int power;
 };
 __host__ __device__ __forceinline__ int part_floats(int HS) { return (HS + 3) & ~3; }
 // Where a row of part p is, whose job's first part is in slot `first`.
@@ -426,11 +428,10 @@ __device__ __forceinline__ uint32_t load_q(const float *p, int first, int step, 
   return most;
 }
 
-// f = |scale| log2(e) of the call, ks of a block and 2^x of a row's whole numbers, as one factor of its scores: a normal
+// |scale| log2(e) of the call, ks of a block and 2^x of a row's whole numbers, as one factor of its scores: a normal
 // number, so that a score of 0 stays 0 and -infinity of a masked one itself.
-__device__ __forceinline__ float score_factor(float f, float ks, int x) {
-  const float y = __builtin_amdgcn_ldexpf(__builtin_amdgcn_frexp_mantf(f) * __builtin_amdgcn_frexp_mantf(ks),
-                                          __builtin_amdgcn_frexp_expf(f) + __builtin_amdgcn_frexp_expf(ks) + x);
+__device__ __forceinline__ float score_factor(const Parts8 &parts, float ks, int x) {
+  const float y = __builtin_amdgcn_ldexpf(parts.factor * __builtin_amdgcn_frexp_mantf(ks), parts.power + __builtin_amdgcn_frexp_expf(ks) + x);
   return fmaxf(fminf(y, 3.402823466e38f), 0x1p-126f);
 }
 // x is computed here, in this branch: the compiler otherwise moves what only the next step of a loop uses behind the branches
@@ -806,7 +807,7 @@ struct Block8 {
   const Job8 &job;
   int lane, j;
   bool there;
-  float f, kscale, vexp;  // f: |scale| log2(e) (its sign goes with q)
+  float kscale, vexp;
   // where the block's m and l of a row go
   __device__ __forceinline__ float2 *stat(int row) const {
     return parts.block + (((size_t)job.b * a.NKV + job.hk) * a.max_q * (a.NH / a.NKV) + row) * parts.ld + j;
@@ -871,7 +872,7 @@ struct Four {
   __device__ __forceinline__ void weights(Scores &p, float mb, const Block8 &k, uint32_t *lp, Weights &ap, float &fo, float &fb) {
     const int col = k.lane & 15, quad = k.lane >> 4;
     // a number where the row sees nothing: the result of one without any key is 0 whatever it holds
-    const float most = max16(mb), fac = here(nan && most != -INFINITY ? NAN : score_factor(k.f, k.kscale, ex));
+    const float most = max16(mb), fac = here(nan && most != -INFINITY ? NAN : score_factor(k.parts, k.kscale, ex));
     mb = top_score(most, fac);
     float less = less_top(mb, 0.0f);
     if (__any(far_score(mb))) {
@@ -1008,7 +1009,7 @@ struct Sixteen {
     return mb;
   }
   __device__ __forceinline__ void weights(Scores &p, float mb, const Block8 &k, uint32_t *, Weights &bp, float &fo, float &fb) {
-    const float most = quarters_max(mb), fac = here(nan && most != -INFINITY ? NAN : score_factor(k.f, k.kscale, ex));
+    const float most = quarters_max(mb), fac = here(nan && most != -INFINITY ? NAN : score_factor(k.parts, k.kscale, ex));
     mb = top_score(most, fac);
     float less = less_top(mb, 0.0f);
     if (__any(far_score(mb))) {
@@ -1109,7 +1110,7 @@ __device__ __forceinline__ void rows_job(float *out, float *lse, const float *q,
     constexpr bool kNext = decltype(next)::value;
     const int id = kNext ? walk.ahead(a, job.b, word) : 0;
     const size_t ahead = block_head(id, a.NKV, hk);
-    const Block8 k{a, parts, job, lane, walk.j, walk.there(), fabsf(a.scale) * kLog2e8, kscale, exponent(vscale)};
+    const Block8 k{a, parts, job, lane, walk.j, walk.there(), kscale, exponent(vscale)};
     typename Rows::Scores p;
     typename Rows::Weights w;
     float fo, fb;
@@ -1346,7 +1347,6 @@ __device__ __forceinline__ void tile_job(float *out, float *lse, const float *q,
   const int wave_first = min(row0 + 32 * wave, rows - 1), wave_last = min(row0 + 32 * wave + 31, rows - 1);
   const int least = s.seen(wave_first / G, a.causal), most_seen = s.seen(wave_last / G, a.causal);
   const bool idle = row0 + 32 * wave >= rows;
-  const float f = fabsf(a.scale) * kLog2e8;  // its sign goes with q
 
   // staging: thread t has words of 16 codes t, t + 256 of the block's keys and of its values
   int kdst[NL], vdst[NL];
@@ -1422,7 +1422,7 @@ __device__ __forceinline__ void tile_job(float *out, float *lse, const float *q,
       *reinterpret_cast<v2u *>(vt + vdst[n] + 48) = halves4(__builtin_amdgcn_perm(t3, t1, 0x07060302u));
     }
     const bool held = there;
-    const float fac = here(score_factor(f, kscale, e)), vnow = exponent(vscale);
+    const float fac = here(score_factor(parts, kscale, e)), vnow = exponent(vscale);
     __syncthreads();
     if (j + 1 < stop) fetch(j + 1);
     if (idle || j * kKeys >= most_seen) continue;
@@ -1757,6 +1757,9 @@ int launch_cache8_attention(float *out, float *lse, const float *q, const void *
   parts.cus = cu_count8();
   parts.ld = blocks_of_keys(a);
   parts.most = (int)p.jobs;
+  int of_scale, of_product;  // the scale's sign goes with q
+  parts.factor = frexpf(frexpf(fabsf(a.scale), &of_scale) * kLog2e8, &of_product);
+  parts.power = of_scale + of_product;
   parts.inverse = G == 1 ? 0u : (unsigned)((1ULL << 32) / G + 1);
   if (p.slots) {
     parts.o = mem;
