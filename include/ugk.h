@@ -504,7 +504,7 @@ int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks,
                     const void *v8, const float *vs, ugk_cache8 a);
 
 /* ugk_attention_forward of q against the cache: out, and lse (rows_q, NH) if not
- * NULL. A row without a key that it sees has out 0 and lse -infinity. A row of q (of one
+ * NULL. A row without a key that it sees has out 0 and lse -infinity, whatever its q. A row of q (of one
  * head) enters as whole numbers of 31 bits next to its largest element and the
  * weights as such next to the largest of their block; or, with more than 64 query
  * rows times heads per key/value head (more than 32, where sequences times key/value heads
@@ -515,7 +515,9 @@ int ugk_cache8_load(float *k, float *v, const void *k8, const float *ks,
  * of q, makes a row's out, lse and what it adds to `weight` NaN; one of about -2^127 or
  * less weighs nothing. out must not overlap q.
  * weight, if not NULL, (nseq, ld_table): weight[b, j] += the sum of the weights over
- * sequence b's rows and heads and the keys of its block j. For up to 256 query rows
+ * sequence b's rows and heads and the keys of its block j, rows of drafts that are refused later among them. It is the
+ * caller's: an entry keeps what it has where k_len shrinks and a store begins its block anew, until ugk_cache8_evict clears
+ * those not in use, or the caller does. For up to 256 query rows
  * times heads per key/value head: tokens, drafts, or the last rows of a prompt. It
  * takes 8 bytes of workspace per row, head and block. Deterministic: the same call
  * gives the same bits. The workspace is attention's: a config's of as many rows and

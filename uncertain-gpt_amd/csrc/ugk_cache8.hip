@@ -1316,7 +1316,7 @@ __global__ __launch_bounds__(kBlock) void k_cache8_finish(float *out, float *lse
 // v_mfma_f32_32x32x16_f16, where fp32 keys and values need three.
 //
 // Bound by matrix and vector instructions, which add up on a SIMD: 64 of the first and some 540 of the others per block and
-// wavefront at heads of 128. 8 x 1,024 rows of 12 heads of 64 42 us, 4 x 2,048 of them 72, of 16/4 heads of 128 160 to 178
+// wavefront at heads of 128. 8 x 1,024 rows of 12 heads of 64 42 to 44 us, 4 x 2,048 of them 72 to 75, of 16/4 heads of 128 160 to 178
 // (of fp32 keys and values 67, 107 and 191). Products of one sum never follow one another, and their operands are two steps
 // ahead (62 us, not 64, of prompts behind long conversations); wavefront priorities changed nothing.
 constexpr int kTileWaves8 = 4, kTileRows8 = 32 * kTileWaves8, kTileThreads8 = kTileWaves8 * kWave;

@@ -275,7 +275,7 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_verify(int *accepted, i
 
 // Segments of a row: whole steps, at most kMaxSegs.
 int seg_floats(int V) { return (int)(((long long)V + (long long)kMaxSegs * kStep - 1) / ((long long)kMaxSegs * kStep)) * kStep; }
-// Sums in a launch of their own while one workgroup per sequence would leave CUs idle (64 x 50,257 tokens 5.9 + 5.8 us, in one
+// Sums in a launch of their own while one workgroup per sequence would leave CUs idle (64 x 50,257 tokens 6.1 + 5.9 us, in one
 // launch 21.6); up to two steps are not worth it.
 bool separate(int nseq, int V) { return V > 2 * kStep && nseq < 256; }
 }  // namespace
